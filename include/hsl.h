@@ -128,8 +128,9 @@ int hsl_poll_error(const void* ws, int* flag, void* stream);
 /* Device errors raised by this library's kernels on the current device since
  * they were last cleared: one sticky word per device, whatever workspace or
  * stream the failing call used.  Bit 0: a persistent kernel gave up a wait
- * between workgroups (hsl_set_spin_timeout_us).  Waits for `stream`, stores the
- * word in *flags and, when clear != 0, resets it.  Such an abort is never
+ * between workgroups (hsl_set_spin_timeout_us).  Bit 1: a token id was at or beyond
+ * its vocabulary (hsl_embed_fwd, hsl_logprob_fwd).  Waits for `stream`, stores the
+ * word in *flags and, when clear != 0, resets it.  An aborted wait is never
  * silent: the aborting workgroups also fill every output they own with NaN
  * (forward: their rows of h_save, c_save, gact, tanh_c; backward: their dW
  * planes, bias partials, dgates and dh0/dc0), so the results of the call are NaN.
@@ -339,6 +340,65 @@ int hsl_gemm_f32(const float* A, const float* Bm, const float* bias, float* C,
  * _parallel.py:56) used by hsl_par_fwd_b16. */
 int hsl_gemm_b16(const void* A, const void* B, const float* bias, float* C,
                  int M, int N, int K, int lda, int ldb, int ldc, int fmt, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Operators of a language model around the recurrent layers (prlstm_amd.lm; no
+ * reference counterpart).  fmt is the element format of the tensors passed as
+ * void*: 0 = bf16, 1 = fp16, 2 = fp32; every other tensor is fp32 (ids as said).
+ * Strides and leading dimensions are in elements.  Sums, states and statistics are
+ * fp32, and each output is rounded once.
+ * ------------------------------------------------------------------------- */
+
+/* out[n] = scale * weight[ids[n]], out [N, D] contiguous, weight [V, D] with row
+ * stride ldw, ids int64 (ids64 != 0) or int32.  A negative id gives a row of zeros;
+ * one >= V gives NaN and raises bit 1 of the device word. */
+int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw, float scale,
+                  void* out, long long N, int V, int D, int fmt, void* stream);
+/* dweight[v] = scale * the sum of dout[n] over n with ids[n] = v, in a fixed order
+ * (the same result every time): dense [V, D], rows without a position are zero.
+ * dout has row stride ldd.  Ids outside 0..V-1 and padding_idx (negative: none) get
+ * no gradient. */
+size_t hsl_embed_bwd_ws_bytes(long long N, int V, int D);
+int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, float scale,
+                  int padding_idx, void* dweight, void* ws, size_t ws_bytes,
+                  long long N, int V, int D, int fmt, void* stream);
+
+/* Gated linear recurrence over zv [T, B, 2H] = (z | v) with f = sigmoid(z):
+ *   h_t = f_t h_{t-1} + (1 - f_t) v_t,   out_t = h_t,   h_{-1} = h0 (NULL: zeros)
+ * and 0 in place of h_{t-1} where reset [T, B] (bytes; NULL: none) is nonzero.  zv,
+ * reset and out have the time and batch strides given after them and dense channels.
+ * h_n [B, H] = h_{T-1} in fp32 (h0 when T = 0); it may be h0 itself when T = 1.  ck
+ * (NULL: no backward follows) receives the hsl_gated_ck_rows(T) rows [B, H] of states
+ * that hsl_gated_bwd starts from.  hsl_gated_ws_bytes serves both directions. */
+int hsl_gated_ck_rows(int T);
+size_t hsl_gated_ws_bytes(int T, int B, int H);
+int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h0,
+                  const void* reset, long long rs_t, long long rs_b,
+                  void* out, long long out_t, long long out_b, float* h_n, float* ck,
+                  void* ws, size_t ws_bytes, int T, int B, int H, int fmt, void* stream);
+/* dzv from dout (NULL: zeros) and dh_n (NULL: zeros); dh0 may be NULL. */
+int hsl_gated_bwd(const void* zv, long long zv_t, long long zv_b,
+                  const void* reset, long long rs_t, long long rs_b, const float* ck,
+                  const void* dout, long long do_t, long long do_b, const float* dh_n,
+                  void* dzv, long long dz_t, long long dz_b, float* dh0,
+                  void* ws, size_t ws_bytes, int T, int B, int H, int fmt, void* stream);
+
+/* Of each row n of logits [N, V] (row stride ld): logp[n] = log softmax at tokens[n]
+ * (int64 or int32; tokens and logp may be NULL), entropy[n], stats[n] = (largest logit m,
+ * log sum exp(x - m)) for the backward, and the `top` (<= 32, <= V) largest: top_logp, top_ids [N, top],
+ * ordered by logit with NaN first and the lowest id first among equals.  -inf masks a
+ * token; a row of nothing else has m = logp = -inf and entropy 0.  A negative token
+ * gives logp 0; one >= V NaN, and raises bit 1 of the device word. */
+size_t hsl_logprob_fwd_ws_bytes(long long N, int V, int top);
+int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int tok64,
+                    float* logp, float* entropy, float* stats, float* top_logp, long long* top_ids,
+                    void* ws, size_t ws_bytes, long long N, int V, int top, int fmt, void* stream);
+/* dlogits [N, V] (row stride ldd) from the gradients of logp, entropy and top_logp (each
+ * may be NULL: zeros); a row with nothing but masks gets zeros. */
+int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int tok64,
+                    const long long* top_ids, const float* stats, const float* entropy,
+                    const float* dlogp, const float* dent, const float* dtop,
+                    void* dlogits, long long ldd, long long N, int V, int top, int fmt, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from .functional import EPS, headstartlstm_parallel, headstartlstm_recurrent
+from .lm import TokenLogprobs, embedding, gated_recurrence, gated_recurrence_step, token_logprobs
 from ._lib import (check_errors, last_recurrent_path, set_exchange_scope, set_recurrent_path, set_spin_timeout_us,
                    set_split_products)
 
@@ -105,5 +106,6 @@ __all__ = [
     "HeadStartLSTM", "headstartlstm_recurrent", "headstartlstm_parallel", "EPS",
     "set_recurrent_path", "set_spin_timeout_us", "set_exchange_scope", "set_split_products", "last_recurrent_path",
     "check_errors",
+    "embedding", "gated_recurrence", "gated_recurrence_step", "token_logprobs", "TokenLogprobs",
     "__version__",
 ]

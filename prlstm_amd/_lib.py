@@ -18,6 +18,7 @@ _I = ctypes.c_int
 _Z = ctypes.c_size_t
 _F = ctypes.c_float
 _D = ctypes.c_double
+_L = ctypes.c_longlong
 
 # name -> (restype, argtypes); must match include/hsl.h
 SIGNATURES = {
@@ -62,6 +63,16 @@ SIGNATURES = {
     "hsl_gemm_ws_bytes": (_Z, [_I, _I, _I]),
     "hsl_gemm_f32": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "hsl_gemm_b16": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "hsl_embed_fwd": (_I, [_P, _I, _P, _L, _F, _P, _L, _I, _I, _I, _P]),
+    "hsl_embed_bwd_ws_bytes": (_Z, [_L, _I, _I]),
+    "hsl_embed_bwd": (_I, [_P, _I, _P, _L, _F, _I, _P, _P, _Z, _L, _I, _I, _I, _P]),
+    "hsl_gated_ck_rows": (_I, [_I]),
+    "hsl_gated_ws_bytes": (_Z, [_I, _I, _I]),
+    "hsl_gated_fwd": (_I, [_P, _L, _L, _P, _P, _L, _L, _P, _L, _L, _P, _P, _P, _Z, _I, _I, _I, _I, _P]),
+    "hsl_gated_bwd": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _P, _P, _Z, _I, _I, _I, _I, _P]),
+    "hsl_logprob_fwd_ws_bytes": (_Z, [_L, _I, _I]),
+    "hsl_logprob_fwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _Z, _L, _I, _I, _I, _P]),
+    "hsl_logprob_bwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _P]),
 }
 
 _lock = threading.Lock()
@@ -133,7 +144,8 @@ def set_spin_timeout_us(us):
 
 def device_errors(device=None, clear=True):
     """The sticky device-error word of the current (or given) device; waits for its
-    current stream.  Bit 0: a persistent kernel gave up a wait between workgroups."""
+    current stream.  Bit 0: a persistent kernel gave up a wait between workgroups; bit 1: a token
+    id was at or beyond its vocabulary."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     flags = ctypes.c_int(0)
     call("hsl_device_errors", ctypes.byref(flags), 1 if clear else 0, stream_of(dev))
@@ -146,6 +158,10 @@ def check_errors(device=None):
     also leaves NaN in the outputs of that call, so the failure shows in the loss
     even without this check; this names it."""
     flags = device_errors(device, clear=True)
+    if flags & 2:
+        raise RuntimeError(
+            f"prlstm_amd: device error word {flags:#x}: a token id was at or beyond the vocabulary of its embedding "
+            "or logits; its row is NaN")
     if flags:
         raise RuntimeError(
             f"prlstm_amd: device error word {flags:#x}: a persistent recurrent kernel gave up a wait "

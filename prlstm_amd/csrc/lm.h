@@ -1,0 +1,60 @@
+// Helpers shared by the language-model operators (embed.hip, gated.hip, logprob.hip).
+#pragma once
+
+#include <type_traits>
+
+#include "hsl_internal.h"
+
+namespace hsl {
+
+// Element formats of the operators' streams, as the C ABI numbers them.
+enum ElemFmt { kElemBf16 = 0, kElemF16 = 1, kElemF32 = 2 };
+inline bool elem_fmt_ok(int fmt) { return fmt >= kElemBf16 && fmt <= kElemF32; }
+
+// Elements are widened to fp32 when they are read and rounded to nearest even once when they
+// are stored.
+template <int F>
+struct Elem;
+template <>
+struct Elem<kElemBf16> {
+  using T = unsigned short;
+  static __device__ __forceinline__ float up(T u) { return __uint_as_float((unsigned)u << 16); }
+  static __device__ __forceinline__ T down(float v) { return __builtin_bit_cast(T, (__bf16)v); }
+};
+template <>
+struct Elem<kElemF16> {
+  using T = unsigned short;
+  static __device__ __forceinline__ float up(T u) { return (float)__builtin_bit_cast(_Float16, u); }
+  static __device__ __forceinline__ T down(float v) {
+    asm("" : "+v"(v));  // not fused into a mixed-precision multiply that would skip fp32's rounding
+    return __builtin_bit_cast(T, (_Float16)v);
+  }
+};
+template <>
+struct Elem<kElemF32> {
+  using T = float;
+  static __device__ __forceinline__ float up(T u) { return u; }
+  static __device__ __forceinline__ T down(float v) { return v; }
+};
+
+// The sticky device word that hsl_device_errors reads, for a kernel's argument (recurrent.hip).
+// Bit 1: an id beyond the vocabulary (bit 0 is the persistent kernels').
+int device_error_word(unsigned** word);
+constexpr unsigned kErrId = 2u;
+
+// Token ids are int32 or int64.
+__device__ __forceinline__ long long load_id(const void* ids, int ids64, size_t i) {
+  return ids64 ? static_cast<const long long*>(ids)[i] : (long long)static_cast<const int*>(ids)[i];
+}
+
+// f(integral_constant<int, fmt>) for the element format of a call.
+template <class Fn>
+int with_fmt(int fmt, Fn f) {
+  switch (fmt) {
+    case kElemBf16: return f(std::integral_constant<int, kElemBf16>{});
+    case kElemF16: return f(std::integral_constant<int, kElemF16>{});
+    default: return f(std::integral_constant<int, kElemF32>{});
+  }
+}
+
+}  // namespace hsl

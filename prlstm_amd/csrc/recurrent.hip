@@ -23,6 +23,7 @@
 // A_b[i][0], B from lane 4b+j is B_b[0][j], result lane 4b+j, reg i holds D_b[i][j].
 // With cbsz=4, abid=0 every block uses block 0's A (lanes 0-3).
 #include <algorithm>
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <optional>
@@ -30,6 +31,7 @@
 #include <type_traits>
 
 #include "gemm_core.h"
+#include "lm.h"
 #include "split_bf16.h"
 
 namespace hsl {
@@ -446,8 +448,8 @@ constexpr unsigned long long kEmpty2 = ~0ull;
 }  // namespace
 
 // Device errors of this library since they were last read (one word per device, sticky):
-// bit 0 = a persistent kernel gave up a wait between workgroups.  Read and cleared by
-// hsl_device_errors.
+// bit 0 = a persistent kernel gave up a wait between workgroups, bit 1 = a token id beyond its
+// vocabulary (embed.hip, logprob.hip).  Read and cleared by hsl_device_errors.
 __device__ unsigned g_device_errors;
 
 namespace {
@@ -2788,6 +2790,20 @@ int bias_grads_from_parts(const double* db_part, int B, const double* rowdot, co
 }  // namespace hsl
 
 namespace hsl {
+int device_error_word(unsigned** word) {
+  static std::atomic<unsigned*> words[64];
+  DeviceInfo di;
+  HSL_CHECK(device_info(&di));
+  unsigned* p = words[di.device].load();
+  if (!p) {
+    void* q = nullptr;
+    HSL_HIP(hipGetSymbolAddress(&q, HIP_SYMBOL(g_device_errors)));
+    words[di.device].store(p = static_cast<unsigned*>(q));
+  }
+  *word = p;
+  return HSL_OK;
+}
+
 namespace {
 __global__ void clear_device_errors_kernel() { g_device_errors = 0u; }
 
