@@ -6,12 +6,26 @@
 // zv holds z in its first H and v in its last H channels.  The state is fp32 throughout; out is
 // h rounded once.  ck keeps h as it enters every 8th step, in fp32, from which the backward runs
 // the steps again (the rounded out would cost dz its precision where h and v are close).
+//
+// Both directions are first-order recurrences, so runs of steps compose into affine maps
+// x -> A x + V.  A workgroup owns kLanes * E neighbouring channels and walks the time in chunks:
+// each of its groups of kLanes lanes takes 8 steps of the chunk, composes them, the maps are
+// joined by one cross-lane move and through LDS, and the group runs its steps again from the
+// state that enters them, all from registers; the next chunk's loads are issued first.  Every
+// stream is read and written once.  With few channels the time is cut into segments that run as
+// workgroups of their own after a pass that composes each segment's map.
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
 #include "lm.h"
 
 namespace hsl {
 namespace {
 
-constexpr int kGatedCk = 8;  // steps per checkpoint row
+constexpr int kSteps = 8;    // of a group in a chunk, and per checkpoint row
+constexpr int kLanes = 32;   // of a group
+constexpr int kMaxWaves = 8;
 
 struct Gates {
   float f, w;
@@ -24,6 +38,25 @@ __device__ __forceinline__ Gates gates_of(float z) {
   return z >= 0.f ? Gates{big, small} : Gates{small, big};
 }
 
+// A of a map with a reset in it is -0 (all others are >= +0): nothing of the state before it
+// passes, not even what is infinite or NaN, where 0 * x would.
+constexpr unsigned kCutBits = 0x80000000u;
+template <bool RESET>
+__device__ __forceinline__ float apply(float A, float V, float x) {
+  const float y = __builtin_fmaf(A, x, V);
+  if constexpr (RESET) return __float_as_uint(A) == kCutBits ? V : y;
+  return y;
+}
+// A of a composed map.  A product of gates is held at the smallest number once it underflows,
+// unless a factor is 0, so that an infinite state stays infinite; a cut stays a cut.
+template <bool RESET>
+__device__ __forceinline__ float compose(float a, float b) {
+  const float p = fmaxf(a * b, fminf(fminf(a, b), __uint_as_float(1u)));
+  if constexpr (RESET)
+    return __float_as_uint(a) == kCutBits || __float_as_uint(b) == kCutBits ? __uint_as_float(kCutBits) : p;
+  return p;
+}
+
 // Strides are in elements.
 struct Stream {
   const void* p;
@@ -34,68 +67,482 @@ struct OutStream {
   long long st, sb;
 };
 
-template <int F>
-__global__ __launch_bounds__(256) void gated_fwd_kernel(Stream zv, const float* h0, Stream reset, OutStream out,
-                                                        float* h_n, float* __restrict__ ck, int T, int B, int H) {
-  using E = Elem<F>;
-  const int ch = blockIdx.x * 256 + threadIdx.x;
-  if (ch >= B * H) return;
-  const int b = ch / H, j = ch % H;
-  float h = h0 ? h0[ch] : 0.f;
-  for (int t = 0; t < T; ++t) {
-    if (ck && t % kGatedCk == 0) ck[(size_t)(t / kGatedCk) * B * H + ch] = h;
-    const auto* row = static_cast<const typename E::T*>(zv.p) + t * zv.st + b * zv.sb;
-    const Gates g = gates_of(E::up(row[j]));
-    const float wv = g.w * E::up(row[H + j]);
-    const bool cut = reset.p && static_cast<const unsigned char*>(reset.p)[t * reset.st + b * reset.sb];
-    h = cut ? wv : __builtin_fmaf(g.f, h, wv);
-    static_cast<typename E::T*>(out.p)[t * out.st + b * out.sb + j] = E::down(h);
+// E neighbouring elements.
+template <int F, int E>
+struct alignas(sizeof(typename Elem<F>::T) * E) Pack {
+  typename Elem<F>::T v[E];
+};
+template <int F, int E>
+__device__ __forceinline__ Pack<F, E> load_pack(const typename Elem<F>::T* p) {
+  return *reinterpret_cast<const Pack<F, E>*>(p);
+}
+template <int E>
+struct alignas(4 * E) Floats {
+  float v[E];
+};
+
+// One workgroup's channels and groups.
+template <int E>
+struct Place {
+  int lane, w, c, g, nw;  // lane in the wave, wave, lane in the group, group in the workgroup, waves
+  int ch;                 // first of the thread's E channels (b * H + j), clamped into range
+  int b, j;
+  bool ok;
+  __device__ __forceinline__ Place(int B, int H) {
+    lane = threadIdx.x & 63;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    nw = blockDim.x >> 6;
+    c = lane % kLanes;
+    g = threadIdx.x / kLanes;
+    const int C = B * H, first = (blockIdx.x * kLanes + c) * E;
+    ok = first < C;
+    ch = ok ? first : C - E;
+    b = ch / H;
+    j = ch - b * H;
   }
-  h_n[ch] = h;
+};
+
+// The reset flags of a group's steps t0 .. t0+7 as bits (steps at or past T: none).
+__device__ __forceinline__ void load_resets(const Stream& reset, int b, int t0, int T, unsigned char (&r)[kSteps]) {
+  const auto* p = static_cast<const unsigned char*>(reset.p) + b * reset.sb;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) r[s] = p[min(t0 + s, T - 1) * reset.st];
 }
 
-template <int F>
-__global__ __launch_bounds__(256) void gated_bwd_kernel(Stream zv, Stream reset, const float* __restrict__ ck,
-                                                        Stream dout, const float* __restrict__ dh_n, OutStream dzv,
-                                                        float* __restrict__ dh0, int T, int B, int H) {
-  using E = Elem<F>;
-  const int ch = blockIdx.x * 256 + threadIdx.x;
-  if (ch >= B * H) return;
-  const int b = ch / H, j = ch % H;
-  float U = dh_n ? dh_n[ch] : 0.f;
-  for (int k = (T - 1) / kGatedCk; k >= 0; --k) {
-    float prev[kGatedCk];
-    float h = ck[(size_t)k * B * H + ch];
-    const int n = min(kGatedCk, T - k * kGatedCk);
-    for (int s = 0; s < n; ++s) {
-      const int t = k * kGatedCk + s;
-      const auto* row = static_cast<const typename E::T*>(zv.p) + t * zv.st + b * zv.sb;
-      const Gates g = gates_of(E::up(row[j]));
-      const float wv = g.w * E::up(row[H + j]);
-      const bool cut = reset.p && static_cast<const unsigned char*>(reset.p)[t * reset.st + b * reset.sb];
-      prev[s] = cut ? 0.f : h;
-      h = cut ? wv : __builtin_fmaf(g.f, h, wv);
+// Joins the maps of a chunk's groups: from each thread's map (A, V) of its group, first (REV:
+// last) group nearest to the incoming state x, returns the state that enters the thread's group
+// and leaves in x the state behind the chunk.  sm is this chunk's [waves][kLanes] part of LDS.
+template <int E, bool RESET, bool REV>
+__device__ __forceinline__ void join(const Place<E>& q, float (&A)[E], float (&V)[E], float (&x)[E], float (&in)[E],
+                                     Floats<2 * E> (*sm)[kLanes]) {
+  // the wave's other group's map; the group further from the state continues the nearer one's
+  float oA[E], oV[E];
+  const bool far = REV ? q.lane < kLanes : q.lane >= kLanes;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    oA[e] = __shfl_xor(A[e], kLanes);
+    oV[e] = __shfl_xor(V[e], kLanes);
+  }
+  if (far) {
+    Floats<2 * E> m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      m.v[2 * e + 1] = apply<RESET>(A[e], V[e], oV[e]);
+      m.v[2 * e] = compose<RESET>(A[e], oA[e]);
     }
-    for (int s = n - 1; s >= 0; --s) {
-      const int t = k * kGatedCk + s;
-      const auto* row = static_cast<const typename E::T*>(zv.p) + t * zv.st + b * zv.sb;
-      const Gates g = gates_of(E::up(row[j]));
-      const float v = E::up(row[H + j]);
-      const bool cut = reset.p && static_cast<const unsigned char*>(reset.p)[t * reset.st + b * reset.sb];
-      const float G =
-          dout.p ? E::up(static_cast<const typename E::T*>(dout.p)[t * dout.st + b * dout.sb + j]) + U : U;
-      auto* drow = static_cast<typename E::T*>(dzv.p) + t * dzv.st + b * dzv.sb;
-      drow[j] = E::down(G * (prev[s] - v) * (g.f * g.w));
-      drow[H + j] = E::down(g.w * G);
-      U = cut ? 0.f : g.f * G;
+    sm[q.w][q.c] = m;
+  }
+  lds_barrier();
+  float cur[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) cur[e] = x[e];
+  for (int i = 0; i < q.nw; ++i) {
+    const int u = REV ? q.nw - 1 - i : i;
+    const Floats<2 * E> m = sm[u][q.c];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (u == q.w) in[e] = cur[e];
+      cur[e] = apply<RESET>(m.v[2 * e], m.v[2 * e + 1], cur[e]);
     }
   }
-  if (dh0) dh0[ch] = U;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    x[e] = cur[e];
+    if (far) in[e] = apply<RESET>(oA[e], oV[e], in[e]);
+  }
+}
+
+// The state that enters a segment: the first (REV: last) state through the maps of the segments
+// before it, maps[i][C] of segment i + 1 (REV) or i.
+template <int E, bool RESET, bool REV>
+__device__ __forceinline__ void enter_segment(const float2* __restrict__ maps, int C, int ch, int seg, int nseg,
+                                              float (&x)[E]) {
+  const int n = REV ? nseg - 1 - seg : seg;
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float2 m[8][E];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = min(i0 + i, n - 1), row = REV ? nseg - 2 - k : k;
+#pragma unroll
+      for (int e = 0; e < E; ++e) m[i][e] = maps[(size_t)row * C + ch + e];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = apply<RESET>(m[i][e].x, m[i][e].y, x[e]);
+      }
+  }
+}
+
+template <int F, int E, bool RESET>
+__global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, const float* h0, Stream reset,
+                                                                  OutStream out, float* h_n, float* __restrict__ ck,
+                                                                  const float2* __restrict__ maps, int T, int B, int H,
+                                                                  int seg_steps) {
+  using T_ = typename Elem<F>::T;
+  __shared__ Floats<2 * E> sm[2][kMaxWaves][kLanes];
+  const Place<E> q(B, H);
+  const int C = B * H, chunk = q.nw * 2 * kSteps;
+  const int seg = blockIdx.y, tb = seg * seg_steps, te = min(T, tb + seg_steps);
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = h0 ? h0[q.ch + e] : 0.f;
+  enter_segment<E, RESET, false>(maps, C, q.ch, seg, gridDim.y, x);
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
+  T_* op = static_cast<T_*>(out.p) + q.b * out.sb + q.j;
+
+  Pack<F, E> rz[2][kSteps], rv[2][kSteps];
+  unsigned char rr[2][kSteps];
+  auto load = [&](int t0, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps], unsigned char(&r)[kSteps]) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const T_* p = zp + min(t0 + s, T - 1) * zv.st;
+      z[s] = load_pack<F, E>(p);
+      v[s] = load_pack<F, E>(p + H);
+    }
+    if constexpr (RESET) load_resets(reset, q.b, t0, T, r);
+  };
+  auto step = [&](int t1, int par, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps], unsigned char(&r)[kSteps]) {
+    const int t0 = t1 + q.g * kSteps;
+    float f[kSteps][E], wv[kSteps][E], A[E], V[E], h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      A[e] = 1.f;
+      V[e] = 0.f;
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const bool in = t0 + s < te;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const Gates g = gates_of(Elem<F>::up(z[s].v[e]));
+        f[s][e] = in ? g.f : 1.f;
+        wv[s][e] = in ? g.w * Elem<F>::up(v[s].v[e]) : 0.f;
+        if (RESET && in && r[s]) f[s][e] = __uint_as_float(kCutBits);
+        V[e] = apply<RESET>(f[s][e], wv[s][e], V[e]);
+        A[e] = compose<RESET>(f[s][e], A[e]);
+      }
+    }
+    join<E, RESET, false>(q, A, V, x, h, sm[par]);
+    if (!q.ok || t0 >= te) return;
+    if (ck) {
+      Floats<E> o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = h[e];
+      *reinterpret_cast<Floats<E>*>(ck + (size_t)(t0 / kSteps) * C + q.ch) = o;
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      Pack<F, E> o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        h[e] = apply<RESET>(f[s][e], wv[s][e], h[e]);
+        o.v[e] = Elem<F>::down(h[e]);
+      }
+      if (t0 + s < te) *reinterpret_cast<Pack<F, E>*>(op + (t0 + s) * out.st) = o;
+    }
+    if (te == T && T - t0 <= kSteps) {  // the steps past T kept h
+#pragma unroll
+      for (int e = 0; e < E; ++e) h_n[q.ch + e] = h[e];
+    }
+  };
+  if (tb < te) load(tb + q.g * kSteps, rz[0], rv[0], rr[0]);
+  int t = tb;
+  for (; t < te; t += 2 * chunk) {
+    if (t + chunk < te) load(t + chunk + q.g * kSteps, rz[1], rv[1], rr[1]);
+    step(t, 0, rz[0], rv[0], rr[0]);
+    if (t + chunk >= te) break;
+    if (t + 2 * chunk < te) load(t + 2 * chunk + q.g * kSteps, rz[0], rv[0], rr[0]);
+    step(t + chunk, 1, rz[1], rv[1], rr[1]);
+  }
+  if (T == 0 && q.g == 0 && q.ok) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) h_n[q.ch + e] = x[e];
+  }
+}
+
+// The map of segment blockIdx.y (never the last, so every step is below T), of whole 8-step parts
+// for each group.
+template <int F, int E, bool RESET>
+__global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv, Stream reset,
+                                                                      float2* __restrict__ maps, int T, int B, int H,
+                                                                      int seg_steps) {
+  using T_ = typename Elem<F>::T;
+  __shared__ Floats<2 * E> sm[kMaxWaves][kLanes];
+  const Place<E> q(B, H);
+  const int part = seg_steps / (q.nw * 2), t0 = blockIdx.y * seg_steps + q.g * part;
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
+  float A[E], V[E], x[E], in[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    A[e] = 1.f;
+    V[e] = x[e] = 0.f;
+  }
+  for (int k = 0; k < part; k += kSteps) {
+    Pack<F, E> z[kSteps], v[kSteps];
+    unsigned char r[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const T_* p = zp + (t0 + k + s) * zv.st;
+      z[s] = load_pack<F, E>(p);
+      v[s] = load_pack<F, E>(p + H);
+    }
+    if constexpr (RESET) load_resets(reset, q.b, t0 + k, T, r);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        Gates g = gates_of(Elem<F>::up(z[s].v[e]));
+        if (RESET && r[s]) g.f = __uint_as_float(kCutBits);
+        V[e] = apply<RESET>(g.f, g.w * Elem<F>::up(v[s].v[e]), V[e]);
+        A[e] = compose<RESET>(g.f, A[e]);
+      }
+  }
+  join<E, RESET, false>(q, A, V, x, in, sm);  // x: V of the whole segment
+  if (threadIdx.x < kLanes && q.ok) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float a = 1.f;
+      for (int u = 0; u < q.nw; ++u) a = compose<RESET>(sm[u][q.c].v[2 * e], a);
+      maps[(size_t)blockIdx.y * B * H + q.ch + e] = float2{a, x[e]};
+    }
+  }
+}
+
+template <int F, int E, bool RESET>
+__global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, Stream reset,
+                                                                  const float* __restrict__ ck, Stream dout,
+                                                                  const float* __restrict__ dh_n, OutStream dzv,
+                                                                  float* __restrict__ dh0,
+                                                                  const float2* __restrict__ maps, int T, int B, int H,
+                                                                  int seg_steps) {
+  using T_ = typename Elem<F>::T;
+  __shared__ Floats<2 * E> sm[2][kMaxWaves][kLanes];
+  const Place<E> q(B, H);
+  const int C = B * H, chunk = q.nw * 2 * kSteps;
+  const int seg = blockIdx.y, tb = seg * seg_steps, te = min(T, tb + seg_steps);
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = dh_n ? dh_n[q.ch + e] : 0.f;
+  enter_segment<E, RESET, true>(maps, C, q.ch, seg, gridDim.y, x);
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
+  const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + q.j;
+  T_* gp = static_cast<T_*>(dzv.p) + q.b * dzv.sb + q.j;
+
+  Pack<F, E> rz[2][kSteps], rv[2][kSteps], rd[2][kSteps];
+  Floats<E> rh[2];
+  unsigned char rr[2][kSteps];
+  auto load = [&](int t0, int i) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int t = min(t0 + s, T - 1);
+      const T_* p = zp + t * zv.st;
+      rz[i][s] = load_pack<F, E>(p);
+      rv[i][s] = load_pack<F, E>(p + H);
+      if (dout.p)
+        rd[i][s] = load_pack<F, E>(dp + t * dout.st);
+      else
+        rd[i][s] = Pack<F, E>{};
+    }
+    rh[i] = *reinterpret_cast<const Floats<E>*>(ck + (size_t)(min(t0, T - 1) / kSteps) * C + q.ch);
+    if constexpr (RESET) load_resets(reset, q.b, t0, T, rr[i]);
+  };
+  auto step = [&](int t1, int i) {
+    const int t0 = t1 + q.g * kSteps;
+    float f[kSteps][E], w[kSteps][E], hp[kSteps][E], A[E], V[E], U[E], h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      A[e] = 1.f;
+      V[e] = 0.f;
+      h[e] = rh[i].v[e];
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const Gates g = gates_of(Elem<F>::up(rz[i][s].v[e]));
+        const float v = Elem<F>::up(rv[i][s].v[e]);
+        f[s][e] = g.f;
+        w[s][e] = g.w;
+        hp[s][e] = RESET && rr[i][s] ? 0.f : h[e];
+        h[e] = RESET && rr[i][s] ? g.w * v : __builtin_fmaf(g.f, h[e], g.w * v);
+      }
+    }
+#pragma unroll
+    for (int s = kSteps - 1; s >= 0; --s) {
+      const bool in = t0 + s < te;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool cut = RESET && rr[i][s];
+        const float d = Elem<F>::up(rd[i][s].v[e]);
+        if (in) {
+          V[e] = cut ? 0.f : f[s][e] * (d + V[e]);
+          A[e] = cut ? __uint_as_float(kCutBits) : compose<RESET>(f[s][e], A[e]);
+        }
+      }
+    }
+    join<E, RESET, true>(q, A, V, x, U, sm[i]);
+    if (!q.ok || t0 >= te) return;
+#pragma unroll
+    for (int s = kSteps - 1; s >= 0; --s) {
+      if (t0 + s < te) {
+        Pack<F, E> oz, ov;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float G = Elem<F>::up(rd[i][s].v[e]) + U[e];
+          const float v = Elem<F>::up(rv[i][s].v[e]);
+          oz.v[e] = Elem<F>::down(G * (hp[s][e] - v) * (f[s][e] * w[s][e]));
+          ov.v[e] = Elem<F>::down(w[s][e] * G);
+          U[e] = RESET && rr[i][s] ? 0.f : f[s][e] * G;
+        }
+        T_* const p = gp + (t0 + s) * dzv.st;
+        *reinterpret_cast<Pack<F, E>*>(p) = oz;
+        *reinterpret_cast<Pack<F, E>*>(p + H) = ov;
+      }
+    }
+    if (t0 == 0 && dh0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) dh0[q.ch + e] = U[e];
+    }
+  };
+  const int n = (te - tb + chunk - 1) / chunk;  // chunks, from the last to the first
+  if (n > 0) load(tb + (n - 1) * chunk + q.g * kSteps, 0);
+  for (int k = n - 1; k >= 0; k -= 2) {
+    if (k >= 1) load(tb + (k - 1) * chunk + q.g * kSteps, 1);
+    step(tb + k * chunk, 0);
+    if (k < 1) break;
+    if (k >= 2) load(tb + (k - 2) * chunk + q.g * kSteps, 0);
+    step(tb + (k - 1) * chunk, 1);
+  }
+  if (T == 0 && dh0 && q.g == 0 && q.ok) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) dh0[q.ch + e] = x[e];
+  }
+}
+
+// The reverse map of segment blockIdx.y + 1, which ends at min(T, ..).
+template <int F, int E, bool RESET>
+__global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_map_kernel(Stream zv, Stream reset, Stream dout,
+                                                                      float2* __restrict__ maps, int T, int B, int H,
+                                                                      int seg_steps) {
+  using T_ = typename Elem<F>::T;
+  __shared__ Floats<2 * E> sm[kMaxWaves][kLanes];
+  const Place<E> q(B, H);
+  const int part = seg_steps / (q.nw * 2), t0 = (blockIdx.y + 1) * seg_steps + q.g * part;
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
+  const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + q.j;
+  float A[E], V[E], x[E], in[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    A[e] = 1.f;
+    V[e] = x[e] = 0.f;
+  }
+  for (int k = part - kSteps; k >= 0; k -= kSteps) {
+    if (t0 + k >= T) continue;
+    Pack<F, E> z[kSteps], d[kSteps];
+    unsigned char r[kSteps];
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const int t = min(t0 + k + s, T - 1);
+      z[s] = load_pack<F, E>(zp + t * zv.st);
+      d[s] = Pack<F, E>{};
+      if (dout.p) d[s] = load_pack<F, E>(dp + t * dout.st);
+    }
+    if constexpr (RESET) load_resets(reset, q.b, t0 + k, T, r);
+#pragma unroll
+    for (int s = kSteps - 1; s >= 0; --s)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (t0 + k + s < T) {
+          const float f = gates_of(Elem<F>::up(z[s].v[e])).f;
+          const bool cut = RESET && r[s];
+          V[e] = cut ? 0.f : f * (Elem<F>::up(d[s].v[e]) + V[e]);
+          A[e] = cut ? __uint_as_float(kCutBits) : compose<RESET>(f, A[e]);
+        }
+  }
+  join<E, RESET, true>(q, A, V, x, in, sm);
+  if (threadIdx.x < kLanes && q.ok) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float a = 1.f;
+      for (int u = q.nw - 1; u >= 0; --u) a = compose<RESET>(sm[u][q.c].v[2 * e], a);
+      maps[(size_t)blockIdx.y * B * H + q.ch + e] = float2{a, x[e]};
+    }
+  }
+}
+
+// A single step: one thread per E channels.  h_n may be h0.
+template <int F, int E, bool RESET>
+__global__ __launch_bounds__(256) void gated_step_kernel(Stream zv, const float* h0, Stream reset, OutStream out,
+                                                         float* h_n, float* ck, int B, int H) {
+  using T_ = typename Elem<F>::T;
+  const int ch = (blockIdx.x * 256 + threadIdx.x) * E;
+  if (ch >= B * H) return;
+  const int b = ch / H, j = ch - b * H;
+  const T_* p = static_cast<const T_*>(zv.p) + b * zv.sb + j;
+  const Pack<F, E> z = load_pack<F, E>(p), v = load_pack<F, E>(p + H);
+  Floats<E> h{};
+  if (h0) h = *reinterpret_cast<const Floats<E>*>(h0 + ch);
+  if (ck) *reinterpret_cast<Floats<E>*>(ck + ch) = h;
+  const bool cut = RESET && static_cast<const unsigned char*>(reset.p)[b * reset.sb];
+  Pack<F, E> o;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const Gates g = gates_of(Elem<F>::up(z.v[e]));
+    const float wv = g.w * Elem<F>::up(v.v[e]);
+    h.v[e] = cut ? wv : __builtin_fmaf(g.f, h.v[e], wv);
+    o.v[e] = Elem<F>::down(h.v[e]);
+  }
+  *reinterpret_cast<Pack<F, E>*>(static_cast<T_*>(out.p) + b * out.sb + j) = o;
+  *reinterpret_cast<Floats<E>*>(h_n + ch) = h;
+}
+
+// The shape of a call's launches: waves of a workgroup, workgroups over the channels, segments.
+struct GatedPlan {
+  int waves, tiles, nseg, seg_steps;
+};
+GatedPlan plan_gated(int T, int B, int H, int E) {
+  GatedPlan p;
+  const long C = (long)B * H;
+  p.tiles = (int)((C + kLanes * E - 1) / (kLanes * E));
+  p.waves = 1;
+  while (p.waves < kMaxWaves && p.waves * 2 * kSteps < T) p.waves *= 2;
+  const int chunk = p.waves * 2 * kSteps, nchunks = (T + chunk - 1) / chunk;
+  p.nseg = 1;
+  p.seg_steps = std::max(1, nchunks) * chunk;
+  if (p.tiles < 192 && nchunks >= 4) {
+    const int want = std::min(nchunks / 2, (512 + p.tiles - 1) / p.tiles);
+    const int per = (nchunks + want - 1) / want;
+    p.seg_steps = per * chunk;
+    p.nseg = (nchunks + per - 1) / per;
+  }
+  return p;
 }
 
 int check_gated(const char* who, int T, int B, int H, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
   return check_shape(who, T, B, 0, H);
+}
+
+// Channels per thread: two where every row of pairs is aligned.
+int channels_each(int H, int es, std::initializer_list<std::pair<const void*, std::pair<long long, long long>>> ps) {
+  if (H % 2) return 1;
+  for (const auto& p : ps) {
+    if (reinterpret_cast<uintptr_t>(p.first) % (2 * es) || p.second.first % 2 || p.second.second % 2) return 1;
+  }
+  return 2;
+}
+
+// f(fmt, channels each, reset) as integral constants.
+template <class Fn>
+int with_instance(int fmt, int e, bool reset, Fn f) {
+  return with_fmt(fmt, [&](auto F) {
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (e == 2) return reset ? f(F, Two{}, std::true_type{}) : f(F, Two{}, std::false_type{});
+    return reset ? f(F, One{}, std::true_type{}) : f(F, One{}, std::false_type{});
+  });
 }
 
 }  // namespace
@@ -105,9 +552,14 @@ using namespace hsl;
 
 extern "C" {
 
-int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kGatedCk - 1) / kGatedCk; }
+int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kSteps - 1) / kSteps; }
 
-size_t hsl_gated_ws_bytes(int T, int B, int H) { return 0; }
+size_t hsl_gated_ws_bytes(int T, int B, int H) {
+  if (T < 0 || B < 0 || H < 0) return 0;
+  size_t n = 0;
+  for (int e = 1; e <= 2; ++e) n = std::max(n, (size_t)(plan_gated(T, B, H, e).nseg - 1));
+  return n * B * H * sizeof(float2);
+}
 
 int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h0, const void* reset, long long rs_t,
                   long long rs_b, void* out, long long out_t, long long out_b, float* h_n, float* ck, void* ws,
@@ -116,10 +568,30 @@ int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h
   if (B == 0 || H == 0) return HSL_OK;
   if (!h_n || (T > 0 && (!zv || !out))) return fail(HSL_ERR_ARG, "hsl_gated_fwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return with_fmt(fmt, [&](auto f) {
-    hipLaunchKernelGGL(gated_fwd_kernel<decltype(f)::value>, dim3((B * H + 255) / 256), dim3(256), 0, s,
-                       Stream{zv, zv_t, zv_b}, h0, Stream{reset, rs_t, rs_b}, OutStream{out, out_t, out_b}, h_n, ck, T,
-                       B, H);
+  const int es = fmt == kElemF32 ? 4 : 2;
+  int e = channels_each(H, es, {{zv, {zv_t, zv_b}}, {out, {out_t, out_b}}});
+  if (reinterpret_cast<uintptr_t>(ck) % 8 || (T == 1 && (reinterpret_cast<uintptr_t>(h0) % 8 ||
+                                                         reinterpret_cast<uintptr_t>(h_n) % 8)))
+    e = 1;
+  const GatedPlan p = plan_gated(T, B, H, e);
+  if (p.nseg > 1 && (!ws || ws_bytes < hsl_gated_ws_bytes(T, B, H)))
+    return fail(HSL_ERR_ARG, "hsl_gated_fwd: workspace %zu bytes, need %zu", ws_bytes, hsl_gated_ws_bytes(T, B, H));
+  float2* const maps = static_cast<float2*>(ws);
+  const Stream z{zv, zv_t, zv_b}, r{reset, rs_t, rs_b};
+  const OutStream o{out, out_t, out_b};
+  return with_instance(fmt, e, reset != nullptr, [&](auto F, auto E, auto R) {
+    constexpr int kF = decltype(F)::value, kE = decltype(E)::value;
+    constexpr bool kR = decltype(R)::value;
+    if (T == 1) {
+      const int n = (B * H + kE * 256 - 1) / (kE * 256);
+      hipLaunchKernelGGL((gated_step_kernel<kF, kE, kR>), dim3(n), dim3(256), 0, s, z, h0, r, o, h_n, ck, B, H);
+    } else {
+      if (p.nseg > 1)
+        hipLaunchKernelGGL((gated_fwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z, r,
+                           maps, T, B, H, p.seg_steps);
+      hipLaunchKernelGGL((gated_fwd_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, h0, r, o,
+                         h_n, ck, maps, T, B, H, p.seg_steps);
+    }
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
   });
@@ -133,10 +605,23 @@ int hsl_gated_bwd(const void* zv, long long zv_t, long long zv_b, const void* re
   if (B == 0 || H == 0) return HSL_OK;
   if (T > 0 && (!zv || !ck || !dzv)) return fail(HSL_ERR_ARG, "hsl_gated_bwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return with_fmt(fmt, [&](auto f) {
-    hipLaunchKernelGGL(gated_bwd_kernel<decltype(f)::value>, dim3((B * H + 255) / 256), dim3(256), 0, s,
-                       Stream{zv, zv_t, zv_b}, Stream{reset, rs_t, rs_b}, ck, Stream{dout, do_t, do_b}, dh_n,
-                       OutStream{dzv, dz_t, dz_b}, dh0, T, B, H);
+  const int es = fmt == kElemF32 ? 4 : 2;
+  int e = channels_each(H, es, {{zv, {zv_t, zv_b}}, {dout, {do_t, do_b}}, {dzv, {dz_t, dz_b}}});
+  if (reinterpret_cast<uintptr_t>(ck) % 8) e = 1;
+  const GatedPlan p = plan_gated(T, B, H, e);
+  if (p.nseg > 1 && (!ws || ws_bytes < hsl_gated_ws_bytes(T, B, H)))
+    return fail(HSL_ERR_ARG, "hsl_gated_bwd: workspace %zu bytes, need %zu", ws_bytes, hsl_gated_ws_bytes(T, B, H));
+  float2* const maps = static_cast<float2*>(ws);
+  const Stream z{zv, zv_t, zv_b}, r{reset, rs_t, rs_b}, d{dout, do_t, do_b};
+  const OutStream g{dzv, dz_t, dz_b};
+  return with_instance(fmt, e, reset != nullptr, [&](auto F, auto E, auto R) {
+    constexpr int kF = decltype(F)::value, kE = decltype(E)::value;
+    constexpr bool kR = decltype(R)::value;
+    if (p.nseg > 1)
+      hipLaunchKernelGGL((gated_bwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z, r,
+                         d, maps, T, B, H, p.seg_steps);
+    hipLaunchKernelGGL((gated_bwd_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, r, ck, d,
+                       dh_n, g, dh0, maps, T, B, H, p.seg_steps);
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
   });
