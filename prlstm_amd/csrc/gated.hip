@@ -15,8 +15,6 @@
 // stream is read and written once.  With few channels the time is cut into segments that run as
 // workgroups of their own after a pass that composes each segment's map.
 #include <algorithm>
-#include <initializer_list>
-#include <utility>
 
 #include "lm.h"
 
@@ -31,9 +29,16 @@ struct Gates {
   float f, w;
 };
 // e = exp(-|z|) is at most 1, so neither gate is a difference: the larger is 1 / (1 + e), the
-// smaller e / (1 + e).
+// smaller e / (1 + e).  A 16-bit z has an error of 2^-9 (bf16) or 2^-12 of itself, against which
+// that of rounding z log2 e to fp32 (|z| 2^-24 of e) does not count, so exp is one product and
+// v_exp_f32 there; an fp32 z gets the corrected exp_f.
+template <int F>
 __device__ __forceinline__ Gates gates_of(float z) {
-  const float e = exp_f(-__builtin_fabsf(z));
+  float e;
+  if constexpr (F == kElemF32)
+    e = exp_f(-__builtin_fabsf(z));
+  else
+    e = __builtin_amdgcn_exp2f(-__builtin_fabsf(z) * 1.44269502162933349609375f);
   const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
   return z >= 0.f ? Gates{big, small} : Gates{small, big};
 }
@@ -67,46 +72,77 @@ struct OutStream {
   long long st, sb;
 };
 
-// E neighbouring elements.
+// E neighbouring elements, at any element's alignment (global memory takes unaligned accesses).
 template <int F, int E>
-struct alignas(sizeof(typename Elem<F>::T) * E) Pack {
+struct Pack {
   typename Elem<F>::T v[E];
 };
 template <int F, int E>
 __device__ __forceinline__ Pack<F, E> load_pack(const typename Elem<F>::T* p) {
-  return *reinterpret_cast<const Pack<F, E>*>(p);
+  Pack<F, E> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <int F, int E>
+__device__ __forceinline__ void store_pack(typename Elem<F>::T* p, const Pack<F, E>& v) {
+  __builtin_memcpy(p, &v, sizeof(v));
 }
 template <int E>
-struct alignas(4 * E) Floats {
+struct Floats {
   float v[E];
 };
+template <int E>
+__device__ __forceinline__ Floats<E> load_floats(const float* p) {
+  Floats<E> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <int E>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[E]) {
+  __builtin_memcpy(p, v, sizeof(v));
+}
 
-// One workgroup's channels and groups.
+// A thread's place: E neighbouring channels j .. j+E-1 of batch row b.  Where H is odd the last
+// thread of a row takes the last two channels, one of them beside its neighbour: both compute and
+// store the same values.
 template <int E>
 struct Place {
   int lane, w, c, g, nw;  // lane in the wave, wave, lane in the group, group in the workgroup, waves
-  int ch;                 // first of the thread's E channels (b * H + j), clamped into range
-  int b, j;
+  int ch, b, j;           // ch = b H + j; clamped into range
   bool ok;
+  __device__ __forceinline__ void channels(int i, int B, int H) {
+    const int per = (H + E - 1) / E;
+    ok = i < B * per;
+    i = ok ? i : B * per - 1;
+    b = i / per;
+    j = min((i - b * per) * E, H - E);
+    ch = b * H + j;
+  }
   __device__ __forceinline__ Place(int B, int H) {
     lane = threadIdx.x & 63;
     w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     nw = blockDim.x >> 6;
     c = lane % kLanes;
     g = threadIdx.x / kLanes;
-    const int C = B * H, first = (blockIdx.x * kLanes + c) * E;
-    ok = first < C;
-    ch = ok ? first : C - E;
-    b = ch / H;
-    j = ch - b * H;
+    channels(blockIdx.x * kLanes + c, B, H);
   }
 };
 
-// The reset flags of a group's steps t0 .. t0+7 as bits (steps at or past T: none).
-__device__ __forceinline__ void load_resets(const Stream& reset, int b, int t0, int T, unsigned char (&r)[kSteps]) {
-  const auto* p = static_cast<const unsigned char*>(reset.p) + b * reset.sb;
+// The reset flags of the 8 steps from t0 on, p at its first (flags of steps past T are not used).
+template <bool TAIL>
+__device__ __forceinline__ void load_resets(const unsigned char* p, long long st, int t0, int T,
+                                            unsigned char (&r)[kSteps]) {
+  if (!TAIL && st == 1) {
+    __builtin_memcpy(r, p, kSteps);
+    return;
+  }
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) r[s] = p[min(t0 + s, T - 1) * reset.st];
+  for (int s = 0; s < kSteps; ++s) r[s] = TAIL && t0 + s >= T ? 0 : p[s * st];
+}
+
+// A of the composed map of a group's steps, from the product and the smallest of the gates.
+__device__ __forceinline__ float held(float prod, float least) {
+  return fmaxf(prod, fminf(least, __uint_as_float(1u)));
 }
 
 // Joins the maps of a chunk's groups: from each thread's map (A, V) of its group, first (REV:
@@ -189,49 +225,72 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = h0 ? h0[q.ch + e] : 0.f;
   enter_segment<E, RESET, false>(maps, C, q.ch, seg, gridDim.y, x);
-  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
-  T_* op = static_cast<T_*>(out.p) + q.b * out.sb + q.j;
+  // the group's first step of the chunk that is loaded (zp, rp) and of the one that is run (op)
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + (tb + q.g * kSteps) * zv.st + q.j;
+  const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + (tb + q.g * kSteps) * reset.st;
+  T_* op = static_cast<T_*>(out.p) + q.b * out.sb + (tb + q.g * kSteps) * out.st + q.j;
+  float* cp = ck + (size_t)(tb / kSteps + q.g) * C + q.ch;
 
   Pack<F, E> rz[2][kSteps], rv[2][kSteps];
   unsigned char rr[2][kSteps];
-  auto load = [&](int t0, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps], unsigned char(&r)[kSteps]) {
+  auto load = [&](int t1, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps], unsigned char(&r)[kSteps]) {
+    if (t1 + chunk <= te) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      const T_* p = zp + min(t0 + s, T - 1) * zv.st;
-      z[s] = load_pack<F, E>(p);
-      v[s] = load_pack<F, E>(p + H);
+      for (int s = 0; s < kSteps; ++s) {
+        z[s] = load_pack<F, E>(zp + s * zv.st);
+        v[s] = load_pack<F, E>(zp + s * zv.st + H);
+      }
+      if constexpr (RESET) load_resets<false>(rp, reset.st, 0, T, r);
+    } else {  // the last chunk: steps past T are not read
+      const int t0 = t1 + q.g * kSteps;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        z[s] = v[s] = Pack<F, E>{};
+        if (t0 + s < te) {
+          z[s] = load_pack<F, E>(zp + s * zv.st);
+          v[s] = load_pack<F, E>(zp + s * zv.st + H);
+        }
+      }
+      if constexpr (RESET) load_resets<true>(rp, reset.st, t0, te, r);
     }
-    if constexpr (RESET) load_resets(reset, q.b, t0, T, r);
+    zp += chunk * zv.st;
+    if constexpr (RESET) rp += chunk * reset.st;
   };
-  auto step = [&](int t1, int par, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps], unsigned char(&r)[kSteps]) {
+  auto step = [&](auto tail, int t1, int par, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps],
+                  unsigned char(&r)[kSteps]) {
+    constexpr bool TAIL = decltype(tail)::value;  // the chunk with step T-1: later ones keep the state
     const int t0 = t1 + q.g * kSteps;
-    float f[kSteps][E], wv[kSteps][E], A[E], V[E], h[E];
+    float f[kSteps][E], wv[kSteps][E], A[E], V[E], h[E], least[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      A[e] = 1.f;
+      A[e] = least[e] = 1.f;
       V[e] = 0.f;
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const bool in = t0 + s < te;
+      const bool in = !TAIL || t0 + s < te;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const Gates g = gates_of(Elem<F>::up(z[s].v[e]));
+        const Gates g = gates_of<F>(Elem<F>::up(z[s].v[e]));
         f[s][e] = in ? g.f : 1.f;
         wv[s][e] = in ? g.w * Elem<F>::up(v[s].v[e]) : 0.f;
         if (RESET && in && r[s]) f[s][e] = __uint_as_float(kCutBits);
         V[e] = apply<RESET>(f[s][e], wv[s][e], V[e]);
-        A[e] = compose<RESET>(f[s][e], A[e]);
+        if constexpr (RESET) {
+          A[e] = compose<RESET>(f[s][e], A[e]);
+        } else {
+          A[e] *= f[s][e];
+          least[e] = fminf(least[e], f[s][e]);
+        }
       }
     }
-    join<E, RESET, false>(q, A, V, x, h, sm[par]);
-    if (!q.ok || t0 >= te) return;
-    if (ck) {
-      Floats<E> o;
+    if constexpr (!RESET) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) o.v[e] = h[e];
-      *reinterpret_cast<Floats<E>*>(ck + (size_t)(t0 / kSteps) * C + q.ch) = o;
+      for (int e = 0; e < E; ++e) A[e] = held(A[e], least[e]);
     }
+    join<E, RESET, false>(q, A, V, x, h, sm[par]);
+    if (!q.ok || (TAIL && t0 >= te)) return;
+    if (ck) store_floats(cp, h);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Pack<F, E> o;
@@ -240,26 +299,26 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
         h[e] = apply<RESET>(f[s][e], wv[s][e], h[e]);
         o.v[e] = Elem<F>::down(h[e]);
       }
-      if (t0 + s < te) *reinterpret_cast<Pack<F, E>*>(op + (t0 + s) * out.st) = o;
+      if (!TAIL || t0 + s < te) store_pack<F, E>(op + s * out.st, o);
     }
-    if (te == T && T - t0 <= kSteps) {  // the steps past T kept h
-#pragma unroll
-      for (int e = 0; e < E; ++e) h_n[q.ch + e] = h[e];
+    if (TAIL && te == T && T - t0 <= kSteps) store_floats(h_n + q.ch, h);
+    op += chunk * out.st;
+    cp += (size_t)(chunk / kSteps) * C;
+  };
+  auto run = [&](int t, int i) {
+    if (t + chunk < te) {
+      load(t + chunk, rz[i ^ 1], rv[i ^ 1], rr[i ^ 1]);
+      step(std::false_type{}, t, i, rz[i], rv[i], rr[i]);
+    } else {
+      step(std::true_type{}, t, i, rz[i], rv[i], rr[i]);
     }
   };
-  if (tb < te) load(tb + q.g * kSteps, rz[0], rv[0], rr[0]);
-  int t = tb;
-  for (; t < te; t += 2 * chunk) {
-    if (t + chunk < te) load(t + chunk + q.g * kSteps, rz[1], rv[1], rr[1]);
-    step(t, 0, rz[0], rv[0], rr[0]);
-    if (t + chunk >= te) break;
-    if (t + 2 * chunk < te) load(t + 2 * chunk + q.g * kSteps, rz[0], rv[0], rr[0]);
-    step(t + chunk, 1, rz[1], rv[1], rr[1]);
+  if (tb < te) load(tb, rz[0], rv[0], rr[0]);
+  for (int t = tb; t < te; t += 2 * chunk) {
+    run(t, 0);
+    if (t + chunk < te) run(t + chunk, 1);
   }
-  if (T == 0 && q.g == 0 && q.ok) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) h_n[q.ch + e] = x[e];
-  }
+  if (T == 0 && q.g == 0 && q.ok) store_floats(h_n + q.ch, x);
 }
 
 // The map of segment blockIdx.y (never the last, so every step is below T), of whole 8-step parts
@@ -272,7 +331,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv
   __shared__ Floats<2 * E> sm[kMaxWaves][kLanes];
   const Place<E> q(B, H);
   const int part = seg_steps / (q.nw * 2), t0 = blockIdx.y * seg_steps + q.g * part;
-  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + t0 * zv.st + q.j;
+  const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + t0 * reset.st;
   float A[E], V[E], x[E], in[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -284,16 +344,19 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv
     unsigned char r[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const T_* p = zp + (t0 + k + s) * zv.st;
-      z[s] = load_pack<F, E>(p);
-      v[s] = load_pack<F, E>(p + H);
+      z[s] = load_pack<F, E>(zp + s * zv.st);
+      v[s] = load_pack<F, E>(zp + s * zv.st + H);
     }
-    if constexpr (RESET) load_resets(reset, q.b, t0 + k, T, r);
+    zp += kSteps * zv.st;
+    if constexpr (RESET) {
+      load_resets<false>(rp, reset.st, 0, T, r);
+      rp += kSteps * reset.st;
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        Gates g = gates_of(Elem<F>::up(z[s].v[e]));
+        Gates g = gates_of<F>(Elem<F>::up(z[s].v[e]));
         if (RESET && r[s]) g.f = __uint_as_float(kCutBits);
         V[e] = apply<RESET>(g.f, g.w * Elem<F>::up(v[s].v[e]), V[e]);
         A[e] = compose<RESET>(g.f, A[e]);
@@ -326,34 +389,46 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] = dh_n ? dh_n[q.ch + e] : 0.f;
   enter_segment<E, RESET, true>(maps, C, q.ch, seg, gridDim.y, x);
-  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
-  const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + q.j;
-  T_* gp = static_cast<T_*>(dzv.p) + q.b * dzv.sb + q.j;
+  // pointers at the group's first step of the chunk that is loaded (gp: run), from the last one on
+  const int n = (te - tb + chunk - 1) / chunk;
+  const long long last = tb + (n - 1) * chunk + q.g * kSteps;
+  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + last * zv.st + q.j;
+  const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + last * dout.st + q.j;
+  const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + last * reset.st;
+  const float* cp = ck + (last / kSteps) * C + q.ch;
+  T_* gp = static_cast<T_*>(dzv.p) + q.b * dzv.sb + last * dzv.st + q.j;
 
   Pack<F, E> rz[2][kSteps], rv[2][kSteps], rd[2][kSteps];
   Floats<E> rh[2];
   unsigned char rr[2][kSteps];
-  auto load = [&](int t0, int i) {
+  auto load = [&](auto tail, int t1, int i) {
+    constexpr bool TAIL = decltype(tail)::value;  // steps past T are not read
+    const int t0 = t1 + q.g * kSteps;
+    rh[i] = Floats<E>{};
+    if (!TAIL || t0 < te) rh[i] = load_floats<E>(cp);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int t = min(t0 + s, T - 1);
-      const T_* p = zp + t * zv.st;
-      rz[i][s] = load_pack<F, E>(p);
-      rv[i][s] = load_pack<F, E>(p + H);
-      if (dout.p)
-        rd[i][s] = load_pack<F, E>(dp + t * dout.st);
-      else
-        rd[i][s] = Pack<F, E>{};
+      if (TAIL) rz[i][s] = rv[i][s] = Pack<F, E>{};
+      rd[i][s] = Pack<F, E>{};
+      if (!TAIL || t0 + s < te) {
+        rz[i][s] = load_pack<F, E>(zp + s * zv.st);
+        rv[i][s] = load_pack<F, E>(zp + s * zv.st + H);
+        if (dout.p) rd[i][s] = load_pack<F, E>(dp + s * dout.st);
+      }
     }
-    rh[i] = *reinterpret_cast<const Floats<E>*>(ck + (size_t)(min(t0, T - 1) / kSteps) * C + q.ch);
-    if constexpr (RESET) load_resets(reset, q.b, t0, T, rr[i]);
+    if constexpr (RESET) load_resets<TAIL>(rp, reset.st, t0, te, rr[i]);
+    zp -= chunk * zv.st;
+    dp -= chunk * dout.st;
+    if constexpr (RESET) rp -= chunk * reset.st;
+    cp -= (size_t)(chunk / kSteps) * C;
   };
-  auto step = [&](int t1, int i) {
+  auto step = [&](auto tail, int t1, int i) {
+    constexpr bool TAIL = decltype(tail)::value;  // the chunk with step T-1: U passes later ones
     const int t0 = t1 + q.g * kSteps;
-    float f[kSteps][E], w[kSteps][E], hp[kSteps][E], A[E], V[E], U[E], h[E];
+    float f[kSteps][E], w[kSteps][E], hp[kSteps][E], A[E], V[E], U[E], h[E], least[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      A[e] = 1.f;
+      A[e] = least[e] = 1.f;
       V[e] = 0.f;
       h[e] = rh[i].v[e];
     }
@@ -361,7 +436,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const Gates g = gates_of(Elem<F>::up(rz[i][s].v[e]));
+        const Gates g = gates_of<F>(Elem<F>::up(rz[i][s].v[e]));
         const float v = Elem<F>::up(rv[i][s].v[e]);
         f[s][e] = g.f;
         w[s][e] = g.w;
@@ -371,54 +446,60 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     }
 #pragma unroll
     for (int s = kSteps - 1; s >= 0; --s) {
-      const bool in = t0 + s < te;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const bool cut = RESET && rr[i][s];
         const float d = Elem<F>::up(rd[i][s].v[e]);
-        if (in) {
+        if (!TAIL || t0 + s < te) {
           V[e] = cut ? 0.f : f[s][e] * (d + V[e]);
-          A[e] = cut ? __uint_as_float(kCutBits) : compose<RESET>(f[s][e], A[e]);
+          if constexpr (RESET) {
+            A[e] = compose<RESET>(cut ? __uint_as_float(kCutBits) : f[s][e], A[e]);
+          } else {
+            A[e] *= f[s][e];
+            least[e] = fminf(least[e], f[s][e]);
+          }
         }
       }
     }
+    if constexpr (!RESET) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) A[e] = held(A[e], least[e]);
+    }
     join<E, RESET, true>(q, A, V, x, U, sm[i]);
-    if (!q.ok || t0 >= te) return;
+    T_* const p0 = gp;
+    gp -= chunk * dzv.st;
+    if (!q.ok || (TAIL && t0 >= te)) return;
 #pragma unroll
     for (int s = kSteps - 1; s >= 0; --s) {
-      if (t0 + s < te) {
+      if (!TAIL || t0 + s < te) {
         Pack<F, E> oz, ov;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float G = Elem<F>::up(rd[i][s].v[e]) + U[e];
-          const float v = Elem<F>::up(rv[i][s].v[e]);
-          oz.v[e] = Elem<F>::down(G * (hp[s][e] - v) * (f[s][e] * w[s][e]));
-          ov.v[e] = Elem<F>::down(w[s][e] * G);
+          const float v = Elem<F>::up(rv[i][s].v[e]), dv = w[s][e] * G;
+          oz.v[e] = Elem<F>::down(dv * ((hp[s][e] - v) * f[s][e]));
+          ov.v[e] = Elem<F>::down(dv);
           U[e] = RESET && rr[i][s] ? 0.f : f[s][e] * G;
         }
-        T_* const p = gp + (t0 + s) * dzv.st;
-        *reinterpret_cast<Pack<F, E>*>(p) = oz;
-        *reinterpret_cast<Pack<F, E>*>(p + H) = ov;
+        store_pack<F, E>(p0 + s * dzv.st, oz);
+        store_pack<F, E>(p0 + s * dzv.st + H, ov);
       }
     }
-    if (t0 == 0 && dh0) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) dh0[q.ch + e] = U[e];
-    }
+    if (t0 == 0 && dh0) store_floats(dh0 + q.ch, U);
   };
-  const int n = (te - tb + chunk - 1) / chunk;  // chunks, from the last to the first
-  if (n > 0) load(tb + (n - 1) * chunk + q.g * kSteps, 0);
-  for (int k = n - 1; k >= 0; k -= 2) {
-    if (k >= 1) load(tb + (k - 1) * chunk + q.g * kSteps, 1);
-    step(tb + k * chunk, 0);
+  if (n > 0) {
+    load(std::true_type{}, tb + (n - 1) * chunk, 0);
+    if (n > 1) load(std::false_type{}, tb + (n - 2) * chunk, 1);
+    step(std::true_type{}, tb + (n - 1) * chunk, 0);
+  }
+  for (int k = n - 2; k >= 0; k -= 2) {
+    if (k >= 1) load(std::false_type{}, tb + (k - 1) * chunk, 0);
+    step(std::false_type{}, tb + k * chunk, 1);
     if (k < 1) break;
-    if (k >= 2) load(tb + (k - 2) * chunk + q.g * kSteps, 0);
-    step(tb + (k - 1) * chunk, 1);
+    if (k >= 2) load(std::false_type{}, tb + (k - 2) * chunk, 1);
+    step(std::false_type{}, tb + (k - 1) * chunk, 0);
   }
-  if (T == 0 && dh0 && q.g == 0 && q.ok) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) dh0[q.ch + e] = x[e];
-  }
+  if (T == 0 && dh0 && q.g == 0 && q.ok) store_floats(dh0 + q.ch, x);
 }
 
 // The reverse map of segment blockIdx.y + 1, which ends at min(T, ..).
@@ -429,9 +510,10 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_map_kernel(Stream zv
   using T_ = typename Elem<F>::T;
   __shared__ Floats<2 * E> sm[kMaxWaves][kLanes];
   const Place<E> q(B, H);
-  const int part = seg_steps / (q.nw * 2), t0 = (blockIdx.y + 1) * seg_steps + q.g * part;
-  const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + q.j;
-  const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + q.j;
+  const int part = seg_steps / (q.nw * 2), t0 = ((int)blockIdx.y + 1) * seg_steps + q.g * part;
+  const T_* const zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + t0 * zv.st + q.j;
+  const T_* const dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + t0 * dout.st + q.j;
+  const unsigned char* const rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + t0 * reset.st;
   float A[E], V[E], x[E], in[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -444,18 +526,19 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_map_kernel(Stream zv
     unsigned char r[kSteps];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      const int t = min(t0 + k + s, T - 1);
-      z[s] = load_pack<F, E>(zp + t * zv.st);
-      d[s] = Pack<F, E>{};
-      if (dout.p) d[s] = load_pack<F, E>(dp + t * dout.st);
+      z[s] = d[s] = Pack<F, E>{};
+      if (t0 + k + s < T) {
+        z[s] = load_pack<F, E>(zp + (k + s) * zv.st);
+        if (dout.p) d[s] = load_pack<F, E>(dp + (k + s) * dout.st);
+      }
     }
-    if constexpr (RESET) load_resets(reset, q.b, t0 + k, T, r);
+    if constexpr (RESET) load_resets<true>(rp + k * reset.st, reset.st, t0 + k, T, r);
 #pragma unroll
     for (int s = kSteps - 1; s >= 0; --s)
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (t0 + k + s < T) {
-          const float f = gates_of(Elem<F>::up(z[s].v[e])).f;
+          const float f = gates_of<F>(Elem<F>::up(z[s].v[e])).f;
           const bool cut = RESET && r[s];
           V[e] = cut ? 0.f : f * (Elem<F>::up(d[s].v[e]) + V[e]);
           A[e] = cut ? __uint_as_float(kCutBits) : compose<RESET>(f, A[e]);
@@ -472,7 +555,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_map_kernel(Stream zv
   }
 }
 
-// A single step: one thread per E channels.  h_n may be h0.
+// A single step: one thread per E channels (H is a multiple of E).  h_n may be h0.
 template <int F, int E, bool RESET>
 __global__ __launch_bounds__(256) void gated_step_kernel(Stream zv, const float* h0, Stream reset, OutStream out,
                                                          float* h_n, float* ck, int B, int H) {
@@ -483,19 +566,19 @@ __global__ __launch_bounds__(256) void gated_step_kernel(Stream zv, const float*
   const T_* p = static_cast<const T_*>(zv.p) + b * zv.sb + j;
   const Pack<F, E> z = load_pack<F, E>(p), v = load_pack<F, E>(p + H);
   Floats<E> h{};
-  if (h0) h = *reinterpret_cast<const Floats<E>*>(h0 + ch);
-  if (ck) *reinterpret_cast<Floats<E>*>(ck + ch) = h;
+  if (h0) h = load_floats<E>(h0 + ch);
+  if (ck) store_floats(ck + ch, h.v);
   const bool cut = RESET && static_cast<const unsigned char*>(reset.p)[b * reset.sb];
   Pack<F, E> o;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const Gates g = gates_of(Elem<F>::up(z.v[e]));
+    const Gates g = gates_of<F>(Elem<F>::up(z.v[e]));
     const float wv = g.w * Elem<F>::up(v.v[e]);
     h.v[e] = cut ? wv : __builtin_fmaf(g.f, h.v[e], wv);
     o.v[e] = Elem<F>::down(h.v[e]);
   }
-  *reinterpret_cast<Pack<F, E>*>(static_cast<T_*>(out.p) + b * out.sb + j) = o;
-  *reinterpret_cast<Floats<E>*>(h_n + ch) = h;
+  store_pack<F, E>(static_cast<T_*>(out.p) + b * out.sb + j, o);
+  store_floats(h_n + ch, h.v);
 }
 
 // The shape of a call's launches: waves of a workgroup, workgroups over the channels, segments.
@@ -504,8 +587,7 @@ struct GatedPlan {
 };
 GatedPlan plan_gated(int T, int B, int H, int E) {
   GatedPlan p;
-  const long C = (long)B * H;
-  p.tiles = (int)((C + kLanes * E - 1) / (kLanes * E));
+  p.tiles = (int)(((long)B * ((H + E - 1) / E) + kLanes - 1) / kLanes);
   p.waves = 1;
   while (p.waves < kMaxWaves && p.waves * 2 * kSteps < T) p.waves *= 2;
   const int chunk = p.waves * 2 * kSteps, nchunks = (T + chunk - 1) / chunk;
@@ -525,14 +607,8 @@ int check_gated(const char* who, int T, int B, int H, int fmt) {
   return check_shape(who, T, B, 0, H);
 }
 
-// Channels per thread: two where every row of pairs is aligned.
-int channels_each(int H, int es, std::initializer_list<std::pair<const void*, std::pair<long long, long long>>> ps) {
-  if (H % 2) return 1;
-  for (const auto& p : ps) {
-    if (reinterpret_cast<uintptr_t>(p.first) % (2 * es) || p.second.first % 2 || p.second.second % 2) return 1;
-  }
-  return 2;
-}
+// Channels of a thread.  (The single step's stay within a row, for its state may be updated in place.)
+int channels_each(int T, int H) { return T == 1 ? 2 - H % 2 : std::min(H, 2); }
 
 // f(fmt, channels each, reset) as integral constants.
 template <class Fn>
@@ -556,9 +632,8 @@ int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kSteps - 1) / kSteps; }
 
 size_t hsl_gated_ws_bytes(int T, int B, int H) {
   if (T < 0 || B < 0 || H < 0) return 0;
-  size_t n = 0;
-  for (int e = 1; e <= 2; ++e) n = std::max(n, (size_t)(plan_gated(T, B, H, e).nseg - 1));
-  return n * B * H * sizeof(float2);
+  if (B == 0 || H == 0) return 0;
+  return (size_t)(plan_gated(T, B, H, std::min(H, 2)).nseg - 1) * B * H * sizeof(float2);
 }
 
 int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h0, const void* reset, long long rs_t,
@@ -568,11 +643,7 @@ int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h
   if (B == 0 || H == 0) return HSL_OK;
   if (!h_n || (T > 0 && (!zv || !out))) return fail(HSL_ERR_ARG, "hsl_gated_fwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int es = fmt == kElemF32 ? 4 : 2;
-  int e = channels_each(H, es, {{zv, {zv_t, zv_b}}, {out, {out_t, out_b}}});
-  if (reinterpret_cast<uintptr_t>(ck) % 8 || (T == 1 && (reinterpret_cast<uintptr_t>(h0) % 8 ||
-                                                         reinterpret_cast<uintptr_t>(h_n) % 8)))
-    e = 1;
+  const int e = channels_each(T, H);
   const GatedPlan p = plan_gated(T, B, H, e);
   if (p.nseg > 1 && (!ws || ws_bytes < hsl_gated_ws_bytes(T, B, H)))
     return fail(HSL_ERR_ARG, "hsl_gated_fwd: workspace %zu bytes, need %zu", ws_bytes, hsl_gated_ws_bytes(T, B, H));
@@ -605,9 +676,7 @@ int hsl_gated_bwd(const void* zv, long long zv_t, long long zv_b, const void* re
   if (B == 0 || H == 0) return HSL_OK;
   if (T > 0 && (!zv || !ck || !dzv)) return fail(HSL_ERR_ARG, "hsl_gated_bwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int es = fmt == kElemF32 ? 4 : 2;
-  int e = channels_each(H, es, {{zv, {zv_t, zv_b}}, {dout, {do_t, do_b}}, {dzv, {dz_t, dz_b}}});
-  if (reinterpret_cast<uintptr_t>(ck) % 8) e = 1;
+  const int e = std::min(H, 2);
   const GatedPlan p = plan_gated(T, B, H, e);
   if (p.nseg > 1 && (!ws || ws_bytes < hsl_gated_ws_bytes(T, B, H)))
     return fail(HSL_ERR_ARG, "hsl_gated_bwd: workspace %zu bytes, need %zu", ws_bytes, hsl_gated_ws_bytes(T, B, H));
