@@ -15,6 +15,7 @@
 // stream is read and written once.  With few channels the time is cut into segments that run as
 // workgroups of their own after a pass that composes each segment's map.
 #include <algorithm>
+#include <initializer_list>
 
 #include "lm.h"
 
@@ -77,15 +78,39 @@ template <int F, int E>
 struct Pack {
   typename Elem<F>::T v[E];
 };
-template <int F, int E>
+// NT: non-temporal, for streams that no cache holds until their next use.
+template <int N>
+struct RawOf;
+template <>
+struct RawOf<2> {
+  using T = unsigned short;
+};
+template <>
+struct RawOf<4> {
+  using T = unsigned;
+};
+template <>
+struct RawOf<8> {
+  using T = unsigned __attribute__((ext_vector_type(2)));
+};
+template <int F, int E, bool NT = false>
 __device__ __forceinline__ Pack<F, E> load_pack(const typename Elem<F>::T* p) {
   Pack<F, E> r;
-  __builtin_memcpy(&r, p, sizeof(r));
+  if constexpr (NT) {
+    typedef typename RawOf<sizeof(r)>::T Raw __attribute__((aligned(alignof(Pack<F, E>)), may_alias));
+    const auto u = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+    __builtin_memcpy(&r, &u, sizeof(r));
+  } else {
+    __builtin_memcpy(&r, p, sizeof(r));
+  }
   return r;
 }
 template <int F, int E>
 __device__ __forceinline__ void store_pack(typename Elem<F>::T* p, const Pack<F, E>& v) {
-  __builtin_memcpy(p, &v, sizeof(v));
+  typedef typename RawOf<sizeof(v)>::T Raw __attribute__((aligned(alignof(Pack<F, E>)), may_alias));
+  typename RawOf<sizeof(v)>::T u;
+  __builtin_memcpy(&u, &v, sizeof(v));
+  __builtin_nontemporal_store(u, reinterpret_cast<Raw*>(p));
 }
 template <int E>
 struct Floats {
@@ -138,6 +163,14 @@ __device__ __forceinline__ void load_resets(const unsigned char* p, long long st
   }
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) r[s] = TAIL && t0 + s >= T ? 0 : p[s * st];
+}
+
+// Whether any lane of the wave has one (most groups of 8 steps have none).
+__device__ __forceinline__ bool any_reset(const unsigned char (&r)[kSteps]) {
+  unsigned any = 0;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) any |= r[s];
+  return __any((int)any);
 }
 
 // A of the composed map of a group's steps, from the product and the smallest of the gates.
@@ -211,7 +244,7 @@ __device__ __forceinline__ void enter_segment(const float2* __restrict__ maps, i
   }
 }
 
-template <int F, int E, bool RESET>
+template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, const float* h0, Stream reset,
                                                                   OutStream out, float* h_n, float* __restrict__ ck,
                                                                   const float2* __restrict__ maps, int T, int B, int H,
@@ -237,8 +270,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
     if (t1 + chunk <= te) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        z[s] = load_pack<F, E>(zp + s * zv.st);
-        v[s] = load_pack<F, E>(zp + s * zv.st + H);
+        z[s] = load_pack<F, E, NT>(zp + s * zv.st);
+        v[s] = load_pack<F, E, NT>(zp + s * zv.st + H);
       }
       if constexpr (RESET) load_resets<false>(rp, reset.st, 0, T, r);
     } else {  // the last chunk: steps past T are not read
@@ -247,8 +280,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
       for (int s = 0; s < kSteps; ++s) {
         z[s] = v[s] = Pack<F, E>{};
         if (t0 + s < te) {
-          z[s] = load_pack<F, E>(zp + s * zv.st);
-          v[s] = load_pack<F, E>(zp + s * zv.st + H);
+          z[s] = load_pack<F, E, NT>(zp + s * zv.st);
+          v[s] = load_pack<F, E, NT>(zp + s * zv.st + H);
         }
       }
       if constexpr (RESET) load_resets<true>(rp, reset.st, t0, te, r);
@@ -256,9 +289,10 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
     zp += chunk * zv.st;
     if constexpr (RESET) rp += chunk * reset.st;
   };
-  auto step = [&](auto tail, int t1, int par, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps],
+  auto step = [&](auto tail, auto resets, int t1, int par, Pack<F, E>(&z)[kSteps], Pack<F, E>(&v)[kSteps],
                   unsigned char(&r)[kSteps]) {
     constexpr bool TAIL = decltype(tail)::value;  // the chunk with step T-1: later ones keep the state
+    constexpr bool CUTS = decltype(resets)::value;  // a reset among the wave's steps
     const int t0 = t1 + q.g * kSteps;
     float f[kSteps][E], wv[kSteps][E], A[E], V[E], h[E], least[E];
 #pragma unroll
@@ -274,43 +308,48 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
         const Gates g = gates_of<F>(Elem<F>::up(z[s].v[e]));
         f[s][e] = in ? g.f : 1.f;
         wv[s][e] = in ? g.w * Elem<F>::up(v[s].v[e]) : 0.f;
-        if (RESET && in && r[s]) f[s][e] = __uint_as_float(kCutBits);
-        V[e] = apply<RESET>(f[s][e], wv[s][e], V[e]);
-        if constexpr (RESET) {
-          A[e] = compose<RESET>(f[s][e], A[e]);
+        if (CUTS && in && r[s]) f[s][e] = __uint_as_float(kCutBits);
+        V[e] = apply<CUTS>(f[s][e], wv[s][e], V[e]);
+        if constexpr (CUTS) {
+          A[e] = compose<CUTS>(f[s][e], A[e]);
         } else {
           A[e] *= f[s][e];
           least[e] = fminf(least[e], f[s][e]);
         }
       }
     }
-    if constexpr (!RESET) {
+    if constexpr (!CUTS) {
 #pragma unroll
       for (int e = 0; e < E; ++e) A[e] = held(A[e], least[e]);
     }
     join<E, RESET, false>(q, A, V, x, h, sm[par]);
+    T_* const o0 = op;
+    float* const c0 = cp;
+    op += chunk * out.st;
+    cp += (size_t)(chunk / kSteps) * C;
     if (!q.ok || (TAIL && t0 >= te)) return;
-    if (ck) store_floats(cp, h);
+    if (ck) store_floats(c0, h);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Pack<F, E> o;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        h[e] = apply<RESET>(f[s][e], wv[s][e], h[e]);
+        h[e] = apply<CUTS>(f[s][e], wv[s][e], h[e]);
         o.v[e] = Elem<F>::down(h[e]);
       }
-      if (!TAIL || t0 + s < te) store_pack<F, E>(op + s * out.st, o);
+      if (!TAIL || t0 + s < te) store_pack<F, E>(o0 + s * out.st, o);
     }
     if (TAIL && te == T && T - t0 <= kSteps) store_floats(h_n + q.ch, h);
-    op += chunk * out.st;
-    cp += (size_t)(chunk / kSteps) * C;
   };
   auto run = [&](int t, int i) {
     if (t + chunk < te) {
       load(t + chunk, rz[i ^ 1], rv[i ^ 1], rr[i ^ 1]);
-      step(std::false_type{}, t, i, rz[i], rv[i], rr[i]);
+      if (RESET && any_reset(rr[i]))
+        step(std::false_type{}, std::integral_constant<bool, RESET>{}, t, i, rz[i], rv[i], rr[i]);
+      else
+        step(std::false_type{}, std::false_type{}, t, i, rz[i], rv[i], rr[i]);
     } else {
-      step(std::true_type{}, t, i, rz[i], rv[i], rr[i]);
+      step(std::true_type{}, std::integral_constant<bool, RESET>{}, t, i, rz[i], rv[i], rr[i]);
     }
   };
   if (tb < te) load(tb, rz[0], rv[0], rr[0]);
@@ -373,7 +412,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv
   }
 }
 
-template <int F, int E, bool RESET>
+template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, Stream reset,
                                                                   const float* __restrict__ ck, Stream dout,
                                                                   const float* __restrict__ dh_n, OutStream dzv,
@@ -398,62 +437,65 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
   const float* cp = ck + (last / kSteps) * C + q.ch;
   T_* gp = static_cast<T_*>(dzv.p) + q.b * dzv.sb + last * dzv.st + q.j;
 
-  Pack<F, E> rz[2][kSteps], rv[2][kSteps], rd[2][kSteps];
-  Floats<E> rh[2];
-  unsigned char rr[2][kSteps];
-  auto load = [&](auto tail, int t1, int i) {
+  struct Chunk {  // of the group, in registers
+    Pack<F, E> z[kSteps], v[kSteps], d[kSteps];
+    Floats<E> h;
+    unsigned char r[kSteps];
+  };
+  auto load = [&](auto tail, int t1, Chunk& m) {
     constexpr bool TAIL = decltype(tail)::value;  // steps past T are not read
     const int t0 = t1 + q.g * kSteps;
-    rh[i] = Floats<E>{};
-    if (!TAIL || t0 < te) rh[i] = load_floats<E>(cp);
+    m.h = Floats<E>{};
+    if (!TAIL || t0 < te) m.h = load_floats<E>(cp);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      if (TAIL) rz[i][s] = rv[i][s] = Pack<F, E>{};
-      rd[i][s] = Pack<F, E>{};
+      if (TAIL) m.z[s] = m.v[s] = Pack<F, E>{};
+      m.d[s] = Pack<F, E>{};
       if (!TAIL || t0 + s < te) {
-        rz[i][s] = load_pack<F, E>(zp + s * zv.st);
-        rv[i][s] = load_pack<F, E>(zp + s * zv.st + H);
-        if (dout.p) rd[i][s] = load_pack<F, E>(dp + s * dout.st);
+        m.z[s] = load_pack<F, E, NT>(zp + s * zv.st);
+        m.v[s] = load_pack<F, E, NT>(zp + s * zv.st + H);
+        if (dout.p) m.d[s] = load_pack<F, E, NT>(dp + s * dout.st);
       }
     }
-    if constexpr (RESET) load_resets<TAIL>(rp, reset.st, t0, te, rr[i]);
+    if constexpr (RESET) load_resets<TAIL>(rp, reset.st, t0, te, m.r);
     zp -= chunk * zv.st;
     dp -= chunk * dout.st;
     if constexpr (RESET) rp -= chunk * reset.st;
     cp -= (size_t)(chunk / kSteps) * C;
   };
-  auto step = [&](auto tail, int t1, int i) {
+  auto step = [&](auto tail, auto resets, int t1, int par, Chunk& m) {
     constexpr bool TAIL = decltype(tail)::value;  // the chunk with step T-1: U passes later ones
+    constexpr bool CUTS = decltype(resets)::value;  // a reset among the wave's steps
     const int t0 = t1 + q.g * kSteps;
     float f[kSteps][E], w[kSteps][E], hp[kSteps][E], A[E], V[E], U[E], h[E], least[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       A[e] = least[e] = 1.f;
       V[e] = 0.f;
-      h[e] = rh[i].v[e];
+      h[e] = m.h.v[e];
     }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const Gates g = gates_of<F>(Elem<F>::up(rz[i][s].v[e]));
-        const float v = Elem<F>::up(rv[i][s].v[e]);
+        const Gates g = gates_of<F>(Elem<F>::up(m.z[s].v[e]));
+        const float v = Elem<F>::up(m.v[s].v[e]);
         f[s][e] = g.f;
         w[s][e] = g.w;
-        hp[s][e] = RESET && rr[i][s] ? 0.f : h[e];
-        h[e] = RESET && rr[i][s] ? g.w * v : __builtin_fmaf(g.f, h[e], g.w * v);
+        hp[s][e] = CUTS && m.r[s] ? 0.f : h[e];
+        h[e] = CUTS && m.r[s] ? g.w * v : __builtin_fmaf(g.f, h[e], g.w * v);
       }
     }
 #pragma unroll
     for (int s = kSteps - 1; s >= 0; --s) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const bool cut = RESET && rr[i][s];
-        const float d = Elem<F>::up(rd[i][s].v[e]);
+        const bool cut = CUTS && m.r[s];
+        const float d = Elem<F>::up(m.d[s].v[e]);
         if (!TAIL || t0 + s < te) {
           V[e] = cut ? 0.f : f[s][e] * (d + V[e]);
-          if constexpr (RESET) {
-            A[e] = compose<RESET>(cut ? __uint_as_float(kCutBits) : f[s][e], A[e]);
+          if constexpr (CUTS) {
+            A[e] = compose<CUTS>(cut ? __uint_as_float(kCutBits) : f[s][e], A[e]);
           } else {
             A[e] *= f[s][e];
             least[e] = fminf(least[e], f[s][e]);
@@ -461,11 +503,11 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
         }
       }
     }
-    if constexpr (!RESET) {
+    if constexpr (!CUTS) {
 #pragma unroll
       for (int e = 0; e < E; ++e) A[e] = held(A[e], least[e]);
     }
-    join<E, RESET, true>(q, A, V, x, U, sm[i]);
+    join<E, RESET, true>(q, A, V, x, U, sm[par]);
     T_* const p0 = gp;
     gp -= chunk * dzv.st;
     if (!q.ok || (TAIL && t0 >= te)) return;
@@ -475,11 +517,11 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
         Pack<F, E> oz, ov;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float G = Elem<F>::up(rd[i][s].v[e]) + U[e];
-          const float v = Elem<F>::up(rv[i][s].v[e]), dv = w[s][e] * G;
+          const float G = Elem<F>::up(m.d[s].v[e]) + U[e];
+          const float v = Elem<F>::up(m.v[s].v[e]), dv = w[s][e] * G;
           oz.v[e] = Elem<F>::down(dv * ((hp[s][e] - v) * f[s][e]));
           ov.v[e] = Elem<F>::down(dv);
-          U[e] = RESET && rr[i][s] ? 0.f : f[s][e] * G;
+          U[e] = CUTS && m.r[s] ? 0.f : f[s][e] * G;
         }
         store_pack<F, E>(p0 + s * dzv.st, oz);
         store_pack<F, E>(p0 + s * dzv.st + H, ov);
@@ -487,17 +529,24 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     }
     if (t0 == 0 && dh0) store_floats(dh0 + q.ch, U);
   };
+  auto whole = [&](int t1, int par, Chunk& m) {
+    if (RESET && any_reset(m.r))
+      step(std::false_type{}, std::integral_constant<bool, RESET>{}, t1, par, m);
+    else
+      step(std::false_type{}, std::false_type{}, t1, par, m);
+  };
+  Chunk m0, m1;
   if (n > 0) {
-    load(std::true_type{}, tb + (n - 1) * chunk, 0);
-    if (n > 1) load(std::false_type{}, tb + (n - 2) * chunk, 1);
-    step(std::true_type{}, tb + (n - 1) * chunk, 0);
+    load(std::true_type{}, tb + (n - 1) * chunk, m0);
+    if (n > 1) load(std::false_type{}, tb + (n - 2) * chunk, m1);
+    step(std::true_type{}, std::integral_constant<bool, RESET>{}, tb + (n - 1) * chunk, 0, m0);
   }
   for (int k = n - 2; k >= 0; k -= 2) {
-    if (k >= 1) load(std::false_type{}, tb + (k - 1) * chunk, 0);
-    step(std::false_type{}, tb + k * chunk, 1);
+    if (k >= 1) load(std::false_type{}, tb + (k - 1) * chunk, m0);
+    whole(tb + k * chunk, 1, m1);
     if (k < 1) break;
-    if (k >= 2) load(std::false_type{}, tb + (k - 2) * chunk, 1);
-    step(std::false_type{}, tb + (k - 1) * chunk, 0);
+    if (k >= 2) load(std::false_type{}, tb + (k - 2) * chunk, m1);
+    whole(tb + (k - 1) * chunk, 0, m0);
   }
   if (T == 0 && dh0 && q.g == 0 && q.ok) store_floats(dh0 + q.ch, x);
 }
@@ -590,10 +639,13 @@ GatedPlan plan_gated(int T, int B, int H, int E) {
   p.tiles = (int)(((long)B * ((H + E - 1) / E) + kLanes - 1) / kLanes);
   p.waves = 1;
   while (p.waves < kMaxWaves && p.waves * 2 * kSteps < T) p.waves *= 2;
-  const int chunk = p.waves * 2 * kSteps, nchunks = (T + chunk - 1) / chunk;
+  int chunk = p.waves * 2 * kSteps, nchunks = (T + chunk - 1) / chunk;
   p.nseg = 1;
   p.seg_steps = std::max(1, nchunks) * chunk;
   if (p.tiles < 192 && nchunks >= 4) {
+    p.waves = std::min(p.waves, 4);
+    chunk = p.waves * 2 * kSteps;
+    nchunks = (T + chunk - 1) / chunk;
     const int want = std::min(nchunks / 2, (512 + p.tiles - 1) / p.tiles);
     const int per = (nchunks + want - 1) / want;
     p.seg_steps = per * chunk;
@@ -610,14 +662,26 @@ int check_gated(const char* who, int T, int B, int H, int fmt) {
 // Channels of a thread.  (The single step's stay within a row, for its state may be updated in place.)
 int channels_each(int T, int H) { return T == 1 ? 2 - H % 2 : std::min(H, 2); }
 
-// f(fmt, channels each, reset) as integral constants.
+// Whether a call's streams (`bytes` in all) are read without keeping them in the caches: where they
+// exceed the 256 MB last-level cache and every workgroup's rows are whole 128-byte lines.
+bool streams_past_cache(size_t bytes, int H, int es, std::initializer_list<Stream> streams) {
+  if (bytes <= (256u << 20) || (size_t)H * es % 128) return false;
+  for (const Stream& s : streams)
+    if (reinterpret_cast<uintptr_t>(s.p) % 128 || s.st * es % 128 || s.sb * es % 128) return false;
+  return true;
+}
+
+// f(fmt, channels each, reset, non-temporal) as integral constants.
 template <class Fn>
-int with_instance(int fmt, int e, bool reset, Fn f) {
+int with_instance(int fmt, int e, bool reset, bool nt, Fn f) {
   return with_fmt(fmt, [&](auto F) {
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
-    if (e == 2) return reset ? f(F, Two{}, std::true_type{}) : f(F, Two{}, std::false_type{});
-    return reset ? f(F, One{}, std::true_type{}) : f(F, One{}, std::false_type{});
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (e == 1) return reset ? f(F, One{}, Yes{}, No{}) : f(F, One{}, No{}, No{});
+    if (nt) return reset ? f(F, Two{}, Yes{}, Yes{}) : f(F, Two{}, No{}, Yes{});
+    return reset ? f(F, Two{}, Yes{}, No{}) : f(F, Two{}, No{}, No{});
   });
 }
 
@@ -650,9 +714,11 @@ int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h
   float2* const maps = static_cast<float2*>(ws);
   const Stream z{zv, zv_t, zv_b}, r{reset, rs_t, rs_b};
   const OutStream o{out, out_t, out_b};
-  return with_instance(fmt, e, reset != nullptr, [&](auto F, auto E, auto R) {
+  const int es = fmt == kElemF32 ? 4 : 2;
+  const bool nt = p.nseg == 1 && streams_past_cache((size_t)3 * T * B * H * es, H, es, {z});
+  return with_instance(fmt, e, reset != nullptr, nt, [&](auto F, auto E, auto R, auto N) {
     constexpr int kF = decltype(F)::value, kE = decltype(E)::value;
-    constexpr bool kR = decltype(R)::value;
+    constexpr bool kR = decltype(R)::value, kN = decltype(N)::value;
     if (T == 1) {
       const int n = (B * H + kE * 256 - 1) / (kE * 256);
       hipLaunchKernelGGL((gated_step_kernel<kF, kE, kR>), dim3(n), dim3(256), 0, s, z, h0, r, o, h_n, ck, B, H);
@@ -660,7 +726,7 @@ int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h
       if (p.nseg > 1)
         hipLaunchKernelGGL((gated_fwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z, r,
                            maps, T, B, H, p.seg_steps);
-      hipLaunchKernelGGL((gated_fwd_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, h0, r, o,
+      hipLaunchKernelGGL((gated_fwd_kernel<kF, kE, kR, kN>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, h0, r, o,
                          h_n, ck, maps, T, B, H, p.seg_steps);
     }
     HSL_HIP(hipGetLastError());
@@ -683,13 +749,15 @@ int hsl_gated_bwd(const void* zv, long long zv_t, long long zv_b, const void* re
   float2* const maps = static_cast<float2*>(ws);
   const Stream z{zv, zv_t, zv_b}, r{reset, rs_t, rs_b}, d{dout, do_t, do_b};
   const OutStream g{dzv, dz_t, dz_b};
-  return with_instance(fmt, e, reset != nullptr, [&](auto F, auto E, auto R) {
+  const int es = fmt == kElemF32 ? 4 : 2;
+  const bool nt = p.nseg == 1 && streams_past_cache((size_t)5 * T * B * H * es, H, es, {z, d});
+  return with_instance(fmt, e, reset != nullptr, nt, [&](auto F, auto E, auto R, auto N) {
     constexpr int kF = decltype(F)::value, kE = decltype(E)::value;
-    constexpr bool kR = decltype(R)::value;
+    constexpr bool kR = decltype(R)::value, kN = decltype(N)::value;
     if (p.nseg > 1)
       hipLaunchKernelGGL((gated_bwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z, r,
                          d, maps, T, B, H, p.seg_steps);
-    hipLaunchKernelGGL((gated_bwd_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, r, ck, d,
+    hipLaunchKernelGGL((gated_bwd_kernel<kF, kE, kR, kN>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, r, ck, d,
                        dh_n, g, dh0, maps, T, B, H, p.seg_steps);
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
