@@ -2,6 +2,7 @@
 //   m = max x,  s = sum exp(x - m),  log p_v = (x_v - m) - log s
 //   H = -sum p log p = log s - (sum e d) / s  with d = x - m, e = exp(d)
 // m and log s stay apart (stats): in a row of the type's lowest value m + log s would be m.
+// Any m within a few units of the largest logit serves: the sums are floating point.
 // -inf is a masked token: probability 0 and nothing to the entropy.  A row of nothing else has
 // logp -inf for every token, entropy 0 and no gradient.  A row with NaN or +inf gives NaN.
 // The alternatives are ordered by logit, NaN above all, the lowest id first among equals.
@@ -9,6 +10,8 @@
 // beyond V gives NaN and raises bit 1 of the sticky device word.
 // Gradient, with S = dlogp + sum of dtop:
 //   dx_v = dlogp [v = token] + sum_j dtop_j [v = id_j] - p_v (S + dH (log p_v + H)).
+#include <algorithm>
+
 #include "lm.h"
 
 namespace hsl {
@@ -16,6 +19,13 @@ namespace {
 
 constexpr int kMaxTop = 32;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxParts = 64;        // of a row; a part has kWaves groups, at most kThreads in all
+constexpr int kCandidates = 2048;    // elements that may be ranked among a row's alternatives
+constexpr float kLog2e = 1.44269502162933349609375f;
+constexpr float kLowest = -3.402823466e38f;
+// A running sum keeps its reference until a logit exceeds it by this much: e^8 is far from
+// overflow, and the terms of sd stay within 8 + their distance from the largest logit.
+constexpr float kSlack = 8.0f;
 
 // The order of the alternatives as whole numbers: the value's order above (-0 as 0, NaN the
 // largest), the smallest index the largest below.
@@ -24,67 +34,138 @@ __device__ __forceinline__ unsigned order_of(float x) {
   const unsigned u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(unsigned o) {
+  if (o == 0xFFFFFFFEu) return __builtin_nanf("");
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
 __device__ __forceinline__ unsigned long long key_of(float x, int v) {
   return (unsigned long long)order_of(x) << 32 | (0xFFFFFFFFu - (unsigned)v);
 }
 
-template <class T>
-__device__ __forceinline__ T wave_max(T v) {
+__device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
   for (int d = 32; d; d >>= 1) {
-    const T o = __shfl_xor(v, d);
+    const unsigned long long o = __shfl_xor(v, d);
     v = o > v ? o : v;
   }
   return v;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+
+// 16 bytes of a row at any element's alignment (global memory takes unaligned accesses).
+template <int F>
+struct Vec {
+  static constexpr int N = 16 / sizeof(typename Elem<F>::T);
+  typename Elem<F>::T v[N];
+};
+template <int F>
+__device__ __forceinline__ Vec<F> load_vec(const typename Elem<F>::T* p) {
+  Vec<F> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+// Vector i of a row of V elements, the part beyond the row masked.
+template <int F>
+__device__ __forceinline__ Vec<F> load_edge(const typename Elem<F>::T* row, int i, int V) {
+  Vec<F> r;
+  const int first = i * Vec<F>::N;
+  if (first + Vec<F>::N <= V) return load_vec<F>(row + first);
+#pragma unroll
+  for (int e = 0; e < Vec<F>::N; ++e)
+    r.v[e] = first + e < V ? row[first + e] : Elem<F>::down(-__builtin_inff());
+  return r;
 }
 
-// One workgroup per row; the alternatives in `top` rounds over the row.
+// s = sum e^(x - r), sd = sum e^(x - r) (x - r) over some elements; r is one of them or kLowest.
+struct Sums {
+  float r, s, sd;
+  // the same with a larger reference
+  __device__ __forceinline__ void rebase(float to) {
+    const float gap = r - to, c = __builtin_amdgcn_exp2f(gap * kLog2e);
+    sd = c == 0.f ? 0.f : c * __builtin_fmaf(gap, s, sd);  // (gap may be -inf)
+    s *= c;
+    r = to;
+  }
+  __device__ __forceinline__ void add(Sums o) {
+    const float to = fmaxf(r, o.r);
+    if (r != to) rebase(to);
+    if (o.r != to) o.rebase(to);
+    s += o.s;
+    sd += o.sd;
+  }
+};
+
+// The running sums and, with TOP, the largest element's value and vector of one thread.
+template <int F, bool TOP>
+struct Running {
+  Sums q{kLowest, 0.f, 0.f};
+  float best = -__builtin_inff();
+  int at = 0x7FFFFFFF;
+  __device__ __forceinline__ void take(const Vec<F>& x, int i) {
+    constexpr int N = Vec<F>::N;
+    float f[N], m = Elem<F>::up(x.v[0]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[e] = Elem<F>::up(x.v[e]);
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, f[e]);
+    if (TOP && (m > best || at == 0x7FFFFFFF)) {  // the first vector too, if it holds -inf alone
+      best = m;
+      at = i;
+    }
+    if (__any(m > q.r + kSlack)) {
+      if (m > q.r) q.rebase(m);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      // exp2 of the rounded product is within 1.3 |d| 2^-24 of e^d, little where e^d counts
+      const float d = f[e] - q.r, p = __builtin_amdgcn_exp2f(d * kLog2e);
+      q.s += p;
+      q.sd = __builtin_fmaf(p, fmaxf(d, -1e30f), q.sd);  // p = 0 for d = -inf
+    }
+  }
+};
+
+// One workgroup's elements: the vectors first .. last-1 of a row.  Four loads are in flight.
+template <int F, bool TOP>
+__device__ __forceinline__ void scan_part(const typename Elem<F>::T* __restrict__ row, int first, int last, int V,
+                                          Running<F, TOP>& a) {
+  constexpr int N = Vec<F>::N, kAhead = 4;
+  const int whole = min(last, V / N);
+  int i = first + threadIdx.x;
+  for (; i + (kAhead - 1) * kThreads < whole; i += kAhead * kThreads) {
+    Vec<F> x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) x[k] = load_vec<F>(row + (size_t)(i + k * kThreads) * N);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) a.take(x[k], i + k * kThreads);
+  }
+  for (; i < last; i += kThreads) a.take(load_edge<F>(row, i, V), i);
+}
+
+// The sums of the whole workgroup, in every thread.
+__device__ __forceinline__ Sums join_block(Sums q, Sums (&lds)[kWaves]) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) q.add(Sums{__shfl_xor(q.r, d), __shfl_xor(q.s, d), __shfl_xor(q.sd, d)});
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = q;
+  __syncthreads();
+  q = lds[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) q.add(lds[w]);
+  return q;
+}
+
+struct Out {
+  float *logp, *entropy, *stats, *top_logp;
+  long long* top_ids;
+};
+
+// Row n's results from its sums; returns whether nothing in it is above -inf.
 template <int F>
-__global__ __launch_bounds__(kThreads) void logprob_fwd_kernel(
-    const typename Elem<F>::T* __restrict__ logits, long long ld, const void* __restrict__ tokens, int tok64,
-    float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logp,
-    long long* __restrict__ top_ids, int V, int top, unsigned* err) {
-  __shared__ float sm[kWaves], ss[kWaves], sw[kWaves];
-  __shared__ unsigned long long sk[kWaves];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const size_t n = blockIdx.x;
-  const auto* const row = logits + (long long)n * ld;
-  float m = -__builtin_inff();
-  for (int v = threadIdx.x; v < V; v += kThreads) m = fmaxf(m, Elem<F>::up(row[v]));
-  m = wave_max(m);
-  if (lane == 0) sm[w] = m;
-  __syncthreads();
-  for (int u = 0; u < kWaves; ++u) m = fmaxf(m, sm[u]);
-  const bool empty = m == -__builtin_inff();
-  const float m0 = empty ? 0.f : m;
-  float s = 0.f, sd = 0.f;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    const float d = Elem<F>::up(row[v]) - m0, e = exp_f(d);
-    s += e;
-    sd += e == 0.f ? 0.f : e * d;
-  }
-  s = wave_sum(s);
-  sd = wave_sum(sd);
-  if (lane == 0) {
-    ss[w] = s;
-    sw[w] = sd;
-  }
-  __syncthreads();
-  s = sd = 0.f;
-  for (int u = 0; u < kWaves; ++u) {
-    s += ss[u];
-    sd += sw[u];
-  }
-  // no element was above -inf and the sum is 0: the row is empty (NaN is not above -inf either)
-  const bool none = empty && s == 0.f;
-  const float ls = logf(s);
+__device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, const typename Elem<F>::T* row,
+                                           const void* tokens, int tok64, int V, const Out& o, unsigned* err) {
+  const bool none = q.s == 0.f;  // (not of a row with NaN)
   if (threadIdx.x == 0) {
-    stats[2 * n] = none ? m : m0;
-    stats[2 * n + 1] = ls;
-    entropy[n] = none ? 0.f : ls - sd / s;
+    o.stats[2 * n] = none ? -__builtin_inff() : q.r;
+    o.stats[2 * n + 1] = ls;
+    o.entropy[n] = none ? 0.f : ls - q.sd / q.s;
     if (tokens) {
       const long long t = load_id(tokens, tok64, n);
       float r = 0.f;
@@ -92,13 +173,81 @@ __global__ __launch_bounds__(kThreads) void logprob_fwd_kernel(
         atomicOr(err, kErrId);
         r = __builtin_nanf("");
       } else if (t >= 0) {
-        r = none ? -__builtin_inff() : Elem<F>::up(row[t]) - m0 - ls;
+        r = none ? -__builtin_inff() : Elem<F>::up(row[t]) - q.r - ls;
       }
-      logp[n] = r;
+      o.logp[n] = r;
     }
   }
+  return none;
+}
+
+// The alternatives of a row.  Each thread knows the largest element of one group of vectors, by
+// its value and its vector (key: 0 if the group is empty).  The k groups with the largest keys hold
+// the k largest elements: any other group's elements are all below those k.  So only these groups
+// are read again, for the elements at or above the k-th group's key, and those are ranked by
+// counting.  Groups are GL lanes wide: group g has vectors (g / (256 / GL)) * part + 256 i +
+// (g mod (256 / GL)) * GL + 0 .. GL-1.
+struct alignas(16) TopShared {
+  unsigned long long key[kThreads];
+  unsigned long long cand[kCandidates];
+  int group[kMaxTop];
+  unsigned long long least;
+  int ncand;
+};
+template <int F, int GL>
+__device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, int top, int part, int nvec,
+                           unsigned long long key, float r, float ls, bool nan_row, bool none, size_t n, const Out& o,
+                           TopShared& sh) {
+  constexpr int N = Vec<F>::N, kPer = kThreads / GL;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  sh.key[threadIdx.x] = key;
+  if (threadIdx.x == 0) sh.ncand = 0;
+  __syncthreads();
+  int rank = 0, groups = 0;
+  for (int u = 0; u < kThreads; u += 2) {
+    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sh.key[u]);
+    rank += (k.x > key) + (k.y > key);
+    groups += (k.x != 0) + (k.y != 0);
+  }
+  groups = min(groups, top);
+  if (rank < groups) sh.group[rank] = threadIdx.x;
+  // the smallest key that an element of that group's vector with that value can have
+  if (rank == groups - 1) sh.least = (key | 0xFFFFFFFFull) - ((0xFFFFFFFFull - (key & 0xFFFFFFFFull)) * N + N - 1);
+  if (rank == groups - 1 && groups < top) sh.least = 0;  // fewer groups than asked for: every element
+  __syncthreads();
+  const unsigned long long least = sh.least;
+  const int each = (part + kThreads - 1) / kThreads * GL;  // vectors of a group
+  for (int i = threadIdx.x; i < groups * each && !nan_row; i += kThreads) {
+    const int g = sh.group[i / each], j = i % each;
+    const int at = (j / GL) * kThreads + (g % kPer) * GL + j % GL, vec = (g / kPer) * part + at;
+    if (at >= part || vec >= nvec) continue;
+    const Vec<F> x = load_edge<F>(row, vec, V);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const unsigned long long k = key_of(Elem<F>::up(x.v[e]), vec * N + e);
+      if (vec * N + e < V && k >= least) {
+        const int c = atomicAdd(&sh.ncand, 1);
+        if (c < kCandidates) sh.cand[c] = k;
+      }
+    }
+  }
+  __syncthreads();
+  const int ncand = sh.ncand;
+  if (!nan_row && ncand <= kCandidates) {
+    for (int c = threadIdx.x; c < ncand; c += kThreads) {
+      const unsigned long long k = sh.cand[c];
+      int above = 0;
+      for (int u = 0; u < ncand; ++u) above += sh.cand[u] > k;
+      if (above < top) {
+        o.top_ids[n * top + above] = 0xFFFFFFFFu - (unsigned)k;
+        o.top_logp[n * top + above] = none ? -__builtin_inff() : value_of((unsigned)(k >> 32)) - r - ls;
+      }
+    }
+    return;
+  }
+  // a row with NaN, or one whose large elements crowd in a few groups: one round over the row each
   unsigned long long last = ~0ull;
-  for (int k = 0; k < top; ++k) {
+  for (int j = 0; j < top; ++j) {
     unsigned long long best = 0;
     for (int v = threadIdx.x; v < V; v += kThreads) {
       const unsigned long long c = key_of(Elem<F>::up(row[v]), v);
@@ -106,42 +255,157 @@ __global__ __launch_bounds__(kThreads) void logprob_fwd_kernel(
     }
     best = wave_max(best);
     __syncthreads();
-    if (lane == 0) sk[w] = best;
+    if (lane == 0) sh.key[w] = best;
     __syncthreads();
-    for (int u = 0; u < kWaves; ++u) best = sk[u] > best ? sk[u] : best;
+    for (int u = 0; u < kWaves; ++u) best = sh.key[u] > best ? sh.key[u] : best;
     last = best;
     if (threadIdx.x == 0) {
-      const int v = (int)(0xFFFFFFFFu - (unsigned)best);
-      top_ids[n * top + k] = v;
-      top_logp[n * top + k] = none ? -__builtin_inff() : Elem<F>::up(row[v]) - m0 - ls;
+      o.top_ids[n * top + j] = 0xFFFFFFFFu - (unsigned)best;
+      o.top_logp[n * top + j] = nan_row ? __builtin_nanf("") : none ? -__builtin_inff()
+                                                                    : value_of((unsigned)(best >> 32)) - r - ls;
     }
   }
 }
 
-template <int F>
+// A group's key: the value's order above, the smallest vector the largest below; 0 without one.
+__device__ __forceinline__ unsigned long long group_key(float best, int at) {
+  return at == 0x7FFFFFFF ? 0 : key_of(best, at);
+}
+
+// One workgroup per row.
+template <int F, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
+                                                               long long ld, const void* __restrict__ tokens,
+                                                               int tok64, Out o, int V, int top, unsigned* err) {
+  __shared__ Sums lds[kWaves];
+  const size_t n = blockIdx.x;
+  const auto* const row = logits + (long long)n * ld;
+  const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N);
+  Running<F, TOP> a;
+  scan_part<F, TOP>(row, 0, nvec, V, a);
+  const Sums q = join_block(a.q, lds);
+  const float ls = logf(q.s);
+  const bool none = finish_row<F>(n, q, ls, row, tokens, tok64, V, o, err);
+  if constexpr (TOP) {
+    __shared__ TopShared sh;
+    choose_top<F, 1>(row, V, top, nvec, nvec, group_key(a.best, a.at), q.r, ls, q.s != q.s, none, n, o, sh);
+  }
+}
+
+// Few rows: each is cut into parts of `part` vectors, whose sums and groups' keys go to ws.
+template <int F, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprob_part_kernel(const typename Elem<F>::T* __restrict__ logits,
+                                                                long long ld, Sums* __restrict__ sums,
+                                                                unsigned long long* __restrict__ keys, int V,
+                                                                int part) {
+  __shared__ Sums lds[kWaves];
+  const size_t n = blockIdx.y;
+  const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N), p = blockIdx.x;
+  Running<F, TOP> a;
+  scan_part<F, TOP>(logits + (long long)n * ld, p * part, min(nvec, (p + 1) * part), V, a);
+  const Sums q = join_block(a.q, lds);
+  if (threadIdx.x == 0) sums[n * gridDim.x + p] = q;
+  if constexpr (TOP) {
+    const unsigned long long key = wave_max(group_key(a.best, a.at));
+    if ((threadIdx.x & 63) == 0) keys[(n * gridDim.x + p) * kWaves + (threadIdx.x >> 6)] = key;
+  }
+}
+
+template <int F, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename Elem<F>::T* __restrict__ logits,
+                                                                long long ld, const Sums* __restrict__ sums,
+                                                                const unsigned long long* __restrict__ keys,
+                                                                const void* __restrict__ tokens, int tok64, Out o,
+                                                                int V, int part, int parts, int top, unsigned* err) {
+  __shared__ Sums lds[kWaves];
+  const size_t n = blockIdx.x;
+  const auto* const row = logits + (long long)n * ld;
+  const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N);
+  Sums q{kLowest, 0.f, 0.f};
+  if ((int)threadIdx.x < parts) q = sums[n * parts + threadIdx.x];
+  unsigned long long key = 0;
+  if (TOP && (int)threadIdx.x < parts * kWaves) key = keys[n * parts * kWaves + threadIdx.x];
+  q = join_block(q, lds);
+  const float ls = logf(q.s);
+  const bool none = finish_row<F>(n, q, ls, row, tokens, tok64, V, o, err);
+  if constexpr (TOP) {
+    __shared__ TopShared sh;
+    choose_top<F, 64>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+  }
+}
+
+// dx = -p (S + dH (log p + H)) for the vectors of one part of a row; then the elements with a
+// gradient of their own, the token and the alternatives, are computed again with it.
+template <int F, bool ENT>
 __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
     const typename Elem<F>::T* __restrict__ logits, long long ld, const void* __restrict__ tokens, int tok64,
     const long long* __restrict__ top_ids, const float* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ dlogp, const float* __restrict__ dent, const float* __restrict__ dtop,
-    typename Elem<F>::T* __restrict__ dlogits, long long ldd, int V, int top) {
-  const size_t n = blockIdx.x;
+    typename Elem<F>::T* __restrict__ dlogits, long long ldd, int V, int top, int part) {
+  constexpr int N = Vec<F>::N;
+  const size_t n = blockIdx.y;
   const auto* const row = logits + (long long)n * ld;
   auto* const drow = dlogits + (long long)n * ldd;
   const float m = stats[2 * n], ls = stats[2 * n + 1];
   const bool none = m == -__builtin_inff();
-  long long tok = tokens && dlogp ? load_id(tokens, tok64, n) : -1;
+  const long long tok = tokens && dlogp ? load_id(tokens, tok64, n) : -1;
   const float dl = tok >= 0 ? (tok < V ? dlogp[n] : __builtin_nanf("")) : 0.f;
   float S = dl;
   for (int k = 0; dtop && k < top; ++k) S += dtop[n * top + k];
-  const float dh = dent ? dent[n] : 0.f, H = dent ? entropy[n] : 0.f;
-  for (int v = threadIdx.x; v < V; v += kThreads) {
-    const float d = Elem<F>::up(row[v]) - m - ls, p = exp_f(d);
-    float g = p == 0.f ? 0.f : -p * (S + dh * (d + H));
-    if (v == tok) g += dl;
-    for (int k = 0; dtop && k < top; ++k)
-      if (top_ids[n * top + k] == v) g += dtop[n * top + k];
-    drow[v] = Elem<F>::down(none ? 0.f : g);
+  const float dh = ENT ? dent[n] : 0.f, SH = ENT ? __builtin_fmaf(dh, entropy[n], S) : S;
+  auto grad = [&](float x) {
+    const float d = x - m - ls, p = __builtin_amdgcn_exp2f(d * kLog2e);
+    if constexpr (ENT) return -p * __builtin_fmaf(dh, fmaxf(d, -1e30f), SH);
+    return -p * SH;
+  };
+  const int nvec = (int)(((long long)V + N - 1) / N), first = blockIdx.x * part, last = min(nvec, first + part);
+  for (int i = first + threadIdx.x; i < last; i += kThreads) {
+    Vec<F> x = load_edge<F>(row, i, V);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x.v[e] = Elem<F>::down(none ? 0.f : grad(Elem<F>::up(x.v[e])));
+    auto* const out = drow + (size_t)i * N;
+    if (i * N + N <= V) {
+      __builtin_memcpy(out, &x, sizeof(x));
+    } else {
+      for (int e = 0; i * N + e < V; ++e) out[e] = x.v[e];
+    }
   }
+  __syncthreads();  // their stores come after the part's
+  const int k = threadIdx.x;
+  if (none || k > top || (k < top && !dtop)) return;
+  const long long v = k < top ? top_ids[n * top + k] : tok;
+  if (v < (long long)first * N || v >= min((long long)V, (long long)last * N)) return;
+  float g = grad(Elem<F>::up(row[v]));
+  if (v == tok) g += dl;
+  for (int j = 0; dtop && j < top; ++j)
+    if (top_ids[n * top + j] == v) g += dtop[n * top + j];
+  drow[v] = Elem<F>::down(g);
+}
+
+// Parts of a row and their vectors: one part where the rows alone fill the chip.
+struct Parts {
+  int count, vectors;
+};
+Parts plan_parts(long long N, int V, int fmt) {
+  const int per = fmt == kElemF32 ? 4 : 8;
+  const int nvec = (int)(((long long)V + per - 1) / per);
+  int count = 1;
+  if (N < 512) count = (int)std::min<long long>({(1024 + N - 1) / std::max(N, 1ll), kMaxParts, (nvec + kThreads - 1) / kThreads});
+  count = std::max(count, 1);
+  // whole rounds of a workgroup's threads
+  const int vectors = ((nvec + count - 1) / count + kThreads - 1) / kThreads * kThreads;
+  return {std::max(1, (nvec + vectors - 1) / vectors), vectors};
+}
+
+struct LogprobWs {
+  Sums* sums;
+  unsigned long long* keys;
+};
+size_t carve_logprob(void* ws, size_t cap, long long N, int parts, LogprobWs* o) {
+  Carver c(ws, cap);
+  o->sums = c.take<Sums>((size_t)N * parts);
+  o->keys = c.take<unsigned long long>((size_t)N * parts * kWaves);
+  return align_up(c.off, 256);
 }
 
 int check_logprob(const char* who, long long N, int V, int top, int fmt) {
@@ -149,7 +413,8 @@ int check_logprob(const char* who, long long N, int V, int top, int fmt) {
   if (N < 0 || V < 0) return fail(HSL_ERR_ARG, "%s: negative size (N=%lld V=%d)", who, N, V);
   if (top < 0 || top > kMaxTop || top > V)
     return fail(HSL_ERR_ARG, "%s: top=%d is not in 0..min(%d, V=%d)", who, top, kMaxTop, V);
-  if (N >= (1ll << 31)) return fail(HSL_ERR_UNSUPPORTED, "%s: N=%lld rows need 2^31 > N", who, N);
+  if (N >= (1ll << 31) || V > 0x7FFFF000)
+    return fail(HSL_ERR_UNSUPPORTED, "%s: N=%lld rows of V=%d need 2^31 > N and V <= 2^31 - 4096", who, N, V);
   return HSL_OK;
 }
 
@@ -160,7 +425,13 @@ using namespace hsl;
 
 extern "C" {
 
-size_t hsl_logprob_fwd_ws_bytes(long long N, int V, int top) { return 0; }
+size_t hsl_logprob_fwd_ws_bytes(long long N, int V, int top) {
+  if (N <= 0 || V < 0) return 0;
+  // the 16-bit and the fp32 cut of a row differ
+  const int parts = std::max(plan_parts(N, V, kElemBf16).count, plan_parts(N, V, kElemF32).count);
+  LogprobWs w;
+  return parts > 1 ? carve_logprob(nullptr, 0, N, parts, &w) : 0;
+}
 
 int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int tok64, float* logp, float* entropy,
                     float* stats, float* top_logp, long long* top_ids, void* ws, size_t ws_bytes, long long N, int V,
@@ -171,12 +442,33 @@ int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int to
     return fail(HSL_ERR_ARG, "hsl_logprob_fwd: null pointer");
   unsigned* err;
   HSL_CHECK(device_error_word(&err));
+  const Parts p = plan_parts(N, V, fmt);
+  LogprobWs w{};
+  if (p.count > 1) {
+    const size_t need = carve_logprob(ws, ws_bytes, N, p.count, &w);
+    if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_logprob_fwd: workspace %zu bytes, need %zu", ws_bytes, need);
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const Out o{logp, entropy, stats, top_logp, top_ids};
   return with_fmt(fmt, [&](auto f) {
-    using T = typename Elem<decltype(f)::value>::T;
-    hipLaunchKernelGGL(logprob_fwd_kernel<decltype(f)::value>, dim3((unsigned)N), dim3(kThreads), 0, s,
-                       static_cast<const T*>(logits), ld, tokens, tok64, logp, entropy, stats, top_logp, top_ids, V, top,
-                       err);
+    constexpr int kF = decltype(f)::value;
+    const auto* x = static_cast<const typename Elem<kF>::T*>(logits);
+    auto run = [&](auto t) {
+      constexpr bool kTop = decltype(t)::value;
+      if (p.count == 1) {
+        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld, tokens, tok64,
+                           o, V, top, err);
+      } else {
+        hipLaunchKernelGGL((logprob_part_kernel<kF, kTop>), dim3(p.count, (unsigned)N), dim3(kThreads), 0, s, x, ld,
+                           w.sums, w.keys, V, p.vectors);
+        hipLaunchKernelGGL((logprob_join_kernel<kF, kTop>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld, w.sums,
+                           w.keys, tokens, tok64, o, V, p.vectors, p.count, top, err);
+      }
+    };
+    if (top)
+      run(std::true_type{});
+    else
+      run(std::false_type{});
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
   });
@@ -190,12 +482,28 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
   if (!logits || !stats || !dlogits || (dlogp && !tokens) || (dent && !entropy) || (dtop && !top_ids))
     return fail(HSL_ERR_ARG, "hsl_logprob_bwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // one part of `part` vectors is a workgroup; blockIdx.y holds 2^16 rows
+  const int per = fmt == kElemF32 ? 4 : 8, part = 4 * kThreads;
+  const int nvec = (int)(((long long)V + per - 1) / per);
   return with_fmt(fmt, [&](auto f) {
-    using T = typename Elem<decltype(f)::value>::T;
-    hipLaunchKernelGGL(logprob_bwd_kernel<decltype(f)::value>, dim3((unsigned)N), dim3(kThreads), 0, s,
-                       static_cast<const T*>(logits), ld, tokens, tok64, top_ids, stats, entropy, dlogp, dent, dtop,
-                       static_cast<T*>(dlogits), ldd, V, top);
-    HSL_HIP(hipGetLastError());
+    constexpr int kF = decltype(f)::value;
+    using T = typename Elem<kF>::T;
+    for (long long n0 = 0; n0 < N; n0 += 65535) {
+      const unsigned rows = (unsigned)std::min<long long>(N - n0, 65535);
+      auto run = [&](auto e) {
+        hipLaunchKernelGGL((logprob_bwd_kernel<kF, decltype(e)::value>), dim3((nvec + part - 1) / part, rows),
+                           dim3(kThreads), 0, s, static_cast<const T*>(logits) + n0 * ld, ld,
+                           tokens ? static_cast<const char*>(tokens) + n0 * (tok64 ? 8 : 4) : nullptr, tok64,
+                           top_ids ? top_ids + n0 * top : nullptr, stats + 2 * n0, entropy ? entropy + n0 : nullptr,
+                           dlogp ? dlogp + n0 : nullptr, dent ? dent + n0 : nullptr, dtop ? dtop + n0 * top : nullptr,
+                           static_cast<T*>(dlogits) + n0 * ldd, ldd, V, top, part);
+      };
+      if (dent)
+        run(std::true_type{});
+      else
+        run(std::false_type{});
+      HSL_HIP(hipGetLastError());
+    }
     return (int)HSL_OK;
   });
 }
