@@ -333,10 +333,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
     for (int s = 0; s < kSteps; ++s) {
       Pack<F, E> o;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        h[e] = apply<CUTS>(f[s][e], wv[s][e], h[e]);
-        o.v[e] = Elem<F>::down(h[e]);
-      }
+      for (int e = 0; e < E; ++e) h[e] = apply<CUTS>(f[s][e], wv[s][e], h[e]);
+      down_all<F, E>(h, o.v);
       if (!TAIL || t0 + s < te) store_pack<F, E>(o0 + s * out.st, o);
     }
     if (TAIL && te == T && T - t0 <= kSteps) store_floats(h_n + q.ch, h);
@@ -515,14 +513,16 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     for (int s = kSteps - 1; s >= 0; --s) {
       if (!TAIL || t0 + s < te) {
         Pack<F, E> oz, ov;
+        float dz[E], dv[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float G = Elem<F>::up(m.d[s].v[e]) + U[e];
-          const float v = Elem<F>::up(m.v[s].v[e]), dv = w[s][e] * G;
-          oz.v[e] = Elem<F>::down(dv * ((hp[s][e] - v) * f[s][e]));
-          ov.v[e] = Elem<F>::down(dv);
+          dv[e] = w[s][e] * G;
+          dz[e] = dv[e] * ((hp[s][e] - Elem<F>::up(m.v[s].v[e])) * f[s][e]);
           U[e] = CUTS && m.r[s] ? 0.f : f[s][e] * G;
         }
+        down_all<F, E>(dz, oz.v);
+        down_all<F, E>(dv, ov.v);
         store_pack<F, E>(p0 + s * dzv.st, oz);
         store_pack<F, E>(p0 + s * dzv.st + H, ov);
       }

@@ -37,6 +37,23 @@ struct Elem<kElemF32> {
   static __device__ __forceinline__ T down(float v) { return v; }
 };
 
+// N values rounded into N neighbouring elements (two bf16 ones are one conversion).
+template <int F, int N>
+__device__ __forceinline__ void down_all(const float (&f)[N], typename Elem<F>::T (&out)[N]) {
+  if constexpr (F == kElemBf16 && N % 2 == 0) {
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const B2 b = __builtin_convertvector((F2){f[i], f[i + 1]}, B2);
+      __builtin_memcpy(&out[i], &b, sizeof(b));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = Elem<F>::down(f[i]);
+  }
+}
+
 // The sticky device word that hsl_device_errors reads, for a kernel's argument (recurrent.hip).
 // Bit 1: an id beyond the vocabulary (bit 0 is the persistent kernels').
 int device_error_word(unsigned** word);

@@ -20,6 +20,9 @@ namespace {
 constexpr int kMaxTop = 32;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxParts = 64;        // of a row; a part has kWaves groups, at most kThreads in all
+constexpr int kBwdVecs = 2;          // vectors of a thread in the backward
+constexpr int kShortRow = 2048;      // logits of a row that one wave takes
+constexpr int kRowLanes = 4;         // of a group in a row of one workgroup
 constexpr int kCandidates = 2048;    // elements that may be ranked among a row's alternatives
 constexpr float kLog2e = 1.44269502162933349609375f;
 constexpr float kLowest = -3.402823466e38f;
@@ -124,31 +127,34 @@ struct Running {
 };
 
 // One workgroup's elements: the vectors first .. last-1 of a row.  Four loads are in flight.
-template <int F, bool TOP>
+template <int F, bool TOP, int W>
 __device__ __forceinline__ void scan_part(const typename Elem<F>::T* __restrict__ row, int first, int last, int V,
                                           Running<F, TOP>& a) {
-  constexpr int N = Vec<F>::N, kAhead = 4;
+  constexpr int N = Vec<F>::N, kAhead = 4, kN = W * 64;
   const int whole = min(last, V / N);
   int i = first + threadIdx.x;
-  for (; i + (kAhead - 1) * kThreads < whole; i += kAhead * kThreads) {
+  for (; i + (kAhead - 1) * kN < whole; i += kAhead * kN) {
     Vec<F> x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) x[k] = load_vec<F>(row + (size_t)(i + k * kThreads) * N);
+    for (int k = 0; k < kAhead; ++k) x[k] = load_vec<F>(row + (size_t)(i + k * kN) * N);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) a.take(x[k], i + k * kThreads);
+    for (int k = 0; k < kAhead; ++k) a.take(x[k], i + k * kN);
   }
-  for (; i < last; i += kThreads) a.take(load_edge<F>(row, i, V), i);
+  for (; i < last; i += kN) a.take(load_edge<F>(row, i, V), i);
 }
 
 // The sums of the whole workgroup, in every thread.
-__device__ __forceinline__ Sums join_block(Sums q, Sums (&lds)[kWaves]) {
+template <int W>
+__device__ __forceinline__ Sums join_block(Sums q, Sums (&lds)[W]) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) q.add(Sums{__shfl_xor(q.r, d), __shfl_xor(q.s, d), __shfl_xor(q.sd, d)});
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = q;
-  __syncthreads();
-  q = lds[0];
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = q;
+    __syncthreads();
+    q = lds[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) q.add(lds[w]);
+    for (int w = 1; w < W; ++w) q.add(lds[w]);
+  }
   return q;
 }
 
@@ -157,23 +163,35 @@ struct Out {
   long long* top_ids;
 };
 
-// Row n's results from its sums; returns whether nothing in it is above -inf.
+// The row's token and its logit, read before anything else.
+struct Token {
+  long long id;  // -1: none
+  float x;
+};
 template <int F>
-__device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, const typename Elem<F>::T* row,
-                                           const void* tokens, int tok64, int V, const Out& o, unsigned* err) {
+__device__ __forceinline__ Token load_token(const void* tokens, int tok64, size_t n, const typename Elem<F>::T* row,
+                                            int V) {
+  Token t{-1, 0.f};
+  if (tokens) t.id = load_id(tokens, tok64, n);
+  if (t.id >= 0 && t.id < V) t.x = Elem<F>::up(row[t.id]);
+  return t;
+}
+
+// Row n's results from its sums; returns whether nothing in it is above -inf.
+__device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, const Token& t, int V, const Out& o,
+                                           unsigned* err) {
   const bool none = q.s == 0.f;  // (not of a row with NaN)
   if (threadIdx.x == 0) {
     o.stats[2 * n] = none ? -__builtin_inff() : q.r;
     o.stats[2 * n + 1] = ls;
     o.entropy[n] = none ? 0.f : ls - q.sd / q.s;
-    if (tokens) {
-      const long long t = load_id(tokens, tok64, n);
+    if (o.logp) {
       float r = 0.f;
-      if (t >= V) {
+      if (t.id >= V) {
         atomicOr(err, kErrId);
         r = __builtin_nanf("");
-      } else if (t >= 0) {
-        r = none ? -__builtin_inff() : Elem<F>::up(row[t]) - q.r - ls;
+      } else if (t.id >= 0) {
+        r = none ? -__builtin_inff() : t.x - q.r - ls;
       }
       o.logp[n] = r;
     }
@@ -185,58 +203,82 @@ __device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, co
 // its value and its vector (key: 0 if the group is empty).  The k groups with the largest keys hold
 // the k largest elements: any other group's elements are all below those k.  So only these groups
 // are read again, for the elements at or above the k-th group's key, and those are ranked by
-// counting.  Groups are GL lanes wide: group g has vectors (g / (256 / GL)) * part + 256 i +
-// (g mod (256 / GL)) * GL + 0 .. GL-1.
+// counting.  Groups are GL lanes wide: group g has vectors (g / (n / GL)) * part + n i +
+// (g mod (n / GL)) * GL + 0 .. GL-1, n the threads.  A row of one workgroup has groups of 4 lanes
+// (64 of 4 waves, which one wave ranks); with 256 of one lane the ranking took 2 us of the workgroup's time instead of 0.1,
+// more than the three vectors more that each lane reads again.
 struct alignas(16) TopShared {
-  unsigned long long key[kThreads];
+  unsigned long long key[kThreads];  // one for each group
   unsigned long long cand[kCandidates];
   int group[kMaxTop];
   unsigned long long least;
   int ncand;
 };
-template <int F, int GL>
+template <int F, int W, int GL, int KEYS>
 __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, int top, int part, int nvec,
                            unsigned long long key, float r, float ls, bool nan_row, bool none, size_t n, const Out& o,
                            TopShared& sh) {
-  constexpr int N = Vec<F>::N, kPer = kThreads / GL;
+  constexpr int N = Vec<F>::N, kN = W * 64, kPer = kN / GL;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  sh.key[threadIdx.x] = key;
+  if (threadIdx.x < KEYS) sh.key[threadIdx.x] = key;
   if (threadIdx.x == 0) sh.ncand = 0;
-  __syncthreads();
-  int rank = 0, groups = 0;
-  for (int u = 0; u < kThreads; u += 2) {
-    const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sh.key[u]);
-    rank += (k.x > key) + (k.y > key);
-    groups += (k.x != 0) + (k.y != 0);
+  const int groups = min(__syncthreads_count(threadIdx.x < KEYS && key != 0), top);
+  if (threadIdx.x < KEYS) {
+    int rank = 0;
+#pragma unroll 8
+    for (int u = 0; u < KEYS; u += 2) {
+      const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sh.key[u]);
+      rank += (k.x > key) + (k.y > key);
+    }
+    if (rank < groups) sh.group[rank] = threadIdx.x;
+    if (rank == groups - 1) {
+      // the smallest key that an element of that group's vector with that value can have; with fewer
+      // groups than asked for, every element is a candidate
+      const unsigned long long back = (0xFFFFFFFFull - (key & 0xFFFFFFFFull)) * N + N - 1;
+      sh.least = groups < top ? 0 : (key | 0xFFFFFFFFull) - back;
+    }
   }
-  groups = min(groups, top);
-  if (rank < groups) sh.group[rank] = threadIdx.x;
-  // the smallest key that an element of that group's vector with that value can have
-  if (rank == groups - 1) sh.least = (key | 0xFFFFFFFFull) - ((0xFFFFFFFFull - (key & 0xFFFFFFFFull)) * N + N - 1);
-  if (rank == groups - 1 && groups < top) sh.least = 0;  // fewer groups than asked for: every element
   __syncthreads();
   const unsigned long long least = sh.least;
-  const int each = (part + kThreads - 1) / kThreads * GL;  // vectors of a group
-  for (int i = threadIdx.x; i < groups * each && !nan_row; i += kThreads) {
-    const int g = sh.group[i / each], j = i % each;
-    const int at = (j / GL) * kThreads + (g % kPer) * GL + j % GL, vec = (g / kPer) * part + at;
-    if (at >= part || vec >= nvec) continue;
-    const Vec<F> x = load_edge<F>(row, vec, V);
+  const int each = (part + kN - 1) / kN * GL;  // vectors of a group
+  const float tau = least ? value_of((unsigned)(least >> 32)) : -__builtin_inff();
+  constexpr int kAhead = 4;  // loads in flight
+  for (int i0 = threadIdx.x; i0 < groups * each && !nan_row; i0 += kAhead * kN) {
+    Vec<F> x[kAhead];
+    int vec[kAhead];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const unsigned long long k = key_of(Elem<F>::up(x.v[e]), vec * N + e);
-      if (vec * N + e < V && k >= least) {
-        const int c = atomicAdd(&sh.ncand, 1);
-        if (c < kCandidates) sh.cand[c] = k;
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = i0 + a * kN;
+      vec[a] = nvec;
+      if (i < groups * each) {
+        const int g = sh.group[i / each], j = i % each;
+        const int at = (j / GL) * kN + (g % kPer) * GL + j % GL;
+        if (at < part) vec[a] = min((g / kPer) * part + at, nvec);
+      }
+      if (vec[a] < nvec) x[a] = load_edge<F>(row, vec[a], V);
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (vec[a] >= nvec) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float f = Elem<F>::up(x[a].v[e]);
+        if (f < tau) continue;  // most
+        const unsigned long long k = key_of(f, vec[a] * N + e);
+        if (k >= least && vec[a] * N + e < V) {
+          const int c = atomicAdd(&sh.ncand, 1);
+          if (c < kCandidates) sh.cand[c] = k;
+        }
       }
     }
   }
   __syncthreads();
   const int ncand = sh.ncand;
   if (!nan_row && ncand <= kCandidates) {
-    for (int c = threadIdx.x; c < ncand; c += kThreads) {
+    for (int c = threadIdx.x; c < ncand; c += kN) {
       const unsigned long long k = sh.cand[c];
       int above = 0;
+#pragma unroll 8
       for (int u = 0; u < ncand; ++u) above += sh.cand[u] > k;
       if (above < top) {
         o.top_ids[n * top + above] = 0xFFFFFFFFu - (unsigned)k;
@@ -249,7 +291,7 @@ __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, i
   unsigned long long last = ~0ull;
   for (int j = 0; j < top; ++j) {
     unsigned long long best = 0;
-    for (int v = threadIdx.x; v < V; v += kThreads) {
+    for (int v = threadIdx.x; v < V; v += kN) {
       const unsigned long long c = key_of(Elem<F>::up(row[v]), v);
       if (c < last && c > best) best = c;
     }
@@ -257,7 +299,7 @@ __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, i
     __syncthreads();
     if (lane == 0) sh.key[w] = best;
     __syncthreads();
-    for (int u = 0; u < kWaves; ++u) best = sh.key[u] > best ? sh.key[u] : best;
+    for (int u = 0; u < W; ++u) best = sh.key[u] > best ? sh.key[u] : best;
     last = best;
     if (threadIdx.x == 0) {
       o.top_ids[n * top + j] = 0xFFFFFFFFu - (unsigned)best;
@@ -273,22 +315,34 @@ __device__ __forceinline__ unsigned long long group_key(float best, int at) {
 }
 
 // One workgroup per row.
-template <int F, bool TOP>
-__global__ __launch_bounds__(kThreads) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
+template <int F, bool TOP, int W>
+__global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                long long ld, const void* __restrict__ tokens,
                                                                int tok64, Out o, int V, int top, unsigned* err) {
-  __shared__ Sums lds[kWaves];
+  __shared__ Sums lds[W];
   const size_t n = blockIdx.x;
   const auto* const row = logits + (long long)n * ld;
   const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N);
+  const Token token = load_token<F>(tokens, tok64, n, row, V);
   Running<F, TOP> a;
-  scan_part<F, TOP>(row, 0, nvec, V, a);
+  scan_part<F, TOP, W>(row, 0, nvec, V, a);
   const Sums q = join_block(a.q, lds);
   const float ls = logf(q.s);
-  const bool none = finish_row<F>(n, q, ls, row, tokens, tok64, V, o, err);
+  const bool none = finish_row(n, q, ls, token, V, o, err);
   if constexpr (TOP) {
     __shared__ TopShared sh;
-    choose_top<F, 1>(row, V, top, nvec, nvec, group_key(a.best, a.at), q.r, ls, q.s != q.s, none, n, o, sh);
+    __shared__ unsigned long long keys[W * 64 / kRowLanes];
+    unsigned long long key = group_key(a.best, a.at);
+#pragma unroll
+    for (int d = 1; d < kRowLanes; d *= 2) {
+      const unsigned long long other = __shfl_xor(key, d);
+      key = other > key ? other : key;
+    }
+    key = __shfl(key, (threadIdx.x * kRowLanes) & 63);  // of thread t: group 16 (t / 64) + t mod 16
+    if ((threadIdx.x & 63) < 64 / kRowLanes) keys[threadIdx.x / 64 * (64 / kRowLanes) + (threadIdx.x & 63)] = key;
+    __syncthreads();
+    key = threadIdx.x < W * 64 / kRowLanes ? keys[threadIdx.x] : 0;
+    choose_top<F, W, kRowLanes, W * 64 / kRowLanes>(row, V, top, nvec, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
   }
 }
 
@@ -302,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const typename E
   const size_t n = blockIdx.y;
   const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N), p = blockIdx.x;
   Running<F, TOP> a;
-  scan_part<F, TOP>(logits + (long long)n * ld, p * part, min(nvec, (p + 1) * part), V, a);
+  scan_part<F, TOP, kWaves>(logits + (long long)n * ld, p * part, min(nvec, (p + 1) * part), V, a);
   const Sums q = join_block(a.q, lds);
   if (threadIdx.x == 0) sums[n * gridDim.x + p] = q;
   if constexpr (TOP) {
@@ -321,16 +375,17 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename E
   const size_t n = blockIdx.x;
   const auto* const row = logits + (long long)n * ld;
   const int nvec = (int)(((long long)V + Vec<F>::N - 1) / Vec<F>::N);
+  const Token token = load_token<F>(tokens, tok64, n, row, V);
   Sums q{kLowest, 0.f, 0.f};
   if ((int)threadIdx.x < parts) q = sums[n * parts + threadIdx.x];
   unsigned long long key = 0;
   if (TOP && (int)threadIdx.x < parts * kWaves) key = keys[n * parts * kWaves + threadIdx.x];
-  q = join_block(q, lds);
+  q = join_block<kWaves>(q, lds);
   const float ls = logf(q.s);
-  const bool none = finish_row<F>(n, q, ls, row, tokens, tok64, V, o, err);
+  const bool none = finish_row(n, q, ls, token, V, o, err);
   if constexpr (TOP) {
     __shared__ TopShared sh;
-    choose_top<F, 64>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+    choose_top<F, kWaves, 64, kThreads>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
   }
 }
 
@@ -341,11 +396,19 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
     const typename Elem<F>::T* __restrict__ logits, long long ld, const void* __restrict__ tokens, int tok64,
     const long long* __restrict__ top_ids, const float* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ dlogp, const float* __restrict__ dent, const float* __restrict__ dtop,
-    typename Elem<F>::T* __restrict__ dlogits, long long ldd, int V, int top, int part) {
+    typename Elem<F>::T* __restrict__ dlogits, long long ldd, int V, int top) {
   constexpr int N = Vec<F>::N;
   const size_t n = blockIdx.y;
   const auto* const row = logits + (long long)n * ld;
   auto* const drow = dlogits + (long long)n * ldd;
+  const int nvec = (int)(((long long)V + N - 1) / N), first = blockIdx.x * kBwdVecs * kThreads;
+  const int last = min(nvec, first + kBwdVecs * kThreads);
+  Vec<F> x[kBwdVecs];  // in flight while the row's numbers arrive
+#pragma unroll
+  for (int k = 0; k < kBwdVecs; ++k) {
+    const int i = first + k * kThreads + threadIdx.x;
+    if (i < last) x[k] = load_edge<F>(row, i, V);
+  }
   const float m = stats[2 * n], ls = stats[2 * n + 1];
   const bool none = m == -__builtin_inff();
   const long long tok = tokens && dlogp ? load_id(tokens, tok64, n) : -1;
@@ -358,16 +421,26 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
     if constexpr (ENT) return -p * __builtin_fmaf(dh, fmaxf(d, -1e30f), SH);
     return -p * SH;
   };
-  const int nvec = (int)(((long long)V + N - 1) / N), first = blockIdx.x * part, last = min(nvec, first + part);
-  for (int i = first + threadIdx.x; i < last; i += kThreads) {
-    Vec<F> x = load_edge<F>(row, i, V);
 #pragma unroll
-    for (int e = 0; e < N; ++e) x.v[e] = Elem<F>::down(none ? 0.f : grad(Elem<F>::up(x.v[e])));
+  for (int k = 0; k < kBwdVecs; ++k) {
+    const int i = first + k * kThreads + threadIdx.x;
+    if (i >= last) break;
+    float g[N];
+    if (none) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) g[e] = 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) g[e] = grad(Elem<F>::up(x[k].v[e]));
+    }
+    down_all<F, N>(g, x[k].v);
     auto* const out = drow + (size_t)i * N;
     if (i * N + N <= V) {
-      __builtin_memcpy(out, &x, sizeof(x));
+      __builtin_memcpy(out, &x[k], sizeof(x[k]));
     } else {
-      for (int e = 0; i * N + e < V; ++e) out[e] = x.v[e];
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i * N + e < V) out[e] = x[k].v[e];
     }
   }
   __syncthreads();  // their stores come after the part's
@@ -449,15 +522,18 @@ int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int to
     if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_logprob_fwd: workspace %zu bytes, need %zu", ws_bytes, need);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const Out o{logp, entropy, stats, top_logp, top_ids};
+  const Out o{tokens ? logp : nullptr, entropy, stats, top_logp, top_ids};
   return with_fmt(fmt, [&](auto f) {
     constexpr int kF = decltype(f)::value;
     const auto* x = static_cast<const typename Elem<kF>::T*>(logits);
     auto run = [&](auto t) {
       constexpr bool kTop = decltype(t)::value;
-      if (p.count == 1) {
-        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld, tokens, tok64,
-                           o, V, top, err);
+      if (p.count == 1 && V <= kShortRow) {
+        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, 1>), dim3((unsigned)N), dim3(64), 0, s, x, ld, tokens, tok64, o,
+                           V, top, err);
+      } else if (p.count == 1) {
+        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, kWaves>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld,
+                           tokens, tok64, o, V, top, err);
       } else {
         hipLaunchKernelGGL((logprob_part_kernel<kF, kTop>), dim3(p.count, (unsigned)N), dim3(kThreads), 0, s, x, ld,
                            w.sums, w.keys, V, p.vectors);
@@ -482,8 +558,8 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
   if (!logits || !stats || !dlogits || (dlogp && !tokens) || (dent && !entropy) || (dtop && !top_ids))
     return fail(HSL_ERR_ARG, "hsl_logprob_bwd: null pointer");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  // one part of `part` vectors is a workgroup; blockIdx.y holds 2^16 rows
-  const int per = fmt == kElemF32 ? 4 : 8, part = 4 * kThreads;
+  // a workgroup takes `part` vectors of a row; blockIdx.y holds fewer than 2^16 rows
+  const int per = fmt == kElemF32 ? 4 : 8, part = kBwdVecs * kThreads;
   const int nvec = (int)(((long long)V + per - 1) / per);
   return with_fmt(fmt, [&](auto f) {
     constexpr int kF = decltype(f)::value;
@@ -496,7 +572,7 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
                            tokens ? static_cast<const char*>(tokens) + n0 * (tok64 ? 8 : 4) : nullptr, tok64,
                            top_ids ? top_ids + n0 * top : nullptr, stats + 2 * n0, entropy ? entropy + n0 : nullptr,
                            dlogp ? dlogp + n0 : nullptr, dent ? dent + n0 : nullptr, dtop ? dtop + n0 * top : nullptr,
-                           static_cast<T*>(dlogits) + n0 * ldd, ldd, V, top, part);
+                           static_cast<T*>(dlogits) + n0 * ldd, ldd, V, top);
       };
       if (dent)
         run(std::true_type{});
