@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kClassTokens = 512;  // tokens of one workgroup at most (its counters: 16 waves of them)
+constexpr int kHits = 512;          // positions of a class that one wave lists in LDS
 constexpr int kBlock = 256;
 constexpr int kJoinLanes = 16, kJoinGroups = kBlock / kJoinLanes;  // 64 columns, 16 shares of the partials
 
@@ -32,112 +33,199 @@ struct Vec {
   static constexpr int N = 16 / sizeof(typename Elem<F>::T);
   typename Elem<F>::T v[N];
 };
-// Vector c of a row of D elements: what is beyond the row is not read or written.
-template <int F>
-__device__ __forceinline__ Vec<F> load_vec(const typename Elem<F>::T* row, int c, int D) {
+// The vector at element o of a row of D elements.  SMALL: D is less than a vector, of which D
+// elements are read and written.
+template <int F, bool SMALL>
+__device__ __forceinline__ Vec<F> load_vec(const typename Elem<F>::T* row, int o, int D) {
   constexpr int N = Vec<F>::N;
   Vec<F> x;
-  if (c * N + N <= D) {
-    __builtin_memcpy(&x, row + c * N, sizeof(x));
+  if constexpr (!SMALL) {
+    __builtin_memcpy(&x, row + o, sizeof(x));
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) x.v[e] = c * N + e < D ? row[c * N + e] : Elem<F>::down(0.f);
+    for (int e = 0; e < N; ++e) x.v[e] = e < D ? row[e] : Elem<F>::down(0.f);
   }
   return x;
 }
-template <int F>
-__device__ __forceinline__ void store_vec(typename Elem<F>::T* row, int c, int D, const Vec<F>& x) {
+template <int F, bool SMALL>
+__device__ __forceinline__ void store_vec(typename Elem<F>::T* row, int o, int D, const Vec<F>& x) {
   constexpr int N = Vec<F>::N;
-  if (c * N + N <= D) {
-    __builtin_memcpy(row + c * N, &x, sizeof(x));
+  if constexpr (!SMALL) {
+    __builtin_memcpy(row + o, &x, sizeof(x));
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c * N + e < D) row[c * N + e] = x.v[e];
+      if (e < D) row[e] = x.v[e];
   }
 }
 
-// A thread per vector of the output (`per` of them in a row).
-template <int F>
+// A row of D elements is `per` vectors, taken by 1 << log2g lanes (the power of two that holds
+// them, a wave at most); a wave has 64 >> log2g rows at a time.
+struct Rows {
+  int n, D, per, log2g;
+  unsigned tiles() const { return (unsigned)((per + (1 << log2g) - 1) >> log2g); }  // of columns
+  // First element of vector c.  The last vector of a row ends with the row, beside its neighbour
+  // where D is no multiple of a vector: both lanes compute and store the same values there.
+  __device__ __forceinline__ int offset(int c, int vec) const { return max(min(c * vec, D - vec), 0); }
+};
+Rows rows_of(long long n, int D, int vec) {
+  Rows r{(int)n, D, (D + vec - 1) / vec, 0};
+  while (r.log2g < 6 && (1 << r.log2g) < r.per) ++r.log2g;
+  return r;
+}
+// A wave has kWaveRows rounds of rows, whose ids (or ranges) are read ahead; the rounds are
+// blocks * rows apart, so that the rows of frequent tokens, which are neighbours, go to different
+// waves.
+constexpr int kWaveRows = 4;
+unsigned row_blocks(const Rows& r) {
+  const long long a_block = (long long)(kBlock >> r.log2g) * kWaveRows;
+  return (unsigned)((r.n + a_block - 1) / a_block);
+}
+// The thread's row of round k (at or past r.n: none).
+__device__ __forceinline__ long long row_at(const Rows& r, unsigned block, unsigned blocks, int k) {
+  return ((long long)k * blocks + block) * (kBlock >> r.log2g) + (threadIdx.x >> r.log2g);
+}
+
+template <int F, bool SMALL>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const void* __restrict__ ids, int ids64,
                                                            const typename Elem<F>::T* __restrict__ w, long long ldw,
-                                                           float scale, typename Elem<F>::T* __restrict__ out, int N,
-                                                           int V, int D, int per, unsigned* err) {
-  const long long i = (long long)blockIdx.x * kBlock + threadIdx.x;
-  const int n = (int)(i / per), c = (int)(i - (long long)n * per);
-  if (n >= N) return;
-  const long long id = load_id(ids, ids64, n);
-  const bool beyond = id >= V;
-  if (beyond && c == 0) atomicOr(err, kErrId);
-  float f[Vec<F>::N];
-  if (id >= 0 && !beyond) {
-    const Vec<F> x = load_vec<F>(w + id * ldw, c, D);
+                                                           float scale, typename Elem<F>::T* __restrict__ out, Rows r,
+                                                           int V, unsigned* err) {
+  constexpr int N = Vec<F>::N;
+  long long id[kWaveRows];
 #pragma unroll
-    for (int e = 0; e < Vec<F>::N; ++e) f[e] = scale * Elem<F>::up(x.v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < Vec<F>::N; ++e) f[e] = beyond ? __builtin_nanf("") : 0.f;
+  for (int k = 0; k < kWaveRows; ++k) {
+    const long long n = row_at(r, blockIdx.x, gridDim.x, k);
+    id[k] = n < r.n ? load_id(ids, ids64, n) : -1;
   }
-  Vec<F> o;
-  down_all<F, Vec<F>::N>(f, o.v);
-  store_vec<F>(out + (size_t)n * D, c, D, o);
+  const int c = (blockIdx.y << r.log2g) + (threadIdx.x & ((1 << r.log2g) - 1));
+  if (c >= r.per) return;
+  const int o = r.offset(c, Vec<F>::N);
+  Vec<F> x[kWaveRows];
+#pragma unroll
+  for (int k = 0; k < kWaveRows; ++k)
+    if (id[k] >= 0 && id[k] < V) x[k] = load_vec<F, SMALL>(w + id[k] * ldw, o, r.D);
+#pragma unroll
+  for (int k = 0; k < kWaveRows; ++k) {
+    const long long n = row_at(r, blockIdx.x, gridDim.x, k);
+    if (n >= r.n) break;
+    float f[N];
+    if (id[k] >= 0 && id[k] < V) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = scale * Elem<F>::up(x[k].v[e]);
+    } else {
+      const bool beyond = id[k] >= V;
+      if (beyond && c == 0) atomicOr(err, kErrId);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = beyond ? __builtin_nanf("") : 0.f;
+    }
+    Vec<F> y;
+    down_all<F, N>(f, y.v);
+    store_vec<F, SMALL>(out + n * r.D, o, r.D, y);
+  }
 }
 
-// What the sort leaves.  Token v is token q = v / nclass of class v mod nclass; a class has
-// kClassTokens + 1 entries of start.
+// What the sort leaves.  Token v is token v >> log2c of class v mod 2^log2c.
 struct Sorted {
-  int* start;   // where a token's positions begin in pos; they end at the next entry
-  int* pos;     // positions by token, rising within one
+  int2* range;  // of a token: where its positions begin and end in pos
+  int* pos;     // positions by token (by class, then within it), rising within one
   int* nlong;   // of a class: its tokens of more than `chunk` positions
   int* longs;   // [class][most]
+  int* count;   // positions in pos
   int log2c, chunk, most;
 };
-__device__ __forceinline__ int2 row_range(const Sorted& s, int v) {
-  const int* const p = s.start + (size_t)(v & ((1 << s.log2c) - 1)) * (kClassTokens + 1) + (v >> s.log2c);
-  return {p[0], p[1]};
-}
 
-// f(i, id) for a wave's part of ids in rounds of 64, kAhead loads in flight; id -1: none.
-template <class Fn>
-__device__ __forceinline__ void each_id(const void* __restrict__ ids, int ids64, int lo, int hi, int V, int padding,
-                                        Fn f) {
+// f(i, there, id) for a wave's part of ids in rounds of 64; there: the id has a row and is not the
+// padding.  The next kAhead rounds are loaded while kAhead are looked at.
+template <class I, class Fn>
+__device__ __forceinline__ void each_id(const I* __restrict__ ids, int lo, int hi, int V, int padding, Fn f) {
   constexpr int kAhead = 8;
+  if (lo >= hi) return;
   const int lane = threadIdx.x & 63;
-  for (int i0 = lo; i0 < hi; i0 += kAhead * 64) {
-    long long id[kAhead];
+  I a[kAhead], b[kAhead];
+  auto load = [&](int i0, I(&x)[kAhead]) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
+    for (int k = 0; k < kAhead; ++k) x[k] = ids[min(i0 + k * 64 + lane, hi - 1)];
+  };
+  auto look = [&](int i0, const I(&x)[kAhead]) {
+    using U = std::make_unsigned_t<I>;
+    if (i0 + kAhead * 64 <= hi) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) f(i0 + k * 64 + lane, (U)x[k] < (U)V && x[k] != padding, (int)x[k]);
+      return;
+    }
+    for (int k = 0; k < kAhead && i0 + k * 64 < hi; ++k) {
+      I v = x[0];
+#pragma unroll
+      for (int u = 1; u < kAhead; ++u) v = u == k ? x[u] : v;
       const int i = i0 + k * 64 + lane;
-      id[k] = i < hi ? load_id(ids, ids64, i) : -1;
+      f(i, (U)v < (U)V && v != padding && i < hi, (int)v);
     }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (i0 + k * 64 >= hi) break;
-      const bool there = id[k] >= 0 && id[k] < V && id[k] != padding;
-      f(i0 + k * 64 + lane, there ? (int)id[k] : -1);
-    }
+  };
+  load(lo, a);
+  for (int i0 = lo; i0 < hi; i0 += 2 * kAhead * 64) {
+    load(i0 + kAhead * 64, b);
+    look(i0, a);
+    load(i0 + 2 * kAhead * 64, a);
+    look(i0 + kAhead * 64, b);
   }
 }
 
-__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const void* __restrict__ ids, int ids64, int N,
-                                                                  int V, int padding, Sorted s) {
+// Places the positions of one round of a wave: q is the lane's token of the class (-1: none), of
+// `bits` bits.  The lanes with the same token are found bit by bit, one ballot each.
+__device__ __forceinline__ void place_round(int q, int i, int bits, int* cnt, int* __restrict__ pos) {
+  const int lane = threadIdx.x & 63;
+  unsigned long long same = __ballot(q >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = q >> b & 1;
+    const unsigned long long ones = __ballot(set);
+    same &= set ? ones : ~ones;
+  }
+  if (q < 0) return;
+  const int at = cnt[q], rank = __popcll(same & ((1ull << lane) - 1));
+  pos[at + rank] = i;
+  if (rank == 0) cnt[q] = at + __popcll(same);  // every lane of the wave has read it
+}
+
+template <class I>
+__global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const I* __restrict__ ids, int N, int V, int padding,
+                                                                  Sorted s) {
   __shared__ int cnt[kSortWaves][kClassTokens];
+  __shared__ int hit_i[kSortWaves][kHits];
+  __shared__ short hit_q[kSortWaves][kHits];
   __shared__ int below_s[kSortWaves], scan_s[kSortWaves], nlong;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = threadIdx.x;
+  const int lane = threadIdx.x & 63, t = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cls = blockIdx.x, mask = (1 << s.log2c) - 1;
   const int tokens = V > cls ? (V - cls + mask) >> s.log2c : 0;  // of this class
   for (int u = 0; u < kSortWaves; ++u)
     if (t < tokens) cnt[u][t] = 0;
   if (t == 0) nlong = 0;
   __syncthreads();
-  // the wave's part of ids, in order: its tokens' counts, and the ids of smaller residues
+  // the wave's part of ids, in order: its tokens' counts, the ids of smaller residues, and a list of
+  // its own positions
   const int part = ((N + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int lo = min(w * part, N), hi = min(lo + part, N);
-  int below = 0;
-  each_id(ids, ids64, lo, hi, V, padding, [&](int, int id) {
-    if (id < 0) return;
-    below += (id & mask) < cls;
-    if ((id & mask) == cls) atomicAdd(&cnt[w][id >> s.log2c], 1);
+  int below = 0, hits = 0;
+  each_id(ids, lo, hi, V, padding, [&](int i, bool there, int id) {
+    const int c = id & mask;
+    below += there && c < cls;
+    const unsigned long long mine = __ballot(there && c == cls);
+    if (mine == 0) return;
+    if (there && c == cls) {
+      const int q = id >> s.log2c, at = hits + __popcll(mine & ((1ull << lane) - 1));
+      // one addition where all are of one token
+      const unsigned long long ours = __ballot(q == __builtin_amdgcn_readfirstlane(q));
+      if (ours != mine)
+        atomicAdd(&cnt[w][q], 1);
+      else if (at == hits)
+        cnt[w][q] += __popcll(mine);
+      if (at < kHits) {
+        hit_i[w][at] = i;
+        hit_q[w][at] = (short)q;
+      }
+    }
+    hits += __popcll(mine);
   });
   for (int d = 32; d; d >>= 1) below += __shfl_xor(below, d);
   if (lane == 0) below_s[w] = below;
@@ -159,103 +247,123 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const void* __
   __syncthreads();
   int first = sum - total;
   for (int u = 0; u < kSortWaves; ++u) first += below_s[u] + (u < w ? scan_s[u] : 0);
-  int* const st = s.start + (size_t)cls * (kClassTokens + 1);
   if (t < tokens) {
-    st[t] = first;
-    if (t == tokens - 1) st[tokens] = first + total;
+    const int v = (t << s.log2c) | cls;
+    s.range[v] = {first, first + total};
+    // the last class with a token ends where all positions do
+    if (t == tokens - 1 && cls == min(mask, V - 1)) *s.count = first + total;
     for (int u = 0; u < kSortWaves; ++u) cnt[u][t] += first;
-    if (total > s.chunk) s.longs[(size_t)cls * s.most + atomicAdd(&nlong, 1)] = (t << s.log2c) | cls;
+    if (total > s.chunk) s.longs[(size_t)cls * s.most + atomicAdd(&nlong, 1)] = v;
   }
   __syncthreads();
   if (t == 0) s.nlong[cls] = nlong;
-  each_id(ids, ids64, lo, hi, V, padding, [&](int i, int id) {
-    const int q = id >= 0 && (id & mask) == cls ? id >> s.log2c : -1;
-    unsigned long long left = __ballot(q >= 0);
-    while (left) {  // the tokens of these 64 positions, one after the other
-      const int one = __shfl(q, __ffsll(left) - 1);
-      const unsigned long long same = __ballot(q == one);
-      if (q == one) {
-        const int at = cnt[w][one], rank = __popcll(same & ((1ull << lane) - 1));
-        s.pos[at + rank] = i;
-        if (rank == 0) cnt[w][one] = at + __popcll(same);  // every lane of the wave has read it
-      }
-      left &= ~same;
+  const int bits = 32 - __clz(max(tokens - 1, 0));
+  if (hits <= kHits) {
+    for (int k0 = 0; k0 < hits; k0 += 64) {
+      const bool in = k0 + lane < hits;
+      place_round(in ? hit_q[w][k0 + lane] : -1, in ? hit_i[w][k0 + lane] : 0, bits, cnt[w], s.pos);
     }
-  });
+  } else {  // more than the list holds: the ids again, and the list as a ring of which 64 are placed at once
+    int put = 0, got = 0;
+    each_id(ids, lo, hi, V, padding, [&](int i, bool there, int id) {
+      const unsigned long long mine = __ballot(there && (id & mask) == cls);
+      if (mine == 0) return;
+      if (there && (id & mask) == cls) {
+        const int at = (put + __popcll(mine & ((1ull << lane) - 1))) % kHits;
+        hit_i[w][at] = i;
+        hit_q[w][at] = (short)(id >> s.log2c);
+      }
+      put += __popcll(mine);
+      if (put - got >= 64) {
+        const int at = (got + lane) % kHits;
+        place_round(hit_q[w][at], hit_i[w][at], bits, cnt[w], s.pos);
+        got += 64;
+      }
+    });
+    const int at = (got + lane) % kHits;
+    const bool in = got + lane < put;
+    place_round(in ? hit_q[w][at] : -1, hit_i[w][at], bits, cnt[w], s.pos);
+  }
 }
 
-// The sum of vector c of dout over the sorted positions lo .. hi-1, in that order, four at a time.
-template <int F>
+// The sum of the vector at element o of dout over the sorted positions lo .. hi-1, in that order, three at a time.
+template <int F, bool SMALL>
 __device__ __forceinline__ void sum_positions(const int* __restrict__ pos, int lo, int hi,
-                                              const typename Elem<F>::T* __restrict__ dout, long long ldd, int c, int D,
+                                              const typename Elem<F>::T* __restrict__ dout, long long ldd, int o, int D,
                                               float (&acc)[Vec<F>::N]) {
-  constexpr int kAhead = 4;
+  constexpr int kAhead = 3;
 #pragma unroll
   for (int e = 0; e < Vec<F>::N; ++e) acc[e] = 0.f;
+  int p[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (lo + k < hi) p[k] = pos[lo + k];
   for (int i = lo; i < hi; i += kAhead) {
-    const int n = min(kAhead, hi - i);
     Vec<F> x[kAhead];
-    int p[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (k < n) p[k] = pos[i + k];
+      if (i + k < hi) x[k] = load_vec<F, SMALL>(dout + p[k] * ldd, o, D);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (k < n) x[k] = load_vec<F>(dout + p[k] * ldd, c, D);
+      if (i + kAhead + k < hi) p[k] = pos[i + kAhead + k];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (k < n) {
+      if (i + k < hi) {
 #pragma unroll
         for (int e = 0; e < Vec<F>::N; ++e) acc[e] += Elem<F>::up(x[k].v[e]);
       }
   }
 }
 
-// The first `chunk_items` threads each take a vector of one chunk: its parts of the chunk's first
-// and last token, where those are long, to partials 2 chunk and 2 chunk + 1 (rows of `pitch`).  The
-// others take a vector of a row of dW that is not long.
-template <int F>
+// The first blocks take a chunk of positions each round: its parts of the chunk's first and last
+// token, where those are long, go to partials 2 chunk and 2 chunk + 1 (rows of `pitch`).  The others
+// take the rows of dW that are not long.
+template <int F, bool SMALL>
 __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const void* __restrict__ ids, int ids64, Sorted s,
                                                            const typename Elem<F>::T* __restrict__ dout, long long ldd,
                                                            float scale, typename Elem<F>::T* __restrict__ dw,
-                                                           float* __restrict__ partial, int pitch, int V, int D,
-                                                           int per, int chunk_blocks) {
+                                                           float* __restrict__ partial, int pitch, Rows r,
+                                                           int chunk_blocks) {
   constexpr int N = Vec<F>::N;
+  const int c = (blockIdx.y << r.log2g) + (threadIdx.x & ((1 << r.log2g) - 1));
+  if (c >= r.per) return;
+  const int o = r.offset(c, Vec<F>::N);
   float acc[N];
   if ((int)blockIdx.x < chunk_blocks) {
-    const int i = blockIdx.x * kBlock + threadIdx.x, k = i / per, c = i - k * per;
-    const int end = min(1 << s.log2c, V) - 1;  // the last class with a token: its end is the table's
-    const int count = s.start[(size_t)end * (kClassTokens + 1) + ((V - 1 - end) >> s.log2c) + 1];
-    const int lo = k * s.chunk, hi = min(lo + s.chunk, count);
+    const int k = blockIdx.x * (kBlock >> r.log2g) + (threadIdx.x >> r.log2g);
+    const int lo = k * s.chunk, hi = min(lo + s.chunk, *s.count);
     if (lo >= hi) return;
     const int first = (int)load_id(ids, ids64, s.pos[lo]), last = (int)load_id(ids, ids64, s.pos[hi - 1]);
-    const int2 a = row_range(s, first), b = row_range(s, last);
-    auto put = [&](int row) {
+    const int2 a = s.range[first], b = s.range[last];
+    const bool head = a.y - a.x > s.chunk, tail = last != first && b.y - b.x > s.chunk;
+#pragma unroll
+    for (int end = 0; end < 2; ++end) {
+      if (end ? !tail : !head) continue;
+      sum_positions<F, SMALL>(s.pos, end ? b.x : lo, end ? hi : min(hi, a.y), dout, ldd, o, r.D, acc);
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (c * N + e < pitch) partial[(size_t)row * pitch + c * N + e] = acc[e];
-    };
-    if (a.y - a.x > s.chunk) {
-      sum_positions<F>(s.pos, lo, min(hi, a.y), dout, ldd, c, D, acc);
-      put(2 * k);
-    }
-    if (last != first && b.y - b.x > s.chunk) {
-      sum_positions<F>(s.pos, b.x, hi, dout, ldd, c, D, acc);
-      put(2 * k + 1);
+        if (!SMALL || e < r.D) partial[(size_t)(2 * k + end) * pitch + o + e] = acc[e];
     }
     return;
   }
-  const long long i = (long long)(blockIdx.x - chunk_blocks) * kBlock + threadIdx.x;
-  const int v = (int)(i / per), c = (int)(i - (long long)v * per);
-  if (v >= V) return;
-  const int2 r = row_range(s, v);
-  if (r.y - r.x > s.chunk) return;
-  sum_positions<F>(s.pos, r.x, r.y, dout, ldd, c, D, acc);
+  const unsigned block = blockIdx.x - chunk_blocks, blocks = gridDim.x - chunk_blocks;
+  int2 at[kWaveRows];
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] *= scale;
-  Vec<F> o;
-  down_all<F, N>(acc, o.v);
-  store_vec<F>(dw + (size_t)v * D, c, D, o);
+  for (int k = 0; k < kWaveRows; ++k) {
+    const long long v = row_at(r, block, blocks, k);
+    at[k] = v < r.n ? s.range[v] : int2{0, 0};
+  }
+#pragma unroll
+  for (int k = 0; k < kWaveRows; ++k) {
+    const long long v = row_at(r, block, blocks, k);
+    if (v >= r.n || at[k].y - at[k].x > s.chunk) continue;
+    sum_positions<F, SMALL>(s.pos, at[k].x, at[k].y, dout, ldd, o, r.D, acc);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] *= scale;
+    Vec<F> y;
+    down_all<F, N>(acc, y.v);
+    store_vec<F, SMALL>(dw + v * r.D, o, r.D, y);
+  }
 }
 
 // The long rows of class blockIdx.y, 64 columns: kJoinGroups shares of a row's partials, each added
@@ -269,7 +377,7 @@ __global__ __launch_bounds__(kBlock) void embed_join_kernel(Sorted s, const floa
   const int n = s.nlong[cls];
   for (int l = 0; l < n; ++l) {
     const int v = s.longs[(size_t)cls * s.most + l];
-    const int2 r = row_range(s, v);
+    const int2 r = s.range[v];
     const int c0 = r.x / s.chunk, parts = (r.y - 1) / s.chunk - c0 + 1;
     const int each = (parts + kJoinGroups - 1) / kJoinGroups, lo = g * each, hi = min(lo + each, parts);
     float4 sum{0.f, 0.f, 0.f, 0.f};
@@ -312,8 +420,9 @@ EmbedPlan plan_embed(long long N, int V, int D) {
   p.log2c = 8;
   while (((long long)kClassTokens << p.log2c) < V) ++p.log2c;
   p.nclass = 1 << p.log2c;
-  p.chunk = 64;  // and at most 2048 chunks
-  while ((long long)p.chunk * 2048 < N) p.chunk *= 2;
+  // short for short calls, whose time is that of one chunk; at most 4096
+  p.chunk = N <= 32768 ? 16 : 32;
+  while ((long long)p.chunk * 4096 < N) p.chunk *= 2;
   p.nchunks = N > p.chunk ? (int)((N + p.chunk - 1) / p.chunk) : 0;  // no token is longer than a chunk
   p.most = (int)std::min<long long>(kClassTokens, N / p.chunk);
   p.pitch = (D + 3) / 4 * 4;
@@ -323,11 +432,12 @@ struct EmbedWs {
   Sorted s;
   float* partial;
 };
-size_t carve_embed(void* ws, size_t cap, long long N, const EmbedPlan& p, EmbedWs* o) {
+size_t carve_embed(void* ws, size_t cap, long long N, int V, const EmbedPlan& p, EmbedWs* o) {
   Carver c(ws, cap);
-  o->s.start = c.take<int>((size_t)p.nclass * (kClassTokens + 1));
+  o->s.range = c.take<int2>(V);
   o->s.pos = c.take<int>((size_t)N);
   o->s.nlong = c.take<int>(p.nclass);
+  o->s.count = c.take<int>(1);
   o->s.longs = c.take<int>((size_t)p.nclass * p.most);
   o->s.log2c = p.log2c;
   o->s.chunk = p.chunk;
@@ -339,9 +449,8 @@ size_t carve_embed(void* ws, size_t cap, long long N, const EmbedPlan& p, EmbedW
 int check_embed(const char* who, long long N, int V, int D, long long ld, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
   if (N < 0 || V < 0 || D < 0 || ld < 0) return fail(HSL_ERR_ARG, "%s: negative size (N=%lld V=%d D=%d)", who, N, V, D);
-  const long long per = (D + 3ll) / 4, lim = 1ll << 31;
-  if (N > 0x7FFF0000 || N * per / kBlock >= lim - 2 || V * per / kBlock >= lim - 2 || D > 0x7FFFFFF0)
-    return fail(HSL_ERR_UNSUPPORTED, "%s: N=%lld V=%d D=%d is beyond 2^31 ids or a grid of 2^31 workgroups", who, N, V, D);
+  if (N > 0x7FFF0000 || V > 0x7FFF0000 || D > 0x7FFF0000)
+    return fail(HSL_ERR_UNSUPPORTED, "%s: N=%lld V=%d D=%d need less than 2^31 - 2^16 each", who, N, V, D);
   return HSL_OK;
 }
 
@@ -362,10 +471,11 @@ int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw,
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_fmt(fmt, [&](auto f) {
     using T = typename Elem<decltype(f)::value>::T;
-    const int per = (D + Vec<decltype(f)::value>::N - 1) / Vec<decltype(f)::value>::N;
-    hipLaunchKernelGGL(embed_fwd_kernel<decltype(f)::value>, dim3((unsigned)((N * per + kBlock - 1) / kBlock)),
-                       dim3(kBlock), 0, s, ids, ids64, static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out),
-                       (int)N, V, D, per, err);
+    const Rows r = rows_of(N, D, Vec<decltype(f)::value>::N);
+    const auto kernel = D < Vec<decltype(f)::value>::N ? embed_fwd_kernel<decltype(f)::value, true>
+                                                       : embed_fwd_kernel<decltype(f)::value, false>;
+    hipLaunchKernelGGL(kernel, dim3(row_blocks(r), r.tiles()), dim3(kBlock), 0, s, ids, ids64,
+                       static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out), r, V, err);
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
   });
@@ -374,7 +484,7 @@ int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw,
 size_t hsl_embed_bwd_ws_bytes(long long N, int V, int D) {
   if (N < 0 || V < 0 || D < 0) return 0;
   EmbedWs w;
-  return carve_embed(nullptr, 0, N, plan_embed(N, V, D), &w);
+  return carve_embed(nullptr, 0, N, V, plan_embed(N, V, D), &w);
 }
 
 int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, float scale, int padding_idx,
@@ -384,20 +494,24 @@ int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, f
   if (!dweight || (N > 0 && (!ids || !dout))) return fail(HSL_ERR_ARG, "hsl_embed_bwd: null pointer");
   const EmbedPlan p = plan_embed(N, V, D);
   EmbedWs w;
-  const size_t need = carve_embed(ws, ws_bytes, N, p, &w);
+  const size_t need = carve_embed(ws, ws_bytes, N, V, p, &w);
   if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_embed_bwd: workspace %zu bytes, need %zu", ws_bytes, need);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(embed_sort_kernel, dim3(p.nclass), dim3(kSortThreads), 0, s, ids, ids64, (int)N, V, padding_idx,
-                     w.s);
+  if (ids64)
+    hipLaunchKernelGGL(embed_sort_kernel<long long>, dim3(p.nclass), dim3(kSortThreads), 0, s,
+                       static_cast<const long long*>(ids), (int)N, V, padding_idx, w.s);
+  else
+    hipLaunchKernelGGL(embed_sort_kernel<int>, dim3(p.nclass), dim3(kSortThreads), 0, s, static_cast<const int*>(ids),
+                       (int)N, V, padding_idx, w.s);
   return with_fmt(fmt, [&](auto f) {
     constexpr int kF = decltype(f)::value;
     using T = typename Elem<kF>::T;
-    const int per = (D + Vec<kF>::N - 1) / Vec<kF>::N;
-    const long long chunk_blocks = ((long long)p.nchunks * per + kBlock - 1) / kBlock;
-    const long long row_blocks = ((long long)V * per + kBlock - 1) / kBlock;
-    hipLaunchKernelGGL(embed_sum_kernel<kF>, dim3((unsigned)(chunk_blocks + row_blocks)), dim3(kBlock), 0, s, ids, ids64,
-                       w.s, static_cast<const T*>(dout), ldd, scale, static_cast<T*>(dweight), w.partial, p.pitch, V, D,
-                       per, (int)chunk_blocks);
+    const Rows r = rows_of(V, D, Vec<kF>::N);
+    const int chunk_blocks = (p.nchunks + (kBlock >> r.log2g) - 1) / (kBlock >> r.log2g);
+    const auto sums = D < Vec<kF>::N ? embed_sum_kernel<kF, true> : embed_sum_kernel<kF, false>;
+    hipLaunchKernelGGL(sums, dim3(chunk_blocks + row_blocks(r), r.tiles()), dim3(kBlock), 0, s, ids, ids64, w.s,
+                       static_cast<const T*>(dout), ldd, scale, static_cast<T*>(dweight), w.partial, p.pitch, r,
+                       chunk_blocks);
     if (p.nchunks)
       hipLaunchKernelGGL(embed_join_kernel<kF>, dim3((D + 4 * kJoinLanes - 1) / (4 * kJoinLanes), p.nclass),
                          dim3(kBlock), 0, s, w.s, w.partial, p.pitch, scale, static_cast<T*>(dweight), D);

@@ -97,6 +97,29 @@ def test_embedding_frequent_token(dev):
     _within("dweight", dw, want, torch.bincount(ids, minlength=V)[:, None].double() * u * mag + u)
 
 
+@pytest.mark.parametrize("kind", ["one", "few", "half"])
+def test_embedding_many_positions_of_few_tokens(dev, kind):
+    """More positions of a class than a workgroup lists: one token, a few, and half of them one."""
+    g = _gen("many", kind)
+    N, V, D = 40003, 600, 24
+    ids = torch.randint(0, V, (N,), generator=g)
+    if kind == "one":
+        ids[:] = 256
+    elif kind == "few":
+        ids = ids % 2 * 256 + 5
+    else:
+        ids[torch.rand(N, generator=g) < 0.5] = 599
+    dout = torch.randn(N, D, generator=g)
+    want = torch.zeros(V, D, dtype=torch.float64).index_add_(0, ids, dout.double())
+    mag = torch.zeros(V, D, dtype=torch.float64).index_add_(0, ids, dout.double().abs())
+    bound = (torch.bincount(ids, minlength=V)[:, None].double() + 2) * u * mag + 1e-36
+    for ids_dtype in (torch.int64, torch.int32):
+        w = torch.zeros(V, D, device=dev, requires_grad=True)
+        out = prlstm_amd.embedding(ids.to(dev, ids_dtype), w)
+        dw, = torch.autograd.grad(out, w, dout.to(dev))
+        _within("dweight", dw, want, bound)
+
+
 def test_embedding_strides_and_broadcast_gradient(dev):
     g = _gen("strides")
     ids = torch.randint(0, 40, (6, 9), generator=g)
