@@ -204,8 +204,8 @@ __device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, co
 // the k largest elements: any other group's elements are all below those k.  So only these groups
 // are read again, for the elements at or above the k-th group's key, and those are ranked by
 // counting.  Groups are GL lanes wide: group g has vectors (g / (n / GL)) * part + n i +
-// (g mod (n / GL)) * GL + 0 .. GL-1, n the threads.  A row of one workgroup has groups of 4 lanes
-// (64 of 4 waves, which one wave ranks); with 256 of one lane the ranking took 2 us of the workgroup's time instead of 0.1,
+// (g mod (n / GL)) * GL + 0 .. GL-1, n the threads.  A row of one workgroup has 64 groups, which one
+// wave ranks; with 256 of one lane the ranking took 2 us of the workgroup's time instead of 0.1,
 // more than the three vectors more that each lane reads again.
 struct alignas(16) TopShared {
   unsigned long long key[kThreads];  // one for each group
@@ -330,19 +330,20 @@ __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem
   const float ls = logf(q.s);
   const bool none = finish_row(n, q, ls, token, V, o, err);
   if constexpr (TOP) {
+    constexpr int GL = W > 1 ? kRowLanes : 1;  // 64 groups
     __shared__ TopShared sh;
-    __shared__ unsigned long long keys[W * 64 / kRowLanes];
+    __shared__ unsigned long long keys[W * 64 / GL];
     unsigned long long key = group_key(a.best, a.at);
 #pragma unroll
-    for (int d = 1; d < kRowLanes; d *= 2) {
+    for (int d = 1; d < GL; d *= 2) {
       const unsigned long long other = __shfl_xor(key, d);
       key = other > key ? other : key;
     }
-    key = __shfl(key, (threadIdx.x * kRowLanes) & 63);  // of thread t: group 16 (t / 64) + t mod 16
-    if ((threadIdx.x & 63) < 64 / kRowLanes) keys[threadIdx.x / 64 * (64 / kRowLanes) + (threadIdx.x & 63)] = key;
+    key = __shfl(key, (threadIdx.x * GL) & 63);  // of thread t: group 16 (t / 64) + t mod 16
+    if ((threadIdx.x & 63) < 64 / GL) keys[threadIdx.x / 64 * (64 / GL) + (threadIdx.x & 63)] = key;
     __syncthreads();
-    key = threadIdx.x < W * 64 / kRowLanes ? keys[threadIdx.x] : 0;
-    choose_top<F, W, kRowLanes, W * 64 / kRowLanes>(row, V, top, nvec, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+    key = threadIdx.x < W * 64 / GL ? keys[threadIdx.x] : 0;
+    choose_top<F, W, GL, W * 64 / GL>(row, V, top, nvec, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
   }
 }
 
@@ -462,12 +463,15 @@ struct Parts {
 Parts plan_parts(long long N, int V, int fmt) {
   const int per = fmt == kElemF32 ? 4 : 8;
   const int nvec = (int)(((long long)V + per - 1) / per);
+  // at least 8 parts: their groups are as many as the alternatives may be
   int count = 1;
-  if (N < 512) count = (int)std::min<long long>({(1024 + N - 1) / std::max(N, 1ll), kMaxParts, (nvec + kThreads - 1) / kThreads});
-  count = std::max(count, 1);
-  // whole rounds of a workgroup's threads
-  const int vectors = ((nvec + count - 1) / count + kThreads - 1) / kThreads * kThreads;
-  return {std::max(1, (nvec + vectors - 1) / vectors), vectors};
+  if (N < 512 && nvec >= 8 * kThreads)
+    count = (int)std::min<long long>({std::max((1024 + N - 1) / std::max(N, 1ll), 8ll), kMaxParts, nvec / kThreads});
+  if (count == 1) return {1, nvec};
+  // whole rounds of a workgroup's threads; rounded down, where that is not too many parts
+  int vectors = nvec / count / kThreads * kThreads;
+  if ((nvec + vectors - 1) / vectors > kMaxParts) vectors += kThreads;
+  return {(nvec + vectors - 1) / vectors, vectors};
 }
 
 struct LogprobWs {

@@ -438,7 +438,7 @@ def _check_logprob(dev, logits, tokens, top, g, dtype, ent=True):
 
 LOGPROB = [  # N, V, top
     (0, 7, 2), (1, 1, 1), (3, 2, 0), (5, 31, 31), (2, 64, 32), (7, 65, 5), (4, 255, 3), (3, 257, 1), (2, 1000, 20),
-    (1, 2049, 32), (6, 4099, 7), (2, 10007, 5), (1, 70001, 20), (300, 100, 4), (2, 33333, 0), (1, 262144, 32),
+    (1, 2049, 32), (6, 4099, 7), (2, 10007, 5), (1, 70001, 20), (300, 100, 4), (2, 33333, 0), (1, 262144, 32), (40, 20001, 32), (3, 16383, 32), (520, 2049, 32),
 ]
 
 
