@@ -19,7 +19,8 @@ namespace {
 
 constexpr int kMaxTop = 32;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kMaxParts = 64;        // of a row; a part has kWaves groups, at most kThreads in all
+constexpr int kMaxParts = 64;        // of a row
+constexpr int kFineParts = 16;       // up to which a part has groups of 16 lanes, not of 64
 constexpr int kBwdVecs = 2;          // vectors of a thread in the backward
 constexpr int kShortRow = 2048;      // logits of a row that one wave takes
 constexpr int kRowLanes = 4;         // of a group in a row of one workgroup
@@ -80,19 +81,12 @@ __device__ __forceinline__ Vec<F> load_edge(const typename Elem<F>::T* row, int 
 // s = sum e^(x - r), sd = sum e^(x - r) (x - r) over some elements; r is one of them or kLowest.
 struct Sums {
   float r, s, sd;
-  // the same with a larger reference
+  // the same with another reference, no smaller
   __device__ __forceinline__ void rebase(float to) {
     const float gap = r - to, c = __builtin_amdgcn_exp2f(gap * kLog2e);
     sd = c == 0.f ? 0.f : c * __builtin_fmaf(gap, s, sd);  // (gap may be -inf)
     s *= c;
     r = to;
-  }
-  __device__ __forceinline__ void add(Sums o) {
-    const float to = fmaxf(r, o.r);
-    if (r != to) rebase(to);
-    if (o.r != to) o.rebase(to);
-    s += o.s;
-    sd += o.sd;
   }
 };
 
@@ -143,17 +137,34 @@ __device__ __forceinline__ void scan_part(const typename Elem<F>::T* __restrict_
   for (; i < last; i += kN) a.take(load_edge<F>(row, i, V), i);
 }
 
-// The sums of the whole workgroup, in every thread.
+// The sums of the whole workgroup, in every thread: the largest reference first, to which each
+// lane's sums are brought once.
 template <int W>
 __device__ __forceinline__ Sums join_block(Sums q, Sums (&lds)[W]) {
+  float to = q.r;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) q.add(Sums{__shfl_xor(q.r, d), __shfl_xor(q.s, d), __shfl_xor(q.sd, d)});
+  for (int d = 32; d; d >>= 1) to = fmaxf(to, __shfl_xor(to, d));
+  if (q.r != to) q.rebase(to);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    q.s += __shfl_xor(q.s, d);
+    q.sd += __shfl_xor(q.sd, d);
+  }
   if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = q;
     __syncthreads();
-    q = lds[0];
+    to = lds[0].r;
 #pragma unroll
-    for (int w = 1; w < W; ++w) q.add(lds[w]);
+    for (int w = 1; w < W; ++w) to = fmaxf(to, lds[w].r);
+    Sums sum{to, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      Sums o = lds[w];
+      if (o.r != to) o.rebase(to);
+      sum.s += o.s;
+      sum.sd += o.sd;
+    }
+    q = sum;
   }
   return q;
 }
@@ -212,6 +223,7 @@ struct alignas(16) TopShared {
   unsigned long long cand[kCandidates];
   int group[kMaxTop];
   unsigned long long least;
+  int count[kWaves];
   int ncand;
 };
 template <int F, int W, int GL, int KEYS>
@@ -242,38 +254,87 @@ __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, i
   const unsigned long long least = sh.least;
   const int each = (part + kN - 1) / kN * GL;  // vectors of a group
   const float tau = least ? value_of((unsigned)(least >> 32)) : -__builtin_inff();
-  constexpr int kAhead = 4;  // loads in flight
-  for (int i0 = threadIdx.x; i0 < groups * each && !nan_row; i0 += kAhead * kN) {
-    Vec<F> x[kAhead];
-    int vec[kAhead];
+  // the selected groups' elements at or above `from`, or above tau alone
+  auto collect = [&](unsigned long long from, bool above_tau) {
+    constexpr int kAhead = 4;  // loads in flight
+    for (int i0 = threadIdx.x; i0 < groups * each; i0 += kAhead * kN) {
+      Vec<F> x[kAhead];
+      int vec[kAhead];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int i = i0 + a * kN;
-      vec[a] = nvec;
-      if (i < groups * each) {
-        const int g = sh.group[i / each], j = i % each;
-        const int at = (j / GL) * kN + (g % kPer) * GL + j % GL;
-        if (at < part) vec[a] = min((g / kPer) * part + at, nvec);
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a * kN;
+        vec[a] = nvec;
+        if (i < groups * each) {
+          const int g = sh.group[i / each], j = i % each;
+          const int at = (j / GL) * kN + (g % kPer) * GL + j % GL;
+          if (at < part) vec[a] = min((g / kPer) * part + at, nvec);
+        }
+        if (vec[a] < nvec) x[a] = load_edge<F>(row, vec[a], V);
       }
-      if (vec[a] < nvec) x[a] = load_edge<F>(row, vec[a], V);
-    }
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      if (vec[a] >= nvec) continue;
+      for (int a = 0; a < kAhead; ++a) {
+        if (vec[a] >= nvec) continue;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float f = Elem<F>::up(x[a].v[e]);
-        if (f < tau) continue;  // most
-        const unsigned long long k = key_of(f, vec[a] * N + e);
-        if (k >= least && vec[a] * N + e < V) {
-          const int c = atomicAdd(&sh.ncand, 1);
-          if (c < kCandidates) sh.cand[c] = k;
+        for (int e = 0; e < N; ++e) {
+          const float f = Elem<F>::up(x[a].v[e]);
+          if (f < tau || (above_tau && f == tau)) continue;  // most
+          const unsigned long long k = key_of(f, vec[a] * N + e);
+          if (k >= from && vec[a] * N + e < V) {
+            const int c = atomicAdd(&sh.ncand, 1);
+            if (c < kCandidates) sh.cand[c] = k;
+          }
         }
       }
     }
-  }
+  };
+  if (!nan_row) collect(least, false);
   __syncthreads();
-  const int ncand = sh.ncand;
+  int ncand = sh.ncand;
+  if (!nan_row && ncand > kCandidates) {
+    // Many equal elements, as in a row of masks: those above tau, and of those equal to it the
+    // first in the row.
+    __syncthreads();
+    if (threadIdx.x == 0) sh.ncand = 0;
+    __syncthreads();
+    collect(0, true);
+    __syncthreads();
+    ncand = sh.ncand;
+    if (ncand <= kCandidates - kMaxTop) {
+      for (int i0 = 0; i0 < nvec && ncand < top; i0 += kN) {
+        const int i = i0 + threadIdx.x;
+        Vec<F> x;
+        int equal = 0;
+        if (i < nvec) {
+          x = load_edge<F>(row, i, V);
+#pragma unroll
+          for (int e = 0; e < N; ++e) equal += i * N + e < V && Elem<F>::up(x.v[e]) == tau;
+        }
+        int upto = equal;  // of the wave's lanes up to this one, then of the workgroup's
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int v = __shfl_up(upto, d);
+          if (lane >= d) upto += v;
+        }
+        if (lane == 63) sh.count[w] = upto;
+        __syncthreads();
+        int at = ncand + upto - equal;
+        for (int u = 0; u < W; ++u) {
+          if (u < w) at += sh.count[u];
+          ncand += sh.count[u];
+        }
+        if (equal) {
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (i * N + e < V && Elem<F>::up(x.v[e]) == tau) {
+              if (at < top) sh.cand[at] = key_of(tau, i * N + e);
+              ++at;
+            }
+        }
+        __syncthreads();
+      }
+      ncand = min(ncand, max(top, sh.ncand));
+    }
+  }
   if (!nan_row && ncand <= kCandidates) {
     for (int c = threadIdx.x; c < ncand; c += kN) {
       const unsigned long long k = sh.cand[c];
@@ -348,7 +409,8 @@ __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem
 }
 
 // Few rows: each is cut into parts of `part` vectors, whose sums and groups' keys go to ws.
-template <int F, bool TOP>
+// GL: lanes of a group, as many as give at most kThreads groups.
+template <int F, bool TOP, int GL>
 __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                 long long ld, Sums* __restrict__ sums,
                                                                 unsigned long long* __restrict__ keys, int V,
@@ -361,12 +423,17 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const typename E
   const Sums q = join_block(a.q, lds);
   if (threadIdx.x == 0) sums[n * gridDim.x + p] = q;
   if constexpr (TOP) {
-    const unsigned long long key = wave_max(group_key(a.best, a.at));
-    if ((threadIdx.x & 63) == 0) keys[(n * gridDim.x + p) * kWaves + (threadIdx.x >> 6)] = key;
+    unsigned long long key = group_key(a.best, a.at);
+#pragma unroll
+    for (int d = GL / 2; d; d >>= 1) {
+      const unsigned long long other = __shfl_xor(key, d);
+      key = other > key ? other : key;
+    }
+    if (threadIdx.x % GL == 0) keys[(n * gridDim.x + p) * (kThreads / GL) + threadIdx.x / GL] = key;
   }
 }
 
-template <int F, bool TOP>
+template <int F, bool TOP, int GL>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                 long long ld, const Sums* __restrict__ sums,
                                                                 const unsigned long long* __restrict__ keys,
@@ -380,13 +447,14 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename E
   Sums q{kLowest, 0.f, 0.f};
   if ((int)threadIdx.x < parts) q = sums[n * parts + threadIdx.x];
   unsigned long long key = 0;
-  if (TOP && (int)threadIdx.x < parts * kWaves) key = keys[n * parts * kWaves + threadIdx.x];
+  constexpr int kPer = kThreads / GL;
+  if (TOP && (int)threadIdx.x < parts * kPer) key = keys[n * parts * kPer + threadIdx.x];
   q = join_block<kWaves>(q, lds);
   const float ls = logf(q.s);
   const bool none = finish_row(n, q, ls, token, V, o, err);
   if constexpr (TOP) {
     __shared__ TopShared sh;
-    choose_top<F, kWaves, 64, kThreads>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+    choose_top<F, kWaves, GL, kThreads>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
   }
 }
 
@@ -463,10 +531,12 @@ struct Parts {
 Parts plan_parts(long long N, int V, int fmt) {
   const int per = fmt == kElemF32 ? 4 : 8;
   const int nvec = (int)(((long long)V + per - 1) / per);
-  // at least 8 parts: their groups are as many as the alternatives may be
+  // At least 9 parts: the groups of all but the last are as many as the alternatives may be.
   int count = 1;
-  if (N < 512 && nvec >= 8 * kThreads)
-    count = (int)std::min<long long>({std::max((1024 + N - 1) / std::max(N, 1ll), 8ll), kMaxParts, nvec / kThreads});
+  if (N < 512 && nvec >= 9 * kThreads) {
+    const long long want = std::max((2048 + N - 1) / std::max(N, 1ll), 9ll);
+    count = (int)std::min<long long>({want, kMaxParts, nvec / kThreads});
+  }
   if (count == 1) return {1, nvec};
   // whole rounds of a workgroup's threads; rounded down, where that is not too many parts
   int vectors = nvec / count / kThreads * kThreads;
@@ -481,7 +551,7 @@ struct LogprobWs {
 size_t carve_logprob(void* ws, size_t cap, long long N, int parts, LogprobWs* o) {
   Carver c(ws, cap);
   o->sums = c.take<Sums>((size_t)N * parts);
-  o->keys = c.take<unsigned long long>((size_t)N * parts * kWaves);
+  o->keys = c.take<unsigned long long>((size_t)N * kThreads);
   return align_up(c.off, 256);
 }
 
@@ -539,10 +609,17 @@ int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int to
         hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, kWaves>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld,
                            tokens, tok64, o, V, top, err);
       } else {
-        hipLaunchKernelGGL((logprob_part_kernel<kF, kTop>), dim3(p.count, (unsigned)N), dim3(kThreads), 0, s, x, ld,
-                           w.sums, w.keys, V, p.vectors);
-        hipLaunchKernelGGL((logprob_join_kernel<kF, kTop>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld, w.sums,
-                           w.keys, tokens, tok64, o, V, p.vectors, p.count, top, err);
+        auto cut = [&](auto lanes) {
+          constexpr int kGL = decltype(lanes)::value;
+          hipLaunchKernelGGL((logprob_part_kernel<kF, kTop, kGL>), dim3(p.count, (unsigned)N), dim3(kThreads), 0, s, x,
+                             ld, w.sums, w.keys, V, p.vectors);
+          hipLaunchKernelGGL((logprob_join_kernel<kF, kTop, kGL>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld,
+                             w.sums, w.keys, tokens, tok64, o, V, p.vectors, p.count, top, err);
+        };
+        if (kTop && p.count <= kFineParts)
+          cut(std::integral_constant<int, kTop ? 16 : 64>{});
+        else
+          cut(std::integral_constant<int, 64>{});
       }
     };
     if (top)

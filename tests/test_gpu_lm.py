@@ -510,10 +510,12 @@ def test_logprobs_alternatives_in_hard_orders(dev, V):
     rows = [torch.zeros(V), torch.zeros(V).index_fill_(0, torch.arange(0, V, 2), -0.0), ramp, -ramp,
             torch.randint(0, 3, (V,), generator=g).float(), (torch.arange(V) // 40).float() * 1e-3,
             -(torch.arange(V) // 9000).float(), torch.where(torch.arange(V) % 256 == 7, ramp + 5, ramp),
-            torch.where(torch.arange(V) < 4000, ramp + 5, ramp)]
+            torch.where(torch.arange(V) < 4000, ramp + 5, ramp), torch.full((V,), -float("inf")),
+            torch.full((V,), -3e38), torch.where(torch.arange(V) % 3000 == 5, ramp, torch.full((V,), -float("inf"))),
+            torch.where(torch.arange(V) > V - 25, ramp + 1, torch.zeros(V))]
     x = torch.stack(rows)
     for dtype in DTYPES:
-        xt = x.to(dtype)
+        xt = x.clamp_min(torch.finfo(dtype).min).where(x != -float("inf"), x).to(dtype)
         for top in (1, 32):
             r = prlstm_amd.token_logprobs(xt.to(dev), top=top)
             assert r.logp is None
