@@ -4,7 +4,7 @@
 // Backward, with U_T = dh_n:  G_t = dout_t + U_{t+1},  U_t = reset_t ? 0 : f_t G_t,
 //   dv_t = w_t G_t,  dz_t = G_t (h'_{t-1} - v_t) f_t w_t,  dh0 = U_0.
 // zv holds z in its first H and v in its last H channels.  The state is fp32 throughout; out is
-// h rounded once.  ck keeps h as it enters every 8th step, in fp32, from which the backward runs
+// h rounded once.  ck keeps h as it enters every 16th step, in fp32, from which the backward runs
 // the steps again (the rounded out would cost dz its precision where h and v are close).
 //
 // Both directions are first-order recurrences, so runs of steps compose into affine maps
@@ -22,7 +22,8 @@
 namespace hsl {
 namespace {
 
-constexpr int kSteps = 8;    // of a group in a chunk, and per checkpoint row
+constexpr int kSteps = 8;    // of a group in a chunk
+constexpr int kCkSteps = 2 * kSteps;  // of a wave's two groups: one checkpoint row
 constexpr int kLanes = 32;   // of a group
 constexpr int kMaxWaves = 8;
 
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
   const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + (tb + q.g * kSteps) * zv.st + q.j;
   const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + (tb + q.g * kSteps) * reset.st;
   T_* op = static_cast<T_*>(out.p) + q.b * out.sb + (tb + q.g * kSteps) * out.st + q.j;
-  float* cp = ck + (size_t)(tb / kSteps + q.g) * C + q.ch;
+  float* cp = ck + (size_t)(tb / kCkSteps + q.w) * C + q.ch;
 
   Pack<F, E> rz[2][kSteps], rv[2][kSteps];
   unsigned char rr[2][kSteps];
@@ -326,15 +327,17 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
     T_* const o0 = op;
     float* const c0 = cp;
     op += chunk * out.st;
-    cp += (size_t)(chunk / kSteps) * C;
+    cp += (size_t)(chunk / kCkSteps) * C;
     if (!q.ok || (TAIL && t0 >= te)) return;
-    if (ck) store_floats(c0, h);
+    if (ck && q.lane < kLanes) store_floats(c0, h);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       Pack<F, E> o;
 #pragma unroll
-      for (int e = 0; e < E; ++e) h[e] = apply<CUTS>(f[s][e], wv[s][e], h[e]);
-      down_all<F, E>(h, o.v);
+      for (int e = 0; e < E; ++e) {
+        h[e] = apply<CUTS>(f[s][e], wv[s][e], h[e]);
+        o.v[e] = Elem<F>::down(h[e]);
+      }
       if (!TAIL || t0 + s < te) store_pack<F, E>(o0 + s * out.st, o);
     }
     if (TAIL && te == T && T - t0 <= kSteps) store_floats(h_n + q.ch, h);
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
   const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + last * zv.st + q.j;
   const T_* dp = static_cast<const T_*>(dout.p) + q.b * dout.sb + last * dout.st + q.j;
   const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + last * reset.st;
-  const float* cp = ck + (last / kSteps) * C + q.ch;
+  const float* cp = ck + (last / kCkSteps) * C + q.ch;
   T_* gp = static_cast<T_*>(dzv.p) + q.b * dzv.sb + last * dzv.st + q.j;
 
   struct Chunk {  // of the group, in registers
@@ -444,7 +447,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     constexpr bool TAIL = decltype(tail)::value;  // steps past T are not read
     const int t0 = t1 + q.g * kSteps;
     m.h = Floats<E>{};
-    if (!TAIL || t0 < te) m.h = load_floats<E>(cp);
+    if (!TAIL || t0 < te) m.h = load_floats<E>(cp);  // of the wave's first group
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       if (TAIL) m.z[s] = m.v[s] = Pack<F, E>{};
@@ -459,7 +462,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
     zp -= chunk * zv.st;
     dp -= chunk * dout.st;
     if constexpr (RESET) rp -= chunk * reset.st;
-    cp -= (size_t)(chunk / kSteps) * C;
+    cp -= (size_t)(chunk / kCkSteps) * C;
   };
   auto step = [&](auto tail, auto resets, int t1, int par, Chunk& m) {
     constexpr bool TAIL = decltype(tail)::value;  // the chunk with step T-1: U passes later ones
@@ -472,16 +475,30 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, St
       V[e] = 0.f;
       h[e] = m.h.v[e];
     }
+    float wv[kSteps][E];
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const Gates g = gates_of<F>(Elem<F>::up(m.z[s].v[e]));
-        const float v = Elem<F>::up(m.v[s].v[e]);
         f[s][e] = g.f;
         w[s][e] = g.w;
+        wv[s][e] = g.w * Elem<F>::up(m.v[s].v[e]);
+        h[e] = CUTS && m.r[s] ? wv[s][e] : __builtin_fmaf(g.f, h[e], wv[s][e]);
+      }
+    }
+    // the state behind the wave's first group enters its second
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float behind = __shfl_xor(h[e], kLanes);
+      h[e] = q.lane < kLanes ? m.h.v[e] : behind;
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
         hp[s][e] = CUTS && m.r[s] ? 0.f : h[e];
-        h[e] = CUTS && m.r[s] ? g.w * v : __builtin_fmaf(g.f, h[e], g.w * v);
+        h[e] = CUTS && m.r[s] ? wv[s][e] : __builtin_fmaf(f[s][e], h[e], wv[s][e]);
       }
     }
 #pragma unroll
@@ -634,16 +651,23 @@ __global__ __launch_bounds__(256) void gated_step_kernel(Stream zv, const float*
 struct GatedPlan {
   int waves, tiles, nseg, seg_steps;
 };
+// Waves: 8 (chunks of 128 steps) where a CU gets one or two workgroups, 4 where it gets more or the
+// time is cut, 1 and 2 for short sequences.  us forward, backward, bf16, 8 waves / 4 waves:
+//   T4096 B16 H1024 (256 workgroups): 73, 152 / 87, 166;  T256 B64 H1024 (1024): 24, 39 / 21, 31
+//   T2048 B32 H1024 (512): 79, 150 / 81, 140;  16 waves at 256 workgroups: 119, 275 (registers)
+// Segments: of at least two chunks, for about 512 workgroups, where the channels alone give fewer
+// than 192.  us of T16383 B2 H256 fp32, 8 tiles: 36, 40 for 512; 47, 45 for 256; 38, 46 for 1024.
 GatedPlan plan_gated(int T, int B, int H, int E) {
   GatedPlan p;
   p.tiles = (int)(((long)B * ((H + E - 1) / E) + kLanes - 1) / kLanes);
+  const int most = p.tiles >= 512 ? kMaxWaves / 2 : kMaxWaves;
   p.waves = 1;
-  while (p.waves < kMaxWaves && p.waves * 2 * kSteps < T) p.waves *= 2;
+  while (p.waves < most && p.waves * 2 * kSteps < T) p.waves *= 2;
   int chunk = p.waves * 2 * kSteps, nchunks = (T + chunk - 1) / chunk;
   p.nseg = 1;
   p.seg_steps = std::max(1, nchunks) * chunk;
   if (p.tiles < 192 && nchunks >= 4) {
-    p.waves = std::min(p.waves, 4);
+    p.waves = std::min(p.waves, kMaxWaves / 2);
     chunk = p.waves * 2 * kSteps;
     nchunks = (T + chunk - 1) / chunk;
     const int want = std::min(nchunks / 2, (512 + p.tiles - 1) / p.tiles);
@@ -692,7 +716,7 @@ using namespace hsl;
 
 extern "C" {
 
-int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kSteps - 1) / kSteps; }
+int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kCkSteps - 1) / kCkSteps; }
 
 size_t hsl_gated_ws_bytes(int T, int B, int H) {
   if (T < 0 || B < 0 || H < 0) return 0;
