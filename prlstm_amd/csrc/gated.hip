@@ -687,9 +687,9 @@ int check_gated(const char* who, int T, int B, int H, int fmt) {
 int channels_each(int T, int H) { return T == 1 ? 2 - H % 2 : std::min(H, 2); }
 
 // Whether a call's streams (`bytes` in all) are read without keeping them in the caches: where they
-// exceed the 256 MB last-level cache and every workgroup's rows are whole 128-byte lines.
+// exceed those and every workgroup's rows are whole 128-byte lines.
 bool streams_past_cache(size_t bytes, int H, int es, std::initializer_list<Stream> streams) {
-  if (bytes <= (256u << 20) || (size_t)H * es % 128) return false;
+  if (bytes <= kCacheBytes || (size_t)H * es % 128) return false;
   for (const Stream& s : streams)
     if (reinterpret_cast<uintptr_t>(s.p) % 128 || s.st * es % 128 || s.sb * es % 128) return false;
   return true;

@@ -54,6 +54,19 @@ __device__ __forceinline__ void down_all(const float (&f)[N], typename Elem<F>::
   }
 }
 
+// 16 bytes to any element's alignment (global memory takes unaligned accesses), non-temporal.
+template <class V>
+__device__ __forceinline__ void store16_nt(void* p, const V& x) {
+  typedef unsigned U4 __attribute__((ext_vector_type(4)));
+  typedef U4 Raw __attribute__((aligned(2), may_alias));
+  static_assert(sizeof(V) == sizeof(U4), "16 bytes");
+  U4 u;
+  __builtin_memcpy(&u, &x, sizeof(u));
+  __builtin_nontemporal_store(u, static_cast<Raw*>(p));
+}
+// What a call streams through beyond this is not kept in the caches (the last-level one has 256 MB).
+constexpr size_t kCacheBytes = 256u << 20;
+
 // The sticky device word that hsl_device_errors reads, for a kernel's argument (recurrent.hip).
 // Bit 1: an id beyond the vocabulary (bit 0 is the persistent kernels').
 int device_error_word(unsigned** word);

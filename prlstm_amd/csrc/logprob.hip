@@ -55,6 +55,7 @@ __device__ __forceinline__ unsigned long long wave_max(unsigned long long v) {
 }
 
 // 16 bytes of a row at any element's alignment (global memory takes unaligned accesses).
+// NT: non-temporal, for rows that no cache holds until their next use.
 template <int F>
 struct Vec {
   static constexpr int N = 16 / sizeof(typename Elem<F>::T);
@@ -65,6 +66,13 @@ __device__ __forceinline__ Vec<F> load_vec(const typename Elem<F>::T* p) {
   Vec<F> r;
   __builtin_memcpy(&r, p, sizeof(r));
   return r;
+}
+template <int F, bool NT>
+__device__ __forceinline__ void store_vec(typename Elem<F>::T* p, const Vec<F>& x) {
+  if constexpr (NT)
+    store16_nt(p, x);
+  else
+    __builtin_memcpy(p, &x, sizeof(x));
 }
 // Vector i of a row of V elements, the part beyond the row masked.
 template <int F>
@@ -459,15 +467,18 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename E
 }
 
 // dx = -p (S + dH (log p + H)) for the vectors of one part of a row; then the elements with a
-// gradient of their own, the token and the alternatives, are computed again with it.
-template <int F, bool ENT>
+// gradient of their own, the token and the alternatives, are computed again with it.  Rows are taken
+// from the last to the first: the forward has just read the last ones, and a cache may still hold
+// them.  Where logits and gradient exceed the caches the gradient is stored past them, so that it
+// does not drive those rows out (both steps at 8192 x 32768 bf16, forward and backward: 294 -> 262 us).
+template <int F, bool ENT, bool NT>
 __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
     const typename Elem<F>::T* __restrict__ logits, long long ld, const void* __restrict__ tokens, int tok64,
     const long long* __restrict__ top_ids, const float* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ dlogp, const float* __restrict__ dent, const float* __restrict__ dtop,
     typename Elem<F>::T* __restrict__ dlogits, long long ldd, int V, int top) {
   constexpr int N = Vec<F>::N;
-  const size_t n = blockIdx.y;
+  const size_t n = gridDim.y - 1 - blockIdx.y;
   const auto* const row = logits + (long long)n * ld;
   auto* const drow = dlogits + (long long)n * ldd;
   const int nvec = (int)(((long long)V + N - 1) / N), first = blockIdx.x * kBwdVecs * kThreads;
@@ -505,7 +516,7 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
     down_all<F, N>(g, x[k].v);
     auto* const out = drow + (size_t)i * N;
     if (i * N + N <= V) {
-      __builtin_memcpy(out, &x[k], sizeof(x[k]));
+      store_vec<F, NT>(out, x[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < N; ++e)
@@ -645,20 +656,23 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
   return with_fmt(fmt, [&](auto f) {
     constexpr int kF = decltype(f)::value;
     using T = typename Elem<kF>::T;
-    for (long long n0 = 0; n0 < N; n0 += 65535) {
+    const bool nt = (size_t)N * V * sizeof(T) * 2 > kCacheBytes;
+    for (long long n0 = (N - 1) / 65535 * 65535; n0 >= 0; n0 -= 65535) {
       const unsigned rows = (unsigned)std::min<long long>(N - n0, 65535);
-      auto run = [&](auto e) {
-        hipLaunchKernelGGL((logprob_bwd_kernel<kF, decltype(e)::value>), dim3((nvec + part - 1) / part, rows),
+      auto run = [&](auto e, auto past) {
+        hipLaunchKernelGGL((logprob_bwd_kernel<kF, decltype(e)::value, decltype(past)::value>), dim3((nvec + part - 1) / part, rows),
                            dim3(kThreads), 0, s, static_cast<const T*>(logits) + n0 * ld, ld,
                            tokens ? static_cast<const char*>(tokens) + n0 * (tok64 ? 8 : 4) : nullptr, tok64,
                            top_ids ? top_ids + n0 * top : nullptr, stats + 2 * n0, entropy ? entropy + n0 : nullptr,
                            dlogp ? dlogp + n0 : nullptr, dent ? dent + n0 : nullptr, dtop ? dtop + n0 * top : nullptr,
                            static_cast<T*>(dlogits) + n0 * ldd, ldd, V, top);
       };
+      using Yes = std::true_type;
+      using No = std::false_type;
       if (dent)
-        run(std::true_type{});
+        nt ? run(Yes{}, Yes{}) : run(Yes{}, No{});
       else
-        run(std::false_type{});
+        nt ? run(No{}, Yes{}) : run(No{}, No{});
       HSL_HIP(hipGetLastError());
     }
     return (int)HSL_OK;
