@@ -544,6 +544,101 @@ def test_logprobs_strides_and_shapes(dev):
     assert torch.equal(many.logp, r.logp[0, 0].expand(5))
 
 
+# ---- sizes beyond the caches, offsets beyond 32 bits ----------------------------------------
+
+
+def test_embedding_beyond_the_caches(dev):
+    g = torch.Generator(device=dev).manual_seed(1)
+    N, V, D = 66000, 70001, 1024
+    ids = (torch.rand(N, device=dev, generator=g) ** 3 * V).int().clamp_max(V - 1)
+    w = torch.randn(V, D, device=dev, generator=g).bfloat16().requires_grad_(True)
+    dout = torch.randn(N, D, device=dev, generator=g).bfloat16()
+    out = prlstm_amd.embedding(ids, w, 3.0)
+    assert torch.equal(out.detach(), (w.detach()[ids].float() * 3.0).bfloat16())
+    dw, = torch.autograd.grad(out, w, dout)
+    at = ids.long()
+    want = torch.zeros(V, D, dtype=torch.float64, device=dev).index_add_(0, at, dout.double()) * 3.0
+    mag = torch.zeros(V, D, dtype=torch.float64, device=dev).index_add_(0, at, dout.double().abs()) * 3.0
+    count = torch.bincount(at, minlength=V)[:, None].double()
+    bound = (count + 2) * u * mag + HALF[torch.bfloat16] * 1.01 * want.abs() + 1e-38
+    assert bool(((dw.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype,T", [(torch.bfloat16, 2900), (torch.float32, 1500)])
+def test_gated_beyond_the_caches(dev, dtype, T):
+    g = torch.Generator(device=dev).manual_seed(2)
+    B, H = 16, 1024
+    zv = torch.randn(T, B, 2 * H, device=dev, generator=g)
+    zv[..., :H] += 2.0
+    zv = zv.to(dtype).requires_grad_(True)
+    dout = torch.randn(T, B, H, device=dev, generator=g).to(dtype)
+    reset = torch.rand(T, B, device=dev, generator=g) < 0.01
+    for r in (None, reset):
+        out, h_n = prlstm_amd.gated_recurrence(zv, None, r)
+        dzv, = torch.autograd.grad(out, zv, dout)
+        pick = torch.randint(0, H, (40,), device=dev, generator=g)  # some channels, in 64 bits
+        part = torch.cat((zv.detach()[..., pick], zv.detach()[..., H + pick]), -1)
+        want = _gated_plain(part.cpu(), None, None if r is None else r.cpu(), dout[..., pick].cpu(), torch.zeros(B, 40))
+        _check_gated("out", out[..., pick], want["out"], dtype)
+        _check_gated("h_n", h_n[..., pick], want["h_n"], dtype)
+        _check_gated("dzv", torch.cat((dzv[..., pick], dzv[..., H + pick]), -1), want["dzv"], dtype)
+
+
+def test_logprobs_beyond_the_caches(dev):
+    """Sampled rows against 64 bits; every row's gradient sums to its own part."""
+    g = torch.Generator().manual_seed(3)
+    N, V = 4100, 17001
+    gd = torch.Generator(device=dev).manual_seed(3)
+    x = (3 * torch.randn(N, V, device=dev, generator=gd)).bfloat16().requires_grad_(True)
+    tokens = torch.randint(0, V, (N,), generator=g)
+    dlogp, dent = torch.randn(N, generator=g), torch.randn(N, generator=g)
+    dtop = torch.randn(N, 3, generator=g)
+    r = prlstm_amd.token_logprobs(x, tokens.to(dev), top=3)
+    for ent in (False, True):
+        outs = [r.logp, r.top_logp] + ([r.entropy] if ent else [])
+        gs = [dlogp.to(dev), dtop.to(dev)] + ([dent.to(dev)] if ent else [])
+        dx, = torch.autograd.grad(outs, x, gs, retain_graph=True)
+        rows = torch.cat((torch.arange(3), torch.randint(0, N, (20,), generator=g), torch.tensor([N - 1])))
+        want = _logprob_plain(x.detach()[rows].cpu(), tokens[rows], 3, dlogp[rows], dent[rows] * ent, dtop[rows])
+        for k in ("logp", "entropy", "top_logp"):
+            _within(k, getattr(r, k)[rows], *want[k])
+        assert torch.equal(r.top_ids[rows].cpu(), want["top_ids"])
+        exact, bound = want["dlogits"]
+        _within("dlogits", dx[rows], exact, bound + HALF[torch.bfloat16] * 1.01 * exact.abs() + 1e-38)
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Rows, steps and batch rows that lie more than 2^32 bytes apart."""
+    g = _gen("far")
+    far = (1 << 31) + 6  # elements
+    buf = torch.empty(2 * far + 4096, dtype=torch.bfloat16, device=dev)
+
+    def place(t):  # [3, n] at rows `far` apart
+        v = buf.as_strided((3, t.shape[1]), (far, 1))
+        v.copy_(t)
+        return v
+
+    x = torch.randn(3, 2001, generator=g).bfloat16()
+    tokens = torch.tensor([5, 2000, 17])
+    v = place(x)
+    near = prlstm_amd.token_logprobs(x.to(dev), tokens.to(dev), top=4)
+    for a, b in zip(prlstm_amd.token_logprobs(v, tokens.to(dev), top=4), near):
+        assert torch.equal(a, b)
+    ids = torch.tensor([2, 0, 1, 2], device=dev)
+    assert torch.equal(prlstm_amd.embedding(ids, v, 2.0), prlstm_amd.embedding(ids, x.to(dev), 2.0))
+    zv = torch.randn(3, 200, generator=g).bfloat16()
+    v = place(zv)
+    dense = zv.to(dev)
+    for a, b in ((v[:, None], dense[:, None]), (v[None], dense[None])):  # far steps, far batch rows
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        oa, ha = prlstm_amd.gated_recurrence(a)
+        ob, hb = prlstm_amd.gated_recurrence(b)
+        assert torch.equal(oa, ob) and torch.equal(ha, hb)
+        ga, = torch.autograd.grad(oa, a, torch.ones_like(oa))
+        gb, = torch.autograd.grad(ob, b, torch.ones_like(ob))
+        assert torch.equal(ga, gb)
+
+
 # ---- gradients against differences ---------------------------------------------------------
 
 
