@@ -13,6 +13,7 @@ Operands that do not fit raise ``RuntimeError``; CPU tensors are rejected.  The 
 differentiable themselves.
 """
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -25,15 +26,38 @@ _IDS = (torch.int64, torch.int32)
 MAX_TOP = 32  # alternatives of a row that token_logprobs gives at most
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_lib.load(), name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _size(name, *args):
+    """A size query of the library (they depend on nothing but their arguments)."""
+    return _entry(name)(*args)
+
+
 def _launch(device, name, *args):
     """The C entry point on the device's current stream, with that device current.  (The raw handle:
     a Stream object takes 3 us of the host, most of a small call.)"""
     index = device.index
-    if index == torch.cuda.current_device():
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+            return _launch(device, name, *args)
+    if _entry(name)(*args, torch._C._cuda_getCurrentRawStream(index)):
+        raise RuntimeError(f"{name} failed: {_lib.load().hsl_last_error().decode(errors='replace')}")
+
+
+def _first_order(backward):
+    """``once_differentiable``, whose wrapping costs a small step some microseconds, only where a
+    graph of the gradient is asked for."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def _fmt(name, t):
@@ -76,7 +100,7 @@ def _embed_check(ids, weight, padding_idx):
 
 def _embed_fwd(ids, weight, scale, fmt, ids64):
     v, d = weight.shape
-    out = weight.new_empty(*ids.shape, d)
+    out = weight.new_empty((*ids.shape, d))
     _launch(weight.device, "hsl_embed_fwd", ids.data_ptr(), ids64, weight.data_ptr(), weight.stride(0), scale,
             out.data_ptr(), ids.numel(), v, d, fmt)
     return out
@@ -91,16 +115,16 @@ class EmbeddingFn(torch.autograd.Function):
         return _embed_fwd(ids, weight, scale, fmt, ids64)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         if dout is None:
             return (None,) * 6
         ids, = ctx.saved_tensors
         (v, d), scale, padding, fmt, ids64 = ctx.meta
         n = ids.numel()
-        dout = _unit_inner(dout.reshape(n, d))
-        dw = dout.new_empty(v, d)
-        nbytes = _lib.load().hsl_embed_bwd_ws_bytes(n, v, d)
+        dout = _unit_inner(dout if dout.dim() == 2 else dout.reshape(n, d))
+        dw = dout.new_empty((v, d))
+        nbytes = _size("hsl_embed_bwd_ws_bytes", n, v, d)
         ws = _ws(nbytes, dw)
         _launch(dw.device, "hsl_embed_bwd", ids.data_ptr(), ids64, dout.data_ptr(), dout.stride(0), scale, padding,
                 dw.data_ptr(), _lib.ptr(ws), nbytes, n, v, d, fmt)
@@ -117,7 +141,7 @@ def embedding(ids, weight, scale=1.0, padding_idx: Optional[int] = None):
     """
     fmt, ids64 = _embed_check(ids, weight, padding_idx)
     ids, weight = ids.contiguous(), _unit_inner(weight)
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if weight.requires_grad and torch.is_grad_enabled():
         return EmbeddingFn.apply(ids, weight, float(scale), padding_idx, fmt, ids64)
     return _embed_fwd(ids, weight, float(scale), fmt, ids64)
 
@@ -159,9 +183,8 @@ def _gated_fwd(zv, h0, reset, fmt, keep):
     out = _like_order(zv, t, b, h)
     f32 = dict(dtype=torch.float32, device=zv.device)
     h_n = torch.empty(b, h, **f32)
-    lib = _lib.load()
-    ck = torch.empty(lib.hsl_gated_ck_rows(t), b, h, **f32) if keep else None
-    nbytes = lib.hsl_gated_ws_bytes(t, b, h)
+    ck = torch.empty(_size("hsl_gated_ck_rows", t), b, h, **f32) if keep else None
+    nbytes = _size("hsl_gated_ws_bytes", t, b, h)
     ws = _ws(nbytes, zv)
     rp, rt, rb = (None, 0, 0) if reset is None else (reset.data_ptr(), *reset.stride())
     _launch(zv.device, "hsl_gated_fwd", zv.data_ptr(), zv.stride(0), zv.stride(1), _lib.ptr(h0), rp, rt, rb,
@@ -180,7 +203,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
         return out, h_n
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout, dh_n):
         zv, reset, ck = ctx.saved_tensors
         if dout is None and dh_n is None:
@@ -191,7 +214,7 @@ class GatedRecurrenceFn(torch.autograd.Function):
         dh_n = None if dh_n is None else dh_n.contiguous()
         dzv = _like_order(zv, t, b, n)
         dh0 = torch.empty(b, h, dtype=torch.float32, device=zv.device) if ctx.needs_input_grad[1] else None
-        nbytes = _lib.load().hsl_gated_ws_bytes(t, b, h)
+        nbytes = _size("hsl_gated_ws_bytes", t, b, h)
         ws = _ws(nbytes, zv)
         rp, rt, rb = (None, 0, 0) if reset is None else (reset.data_ptr(), *reset.stride())
         dp, dt, db = (None, 0, 0) if dout is None else (dout.data_ptr(), dout.stride(0), dout.stride(1))
@@ -261,7 +284,7 @@ def _logprob_fwd(x, tokens, top, fmt, ids64):
     entropy, stats = torch.empty(n, **f32), torch.empty(n, 2, **f32)
     top_logp = torch.empty(n, top, **f32) if top else None
     top_ids = torch.empty(n, top, dtype=torch.int64, device=x.device) if top else None
-    nbytes = _lib.load().hsl_logprob_fwd_ws_bytes(n, v, top)
+    nbytes = _size("hsl_logprob_fwd_ws_bytes", n, v, top)
     ws = _ws(nbytes, x)
     P = _lib.ptr
     _launch(x.device, "hsl_logprob_fwd", x.data_ptr(), x.stride(0), P(tokens), ids64, P(logp), entropy.data_ptr(),
@@ -281,7 +304,7 @@ class TokenLogprobsFn(torch.autograd.Function):
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dlogp, dent, dtop, _):
         x, tokens, top_ids, stats, entropy = ctx.saved_tensors
         top, fmt, ids64 = ctx.meta
