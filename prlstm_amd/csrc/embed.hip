@@ -89,6 +89,8 @@ __device__ __forceinline__ long long row_at(const Rows& r, unsigned block, unsig
   return ((long long)k * blocks + block) * (kBlock >> r.log2g) + (threadIdx.x >> r.log2g);
 }
 
+// The forward: a gather, bound by its rows' traffic; four rows a lane are in flight.  N65536 V131072
+// D1024 bf16: 33 us for 134 MB written (4.1 TB/s; the rows read are mostly in the caches).
 template <int F, bool SMALL>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const void* __restrict__ ids, int ids64,
                                                            const typename Elem<F>::T* __restrict__ w, long long ldw,
@@ -190,6 +192,9 @@ __device__ __forceinline__ void place_round(int q, int i, int bits, int* cnt, in
   if (rank == 0) cnt[q] = at + __popcll(same);  // every lane of the wave has read it
 }
 
+// The sort of one class.  Every workgroup reads all ids (from its XCD's L2) rather than exchange
+// anything with the others, so it is one launch; it is bound by the instructions of that look (65536
+// int32 ids: 24 us, of which the loads alone are 4; 8192: 9; 700: 6).
 template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const I* __restrict__ ids, int N, int V, int padding,
                                                                   Sorted s) {
@@ -318,6 +323,8 @@ __device__ __forceinline__ void sum_positions(const int* __restrict__ pos, int l
   }
 }
 
+// The sums, bound by dout read and dW written once: N65536 V131072 D1024 bf16 88 us for 403 MB (4.6
+// TB/s).  Three positions a lane are in flight: with eight the registers halve the waves (138 us).
 // The first blocks take a chunk of positions each round: its parts of the chunk's first and last
 // token, where those are long, go to partials 2 chunk and 2 chunk + 1 (rows of `pitch`).  The others
 // take the rows of dW that are not long.  NT: dout and dW exceed the caches, and dW is stored past them
@@ -370,7 +377,7 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const void* __restric
   }
 }
 
-// The long rows of class blockIdx.y, 64 columns: kJoinGroups shares of a row's partials, each added
+// The long rows of class blockIdx.y, 64 columns (7 us at the size above, 3 to 4 of them the launch): kJoinGroups shares of a row's partials, each added
 // in order, then the shares in order.
 template <int F>
 __global__ __launch_bounds__(kBlock) void embed_join_kernel(Sorted s, const float* __restrict__ partial, int pitch,

@@ -218,30 +218,31 @@ __device__ __forceinline__ bool finish_row(size_t n, const Sums& q, float ls, co
   return none;
 }
 
-// The alternatives of a row.  Each thread knows the largest element of one group of vectors, by
-// its value and its vector (key: 0 if the group is empty).  The k groups with the largest keys hold
-// the k largest elements: any other group's elements are all below those k.  So only these groups
-// are read again, for the elements at or above the k-th group's key, and those are ranked by
+// The alternatives of a row.  The vectors are in groups, of each of which the largest element is
+// known by its value and its vector (key: 0 if the group is empty).  The k groups with the largest
+// keys hold the k largest elements: any other group's elements are all below those k.  So only these
+// groups are read again, for the elements at or above the k-th group's key, and those are ranked by
 // counting.  Groups are GL lanes wide: group g has vectors (g / (n / GL)) * part + n i +
 // (g mod (n / GL)) * GL + 0 .. GL-1, n the threads.  A row of one workgroup has 64 groups, which one
-// wave ranks; with 256 of one lane the ranking took 2 us of the workgroup's time instead of 0.1,
-// more than the three vectors more that each lane reads again.
+// wave ranks; with 256 of one lane the ranking took 2 us of the workgroup's time instead of 0.1.
+// There each lane's own key (LANES) then says whether its part of a group has to be read: with 20
+// alternatives that is 9% of the row, not 31%.
 struct alignas(16) TopShared {
   unsigned long long key[kThreads];  // one for each group
   unsigned long long cand[kCandidates];
-  int group[kMaxTop];
+  int unit[kThreads];  // what is read again: groups, or lanes
   unsigned long long least;
   int count[kWaves];
-  int ncand;
+  int ncand, nunit;
 };
-template <int F, int W, int GL, int KEYS>
+template <int F, int W, int GL, int KEYS, bool LANES>
 __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, int top, int part, int nvec,
-                           unsigned long long key, float r, float ls, bool nan_row, bool none, size_t n, const Out& o,
+                           unsigned long long key, unsigned long long lane_key, float r, float ls, bool nan_row, bool none, size_t n, const Out& o,
                            TopShared& sh) {
-  constexpr int N = Vec<F>::N, kN = W * 64, kPer = kN / GL;
+  constexpr int N = Vec<F>::N, kN = W * 64;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (threadIdx.x < KEYS) sh.key[threadIdx.x] = key;
-  if (threadIdx.x == 0) sh.ncand = 0;
+  if (threadIdx.x == 0) sh.ncand = sh.nunit = 0;
   const int groups = min(__syncthreads_count(threadIdx.x < KEYS && key != 0), top);
   if (threadIdx.x < KEYS) {
     int rank = 0;
@@ -250,7 +251,7 @@ __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, i
       const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&sh.key[u]);
       rank += (k.x > key) + (k.y > key);
     }
-    if (rank < groups) sh.group[rank] = threadIdx.x;
+    if (!LANES && rank < groups) sh.unit[rank] = threadIdx.x;
     if (rank == groups - 1) {
       // the smallest key that an element of that group's vector with that value can have; with fewer
       // groups than asked for, every element is a candidate
@@ -260,22 +261,30 @@ __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, i
   }
   __syncthreads();
   const unsigned long long least = sh.least;
-  const int each = (part + kN - 1) / kN * GL;  // vectors of a group
+  if constexpr (LANES) {
+    // the largest key that an element of the lane's vectors can have
+    const unsigned long long most = (lane_key | 0xFFFFFFFFull) - (0xFFFFFFFFull - (lane_key & 0xFFFFFFFFull)) * N;
+    if (lane_key && most >= least) sh.unit[atomicAdd(&sh.nunit, 1)] = threadIdx.x;
+    __syncthreads();
+  }
+  constexpr int kUnit = LANES ? 1 : GL, kUnits = kN / kUnit;  // lanes of a unit, units of a round
+  const int units = LANES ? sh.nunit : groups;
+  const int each = (part + kN - 1) / kN * kUnit;  // vectors of a unit
   const float tau = least ? value_of((unsigned)(least >> 32)) : -__builtin_inff();
-  // the selected groups' elements at or above `from`, or above tau alone
+  // the units' elements at or above `from`, or above tau alone
   auto collect = [&](unsigned long long from, bool above_tau) {
     constexpr int kAhead = 4;  // loads in flight
-    for (int i0 = threadIdx.x; i0 < groups * each; i0 += kAhead * kN) {
+    for (int i0 = threadIdx.x; i0 < units * each; i0 += kAhead * kN) {
       Vec<F> x[kAhead];
       int vec[kAhead];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
         const int i = i0 + a * kN;
         vec[a] = nvec;
-        if (i < groups * each) {
-          const int g = sh.group[i / each], j = i % each;
-          const int at = (j / GL) * kN + (g % kPer) * GL + j % GL;
-          if (at < part) vec[a] = min((g / kPer) * part + at, nvec);
+        if (i < units * each) {
+          const int g = sh.unit[i / each], j = i % each;
+          const int at = (j / kUnit) * kN + (g % kUnits) * kUnit + j % kUnit;
+          if (at < part) vec[a] = min((g / kUnits) * part + at, nvec);
         }
         if (vec[a] < nvec) x[a] = load_edge<F>(row, vec[a], V);
       }
@@ -383,7 +392,9 @@ __device__ __forceinline__ unsigned long long group_key(float best, int at) {
   return at == 0x7FFFFFFF ? 0 : key_of(best, at);
 }
 
-// One workgroup per row.
+// One workgroup per row, one pass: the running sums and each group's largest element.  Bound by HBM:
+// N8192 V32768 bf16 95 us for 537 MB (5.7 TB/s), with 20 alternatives 122.  A row of up to kShortRow
+// logits takes one wave, which needs no barriers (N8192 V1000 with 4: 22 us, 30 with four waves).
 template <int F, bool TOP, int W>
 __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                long long ld, const void* __restrict__ tokens,
@@ -402,7 +413,8 @@ __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem
     constexpr int GL = W > 1 ? kRowLanes : 1;  // 64 groups
     __shared__ TopShared sh;
     __shared__ unsigned long long keys[W * 64 / GL];
-    unsigned long long key = group_key(a.best, a.at);
+    const unsigned long long lane_key = group_key(a.best, a.at);
+    unsigned long long key = lane_key;
 #pragma unroll
     for (int d = 1; d < GL; d *= 2) {
       const unsigned long long other = __shfl_xor(key, d);
@@ -412,12 +424,14 @@ __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem
     if ((threadIdx.x & 63) < 64 / GL) keys[threadIdx.x / 64 * (64 / GL) + (threadIdx.x & 63)] = key;
     __syncthreads();
     key = threadIdx.x < W * 64 / GL ? keys[threadIdx.x] : 0;
-    choose_top<F, W, GL, W * 64 / GL>(row, V, top, nvec, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+    choose_top<F, W, GL, W * 64 / GL, (GL > 1)>(row, V, top, nvec, nvec, key, lane_key, q.r, ls, q.s != q.s, none, n, o,
+                                                sh);
   }
 }
 
-// Few rows: each is cut into parts of `part` vectors, whose sums and groups' keys go to ws.
-// GL: lanes of a group, as many as give at most kThreads groups.
+// Fewer than 512 rows leave CUs idle: each is cut into parts of `part` vectors, whose sums and groups'
+// keys go to ws, and a workgroup per row joins them (4 rows of 131072 bf16 with 20 alternatives: 4 and
+// 10 us, latency).  GL: lanes of a group, as many as give at most kThreads groups.
 template <int F, bool TOP, int GL>
 __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                 long long ld, Sums* __restrict__ sums,
@@ -462,10 +476,11 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const typename E
   const bool none = finish_row(n, q, ls, token, V, o, err);
   if constexpr (TOP) {
     __shared__ TopShared sh;
-    choose_top<F, kWaves, GL, kThreads>(row, V, top, part, nvec, key, q.r, ls, q.s != q.s, none, n, o, sh);
+    choose_top<F, kWaves, GL, kThreads, false>(row, V, top, part, nvec, key, 0, q.r, ls, q.s != q.s, none, n, o, sh);
   }
 }
 
+// Bound by HBM: N8192 V32768 bf16 164 us for 1074 MB (6.5 TB/s) behind the forward.
 // dx = -p (S + dH (log p + H)) for the vectors of one part of a row; then the elements with a
 // gradient of their own, the token and the alternatives, are computed again with it.  Rows are taken
 // from the last to the first: the forward has just read the last ones, and a cache may still hold
