@@ -90,7 +90,8 @@ __device__ __forceinline__ long long row_at(const Rows& r, unsigned block, unsig
 }
 
 // The forward: a gather, bound by its rows' traffic; four rows a lane are in flight.  N65536 V131072
-// D1024 bf16: 33 us for 134 MB written (4.1 TB/s; the rows read are mostly in the caches).
+// D1024 bf16: 33 us for 134 MB written (4.1 TB/s; the rows read are mostly in the caches),
+// 46 on average in training passes on inputs in turn (the cause of the difference is not measured).
 template <int F, bool SMALL>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const void* __restrict__ ids, int ids64,
                                                            const typename Elem<F>::T* __restrict__ w, long long ldw,

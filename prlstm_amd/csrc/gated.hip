@@ -245,7 +245,8 @@ __device__ __forceinline__ void enter_segment(const float2* __restrict__ maps, i
   }
 }
 
-// Forward.  Bound by HBM: T4096 B16 H1024 bf16 74 us for 419 MB (5.7 TB/s, a large copy has 5.1), fp32
+// Forward.  Bound by HBM: T4096 B16 H1024 bf16 74 us for 419 MB (5.7 TB/s, a large copy has 5.1; 83 on
+// average in training passes on inputs in turn), fp32
 // 150 us for 822 MB.  Two channels a lane make 128-byte (bf16) and 256-byte (fp32) rows of a group.
 template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, const float* h0, Stream reset,
@@ -417,7 +418,7 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv
 
 // Backward: the group's steps forward from the checkpoint (by way of the wave's first group for its
 // second), then the reverse map and, from the joined U, the gradients.  T4096 B16 H1024 bf16 136 us for
-// 688 MB (5.1 TB/s), fp32 228 us for 1359 MB (6.0).  A third or fourth chunk in flight changes nothing.
+// 688 MB (5.1 TB/s; 145 on average in training passes on inputs in turn), fp32 228 us for 1359 MB (6.0).  A third or fourth chunk in flight changes nothing.
 template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, Stream reset,
                                                                   const float* __restrict__ ck, Stream dout,

@@ -393,7 +393,7 @@ __device__ __forceinline__ unsigned long long group_key(float best, int at) {
 }
 
 // One workgroup per row, one pass: the running sums and each group's largest element.  Bound by HBM:
-// N8192 V32768 bf16 95 us for 537 MB (5.7 TB/s), with 20 alternatives 122.  A row of up to kShortRow
+// N8192 V32768 bf16 95 us for 537 MB (5.7 TB/s; 105 on average in training passes on inputs in turn), with 20 alternatives 122.  A row of up to kShortRow
 // logits takes one wave, which needs no barriers (N8192 V1000 with 4: 22 us, 30 with four waves).
 template <int F, bool TOP, int W>
 __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
