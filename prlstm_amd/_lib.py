@@ -152,21 +152,25 @@ def device_errors(device=None, clear=True):
     return flags.value
 
 
+# what each bit of the device word says
+_ERRORS = {
+    1: "a persistent recurrent kernel gave up a wait between workgroups (not all of its workgroups were resident "
+       "at once, or a wait exceeded the spin timeout); the outputs of that call are NaN",
+    2: "a token id was at or beyond the vocabulary of its embedding or logits; its row is NaN",
+}
+
+
 def check_errors(device=None):
     """Raise RuntimeError if a kernel of this library reported an error on the device
-    since the last check (and clear it).  A persistent kernel that gives up a wait
-    also leaves NaN in the outputs of that call, so the failure shows in the loss
-    even without this check; this names it."""
+    since the last check (and clear it), with every kind of error that it reported.  A
+    persistent kernel that gives up a wait also leaves NaN in the outputs of that call, so
+    the failure shows in the loss even without this check; this names it."""
     flags = device_errors(device, clear=True)
-    if flags & 2:
-        raise RuntimeError(
-            f"prlstm_amd: device error word {flags:#x}: a token id was at or beyond the vocabulary of its embedding "
-            "or logits; its row is NaN")
     if flags:
-        raise RuntimeError(
-            f"prlstm_amd: device error word {flags:#x}: a persistent recurrent kernel gave up a wait "
-            "between workgroups (not all of its workgroups were resident at once, or a wait exceeded "
-            "the spin timeout); the outputs of that call are NaN")
+        said = [text for bit, text in _ERRORS.items() if flags & bit]
+        if flags & ~sum(_ERRORS):
+            said.append("an unknown error")
+        raise RuntimeError(f"prlstm_amd: device error word {flags:#x}: {'; and '.join(said)}")
 
 
 def last_recurrent_path():
