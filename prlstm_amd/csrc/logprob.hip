@@ -23,6 +23,7 @@ constexpr int kMaxParts = 64;        // of a row
 constexpr int kFineParts = 16;       // up to which a part has groups of 16 lanes, not of 64
 constexpr int kBwdVecs = 2;          // vectors of a thread in the backward
 constexpr int kShortRow = 2048;      // logits of a row that one wave takes
+constexpr long long kLaunchRows = 1 << 23;  // workgroups of a launch: their threads stay below 2^32
 constexpr int kRowLanes = 4;         // of a group in a row of one workgroup
 constexpr int kCandidates = 2048;    // elements that may be ranked among a row's alternatives
 constexpr float kLog2e = 1.44269502162933349609375f;
@@ -628,12 +629,20 @@ int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int to
     const auto* x = static_cast<const typename Elem<kF>::T*>(logits);
     auto run = [&](auto t) {
       constexpr bool kTop = decltype(t)::value;
-      if (p.count == 1 && V <= kShortRow) {
-        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, 1>), dim3((unsigned)N), dim3(64), 0, s, x, ld, tokens, tok64, o,
-                           V, top, err);
-      } else if (p.count == 1) {
-        hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, kWaves>), dim3((unsigned)N), dim3(kThreads), 0, s, x, ld,
-                           tokens, tok64, o, V, top, err);
+      if (p.count == 1) {
+        for (long long n0 = 0; n0 < N; n0 += kLaunchRows) {
+          const dim3 rows((unsigned)std::min(N - n0, kLaunchRows));
+          const auto* const xn = x + n0 * ld;
+          const void* const tn = tokens ? static_cast<const char*>(tokens) + n0 * (tok64 ? 8 : 4) : nullptr;
+          const Out on{o.logp ? o.logp + n0 : nullptr, entropy + n0, stats + 2 * n0,
+                       top ? top_logp + n0 * top : nullptr, top ? top_ids + n0 * top : nullptr};
+          if (V <= kShortRow)
+            hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, 1>), rows, dim3(64), 0, s, xn, ld, tn, tok64, on, V, top,
+                               err);
+          else
+            hipLaunchKernelGGL((logprob_row_kernel<kF, kTop, kWaves>), rows, dim3(kThreads), 0, s, xn, ld, tn, tok64,
+                               on, V, top, err);
+        }
       } else {
         auto cut = [&](auto lanes) {
           constexpr int kGL = decltype(lanes)::value;
