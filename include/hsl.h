@@ -357,7 +357,7 @@ int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw,
 /* dweight[v] = scale * the sum of dout[n] over n with ids[n] = v, in a fixed order
  * (the same result every time): dense [V, D], rows without a position are zero.
  * dout has row stride ldd.  Ids outside 0..V-1 and padding_idx (negative: none) get
- * no gradient. */
+ * no gradient.  V is at most 2^30 and dweight less than 2^37 bytes. */
 size_t hsl_embed_bwd_ws_bytes(long long N, int V, int D);
 int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, float scale,
                   int padding_idx, void* dweight, void* ws, size_t ws_bytes,

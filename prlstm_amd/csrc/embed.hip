@@ -23,6 +23,7 @@ namespace {
 
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 constexpr int kClassTokens = 512;  // tokens of one workgroup at most (its counters: 16 waves of them)
+constexpr int kMostTokens = 1 << 30;  // of the gradient: the sort's threads stay below 2^32
 constexpr int kHits = 512;          // positions of a class that one wave lists in LDS
 constexpr int kBlock = 256;
 constexpr int kJoinLanes = 16, kJoinGroups = kBlock / kJoinLanes;  // 64 columns, 16 shares of the partials
@@ -80,6 +81,8 @@ Rows rows_of(long long n, int D, int vec) {
 // blocks * rows apart, so that the rows of frequent tokens, which are neighbours, go to different
 // waves.
 constexpr int kWaveRows = 4;
+// Workgroups of a launch in x at most: HIP keeps the threads there in 32 bits, and wraps beyond.
+constexpr unsigned kLaunchBlocks = (1u << 24) - 1;
 unsigned row_blocks(const Rows& r) {
   const long long a_block = (long long)(kBlock >> r.log2g) * kWaveRows;
   return (unsigned)((r.n + a_block - 1) / a_block);
@@ -206,7 +209,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const I* __res
   const int lane = threadIdx.x & 63, t = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cls = blockIdx.x, mask = (1 << s.log2c) - 1;
-  const int tokens = V > cls ? (V - cls + mask) >> s.log2c : 0;  // of this class
+  const int tokens = V > cls ? ((V - 1 - cls) >> s.log2c) + 1 : 0;  // of this class
   for (int u = 0; u < kSortWaves; ++u)
     if (t < tokens) cnt[u][t] = 0;
   if (t == 0) nlong = 0;
@@ -378,14 +381,14 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const void* __restric
   }
 }
 
-// The long rows of class blockIdx.y, 64 columns (7 us at the size above, 3 to 4 of them the launch): kJoinGroups shares of a row's partials, each added
+// The long rows of class blockIdx.x, 64 columns (7 us at the size above, 3 to 4 of them the launch): kJoinGroups shares of a row's partials, each added
 // in order, then the shares in order.
 template <int F>
 __global__ __launch_bounds__(kBlock) void embed_join_kernel(Sorted s, const float* __restrict__ partial, int pitch,
                                                             float scale, typename Elem<F>::T* __restrict__ dw, int D) {
   __shared__ float4 share[kJoinGroups][kJoinLanes];
-  const int cls = blockIdx.y, lane = threadIdx.x % kJoinLanes, g = threadIdx.x / kJoinLanes;
-  const int col = (blockIdx.x * kJoinLanes + lane) * 4;
+  const int cls = blockIdx.x, lane = threadIdx.x % kJoinLanes, g = threadIdx.x / kJoinLanes;
+  const int col = (blockIdx.y * kJoinLanes + lane) * 4;
   const int n = s.nlong[cls];
   for (int l = 0; l < n; ++l) {
     const int v = s.longs[(size_t)cls * s.most + l];
@@ -482,12 +485,16 @@ int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw,
   HSL_CHECK(device_error_word(&err));
   hipStream_t s = static_cast<hipStream_t>(stream);
   return with_fmt(fmt, [&](auto f) {
-    using T = typename Elem<decltype(f)::value>::T;
-    const Rows r = rows_of(N, D, Vec<decltype(f)::value>::N);
-    const auto kernel = D < Vec<decltype(f)::value>::N ? embed_fwd_kernel<decltype(f)::value, true>
-                                                       : embed_fwd_kernel<decltype(f)::value, false>;
-    hipLaunchKernelGGL(kernel, dim3(row_blocks(r), r.tiles()), dim3(kBlock), 0, s, ids, ids64,
-                       static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out), r, V, err);
+    constexpr int kF = decltype(f)::value;
+    using T = typename Elem<kF>::T;
+    const auto kernel = D < Vec<kF>::N ? embed_fwd_kernel<kF, true> : embed_fwd_kernel<kF, false>;
+    const long long most = (long long)kLaunchBlocks * (kBlock >> rows_of(N, D, Vec<kF>::N).log2g) * kWaveRows;
+    for (long long n0 = 0; n0 < N; n0 += most) {
+      const Rows r = rows_of(std::min(N - n0, most), D, Vec<kF>::N);
+      hipLaunchKernelGGL(kernel, dim3(row_blocks(r), r.tiles()), dim3(kBlock), 0, s,
+                         static_cast<const void*>(static_cast<const char*>(ids) + n0 * (ids64 ? 8 : 4)), ids64,
+                         static_cast<const T*>(weight), ldw, scale, static_cast<T*>(out) + n0 * D, r, V, err);
+    }
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;
   });
@@ -505,6 +512,11 @@ int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, f
   if (V == 0 || D == 0) return HSL_OK;
   if (!dweight || (N > 0 && (!ids || !dout))) return fail(HSL_ERR_ARG, "hsl_embed_bwd: null pointer");
   const EmbedPlan p = plan_embed(N, V, D);
+  const Rows all = rows_of(V, D, fmt == kElemF32 ? Vec<kElemF32>::N : Vec<kElemBf16>::N);
+  const int chunk_blocks = (p.nchunks + (kBlock >> all.log2g) - 1) / (kBlock >> all.log2g);
+  if (V > kMostTokens || row_blocks(all) + chunk_blocks > kLaunchBlocks)
+    return fail(HSL_ERR_UNSUPPORTED, "hsl_embed_bwd: V=%d D=%d are beyond one launch (V at most 2^30, dweight below 2^37 bytes)",
+                V, D);
   EmbedWs w;
   const size_t need = carve_embed(ws, ws_bytes, N, V, p, &w);
   if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_embed_bwd: workspace %zu bytes, need %zu", ws_bytes, need);
@@ -518,17 +530,15 @@ int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, f
   return with_fmt(fmt, [&](auto f) {
     constexpr int kF = decltype(f)::value;
     using T = typename Elem<kF>::T;
-    const Rows r = rows_of(V, D, Vec<kF>::N);
-    const int chunk_blocks = (p.nchunks + (kBlock >> r.log2g) - 1) / (kBlock >> r.log2g);
     const bool nt = (size_t)(N + V) * D * sizeof(T) > kCacheBytes;
     const auto sums = D < Vec<kF>::N ? embed_sum_kernel<kF, true, false>
                       : nt           ? embed_sum_kernel<kF, false, true>
                                      : embed_sum_kernel<kF, false, false>;
-    hipLaunchKernelGGL(sums, dim3(chunk_blocks + row_blocks(r), r.tiles()), dim3(kBlock), 0, s, ids, ids64, w.s,
-                       static_cast<const T*>(dout), ldd, scale, static_cast<T*>(dweight), w.partial, p.pitch, r,
+    hipLaunchKernelGGL(sums, dim3(chunk_blocks + row_blocks(all), all.tiles()), dim3(kBlock), 0, s, ids, ids64, w.s,
+                       static_cast<const T*>(dout), ldd, scale, static_cast<T*>(dweight), w.partial, p.pitch, all,
                        chunk_blocks);
     if (p.nchunks)
-      hipLaunchKernelGGL(embed_join_kernel<kF>, dim3((D + 4 * kJoinLanes - 1) / (4 * kJoinLanes), p.nclass),
+      hipLaunchKernelGGL(embed_join_kernel<kF>, dim3(p.nclass, (D + 4 * kJoinLanes - 1) / (4 * kJoinLanes)),
                          dim3(kBlock), 0, s, w.s, w.partial, p.pitch, scale, static_cast<T*>(dweight), D);
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;

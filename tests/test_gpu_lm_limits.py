@@ -26,3 +26,35 @@ def test_logprobs_of_more_rows_than_a_launch_has(dev, N, V):
     at = torch.arange(N, device=dev) % k
     assert torch.equal(r.entropy, few.entropy[at])
     assert torch.equal(r.top_ids[:, 0], few.top_ids[at, 0]) and torch.equal(r.top_logp[:, 0], few.top_logp[at, 0])
+
+
+def test_embedding_gradient_of_more_rows_than_a_grid_has_in_y(dev):
+    """33.6 million tokens: 131072 classes."""
+    V, D = (1 << 25) + 40000, 1
+    ids = torch.tensor([0, V - 1, 1 << 25, 5, V - 1, 65536 * 511, -1], device=dev)
+    # one token of more than a chunk of positions, in a class above 65535
+    ids = torch.cat((ids, torch.full((40,), 100000, device=dev)))
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    dout = torch.arange(1, len(ids) + 1, device=dev, dtype=torch.bfloat16)[:, None]
+    dw, = torch.autograd.grad(prlstm_amd.embedding(ids, w), w, dout)
+    want = torch.zeros(V, device=dev).index_add_(0, ids.clamp_min(0), dout[:, 0].float() * (ids >= 0))
+    assert torch.equal(dw[:, 0].float(), want.bfloat16().float())
+
+
+def test_embedding_of_more_rows_than_a_launch_has(dev):
+    """257 columns are 33 vectors, so a workgroup of 256 threads has 16 rows, and 2^28 rows are two
+    launches."""
+    N, D = (1 << 28) + 100, 257
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 170e9:
+        pytest.skip("needs 138 GB")
+    ids = torch.zeros(N, dtype=torch.int32, device=dev)
+    ids[-1], ids[-50], ids[5] = 2, -1, 1
+    w = torch.arange(3 * D, device=dev).reshape(3, D).remainder(256).bfloat16()
+    out = prlstm_amd.embedding(ids, w)
+    assert torch.equal(out[-1], w[2]) and torch.equal(out[5], w[1]) and not bool(out[-50].any())
+    out[-1] = out[5] = out[-50] = w[0]
+    for rows in out.split(1 << 24):
+        assert bool((rows == w[0]).all())
+    del out, rows
+    torch.cuda.empty_cache()

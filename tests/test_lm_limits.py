@@ -1,0 +1,21 @@
+"""The ends of the sizes that the language-model operators take, as the host refuses them (no GPU)."""
+
+from prlstm_amd import _lib
+
+UNSUPPORTED = 2
+
+
+def _refused(rc, text):
+    assert rc == UNSUPPORTED and text in _lib.load().hsl_last_error(), (rc, _lib.load().hsl_last_error())
+
+
+def test_embedding_gradients_beyond_one_launch_are_refused():
+    """The sort has 1024 threads for 512 tokens, the sums 256 for 16 kB of the gradient; a launch holds
+    fewer than 2^32 threads.  (The pointers are not looked at before the sizes.)"""
+    bwd = _lib.load().hsl_embed_bwd
+    for v, d, fmt in (((1 << 30) + 1, 1, 0), (1 << 28, 512, 0), (1 << 28, 264, 1), (1 << 28, 256, 2)):
+        _refused(bwd(1, 0, 1, d, 1.0, -1, 1, 1, 0, 8, v, d, fmt, None), b"beyond one launch")
+    # the last sizes that are taken get as far as the workspace
+    for v, d, fmt in ((1 << 30, 1, 0), ((1 << 28) - 64, 512, 0), (1 << 28, 256, 0)):
+        assert bwd(1, 0, 1, d, 1.0, -1, 1, 1, 0, 8, v, d, fmt, None) == 1
+        assert b"workspace 0 bytes" in _lib.load().hsl_last_error()
