@@ -10,13 +10,14 @@ Tensors are bf16, fp16 or fp32; states, statistics and log probabilities are fp3
 streams are.  Every call runs on the current HIP stream of its tensors' device, allocates only
 through torch's caching allocator and synchronises nothing, so it can be captured in a graph.
 Operands that do not fit raise ``RuntimeError``; CPU tensors are rejected.  The gradients are not
-differentiable themselves.
+differentiable themselves, and forward-mode derivatives are refused (``NotImplementedError``).
 """
 
 import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -48,6 +49,13 @@ def _launch(device, name, *args):
         raise RuntimeError(f"{name} failed: {_lib.load().hsl_last_error().decode(errors='replace')}")
 
 
+def _no_tangents(*tensors):
+    """The kernels compute no forward-mode derivative; a launch alone would pass on one of zero."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the operators of prlstm_amd.lm have no forward-mode derivatives")
+
+
 def _first_order(backward):
     """``once_differentiable``, whose wrapping costs a small step some microseconds, only where a
     graph of the gradient is asked for."""
@@ -55,6 +63,7 @@ def _first_order(backward):
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        _no_tangents(*grads)
         return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
@@ -93,6 +102,7 @@ def _embed_check(ids, weight, padding_idx):
     if weight.dim() != 2:
         raise RuntimeError(f"weight must be [V, D], got shape {tuple(weight.shape)}")
     fmt = _fmt("weight", weight)
+    _no_tangents(weight)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise RuntimeError(f"padding_idx {padding_idx} is not a row of weight {tuple(weight.shape)}")
     return fmt, _ids("ids", ids, weight.device)
@@ -161,6 +171,7 @@ def _gated_check(zv, h0, reset, dims):
     if zv.dim() != dims + 1 or zv.shape[-1] % 2:
         raise RuntimeError(f"zv must be [{', '.join(lead)}, 2H], got shape {tuple(zv.shape)}")
     fmt = _fmt("zv", zv)
+    _no_tangents(zv, h0)
     state = (zv.shape[-2], zv.shape[-1] // 2)
     if h0 is not None:
         if tuple(h0.shape) != state:
@@ -333,6 +344,7 @@ def token_logprobs(logits, tokens=None, top=0):
     if logits.dim() < 1:
         raise RuntimeError("logits must be [..., V]")
     fmt = _fmt("logits", logits)
+    _no_tangents(logits)
     lead, v = logits.shape[:-1], logits.shape[-1]
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, v):

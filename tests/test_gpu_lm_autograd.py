@@ -1,0 +1,45 @@
+"""What the language-model operators (prlstm_amd.lm) refuse or notice as torch's own operations do."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import prlstm_amd
+
+pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    """The operators have no forward-mode derivative: a tangent is an error, not a derivative of zero."""
+    ids = torch.zeros(3, dtype=torch.int64, device=dev)
+    zeros = lambda *s: torch.zeros(*s, device=dev)  # noqa: E731
+    with forward_ad.dual_level():
+        dual = lambda *s: forward_ad.make_dual(zeros(*s), torch.ones(*s, device=dev))  # noqa: E731
+        for call in (lambda: prlstm_amd.embedding(ids, dual(4, 6)),
+                     lambda: prlstm_amd.gated_recurrence(dual(5, 2, 8)),
+                     lambda: prlstm_amd.gated_recurrence(zeros(5, 2, 8), dual(2, 4)),
+                     lambda: prlstm_amd.gated_recurrence_step(dual(2, 8), zeros(2, 4)),
+                     lambda: prlstm_amd.gated_recurrence_step(zeros(2, 8), dual(2, 4)),
+                     lambda: prlstm_amd.token_logprobs(dual(3, 5), ids)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    call()
+        # without a tangent the calls are as ever
+        assert prlstm_amd.embedding(ids, zeros(4, 6)).shape == (3, 6)
+        assert prlstm_amd.gated_recurrence(zeros(5, 2, 8))[0].shape == (5, 2, 4)
+        assert prlstm_amd.gated_recurrence_step(zeros(2, 8), zeros(2, 4))[0].shape == (2, 4)
+        assert prlstm_amd.token_logprobs(zeros(3, 5), ids).logp.shape == (3,)
+
+
+def test_tangents_of_incoming_gradients_are_refused(dev):
+    ids = torch.zeros(3, dtype=torch.int64, device=dev)
+    w = torch.zeros(4, 6, device=dev, requires_grad=True)
+    zv = torch.zeros(5, 2, 8, device=dev, requires_grad=True)
+    x = torch.zeros(3, 5, device=dev, requires_grad=True)
+    for out, arg in ((prlstm_amd.embedding(ids, w), w), (prlstm_amd.gated_recurrence(zv)[0], zv),
+                     (prlstm_amd.gated_recurrence(zv)[1], zv), (prlstm_amd.token_logprobs(x, ids).logp, x),
+                     (prlstm_amd.token_logprobs(x).entropy, x)):
+        with forward_ad.dual_level():
+            g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(out, arg, g)
