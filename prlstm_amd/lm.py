@@ -98,6 +98,15 @@ def _ws(nbytes, like):
 # ---- embedding -----------------------------------------------------------------------------
 
 
+def _scale(scale):
+    if isinstance(scale, torch.Tensor):
+        _no_tangents(scale)
+        if scale.is_cuda or (scale.requires_grad and torch.is_grad_enabled()):
+            raise RuntimeError(f"scale must be a number (it has no gradient and is not read from the GPU), got a tensor "
+                               f"on {scale.device} with requires_grad={scale.requires_grad}")
+    return float(scale)
+
+
 def _embed_check(ids, weight, padding_idx):
     if weight.dim() != 2:
         raise RuntimeError(f"weight must be [V, D], got shape {tuple(weight.shape)}")
@@ -147,13 +156,13 @@ def embedding(ids, weight, scale=1.0, padding_idx: Optional[int] = None):
     A negative id is a position without a token: a row of zeros, no gradient.  An id at or beyond V
     gives a row of NaN and raises the device word that ``prlstm_amd.check_errors`` reports.  The
     gradient of weight is dense and sums each row's positions in fp32 in a fixed order;
-    ``padding_idx`` is a row that gets none.
+    ``padding_idx`` is a row that gets none.  scale is a number and has no gradient.
     """
     fmt, ids64 = _embed_check(ids, weight, padding_idx)
-    ids, weight = ids.contiguous(), _unit_inner(weight)
+    ids, weight, scale = ids.contiguous(), _unit_inner(weight), _scale(scale)
     if weight.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFn.apply(ids, weight, float(scale), padding_idx, fmt, ids64)
-    return _embed_fwd(ids, weight, float(scale), fmt, ids64)
+        return EmbeddingFn.apply(ids, weight, scale, padding_idx, fmt, ids64)
+    return _embed_fwd(ids, weight, scale, fmt, ids64)
 
 
 # ---- gated recurrence ----------------------------------------------------------------------

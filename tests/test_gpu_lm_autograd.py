@@ -43,3 +43,20 @@ def test_tangents_of_incoming_gradients_are_refused(dev):
             g = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(out, arg, g)
+
+
+def test_scale_that_is_a_tensor(dev):
+    """The scale has no gradient and is not fetched from the device: a tensor that asks for either
+    is refused; a number of another kind is one."""
+    ids, w = torch.zeros(3, dtype=torch.int64, device=dev), torch.ones(4, 6, device=dev)
+    for scale in (torch.tensor(2.0, requires_grad=True), torch.tensor(2.0, device=dev, requires_grad=True),
+                  torch.tensor(2.0, device=dev)):
+        with pytest.raises(RuntimeError, match="scale must be a number"):
+            prlstm_amd.embedding(ids, w, scale)
+    for scale in (2, 2.0, torch.tensor(2.0), torch.tensor(2)):
+        assert torch.equal(prlstm_amd.embedding(ids, w, scale), torch.full((3, 6), 2.0, device=dev))
+    with torch.no_grad():
+        out = prlstm_amd.embedding(ids, w, torch.nn.Parameter(torch.tensor(2.0)))
+        assert torch.equal(out, torch.full((3, 6), 2.0, device=dev))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        prlstm_amd.embedding(ids, w, forward_ad.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
