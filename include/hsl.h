@@ -130,13 +130,16 @@ int hsl_poll_error(const void* ws, int* flag, void* stream);
  * stream the failing call used.  Bit 0: a persistent kernel gave up a wait
  * between workgroups (hsl_set_spin_timeout_us).  Bit 1: a token id was at or beyond
  * its vocabulary (hsl_embed_fwd, hsl_logprob_fwd).  Waits for `stream`, stores the
- * word in *flags and, when clear != 0, resets it.  An aborted wait is never
+ * word in *flags and, when clear != 0, resets the bits that it stored (one raised on
+ * another stream meanwhile stays).  An aborted wait is never
  * silent: the aborting workgroups also fill every output they own with NaN
  * (forward: their rows of h_save, c_save, gact, tanh_c; backward: their dW
  * planes, bias partials, dgates and dh0/dc0), so the results of the call are NaN.
  * Counterpart of the reference's loud failures (TORCH_CHECK at
  * _csrc/lstm_cell.cpp:38-43, RuntimeError at _metal.py:85-87). */
 int hsl_device_errors(int* flags, int clear, void* stream);
+/* Resets these bits of the word alone, and waits for `stream`. */
+int hsl_clear_device_errors(int bits, void* stream);
 /* Test hook (no reference counterpart): y[i] = f(x[i]) for n fp32 values with
  * the device math of the kernels, fn 0 = exp, 1 = sigmoid, 2 = tanh, and
  * fn 3 = sigmoid(x[i]) sigmoid(x[n-1-i]) as the scans form i*g (the reference

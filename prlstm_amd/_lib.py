@@ -35,6 +35,7 @@ SIGNATURES = {
     "hsl_set_split_products": (_I, [_I]),
     "hsl_poll_error": (_I, [_P, _P, _P]),
     "hsl_device_errors": (_I, [_P, _I, _P]),
+    "hsl_clear_device_errors": (_I, [_I, _P]),
     "hsl_eval_math": (_I, [_I, _P, _P, _Z, _P]),
     "hsl_set_timing": (_I, [_I]),
     "hsl_timing_collect": (_I, [_I, _P, _P]),
@@ -152,10 +153,17 @@ def device_errors(device=None, clear=True):
     return flags.value
 
 
+def clear_device_errors(bits, device=None):
+    """Resets these bits of the device word and no others."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    call("hsl_clear_device_errors", bits, stream_of(dev))
+
+
+GAVE_UP = 1  # the bit of an abandoned wait
 # what each bit of the device word says
 _ERRORS = {
-    1: "a persistent recurrent kernel gave up a wait between workgroups (not all of its workgroups were resident "
-       "at once, or a wait exceeded the spin timeout); the outputs of that call are NaN",
+    GAVE_UP: "a persistent recurrent kernel gave up a wait between workgroups (not all of its workgroups were "
+             "resident at once, or a wait exceeded the spin timeout); the outputs of that call are NaN",
     2: "a token id was at or beyond the vocabulary of its embedding or logits; its row is NaN",
 }
 

@@ -2805,7 +2805,7 @@ int device_error_word(unsigned** word) {
 }
 
 namespace {
-__global__ void clear_device_errors_kernel() { g_device_errors = 0u; }
+__global__ void clear_device_errors_kernel(unsigned bits) { atomicAnd(&g_device_errors, ~bits); }
 
 // ---- the allocation-free forward (hsl_rec_fwd_noalloc) ----------------------------
 // Its workspace is `scratch`, a static device array: each device that loads the library
@@ -2992,12 +2992,17 @@ int hsl_device_errors(int* flags, int clear, void* stream) {
   unsigned v = 0;
   HSL_HIP(hipMemcpyFromSymbolAsync(&v, HIP_SYMBOL(g_device_errors), sizeof(v), 0, hipMemcpyDeviceToHost, s));
   HSL_HIP(hipStreamSynchronize(s));
-  if (clear && v) {
-    hipLaunchKernelGGL(clear_device_errors_kernel, dim3(1), dim3(1), 0, s);
-    HSL_HIP(hipGetLastError());
-    HSL_HIP(hipStreamSynchronize(s));
-  }
+  // what another stream raises meanwhile stays
+  if (clear && v) HSL_CHECK(hsl_clear_device_errors(static_cast<int>(v), stream));
   *flags = static_cast<int>(v);
+  return HSL_OK;
+}
+
+int hsl_clear_device_errors(int bits, void* stream) {
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(clear_device_errors_kernel, dim3(1), dim3(1), 0, s, static_cast<unsigned>(bits));
+  HSL_HIP(hipGetLastError());
+  HSL_HIP(hipStreamSynchronize(s));
   return HSL_OK;
 }
 

@@ -34,7 +34,7 @@ def _poll(ws, device):
     flag = ctypes.c_int(0)
     _lib.call("hsl_poll_error", _lib.ptr(ws), ctypes.byref(flag), _lib.stream_of(device))
     if flag.value:
-        _lib.device_errors(device, clear=True)
+        _lib.clear_device_errors(_lib.GAVE_UP, device)  # this one; others are not this call's to report
         raise RuntimeError(f"a persistent kernel reported device error flag {flag.value} "
                            "(a wait between workgroups timed out); its outputs are NaN")
 
