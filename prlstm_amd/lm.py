@@ -169,10 +169,11 @@ def embedding(ids, weight, scale=1.0, padding_idx: Optional[int] = None):
 
 
 def _like_order(zv, t, b, n):
-    """An empty [t, b, n] whose outer of time and batch in memory is zv's."""
+    """An empty [t, b, n] whose outer of time and batch in memory is zv's.  (No view of another tensor:
+    torch allows no change in place to a view that a Function returns.)"""
     if zv.stride(0) >= zv.stride(1):
         return zv.new_empty(t, b, n)
-    return zv.new_empty(b, t, n).transpose(0, 1)
+    return zv.new_empty_strided((t, b, n), (n, t * n, 1))
 
 
 def _gated_check(zv, h0, reset, dims):

@@ -60,3 +60,20 @@ def test_scale_that_is_a_tensor(dev):
         assert torch.equal(out, torch.full((3, 6), 2.0, device=dev))
     with forward_ad.dual_level(), pytest.raises(NotImplementedError):
         prlstm_amd.embedding(ids, w, forward_ad.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
+
+
+@pytest.mark.parametrize("order", ["time", "batch"])
+def test_output_changed_in_place(dev, order):
+    """A residual added to the output in place, in either order of time and batch."""
+    g = torch.Generator().manual_seed(0)
+    zv = torch.randn(6, 3, 10, generator=g).to(dev)
+    if order == "batch":
+        zv = zv.transpose(0, 1).contiguous().transpose(0, 1)
+    dout = torch.randn(6, 3, 5, generator=g).to(dev)
+    a, b = (zv.clone(memory_format=torch.preserve_format).requires_grad_(True) for _ in range(2))
+    out, _ = prlstm_amd.gated_recurrence(a)
+    assert (out.stride(0) > out.stride(1)) == (order == "time")
+    out += a[..., 5:]
+    want = prlstm_amd.gated_recurrence(b)[0] + b[..., 5:]
+    assert torch.equal(out, want)
+    assert torch.equal(*(torch.autograd.grad(o, x, dout)[0] for o, x in ((out, a), (want, b))))
