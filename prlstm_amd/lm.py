@@ -19,6 +19,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -277,11 +278,14 @@ def gated_recurrence_step(zv, h, reset=None, h_out=None):
                                f"{tuple(t.shape)} on {t.device}")
     zv = _unit_inner(zv)
     out = zv.new_empty(state)
-    if h_out is None:
+    given = h_out is not None
+    if not given:
         h_out = torch.empty(state, dtype=torch.float32, device=zv.device)
     rp, rb = (None, 0) if reset is None else (reset.data_ptr(), reset.stride(0))
     _launch(zv.device, "hsl_gated_fwd", zv.data_ptr(), 0, zv.stride(0), _lib.ptr(h), rp, 0, rb, out.data_ptr(), 0,
             n // 2, h_out.data_ptr(), None, None, 0, 1, b, n // 2, fmt)
+    if given:
+        increment_version(h_out)  # for a backward pass that has saved it
     return out, h_out
 
 

@@ -77,3 +77,19 @@ def test_output_changed_in_place(dev, order):
     want = prlstm_amd.gated_recurrence(b)[0] + b[..., 5:]
     assert torch.equal(out, want)
     assert torch.equal(*(torch.autograd.grad(o, x, dout)[0] for o, x in ((out, a), (want, b))))
+
+
+def test_state_updated_in_place_is_noticed(dev):
+    """A state that a backward pass needs and a step has overwritten is an error there."""
+    w = torch.ones(2, 4, device=dev, requires_grad=True)
+    h = torch.ones(2, 4, device=dev)
+    y = (w * h).sum()
+    version = h._version
+    prlstm_amd.gated_recurrence_step(torch.zeros(2, 8, device=dev), h, h_out=h)
+    assert h._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # whose tensors have no version
+        h = torch.zeros(2, 4, device=dev)
+        _, h2 = prlstm_amd.gated_recurrence_step(torch.zeros(2, 8, device=dev), h, h_out=h)
+        assert h2 is h
