@@ -501,7 +501,7 @@ int hsl_embed_fwd(const void* ids, int ids64, const void* weight, long long ldw,
 }
 
 size_t hsl_embed_bwd_ws_bytes(long long N, int V, int D) {
-  if (N < 0 || V < 0 || D < 0) return 0;
+  if (check_embed("hsl_embed_bwd_ws_bytes", N, V, D, D, kElemF32) != HSL_OK) return 0;
   EmbedWs w;
   return carve_embed(nullptr, 0, N, V, plan_embed(N, V, D), &w);
 }

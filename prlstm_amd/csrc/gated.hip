@@ -725,8 +725,7 @@ extern "C" {
 int hsl_gated_ck_rows(int T) { return T <= 0 ? 0 : (T + kCkSteps - 1) / kCkSteps; }
 
 size_t hsl_gated_ws_bytes(int T, int B, int H) {
-  if (T < 0 || B < 0 || H < 0) return 0;
-  if (B == 0 || H == 0) return 0;
+  if (check_gated("hsl_gated_ws_bytes", T, B, H, kElemF32) != HSL_OK || B == 0 || H == 0) return 0;
   return (size_t)(plan_gated(T, B, H, std::min(H, 2)).nseg - 1) * B * H * sizeof(float2);
 }
 

@@ -19,3 +19,17 @@ def test_embedding_gradients_beyond_one_launch_are_refused():
     for v, d, fmt in ((1 << 30, 1, 0), ((1 << 28) - 64, 512, 0), (1 << 28, 256, 0)):
         assert bwd(1, 0, 1, d, 1.0, -1, 1, 1, 0, 8, v, d, fmt, None) == 1
         assert b"workspace 0 bytes" in _lib.load().hsl_last_error()
+
+
+def test_size_queries_of_refused_sizes():
+    """They end, and say 0, whatever they are asked."""
+    lib = _lib.load()
+    most = (1 << 63) - 1
+    for n in (0x7FFF0001, 1 << 43, 1 << 60, most):
+        assert lib.hsl_embed_bwd_ws_bytes(n, 5, 5) == 0
+    for t, b, h in ((4096, 1 << 20, 1 << 18), (4096, 1 << 30, 1 << 30), (0x7FFFFFFF, 1, 64), (1 << 20, 0x7FFFFFFF, 1)):
+        assert lib.hsl_gated_ws_bytes(t, b, h) == 0
+    for n in (1 << 40, most):
+        assert lib.hsl_logprob_fwd_ws_bytes(n, 0x7FFF0000, 1) == 0
+    assert lib.hsl_embed_bwd_ws_bytes(0x7FFF0000, 0x7FFF0000, 1) > 0
+    assert lib.hsl_gated_ws_bytes((1 << 30) - 1, 1, 64) > 0
