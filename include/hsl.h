@@ -372,7 +372,8 @@ int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, f
  * reset and out have the time and batch strides given after them and dense channels.
  * h_n [B, H] = h_{T-1} in fp32 (h0 when T = 0); it may be h0 itself when T = 1.  ck
  * (NULL: no backward follows) receives the hsl_gated_ck_rows(T) rows [B, H] of states
- * that hsl_gated_bwd starts from.  hsl_gated_ws_bytes serves both directions. */
+ * that hsl_gated_bwd starts from.  hsl_gated_ws_bytes serves both directions.
+ * T is less than 2^30 and B*H less than 2^27. */
 int hsl_gated_ck_rows(int T);
 size_t hsl_gated_ws_bytes(int T, int B, int H);
 int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h0,

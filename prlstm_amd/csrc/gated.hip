@@ -686,7 +686,13 @@ GatedPlan plan_gated(int T, int B, int H, int E) {
 
 int check_gated(const char* who, int T, int B, int H, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
-  return check_shape(who, T, B, 0, H);
+  if (T < 0 || B < 0 || H < 0) return fail(HSL_ERR_ARG, "%s: negative size (T=%d B=%d H=%d)", who, T, B, H);
+  // steps and channels are counted in 32 bits, and 2^27 channels are 2^30 threads
+  if (T >= (1 << 30) || (long long)B * H >= (1ll << 27))
+    return fail(HSL_ERR_UNSUPPORTED,
+                "%s: T=%d B=%d H=%d is beyond the kernels' 32-bit index range (needs T < 2^30 and B*H < 2^27)", who, T,
+                B, H);
+  return HSL_OK;
 }
 
 // Channels of a thread.  (The single step's stay within a row, for its state may be updated in place.)

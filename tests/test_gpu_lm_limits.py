@@ -58,3 +58,19 @@ def test_embedding_of_more_rows_than_a_launch_has(dev):
         assert bool((rows == w[0]).all())
     del out, rows
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_gated_recurrence_of_many_channels(dev, T):
+    """More channels than a square weight of 2^31 elements would have."""
+    B, H = 2, 40001
+    g = torch.Generator().manual_seed(T)
+    zv = torch.randn(T, B, 2 * H, generator=g).to(dev).requires_grad_(True)
+    out, h_n = prlstm_amd.gated_recurrence(zv)
+    dz, = torch.autograd.grad(h_n.sum(), zv)
+    for lo in (0, H // 2, H - 7):
+        part = torch.cat((zv.detach()[..., lo:lo + 7], zv.detach()[..., H + lo:H + lo + 7]), -1).requires_grad_(True)
+        o, h = prlstm_amd.gated_recurrence(part)
+        d, = torch.autograd.grad(h.sum(), part)
+        assert torch.equal(out[..., lo:lo + 7], o) and torch.equal(h_n[:, lo:lo + 7], h)
+        assert torch.equal(torch.cat((dz[..., lo:lo + 7], dz[..., H + lo:H + lo + 7]), -1), d)

@@ -33,3 +33,13 @@ def test_size_queries_of_refused_sizes():
         assert lib.hsl_logprob_fwd_ws_bytes(n, 0x7FFF0000, 1) == 0
     assert lib.hsl_embed_bwd_ws_bytes(0x7FFF0000, 0x7FFF0000, 1) > 0
     assert lib.hsl_gated_ws_bytes((1 << 30) - 1, 1, 64) > 0
+
+
+def test_channels_of_the_gated_recurrence():
+    """It has no weight whose elements could pass 2^31: any width is taken up to 2^27 channels in all."""
+    fwd = _lib.load().hsl_gated_fwd
+    call = lambda t, b, h: fwd(None, 0, 0, None, None, 0, 0, None, 0, 0, None, None, None, 0, t, b, h, 0, None)  # noqa: E731
+    for t, b, h in ((1, 2, 40001), (3, 1, (1 << 27) - 1), ((1 << 30) - 1, 1000, 1000)):
+        assert call(t, b, h) == 1 and b"null pointer" in _lib.load().hsl_last_error()
+    for t, b, h in ((3, 1, 1 << 27), (3, 1 << 20, 1 << 10), (1 << 30, 1, 1), (1, 0x7FFFFFFF, 0x7FFFFFFF)):
+        _refused(call(t, b, h), b"index range")
