@@ -87,6 +87,12 @@ def _ids(name, t, device):
     return 1 if t.dtype is torch.int64 else 0
 
 
+def _fits(name, t):
+    """Sizes pass to the library in 32 bits, where 2^32 + 5 would be 5."""
+    if max(t.shape) >= 1 << 31:
+        raise RuntimeError(f"{name} {tuple(t.shape)} has a size of 2^31 or more")
+
+
 def _unit_inner(t):
     """t with its last dimension dense (a copy where it is not)."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
@@ -112,6 +118,7 @@ def _embed_check(ids, weight, padding_idx):
     if weight.dim() != 2:
         raise RuntimeError(f"weight must be [V, D], got shape {tuple(weight.shape)}")
     fmt = _fmt("weight", weight)
+    _fits("weight", weight)
     _no_tangents(weight)
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise RuntimeError(f"padding_idx {padding_idx} is not a row of weight {tuple(weight.shape)}")
@@ -182,6 +189,7 @@ def _gated_check(zv, h0, reset, dims):
     if zv.dim() != dims + 1 or zv.shape[-1] % 2:
         raise RuntimeError(f"zv must be [{', '.join(lead)}, 2H], got shape {tuple(zv.shape)}")
     fmt = _fmt("zv", zv)
+    _fits("zv", zv)
     _no_tangents(zv, h0)
     state = (zv.shape[-2], zv.shape[-1] // 2)
     if h0 is not None:
@@ -360,6 +368,7 @@ def token_logprobs(logits, tokens=None, top=0):
     fmt = _fmt("logits", logits)
     _no_tangents(logits)
     lead, v = logits.shape[:-1], logits.shape[-1]
+    _fits("logits", logits)
     top = int(top)
     if not 0 <= top <= min(MAX_TOP, v):
         raise RuntimeError(f"top must be in 0..{min(MAX_TOP, v)}, got {top}")

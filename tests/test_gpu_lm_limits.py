@@ -74,3 +74,19 @@ def test_gated_recurrence_of_many_channels(dev, T):
         d, = torch.autograd.grad(h.sum(), part)
         assert torch.equal(out[..., lo:lo + 7], o) and torch.equal(h_n[:, lo:lo + 7], h)
         assert torch.equal(torch.cat((dz[..., lo:lo + 7], dz[..., H + lo:H + lo + 7]), -1), d)
+
+
+def test_sizes_beyond_32_bits_are_refused(dev):
+    """Sizes that a 32-bit argument would take for others: 2^32 + 5 is not 5."""
+    n = (1 << 32) + 5
+    one = torch.zeros(1, 1, device=dev)
+    ids = torch.tensor([7], device=dev)
+    for call in (lambda: prlstm_amd.embedding(ids, one.expand(n, 1)),
+                 lambda: prlstm_amd.embedding(ids[:0], one.expand(3, n)),
+                 lambda: prlstm_amd.gated_recurrence(one[None].expand(n, 0, 2)),
+                 lambda: prlstm_amd.gated_recurrence(one[None].expand(0, n, 2)),
+                 lambda: prlstm_amd.gated_recurrence_step(one.expand(0, 2 * n), None),
+                 lambda: prlstm_amd.token_logprobs(one.expand(0, n))):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            call()
+    prlstm_amd.check_errors(dev)
