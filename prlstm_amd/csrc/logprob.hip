@@ -514,8 +514,9 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(
   const float dh = ENT ? dent[n] : 0.f, SH = ENT ? __builtin_fmaf(dh, entropy[n], S) : S;
   auto grad = [&](float x) {
     const float d = x - m - ls, p = __builtin_amdgcn_exp2f(d * kLog2e);
-    if constexpr (ENT) return -p * __builtin_fmaf(dh, fmaxf(d, -1e30f), SH);
-    return -p * SH;
+    // p = 0: no gradient, though d may be -inf, dh d beyond fp32, or what arrives not finite
+    const float pull = ENT ? __builtin_fmaf(dh, d, SH) : SH;
+    return p == 0.f ? 0.f : -p * pull;
   };
 #pragma unroll
   for (int k = 0; k < kBwdVecs; ++k) {

@@ -90,3 +90,31 @@ def test_sizes_beyond_32_bits_are_refused(dev):
         with pytest.raises(RuntimeError, match="2\\^31"):
             call()
     prlstm_amd.check_errors(dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_tokens_of_a_large_entropy_gradient(dev, dtype):
+    """A masked token has no gradient, whatever the entropy's is; the others' are finite."""
+    x = torch.tensor([[0.0, -float("inf"), 1.0, -500.0, 2.0]]).to(dtype)
+    want = torch.zeros(1, 5, dtype=torch.float64)
+    y = x.double()[:, [0, 2, 4]].requires_grad_(True)
+    p = torch.softmax(y, 1)
+    want[:, [0, 2, 4]] = torch.autograd.grad(-(p * torch.log(p)).sum(), y)[0]
+    for dent in (1.0, 1e9, 1e30):
+        xd = x.to(dev).requires_grad_(True)
+        dx, = torch.autograd.grad(prlstm_amd.token_logprobs(xd).entropy, xd, torch.tensor([dent], device=dev))
+        got = dx.double().cpu() / dent
+        # fp32 statistics of order 1 and one rounding to the type
+        u = 2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -24
+        assert bool(((got - want).abs() <= 1.01 * u * want.abs() + 64 * 2.0 ** -24).all()), (dent, got, want)
+        assert float(got[0, 1]) == 0.0
+
+
+def test_masked_tokens_of_an_infinite_gradient(dev):
+    inf = float("inf")
+    x = torch.tensor([[0.0, -inf, 1.0, -inf, 2.0]], device=dev, requires_grad=True)
+    r = prlstm_amd.token_logprobs(x, torch.tensor([2], device=dev), top=1)
+    for out in (r.logp, r.entropy, r.top_logp):
+        for g in (inf, float("nan")):
+            dx, = torch.autograd.grad(out, x, torch.full_like(out, g), retain_graph=True)
+            assert dx[0, 1] == 0.0 and dx[0, 3] == 0.0 and not bool(torch.isfinite(dx[0, 4]))
