@@ -1,8 +1,9 @@
 """A small language model on the package's operators, as an example of their use together.
 
 Token ids are embedded (``embedding``), run through a ``HeadStartLSTM`` layer and gated recurrences
-(``gated_recurrence``), and projected on the vocabulary; the log probabilities of the next tokens (``token_logprobs``) are the training loss and what a server answers with.  ``step`` takes one
-token of each of a batch of streams and updates their state in place.
+(``gated_recurrence``), and projected on the vocabulary; the log probabilities of the next tokens
+(``token_logprobs``) are the training loss and what a server answers with.  ``step`` takes one token of
+each of a batch of streams and updates their state in place.
 
 ``python -m prlstm_amd.language_model`` trains one on walks around a circle and continues them.
 """
@@ -56,18 +57,34 @@ class LanguageModel(nn.Module):
     def logits(self, x):
         return self.head(self.norm(x))
 
+    def run_lstm(self, x, h, c, reset):
+        """The LSTM over x from (h, c).  It has no reset of its own, so the sequence is run in parts
+        that begin at the steps where a row has one (which the host reads)."""
+        starts = [] if reset is None else reset.any(1).nonzero()[:, 0].tolist()
+        if not starts:
+            y, (h, c) = self.lstm(x, (h, c))
+            return y, h[0], c[0]
+        parts, bounds = [], [0, *(t for t in starts if t > 0), len(x)]
+        for t0, t1 in zip(bounds, bounds[1:]):
+            keep = ~reset[t0].bool()[:, None]
+            h, c = (torch.where(keep, s, torch.zeros_like(s)) for s in (h, c))
+            y, (h, c) = self.lstm(x[t0:t1], (h, c))
+            h, c = h[0], c[0]
+            parts.append(y)
+        return torch.cat(parts), h, c
+
     def forward(self, ids, state=None, reset=None):
-        """(logits [T, B, V], the state behind them).  ``reset`` [T, B] cuts the gated layers' state
-        between documents."""
+        """(logits [T, B, V], the state behind them).  Where ``reset`` [T, B] is set a new document
+        begins: nothing of any layer's state passes."""
         (h, c), gated = self.state(ids.shape[1]) if state is None else state
         x = embedding(ids, self.weight, scale=self.width ** 0.5)
-        y, (h, c) = self.lstm(x, (h.to(x.dtype), c.to(x.dtype)))
+        y, h, c = self.run_lstm(x, h.to(x.dtype), c.to(x.dtype), reset)
         x = x + y
         after = []
         for layer, h0 in zip(self.layers, gated):
             x, h1 = layer(x, h0, reset)
             after.append(h1)
-        return self.logits(x), ((h[0].float(), c[0].float()), after)
+        return self.logits(x), ((h.float(), c.float()), after)
 
     def loss(self, ids, targets, reset=None):
         """Mean negative log probability of targets [T, B] (negative: not scored)."""
