@@ -43,3 +43,9 @@ def test_channels_of_the_gated_recurrence():
         assert call(t, b, h) == 1 and b"null pointer" in _lib.load().hsl_last_error()
     for t, b, h in ((3, 1, 1 << 27), (3, 1 << 20, 1 << 10), (1 << 30, 1, 1), (1, 0x7FFFFFFF, 0x7FFFFFFF)):
         _refused(call(t, b, h), b"index range")
+
+
+def test_checkpoint_rows():
+    """One state for each 16 steps that begin."""
+    rows = _lib.load().hsl_gated_ck_rows
+    assert [rows(t) for t in (-1, 0, 1, 15, 16, 17, 32, 33, 4096, 4097)] == [0, 0, 1, 1, 1, 2, 2, 3, 256, 257]
