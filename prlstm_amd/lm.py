@@ -89,7 +89,8 @@ def _ids(name, t, device):
 
 def _fits(name, t):
     """Sizes pass to the library in 32 bits, where 2^32 + 5 would be 5."""
-    if max(t.shape) >= 1 << 31:
+    n = t.numel()
+    if (n >= 1 << 31 or n == 0) and max(t.shape) >= 1 << 31:
         raise RuntimeError(f"{name} {tuple(t.shape)} has a size of 2^31 or more")
 
 
@@ -109,8 +110,8 @@ def _scale(scale):
     if isinstance(scale, torch.Tensor):
         _no_tangents(scale)
         if scale.is_cuda or (scale.requires_grad and torch.is_grad_enabled()):
-            raise RuntimeError(f"scale must be a number (it has no gradient and is not read from the GPU), got a tensor "
-                               f"on {scale.device} with requires_grad={scale.requires_grad}")
+            raise RuntimeError(f"scale must be a number (it has no gradient and is not read from the GPU), got a "
+                               f"tensor on {scale.device} with requires_grad={scale.requires_grad}")
     return float(scale)
 
 
@@ -167,7 +168,7 @@ def embedding(ids, weight, scale=1.0, padding_idx: Optional[int] = None):
     ``padding_idx`` is a row that gets none.  scale is a number and has no gradient.
     """
     fmt, ids64 = _embed_check(ids, weight, padding_idx)
-    ids, weight, scale = ids.contiguous(), _unit_inner(weight), _scale(scale)
+    ids, weight, scale = ids.contiguous(), _unit_inner(weight), scale if type(scale) is float else _scale(scale)
     if weight.requires_grad and torch.is_grad_enabled():
         return EmbeddingFn.apply(ids, weight, scale, padding_idx, fmt, ids64)
     return _embed_fwd(ids, weight, scale, fmt, ids64)
