@@ -388,17 +388,19 @@ int hsl_gated_bwd(const void* zv, long long zv_t, long long zv_b,
                   void* ws, size_t ws_bytes, int T, int B, int H, int fmt, void* stream);
 
 /* Of each row n of logits [N, V] (row stride ld): logp[n] = log softmax at tokens[n]
- * (int64 or int32; tokens and logp may be NULL), entropy[n], stats[n] = (largest logit m,
- * log sum exp(x - m)) for the backward, and the `top` (<= 32, <= V) largest: top_logp, top_ids [N, top],
- * ordered by logit with NaN first and the lowest id first among equals.  -inf masks a
- * token; a row of nothing else has m = logp = -inf and entropy 0.  A negative token
- * gives logp 0; one >= V NaN, and raises bit 1 of the device word. */
+ * (int64 or int32; tokens and logp may be NULL), entropy[n], stats[n] = (m, log sum exp(x - m))
+ * for the backward, with m a reference about 8 below the largest logit at most, and the
+ * `top` (<= 32, <= V) largest: top_logp, top_ids [N, top], ordered by logit with NaN first and
+ * the lowest id first among equals.  -inf masks a token; a row of nothing else has
+ * m = logp = -inf and entropy 0.  A negative token gives logp 0; one >= V NaN, and raises
+ * bit 1 of the device word. */
 size_t hsl_logprob_fwd_ws_bytes(long long N, int V, int top);
 int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int tok64,
                     float* logp, float* entropy, float* stats, float* top_logp, long long* top_ids,
                     void* ws, size_t ws_bytes, long long N, int V, int top, int fmt, void* stream);
 /* dlogits [N, V] (row stride ldd) from the gradients of logp, entropy and top_logp (each
- * may be NULL: zeros); a row with nothing but masks gets zeros. */
+ * may be NULL: zeros); a row with nothing but masks gets zeros, and so does a masked token
+ * whatever arrives. */
 int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int tok64,
                     const long long* top_ids, const float* stats, const float* entropy,
                     const float* dlogp, const float* dent, const float* dtop,

@@ -93,8 +93,9 @@ __device__ __forceinline__ long long row_at(const Rows& r, unsigned block, unsig
 }
 
 // The forward: a gather, bound by its rows' traffic; four rows a lane are in flight.  N65536 V131072
-// D1024 bf16: 33 us for 134 MB written (4.1 TB/s; the rows read are mostly in the caches),
-// 46 on average in training passes on inputs in turn (the cause of the difference is not measured).
+// D1024 bf16: 33 us for 134 MB written (4.1 TB/s) where the 41 MB of distinct rows are in the caches; 6
+// more where they are not, and up to 15 more behind a pass whose stores are still on their way to memory
+// (46 on average in training passes on inputs in turn).
 template <int F, bool SMALL>
 __global__ __launch_bounds__(kBlock) void embed_fwd_kernel(const void* __restrict__ ids, int ids64,
                                                            const typename Elem<F>::T* __restrict__ w, long long ldw,
@@ -198,7 +199,7 @@ __device__ __forceinline__ void place_round(int q, int i, int bits, int* cnt, in
 
 // The sort of one class.  Every workgroup reads all ids (from its XCD's L2) rather than exchange
 // anything with the others, so it is one launch; it is bound by the instructions of that look (65536
-// int32 ids: 24 us, of which the loads alone are 4; 8192: 9; 700: 6).
+// int32 ids: 26 us, of which the loads alone are 4; 8192 int64 ids: 9; 700: 6).
 template <class I>
 __global__ __launch_bounds__(kSortThreads) void embed_sort_kernel(const I* __restrict__ ids, int N, int V, int padding,
                                                                   Sorted s) {
@@ -381,8 +382,8 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const void* __restric
   }
 }
 
-// The long rows of class blockIdx.x, 64 columns (7 us at the size above, 3 to 4 of them the launch): kJoinGroups shares of a row's partials, each added
-// in order, then the shares in order.
+// The long rows of class blockIdx.x, 64 columns: kJoinGroups shares of a row's partials, each added in
+// order, then the shares in order.  6.5 us at the size above, 3 to 4 of them the launch.
 template <int F>
 __global__ __launch_bounds__(kBlock) void embed_join_kernel(Sorted s, const float* __restrict__ partial, int pitch,
                                                             float scale, typename Elem<F>::T* __restrict__ dw, int D) {
@@ -435,7 +436,11 @@ EmbedPlan plan_embed(long long N, int V, int D) {
   p.log2c = 8;
   while (((long long)kClassTokens << p.log2c) < V) ++p.log2c;
   p.nclass = 1 << p.log2c;
-  // short for short calls, whose time is that of one chunk; at most 4096
+  // Short for short calls, whose time is that of one chunk; at most 4096.  us of the whole gradient, bf16
+  // V32768, ids with a share of 1 / rank, chunks of 16 / 32 / 64:
+  //   D256:  N500 16 / 18 / 19;  N8192 22 / 27 / 39;  N32768 34 / 42 / 60;  N65536 49 / 54 / 69
+  //   D1024: N500 24 / 28 / 28;  N8192 29 / 32 / 42;  N32768 44 / 45 / 53;  N65536 70 / 65 / 69
+  // (8: within 2 of 16, but 50 at N32768 D1024; at N131072 all are within 2 but 64 at D256, 117 to 104.)
   p.chunk = N <= 32768 ? 16 : 32;
   while ((long long)p.chunk * 4096 < N) p.chunk *= 2;
   p.nchunks = N > p.chunk ? (int)((N + p.chunk - 1) / p.chunk) : 0;  // no token is longer than a chunk
@@ -515,8 +520,8 @@ int hsl_embed_bwd(const void* ids, int ids64, const void* dout, long long ldd, f
   const Rows all = rows_of(V, D, fmt == kElemF32 ? Vec<kElemF32>::N : Vec<kElemBf16>::N);
   const int chunk_blocks = (p.nchunks + (kBlock >> all.log2g) - 1) / (kBlock >> all.log2g);
   if (V > kMostTokens || row_blocks(all) + chunk_blocks > kLaunchBlocks)
-    return fail(HSL_ERR_UNSUPPORTED, "hsl_embed_bwd: V=%d D=%d are beyond one launch (V at most 2^30, dweight below 2^37 bytes)",
-                V, D);
+    return fail(HSL_ERR_UNSUPPORTED,
+                "hsl_embed_bwd: V=%d D=%d are beyond one launch (V at most 2^30, dweight below 2^37 bytes)", V, D);
   EmbedWs w;
   const size_t need = carve_embed(ws, ws_bytes, N, V, p, &w);
   if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_embed_bwd: workspace %zu bytes, need %zu", ws_bytes, need);

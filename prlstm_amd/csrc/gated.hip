@@ -245,9 +245,9 @@ __device__ __forceinline__ void enter_segment(const float2* __restrict__ maps, i
   }
 }
 
-// Forward.  Bound by HBM: T4096 B16 H1024 bf16 74 us for 419 MB (5.7 TB/s, a large copy has 5.1; 83 on
-// average in training passes on inputs in turn), fp32
-// 150 us for 822 MB.  Two channels a lane make 128-byte (bf16) and 256-byte (fp32) rows of a group.
+// Forward.  Bound by HBM: T4096 B16 H1024 bf16 74 us for 419 MB (5.7 TB/s, a large copy has 5.1; 79 to 83
+// on average in training passes on inputs in turn), fp32 150 us for 822 MB.  Two channels a lane make
+// 128-byte (bf16) and 256-byte (fp32) rows of a group.
 template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, const float* h0, Stream reset,
                                                                   OutStream out, float* h_n, float* __restrict__ ck,
@@ -264,7 +264,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_kernel(Stream zv, co
   enter_segment<E, RESET, false>(maps, C, q.ch, seg, gridDim.y, x);
   // the group's first step of the chunk that is loaded (zp, rp) and of the one that is run (op)
   const T_* zp = static_cast<const T_*>(zv.p) + q.b * zv.sb + (tb + q.g * kSteps) * zv.st + q.j;
-  const unsigned char* rp = static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + (tb + q.g * kSteps) * reset.st;
+  const unsigned char* rp =
+      static_cast<const unsigned char*>(reset.p) + q.b * reset.sb + (tb + q.g * kSteps) * reset.st;
   T_* op = static_cast<T_*>(out.p) + q.b * out.sb + (tb + q.g * kSteps) * out.st + q.j;
   float* cp = ck + (size_t)(tb / kCkSteps + q.w) * C + q.ch;
 
@@ -418,7 +419,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_fwd_map_kernel(Stream zv
 
 // Backward: the group's steps forward from the checkpoint (by way of the wave's first group for its
 // second), then the reverse map and, from the joined U, the gradients.  T4096 B16 H1024 bf16 136 us for
-// 688 MB (5.1 TB/s; 145 on average in training passes on inputs in turn), fp32 228 us for 1359 MB (6.0).  A third or fourth chunk in flight changes nothing.
+// 688 MB (5.1 TB/s; 141 to 145 on average in training passes on inputs in turn), fp32 228 us for 1359 MB
+// (6.0).  A third or fourth chunk in flight changes nothing.
 template <int F, int E, bool RESET, bool NT>
 __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_kernel(Stream zv, Stream reset,
                                                                   const float* __restrict__ ck, Stream dout,
@@ -627,7 +629,8 @@ __global__ __launch_bounds__(kMaxWaves * 64) void gated_bwd_map_kernel(Stream zv
   }
 }
 
-// A single step, bound by its launch (2.5 us for B32 H1024): one thread per E channels (H is a multiple of E).  h_n may be h0.
+// A single step, bound by its launch (2.5 us for B32 H1024): one thread per E channels (H is a multiple
+// of E).  h_n may be h0.
 template <int F, int E, bool RESET>
 __global__ __launch_bounds__(256) void gated_step_kernel(Stream zv, const float* h0, Stream reset, OutStream out,
                                                          float* h_n, float* ck, int B, int H) {
@@ -658,11 +661,19 @@ struct GatedPlan {
   int waves, tiles, nseg, seg_steps;
 };
 // Waves: 8 (chunks of 128 steps) where a CU gets one or two workgroups, 4 where it gets more or the
-// time is cut, 1 and 2 for short sequences.  us forward, backward, bf16, 8 waves / 4 waves:
-//   T4096 B16 H1024 (256 workgroups): 73, 152 / 87, 166;  T256 B64 H1024 (1024): 24, 39 / 21, 31
-//   T2048 B32 H1024 (512): 79, 150 / 81, 140;  16 waves at 256 workgroups: 119, 275 (registers)
+// time is cut, 1 and 2 for short sequences.  us forward, backward, 8 waves / 4 waves, H1024:
+//   bf16 T4096 B16 (256 workgroups): 73, 152 / 87, 166;  16 waves: 119, 275 (registers)
+//   bf16 T4096 B20 (320): 132, 244 / 137, 209;  B28 (448): 142, 263 / 146, 248;  B32 (512): 158, 281 / 167, 272
+//   fp32 T4096 B20 (320): 260, 389 / 238, 387;  B28 (448): 284, 444 / 268, 461;  B32 (512): 306, 482 / 291, 499
+//   bf16 T256  B20 (320): 12, 17 / 11, 14;  B64 (1024): 25, 39 / 22, 31;   T2048 B32 (512): 79, 150 / 81, 140
+// so that between 257 and 511 workgroups 4 waves would gain up to a fifth of a bf16 backward.
 // Segments: of at least two chunks, for about 512 workgroups, where the channels alone give fewer
-// than 192.  us of T16383 B2 H256 fp32, 8 tiles: 36, 40 for 512; 47, 45 for 256; 38, 46 for 1024.
+// than 192.  us of T16383 B2 H256 fp32, 8 tiles: 36, 40 for 512; 47, 45 for 256; 38, 46 for 1024.  With
+// segments / without, T4096 H1024:
+//   bf16 B8 H512 (64 workgroups): 32, 46 / 56, 79;  B8 (128): 57, 83 / 56, 107;  B10 (160): 73, 114 / 57, 117;
+//        B12 (192): 96, 162 / 68, 121
+//   fp32 B8 H512: 65, 75 / 75, 148;  B8: 126, 149 / 117, 167;  B10: 170, 206 / 124, 181;  B12: 240, 263 / 130, 192
+// so that the two meet at about 128 workgroups, and those from there to 191 would gain a little without.
 GatedPlan plan_gated(int T, int B, int H, int E) {
   GatedPlan p;
   p.tiles = (int)(((long)B * ((H + E - 1) / E) + kLanes - 1) / kLanes);
@@ -759,10 +770,10 @@ int hsl_gated_fwd(const void* zv, long long zv_t, long long zv_b, const float* h
       hipLaunchKernelGGL((gated_step_kernel<kF, kE, kR>), dim3(n), dim3(256), 0, s, z, h0, r, o, h_n, ck, B, H);
     } else {
       if (p.nseg > 1)
-        hipLaunchKernelGGL((gated_fwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z, r,
-                           maps, T, B, H, p.seg_steps);
-      hipLaunchKernelGGL((gated_fwd_kernel<kF, kE, kR, kN>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, h0, r, o,
-                         h_n, ck, maps, T, B, H, p.seg_steps);
+        hipLaunchKernelGGL((gated_fwd_map_kernel<kF, kE, kR>), dim3(p.tiles, p.nseg - 1), dim3(p.waves * 64), 0, s, z,
+                           r, maps, T, B, H, p.seg_steps);
+      hipLaunchKernelGGL((gated_fwd_kernel<kF, kE, kR, kN>), dim3(p.tiles, p.nseg), dim3(p.waves * 64), 0, s, z, h0, r,
+                         o, h_n, ck, maps, T, B, H, p.seg_steps);
     }
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;

@@ -2,7 +2,8 @@
 //   m = max x,  s = sum exp(x - m),  log p_v = (x_v - m) - log s
 //   H = -sum p log p = log s - (sum e d) / s  with d = x - m, e = exp(d)
 // m and log s stay apart (stats): in a row of the type's lowest value m + log s would be m.
-// Any m within a few units of the largest logit serves: the sums are floating point.
+// Any m near the largest logit serves, for the sums are floating point: stats holds a running
+// reference that is up to kSlack below it.
 // -inf is a masked token: probability 0 and nothing to the entropy.  A row of nothing else has
 // logp -inf for every token, entropy 0 and no gradient.  A row with NaN or +inf gives NaN.
 // The alternatives are ordered by logit, NaN above all, the lowest id first among equals.
@@ -238,8 +239,8 @@ struct alignas(16) TopShared {
 };
 template <int F, int W, int GL, int KEYS, bool LANES>
 __device__ void choose_top(const typename Elem<F>::T* __restrict__ row, int V, int top, int part, int nvec,
-                           unsigned long long key, unsigned long long lane_key, float r, float ls, bool nan_row, bool none, size_t n, const Out& o,
-                           TopShared& sh) {
+                           unsigned long long key, unsigned long long lane_key, float r, float ls, bool nan_row,
+                           bool none, size_t n, const Out& o, TopShared& sh) {
   constexpr int N = Vec<F>::N, kN = W * 64;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   if (threadIdx.x < KEYS) sh.key[threadIdx.x] = key;
@@ -394,8 +395,12 @@ __device__ __forceinline__ unsigned long long group_key(float best, int at) {
 }
 
 // One workgroup per row, one pass: the running sums and each group's largest element.  Bound by HBM:
-// N8192 V32768 bf16 95 us for 537 MB (5.7 TB/s; 105 on average in training passes on inputs in turn), with 20 alternatives 122.  A row of up to kShortRow
-// logits takes one wave, which needs no barriers (N8192 V1000 with 4: 22 us, 30 with four waves).
+// N8192 V32768 bf16 95 us for 537 MB (5.7 TB/s; 105 on average in training passes on inputs in turn),
+// with 20 alternatives 122.  A row of up to kShortRow logits takes one wave, which needs no barriers.  us
+// without and with 4 alternatives, one wave / four:
+//   bf16 N8192 V512: 5.7, 21 / 11, 27;  V2048: 8.9, 25 / 14, 29;  V4096: 16, 31 / 19, 33
+//   fp32 N8192 V512: 5.9, 20 / 11, 25;  V2048: 14, 26 / 16, 30;  V4096: 23, 35 / 22, 32
+// With 64 rows the two are within 0.5 up to V2048.
 template <int F, bool TOP, int W>
 __global__ __launch_bounds__(W * 64) void logprob_row_kernel(const typename Elem<F>::T* __restrict__ logits,
                                                                long long ld, const void* __restrict__ tokens,
@@ -621,7 +626,8 @@ int hsl_logprob_fwd(const void* logits, long long ld, const void* tokens, int to
   LogprobWs w{};
   if (p.count > 1) {
     const size_t need = carve_logprob(ws, ws_bytes, N, p.count, &w);
-    if (!ws || ws_bytes < need) return fail(HSL_ERR_ARG, "hsl_logprob_fwd: workspace %zu bytes, need %zu", ws_bytes, need);
+    if (!ws || ws_bytes < need)
+      return fail(HSL_ERR_ARG, "hsl_logprob_fwd: workspace %zu bytes, need %zu", ws_bytes, need);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Out o{tokens ? logp : nullptr, entropy, stats, top_logp, top_ids};
@@ -685,8 +691,9 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
     for (long long n0 = (N - 1) / 65535 * 65535; n0 >= 0; n0 -= 65535) {
       const unsigned rows = (unsigned)std::min<long long>(N - n0, 65535);
       auto run = [&](auto e, auto past) {
-        hipLaunchKernelGGL((logprob_bwd_kernel<kF, decltype(e)::value, decltype(past)::value>), dim3((nvec + part - 1) / part, rows),
-                           dim3(kThreads), 0, s, static_cast<const T*>(logits) + n0 * ld, ld,
+        hipLaunchKernelGGL((logprob_bwd_kernel<kF, decltype(e)::value, decltype(past)::value>),
+                           dim3((nvec + part - 1) / part, rows), dim3(kThreads), 0, s,
+                           static_cast<const T*>(logits) + n0 * ld, ld,
                            tokens ? static_cast<const char*>(tokens) + n0 * (tok64 ? 8 : 4) : nullptr, tok64,
                            top_ids ? top_ids + n0 * top : nullptr, stats + 2 * n0, entropy ? entropy + n0 : nullptr,
                            dlogp ? dlogp + n0 : nullptr, dent ? dent + n0 : nullptr, dtop ? dtop + n0 * top : nullptr,
