@@ -406,6 +406,66 @@ int hsl_logprob_bwd(const void* logits, long long ld, const void* tokens, int to
                     const float* dlogp, const float* dent, const float* dtop,
                     void* dlogits, long long ldd, long long N, int V, int top, int fmt, void* stream);
 
+/* Causal depthwise convolution of K (1..4) taps, x [T, B, D]:
+ *   u_t = bias + sum_j w[:, j] x_{t-K+1+j},   y_t = silu ? u_t sigmoid(u_t) : u_t
+ * with w [D, K] and bias [D] in fp32 (bias may be NULL).  state [B, K-1, D] in x's format
+ * holds the inputs before the first step, the oldest first (NULL: zeros); state_n receives the
+ * last K-1 inputs the same way (it may be state itself when T = 1).  Where reset [T, B] (bytes;
+ * NULL: none) is nonzero a new sequence begins: inputs before it count as 0, in state_n too.
+ * x, reset, y and the gradients have the time and batch strides given after them and dense
+ * channels.  T is less than 2^30, B*D less than 2^27 and T*B*D less than 2^38. */
+int hsl_conv_fwd(const void* x, long long x_t, long long x_b, const float* w, const float* bias,
+                 const void* state, const void* reset, long long rs_t, long long rs_b,
+                 void* y, long long y_t, long long y_b, void* state_n, int silu,
+                 int T, int B, int D, int K, int fmt, void* stream);
+/* dx, dw [D, K], dbias [D] (may be NULL) and dstate [B, K-1, D] (may be NULL) from dy and
+ * dstate_n (each may be NULL: zeros). */
+size_t hsl_conv_ws_bytes(int T, int B, int D, int K);
+int hsl_conv_bwd(const void* x, long long x_t, long long x_b, const float* w, const float* bias,
+                 const void* state, const void* reset, long long rs_t, long long rs_b,
+                 const void* dy, long long dy_t, long long dy_b, const void* dstate_n,
+                 void* dx, long long dx_t, long long dx_b, float* dw, float* dbias, void* dstate,
+                 int silu, void* ws, size_t ws_bytes, int T, int B, int D, int K, int fmt, void* stream);
+
+/* Selective scan of N (1..64) states per channel:
+ *   dt_t = softplus ? log(1 + exp(delta_t + delta_bias)) : delta_t + delta_bias
+ *   h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t,   h_{-1} = h0 (NULL: zeros)
+ *   y_t = sum_n c_t[n] h_t[n] + d x_t,   out_t = z ? y_t z_t sigmoid(z_t) : y_t
+ * and 0 in place of h_{t-1} where reset [T, B] (bytes; NULL: none) is nonzero.  x, delta, z (may
+ * be NULL) and out are [T, B, D], b and c [T, B, N], all of one format; a [D, N], d and
+ * delta_bias [D] (each may be NULL), h0 and h_n [B, D, N] are fp32.  h_n = h_{T-1} (h0 when
+ * T = 0); it may be h0 itself when T = 1 and ck is NULL.  ck (NULL: no backward follows) receives
+ * hsl_selective_ck_floats(T, B, D, N) values that hsl_selective_bwd starts from.  T is less than
+ * 2^30, B*D less than 2^27 and B*ceil(D/64)*ceil(N/4) less than 2^25. */
+size_t hsl_selective_ck_floats(int T, int B, int D, int N);
+size_t hsl_selective_fwd_ws_bytes(int T, int B, int D, int N);
+int hsl_selective_fwd(const void* x, long long x_t, long long x_b,
+                      const void* delta, long long de_t, long long de_b, const float* a,
+                      const void* b, long long b_t, long long b_b,
+                      const void* c, long long c_t, long long c_b, const float* d,
+                      const void* z, long long z_t, long long z_b, const float* delta_bias,
+                      const float* h0, const void* reset, long long rs_t, long long rs_b,
+                      void* out, long long out_t, long long out_b, float* h_n, float* ck,
+                      int softplus, void* ws, size_t ws_bytes,
+                      int T, int B, int D, int N, int fmt, void* stream);
+/* The gradients from dout and dh_n (each may be NULL: zeros); dd, ddelta_bias and dh0 may be
+ * NULL, dz where z is. */
+size_t hsl_selective_bwd_ws_bytes(int T, int B, int D, int N);
+int hsl_selective_bwd(const void* x, long long x_t, long long x_b,
+                      const void* delta, long long de_t, long long de_b, const float* a,
+                      const void* b, long long b_t, long long b_b,
+                      const void* c, long long c_t, long long c_b, const float* d,
+                      const void* z, long long z_t, long long z_b, const float* delta_bias,
+                      const void* reset, long long rs_t, long long rs_b, const float* ck,
+                      const void* dout, long long do_t, long long do_b, const float* dh_n,
+                      void* dx, long long dx_t, long long dx_b,
+                      void* ddelta, long long dd_t, long long dd_b, float* da,
+                      void* db, long long db_t, long long db_b,
+                      void* dc, long long dc_t, long long dc_b, float* dd,
+                      void* dz, long long dz_t, long long dz_b, float* ddelta_bias, float* dh0,
+                      int softplus, void* ws, size_t ws_bytes,
+                      int T, int B, int D, int N, int fmt, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ import torch.nn as nn
 
 from .functional import EPS, headstartlstm_parallel, headstartlstm_recurrent
 from .lm import TokenLogprobs, embedding, gated_recurrence, gated_recurrence_step, token_logprobs
+from .selective import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from ._lib import (check_errors, last_recurrent_path, set_exchange_scope, set_recurrent_path, set_spin_timeout_us,
                    set_split_products)
 
@@ -107,5 +108,6 @@ __all__ = [
     "set_recurrent_path", "set_spin_timeout_us", "set_exchange_scope", "set_split_products", "last_recurrent_path",
     "check_errors",
     "embedding", "gated_recurrence", "gated_recurrence_step", "token_logprobs", "TokenLogprobs",
+    "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step",
     "__version__",
 ]

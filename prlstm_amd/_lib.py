@@ -74,6 +74,18 @@ SIGNATURES = {
     "hsl_logprob_fwd_ws_bytes": (_Z, [_L, _I, _I]),
     "hsl_logprob_fwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _Z, _L, _I, _I, _I, _P]),
     "hsl_logprob_bwd": (_I, [_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _I, _I, _I, _P]),
+    "hsl_conv_fwd": (_I, [_P, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L, _L, _P] + [_I] * 6 + [_P]),
+    "hsl_conv_ws_bytes": (_Z, [_I, _I, _I, _I]),
+    "hsl_conv_bwd": (_I, [_P, _L, _L, _P, _P, _P, _P, _L, _L, _P, _L, _L, _P, _P, _L, _L, _P, _P, _P, _I, _P, _Z]
+                     + [_I] * 5 + [_P]),
+    "hsl_selective_ck_floats": (_Z, [_I, _I, _I, _I]),
+    "hsl_selective_fwd_ws_bytes": (_Z, [_I, _I, _I, _I]),
+    "hsl_selective_fwd": (_I, [_P, _L, _L] * 2 + [_P] + [_P, _L, _L] * 2 + [_P, _P, _L, _L, _P, _P, _P, _L, _L]
+                          + [_P, _L, _L, _P, _P, _I, _P, _Z] + [_I] * 5 + [_P]),
+    "hsl_selective_bwd_ws_bytes": (_Z, [_I, _I, _I, _I]),
+    "hsl_selective_bwd": (_I, [_P, _L, _L] * 2 + [_P] + [_P, _L, _L] * 2 + [_P, _P, _L, _L, _P, _P, _L, _L, _P]
+                          + [_P, _L, _L, _P] + [_P, _L, _L] * 2 + [_P] + [_P, _L, _L] * 2 + [_P]
+                          + [_P, _L, _L, _P, _P, _I, _P, _Z] + [_I] * 5 + [_P]),
 }
 
 _lock = threading.Lock()

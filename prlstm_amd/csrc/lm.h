@@ -1,4 +1,5 @@
-// Helpers shared by the language-model operators (embed.hip, gated.hip, logprob.hip).
+// Helpers shared by the language-model operators (embed.hip, gated.hip, logprob.hip, conv.hip,
+// selective.hip, xent.hip).
 #pragma once
 
 #include <type_traits>
@@ -64,6 +65,74 @@ __device__ __forceinline__ void store16_nt(void* p, const V& x) {
   __builtin_memcpy(&u, &x, sizeof(u));
   __builtin_nontemporal_store(u, static_cast<Raw*>(p));
 }
+// Strides are in elements.
+struct Stream {
+  const void* p;
+  long long st, sb;
+};
+struct OutStream {
+  void* p;
+  long long st, sb;
+};
+
+// E neighbouring elements, at any element's alignment (global memory takes unaligned accesses).
+template <int F, int E>
+struct Pack {
+  typename Elem<F>::T v[E];
+};
+// NT: non-temporal, for streams that no cache holds until their next use.
+template <int N>
+struct RawOf;
+template <>
+struct RawOf<2> {
+  using T = unsigned short;
+};
+template <>
+struct RawOf<4> {
+  using T = unsigned;
+};
+template <>
+struct RawOf<8> {
+  using T = unsigned __attribute__((ext_vector_type(2)));
+};
+template <>
+struct RawOf<16> {
+  using T = unsigned __attribute__((ext_vector_type(4)));
+};
+template <int F, int E, bool NT = false>
+__device__ __forceinline__ Pack<F, E> load_pack(const typename Elem<F>::T* p) {
+  Pack<F, E> r;
+  if constexpr (NT) {
+    typedef typename RawOf<sizeof(r)>::T Raw __attribute__((aligned(alignof(Pack<F, E>)), may_alias));
+    const auto u = __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+    __builtin_memcpy(&r, &u, sizeof(r));
+  } else {
+    __builtin_memcpy(&r, p, sizeof(r));
+  }
+  return r;
+}
+template <int F, int E>
+__device__ __forceinline__ void store_pack(typename Elem<F>::T* p, const Pack<F, E>& v) {
+  typedef typename RawOf<sizeof(v)>::T Raw __attribute__((aligned(alignof(Pack<F, E>)), may_alias));
+  typename RawOf<sizeof(v)>::T u;
+  __builtin_memcpy(&u, &v, sizeof(v));
+  __builtin_nontemporal_store(u, reinterpret_cast<Raw*>(p));
+}
+template <int E>
+struct Floats {
+  float v[E];
+};
+template <int E>
+__device__ __forceinline__ Floats<E> load_floats(const float* p) {
+  Floats<E> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+template <int E>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[E]) {
+  __builtin_memcpy(p, v, sizeof(v));
+}
+
 // What a call streams through beyond this is not kept in the caches (the last-level one has 256 MB).
 constexpr size_t kCacheBytes = 256u << 20;
 
