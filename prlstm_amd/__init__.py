@@ -21,6 +21,7 @@ import torch.nn as nn
 
 from .functional import EPS, headstartlstm_parallel, headstartlstm_recurrent
 from .lm import TokenLogprobs, embedding, gated_recurrence, gated_recurrence_step, token_logprobs
+from .cross_entropy import linear_cross_entropy
 from .selective import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from ._lib import (check_errors, last_recurrent_path, set_exchange_scope, set_recurrent_path, set_spin_timeout_us,
                    set_split_products)
@@ -109,5 +110,6 @@ __all__ = [
     "check_errors",
     "embedding", "gated_recurrence", "gated_recurrence_step", "token_logprobs", "TokenLogprobs",
     "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step",
+    "linear_cross_entropy",
     "__version__",
 ]

@@ -86,6 +86,9 @@ SIGNATURES = {
     "hsl_selective_bwd": (_I, [_P, _L, _L] * 2 + [_P] + [_P, _L, _L] * 2 + [_P, _P, _L, _L, _P, _P, _L, _L, _P]
                           + [_P, _L, _L, _P] + [_P, _L, _L] * 2 + [_P] + [_P, _L, _L] * 2 + [_P]
                           + [_P, _L, _L, _P, _P, _I, _P, _Z] + [_I] * 5 + [_P]),
+    "hsl_xent_ws_bytes": (_Z, [_L, _I, _I, _I, _I]),
+    "hsl_xent_fwd": (_I, [_P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _Z, _L, _I, _I, _I, _P]),
+    "hsl_xent_bwd": (_I, [_P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _P, _P, _P, _Z, _L, _I, _I, _I, _P]),
 }
 
 _lock = threading.Lock()

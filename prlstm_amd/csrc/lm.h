@@ -146,6 +146,35 @@ __device__ __forceinline__ long long load_id(const void* ids, int ids64, size_t 
   return ids64 ? static_cast<const long long*>(ids)[i] : (long long)static_cast<const int*>(ids)[i];
 }
 
+// Sums over lanes that many values need at once: an exchange of halves between two registers and an
+// addition leave one register with half of each value's lanes, so n values take about 2 n operations
+// where a sum of each alone takes 6 n.
+// Lower half-wave: a over lanes l and l + 32; upper half-wave: b.
+__device__ __forceinline__ float add32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Even rows of 16 lanes: a over the pair of rows; odd rows: b.
+__device__ __forceinline__ float add16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// r[i] over the 16 lanes of a row, i = lane % 16.
+__device__ __forceinline__ float sum_rows(float (&r)[16], int lane) {
+  const bool b8 = lane & 8, b4 = lane & 4, b2 = lane & 2, b1 = lane & 1;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (b8 ? r[i + 8] : r[i]) + lane_move<0x128>(b8 ? r[i] : r[i + 8]);  // row_ror:8
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = (b4 ? r[i + 4] : r[i]) + lane_move<0x141>(b4 ? r[i] : r[i + 4]);  // half mirror
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r[i] = (b2 ? r[i + 2] : r[i]) + lane_move<0x4e>(b2 ? r[i] : r[i + 2]);  // quad 2,3,0,1
+  return (b1 ? r[1] : r[0]) + lane_move<0xb1>(b1 ? r[0] : r[1]);                                       // quad 1,0,3,2
+}
+
 // f(integral_constant<int, fmt>) for the element format of a call.
 template <class Fn>
 int with_fmt(int fmt, Fn f) {

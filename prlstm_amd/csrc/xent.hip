@@ -1,0 +1,802 @@
+// Cross entropy of a projection on the vocabulary, without keeping the logits:
+//   l[n][v] = x[n] . w[v] + bias[v],   loss[n] = log sum_v exp l[n][v] - l[n][target[n]],
+//   dl[n][v] = g[n] (exp(l[n][v]) / sum - [v = target[n]]),   g = dloss (0 for a target < 0),
+//   dx = dl w,   dw = dl^T x,   dbias = sum_n dl.
+//
+// 16-bit operands: one kernel multiplies 256 x 256 tiles (mm16.h) whose rows are tokens of the
+// vocabulary and whose columns are the positions, so that a lane has 64 logits of one position in
+// registers.  The forward reduces them to the tile's largest logit and sum of exponentials, from which a
+// second kernel makes the loss; no logit leaves the registers.  The backward computes the logits again,
+// a piece of the vocabulary at a time, and writes the piece's dl, rounded to 16 bits (as every operand
+// of a product on these instructions is; its error of half a step is what rounding dx and dw once costs
+// again), from which one launch makes the piece's dw and adds to dx, both in fp32.
+// fp32 operands: pieces of the logits are products on the library's fp32 kernels, kept in fp32.
+#include <algorithm>
+
+#include "mm16.h"
+
+namespace hsl {
+namespace {
+
+constexpr float kLog2eX = 1.44269502162933349609375f;
+constexpr size_t kPieceBytes = 128u << 20;  // of a piece's dl: what the last-level cache keeps beside its operands
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// A row of nothing but masks (m is -inf beside a sum of NaN where every logit is NaN).
+__device__ __forceinline__ bool all_masked(float m, float s) { return m == neg_inf() && s == 0.f; }
+
+// Joins (m, sum exp(l - m)) of two parts of a row.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float big = fmaxf(m, m2), r = big == neg_inf() ? 0.f : big;
+  s = s * __builtin_amdgcn_exp2f((m - r) * kLog2eX) + s2 * __builtin_amdgcn_exp2f((m2 - r) * kLog2eX);
+  m = big;
+}
+
+struct LogitArgs {
+  MmOperand w, x;   // from the piece's first token on; from the first position on
+  const float* bias;
+  const int* target;  // the positions' targets (of the whole vocabulary)
+  int v_first;        // the piece's first token
+  int V, N, D, tiles_v, tiles_n;
+  float2* part;     // [tile_v][N]: forward
+  float* own;       // [N]: the target's logit
+  // backward
+  const float4* rows;  // [N]: m, 1 / sum, g (scaled), -
+  unsigned short* dl;  // [N][tiles_v * 256]
+  float* dbias;        // [tile_n][tiles_v * 256], or null
+};
+
+__device__ __forceinline__ void xent_tile_order(int tiles_m, int tiles_n, int id, int* tm, int* tn) {
+  // workgroup i runs on XCD i % 8: each XCD takes a contiguous range of the tiles, which go down 8 row
+  // panels before they move to the next column
+  const int total = tiles_m * tiles_n, even = total & ~7;
+  if (id < even) id = (id % 8) * (even / 8) + id / 8;
+  constexpr int GM = 8;
+  const int group = id / (GM * tiles_n), first = group * GM, rows = min(GM, tiles_m - first);
+  const int in = id - group * GM * tiles_n;
+  *tm = first + in % rows;
+  *tn = in / rows;
+}
+
+// The logits of the lane's 64 tokens and 2 positions, bias added; -inf for tokens beyond the vocabulary.
+__device__ __forceinline__ void finish_logits(const LogitArgs& a, int v0, f16v (&acc)[4][2]) {
+  if (!a.bias && v0 + 128 <= a.V) return;
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int v = v0 + i * 32 + 8 * q + 4 * half;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = v + e < a.V;
+        const float add = a.bias && in ? a.bias[v + e] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j][4 * q + e] = in ? acc[i][j][4 * q + e] + add : neg_inf();
+      }
+    }
+}
+
+__device__ __forceinline__ MmOperand tile_rows(const MmOperand& o, int first) {
+  return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), o.k};
+}
+
+template <bool FP16>
+__global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
+  int tv, tn;
+  xent_tile_order(a.tiles_v, a.tiles_n, blockIdx.x, &tv, &tn);
+  f16v acc[4][2];
+  mm_tile<FP16, false, false>(tile_rows(a.w, tv * kMmTile), tile_rows(a.x, tn * kMmTile),
+                              (a.D + kMmSlice - 1) / kMmSlice, lds, acc);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int v0 = tv * kMmTile + (wave >> 2) * 128, c0 = (wave & 3) * 64 + (lane & 31);
+  finish_logits(a, v0, acc);
+  float2(*const sm)[kMmTile] = reinterpret_cast<float2(*)[kMmTile]>(lds);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * kMmTile + c0 + j * 32;
+    const int own = n < a.N ? a.target[n] - a.v_first - v0 - 4 * half : -1;
+    float m = neg_inf();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+    if (__any((unsigned)own < 128u)) {  // few waves have a target among their tokens
+      float l = 0.f;
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (own == i * 32 + 8 * (r >> 2) + (r & 3)) {
+            l = acc[i][j][r];
+            found = true;
+          }
+      if (found) a.own[n] = l;
+    }
+    const float ref = m == neg_inf() ? 0.f : m;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2eX);
+    join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
+    if (half == 0) sm[wave >> 2][c0 + j * 32] = float2{m, s};
+  }
+  __syncthreads();
+  const int c = threadIdx.x, n = tn * kMmTile + c;
+  if (c < kMmTile && n < a.N) {
+    float2 p = sm[0][c];
+    join(p.x, p.y, sm[1][c].x, sm[1][c].y);
+    a.part[(size_t)tv * a.N + n] = p;
+  }
+}
+
+// Targets as 32-bit numbers (-1: not scored, -2: beyond the vocabulary).
+__global__ __launch_bounds__(256) void xent_targets_kernel(const void* targets, int tgt64, int* out, int N, int V) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  const long long t = load_id(targets, tgt64, n);
+  out[n] = t < 0 ? -1 : t >= V ? -2 : (int)t;
+}
+
+// The loss and the row's (m, sum exp(l - m)) from its tiles' parts: 32 positions by 8 strips of the tiles.
+__global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ own,
+                                                        const int* __restrict__ target, float* loss, float2* stats,
+                                                        unsigned* err, int N, int tiles) {
+  __shared__ float2 sm[8][32];
+  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+  float m = neg_inf(), s = 0.f;
+  if (n < N)
+    for (int t = strip; t < tiles; t += 8) {
+      const float2 p = part[(size_t)t * N + n];
+      join(m, s, p.x, p.y);
+    }
+  sm[strip][c] = float2{m, s};
+  __syncthreads();
+  if (strip || n >= N) return;
+  for (int k = 1; k < 8; ++k) join(m, s, sm[k][c].x, sm[k][c].y);
+  stats[n] = float2{m, s};
+  const bool masked = all_masked(m, s);
+  const int t = target[n];
+  float v = 0.f;
+  if (t >= 0)
+    v = masked ? __builtin_inff() : (m - own[n]) + logf(s);
+  else if (t == -2) {
+    v = __builtin_nanf("");
+    atomicOr(err, kErrId);
+  }
+  loss[n] = v;
+}
+
+
+// A power of two that brings the largest |dloss| to 2^14 .. 2^15, and its inverse: fp16 has 2^-14 for
+// its smallest normal number, and the gradients of a mean over thousands of rows are far below it.
+__global__ __launch_bounds__(1024) void xent_scale_kernel(const float* dloss, float* scale, int N) {
+  __shared__ float sm[16];
+  float m = 0.f;
+  for (long long n = threadIdx.x; n < N; n += 1024) m = fmaxf(m, __builtin_fabsf(dloss[n]));
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) m = fmaxf(m, __shfl_xor(m, k));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int k = 1; k < 16; ++k) m = fmaxf(m, sm[k]);
+  const int e = m == 0.f ? 14 : (int)(__float_as_uint(m) >> 23) - 127;
+  const int up = min(100, max(-100, 14 - e));
+  scale[0] = __uint_as_float((unsigned)(127 + up) << 23);
+  scale[1] = __uint_as_float((unsigned)(127 - up) << 23);
+}
+
+// What the backward needs of each row.  No gradient where the target is outside of the vocabulary or
+// nothing but masks is in the row.
+__global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ stats, const int* __restrict__ target,
+                                                        const float* __restrict__ dloss, const float* scale,
+                                                        float4* rows, int N) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  const float2 s = stats[n];
+  const bool on = target[n] >= 0 && !all_masked(s.x, s.y);
+  rows[n] = float4{s.x, 1.f / s.y, on ? dloss[n] * (scale ? scale[0] : 1.f) : 0.f, 0.f};
+}
+
+// dl of one logit: nothing for a masked one, whatever arrives.
+__device__ __forceinline__ float dlogit(float l, const float4& row, float gi) {
+  const float d = __builtin_amdgcn_exp2f((l - row.x) * kLog2eX) * gi;
+  return l == neg_inf() ? 0.f : d;
+}
+
+constexpr int kDlRow = kMmTile * 2 + 16;  // bytes of a position's row in LDS
+
+template <bool FP16>
+__global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kMmTile * kDlRow];
+  __shared__ float sums[4][kMmTile];
+  static_assert(sizeof(lds) >= kMmLds, "the slices' place");
+  int tv, tn;
+  xent_tile_order(a.tiles_v, a.tiles_n, blockIdx.x, &tv, &tn);
+  f16v acc[4][2];
+  mm_tile<FP16, false, false>(tile_rows(a.w, tv * kMmTile), tile_rows(a.x, tn * kMmTile),
+                              (a.D + kMmSlice - 1) / kMmSlice, lds, acc);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int vw = (wave >> 2) * 128, v0 = tv * kMmTile + vw, c0 = (wave & 3) * 64 + (lane & 31);
+  finish_logits(a, v0, acc);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int n = tn * kMmTile + c0 + j * 32;
+    const float4 row = n < a.N ? a.rows[n] : float4{0.f, 0.f, 0.f, 0.f};
+    const int own = n < a.N ? a.target[n] - a.v_first - v0 - 4 * half : -1;
+    const float gi = row.z * row.y;
+    const bool on = row.z != 0.f;  // NaN is on
+    const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
+    float hot = row.z;
+    if (owns) {  // a masked target has no gradient either
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (own == i * 32 + 8 * (r >> 2) + (r & 3) && acc[i][j][r] == neg_inf()) hot = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float d = dlogit(acc[i][j][r], row, gi);
+        acc[i][j][r] = on ? d : 0.f;
+      }
+    if (owns) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] -= own == i * 32 + 8 * (r >> 2) + (r & 3) ? hot : 0.f;
+    }
+    char* const p = lds + (c0 + j * 32) * kDlRow + (vw + 4 * half) * 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float f[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        unsigned short h[4];
+        down_all<FP16 ? kElemF16 : kElemBf16, 4>(f, h);
+        __builtin_memcpy(__builtin_assume_aligned(p + (i * 32 + 8 * q) * 2, 8), h, 8);
+      }
+  }
+  if (a.dbias) {  // in fp32, from before the rounding
+    float f[2][16];
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      const int u = 2 * k, i = u / 16, r = u % 16;
+      f[k / 16][k % 16] = add16(acc[i][0][r] + acc[i][1][r], acc[i][0][r + 1] + acc[i][1][r + 1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float v = sum_rows(f[k], lane);
+      const int u = 2 * (16 * k + (lane & 15)) + ((lane >> 4) & 1), i = u / 16, r = u % 16;
+      sums[wave & 3][vw + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3)] = v;
+    }
+  }
+  __syncthreads();
+  const long long ld = (long long)a.tiles_v * kMmTile;
+  for (int p = threadIdx.x; p < kMmTile * 32; p += kMmThreads) {
+    const int c = p >> 5, n = tn * kMmTile + c;
+    if (n >= a.N) break;
+    const mm_u4 v = *reinterpret_cast<const mm_u4*>(lds + c * kDlRow + (p & 31) * 16);
+    *reinterpret_cast<mm_u4*>(a.dl + n * ld + tv * kMmTile + (p & 31) * 8) = v;
+  }
+  if (a.dbias && threadIdx.x < kMmTile) {
+    const int c = threadIdx.x;
+    a.dbias[(size_t)tn * ld + tv * kMmTile + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  }
+}
+
+// dbias of a piece from its tiles' sums, in fp64.
+__global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict__ part, const float* scale, float* dbias,
+                                                        int V, long long ld, int tiles) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  double s = 0.0;
+  for (int t = 0; t < tiles; ++t) s += part[t * ld + v];
+  dbias[v] = (float)(scale ? s * scale[1] : s);
+}
+
+struct OutArgs {
+  const unsigned short *dl, *w, *x;
+  long long ld, ldw, ldx;   // of dl (the piece's padded width), w and x
+  float *dx, *dw;           // planes [split][N][D] and [split][ld][D]; dw null: straight to dw16
+  unsigned short* dw16;
+  const float* scale;
+  int N, V, D, Dk;          // V: the piece's tokens; Dk: the width that x and w have in memory
+  int tiles_n, tiles_d, tiles_v, splits_x, splits_w, k_x, k_w, add;
+};
+
+// One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.
+template <bool FP16>
+__global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
+  const int count_x = a.splits_x * a.tiles_n * a.tiles_d;
+  const bool is_x = (int)blockIdx.x < count_x;
+  int id = is_x ? blockIdx.x : blockIdx.x - count_x;
+  const int td = id % a.tiles_d;
+  id /= a.tiles_d;
+  const int tiles = is_x ? a.tiles_n : a.tiles_v, tm = id % tiles, split = id / tiles;
+  f16v acc[4][2];
+  const int dcols = a.Dk - td * kMmTile;
+  if (is_x) {
+    const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
+    const MmOperand A{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
+    const MmOperand B{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
+    mm_tile<FP16, false, true>(A, B, (k1 - k0 + kMmSlice - 1) / kMmSlice, lds, acc);
+  } else {
+    const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
+    const MmOperand A{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
+    const MmOperand B{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
+    mm_tile<FP16, true, true>(A, B, (k1 - k0 + kMmSlice - 1) / kMmSlice, lds, acc);
+  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int r0 = tm * kMmTile + (wave >> 2) * 128 + 4 * half, c0 = td * kMmTile + (wave & 3) * 64 + (lane & 31);
+  const int rows = is_x ? a.N : a.V;
+  const float back = a.scale ? a.scale[1] : 1.f;
+  float* const plane = is_x ? a.dx + (size_t)split * a.N * a.D : a.dw ? a.dw + (size_t)split * a.ld * a.D : nullptr;
+  const bool add = is_x && a.add;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int row = r0 + i * 32 + 8 * (r >> 2) + (r & 3);
+      if (row >= rows) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = c0 + j * 32;
+        if (c >= a.D) continue;
+        const size_t at = (size_t)row * a.D + c;
+        if (plane)
+          plane[at] = add ? plane[at] + acc[i][j][r] : acc[i][j][r];
+        else
+          a.dw16[at] = Elem<FP16 ? kElemF16 : kElemBf16>::down(acc[i][j][r] * back);
+      }
+    }
+}
+
+// out = the planes' sum, in their order.
+template <int F>
+__global__ __launch_bounds__(256) void xent_planes_kernel(const float* __restrict__ planes, size_t plane, int splits,
+                                                          const float* scale, void* out, size_t n) {
+  using T_ = typename Elem<F>::T;
+  const float back = scale ? scale[1] : 1.f;
+  const size_t stride = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+    float v = planes[i];
+    for (int s = 1; s < splits; ++s) v += planes[s * plane + i];
+    static_cast<T_*>(out)[i] = Elem<F>::down(v * back);
+  }
+}
+
+template <int F>
+__global__ __launch_bounds__(256) void xent_zero_kernel(void* out, size_t n) {
+  const size_t stride = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride)
+    static_cast<typename Elem<F>::T*>(out)[i] = typename Elem<F>::T{};
+}
+
+// Rows of 16-bit elements with zeros up to a width that is a multiple of 8.
+__global__ __launch_bounds__(256) void xent_pack_kernel(const unsigned short* __restrict__ src, long long ld,
+                                                        unsigned short* dst, long long rows, int cols, int width) {
+  const size_t all = (size_t)rows * width, stride = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < all; i += stride) {
+    const size_t r = i / width;
+    const int c = (int)(i - r * width);
+    dst[i] = c < cols ? src[(long long)r * ld + c] : (unsigned short)0;
+  }
+}
+
+// ---- fp32 operands ------------------------------------------------------------------------
+
+// Joins a piece of the logits [N][ld] with what the pieces before it gave, a workgroup a row.
+__global__ __launch_bounds__(256) void xent_f32_stats_kernel(const float* __restrict__ l, long long ld, int V, int v0,
+                                                             const int* __restrict__ target, float2* stats, float* own,
+                                                             int first) {
+  __shared__ float2 sm[4];
+  const int n = blockIdx.x;
+  const float* const row = l + n * ld;
+  float m = neg_inf(), s = 0.f;
+  for (int v = threadIdx.x; v < V; v += 256) {
+    const float x = row[v];
+    const float big = fmaxf(m, x), r = big == neg_inf() ? 0.f : big;
+    s = s * __builtin_amdgcn_exp2f((m - r) * kLog2eX) + exp_f(x - r);
+    m = big;
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) join(m, s, __shfl_xor(m, k), __shfl_xor(s, k));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = float2{m, s};
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int k = 1; k < 4; ++k) join(m, s, sm[k].x, sm[k].y);
+  if (!first) {
+    const float2 p = stats[n];
+    float m0 = p.x, s0 = p.y;
+    join(m0, s0, m, s);
+    m = m0;
+    s = s0;
+  }
+  stats[n] = float2{m, s};
+  const int t = target[n] - v0;
+  if (t >= 0 && t < V) own[n] = row[t];
+}
+
+// dl of a piece in place of its logits.
+__global__ __launch_bounds__(256) void xent_f32_grad_kernel(float* __restrict__ l, long long ld, int V, int v0,
+                                                            const int* __restrict__ target,
+                                                            const float4* __restrict__ rows) {
+  const int n = blockIdx.x;
+  float* const p = l + n * ld;
+  const float4 row = rows[n];
+  const int own = target[n] - v0;
+  const float gi = row.z * row.y;
+  for (int v = threadIdx.x; v < V; v += 256) {
+    const float x = p[v];
+    float d = exp_f(x - row.x) * gi;
+    if (v == own) d -= row.z;
+    p[v] = row.z == 0.f || x == neg_inf() ? 0.f : d;
+  }
+}
+
+// Sums of columns of [N][ld]: 64 columns a workgroup, 4 strips of the rows, in fp64.
+__global__ __launch_bounds__(256) void xent_f32_bias_kernel(const float* __restrict__ l, long long ld, float* dbias,
+                                                            int V, int N) {
+  __shared__ double sm[4][64];
+  const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, v = blockIdx.x * 64 + c;
+  double s = 0.0;
+  if (v < V)
+    for (int n = strip; n < N; n += 4) s += l[n * ld + v];
+  sm[strip][c] = s;
+  __syncthreads();
+  if (strip == 0 && v < V) dbias[v] = (float)((sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]));
+}
+
+__global__ __launch_bounds__(256) void xent_f32_add_kernel(float* __restrict__ out, const float* __restrict__ v,
+                                                           size_t n) {
+  const size_t stride = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) out[i] += v[i];
+}
+
+// ---- host ---------------------------------------------------------------------------------
+
+int up_to(long long n, int unit) { return (int)((n + unit - 1) / unit * unit); }
+unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 1 << 16); }
+
+struct XentPlan {
+  int piece, pieces;  // tokens of a piece: a multiple of 256
+  int tiles_n, tiles_d, tiles_v;
+  int splits_x, splits_w, k_x, k_w;
+};
+XentPlan plan_xent(int N, int V, int D, int fmt) {
+  XentPlan p;
+  const size_t es = fmt == kElemF32 ? 4 : 2;
+  const int all = up_to(V, kMmTile);
+  const long long fit = std::max<long long>(1, (long long)(kPieceBytes / es / std::max(1, N)) / kMmTile) * kMmTile;
+  p.piece = (int)std::min<long long>(all, fit);
+  p.pieces = (all + p.piece - 1) / p.piece;
+  p.piece = up_to((all + p.pieces - 1) / p.pieces, kMmTile);
+  p.pieces = (all + p.piece - 1) / p.piece;
+  p.tiles_n = (N + kMmTile - 1) / kMmTile;
+  p.tiles_d = (D + kMmTile - 1) / kMmTile;
+  p.tiles_v = p.piece / kMmTile;
+  // k of a workgroup such that the two products' work makes about 256 equal shares
+  const double total = (double)p.tiles_d * ((double)p.tiles_n * p.piece + (double)p.tiles_v * N);
+  const int share = std::max(512, (int)std::min(1e9, total / 256));
+  auto split = [&](int k, int* splits, int* each) {
+    *splits = std::max(1, (int)(((long long)k + share / 2) / share));
+    *each = std::max(kMmSlice, up_to((k + *splits - 1) / *splits, kMmSlice));
+    *splits = std::max(1, (k + *each - 1) / *each);
+  };
+  split(p.piece, &p.splits_x, &p.k_x);
+  split(N, &p.splits_w, &p.k_w);
+  return p;
+}
+
+int check_xent(const char* who, long long N, int V, int D, int fmt) {
+  if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
+  if (N < 0 || V < 0 || D < 0) return fail(HSL_ERR_ARG, "%s: negative size (N=%lld V=%d D=%d)", who, N, V, D);
+  if (V == 0 || D == 0) return fail(HSL_ERR_ARG, "%s: an empty projection (V=%d D=%d)", who, V, D);
+  // a launch holds fewer than 2^32 threads, and rows of a tile lie within 2^31 bytes
+  if (N >= (1ll << 31) - 256 || V >= 0x7fffffff - 256 || D >= (1 << 20) ||
+      ((N + 255) / 256) * (((long long)V + 255) / 256) >= (1ll << 22) ||
+      ((N + 255) / 256 + ((long long)V + 255) / 256) * ((D + 255) / 256) >= (1ll << 22))
+    return fail(HSL_ERR_UNSUPPORTED,
+                "%s: N=%lld V=%d D=%d is beyond one launch (needs D < 2^20 and fewer than 2^22 tiles of 256 x 256 of "
+                "each product)",
+                who, N, V, D);
+  return HSL_OK;
+}
+
+int check_rows(const char* who, long long ldx, long long ldw, int D) {
+  if (ldx < D || ldw < D || ldx >= (1ll << 31) || ldw >= (1ll << 31))
+    return fail(HSL_ERR_ARG, "%s: row strides %lld and %lld, must be D=%d or more and below 2^31", who, ldx, ldw, D);
+  return HSL_OK;
+}
+
+// The pieces of a call's workspace.  base = nullptr: to find its size.
+struct XentSpace {
+  int* target;
+  float* own;
+  float2* part;
+  float4* rows;
+  float* scale;
+  unsigned short *packed_x, *packed_w;
+  char* dl;  // 16-bit dl, or fp32 logits
+  float *bias, *dx, *dw;
+  void* gemm;
+  size_t gemm_bytes, bytes;
+};
+constexpr size_t kGemmRoom = 64u << 20;
+
+XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
+  XentSpace s{};
+  const XentPlan p = plan_xent(N, V, D, fmt);
+  Carver c(base, 0);
+  s.target = c.take<int>(N);
+  if (!backward) {
+    s.own = c.take<float>(N);
+    s.part = c.take<float2>(fmt == kElemF32 ? (size_t)N : (size_t)N * ((V + kMmTile - 1) / kMmTile));
+  } else {
+    s.rows = c.take<float4>(N);
+    s.scale = c.take<float>(2);
+  }
+  if (fmt == kElemF32) {
+    s.dl = c.take<char>((size_t)N * p.piece * 4);
+    if (backward) s.dx = c.take<float>((size_t)N * D);
+    s.gemm_bytes = kGemmRoom;
+    s.gemm = c.take<char>(kGemmRoom);
+  } else {
+    s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
+    s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
+    if (backward) {
+      s.dl = c.take<char>((size_t)N * p.piece * 2);
+      s.bias = c.take<float>((size_t)p.tiles_n * p.piece);
+      s.dx = c.take<float>((size_t)p.splits_x * N * D);
+      if (p.splits_w > 1) s.dw = c.take<float>((size_t)p.splits_w * p.piece * D);
+    }
+  }
+  s.bytes = c.off;
+  return s;
+}
+
+// 16-bit operands as the tiles read them: rows of a multiple of 8 elements at 16-byte steps.
+struct XentOperands {
+  const unsigned short *x, *w;
+  long long ldx, ldw;
+  int width;
+};
+bool tiles_read(const void* p, long long ld, int D) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 21) && D % 8 == 0;
+}
+int xent_operands(const void* x, long long ldx, const void* w, long long ldw, const XentSpace& s, int N, int V, int D,
+                  hipStream_t st, XentOperands* o) {
+  o->width = up_to(D, 8);
+  o->x = static_cast<const unsigned short*>(x);
+  o->w = static_cast<const unsigned short*>(w);
+  o->ldx = ldx;
+  o->ldw = ldw;
+  if (!tiles_read(x, ldx, D)) {
+    hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)N * o->width)), dim3(256), 0, st, o->x, ldx, s.packed_x,
+                       (long long)N, D, o->width);
+    o->x = s.packed_x;
+    o->ldx = o->width;
+  }
+  if (!tiles_read(w, ldw, D)) {
+    hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)V * o->width)), dim3(256), 0, st, o->w, ldw, s.packed_w,
+                       (long long)V, D, o->width);
+    o->w = s.packed_w;
+    o->ldw = o->width;
+  }
+  HSL_HIP(hipGetLastError());
+  return HSL_OK;
+}
+
+GemmDesc f32_product(const float* A, const float* B, const float* bias, float* C, int M, int N, int K, int lda, int ldb,
+                     int ldc, int trans_a, int trans_b, int acc64) {
+  return GemmDesc{A, B, bias, C, M, N, K, lda, ldb, ldc, trans_a, trans_b, acc64};
+}
+
+}  // namespace
+}  // namespace hsl
+
+using namespace hsl;
+
+extern "C" {
+
+size_t hsl_xent_ws_bytes(long long N, int V, int D, int fmt, int backward) {
+  if (check_xent("hsl_xent_ws_bytes", N, V, D, fmt) != HSL_OK || N == 0) return 0;
+  return xent_space(nullptr, (int)N, V, D, fmt, backward != 0).bytes;
+}
+
+int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* targets,
+                 int tgt64, float* loss, float* stats, void* ws, size_t ws_bytes, long long N, int V, int D, int fmt,
+                 void* stream) {
+  HSL_CHECK(check_xent("hsl_xent_fwd", N, V, D, fmt));
+  if (N == 0) return HSL_OK;
+  if (!targets || !loss || !stats || !x || !w) return fail(HSL_ERR_ARG, "hsl_xent_fwd: null pointer");
+  HSL_CHECK(check_rows("hsl_xent_fwd", ldx, ldw, D));
+  const int n = (int)N;
+  XentSpace s = xent_space(ws, n, V, D, fmt, false);
+  if (!ws || ws_bytes < s.bytes)
+    return fail(HSL_ERR_ARG, "hsl_xent_fwd: workspace %zu bytes, need %zu", ws_bytes, s.bytes);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  unsigned* err = nullptr;
+  HSL_CHECK(device_error_word(&err));
+  hipLaunchKernelGGL(xent_targets_kernel, dim3((n + 255) / 256), dim3(256), 0, st, targets, tgt64, s.target, n, V);
+  int tiles = 1;
+  if (fmt == kElemF32) {
+    const XentPlan p = plan_xent(n, V, D, fmt);
+    for (int v0 = 0; v0 < V; v0 += p.piece) {
+      const int v = std::min(p.piece, V - v0);
+      float* const l = reinterpret_cast<float*>(s.dl);
+      HSL_CHECK(gemm_run(f32_product(static_cast<const float*>(x), static_cast<const float*>(w) + v0 * ldw,
+                                     bias ? bias + v0 : nullptr, l, n, v, D, (int)ldx, (int)ldw, p.piece, 0, 1, 0),
+                         s.gemm, s.gemm_bytes, st));
+      hipLaunchKernelGGL(xent_f32_stats_kernel, dim3(n), dim3(256), 0, st, l, (long long)p.piece, v, v0, s.target,
+                         s.part, s.own, v0 == 0);
+    }
+  } else {
+    XentOperands o;
+    HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
+    LogitArgs a{};
+    a.w = {o.w, o.ldw, V, o.width};
+    a.x = {o.x, o.ldx, n, o.width};
+    a.bias = bias;
+    a.target = s.target;
+    a.V = V;
+    a.N = n;
+    a.D = D;
+    a.tiles_v = tiles = (V + kMmTile - 1) / kMmTile;
+    a.tiles_n = (n + kMmTile - 1) / kMmTile;
+    a.part = s.part;
+    a.own = s.own;
+    const dim3 grid(a.tiles_v * a.tiles_n), block(kMmThreads);
+    if (fmt == kElemF16)
+      hipLaunchKernelGGL(xent_stats_kernel<true>, grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL(xent_stats_kernel<false>, grid, block, 0, st, a);
+  }
+  hipLaunchKernelGGL(xent_join_kernel, dim3((n + 31) / 32), dim3(256), 0, st, s.part, s.own, s.target, loss,
+                     reinterpret_cast<float2*>(stats), err, n, tiles);
+  HSL_HIP(hipGetLastError());
+  return HSL_OK;
+}
+
+int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias, const void* targets,
+                 int tgt64, const float* stats, const float* dloss, void* dx, void* dw, float* dbias, void* ws,
+                 size_t ws_bytes, long long N, int V, int D, int fmt, void* stream) {
+  HSL_CHECK(check_xent("hsl_xent_bwd", N, V, D, fmt));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int n = (int)N;
+  if (N > 0 && (!targets || !stats || !dloss || !x || !w))
+    return fail(HSL_ERR_ARG, "hsl_xent_bwd: null pointer");
+  if (N > 0) HSL_CHECK(check_rows("hsl_xent_bwd", ldx, ldw, D));
+  const XentPlan p = plan_xent(n, V, D, fmt);
+  XentSpace s = xent_space(ws, n, V, D, fmt, true);
+  if (N > 0 && (!ws || ws_bytes < s.bytes))
+    return fail(HSL_ERR_ARG, "hsl_xent_bwd: workspace %zu bytes, need %zu", ws_bytes, s.bytes);
+  if (N == 0) {  // no position: the weights' gradients are zeros
+    if (!dw && !dbias) return HSL_OK;
+    const size_t count = (size_t)V * D;
+    if (dw) {
+      HSL_CHECK(with_fmt(fmt, [&](auto F) {
+        hipLaunchKernelGGL((xent_zero_kernel<decltype(F)::value>), dim3(grid_of(count)), dim3(256), 0, st, dw, count);
+        HSL_HIP(hipGetLastError());
+        return (int)HSL_OK;
+      }));
+    }
+    if (dbias) hipLaunchKernelGGL((xent_zero_kernel<kElemF32>), dim3(grid_of(V)), dim3(256), 0, st, dbias, (size_t)V);
+    HSL_HIP(hipGetLastError());
+    return HSL_OK;
+  }
+  const float* scale = nullptr;
+  if (fmt == kElemF16) {
+    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, dloss, s.scale, n);
+    scale = s.scale;
+  }
+  hipLaunchKernelGGL(xent_targets_kernel, dim3((n + 255) / 256), dim3(256), 0, st, targets, tgt64, s.target, n, V);
+  hipLaunchKernelGGL(xent_rows_kernel, dim3((n + 255) / 256), dim3(256), 0, st,
+                     reinterpret_cast<const float2*>(stats), s.target, dloss, scale, s.rows, n);
+  HSL_HIP(hipGetLastError());
+  if (fmt == kElemF32) {
+    float* const l = reinterpret_cast<float*>(s.dl);
+    const float *xf = static_cast<const float*>(x), *wf = static_cast<const float*>(w);
+    for (int v0 = 0; v0 < V; v0 += p.piece) {
+      const int v = std::min(p.piece, V - v0);
+      HSL_CHECK(gemm_run(f32_product(xf, wf + v0 * ldw, bias ? bias + v0 : nullptr, l, n, v, D, (int)ldx, (int)ldw,
+                                     p.piece, 0, 1, 0),
+                         s.gemm, s.gemm_bytes, st));
+      hipLaunchKernelGGL(xent_f32_grad_kernel, dim3(n), dim3(256), 0, st, l, (long long)p.piece, v, v0, s.target,
+                         s.rows);
+      if (dbias)
+        hipLaunchKernelGGL(xent_f32_bias_kernel, dim3((v + 63) / 64), dim3(256), 0, st, l, (long long)p.piece,
+                           dbias + v0, v, n);
+      if (dx) {
+        float* const out = v0 ? s.dx : static_cast<float*>(dx);
+        HSL_CHECK(gemm_run(f32_product(l, wf + v0 * ldw, nullptr, out, n, D, v, p.piece, (int)ldw, D, 0, 0, 1),
+                           s.gemm, s.gemm_bytes, st));
+        if (v0)
+          hipLaunchKernelGGL(xent_f32_add_kernel, dim3(grid_of((size_t)n * D)), dim3(256), 0, st,
+                             static_cast<float*>(dx), s.dx, (size_t)n * D);
+      }
+      if (dw)
+        HSL_CHECK(gemm_run(f32_product(l, xf, nullptr, static_cast<float*>(dw) + (size_t)v0 * D, v, D, n, p.piece,
+                                       (int)ldx, D, 1, 0, 1),
+                           s.gemm, s.gemm_bytes, st));
+      HSL_HIP(hipGetLastError());
+    }
+    return HSL_OK;
+  }
+  XentOperands o;
+  HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
+  for (int v0 = 0; v0 < V; v0 += p.piece) {
+    const int v = std::min(p.piece, V - v0);
+    const int tiles_v = (v + kMmTile - 1) / kMmTile;  // the last piece may have fewer
+    LogitArgs a{};
+    a.w = {o.w + v0 * o.ldw, o.ldw, v, o.width};
+    a.x = {o.x, o.ldx, n, o.width};
+    a.bias = bias ? bias + v0 : nullptr;
+    a.target = s.target;
+    a.v_first = v0;
+    a.V = v;
+    a.N = n;
+    a.D = D;
+    a.tiles_v = tiles_v;
+    a.tiles_n = p.tiles_n;
+    a.rows = s.rows;
+    a.dl = reinterpret_cast<unsigned short*>(s.dl);
+    a.dbias = dbias ? s.bias : nullptr;
+    OutArgs g{};
+    g.dl = a.dl;
+    g.w = a.w.p;
+    g.x = o.x;
+    g.ld = (long long)tiles_v * kMmTile;
+    g.ldw = o.ldw;
+    g.ldx = o.ldx;
+    g.dx = s.dx;
+    g.dw = p.splits_w > 1 ? s.dw : nullptr;
+    g.dw16 = static_cast<unsigned short*>(dw) + (size_t)v0 * D;
+    g.scale = scale;
+    g.N = n;
+    g.V = v;
+    g.D = D;
+    g.Dk = o.width;
+    g.tiles_n = p.tiles_n;
+    g.tiles_d = p.tiles_d;
+    g.tiles_v = tiles_v;
+    g.splits_x = dx ? p.splits_x : 0;
+    g.splits_w = dw ? p.splits_w : 0;
+    g.k_x = p.k_x;
+    g.k_w = p.k_w;
+    g.add = v0 > 0;
+    const dim3 grid(tiles_v * p.tiles_n), block(kMmThreads);
+    const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
+    if (fmt == kElemF16) {
+      hipLaunchKernelGGL(xent_grad_kernel<true>, grid, block, 0, st, a);
+      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<true>, grid_out, block, 0, st, g);
+    } else {
+      hipLaunchKernelGGL(xent_grad_kernel<false>, grid, block, 0, st, a);
+      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<false>, grid_out, block, 0, st, g);
+    }
+    if (dbias)
+      hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 255) / 256), dim3(256), 0, st, s.bias, scale, dbias + v0, v, g.ld,
+                         p.tiles_n);
+    if (dw && g.dw)
+      hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>,
+                         dim3(grid_of((size_t)v * D)), dim3(256), 0, st, s.dw, (size_t)g.ld * D, p.splits_w, scale,
+                         static_cast<void*>(g.dw16), (size_t)v * D);
+    HSL_HIP(hipGetLastError());
+  }
+  if (dx)
+    hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>,
+                       dim3(grid_of((size_t)n * D)), dim3(256), 0, st, s.dx, (size_t)n * D, p.splits_x, scale, dx,
+                       (size_t)n * D);
+  HSL_HIP(hipGetLastError());
+  return HSL_OK;
+}
+
+}  // extern "C"

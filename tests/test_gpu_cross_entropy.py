@@ -1,0 +1,275 @@
+"""linear_cross_entropy against its formulas in 64 bits.
+
+Tolerances.  A logit is a sum of D exact products (16-bit operands) or of D products, in fp32: off by at most
+(D + 4) 2^-24 of the sum of the products' sizes; `shift` is the largest of these of a row.  The loss is off
+by twice that and a few roundings of its parts.  A probability is off by the factor exp(2 shift + 2^-18), the
+last for exp's and the sum's own roundings.  16-bit operands: dl is rounded to the operands' type (half a
+step of itself; fp16 has it scaled, with 2^-38 of the largest |dloss| for its smallest step), then a
+product's sum of n terms is off by (n + 8) 2^-24 of their sizes, and the result is rounded once.  What is
+below the smallest normal number, 2^-126, may be 0: a probability, a gradient dl, or either of the later two
+of the three pieces that an fp32 product's operand is split into: 4 2^-126 of each dl.
+"""
+
+import math
+
+import pytest
+import torch
+
+import prlstm_amd
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def reference(x, w, targets, bias, dloss):
+    """loss, dl, and the sizes that the tolerances are measured against, in 64 bits on the CPU."""
+    x, w, dloss = (t.detach().double().cpu() for t in (x, w, dloss))
+    t = targets.cpu().long()
+    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.detach().double().cpu()
+    l = x @ w.t() + b
+    size = x.abs() @ w.abs().t() + torch.where(torch.isinf(b), torch.zeros_like(b), b.abs())
+    there = (t >= 0) & (t < w.shape[0])
+    empty = (l == -math.inf).all(1)
+    lse = torch.logsumexp(l, 1)
+    loss = torch.where(there, lse - l.gather(1, t.clamp(0, w.shape[0] - 1)[:, None])[:, 0], torch.zeros_like(lse))
+    loss[there & empty] = math.inf
+    loss[t >= w.shape[0]] = math.nan
+    g = torch.where(there & ~empty, dloss, torch.zeros_like(dloss))
+    p = torch.exp(l - torch.where(empty, torch.zeros_like(lse), lse)[:, None])
+    hot = torch.zeros_like(p)
+    hot[there, t[there]] = 1.0
+    masked = l == -math.inf
+    dl = torch.where(masked, torch.zeros_like(p), g[:, None] * (p - hot))
+    parts = torch.where(masked, torch.zeros_like(p), g.abs()[:, None] * (p + hot))  # of dl
+    return loss, dl, parts, size.amax(1) if size.numel() else lse * 0
+
+
+def within(name, got, want, bound):
+    half = torch.finfo(got.dtype).eps / 2
+    tiny = 2.0 ** -25 if got.dtype is torch.float16 else 0.0
+    g = got.detach().double().cpu()
+    assert g.shape == want.shape, (name, g.shape, want.shape)
+    same = (g == want) | (torch.isnan(g) & torch.isnan(want))
+    off = (g - want).abs() - (half * want.abs() + bound + tiny)
+    bad = ~same & ~(off <= 0)
+    assert not bool(bad.any()), (name, int(bad.sum()), off[bad].max().item())
+
+
+def check(x, w, targets, bias, dloss):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, bias) if t is not None]
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], targets, bias=leaves[2] if bias is not None else None)
+    grads = torch.autograd.grad(loss, leaves, dloss)
+    with torch.no_grad():
+        assert torch.equal(torch.nan_to_num(prlstm_amd.linear_cross_entropy(x, w, targets, bias=bias), -1.0),
+                           torch.nan_to_num(loss, -1.0))
+    want, dl, parts, size = reference(x, w, targets, bias, dloss)
+    n, d = x.shape
+    v = w.shape[0]
+    shift = (d + 4) * U * size
+    finite = torch.where(torch.isfinite(want), want.abs(), torch.zeros_like(want))
+    within("loss", loss, want, 2 * shift + 16 * U * (finite + size + math.log(v + 1)) + 2 ** -20)
+    step = torch.finfo(x.dtype).eps / 2 if x.dtype is not torch.float32 else 0.0
+    least = dloss.abs().max().item() * 2.0 ** -38 if x.dtype is torch.float16 and n else 4 * 2.0 ** -126
+    # of dl: the probability's error and its rounding
+    slack = (torch.expm1(2 * shift)[:, None] + 2 ** -18) * parts
+    err = slack + step * dl.abs() + least
+    x64, w64 = x.detach().double().cpu(), w.detach().double().cpu()
+    assert grads[0].dtype is x.dtype and grads[1].dtype is w.dtype
+    within("dx", grads[0], dl @ w64, err @ w64.abs() + (v + 8) * U * (parts @ w64.abs()))
+    within("dw", grads[1], dl.t() @ x64, err.t() @ x64.abs() + (n + 8) * U * (parts.t() @ x64.abs()))
+    if bias is not None:
+        within("dbias", grads[2], dl.sum(0), slack.sum(0) + 40 * U * parts.sum(0))
+    return loss, grads
+
+
+def inputs(dev, dtype, n, v, d, bias=False, pad=False, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x, w = torch.randn(n, d, generator=g), 1.5 * d ** -0.5 * torch.randn(v, d, generator=g)
+    t = torch.randint(0, v, (n,), generator=g)
+    if n:
+        x = x + 3 * torch.rand(n, 1, generator=g) * w[t]
+    b = torch.randn(v, generator=g).to(dev) if bias else None
+    if pad and n:
+        t[torch.rand(n, generator=g) < 0.3] = -1
+    dloss = torch.randn(n, generator=g) / max(1, n)
+    return x.to(dtype).to(dev), w.to(dtype).to(dev), t.to(dev), b, dloss.to(dev)
+
+
+SIZES = [(1, 1, 1), (1, 300, 8), (2, 2, 5), (3, 257, 64), (5, 1000, 72), (70, 513, 130), (256, 256, 64),
+         (300, 700, 264), (257, 255, 17), (33, 5000, 40), (600, 90, 500), (1, 20000, 128)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", SIZES)
+@pytest.mark.parametrize("extra", [False, True])
+def test_against_64_bits(dev, dtype, n, v, d, extra):
+    check(*inputs(dev, dtype, n, v, d, bias=extra, pad=extra))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,v,d", [(64, 70000, 32), (20000, 500, 24)])
+def test_sums_split_between_workgroups(dev, dtype, n, v, d):
+    """Long sums of few results."""
+    check(*inputs(dev, dtype, n, v, d, bias=True))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_tokens(dev, dtype):
+    """-inf in the bias: no probability and no gradient; a masked target has loss inf."""
+    x, w, t, b, dloss = inputs(dev, dtype, 40, 600, 48, bias=True)
+    b[::3] = -math.inf
+    b[300:560] = -math.inf  # a whole tile's worth
+    t = t // 3 * 3 + 1
+    t[t >= 300] = 1
+    t[7] = 3
+    t[9] = -5
+    loss, grads = check(x, w, t, b, dloss)
+    assert loss[7].item() == math.inf and loss[9].item() == 0
+    assert not bool(grads[1][::3].any()) and not bool(grads[2][::3].any()) and not bool(grads[0][9].any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_but_masks(dev, dtype):
+    x, w, t, b, dloss = inputs(dev, dtype, 5, 300, 16, bias=True)
+    b[:] = -math.inf
+    t[1] = -1
+    leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+    assert loss.tolist() == [math.inf, 0.0] + [math.inf] * 3
+    for g in torch.autograd.grad(loss, leaves, dloss):
+        assert not bool(g.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_non_finite_rows_stay_apart(dev, dtype):
+    """A row of x with NaN or infinities makes its own loss and gradient NaN and no other row's; where its
+    target is negative it makes nothing but its loss of 0."""
+    x, w, t, b, dloss = inputs(dev, dtype, 300, 700, 40)
+    loss, _ = check(x, w, t, b, dloss)
+    bad = x.clone()
+    bad[5], bad[290, 3] = math.nan, math.inf
+    xs = bad.requires_grad_(True)
+    l2 = prlstm_amd.linear_cross_entropy(xs, w, t)
+    dx, = torch.autograd.grad(l2, xs, dloss)
+    rest = torch.ones(300, dtype=torch.bool, device=dev)
+    rest[[5, 290]] = False
+    assert torch.isnan(l2[~rest]).all() and torch.equal(l2[rest], loss[rest])
+    assert bool(torch.isnan(dx[~rest]).any(1).all()) and bool(torch.isfinite(dx[rest]).all())
+
+
+def test_large_logits(dev):
+    """Logits far beyond exp's range, of both signs."""
+    x, w, t, b, dloss = inputs(dev, torch.float32, 50, 400, 24)
+    check(x * 100, w, t, b, dloss)
+    x, w, t, b, dloss = inputs(dev, torch.bfloat16, 50, 400, 24)
+    check(x * 64, w, t, b, dloss)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e30])
+def test_sizes_of_the_gradient(dev, scale):
+    """fp16's products run on scaled gradients."""
+    x, w, t, b, dloss = inputs(dev, torch.float16, 30, 400, 24, bias=True)
+    leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+    got = torch.autograd.grad(loss, leaves, dloss * scale)
+    assert all(bool(torch.isfinite(g).all()) for g in (got if scale < 1 else got[2:]))
+    _, dl, parts, size = reference(x, w, t, b, dloss * scale)  # a gradient may cancel, its parts do not
+    slack = (torch.expm1(2 * (24 + 4) * U * size)[:, None] + 2 ** -18) * parts + 4 * 2.0 ** -126
+    within("dbias", got[2], dl.sum(0), slack.sum(0) + 40 * U * parts.sum(0))
+    if scale == 1e30:
+        assert not bool(torch.isnan(got[0]).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_shapes(dev, dtype):
+    """Rows cut from wider tensors, at odd offsets, transposed, repeated; leading dimensions; int32."""
+    x, w, t, b, dloss = inputs(dev, dtype, 60, 300, 40, bias=True)
+    want, grads = check(x, w, t, b, dloss)
+    wide_x, wide_w = torch.zeros(60, 101, device=dev, dtype=dtype), torch.zeros(300, 64, device=dev, dtype=dtype)
+    wide_x[:, 3:43], wide_w[:, 8:48] = x, w
+    for xs, ws in ((wide_x[:, 3:43], wide_w[:, 8:48]), (x.t().contiguous().t(), w.t().contiguous().t())):
+        leaves = [s.detach().requires_grad_(True) for s in (xs, ws, b)]
+        loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t.int(), bias=leaves[2])
+        assert torch.equal(loss, want)
+        for g, k in zip(torch.autograd.grad(loss, leaves, dloss), grads):
+            assert torch.equal(g, k)
+    lead = prlstm_amd.linear_cross_entropy(x.reshape(3, 4, 5, 40), w, t.reshape(3, 4, 5), bias=b)
+    assert lead.shape == (3, 4, 5) and torch.equal(lead.reshape(-1), want)
+    check(x[:1].expand(60, 40), w, t, b, dloss)
+    assert prlstm_amd.linear_cross_entropy(x[0], w, t[0], bias=b).shape == ()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_of_nothing(dev, dtype):
+    x, w, t, b, dloss = inputs(dev, dtype, 0, 30, 8, bias=True)
+    leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+    assert loss.shape == (0,)
+    for g in torch.autograd.grad(loss, leaves, dloss):
+        assert not bool(g.any())
+
+
+def test_some_gradients(dev):
+    """Only what is asked for, whatever the rest is."""
+    x, w, t, b, dloss = inputs(dev, torch.bfloat16, 60, 300, 40, bias=True)
+    leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+    all_of = torch.autograd.grad(prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2]), leaves, dloss)
+    for k in range(3):
+        args = [x, w, b]
+        args[k] = leaves[k]
+        g, = torch.autograd.grad(prlstm_amd.linear_cross_entropy(args[0], args[1], t, bias=args[2]), leaves[k], dloss)
+        assert torch.equal(g, all_of[k])
+
+
+def test_targets_beyond_the_vocabulary(dev):
+    prlstm_amd.check_errors()
+    x, w, t, b, dloss = inputs(dev, torch.bfloat16, 60, 300, 40)
+    t[3], t[5] = 300, 1 << 40
+    leaves = [s.detach().requires_grad_(True) for s in (x, w)]
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t)
+    assert torch.isnan(loss).nonzero()[:, 0].tolist() == [3, 5]
+    dx, dw = torch.autograd.grad(loss, leaves, dloss)
+    assert not bool(dx[[3, 5]].any()) and bool(torch.isfinite(dw).all())
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        prlstm_amd.check_errors()
+
+
+def test_refusals(dev):
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device=dev)  # noqa: E731
+    t = torch.zeros(3, dtype=torch.int64, device=dev)
+    f = prlstm_amd.linear_cross_entropy
+    for call, text in ((lambda: f(z(3, 4), z(5, 6), t), "weight"), (lambda: f(z(3, 4), z(5, 4), t[:2]), "targets must"),
+                       (lambda: f(z(3, 4), z(5, 4, dt=torch.bfloat16), t), "weight must be"),
+                       (lambda: f(z(3, 4, dt=torch.float64), z(5, 4, dt=torch.float64), t), "x must be"),
+                       (lambda: f(z(3, 4), z(5, 4), t.float()), "int64 or int32"),
+                       (lambda: f(z(3, 4), z(5, 4), t, bias=z(4)), "bias must"),
+                       (lambda: f(z(3, 4), z(0, 4), t), "must not be empty"), (lambda: f(z(3, 0), z(5, 0), t), "must not be empty"),
+                       (lambda: f(z(3, 4), z(5, 4), t.cpu()), "targets is on"),
+                       (lambda: f(z(3, 4), z(5, 4).cpu(), t), "weight must be")):
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_captured_training_step(dev, dtype):
+    x, w, t, b, dloss = inputs(dev, dtype, 300, 700, 40, bias=True)
+
+    def step():
+        leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+        loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+        return loss.detach(), *torch.autograd.grad(loss, leaves, dloss)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in range(3):
+        for old, new in zip((x, w, t, b, dloss), inputs(dev, dtype, 300, 700, 40, bias=True, seed=seed + 3)):
+            old.copy_(new)
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for got, k in zip(captured, want):
+            assert torch.equal(got, k)
