@@ -436,7 +436,7 @@ int hsl_conv_bwd(const void* x, long long x_t, long long x_b, const float* w, co
  * delta_bias [D] (each may be NULL), h0 and h_n [B, D, N] are fp32.  h_n = h_{T-1} (h0 when
  * T = 0); it may be h0 itself when T = 1 and ck is NULL.  ck (NULL: no backward follows) receives
  * hsl_selective_ck_floats(T, B, D, N) values that hsl_selective_bwd starts from.  T is less than
- * 2^30, B*D less than 2^27 and B*ceil(D/64)*ceil(N/4) less than 2^25. */
+ * 2^30, B*D less than 2^27 and B*ceil(D/64)*ceil(N/4) less than 2^24. */
 size_t hsl_selective_ck_floats(int T, int B, int D, int N);
 size_t hsl_selective_fwd_ws_bytes(int T, int B, int D, int N);
 int hsl_selective_fwd(const void* x, long long x_t, long long x_b,

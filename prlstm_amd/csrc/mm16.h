@@ -1,32 +1,49 @@
 // A 256 x 256 tile of a product of 16-bit operands (bf16 or fp16) with fp32 sums, for kernels with
 // their own epilogues (xent.hip): C[i][j] = sum_k A(i, k) B(j, k).
 //
-// Workgroup = 8 waves, 2 (rows) x 4 (columns) of 128 x 64 each, in 4 x 2 fragments of the 32x32x16
-// instruction.  A slice is 64 deep; two slices are in LDS (128 KB), and the next one is copied from
-// memory straight to LDS while this one multiplies.  A copy instruction moves 64 pieces of 16 bytes to
-// consecutive addresses, so the layout in LDS is made by choosing which piece each lane fetches:
-//   an operand whose k are neighbours in memory ([row][k]) lies as [256 rows][8 pieces of 8 k], piece p of
-//   row r at place p ^ f(r), f(r) = (r ^ r >> 3) & 7, so that the 16 rows that a read serves at a time are
-//   in different banks;
-//   an operand whose rows are neighbours ([k][row]) lies as [64 k][32 pieces of 8 rows], piece p of k at
+// Workgroup = 8 waves, two a SIMD, 2 (rows) x 4 (columns) of 128 x 64 each, in 4 x 2 fragments of the
+// 32x32x16 instruction.  A slice is 32 deep; four are in LDS (128 KB), copied from memory straight to LDS.
+// While half a slice multiplies, the other half's operands, or the next slice's first ones, are read
+// from LDS; the one barrier a slice, between its halves, says that the next slice has arrived and that this
+// one's place is free for the slice four further.
+//
+// A copy instruction moves 64 pieces of 16 bytes to consecutive addresses, so the layout in LDS is made
+// by choosing which piece each lane fetches:
+//   an operand whose k are neighbours in memory ([row][k]) lies as [256 rows][4 pieces of 8 k], piece p of
+//   row r at place p ^ (r >> 2 & 3), so that the 16 rows that a read serves at a time are in different
+//   banks;
+//   an operand whose rows are neighbours ([k][row]) lies as [32 k][32 pieces of 8 rows], piece p of k at
 //   place p ^ 4 (k & 3), and is read by the transposing LDS read, which gives lane i of 16 the four
 //   values (k .. k+3, row i) from 16 addresses of 4 rows each.
 // Pieces beyond the operand's rows or k read as zeros (a buffer's bounds), nothing outside is touched.
 // Operands have 16-byte aligned rows.
+//
+// The copies are written in assembly because the compiler, which cannot tell the four slices apart, would
+// wait for all copies before each read.  So the waits for them are written too: a wave's copies, loads and
+// stores end in order, so a wait for all but the last n is right where at least n were issued behind
+// those that it is for.
 #pragma once
 
 #include "lm.h"
 
 namespace hsl {
 
-constexpr int kMmTile = 256, kMmSlice = 64, kMmThreads = 512;
+constexpr int kMmTile = 256, kMmSlice = 32, kMmThreads = 512, kMmStages = 4;
 constexpr int kMmOperand = kMmTile * kMmSlice * 2;  // bytes of one operand's slice
-constexpr int kMmLds = 4 * kMmOperand;
+constexpr int kMmStage = 2 * kMmOperand;
+constexpr int kMmLds = kMmStages * kMmStage;
+constexpr int kMmCopies = kMmOperand / 1024 / (kMmThreads / 64);  // instructions of a wave for an operand's slice
+static_assert(kMmCopies == 2, "the counts in MmTile's waits");
 
 typedef __bf16 mm_bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 mm_h8 __attribute__((ext_vector_type(8)));
 typedef unsigned mm_u4 __attribute__((ext_vector_type(4)));
 typedef short mm_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char mm_lds_char;
+
+// acc[i][j]: rows 32 i, columns 32 j of the wave's block (rows from 128 (wave / 4), columns from
+// 64 (wave % 4)): lane l, register r is row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
+typedef float MmAcc[4][2][16];
 
 // An operand from its tile's first row and first k on: `rows` of its tile's 256 exist, and k of them.
 // ld (elements) is between rows in memory, or between k where TRANS.
@@ -36,70 +53,94 @@ struct MmOperand {
   int rows, k;
 };
 
+// For an operand of assembly that has to be in a scalar register.
+__device__ __forceinline__ unsigned mm_uniform(unsigned v) { return (unsigned)__builtin_amdgcn_readfirstlane((int)v); }
+
 template <bool TRANS>
 struct MmLoad {
-  unsigned off[4];  // bytes from the slice's first element
-  int at[4];        // the piece's first k (TRANS: its k) in the slice; beyond every k where no row exists
-  __device__ __forceinline__ void init(const MmOperand& o, int wave, int lane) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int p = (wave * 4 + j) * 64 + lane;
-      if constexpr (TRANS) {
-        const int k = p >> 5, c = (p & 31) ^ (4 * (k & 3));
-        off[j] = (unsigned)((k * o.ld + c * 8) * 2);
-        at[j] = c * 8 < o.rows ? k : 0x7fffffff;
-      } else {
-        const int r = p >> 3, c = (p & 7) ^ ((r ^ (r >> 3)) & 7);
-        off[j] = (unsigned)((r * o.ld + c * 8) * 2);
-        at[j] = r < o.rows ? c * 8 : 0x7fffffff;
-      }
-    }
+  unsigned row, ld;  // bytes: of the lane's row (TRANS: k) among a copy's 16 (2), between rows
+  int lane;
+  __device__ __forceinline__ void init(const MmOperand& o, int l) {
+    lane = l;
+    ld = (unsigned)(o.ld * 2);
+    row = (TRANS ? lane >> 5 : lane >> 2) * ld;
   }
   // Copies the slice from k0 on to the operand's place in LDS.
-  __device__ __forceinline__ void copy(const MmOperand& o, int k0, char* lds, int wave) const {
-    const unsigned short* base = o.p + (TRANS ? k0 * o.ld : (long long)k0);
+  __device__ __forceinline__ void copy(const MmOperand& o, int k0, unsigned lds, int wave) const {
+    const unsigned long long base = (unsigned long long)(o.p + (TRANS ? k0 * o.ld : (long long)k0));
+    const unsigned lo = mm_uniform((unsigned)base), hi = mm_uniform((unsigned)(base >> 32));
+    const mm_u4 rsrc = {lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u};
+    const unsigned step = mm_uniform(ld), to = mm_uniform(lds);
     const int left = o.k - k0;
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(base), (short)0, 0x7fffffff, 0x00020000);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned v = at[j] < left ? off[j] : kOffNone;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void*)(lds + (wave * 4 + j) * 1024), 16, (int)v, 0, 0, 0);
+    for (int j = 0; j < kMmCopies; ++j) {
+      const int n = wave * kMmCopies + j;  // of the operand's 16 copies
+      int c, first;
+      bool in;
+      if constexpr (TRANS) {
+        first = n * 2;
+        c = (lane & 31) ^ (4 * ((first + (lane >> 5)) & 3));
+        in = c * 8 < o.rows && (lane >> 5) < left - first;
+      } else {
+        first = n * 16;
+        c = (lane & 3) ^ ((lane >> 4) & 3);
+        in = c * 8 < left && (lane >> 2) < o.rows - first;
+      }
+      const unsigned off = in ? row + c * 16 : kOffNone;
+      // (m0 is never kept by the compiler; a write of it may not be followed at once by a copy to LDS)
+      asm volatile(
+          "s_mov_b32 m0, %0\n\t"
+          "s_nop 0\n\t"
+          "buffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to + n * 1024),
+          "v"(off), "s"(rsrc), "s"(first * step)
+          : "memory");
     }
   }
 };
 
-// Reads one 32-row fragment (row or column fragment i of the wave) of k-step ks.
-template <bool TRANS>
+// Wave `wave` copies the 1 KB at `from` (16-byte aligned) to piece `wave` of `to`, or zeros.
+__device__ __forceinline__ void mm_copy_kb(const void* from, bool in, const void* to, int wave) {
+  const unsigned long long base = (unsigned long long)from;
+  const unsigned lo = mm_uniform((unsigned)base), hi = mm_uniform((unsigned)(base >> 32));
+  const mm_u4 rsrc = {lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u};
+  const unsigned at = mm_uniform((unsigned)(unsigned long long)(const mm_lds_char*)to + wave * 1024);
+  const unsigned off = in ? (threadIdx.x & 63) * 16 : kOffNone;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc)
+      : "memory");
+}
+
+// Reads a wave's N 32-row fragments of a slice's two k-steps.
+template <bool TRANS, int N>
 struct MmRead {
-  int base, x[4];
-  __device__ __forceinline__ void init(int first, int lane) {  // first row of the wave: a multiple of 64
+  int x[TRANS ? N : 2];  // bytes: of fragment i where TRANS, otherwise of k-step ks
+  __device__ __forceinline__ void init(int first, int lane) {  // first row of the wave
     if constexpr (TRANS) {
       const int j = lane & 15, g = lane >> 4;
-      base = (8 * (g >> 1) + (j >> 2)) * 512 + (j & 1) * 8;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = ((first / 8 + i * 4 + 2 * (g & 1) + ((j & 3) >> 1)) ^ (4 * (j >> 2))) * 16;
+      for (int i = 0; i < N; ++i)
+        x[i] = (8 * (g >> 1) + (j >> 2)) * 512 + (j & 1) * 8 +
+               ((first / 8 + i * 4 + 2 * (g & 1) + ((j & 3) >> 1)) ^ (4 * (j >> 2))) * 16;
     } else {
       const int r = lane & 31, half = lane >> 5;
-      base = (first + r) * 128;
-      const int f = (r ^ ((first + r) >> 3)) & 7;
 #pragma unroll
-      for (int s = 0; s < 4; ++s) x[s] = ((s * 2 + half) ^ f) * 16;
+      for (int s = 0; s < 2; ++s) x[s] = (first + r) * 64 + ((s * 2 + half) ^ ((r >> 2) & 3)) * 16;
     }
   }
-  __device__ __forceinline__ mm_u4 read(const char* lds, int i, int ks) const {
+  __device__ __forceinline__ mm_u4 read(const char* lds, int ks, int i) const {
     if constexpr (TRANS) {
       typedef __attribute__((address_space(3))) mm_s4* P;
-      const char* p = lds + base + x[i] + ks * (16 * 512);
+      const char* p = lds + x[i] + ks * (16 * 512);
       const mm_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p));
       const mm_s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * 512));
-      mm_u4 r;
-      __builtin_memcpy(&r, &lo, 8);
-      __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
-      return r;
+      mm_u4 f;
+      __builtin_memcpy(&f, &lo, 8);
+      __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &hi, 8);
+      return f;
     } else {
-      // rows 32 further have f with bit 2 turned over, which is the step two further
-      return *reinterpret_cast<const mm_u4*>(lds + base + i * (32 * 128) + x[i & 1 ? ks ^ 2 : ks]);
+      return *reinterpret_cast<const mm_u4*>(lds + x[ks] + i * (32 * 64));
     }
   }
 };
@@ -114,48 +155,119 @@ __device__ __forceinline__ f16v mm_mfma(mm_u4 a, mm_u4 b, f16v c) {
                                                    0, 0);
 }
 
-// acc[i][j]: rows 32 i, columns 32 j of the wave's block (rows from 128 (wave / 4), columns from
-// 64 (wave % 4)): lane l, register r is row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
-// nk: slices.  lds: kMmLds bytes, free when the call returns (after a barrier).
+// The products of a workgroup's tiles, one after the other: while a tile's last slices multiply, the next
+// one's first are copied, so that they have arrived when its product begins.  lds: kMmLds bytes that hold
+// nothing else from begin() on.
 template <bool FP16, bool TA, bool TB>
-__device__ __forceinline__ void mm_tile(const MmOperand& A, const MmOperand& B, int nk, char* lds, f16v (&acc)[4][2]) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+struct MmPipe {
+  MmOperand A, B;
   MmLoad<TA> la;
   MmLoad<TB> lb;
-  la.init(A, wave, lane);
-  lb.init(B, wave, lane);
-  MmRead<TA> ra;
-  MmRead<TB> rb;
-  ra.init((wave >> 2) * 128, lane);
-  rb.init((wave & 3) * 64, lane);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f16v{};
-  la.copy(A, 0, lds, wave);
-  lb.copy(B, 0, lds + kMmOperand, wave);
-  __syncthreads();
-  for (int it = 0; it < nk; ++it) {
-    char* const now = lds + (it & 1) * (2 * kMmOperand);
-    char* const next = lds + (~it & 1) * (2 * kMmOperand);
-    if (it + 1 < nk) {
-      la.copy(A, (it + 1) * kMmSlice, next, wave);
-      lb.copy(B, (it + 1) * kMmSlice, next + kMmOperand, wave);
-    }
-#pragma unroll
-    for (int ks = 0; ks < kMmSlice / 16; ++ks) {
-      mm_u4 a[4], b[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) b[j] = rb.read(now + kMmOperand, j, ks);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = ra.read(now, i, ks);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mm_mfma<FP16>(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
+  MmRead<TA, 4> ra;
+  MmRead<TB, 2> rb;
+  const char* lds;
+  int wave, stage, slices;  // stage: where the tile's first slice lies; slices: of a tile
+
+  __device__ __forceinline__ void copy(const MmOperand& a, const MmOperand& b, int slice, int at) const {
+    const unsigned p = (unsigned)(unsigned long long)(const mm_lds_char*)lds + (at % kMmStages) * kMmStage;
+    la.copy(a, slice * kMmSlice, p, wave);
+    lb.copy(b, slice * kMmSlice, p + kMmOperand, wave);
   }
-}
+  // Every tile has k up to K and the same strides as this first one.
+  __device__ __forceinline__ void begin(const char* space, const MmOperand& a, const MmOperand& b, int K) {
+    const int lane = threadIdx.x & 63;
+    A = a;
+    B = b;
+    lds = space;
+    stage = 0;
+    slices = max(kMmStages, (K + kMmSlice - 1) / kMmSlice);  // slices beyond K are zeros
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    la.init(A, lane);
+    lb.init(B, lane);
+    ra.init((wave >> 2) * 128, lane);
+    rb.init((wave & 3) * 64, lane);
+#pragma unroll
+    for (int s = 0; s < kMmStages; ++s) copy(A, B, s, s);
+    asm volatile("s_waitcnt vmcnt(12)\n\ts_barrier" ::: "memory");  // 3 slices of 4 copies may be on their way
+  }
+  // acc = this tile's product; nextA, nextB: the next tile, or operands without k.  with_next() is called
+  // before the first copy for it.  LATER (a count): loads and stores that the wave has issued for sure since the
+  // product before, which the waits for the copies before them leave out; later: whether there was one.
+  template <int LATER, class Fn>
+  __device__ __forceinline__ void run(MmAcc& acc, const MmOperand& nextA, const MmOperand& nextB, bool later,
+                                      Fn with_next) {
+    f16v sum[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sum[i][j] = f16v{};
+    auto place = [&](int slice) { return lds + ((stage + slice) % kMmStages) * kMmStage; };
+    mm_u4 a0[4], b0[2], a1[4], b1[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a0[i] = ra.read(place(0), 0, i);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) b0[j] = rb.read(place(0) + kMmOperand, 0, j);
+    // The order is fixed: between two products there is always something to issue, and there is a product
+    // to run while the wave is at the barrier.
+    auto fixed = [] { __builtin_amdgcn_sched_barrier(0); };
+    auto product = [&](mm_u4 a, const mm_u4(&b)[2], int i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) sum[i][j] = mm_mfma<FP16>(a, b[j], sum[i][j]);
+      fixed();
+    };
+    auto slice = [&](int it, const MmOperand& from_a, const MmOperand& from_b, int ahead) {
+      const char* const now = place(it);
+      const char* const next = place(it + 1);
+      product(a0[0], b0, 0);
+      b1[0] = rb.read(now + kMmOperand, 1, 0);
+      b1[1] = rb.read(now + kMmOperand, 1, 1);
+      a1[0] = ra.read(now, 1, 0);
+      fixed();
+      product(a0[1], b0, 1);
+      a1[1] = ra.read(now, 1, 1);
+      a1[2] = ra.read(now, 1, 2);
+      a1[3] = ra.read(now, 1, 3);
+      fixed();
+      product(a0[2], b0, 2);
+      product(a0[3], b0, 3);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      product(a1[0], b1, 0);
+      // this slice is in registers and the next one has arrived: 2 more may be on their way, and behind the
+      // slices that were copied before it, what `later` says
+      if (LATER > 0 && later && it < kMmStages - 1)
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(8 + LATER) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+      fixed();
+      // (the last time, of the next tile: they are read again behind the epilogue rather than kept)
+      b0[0] = rb.read(next + kMmOperand, 0, 0);
+      b0[1] = rb.read(next + kMmOperand, 0, 1);
+      a0[0] = ra.read(next, 0, 0);
+      fixed();
+      product(a1[1], b1, 1);
+      a0[1] = ra.read(next, 0, 1);
+      a0[2] = ra.read(next, 0, 2);
+      a0[3] = ra.read(next, 0, 3);
+      fixed();
+      product(a1[2], b1, 2);
+      copy(from_a, from_b, ahead, stage + it);  // to where this slice lay
+      fixed();
+      product(a1[3], b1, 3);
+    };
+    int it = 0;
+    for (; it < slices - kMmStages; ++it) slice(it, A, B, it + kMmStages);
+    with_next();
+    for (; it < slices; ++it) slice(it, nextA, nextB, it + kMmStages - slices);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = sum[i][j][r];
+    stage = (stage + slices) % kMmStages;
+    A = nextA;
+    B = nextB;
+  }
+};
 
 }  // namespace hsl

@@ -3,7 +3,7 @@
 //   h_t = exp(dt_t a) h_{t-1} + dt_t x_t b_t,   h_{-1} = h0, and 0 in place of h_{t-1} at a reset,
 //   y_t = sum_n c_t[n] h_t[n] + d x_t,   out_t = y_t z_t sigmoid(z_t) (or y_t).
 //
-// A workgroup has 64 neighbouring channels of one batch row, a lane each, and W waves of kS = 4 states
+// A workgroup has 64 neighbouring channels of one batch row, a lane each, and W waves of S states
 // each, so the states need no cross-lane sums, b and c are the same for all lanes and y is a sum over
 // the waves.  It walks the time in chunks of L steps:
 //   A  every wave makes dt and dt x of L / W steps of its 64 channels from loads that a chunk before
@@ -12,23 +12,27 @@
 //   C  every wave sums, gates and stores y of the steps that it had in A.
 // Steps behind the last have dt = 0 and x = 0, which keeps the state.  What bounds it is the vector
 // units: 8 issue slots per state and step (v_exp_f32 takes four), about 60 per channel and step.
+// Streams are read and written through buffers whose bounds drop what lies outside, without branches.
 #pragma once
 
 #include "lm.h"
 
 namespace hsl {
 
-constexpr int kS = 4;          // states of a wave
 constexpr int kChannels = 64;  // of a workgroup
 constexpr int kMaxStates = 64;
 
-// Steps of a chunk, which is also what lies between two kept states.  Sixteen waves have 128
-// registers each, which hold the backward's copy of 8 steps.
-template <int W>
-constexpr int chunk_steps() {
-  return W == 16 ? 8 : 16;
-}
-inline int scan_waves(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+// Waves of a workgroup and states of a wave.
+template <int W_, int S_>
+struct ScanShape {
+  static constexpr int W = W_, S = S_, N = W * S;
+  // Steps of a chunk, which is also what lies between two kept states.  Sixteen waves have 128
+  // registers each, which hold the backward's copy of 8 steps.
+  static constexpr int L = N > 32 ? 8 : 16;
+  static constexpr int PS = L >= W ? L / W : 1;  // steps that a wave has in A and C
+};
+// The states that a call's are filled up to.
+inline int scan_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 inline int scan_chunk(int N) { return N > 32 ? 8 : 16; }
 
 struct ScanPlan {
@@ -42,10 +46,11 @@ struct ScanArgs {
   OutStream y, dx, ddelta, dz;
   const float *a, *d, *bias, *h0, *dh_n;
   float *h_n, *ck, *dh0;
-  float* map_h;     // [segment][B][W][D][4]: the state behind the segment if it began with zeros
+  // Kept states lie in pairs, [..][B][pair][D][2].
+  float* map_h;     // of [segment]: the state behind the segment if it began with zeros
   float2* map_s;    // [segment][B][D]: its sum of dt, and whether it has a reset
-  float* part_bc;   // [tile][T][B][2][4 W]: the tile's sums for db and dc
-  float* part_a;    // [B segments][W][D][4]
+  float* part_bc;   // [tile][T][B][2][states]: the tile's sums for db and dc
+  float* part_a;    // [B segments][pair][D][2]
   float* part_d;    // [B segments][2][D]
   int T, B, D, N, softplus, seg_steps, nseg;
 };
@@ -67,6 +72,7 @@ __device__ __forceinline__ float segment_decay(float a2, float S) {
 }
 
 // A workgroup's place, and its lane's channel (clamped into the row where `ok` is false).
+template <class P>
 struct ScanPlace {
   int lane, w, b, tile, ch, n0;
   bool ok;
@@ -79,82 +85,154 @@ struct ScanPlace {
     ch = tile * kChannels + lane;
     ok = ch < a.D;
     ch = min(ch, a.D - 1);
-    n0 = w * kS;
+    n0 = w * P::S;
   }
 };
 
-// The wave's states of the lane's channel from [.., D, N], 0 beyond.
-__device__ __forceinline__ void load_states(const float* p, const ScanPlace& q, const ScanArgs& a, float (&v)[kS]) {
+// The wave's states of the lane's channel from [B, D, N], 0 beyond.
+template <class P>
+__device__ __forceinline__ void load_states(const float* p, const ScanPlace<P>& q, const ScanArgs& a,
+                                            float (&v)[P::S]) {
   const float* r = p + ((size_t)q.b * a.D + q.ch) * a.N + q.n0;
 #pragma unroll
-  for (int n = 0; n < kS; ++n) v[n] = p && q.ok && q.n0 + n < a.N ? r[n] : 0.f;
+  for (int n = 0; n < P::S; ++n) v[n] = p && q.ok && q.n0 + n < a.N ? r[n] : 0.f;
 }
-__device__ __forceinline__ void store_states(float* p, const ScanPlace& q, const ScanArgs& a, const float (&v)[kS]) {
+template <class P>
+__device__ __forceinline__ void store_states(float* p, const ScanPlace<P>& q, const ScanArgs& a,
+                                             const float (&v)[P::S]) {
   float* r = p + ((size_t)q.b * a.D + q.ch) * a.N + q.n0;
 #pragma unroll
-  for (int n = 0; n < kS; ++n)
+  for (int n = 0; n < P::S; ++n)
     if (q.ok && q.n0 + n < a.N) r[n] = v[n];
 }
-__device__ __forceinline__ void load_a2(const ScanPlace& q, const ScanArgs& a, float (&a2)[kS]) {
+// The wave's states in row `row` (of B each) of states kept in pairs.
+template <class P>
+__device__ __forceinline__ size_t pair_at(const ScanPlace<P>& q, const ScanArgs& a, size_t row) {
+  return ((row * (P::N / 2) + q.n0 / 2) * a.D + q.ch) * 2;
+}
+template <class P>
+__device__ __forceinline__ void load_pairs(const float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
+                                           float (&v)[P::S]) {
 #pragma unroll
-  for (int n = 0; n < kS; ++n) a2[n] = q.n0 + n < a.N ? a.a[(size_t)q.ch * a.N + q.n0 + n] * kLog2e : 0.f;
+  for (int n = 0; n < P::S; n += 2) {
+    const float2 u = *reinterpret_cast<const float2*>(p + pair_at(q, a, row) + (size_t)n * a.D);
+    v[n] = u.x;
+    v[n + 1] = u.y;
+  }
+}
+template <class P>
+__device__ __forceinline__ void store_pairs(float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
+                                            const float (&v)[P::S]) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int n = 0; n < P::S; n += 2)
+    __builtin_nontemporal_store((F2){v[n], v[n + 1]}, reinterpret_cast<F2*>(p + pair_at(q, a, row) + (size_t)n * a.D));
+}
+template <class P>
+__device__ __forceinline__ void load_a2(const ScanPlace<P>& q, const ScanArgs& a, float (&a2)[P::S]) {
+#pragma unroll
+  for (int n = 0; n < P::S; ++n) a2[n] = q.n0 + n < a.N ? a.a[(size_t)q.ch * a.N + q.n0 + n] * kLog2e : 0.f;
 }
 
-// One element of a stream per lane; 0 where `in` is false.
-template <int F>
-__device__ __forceinline__ typename Elem<F>::T load_at(const Stream& s, int t, int b, int j, bool in) {
+// The rows of a stream that a wave has in a chunk, one every W steps; the addresses are the wave's, so
+// they cost the vector units nothing, and they move on by additions.
+template <int F, class P>
+struct Rows {
   using T_ = typename Elem<F>::T;
-  return in ? static_cast<const T_*>(s.p)[t * s.st + b * s.sb + j] : T_{};
-}
+  char* p;             // of the chunk's first row
+  long long row, chunk;  // bytes between the wave's rows, and between chunks
+  bool there;
+  template <class S>
+  __device__ __forceinline__ Rows(const S& s, const ScanPlace<P>& q, int t0) {
+    there = s.p != nullptr;
+    row = s.st * (long long)(P::W * sizeof(T_));
+    chunk = s.st * (long long)(P::L * sizeof(T_));
+    p = reinterpret_cast<char*>(const_cast<void*>(static_cast<const void*>(s.p))) +
+        ((t0 + q.w) * s.st + q.b * s.sb) * (long long)sizeof(T_);
+  }
+  __device__ __forceinline__ void move(int chunks) { p += chunks * chunk; }
+  // Row i; reads as zeros, and is not stored, where `in` is false.
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int i, bool in) const {
+    return __builtin_amdgcn_make_buffer_rsrc(p + i * row, (short)0, in && there ? 0x7fffffff : 0, 0x00020000);
+  }
+  // off: the lane's bytes from the row's start, or kOffNone.
+  __device__ __forceinline__ T_ load(int i, unsigned off, bool in) const {
+    if constexpr (F == kElemF32)
+      return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(at(i, in), (int)off, 0, 0));
+    else
+      return (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(at(i, in), (int)off, 0, 0);
+  }
+  __device__ __forceinline__ void store(int i, unsigned off, bool in, float v) const {
+    if constexpr (F == kElemF32)
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), at(i, in), (int)off, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b16(Elem<F>::down(v), at(i, in), (int)off, 0, 0);
+  }
+};
 
-// Bit s: whether step t0 + s begins a sequence (the same for the whole workgroup).
+// Lane s: whether step t0 + s begins a sequence; the lanes' answers are put together when they are
+// needed (cuts_of: bit s, the same for the whole workgroup), for that waits for the load.
 template <int L>
-__device__ __forceinline__ unsigned load_cuts(const Stream& reset, int t0, int te, int b, int lane) {
-  if (!reset.p) return 0;
-  const bool cut = lane < L && t0 + lane < te &&
-                   static_cast<const unsigned char*>(reset.p)[(t0 + lane) * reset.st + b * reset.sb] != 0;
-  return (unsigned)__ballot(cut);
+__device__ __forceinline__ unsigned char load_cut(const Stream& reset, int t0, int te, int b, int lane) {
+  unsigned char cut = 0;
+  if (reset.p && lane < L && t0 + lane < te)
+    cut = static_cast<const unsigned char*>(reset.p)[(t0 + lane) * reset.st + b * reset.sb];
+  return cut;
+}
+__device__ __forceinline__ unsigned cuts_of(const Stream& reset, unsigned char cut) {
+  return reset.p ? (unsigned)__ballot(cut != 0) : 0u;
 }
 
 // b and c of a chunk in LDS, [step][state], 0 beyond the last state and step.
-template <int F, int W>
+template <int F, class P>
 struct BcTile {
-  static constexpr int L = chunk_steps<W>(), kN = W * kS, kEach = (L * kN + W * 64 - 1) / (W * 64);
-  typename Elem<F>::T rb[kEach], rc[kEach];
+  using T_ = typename Elem<F>::T;
+  static constexpr int kEach = (P::L * P::N + P::W * 64 - 1) / (P::W * 64);
+  T_ rb[kEach], rc[kEach];
   __device__ __forceinline__ void load(const ScanArgs& a, int b, int t0, int te) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int k = threadIdx.x + i * W * 64, s = k / kN, n = k % kN;
-      const bool in = k < L * kN && t0 + s < te && n < a.N;
-      rb[i] = load_at<F>(a.b, t0 + s, b, n, in);
-      rc[i] = load_at<F>(a.c, t0 + s, b, n, in);
+      const int k = threadIdx.x + i * P::W * 64, s = k / P::N, n = k % P::N;
+      const bool in = k < P::L * P::N && t0 + s < te && n < a.N;
+      const T_* const bp = static_cast<const T_*>(a.b.p) + (t0 * a.b.st + b * a.b.sb);
+      const T_* const cp = static_cast<const T_*>(a.c.p) + (t0 * a.c.st + b * a.c.sb);
+      const int row = in ? s : 0, m = in ? n : 0;
+      rb[i] = bp[row * a.b.st + m];
+      rc[i] = cp[row * a.c.st + m];
+      if (!in) rb[i] = rc[i] = T_{};
     }
   }
-  __device__ __forceinline__ void store(float (*sb)[kN], float (*sc)[kN]) const {
+  __device__ __forceinline__ void store(float (*sb)[P::N], float (*sc)[P::N]) const {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int k = threadIdx.x + i * W * 64;
-      if (k >= L * kN) break;
-      sb[k / kN][k % kN] = Elem<F>::up(rb[i]);
-      sc[k / kN][k % kN] = Elem<F>::up(rc[i]);
+      const int k = threadIdx.x + i * P::W * 64;
+      if (P::L * P::N % (P::W * 64) && k >= P::L * P::N) break;
+      sb[k / P::N][k % P::N] = Elem<F>::up(rb[i]);
+      sc[k / P::N][k % P::N] = Elem<F>::up(rc[i]);
     }
   }
 };
 
-__device__ __forceinline__ f4 load4(const float* p) { return *reinterpret_cast<const f4*>(p); }
+// A wave's S values of b or c.
+template <int S>
+__device__ __forceinline__ void load_row(const float* p, float (&v)[S]) {
+  typedef float V __attribute__((ext_vector_type(S)));
+  const V u = *reinterpret_cast<const V*>(p);
+#pragma unroll
+  for (int n = 0; n < S; ++n) v[n] = u[n];
+}
 
-// f(integral_constant fmt, integral_constant waves).
-template <class Fn>
-int with_scan(int fmt, int N, Fn f) {
-  return with_fmt(fmt, [&](auto F) {
-    switch (scan_waves(N)) {
-      case 1: return f(F, std::integral_constant<int, 1>{});
-      case 2: return f(F, std::integral_constant<int, 2>{});
-      case 4: return f(F, std::integral_constant<int, 4>{});
-      case 8: return f(F, std::integral_constant<int, 8>{});
-      default: return f(F, std::integral_constant<int, 16>{});
-    }
-  });
+// sigmoid(z).  A 16-bit z has an error of 2^-9 (bf16) or 2^-12 of itself, against which that of rounding
+// z log2 e to fp32 does not count, so exp is one product and v_exp_f32 there.
+template <int F>
+__device__ __forceinline__ float gate_sigmoid(float z) {
+  if constexpr (F == kElemF32) return sigmoid_f(z);
+  return __builtin_amdgcn_rcpf(1.f + exp2_f(-kLog2e * z));
+}
+// z sigmoid(z), 1 where there is no z.
+template <int F>
+__device__ __forceinline__ float gate_of(float z, bool there) {
+  return there ? z * gate_sigmoid<F>(z) : 1.f;
 }
 
 }  // namespace hsl

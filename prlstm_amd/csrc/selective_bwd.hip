@@ -7,11 +7,11 @@
 // A workgroup walks its chunks from the last to the first: it runs a chunk's steps again from the
 // state that the forward kept, with every decay and state in registers, and then backwards.  The sums
 // over states go through LDS as y does in the forward.  db and dc are sums over channels, which are
-// lanes: four values of a step (the wave's states) are added over the four rows of 16 lanes while the
-// rows are exchanged between registers, which leaves one register with a state in each row, and the 16
-// such registers of a chunk are added over the 16 lanes of a row the same way (a lane keeps half of
-// what it has and hands on the other half), so that each lane ends with one finished sum; about 2 issue
-// slots a value instead of 6.  The workgroups' sums are added by a second kernel in their order.
+// lanes: four values of a step are added over the four rows of 16 lanes while the rows are exchanged
+// between registers, which leaves one register with a value in each row, and the 16 such registers of a
+// chunk are added over the 16 lanes of a row the same way (a lane keeps half of what it has and hands on
+// the other half), so that each lane ends with one finished sum; about 2 issue slots a value instead
+// of 6.  The workgroups' sums are added by a second kernel in their order.
 #include <algorithm>
 
 #include "selective.h"
@@ -29,95 +29,102 @@ struct Acc {
   }
 };
 
-// The state of the wave that add16(add32(v0, v1), add32(v2, v3)) leaves in row r.
-__device__ __forceinline__ int state_of_row(int r) { return (r & 1) * 2 + (r >> 1); }
-
-template <int F, int W>
+template <int F, class P>
 struct BwdChunk {
-  static constexpr int L = chunk_steps<W>(), PS = L >= W ? L / W : 1;
   using T_ = typename Elem<F>::T;
-  T_ x[PS], delta[PS], z[PS], dout[PS];
-  BcTile<F, W> bc;
-  unsigned cuts;
-  f4 h;
-  template <bool MAP>
-  __device__ __forceinline__ void load(const ScanArgs& a, const ScanPlace& q, int t0, int te, size_t row4) {
+  T_ x[P::PS], delta[P::PS], z[P::PS], dout[P::PS];
+  BcTile<F, P> bc;
+  unsigned char cut;
+  float h[P::S];
+};
+
+// The streams' rows of a wave, from the chunk that is loaded next, towards the first.
+template <int F, class P, bool MAP>
+struct BwdRows {
+  Rows<F, P> x, delta, z, dout;
+  __device__ __forceinline__ BwdRows(const ScanArgs& a, const ScanPlace<P>& q, int t0)
+      : x(a.x, q, t0), delta(a.delta, q, t0), z(a.z, q, t0), dout(a.dout, q, t0) {}
+  __device__ __forceinline__ void load(const ScanArgs& a, const ScanPlace<P>& q, unsigned off, int t0, int te,
+                                       BwdChunk<F, P>& m) {
 #pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      const int s = q.w + W * i, t = t0 + s;
-      const bool in = s < L && t < te && q.ok;
-      if (!MAP) x[i] = load_at<F>(a.x, t, q.b, q.ch, in);
-      delta[i] = load_at<F>(a.delta, t, q.b, q.ch, in);
-      z[i] = load_at<F>(a.z, t, q.b, q.ch, in && a.z.p);
-      dout[i] = load_at<F>(a.dout, t, q.b, q.ch, in && a.dout.p);
+    for (int i = 0; i < P::PS; ++i) {
+      const int s = q.w + P::W * i;
+      const bool in = s < P::L && t0 + s < te;
+      if (!MAP) m.x[i] = x.load(i, off, in);
+      m.delta[i] = delta.load(i, off, in);
+      m.z[i] = z.load(i, off, in);
+      m.dout[i] = dout.load(i, off, in);
     }
-    bc.load(a, q.b, t0, te);
-    cuts = load_cuts<L>(a.reset, t0, te, q.b, q.lane);
-    if (!MAP) {
-      h = f4{};
-      if (q.ok) h = load4(a.ck + ((size_t)(t0 / L) * a.B + q.b) * W * a.D * kS + row4);
-    }
+    m.bc.load(a, q.b, t0, te);
+    m.cut = load_cut<P::L>(a.reset, t0, te, q.b, q.lane);
+    if (!MAP) load_pairs(a.ck, q, a, (size_t)(t0 / P::L) * a.B + q.b, m.h);
+    x.move(-1);
+    delta.move(-1);
+    z.move(-1);
+    dout.move(-1);
   }
 };
 
 // U as it leaves the segments behind this one.
-template <int W>
-__device__ __forceinline__ void enter_reverse(const ScanArgs& a, const ScanPlace& q, int seg, const float (&a2)[kS],
-                                              float (&U)[kS]) {
+template <class P>
+__device__ __forceinline__ void enter_reverse(const ScanArgs& a, const ScanPlace<P>& q, int seg,
+                                              const float (&a2)[P::S], float (&U)[P::S]) {
   load_states(a.dh_n, q, a, U);
   for (int i = a.nseg - 1; i > seg; --i) {
     const float2 m = a.map_s[((size_t)(i - 1) * a.B + q.b) * a.D + q.ch];
-    const f4 v = load4(a.map_h + (((size_t)(i - 1) * a.B + q.b) * W * a.D + (size_t)q.w * a.D + q.ch) * kS);
+    float v[P::S];
+    load_pairs(a.map_h, q, a, (size_t)(i - 1) * a.B + q.b, v);
 #pragma unroll
-    for (int n = 0; n < kS; ++n)
-      U[n] = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), U[n], v[n]);
-    if (!q.ok)
-#pragma unroll
-      for (int n = 0; n < kS; ++n) U[n] = 0.f;
+    for (int n = 0; n < P::S; ++n) {
+      const float u = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), U[n], v[n]);
+      U[n] = q.ok ? u : 0.f;
+    }
   }
 }
 
 // The reverse map of segment blockIdx.y + 1.
-template <int F, int W>
-__global__ __launch_bounds__(W * 64) void scan_bwd_map_kernel(ScanArgs a) {
-  using Chunk = BwdChunk<F, W>;
-  constexpr int L = Chunk::L, PS = Chunk::PS;
+template <int F, class P>
+__global__ __launch_bounds__(P::W * 64) void scan_bwd_map_kernel(ScanArgs a) {
+  constexpr int L = P::L, S = P::S;
   __shared__ float2 sdt[L][64];  // dt, dy
-  __shared__ __attribute__((aligned(16))) float sb[L][W * kS], sc[L][W * kS];
-  const ScanPlace q(a);
+  __shared__ __attribute__((aligned(16))) float sb[L][P::N], sc[L][P::N];
+  const ScanPlace<P> q(a);
+  const unsigned off = q.ok ? q.ch * (unsigned)sizeof(typename Elem<F>::T) : kOffNone;
   const int seg = blockIdx.y + 1, tb = seg * a.seg_steps, te = min(a.T, tb + a.seg_steps);
-  const size_t row4 = ((size_t)q.w * a.D + q.ch) * kS;
-  float a2[kS], U[kS] = {};
+  const bool gated = a.z.p != nullptr, soft = a.softplus != 0;
+  float a2[S], U[S] = {};
   load_a2(q, a, a2);
   const float bias = a.bias ? a.bias[q.ch] : 0.f;
   Acc total;
   unsigned any = 0;
-  Chunk m;
+  BwdChunk<F, P> m;
   const int first = tb + (te - tb - 1) / L * L;
-  m.template load<true>(a, q, first, te, row4);
+  BwdRows<F, P, true> rows(a, q, first);
+  rows.load(a, q, off, first, te, m);
   for (int t0 = first; t0 >= tb; t0 -= L) {
 #pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      const int s = q.w + W * i;
-      if (s >= L) break;
-      const float u = Elem<F>::up(m.delta[i]) + bias, z = Elem<F>::up(m.z[i]);
-      float dt = a.softplus ? softplus_f(u, exp_f(-__builtin_fabsf(u))) : u, dy = Elem<F>::up(m.dout[i]);
-      if (t0 + s >= te || !q.ok) dt = 0.f;
-      if (a.z.p) dy *= z * sigmoid_f(z);
-      sdt[s][q.lane] = float2{dt, dy};
+    for (int i = 0; i < P::PS; ++i) {
+      const int s = q.w + P::W * i;
+      if (L < P::W && s >= L) break;
+      const float u = Elem<F>::up(m.delta[i]) + bias;
+      float dt = softplus_f(u, exp_f(-__builtin_fabsf(u)));
+      dt = soft ? dt : u;
+      dt = t0 + s < te && q.ok ? dt : 0.f;
+      sdt[s][q.lane] = float2{dt, Elem<F>::up(m.dout[i]) * gate_of<F>(Elem<F>::up(m.z[i]), gated)};
     }
     m.bc.store(sb, sc);
-    const unsigned cuts = m.cuts;
+    const unsigned cuts = cuts_of(a.reset, m.cut);
     any |= cuts;
     lds_barrier();
-    if (t0 > tb) m.template load<true>(a, q, t0 - L, te, row4);
+    if (t0 > tb) rows.load(a, q, off, t0 - L, te, m);
     float part = 0.f;
 #pragma unroll
     for (int s = L - 1; s >= 0; --s) {
       const float2 d = sdt[s][q.lane];
-      const f4 c = load4(&sc[s][q.n0]);
+      float c[S];
+      load_row<S>(&sc[s][q.n0], c);
 #pragma unroll
-      for (int n = 0; n < kS; ++n) {
+      for (int n = 0; n < S; ++n) {
         const float v = exp2_f(d.x * a2[n]) * __builtin_fmaf(c[n], d.y, U[n]);
         U[n] = cuts >> s & 1 ? 0.f : v;
       }
@@ -127,98 +134,133 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_map_kernel(ScanArgs a) {
     lds_barrier();
   }
   if (!q.ok) return;
-  const f4 v = {U[0], U[1], U[2], U[3]};
-  *reinterpret_cast<f4*>(a.map_h + ((size_t)blockIdx.y * a.B + q.b) * W * a.D * kS + row4) = v;
+  store_pairs(a.map_h, q, a, (size_t)blockIdx.y * a.B + q.b, U);
   if (q.w == 0) a.map_s[((size_t)blockIdx.y * a.B + q.b) * a.D + q.ch] = float2{total.sum, any ? 1.f : 0.f};
 }
 
-template <int F, int W>
-__global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanArgs a) {
-  using Chunk = BwdChunk<F, W>;
-  using T_ = typename Elem<F>::T;
-  constexpr int L = Chunk::L, PS = Chunk::PS;
+template <int F, class P>
+__global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
+  constexpr int L = P::L, PS = P::PS, S = P::S, W = P::W;
   __shared__ float2 sdt[L][64];  // dt, dt x
   __shared__ float sdy[L][64];
-  __shared__ __attribute__((aligned(16))) float sb[L][W * kS], sc[L][W * kS];
+  __shared__ __attribute__((aligned(16))) float sb[L][P::N], sc[L][P::N];
   __shared__ float sp[3][W][L][64];  // the waves' parts of sum G b, sum a P and y
-  const ScanPlace q(a);
+  const ScanPlace<P> q(a);
+  const unsigned off = q.ok ? q.ch * (unsigned)sizeof(typename Elem<F>::T) : kOffNone;
   const int seg = blockIdx.y, tb = seg * a.seg_steps, te = min(a.T, tb + a.seg_steps);
-  const size_t row4 = ((size_t)q.w * a.D + q.ch) * kS;
+  const bool gated = a.z.p != nullptr, soft = a.softplus != 0;
   const bool tail = (q.tile + 1) * kChannels > a.D;  // lanes without a channel
-  float a2[kS], an[kS], U[kS];
+  float a2[S], an[S], U[S];
   load_a2(q, a, a2);
 #pragma unroll
-  for (int n = 0; n < kS; ++n) an[n] = q.n0 + n < a.N ? a.a[(size_t)q.ch * a.N + q.n0 + n] : 0.f;
+  for (int n = 0; n < S; ++n) an[n] = q.n0 + n < a.N ? a.a[(size_t)q.ch * a.N + q.n0 + n] : 0.f;
   const float bias = a.bias ? a.bias[q.ch] : 0.f, skip = a.d ? a.d[q.ch] : 0.f;
-  enter_reverse<W>(a, q, seg, a2, U);
-  Acc da[kS], dskip, dbias;
+  enter_reverse(a, q, seg, a2, U);
+  Acc da[S], dskip, dbias;
 
-  Chunk m;
+  BwdChunk<F, P> m;  // the loads of the next chunk
   // what A leaves for C
-  float kx[PS], kdt[PS], ksig[PS], kdy[PS], kdo[PS], kz[PS];
+  float kx[PS], kdt[PS], ksig[PS], kdo[PS], kz[PS];
   unsigned cuts = 0;
-  f4 h0v{};
+  float hin[S];
   auto stage = [&](int t0) {
-    cuts = m.cuts;
-    h0v = m.h;
+    cuts = cuts_of(a.reset, m.cut);
+#pragma unroll
+    for (int n = 0; n < S; ++n) hin[n] = q.ok ? m.h[n] : 0.f;
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
       const int s = q.w + W * i;
-      if (s >= L) break;
-      const float x = Elem<F>::up(m.x[i]), u = Elem<F>::up(m.delta[i]) + bias, z = Elem<F>::up(m.z[i]);
-      float dt = u, sig = 1.f, dy = Elem<F>::up(m.dout[i]);
-      kdo[i] = dy;
-      if (a.softplus) {
-        const float e = exp_f(-__builtin_fabsf(u)), r = __builtin_amdgcn_rcpf(1.f + e);
-        dt = softplus_f(u, e);
-        sig = u >= 0.f ? r : e * r;
-        if (u != u) sig = u;
-      }
-      if (t0 + s >= te || !q.ok) dt = 0.f;
-      if (a.z.p) dy *= z * sigmoid_f(z);
+      if (L < W && s >= L) break;
+      const float x = Elem<F>::up(m.x[i]), u = Elem<F>::up(m.delta[i]) + bias;
+      const float e = exp_f(-__builtin_fabsf(u)), r = __builtin_amdgcn_rcpf(1.f + e);
+      float dt = softplus_f(u, e), sig = u >= 0.f ? r : e * r;
+      dt = soft ? dt : u;
+      ksig[i] = soft ? sig : 1.f;
+      dt = t0 + s < te && q.ok ? dt : 0.f;
+      kdo[i] = Elem<F>::up(m.dout[i]);
+      kz[i] = Elem<F>::up(m.z[i]);
       sdt[s][q.lane] = float2{dt, dt * x};
-      sdy[s][q.lane] = dy;
+      sdy[s][q.lane] = kdo[i] * gate_of<F>(kz[i], gated);
       kx[i] = x;
       kdt[i] = dt;
-      ksig[i] = sig;
-      kdy[i] = dy;
-      kz[i] = z;
     }
     m.bc.store(sb, sc);
   };
   // SLOW: a reset in the chunk, or lanes without a channel
   auto run = [&](auto slow, int t0) {
     constexpr bool SLOW = decltype(slow)::value;
-    float f[L][kS], hs[L][kS], h[kS] = {h0v[0], h0v[1], h0v[2], h0v[3]};
+    constexpr int G = 4;  // steps whose operands are read from LDS ahead
+    float f[L][S], hs[L][S], h[S];
 #pragma unroll
-    for (int s = 0; s < L; ++s) {
-      const float2 dt = sdt[s][q.lane];
-      const f4 b = load4(&sb[s][q.n0]);
+    for (int n = 0; n < S; ++n) h[n] = hin[n];
+    {
+      struct Ahead {
+        float2 dt[G];
+        float b[G][S];
+      } r[2];
+      auto read = [&](int s0, Ahead& v) {
 #pragma unroll
-      for (int n = 0; n < kS; ++n) {
-        f[s][n] = exp2_f(dt.x * a2[n]);
-        const float v = dt.y * b[n], g = __builtin_fmaf(f[s][n], h[n], v);
-        h[n] = SLOW && (cuts >> s & 1) ? v : g;
-        hs[s][n] = h[n];
+        for (int s = 0; s < G; ++s) {
+          v.dt[s] = sdt[s0 + s][q.lane];
+          load_row<S>(&sb[s0 + s][q.n0], v.b[s]);
+        }
+      };
+      read(0, r[0]);
+#pragma unroll
+      for (int s0 = 0; s0 < L; s0 += G) {
+        if (s0 + G < L) read(s0 + G, r[(s0 / G + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
+        const Ahead& v = r[(s0 / G) & 1];
+#pragma unroll
+        for (int k = 0; k < G; ++k)
+#pragma unroll
+          for (int n = 0; n < S; ++n) {
+            const int s = s0 + k;
+            f[s][n] = exp2_f(v.dt[k].x * a2[n]);
+            const float e = v.dt[k].y * v.b[k][n], g = __builtin_fmaf(f[s][n], h[n], e);
+            h[n] = SLOW && (cuts >> s & 1) ? e : g;
+            hs[s][n] = h[n];
+          }
       }
     }
-    float rb[16], rc[16], cda[kS] = {};
+    constexpr int kRegs = L * S / 2;  // of sums over rows, four values each
+    float sums[kRegs / 16][16], cda[S] = {};
+    struct Ahead {
+      float2 dt[G];
+      float dy[G], b[G][S], c[G][S];
+    } r[2];
+    auto read = [&](int s0, Ahead& v) {
+#pragma unroll
+      for (int s = 0; s < G; ++s) {
+        v.dt[s] = sdt[s0 + s][q.lane];
+        v.dy[s] = sdy[s0 + s][q.lane];
+        load_row<S>(&sb[s0 + s][q.n0], v.b[s]);
+        load_row<S>(&sc[s0 + s][q.n0], v.c[s]);
+      }
+    };
+    read(L - G, r[(L / G - 1) & 1]);
 #pragma unroll
     for (int s = L - 1; s >= 0; --s) {
-      const float2 dt = sdt[s][q.lane];
-      const float dy = sdy[s][q.lane];
-      const f4 b = load4(&sb[s][q.n0]), c = load4(&sc[s][q.n0]);
+      if (s % G == G - 1) {
+        if (s >= G) read(s / G * G - G, r[(s / G - 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
+      }
+      const Ahead& v = r[(s / G) & 1];
+      const float2 dt = v.dt[s % G];
+      const float dy = v.dy[s % G];
+      const float(&b)[S] = v.b[s % G];
+      const float(&c)[S] = v.c[s % G];
       const bool cut = SLOW && (cuts >> s & 1);
-      float gb = 0.f, ap = 0.f, y = 0.f, vb[kS], vc[kS];
+      float gb = 0.f, ap = 0.f, y = 0.f, vb[S], vc[S];
 #pragma unroll
-      for (int n = 0; n < kS; ++n) {
+      for (int n = 0; n < S; ++n) {
         const float G = __builtin_fmaf(c[n], dy, U[n]);
         y = __builtin_fmaf(c[n], hs[s][n], y);
         gb = __builtin_fmaf(G, b[n], gb);
         vb[n] = G * dt.y;
         vc[n] = dy * hs[s][n];
         U[n] = G * f[s][n];
-        float p = U[n] * (s ? hs[s ? s - 1 : 0][n] : h0v[n]);
+        float p = U[n] * (s ? hs[s ? s - 1 : 0][n] : hin[n]);
         if (cut) U[n] = p = 0.f;
         ap = __builtin_fmaf(an[n], p, ap);
         cda[n] = __builtin_fmaf(dt.x, p, cda[n]);
@@ -227,42 +269,36 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanArgs a) {
       sp[0][q.w][s][q.lane] = gb;
       sp[1][q.w][s][q.lane] = ap;
       sp[2][q.w][s][q.lane] = y;
-      const float sum_b = add16(add32(vb[0], vb[1]), add32(vb[2], vb[3]));
-      const float sum_c = add16(add32(vc[0], vc[1]), add32(vc[2], vc[3]));
-      if constexpr (L == 16) {
-        rb[s] = sum_b;
-        rc[s] = sum_c;
-      } else {
-        rb[s] = sum_b;
-        rb[8 + s] = sum_c;
+      // rows 0..3: b of state n, c of state n, b of state n + 1, c of state n + 1
+#pragma unroll
+      for (int n = 0; n < S; n += 2) {
+        const int r = s * (S / 2) + n / 2;
+        sums[r / 16][r % 16] = add16(add32(vb[n], vb[n + 1]), add32(vc[n], vc[n + 1]));
       }
     }
 #pragma unroll
-    for (int n = 0; n < kS; ++n) da[n].add(cda[n]);
-    const int i = q.lane & 15, n = q.n0 + state_of_row(q.lane >> 4);
-    float* const out = a.part_bc + ((size_t)q.tile * a.T * a.B + q.b) * (2 * W * kS) + n;
-    const size_t step = (size_t)a.B * (2 * W * kS);
-    if constexpr (L == 16) {
-      const float vb = sum_rows(rb, q.lane), vc = sum_rows(rc, q.lane);
-      if (t0 + i < te) {
-        out[(t0 + i) * step] = vb;
-        out[(t0 + i) * step + W * kS] = vc;
-      }
-    } else {
-      const float v = sum_rows(rb, q.lane);
-      const int s = i & 7;
-      if (t0 + s < te) out[(t0 + s) * step + (i >> 3) * (W * kS)] = v;
+    for (int n = 0; n < S; ++n) da[n].add(cda[n]);
+    const int row = q.lane >> 4;
+    float* const out = a.part_bc + (((size_t)q.tile * a.T + t0) * a.B + q.b) * (2 * P::N) + (row & 1) * P::N + q.n0 +
+                       (row >> 1);
+#pragma unroll
+    for (int k = 0; k < kRegs / 16; ++k) {
+      const float v = sum_rows(sums[k], q.lane);
+      const int r = 16 * k + (q.lane & 15), s = r / (S / 2), n = r % (S / 2) * 2;
+      if (t0 + s < te) out[(size_t)s * a.B * (2 * P::N) + n] = v;
     }
   };
 
   const int first = te > tb ? tb + (te - tb - 1) / L * L : tb - L;
+  BwdRows<F, P, false> rows(a, q, first);
+  Rows<F, P> dxr(a.dx, q, first), ddr(a.ddelta, q, first), dzr(a.dz, q, first);
   if (te > tb) {
-    m.template load<false>(a, q, first, te, row4);
+    rows.load(a, q, off, first, te, m);
     stage(first);
   }
   lds_barrier();
   for (int t0 = first; t0 >= tb; t0 -= L) {
-    if (t0 > tb) m.template load<false>(a, q, t0 - L, te, row4);
+    if (t0 > tb) rows.load(a, q, off, t0 - L, te, m);
     if (cuts || tail)
       run(std::true_type{}, t0);
     else
@@ -272,7 +308,7 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
       const int s = q.w + W * i, t = t0 + s;
-      if (s >= L || t >= te || !q.ok) continue;
+      if (L < W && s >= L) break;
       float gb = 0.f, ap = 0.f, y = skip * kx[i];
 #pragma unroll
       for (int v = 0; v < W; ++v) {
@@ -280,27 +316,31 @@ __global__ __launch_bounds__(W * 64) void scan_bwd_kernel(ScanArgs a) {
         ap += sp[1][v][s][q.lane];
         y += sp[2][v][s][q.lane];
       }
+      const float sg = gate_sigmoid<F>(kz[i]), slope = __builtin_fmaf(kz[i] * sg, 1.f - sg, sg);
+      const float dy = kdo[i] * (gated ? kz[i] * sg : 1.f);
       const float ddelta = __builtin_fmaf(kx[i], gb, ap) * ksig[i];
-      cskip = __builtin_fmaf(kdy[i], kx[i], cskip);
-      cbias += ddelta;
-      const float dx = __builtin_fmaf(kdt[i], gb, skip * kdy[i]);
-      static_cast<T_*>(a.dx.p)[t * a.dx.st + q.b * a.dx.sb + q.ch] = Elem<F>::down(dx);
-      static_cast<T_*>(a.ddelta.p)[t * a.ddelta.st + q.b * a.ddelta.sb + q.ch] = Elem<F>::down(ddelta);
-      if (a.z.p) {
-        const float sg = sigmoid_f(kz[i]), slope = __builtin_fmaf(kz[i] * sg, 1.f - sg, sg);
-        static_cast<T_*>(a.dz.p)[t * a.dz.st + q.b * a.dz.sb + q.ch] = Elem<F>::down(kdo[i] * y * slope);
-      }
+      const bool in = t < te;
+      cskip = __builtin_fmaf(dy, kx[i], cskip);
+      cbias += in && q.ok ? ddelta : 0.f;
+      dxr.store(i, off, in, __builtin_fmaf(kdt[i], gb, skip * dy));
+      ddr.store(i, off, in, ddelta);
+      dzr.store(i, off, in && gated, kdo[i] * y * slope);
     }
     dskip.add(cskip);
     dbias.add(cbias);
+    dxr.move(-1);
+    ddr.move(-1);
+    dzr.move(-1);
     if (t0 > tb) stage(t0 - L);
     lds_barrier();
   }
   if (seg == 0 && a.dh0) store_states(a.dh0, q, a, U);
   const size_t part = (size_t)q.b * a.nseg + seg;
   if (q.ok) {
-    const f4 v = {da[0].sum, da[1].sum, da[2].sum, da[3].sum};
-    *reinterpret_cast<f4*>(a.part_a + part * W * a.D * kS + row4) = v;
+    float v[S];
+#pragma unroll
+    for (int n = 0; n < S; ++n) v[n] = da[n].sum;
+    store_pairs(a.part_a, q, a, part, v);
   }
   sp[0][q.w][0][q.lane] = dskip.sum;
   sp[1][q.w][0][q.lane] = dbias.sum;
@@ -337,10 +377,10 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
 // da [D][N], dd and ddelta_bias [D] from the workgroups' sums, in fp64.
 __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__ part_a,
                                                        const float* __restrict__ part_d, float* da, float* dd,
-                                                       float* dbias, int rows, int D, int N, int W) {
+                                                       float* dbias, int rows, int D, int N, int states) {
   __shared__ double sm[4][64];
   const int c = threadIdx.x & 63, strip = threadIdx.x >> 6;
-  const long long na = (long long)W * D * kS, all = na + 2 * D, i = (long long)blockIdx.x * 64 + c;
+  const long long na = (long long)states * D, all = na + 2 * D, i = (long long)blockIdx.x * 64 + c;
   double v = 0.0;
   if (i < all)
     for (int r = strip; r < rows; r += 4)
@@ -350,14 +390,28 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__
   if (strip || i >= all) return;
   const float s = (float)((sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]));
   if (i < na) {
-    const long long wd = i / kS;
-    const int n = (int)(wd / D) * kS + (int)(i % kS);
-    if (n < N) da[wd % D * N + n] = s;
+    const long long pd = i / 2;
+    const int n = (int)(pd / D) * 2 + (int)(i % 2);
+    if (n < N) da[pd % D * N + n] = s;
   } else {
     const long long j = i - na;
     float* const o = j < D ? dd : dbias;
     if (o) o[j % D] = s;
   }
+}
+
+// f(integral_constant fmt, ScanShape).
+template <class Fn>
+int with_bwd_shape(int fmt, int N, Fn f) {
+  return with_fmt(fmt, [&](auto F) {
+    switch (scan_states(N)) {
+      case 4: return f(F, ScanShape<2, 2>{});
+      case 8: return f(F, ScanShape<4, 2>{});
+      case 16: return f(F, ScanShape<8, 2>{});
+      case 32: return f(F, ScanShape<8, 4>{});
+      default: return f(F, ScanShape<16, 4>{});
+    }
+  });
 }
 
 // The pieces of a workspace, in floats.
@@ -366,7 +420,7 @@ struct BwdLayout {
 };
 BwdLayout bwd_layout(int T, int B, int D, int N) {
   const ScanPlan p = plan_scan(T, B, D, N);
-  const size_t states = (size_t)scan_waves(N) * kS, bd = (size_t)B * D;
+  const size_t states = scan_states(N), bd = (size_t)B * D;
   BwdLayout l;
   size_t off = 0;
   auto take = [&](size_t n) {
@@ -445,26 +499,26 @@ int hsl_selective_bwd(const void* x, long long x_t, long long x_b, const void* d
   g.softplus = softplus;
   g.seg_steps = p.seg_steps;
   g.nseg = p.nseg;
-  const int W = scan_waves(N);
   if (B > 0)
-    HSL_CHECK(with_scan(fmt, N, [&](auto F, auto WW) {
-      constexpr int kF = decltype(F)::value, kW = decltype(WW)::value;
+    HSL_CHECK(with_bwd_shape(fmt, N, [&](auto F, auto shape) {
+      constexpr int kF = decltype(F)::value;
+      using P = decltype(shape);
       if (p.nseg > 1 && D > 0)
-        hipLaunchKernelGGL((scan_bwd_map_kernel<kF, kW>), dim3(p.tiles * B, p.nseg - 1), dim3(kW * 64), 0, s, g);
+        hipLaunchKernelGGL((scan_bwd_map_kernel<kF, P>), dim3(p.tiles * B, p.nseg - 1), dim3(P::W * 64), 0, s, g);
       if (D > 0)
-        hipLaunchKernelGGL((scan_bwd_kernel<kF, kW>), dim3(p.tiles * B, p.nseg), dim3(kW * 64), 0, s, g);
+        hipLaunchKernelGGL((scan_bwd_kernel<kF, P>), dim3(p.tiles * B, p.nseg), dim3(P::W * 64), 0, s, g);
       if (T > 0) {  // zeros where there is no channel
-        const long long n = ((long long)T * B * 2 * kW * kS + 255) / 256;
+        const long long n = ((long long)T * B * 2 * P::N + 255) / 256;
         hipLaunchKernelGGL((scan_bc_kernel<kF>), dim3((unsigned)std::min<long long>(n, 1 << 20)), dim3(256), 0, s,
-                           g.part_bc, OutStream{db, db_t, db_b}, OutStream{dc, dc_t, dc_b}, T, B, N, kW * kS, p.tiles);
+                           g.part_bc, OutStream{db, db_t, db_b}, OutStream{dc, dc_t, dc_b}, T, B, N, P::N, p.tiles);
       }
       HSL_HIP(hipGetLastError());
       return (int)HSL_OK;
     }));
   if (D == 0) return HSL_OK;
-  const long long cols = (long long)W * D * kS + 2 * D;
+  const long long cols = ((long long)scan_states(N) + 2) * D;
   hipLaunchKernelGGL(scan_sum_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, g.part_a, g.part_d, da, dd,
-                     ddelta_bias, B * p.nseg, D, N, W);
+                     ddelta_bias, B * p.nseg, D, N, scan_states(N));
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }

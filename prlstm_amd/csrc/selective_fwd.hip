@@ -11,13 +11,12 @@ namespace hsl {
 ScanPlan plan_scan(int T, int B, int D, int N) {
   ScanPlan p;
   p.tiles = (D + kChannels - 1) / kChannels;
-  const int chunk = scan_chunk(N), waves = scan_waves(N);
-  const int nchunks = (T + chunk - 1) / chunk;
-  const long long have = (long long)p.tiles * B * waves;
+  const int chunk = scan_chunk(N), nchunks = (T + chunk - 1) / chunk;
+  const long long have = (long long)p.tiles * B;
   p.nseg = 1;
   p.seg_steps = std::max(1, nchunks) * chunk;
-  if (have < 768 && nchunks >= 8) {
-    const int want = (int)std::min<long long>(nchunks / 4, (2048 + have - 1) / std::max(1ll, have));
+  if (have < 192 && nchunks >= 8) {
+    const int want = (int)std::min<long long>(nchunks / 4, (512 + have - 1) / std::max(1ll, have));
     const int per = (nchunks + want - 1) / want;
     p.seg_steps = per * chunk;
     p.nseg = (nchunks + per - 1) / per;
@@ -31,154 +30,199 @@ int check_scan(const char* who, int T, int B, int D, int N, int fmt) {
   if (N < 1 || N > kMaxStates) return fail(HSL_ERR_ARG, "%s: %d states, must be 1..%d", who, N, kMaxStates);
   // steps and channels are counted in 32 bits; a launch holds fewer than 2^32 threads
   if (T >= (1 << 30) || (long long)B * D >= (1ll << 27) ||
-      (long long)B * ((D + kChannels - 1) / kChannels) * scan_waves(N) >= (1ll << 25))
+      (long long)B * ((D + kChannels - 1) / kChannels) * (scan_states(N) / 4) >= (1ll << 24))
     return fail(HSL_ERR_UNSUPPORTED,
                 "%s: T=%d B=%d D=%d N=%d is beyond the kernels' 32-bit index range (needs T < 2^30, B*D < 2^27 and "
-                "B*ceil(D/64)*ceil(N/4) < 2^25)",
+                "B*ceil(D/64)*ceil(N/4) < 2^24)",
                 who, T, B, D, N);
   return HSL_OK;
 }
 
 namespace {
 
-template <int F, int W>
+template <int F, class P>
 struct FwdChunk {
-  static constexpr int L = chunk_steps<W>(), PS = L >= W ? L / W : 1;
   using T_ = typename Elem<F>::T;
-  T_ x[PS], delta[PS], z[PS];
-  BcTile<F, W> bc;
-  unsigned cuts;
-  template <bool MAP>
-  __device__ __forceinline__ void load(const ScanArgs& a, const ScanPlace& q, int t0, int te) {
-#pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      const int s = q.w + W * i, t = t0 + s;
-      const bool in = s < L && t < te && q.ok;
-      x[i] = load_at<F>(a.x, t, q.b, q.ch, in);
-      delta[i] = load_at<F>(a.delta, t, q.b, q.ch, in);
-      if (!MAP) z[i] = load_at<F>(a.z, t, q.b, q.ch, in && a.z.p);
-    }
-    bc.load(a, q.b, t0, te);
-    cuts = load_cuts<L>(a.reset, t0, te, q.b, q.lane);
-  }
+  T_ x[P::PS], delta[P::PS], z[P::PS];
+  BcTile<F, P> bc;
+  unsigned char cut;
 };
 
-// MAP: only each segment's map (nothing of the last segment, whose map nothing reads).
-template <int F, int W, bool MAP>
-__global__ __launch_bounds__(W * 64) void scan_fwd_kernel(ScanArgs a) {
-  constexpr int L = chunk_steps<W>(), PS = FwdChunk<F, W>::PS;
-  using T_ = typename Elem<F>::T;
-  __shared__ float2 sdt[L][64];
-  __shared__ __attribute__((aligned(16))) float sb[L][W * kS], sc[L][W * kS];
-  __shared__ float sy[MAP ? 1 : W][MAP ? 1 : L][64];
-  const ScanPlace q(a);
+// MAP: only each segment's map (nothing of the last segment, whose map nothing reads).  What B and C
+// read is kept twice, so that one barrier a chunk is enough: a wave is in C of chunk k or B of chunk
+// k + 1 while another still is in C of chunk k, and A of chunk k + 2 comes behind the next barrier.
+template <int F, class P, bool MAP>
+__global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
+  constexpr int L = P::L, PS = P::PS, S = P::S, W = P::W;
+  __shared__ float2 sdt[2][L][64];
+  __shared__ __attribute__((aligned(16))) float sb[2][L][P::N], sc[2][L][P::N];
+  __shared__ float sy[2][MAP ? 1 : W][MAP ? 1 : L][64];
+  const ScanPlace<P> q(a);
+  const unsigned off = q.ok ? q.ch * (unsigned)sizeof(typename Elem<F>::T) : kOffNone;
   const int seg = blockIdx.y, tb = seg * a.seg_steps, te = min(a.T, tb + a.seg_steps);
-  float a2[kS], h[kS];
+  const bool gated = a.z.p != nullptr, soft = a.softplus != 0;
+  float a2[S], h[S];
   load_a2(q, a, a2);
   const float bias = a.bias ? a.bias[q.ch] : 0.f, skip = a.d ? a.d[q.ch] : 0.f;
-  const size_t row4 = ((size_t)q.w * a.D + q.ch) * kS, rows4 = (size_t)W * a.D * kS;  // of a [B][W][D][4]
   if (MAP) {
 #pragma unroll
-    for (int n = 0; n < kS; ++n) h[n] = 0.f;
+    for (int n = 0; n < S; ++n) h[n] = 0.f;
   } else {
     load_states(a.h0, q, a, h);
     for (int i = 0; i < seg; ++i) {
       const float2 m = a.map_s[((size_t)i * a.B + q.b) * a.D + q.ch];
-      const f4 v = load4(a.map_h + ((size_t)i * a.B + q.b) * rows4 + row4);
+      float v[S];
+      load_pairs(a.map_h, q, a, (size_t)i * a.B + q.b, v);
 #pragma unroll
-      for (int n = 0; n < kS; ++n)
+      for (int n = 0; n < S; ++n)
         h[n] = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), h[n], v[n]);
     }
   }
   float total = 0.f, low = 0.f;  // the sum of dt and what its roundings lost
-  unsigned any = 0;
+  unsigned any = 0, cuts = 0;
 
-  FwdChunk<F, W> now, next;
-  // what A leaves for C
-  float keep_x[PS], keep_z[PS];
-  auto stage = [&](const FwdChunk<F, W>& m, int t0) {
-    now.cuts = m.cuts;
+  FwdChunk<F, P> next;  // the loads of the next chunk
+  Rows<F, P> xr(a.x, q, tb), dr(a.delta, q, tb), zr(a.z, q, tb), yr(a.y, q, tb);
+  auto load = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
       const int s = q.w + W * i;
-      if (s >= L) break;
-      const float x = Elem<F>::up(m.x[i]), u = Elem<F>::up(m.delta[i]) + bias;
-      float dt = a.softplus ? softplus_f(u, exp_f(-__builtin_fabsf(u))) : u;
-      if (t0 + s >= te || !q.ok) dt = 0.f;
-      sdt[s][q.lane] = float2{dt, dt * x};
-      keep_x[i] = x;
-      if (!MAP) keep_z[i] = Elem<F>::up(m.z[i]);
+      const bool in = s < L && t0 + s < te;
+      next.x[i] = xr.load(i, off, in);
+      next.delta[i] = dr.load(i, off, in);
+      if (!MAP) next.z[i] = zr.load(i, off, in);
     }
-    m.bc.store(sb, sc);
+    next.bc.load(a, q.b, t0, te);
+    next.cut = load_cut<L>(a.reset, t0, te, q.b, q.lane);
+    xr.move(1);
+    dr.move(1);
+    zr.move(1);
   };
-  auto run = [&](auto cut) {
+  float x_now[PS], z_now[PS], x_next[PS], z_next[PS];  // what A leaves for C
+  auto stage = [&](int t0, int par) {  // A
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const int s = q.w + W * i;
+      if (L < W && s >= L) break;
+      const float x = Elem<F>::up(next.x[i]), u = Elem<F>::up(next.delta[i]) + bias;
+      float dt = softplus_f(u, exp_f(-__builtin_fabsf(u)));
+      dt = soft ? dt : u;
+      dt = t0 + s < te && q.ok ? dt : 0.f;
+      sdt[par][s][q.lane] = float2{dt, dt * x};
+      x_next[i] = x;
+      if (!MAP) z_next[i] = Elem<F>::up(next.z[i]);
+    }
+    next.bc.store(sb[par], sc[par]);
+  };
+  auto run = [&](auto cut, int par) {  // B
     constexpr bool CUT = decltype(cut)::value;
-    float part = 0.f;
+    constexpr int G = 4;  // steps whose operands are read from LDS ahead
+    struct Ahead {
+      float2 dt[G];
+      float b[G][S], c[G][S];
+    } r[2];
+    auto read = [&](int s0, Ahead& v) {
 #pragma unroll
-    for (int s = 0; s < L; ++s) {
-      const float2 dt = sdt[s][q.lane];
-      const f4 b = load4(&sb[s][q.n0]), c = MAP ? f4{} : load4(&sc[s][q.n0]);
-      const bool zero = CUT && (now.cuts >> s & 1);
-      float y = 0.f;
-#pragma unroll
-      for (int n = 0; n < kS; ++n) {
-        const float f = exp2_f(dt.x * a2[n]), v = dt.y * b[n];
-        const float g = __builtin_fmaf(f, h[n], v);
-        h[n] = zero ? v : g;
-        if (!MAP) y = n ? __builtin_fmaf(c[n], h[n], y) : c[n] * h[n];
+      for (int s = 0; s < G; ++s) {
+        v.dt[s] = sdt[par][s0 + s][q.lane];
+        load_row<S>(&sb[par][s0 + s][q.n0], v.b[s]);
+        if (!MAP) load_row<S>(&sc[par][s0 + s][q.n0], v.c[s]);
       }
-      if (MAP) part += dt.x;
-      if (!MAP) sy[q.w][s][q.lane] = y;
+    };
+    float part = 0.f;
+    read(0, r[0]);
+#pragma unroll
+    for (int s0 = 0; s0 < L; s0 += G) {
+      if (s0 + G < L) read(s0 + G, r[(s0 / G + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
+      const Ahead& v = r[(s0 / G) & 1];
+#pragma unroll
+      for (int k = 0; k < G; ++k) {
+        const int s = s0 + k;
+        const bool zero = CUT && (cuts >> s & 1);
+        float y = 0.f;
+#pragma unroll
+        for (int n = 0; n < S; ++n) {
+          const float f = exp2_f(v.dt[k].x * a2[n]), e = v.dt[k].y * v.b[k][n];
+          const float g = __builtin_fmaf(f, h[n], e);
+          h[n] = zero ? e : g;
+          if (!MAP) y = n ? __builtin_fmaf(v.c[k][n], h[n], y) : v.c[k][n] * h[n];
+        }
+        if (MAP) part += v.dt[k].x;
+        if (!MAP) sy[par][q.w][s][q.lane] = y;
+      }
     }
     if (MAP) {  // compensated: thousands of small dt
       const float v = part - low, t = total + v;
       low = (t - total) - v;
       total = t;
-      any |= now.cuts;
+      any |= cuts;
     }
   };
 
   if (tb < te) {
-    next.template load<MAP>(a, q, tb, te);
-    stage(next, tb);
+    load(tb);
+    stage(tb, 0);
+    cuts = cuts_of(a.reset, next.cut);
+    if (tb + L < te) load(tb + L);
   }
   lds_barrier();
-  for (int t0 = tb; t0 < te; t0 += L) {
-    const bool more = t0 + L < te;
-    if (more) next.template load<MAP>(a, q, t0 + L, te);
-    if (!MAP && a.ck && q.ok) {
-      const f4 v = {h[0], h[1], h[2], h[3]};
-      __builtin_nontemporal_store(v, reinterpret_cast<f4*>(a.ck + ((size_t)(t0 / L) * a.B + q.b) * rows4 + row4));
+  int par = 0;
+  for (int t0 = tb; t0 < te; t0 += L, par ^= 1) {
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      x_now[i] = x_next[i];
+      if (!MAP) z_now[i] = z_next[i];
     }
-    if (now.cuts)
-      run(std::true_type{});
+    if (!MAP && a.ck && q.ok) store_pairs(a.ck, q, a, (size_t)(t0 / L) * a.B + q.b, h);
+    if (cuts)
+      run(std::true_type{}, par);
     else
-      run(std::false_type{});
+      run(std::false_type{}, par);
+    if (t0 + L < te) {
+      stage(t0 + L, par ^ 1);
+      cuts = cuts_of(a.reset, next.cut);
+      if (t0 + 2 * L < te) load(t0 + 2 * L);
+    }
     lds_barrier();
-    if (!MAP) {
+    if (!MAP) {  // C
 #pragma unroll
       for (int i = 0; i < PS; ++i) {
         const int s = q.w + W * i, t = t0 + s;
-        if (s >= L || t >= te || !q.ok) continue;
-        float y = skip * keep_x[i];
+        if (L < W && s >= L) break;
+        float y = skip * x_now[i];
 #pragma unroll
-        for (int v = 0; v < W; ++v) y += sy[v][s][q.lane];
-        if (a.z.p) y *= keep_z[i] * sigmoid_f(keep_z[i]);
-        static_cast<T_*>(a.y.p)[t * a.y.st + q.b * a.y.sb + q.ch] = Elem<F>::down(y);
+        for (int v = 0; v < W; ++v) y += sy[par][v][s][q.lane];
+        y *= gate_of<F>(z_now[i], gated);
+        yr.store(i, off, t < te, y);
       }
+      yr.move(1);
     }
-    if (more) stage(next, t0 + L);
-    lds_barrier();
   }
   if (MAP) {
     if (!q.ok) return;
-    const f4 v = {h[0], h[1], h[2], h[3]};
-    *reinterpret_cast<f4*>(a.map_h + ((size_t)seg * a.B + q.b) * rows4 + row4) = v;
+    store_pairs(a.map_h, q, a, (size_t)seg * a.B + q.b, h);
     if (q.w == 0) a.map_s[((size_t)seg * a.B + q.b) * a.D + q.ch] = float2{total, any ? 1.f : 0.f};
   } else if (te == a.T) {
     store_states(a.h_n, q, a, h);
   }
 }
+
+// f(integral_constant fmt, ScanShape).
+template <class Fn>
+int with_fwd_shape(int fmt, int N, Fn f) {
+  return with_fmt(fmt, [&](auto F) {
+    switch (scan_states(N)) {
+      case 4: return f(F, ScanShape<2, 2>{});
+      case 8: return f(F, ScanShape<4, 2>{});
+      case 16: return f(F, ScanShape<8, 2>{});
+      case 32: return f(F, ScanShape<16, 2>{});
+      default: return f(F, ScanShape<16, 4>{});
+    }
+  });
+}
+
+constexpr int kStepStates = 4;  // of a lane of the single step
 
 // A single step: a group of G lanes has a channel, a lane up to four of its states.  h_n may be h0.
 template <int F, int G>
@@ -189,8 +233,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
   const long long ch = i / G;
   const bool ok = ch < (long long)a.B * a.D;  // whole groups
   const int b = ok ? (int)(ch / a.D) : 0, j = ok ? (int)(ch - (long long)b * a.D) : 0;
-  const float x = Elem<F>::up(load_at<F>(a.x, 0, b, j, ok));
-  const float u = Elem<F>::up(load_at<F>(a.delta, 0, b, j, ok)) + (a.bias ? a.bias[j] : 0.f);
+  float x = 0.f, u = 0.f;
+  if (ok) {
+    x = Elem<F>::up(static_cast<const T_*>(a.x.p)[b * a.x.sb + j]);
+    u = Elem<F>::up(static_cast<const T_*>(a.delta.p)[b * a.delta.sb + j]) + (a.bias ? a.bias[j] : 0.f);
+  }
   const float dt = a.softplus ? softplus_f(u, exp_f(-__builtin_fabsf(u))) : u;
   const bool cut = a.reset.p && static_cast<const unsigned char*>(a.reset.p)[b * a.reset.sb];
   float y = 0.f;
@@ -199,8 +246,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     const T_* const cp = static_cast<const T_*>(a.c.p) + b * a.c.sb;
     const size_t row = (size_t)ch * a.N;
 #pragma unroll
-    for (int n4 = 0; n4 < kS; ++n4) {
-      const int n = g * kS + n4;
+    for (int n4 = 0; n4 < kStepStates; ++n4) {
+      const int n = g * kStepStates + n4;
       if (n >= a.N) break;
       float h = a.h0 && !cut ? a.h0[row + n] : 0.f;
       h = __builtin_fmaf(exp2_f(dt * (a.a[(size_t)j * a.N + n] * kLog2e)), h, dt * x * Elem<F>::up(bp[n]));
@@ -230,12 +277,12 @@ extern "C" {
 size_t hsl_selective_ck_floats(int T, int B, int D, int N) {
   if (check_scan("hsl_selective_ck_floats", T, B, D, N, kElemF32) != HSL_OK) return 0;
   const int chunk = scan_chunk(N);
-  return (size_t)((T + chunk - 1) / chunk) * B * D * scan_waves(N) * kS;
+  return (size_t)((T + chunk - 1) / chunk) * B * D * scan_states(N);
 }
 
 size_t hsl_selective_fwd_ws_bytes(int T, int B, int D, int N) {
   if (check_scan("hsl_selective_fwd_ws_bytes", T, B, D, N, kElemF32) != HSL_OK || B == 0 || D == 0 || T == 1) return 0;
-  return (size_t)(plan_scan(T, B, D, N).nseg - 1) * B * D * (scan_waves(N) * kS + 2) * sizeof(float);
+  return (size_t)(plan_scan(T, B, D, N).nseg - 1) * B * D * (scan_states(N) + 2) * sizeof(float);
 }
 
 int hsl_selective_fwd(const void* x, long long x_t, long long x_b, const void* delta, long long de_t, long long de_b,
@@ -276,17 +323,19 @@ int hsl_selective_fwd(const void* x, long long x_t, long long x_b, const void* d
   g.seg_steps = p.seg_steps;
   g.nseg = p.nseg;
   g.map_h = static_cast<float*>(ws);
-  return with_scan(fmt, N, [&](auto F, auto WW) {
-    constexpr int kF = decltype(F)::value, kW = decltype(WW)::value;
+  return with_fwd_shape(fmt, N, [&](auto F, auto shape) {
+    constexpr int kF = decltype(F)::value;
+    using P = decltype(shape);
     if (step) {
-      const long long n = (long long)B * D * kW;
-      hipLaunchKernelGGL((scan_step_kernel<kF, kW>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g);
+      constexpr int kLanes = P::N / kStepStates;  // of a channel
+      const long long n = (long long)B * D * kLanes;
+      hipLaunchKernelGGL((scan_step_kernel<kF, kLanes>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g);
     } else {
       if (p.nseg > 1) {
-        g.map_s = reinterpret_cast<float2*>(g.map_h + (size_t)(p.nseg - 1) * B * D * kW * kS);
-        hipLaunchKernelGGL((scan_fwd_kernel<kF, kW, true>), dim3(p.tiles * B, p.nseg - 1), dim3(kW * 64), 0, s, g);
+        g.map_s = reinterpret_cast<float2*>(g.map_h + (size_t)(p.nseg - 1) * B * D * P::N);
+        hipLaunchKernelGGL((scan_fwd_kernel<kF, P, true>), dim3(p.tiles * B, p.nseg - 1), dim3(P::W * 64), 0, s, g);
       }
-      hipLaunchKernelGGL((scan_fwd_kernel<kF, kW, false>), dim3(p.tiles * B, p.nseg), dim3(kW * 64), 0, s, g);
+      hipLaunchKernelGGL((scan_fwd_kernel<kF, P, false>), dim3(p.tiles * B, p.nseg), dim3(P::W * 64), 0, s, g);
     }
     HSL_HIP(hipGetLastError());
     return (int)HSL_OK;

@@ -4,7 +4,7 @@
 //   dx = dl w,   dw = dl^T x,   dbias = sum_n dl.
 //
 // 16-bit operands: one kernel multiplies 256 x 256 tiles (mm16.h) whose rows are tokens of the
-// vocabulary and whose columns are the positions, so that a lane has 64 logits of one position in
+// vocabulary and whose columns are the positions, so that a lane has 64 logits of each of 2 positions in
 // registers.  The forward reduces them to the tile's largest logit and sum of exponentials, from which a
 // second kernel makes the loss; no logit leaves the registers.  The backward computes the logits again,
 // a piece of the vocabulary at a time, and writes the piece's dl, rounded to 16 bits (as every operand
@@ -19,12 +19,18 @@ namespace hsl {
 namespace {
 
 constexpr float kLog2eX = 1.44269502162933349609375f;
-constexpr size_t kPieceBytes = 128u << 20;  // of a piece's dl: what the last-level cache keeps beside its operands
+constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl (or fp32 logits)
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
 // A row of nothing but masks (m is -inf beside a sum of NaN where every logit is NaN).
 __device__ __forceinline__ bool all_masked(float m, float s) { return m == neg_inf() && s == 0.f; }
+
+// exp(l + ref / log2 e): the product and the difference are rounded once, which moves the result by
+// 2^-24 of l's and the reference's size, as much as their own roundings do.
+__device__ __forceinline__ float exp2_of(float l, float ref) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2eX, ref));
+}
 
 // Joins (m, sum exp(l - m)) of two parts of a row.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -35,16 +41,16 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 
 struct LogitArgs {
   MmOperand w, x;   // from the piece's first token on; from the first position on
-  const float* bias;
+  // Filled up to whole tiles:
+  const float* bias;  // the piece's, zeros where there is none; -inf beyond the vocabulary
   const int* target;  // the positions' targets (of the whole vocabulary)
+  const float4* rows;  // backward: m, 1 / sum, g (scaled), g or 0 where the target is masked; zeros beyond N
   int v_first;        // the piece's first token
   int V, N, D, tiles_v, tiles_n;
-  float2* part;     // [tile_v][N]: forward
-  float* own;       // [N]: the target's logit
-  // backward
-  const float4* rows;  // [N]: m, 1 / sum, g (scaled), -
-  unsigned short* dl;  // [N][tiles_v * 256]
-  float* dbias;        // [tile_n][tiles_v * 256], or null
+  float2* part;     // forward: [tile_v][N]
+  float* own;       // forward: [N], the target's logit
+  unsigned short* dl;  // backward: [N][tiles_v * 256]
+  float* dbias;        // backward: [tile_n][tiles_v * 256], or null
 };
 
 __device__ __forceinline__ void xent_tile_order(int tiles_m, int tiles_n, int id, int* tm, int* tn) {
@@ -59,87 +65,145 @@ __device__ __forceinline__ void xent_tile_order(int tiles_m, int tiles_n, int id
   *tn = in / rows;
 }
 
-// The logits of the lane's 64 tokens and 2 positions, bias added; -inf for tokens beyond the vocabulary.
-__device__ __forceinline__ void finish_logits(const LogitArgs& a, int v0, f16v (&acc)[4][2]) {
-  if (!a.bias && v0 + 128 <= a.V) return;
-  const int half = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int v = v0 + i * 32 + 8 * q + 4 * half;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool in = v + e < a.V;
-        const float add = a.bias && in ? a.bias[v + e] : 0.f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j][4 * q + e] = in ? acc[i][j][4 * q + e] + add : neg_inf();
-      }
-    }
-}
+// What a tile's epilogue needs, copied to LDS with the tile's first slice.
+struct TileInfo {
+  float4 rows[kMmTile];
+  int target[kMmTile];
+  float bias[kMmTile];
+  char rest[2048];  // of the two waves that have nothing to copy
+};
+static_assert(sizeof(TileInfo) == 8 * 1024, "a copy of 1 KB by each wave");
 
-__device__ __forceinline__ MmOperand tile_rows(const MmOperand& o, int first) {
-  return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), o.k};
+// One workgroup's walk over the tiles.
+struct LogitWalk {
+  const LogitArgs& a;
+  int id, tv, tn;
+  __device__ __forceinline__ LogitWalk(const LogitArgs& args) : a(args), id(blockIdx.x) { find(); }
+  __device__ __forceinline__ void find() { xent_tile_order(a.tiles_v, a.tiles_n, id, &tv, &tn); }
+  __device__ __forceinline__ bool there() const { return id < a.tiles_v * a.tiles_n; }
+  __device__ __forceinline__ void next() {
+    id += gridDim.x;
+    if (there()) find();
+  }
+  __device__ __forceinline__ MmOperand rows_of(const MmOperand& o, int tile) const {
+    const int first = tile * kMmTile;
+    return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), there() ? o.k : 0};
+  }
+  __device__ __forceinline__ MmOperand w() const { return rows_of(a.w, there() ? tv : 0); }
+  __device__ __forceinline__ MmOperand x() const { return rows_of(a.x, there() ? tn : 0); }
+  // Wave w copies piece w of the tile's information.
+  __device__ __forceinline__ void info(TileInfo* to, int wave) const {
+    const char* from = reinterpret_cast<const char*>(a.target + tn * kMmTile);
+    bool in = there() && wave < 6;
+    if (wave < 4) {
+      from = reinterpret_cast<const char*>(a.rows + tn * kMmTile) + wave * 1024;
+      in = in && a.rows;
+    } else if (wave == 5) {
+      from = reinterpret_cast<const char*>(a.bias + tv * kMmTile);
+    }
+    mm_copy_kb(from, in, to, wave);
+  }
+};
+
+// A lane's place in a tile: tokens v0 + 32 i + 8 q + e (q, e < 4) and positions n0 + 32 j.
+struct LogitPlace {
+  int lane, wave, half, v, c, v0, n0;
+  __device__ __forceinline__ LogitPlace(int tv, int tn) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    half = lane >> 5;
+    v = (wave >> 2) * 128;
+    c = (wave & 3) * 64 + (lane & 31);
+    v0 = tv * kMmTile + v + 4 * half;
+    n0 = tn * kMmTile + c;
+  }
+};
+
+// Adds the bias, which is there for every call: a branch around it would have the compiler move all sums.
+__device__ __forceinline__ void add_bias(const LogitPlace& q, const float* bias, MmAcc& acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f4 b = *reinterpret_cast<const f4*>(bias + q.v + 4 * q.half + i * 32 + 8 * k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j][4 * k + e] += b[e];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 template <bool FP16>
 __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
-  int tv, tn;
-  xent_tile_order(a.tiles_v, a.tiles_n, blockIdx.x, &tv, &tn);
-  f16v acc[4][2];
-  mm_tile<FP16, false, false>(tile_rows(a.w, tv * kMmTile), tile_rows(a.x, tn * kMmTile),
-                              (a.D + kMmSlice - 1) / kMmSlice, lds, acc);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int v0 = tv * kMmTile + (wave >> 2) * 128, c0 = (wave & 3) * 64 + (lane & 31);
-  finish_logits(a, v0, acc);
-  float2(*const sm)[kMmTile] = reinterpret_cast<float2(*)[kMmTile]>(lds);
+  __shared__ __attribute__((aligned(1024))) TileInfo info[2];
+  __shared__ float2 sm[2][kMmTile];
+  MmPipe<FP16, false, false> mm;
+  LogitWalk walk(a);
+  walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  mm.begin(lds, walk.w(), walk.x(), a.D);
+  for (int par = 0; walk.there(); par ^= 1) {
+    const int tv = walk.tv, tn = walk.tn;
+    walk.next();
+    MmAcc acc;
+    mm.template run<0>(acc, walk.w(), walk.x(), false, [&] { walk.info(&info[par ^ 1], mm.wave); });
+    const LogitPlace q(tv, tn);
+    add_bias(q, info[par].bias, acc);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = tn * kMmTile + c0 + j * 32;
-    const int own = n < a.N ? a.target[n] - a.v_first - v0 - 4 * half : -1;
-    float m = neg_inf();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-    if (__any((unsigned)own < 128u)) {  // few waves have a target among their tokens
-      float l = 0.f;
-      bool found = false;
+    for (int j = 0; j < 2; ++j) {
+      const int n = q.n0 + j * 32, own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
+      float m = neg_inf();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (own == i * 32 + 8 * (r >> 2) + (r & 3)) {
-            l = acc[i][j][r];
-            found = true;
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+      if (__any((unsigned)own < 128u)) {  // few waves have a target among their tokens
+        float l = 0.f;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool here = own == i * 32 + 8 * (r >> 2) + (r & 3);
+            l = here ? acc[i][j][r] : l;
+            found |= here;
           }
-      if (found) a.own[n] = l;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (found && n < a.N) a.own[n] = l;
+      }
+      const float ref = m == neg_inf() ? 0.f : -m * kLog2eX;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += exp2_of(acc[i][j][r], ref);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
+      if (q.half == 0) sm[q.wave >> 2][q.c + j * 32] = float2{m, s};
     }
-    const float ref = m == neg_inf() ? 0.f : m;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - ref) * kLog2eX);
-    join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
-    if (half == 0) sm[wave >> 2][c0 + j * 32] = float2{m, s};
-  }
-  __syncthreads();
-  const int c = threadIdx.x, n = tn * kMmTile + c;
-  if (c < kMmTile && n < a.N) {
-    float2 p = sm[0][c];
-    join(p.x, p.y, sm[1][c].x, sm[1][c].y);
-    a.part[(size_t)tv * a.N + n] = p;
+    lds_barrier();
+    const int n = tn * kMmTile + threadIdx.x;
+    if (threadIdx.x < kMmTile && n < a.N) {
+      float2 p = sm[0][threadIdx.x];
+      join(p.x, p.y, sm[1][threadIdx.x].x, sm[1][threadIdx.x].y);
+      a.part[(size_t)tv * a.N + n] = p;
+    }
   }
 }
 
-// Targets as 32-bit numbers (-1: not scored, -2: beyond the vocabulary).
-__global__ __launch_bounds__(256) void xent_targets_kernel(const void* targets, int tgt64, int* out, int N, int V) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  const long long t = load_id(targets, tgt64, n);
-  out[n] = t < 0 ? -1 : t >= V ? -2 : (int)t;
+// Targets as 32-bit numbers (-1: not scored, -2: beyond the vocabulary), and the bias, up to whole tiles.
+__global__ __launch_bounds__(256) void xent_prepare_kernel(const void* targets, int tgt64, const float* bias,
+                                                          int* target, float* bias_out, int N, int V) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < (N + kMmTile - 1) / kMmTile * kMmTile) {
+    const long long t = i < N ? load_id(targets, tgt64, i) : -1;
+    target[i] = t < 0 ? -1 : t >= V ? -2 : (int)t;
+  }
+  if (i < (V + kMmTile - 1) / kMmTile * kMmTile) bias_out[i] = i >= V ? neg_inf() : bias ? bias[i] : 0.f;
 }
 
 // The loss and the row's (m, sum exp(l - m)) from its tiles' parts: 32 positions by 8 strips of the tiles.
@@ -193,111 +257,128 @@ __global__ __launch_bounds__(1024) void xent_scale_kernel(const float* dloss, fl
 // What the backward needs of each row.  No gradient where the target is outside of the vocabulary or
 // nothing but masks is in the row.
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ stats, const int* __restrict__ target,
-                                                        const float* __restrict__ dloss, const float* scale,
-                                                        float4* rows, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+                                                        const float* __restrict__ dloss, const float* bias,
+                                                        const float* scale, float4* rows, int N) {
+  const int n = blockIdx.x * 256 + threadIdx.x;  // up to whole tiles
+  if (n >= N) {
+    rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+    return;
+  }
   const float2 s = stats[n];
-  const bool on = target[n] >= 0 && !all_masked(s.x, s.y);
-  rows[n] = float4{s.x, 1.f / s.y, on ? dloss[n] * (scale ? scale[0] : 1.f) : 0.f, 0.f};
+  const int t = target[n];
+  const float g = t >= 0 && !all_masked(s.x, s.y) ? dloss[n] * (scale ? scale[0] : 1.f) : 0.f;
+  rows[n] = float4{s.x, 1.f / s.y, g, t >= 0 && bias && bias[t] == neg_inf() ? 0.f : g};
 }
 
-// dl of one logit: nothing for a masked one, whatever arrives.
-__device__ __forceinline__ float dlogit(float l, const float4& row, float gi) {
-  const float d = __builtin_amdgcn_exp2f((l - row.x) * kLog2eX) * gi;
-  return l == neg_inf() ? 0.f : d;
-}
-
-constexpr int kDlRow = kMmTile * 2 + 16;  // bytes of a position's row in LDS
-
+// The tile's dl goes from the registers to memory: an exchange between the half-waves gives every lane 8
+// neighbouring tokens of a position.  The 16 stores of a lane are always issued, whatever lies outside, so
+// that the next product's waits can leave them out.
 template <bool FP16>
 __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kMmTile * kDlRow];
+  constexpr int kStores = 16;
+  __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
+  __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float sums[4][kMmTile];
-  static_assert(sizeof(lds) >= kMmLds, "the slices' place");
-  int tv, tn;
-  xent_tile_order(a.tiles_v, a.tiles_n, blockIdx.x, &tv, &tn);
-  f16v acc[4][2];
-  mm_tile<FP16, false, false>(tile_rows(a.w, tv * kMmTile), tile_rows(a.x, tn * kMmTile),
-                              (a.D + kMmSlice - 1) / kMmSlice, lds, acc);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int vw = (wave >> 2) * 128, v0 = tv * kMmTile + vw, c0 = (wave & 3) * 64 + (lane & 31);
-  finish_logits(a, v0, acc);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int n = tn * kMmTile + c0 + j * 32;
-    const float4 row = n < a.N ? a.rows[n] : float4{0.f, 0.f, 0.f, 0.f};
-    const int own = n < a.N ? a.target[n] - a.v_first - v0 - 4 * half : -1;
-    const float gi = row.z * row.y;
-    const bool on = row.z != 0.f;  // NaN is on
-    const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
-    float hot = row.z;
-    if (owns) {  // a masked target has no gradient either
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (own == i * 32 + 8 * (r >> 2) + (r & 3) && acc[i][j][r] == neg_inf()) hot = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float d = dlogit(acc[i][j][r], row, gi);
-        acc[i][j][r] = on ? d : 0.f;
-      }
-    if (owns) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] -= own == i * 32 + 8 * (r >> 2) + (r & 3) ? hot : 0.f;
-    }
-    char* const p = lds + (c0 + j * 32) * kDlRow + (vw + 4 * half) * 2;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float f[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        unsigned short h[4];
-        down_all<FP16 ? kElemF16 : kElemBf16, 4>(f, h);
-        __builtin_memcpy(__builtin_assume_aligned(p + (i * 32 + 8 * q) * 2, 8), h, 8);
-      }
-  }
-  if (a.dbias) {  // in fp32, from before the rounding
-    float f[2][16];
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const int u = 2 * k, i = u / 16, r = u % 16;
-      f[k / 16][k % 16] = add16(acc[i][0][r] + acc[i][1][r], acc[i][0][r + 1] + acc[i][1][r + 1]);
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float v = sum_rows(f[k], lane);
-      const int u = 2 * (16 * k + (lane & 15)) + ((lane >> 4) & 1), i = u / 16, r = u % 16;
-      sums[wave & 3][vw + i * 32 + 8 * (r >> 2) + 4 * half + (r & 3)] = v;
-    }
-  }
-  __syncthreads();
   const long long ld = (long long)a.tiles_v * kMmTile;
-  for (int p = threadIdx.x; p < kMmTile * 32; p += kMmThreads) {
-    const int c = p >> 5, n = tn * kMmTile + c;
-    if (n >= a.N) break;
-    const mm_u4 v = *reinterpret_cast<const mm_u4*>(lds + c * kDlRow + (p & 31) * 16);
-    *reinterpret_cast<mm_u4*>(a.dl + n * ld + tv * kMmTile + (p & 31) * 8) = v;
-  }
-  if (a.dbias && threadIdx.x < kMmTile) {
-    const int c = threadIdx.x;
-    a.dbias[(size_t)tn * ld + tv * kMmTile + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  MmPipe<FP16, false, false> mm;
+  LogitWalk walk(a);
+  walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  mm.begin(lds, walk.w(), walk.x(), a.D);
+  bool first = true;
+  for (int par = 0; walk.there(); par ^= 1, first = false) {
+    const int tv = walk.tv, tn = walk.tn;
+    walk.next();
+    MmAcc acc;
+    mm.template run<kStores>(acc, walk.w(), walk.x(), !first, [&] { walk.info(&info[par ^ 1], mm.wave); });
+    const LogitPlace q(tv, tn);
+    add_bias(q, info[par].bias, acc);
+    const auto out = __builtin_amdgcn_make_buffer_rsrc(a.dl + (long long)tn * kMmTile * ld + tv * kMmTile, (short)0,
+                                                       0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 row = info[par].rows[q.c + j * 32];
+      const int own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
+      const float gi = row.z * row.y, ref = -row.x * kLog2eX;
+      const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
+      // a masked logit has none whatever arrives, nor has a row without a gradient whatever it holds
+      const bool plain =
+          __all(__builtin_fabsf(gi) < __builtin_inff() && __builtin_fabsf(row.x) < __builtin_inff());
+      // the lower half-wave takes the 8 tokens from 16 k on, the upper one those 8 further
+      const unsigned off =
+          q.n0 + j * 32 < a.N ? (unsigned)((q.c + j * 32) * ld + q.v + 8 * q.half) * 2 : kOffNone;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_barrier(0);  // 16 values at a time in registers beside the rest
+        if (plain) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = exp2_of(acc[i][j][r], ref) * gi;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float d = exp2_of(acc[i][j][r], ref) * gi;
+            acc[i][j][r] = row.z == 0.f || acc[i][j][r] == neg_inf() ? 0.f : d;
+          }
+        }
+        if (owns) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] -= own == i * 32 + 8 * (r >> 2) + (r & 3) ? row.w : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          unsigned lo[2], hi[2];  // 4 tokens of groups 2 k and 2 k + 1
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f[4] = {acc[i][j][8 * k + 2 * e], acc[i][j][8 * k + 2 * e + 1], acc[i][j][8 * k + 4 + 2 * e],
+                                acc[i][j][8 * k + 5 + 2 * e]};
+            unsigned short h[4];
+            down_all<FP16 ? kElemF16 : kElemBf16, 4>(f, h);
+            __builtin_memcpy(&lo[e], h, 4);
+            __builtin_memcpy(&hi[e], h + 2, 4);
+          }
+          mm_u4 v;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const auto x = __builtin_amdgcn_permlane32_swap(lo[e], hi[e], false, false);
+            v[e] = x[0];
+            v[2 + e] = x[1];
+          }
+          __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)off + (i * 32 + 16 * k) * 2, 0, 0);
+        }
+      }
+    }
+    if (a.dbias) {  // in fp32, from before the rounding
+      float f[2][16];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int u = 2 * k, i = u / 16, r = u % 16;
+        f[k / 16][k % 16] = add16(acc[i][0][r] + acc[i][1][r], acc[i][0][r + 1] + acc[i][1][r + 1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float v = sum_rows(f[k], q.lane);
+        const int u = 2 * (16 * k + (q.lane & 15)) + ((q.lane >> 4) & 1), i = u / 16, r = u % 16;
+        sums[q.wave & 3][q.v + i * 32 + 8 * (r >> 2) + 4 * q.half + (r & 3)] = v;
+      }
+      lds_barrier();
+      const int c = threadIdx.x;
+      if (c < kMmTile)
+        a.dbias[(size_t)tn * ld + tv * kMmTile + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    }
   }
 }
 
-// dbias of a piece from its tiles' sums, in fp64.
+// dbias of a piece from its tiles' sums, in fp64: 32 tokens by 8 strips of the tiles.
 __global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict__ part, const float* scale, float* dbias,
                                                         int V, long long ld, int tiles) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
+  __shared__ double sm[8][32];
+  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, v = blockIdx.x * 32 + c;
   double s = 0.0;
-  for (int t = 0; t < tiles; ++t) s += part[t * ld + v];
+  if (v < V)
+    for (int t = strip; t < tiles; t += 8) s += part[t * ld + v];
+  sm[strip][c] = s;
+  __syncthreads();
+  if (strip || v >= V) return;
+  for (int k = 1; k < 8; ++k) s += sm[k][c];
   dbias[v] = (float)(scale ? s * scale[1] : s);
 }
 
@@ -321,18 +402,22 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   const int td = id % a.tiles_d;
   id /= a.tiles_d;
   const int tiles = is_x ? a.tiles_n : a.tiles_v, tm = id % tiles, split = id / tiles;
-  f16v acc[4][2];
+  MmAcc acc;
   const int dcols = a.Dk - td * kMmTile;
   if (is_x) {
     const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
     const MmOperand A{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
     const MmOperand B{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
-    mm_tile<FP16, false, true>(A, B, (k1 - k0 + kMmSlice - 1) / kMmSlice, lds, acc);
+    MmPipe<FP16, false, true> mm;
+    mm.begin(lds, A, B, k1 - k0);
+    mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   } else {
     const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
     const MmOperand A{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
     const MmOperand B{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
-    mm_tile<FP16, true, true>(A, B, (k1 - k0 + kMmSlice - 1) / kMmSlice, lds, acc);
+    MmPipe<FP16, true, true> mm;
+    mm.begin(lds, A, B, k1 - k0);
+    mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int r0 = tm * kMmTile + (wave >> 2) * 128 + 4 * half, c0 = td * kMmTile + (wave & 3) * 64 + (lane & 31);
@@ -442,17 +527,28 @@ __global__ __launch_bounds__(256) void xent_f32_grad_kernel(float* __restrict__ 
   }
 }
 
-// Sums of columns of [N][ld]: 64 columns a workgroup, 4 strips of the rows, in fp64.
-__global__ __launch_bounds__(256) void xent_f32_bias_kernel(const float* __restrict__ l, long long ld, float* dbias,
-                                                            int V, int N) {
-  __shared__ double sm[4][64];
-  const int c = threadIdx.x & 63, strip = threadIdx.x >> 6, v = blockIdx.x * 64 + c;
+// Sums of columns of [N][ld], in fp64: 32 columns a workgroup, 32 strips of the rows.
+__global__ __launch_bounds__(1024) void xent_f32_bias_kernel(const float* __restrict__ l, long long ld, float* dbias,
+                                                             int V, int N) {
+  __shared__ double sm[32][32];
+  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, v = blockIdx.x * 32 + c;
   double s = 0.0;
-  if (v < V)
-    for (int n = strip; n < N; n += 4) s += l[n * ld + v];
+  if (v < V) {
+    int n = strip;
+    for (; n + 96 < N; n += 128) {
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = l[(n + 32 * k) * ld + v];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += x[k];
+    }
+    for (; n < N; n += 32) s += l[n * ld + v];
+  }
   sm[strip][c] = s;
   __syncthreads();
-  if (strip == 0 && v < V) dbias[v] = (float)((sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]));
+  if (strip || v >= V) return;
+  for (int k = 1; k < 32; ++k) s += sm[k][c];
+  dbias[v] = (float)s;
 }
 
 __global__ __launch_bounds__(256) void xent_f32_add_kernel(float* __restrict__ out, const float* __restrict__ v,
@@ -526,7 +622,7 @@ struct XentSpace {
   float* scale;
   unsigned short *packed_x, *packed_w;
   char* dl;  // 16-bit dl, or fp32 logits
-  float *bias, *dx, *dw;
+  float *bias, *dbias, *dx, *dw;
   void* gemm;
   size_t gemm_bytes, bytes;
 };
@@ -536,12 +632,13 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   XentSpace s{};
   const XentPlan p = plan_xent(N, V, D, fmt);
   Carver c(base, 0);
-  s.target = c.take<int>(N);
+  s.target = c.take<int>(up_to(N, kMmTile));
+  s.bias = c.take<float>(up_to(V, kMmTile));
   if (!backward) {
     s.own = c.take<float>(N);
     s.part = c.take<float2>(fmt == kElemF32 ? (size_t)N : (size_t)N * ((V + kMmTile - 1) / kMmTile));
   } else {
-    s.rows = c.take<float4>(N);
+    s.rows = c.take<float4>(up_to(N, kMmTile));
     s.scale = c.take<float>(2);
   }
   if (fmt == kElemF32) {
@@ -554,7 +651,7 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
     if (backward) {
       s.dl = c.take<char>((size_t)N * p.piece * 2);
-      s.bias = c.take<float>((size_t)p.tiles_n * p.piece);
+      s.dbias = c.take<float>((size_t)p.tiles_n * p.piece);
       s.dx = c.take<float>((size_t)p.splits_x * N * D);
       if (p.splits_w > 1) s.dw = c.take<float>((size_t)p.splits_w * p.piece * D);
     }
@@ -626,7 +723,10 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   hipStream_t st = static_cast<hipStream_t>(stream);
   unsigned* err = nullptr;
   HSL_CHECK(device_error_word(&err));
-  hipLaunchKernelGGL(xent_targets_kernel, dim3((n + 255) / 256), dim3(256), 0, st, targets, tgt64, s.target, n, V);
+  DeviceInfo info;
+  HSL_CHECK(device_info(&info));
+  hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
+                     tgt64, bias, s.target, s.bias, n, V);
   int tiles = 1;
   if (fmt == kElemF32) {
     const XentPlan p = plan_xent(n, V, D, fmt);
@@ -645,7 +745,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     LogitArgs a{};
     a.w = {o.w, o.ldw, V, o.width};
     a.x = {o.x, o.ldx, n, o.width};
-    a.bias = bias;
+    a.bias = s.bias;
     a.target = s.target;
     a.V = V;
     a.N = n;
@@ -654,7 +754,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.tiles_n = (n + kMmTile - 1) / kMmTile;
     a.part = s.part;
     a.own = s.own;
-    const dim3 grid(a.tiles_v * a.tiles_n), block(kMmThreads);
+    const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
     if (fmt == kElemF16)
       hipLaunchKernelGGL(xent_stats_kernel<true>, grid, block, 0, st, a);
     else
@@ -698,9 +798,10 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, dloss, s.scale, n);
     scale = s.scale;
   }
-  hipLaunchKernelGGL(xent_targets_kernel, dim3((n + 255) / 256), dim3(256), 0, st, targets, tgt64, s.target, n, V);
+  hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
+                     tgt64, bias, s.target, s.bias, n, V);
   hipLaunchKernelGGL(xent_rows_kernel, dim3((n + 255) / 256), dim3(256), 0, st,
-                     reinterpret_cast<const float2*>(stats), s.target, dloss, scale, s.rows, n);
+                     reinterpret_cast<const float2*>(stats), s.target, dloss, bias, scale, s.rows, n);
   HSL_HIP(hipGetLastError());
   if (fmt == kElemF32) {
     float* const l = reinterpret_cast<float*>(s.dl);
@@ -713,7 +814,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
       hipLaunchKernelGGL(xent_f32_grad_kernel, dim3(n), dim3(256), 0, st, l, (long long)p.piece, v, v0, s.target,
                          s.rows);
       if (dbias)
-        hipLaunchKernelGGL(xent_f32_bias_kernel, dim3((v + 63) / 64), dim3(256), 0, st, l, (long long)p.piece,
+        hipLaunchKernelGGL(xent_f32_bias_kernel, dim3((v + 31) / 32), dim3(1024), 0, st, l, (long long)p.piece,
                            dbias + v0, v, n);
       if (dx) {
         float* const out = v0 ? s.dx : static_cast<float*>(dx);
@@ -731,6 +832,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     }
     return HSL_OK;
   }
+  DeviceInfo info;
+  HSL_CHECK(device_info(&info));
   XentOperands o;
   HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
   for (int v0 = 0; v0 < V; v0 += p.piece) {
@@ -739,7 +842,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     LogitArgs a{};
     a.w = {o.w + v0 * o.ldw, o.ldw, v, o.width};
     a.x = {o.x, o.ldx, n, o.width};
-    a.bias = bias ? bias + v0 : nullptr;
+    a.bias = s.bias + v0;
     a.target = s.target;
     a.v_first = v0;
     a.V = v;
@@ -749,7 +852,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.tiles_n = p.tiles_n;
     a.rows = s.rows;
     a.dl = reinterpret_cast<unsigned short*>(s.dl);
-    a.dbias = dbias ? s.bias : nullptr;
+    a.dbias = dbias ? s.dbias : nullptr;
     OutArgs g{};
     g.dl = a.dl;
     g.w = a.w.p;
@@ -773,7 +876,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.k_x = p.k_x;
     g.k_w = p.k_w;
     g.add = v0 > 0;
-    const dim3 grid(tiles_v * p.tiles_n), block(kMmThreads);
+    const dim3 grid(std::min(tiles_v * p.tiles_n, info.num_cus)), block(kMmThreads);
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
     if (fmt == kElemF16) {
       hipLaunchKernelGGL(xent_grad_kernel<true>, grid, block, 0, st, a);
@@ -783,7 +886,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
       if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<false>, grid_out, block, 0, st, g);
     }
     if (dbias)
-      hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 255) / 256), dim3(256), 0, st, s.bias, scale, dbias + v0, v, g.ld,
+      hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, scale, dbias + v0, v, g.ld,
                          p.tiles_n);
     if (dw && g.dw)
       hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>,
