@@ -46,11 +46,11 @@ struct ScanArgs {
   OutStream y, dx, ddelta, dz;
   const float *a, *d, *bias, *h0, *dh_n;
   float *h_n, *ck, *dh0;
-  // Kept states lie in pairs, [..][B][pair][D][2].
+  // Kept states lie as [..][B][state][D].
   float* map_h;     // of [segment]: the state behind the segment if it began with zeros
   float2* map_s;    // [segment][B][D]: its sum of dt, and whether it has a reset
   float* part_bc;   // [tile][T][B][2][states]: the tile's sums for db and dc
-  float* part_a;    // [B segments][pair][D][2]
+  float* part_a;    // [B segments][state][D]
   float* part_d;    // [B segments][2][D]
   int T, B, D, N, softplus, seg_steps, nseg;
 };
@@ -105,28 +105,22 @@ __device__ __forceinline__ void store_states(float* p, const ScanPlace<P>& q, co
   for (int n = 0; n < P::S; ++n)
     if (q.ok && q.n0 + n < a.N) r[n] = v[n];
 }
-// The wave's states in row `row` (of B each) of states kept in pairs.
+// The wave's states in row `row` (of B each) of kept states.
 template <class P>
-__device__ __forceinline__ size_t pair_at(const ScanPlace<P>& q, const ScanArgs& a, size_t row) {
-  return ((row * (P::N / 2) + q.n0 / 2) * a.D + q.ch) * 2;
+__device__ __forceinline__ size_t kept_at(const ScanPlace<P>& q, const ScanArgs& a, size_t row) {
+  return (row * P::N + q.n0) * a.D + q.ch;
 }
 template <class P>
-__device__ __forceinline__ void load_pairs(const float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
-                                           float (&v)[P::S]) {
+__device__ __forceinline__ void load_kept(const float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
+                                          float (&v)[P::S]) {
 #pragma unroll
-  for (int n = 0; n < P::S; n += 2) {
-    const float2 u = *reinterpret_cast<const float2*>(p + pair_at(q, a, row) + (size_t)n * a.D);
-    v[n] = u.x;
-    v[n + 1] = u.y;
-  }
+  for (int n = 0; n < P::S; ++n) v[n] = p[kept_at(q, a, row) + (size_t)n * a.D];
 }
 template <class P>
-__device__ __forceinline__ void store_pairs(float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
-                                            const float (&v)[P::S]) {
-  typedef float F2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void store_kept(float* p, const ScanPlace<P>& q, const ScanArgs& a, size_t row,
+                                           const float (&v)[P::S]) {
 #pragma unroll
-  for (int n = 0; n < P::S; n += 2)
-    __builtin_nontemporal_store((F2){v[n], v[n + 1]}, reinterpret_cast<F2*>(p + pair_at(q, a, row) + (size_t)n * a.D));
+  for (int n = 0; n < P::S; ++n) __builtin_nontemporal_store(v[n], p + kept_at(q, a, row) + (size_t)n * a.D);
 }
 template <class P>
 __device__ __forceinline__ void load_a2(const ScanPlace<P>& q, const ScanArgs& a, float (&a2)[P::S]) {
@@ -194,8 +188,9 @@ struct BcTile {
     for (int i = 0; i < kEach; ++i) {
       const int k = threadIdx.x + i * P::W * 64, s = k / P::N, n = k % P::N;
       const bool in = k < P::L * P::N && t0 + s < te && n < a.N;
-      const T_* const bp = static_cast<const T_*>(a.b.p) + (t0 * a.b.st + b * a.b.sb);
-      const T_* const cp = static_cast<const T_*>(a.c.p) + (t0 * a.c.st + b * a.c.sb);
+      const int from = min(t0, te - 1);
+      const T_* const bp = static_cast<const T_*>(a.b.p) + (from * a.b.st + b * a.b.sb);
+      const T_* const cp = static_cast<const T_*>(a.c.p) + (from * a.c.st + b * a.c.sb);
       const int row = in ? s : 0, m = in ? n : 0;
       rb[i] = bp[row * a.b.st + m];
       rc[i] = cp[row * a.c.st + m];
@@ -216,10 +211,14 @@ struct BcTile {
 // A wave's S values of b or c.
 template <int S>
 __device__ __forceinline__ void load_row(const float* p, float (&v)[S]) {
-  typedef float V __attribute__((ext_vector_type(S)));
-  const V u = *reinterpret_cast<const V*>(p);
+  if constexpr (S == 1) {
+    v[0] = *p;
+  } else {
+    typedef float V __attribute__((ext_vector_type(S)));
+    const V u = *reinterpret_cast<const V*>(p);
 #pragma unroll
-  for (int n = 0; n < S; ++n) v[n] = u[n];
+    for (int n = 0; n < S; ++n) v[n] = u[n];
+  }
 }
 
 // sigmoid(z).  A 16-bit z has an error of 2^-9 (bf16) or 2^-12 of itself, against which that of rounding

@@ -57,7 +57,7 @@ struct BwdRows {
     }
     m.bc.load(a, q.b, t0, te);
     m.cut = load_cut<P::L>(a.reset, t0, te, q.b, q.lane);
-    if (!MAP) load_pairs(a.ck, q, a, (size_t)(t0 / P::L) * a.B + q.b, m.h);
+    if (!MAP) load_kept(a.ck, q, a, (size_t)(t0 / P::L) * a.B + q.b, m.h);
     x.move(-1);
     delta.move(-1);
     z.move(-1);
@@ -73,7 +73,7 @@ __device__ __forceinline__ void enter_reverse(const ScanArgs& a, const ScanPlace
   for (int i = a.nseg - 1; i > seg; --i) {
     const float2 m = a.map_s[((size_t)(i - 1) * a.B + q.b) * a.D + q.ch];
     float v[P::S];
-    load_pairs(a.map_h, q, a, (size_t)(i - 1) * a.B + q.b, v);
+    load_kept(a.map_h, q, a, (size_t)(i - 1) * a.B + q.b, v);
 #pragma unroll
     for (int n = 0; n < P::S; ++n) {
       const float u = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), U[n], v[n]);
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_map_kernel(ScanArgs a) {
     lds_barrier();
   }
   if (!q.ok) return;
-  store_pairs(a.map_h, q, a, (size_t)blockIdx.y * a.B + q.b, U);
+  store_kept(a.map_h, q, a, (size_t)blockIdx.y * a.B + q.b, U);
   if (q.w == 0) a.map_s[((size_t)blockIdx.y * a.B + q.b) * a.D + q.ch] = float2{total.sum, any ? 1.f : 0.f};
 }
 
@@ -186,107 +186,138 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
     }
     m.bc.store(sb, sc);
   };
+  // A chunk's steps forwards with their decays and states kept, then backwards: in two halves where four
+  // states a wave would not leave the registers for all of it (the first half then runs three times).
   // SLOW: a reset in the chunk, or lanes without a channel
+  constexpr int kHalves = S == 4 ? 2 : 1, H = L / kHalves, G = S == 4 ? 1 : 4;  // G: steps whose operands are read from LDS ahead
   auto run = [&](auto slow, int t0) {
     constexpr bool SLOW = decltype(slow)::value;
-    constexpr int G = 4;  // steps whose operands are read from LDS ahead
-    float f[L][S], hs[L][S], h[S];
-#pragma unroll
-    for (int n = 0; n < S; ++n) h[n] = hin[n];
-    {
+    float f[H][S], hs[H][S], start[S], cda[S] = {};
+    // the states behind steps s0 .. s0 + H - 1, from `start`
+    auto forwards = [&](int s0, auto keep) {
+      constexpr bool KEEP = decltype(keep)::value;
       struct Ahead {
         float2 dt[G];
         float b[G][S];
       } r[2];
-      auto read = [&](int s0, Ahead& v) {
+      auto read = [&](int s1, Ahead& v) {
 #pragma unroll
         for (int s = 0; s < G; ++s) {
-          v.dt[s] = sdt[s0 + s][q.lane];
-          load_row<S>(&sb[s0 + s][q.n0], v.b[s]);
+          v.dt[s] = sdt[s1 + s][q.lane];
+          load_row<S>(&sb[s1 + s][q.n0], v.b[s]);
         }
       };
-      read(0, r[0]);
+      float h[S];
 #pragma unroll
-      for (int s0 = 0; s0 < L; s0 += G) {
-        if (s0 + G < L) read(s0 + G, r[(s0 / G + 1) & 1]);
+      for (int n = 0; n < S; ++n) h[n] = start[n];
+      read(s0, r[0]);
+#pragma unroll
+      for (int g = 0; g < H; g += G) {
+        if (g + G < H) read(s0 + g + G, r[(g / G + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
-        const Ahead& v = r[(s0 / G) & 1];
+        const Ahead& v = r[(g / G) & 1];
 #pragma unroll
         for (int k = 0; k < G; ++k)
 #pragma unroll
           for (int n = 0; n < S; ++n) {
-            const int s = s0 + k;
-            f[s][n] = exp2_f(v.dt[k].x * a2[n]);
-            const float e = v.dt[k].y * v.b[k][n], g = __builtin_fmaf(f[s][n], h[n], e);
-            h[n] = SLOW && (cuts >> s & 1) ? e : g;
-            hs[s][n] = h[n];
+            const float decay = exp2_f(v.dt[k].x * a2[n]), e = v.dt[k].y * v.b[k][n];
+            const float w = __builtin_fmaf(decay, h[n], e);
+            h[n] = SLOW && (cuts >> (s0 + g + k) & 1) ? e : w;
+            if (KEEP) {
+              f[g + k][n] = decay;
+              hs[g + k][n] = h[n];
+            }
           }
       }
-    }
-    constexpr int kRegs = L * S / 2;  // of sums over rows, four values each
-    float sums[kRegs / 16][16], cda[S] = {};
-    struct Ahead {
-      float2 dt[G];
-      float dy[G], b[G][S], c[G][S];
-    } r[2];
-    auto read = [&](int s0, Ahead& v) {
+      if (!KEEP) {
 #pragma unroll
-      for (int s = 0; s < G; ++s) {
-        v.dt[s] = sdt[s0 + s][q.lane];
-        v.dy[s] = sdy[s0 + s][q.lane];
-        load_row<S>(&sb[s0 + s][q.n0], v.b[s]);
-        load_row<S>(&sc[s0 + s][q.n0], v.c[s]);
+        for (int n = 0; n < S; ++n) start[n] = h[n];
       }
     };
-    read(L - G, r[(L / G - 1) & 1]);
+    constexpr int kRegs = H * S / 2;  // of sums over rows, four values each
+    static_assert(L * S / 2 % 16 == 0, "sum_rows takes 16");
+    float sums[kHalves * kRegs > 16 ? kRegs : kHalves * kRegs];
+    constexpr bool kEach = kHalves * kRegs > 16;  // the half's sums are finished with it
+    auto finish_sums = [&](int s0, int count) {
+      const int row = q.lane >> 4;
+      float* const out = a.part_bc + (((size_t)q.tile * a.T + t0) * a.B + q.b) * (2 * P::N) + (row & 1) * P::N +
+                         q.n0 + (row >> 1);
 #pragma unroll
-    for (int s = L - 1; s >= 0; --s) {
-      if (s % G == G - 1) {
-        if (s >= G) read(s / G * G - G, r[(s / G - 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
-      }
-      const Ahead& v = r[(s / G) & 1];
-      const float2 dt = v.dt[s % G];
-      const float dy = v.dy[s % G];
-      const float(&b)[S] = v.b[s % G];
-      const float(&c)[S] = v.c[s % G];
-      const bool cut = SLOW && (cuts >> s & 1);
-      float gb = 0.f, ap = 0.f, y = 0.f, vb[S], vc[S];
+      for (int k = 0; k < count / 16; ++k) {
+        float r16[16];
 #pragma unroll
-      for (int n = 0; n < S; ++n) {
-        const float G = __builtin_fmaf(c[n], dy, U[n]);
-        y = __builtin_fmaf(c[n], hs[s][n], y);
-        gb = __builtin_fmaf(G, b[n], gb);
-        vb[n] = G * dt.y;
-        vc[n] = dy * hs[s][n];
-        U[n] = G * f[s][n];
-        float p = U[n] * (s ? hs[s ? s - 1 : 0][n] : hin[n]);
-        if (cut) U[n] = p = 0.f;
-        ap = __builtin_fmaf(an[n], p, ap);
-        cda[n] = __builtin_fmaf(dt.x, p, cda[n]);
-        if (SLOW && !q.ok) vb[n] = vc[n] = 0.f;
+        for (int i = 0; i < 16; ++i) r16[i] = sums[16 * k + i];
+        const float v = sum_rows(r16, q.lane);
+        const int r = 16 * k + (q.lane & 15), s = s0 + r / (S / 2), n = r % (S / 2) * 2;
+        if (t0 + s < te) out[(size_t)s * a.B * (2 * P::N) + n] = v;
       }
-      sp[0][q.w][s][q.lane] = gb;
-      sp[1][q.w][s][q.lane] = ap;
-      sp[2][q.w][s][q.lane] = y;
-      // rows 0..3: b of state n, c of state n, b of state n + 1, c of state n + 1
+    };
 #pragma unroll
-      for (int n = 0; n < S; n += 2) {
-        const int r = s * (S / 2) + n / 2;
-        sums[r / 16][r % 16] = add16(add32(vb[n], vb[n + 1]), add32(vc[n], vc[n + 1]));
+    for (int half = kHalves - 1; half >= 0; --half) {
+      const int s0 = half * H;
+#pragma unroll
+      for (int n = 0; n < S; ++n) start[n] = hin[n];
+      if (half) {
+        forwards(0, std::false_type{});
+        asm volatile("" ::: "memory");  // what it read is read again rather than kept for the other half
       }
+      forwards(s0, std::true_type{});
+      struct Ahead {
+        float2 dt[G];
+        float dy[G], b[G][S], c[G][S];
+      } r[2];
+      auto read = [&](int s1, Ahead& v) {
+#pragma unroll
+        for (int s = 0; s < G; ++s) {
+          v.dt[s] = sdt[s1 + s][q.lane];
+          v.dy[s] = sdy[s1 + s][q.lane];
+          load_row<S>(&sb[s1 + s][q.n0], v.b[s]);
+          load_row<S>(&sc[s1 + s][q.n0], v.c[s]);
+        }
+      };
+      read(s0 + H - G, r[(H / G - 1) & 1]);
+#pragma unroll
+      for (int k = H - 1; k >= 0; --k) {
+        const int s = s0 + k;
+        if (k % G == G - 1) {
+          if (k >= G) read(s0 + k / G * G - G, r[(k / G - 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
+        }
+        const Ahead& v = r[(k / G) & 1];
+        const float2 dt = v.dt[k % G];
+        const float dy = v.dy[k % G];
+        const float(&b)[S] = v.b[k % G];
+        const float(&c)[S] = v.c[k % G];
+        const bool cut = SLOW && (cuts >> s & 1);
+        float gb = 0.f, ap = 0.f, y = 0.f, vb[S], vc[S];
+#pragma unroll
+        for (int n = 0; n < S; ++n) {
+          const float g = __builtin_fmaf(c[n], dy, U[n]);
+          y = __builtin_fmaf(c[n], hs[k][n], y);
+          gb = __builtin_fmaf(g, b[n], gb);
+          vb[n] = g * dt.y;
+          vc[n] = dy * hs[k][n];
+          U[n] = g * f[k][n];
+          float p = U[n] * (k ? hs[k ? k - 1 : 0][n] : start[n]);
+          if (cut) U[n] = p = 0.f;
+          ap = __builtin_fmaf(an[n], p, ap);
+          cda[n] = __builtin_fmaf(dt.x, p, cda[n]);
+          if (SLOW && !q.ok) vb[n] = vc[n] = 0.f;
+        }
+        sp[0][q.w][s][q.lane] = gb;
+        sp[1][q.w][s][q.lane] = ap;
+        sp[2][q.w][s][q.lane] = y;
+        // rows 0..3: b of state n, c of state n, b of state n + 1, c of state n + 1
+#pragma unroll
+        for (int n = 0; n < S; n += 2)
+          sums[(kEach ? k : s) * (S / 2) + n / 2] = add16(add32(vb[n], vb[n + 1]), add32(vc[n], vc[n + 1]));
+      }
+      if (kEach) finish_sums(s0, kRegs);
+      asm volatile("" ::: "memory");
     }
+    if (!kEach) finish_sums(0, kHalves * kRegs);
 #pragma unroll
     for (int n = 0; n < S; ++n) da[n].add(cda[n]);
-    const int row = q.lane >> 4;
-    float* const out = a.part_bc + (((size_t)q.tile * a.T + t0) * a.B + q.b) * (2 * P::N) + (row & 1) * P::N + q.n0 +
-                       (row >> 1);
-#pragma unroll
-    for (int k = 0; k < kRegs / 16; ++k) {
-      const float v = sum_rows(sums[k], q.lane);
-      const int r = 16 * k + (q.lane & 15), s = r / (S / 2), n = r % (S / 2) * 2;
-      if (t0 + s < te) out[(size_t)s * a.B * (2 * P::N) + n] = v;
-    }
   };
 
   const int first = te > tb ? tb + (te - tb - 1) / L * L : tb - L;
@@ -340,7 +371,7 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
     float v[S];
 #pragma unroll
     for (int n = 0; n < S; ++n) v[n] = da[n].sum;
-    store_pairs(a.part_a, q, a, part, v);
+    store_kept(a.part_a, q, a, part, v);
   }
   sp[0][q.w][0][q.lane] = dskip.sum;
   sp[1][q.w][0][q.lane] = dbias.sum;
@@ -390,9 +421,8 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__
   if (strip || i >= all) return;
   const float s = (float)((sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]));
   if (i < na) {
-    const long long pd = i / 2;
-    const int n = (int)(pd / D) * 2 + (int)(i % 2);
-    if (n < N) da[pd % D * N + n] = s;
+    const int n = (int)(i / D);
+    if (n < N) da[i % D * N + n] = s;
   } else {
     const long long j = i - na;
     float* const o = j < D ? dd : dbias;
@@ -400,7 +430,8 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__
   }
 }
 
-// f(integral_constant fmt, ScanShape).
+// f(integral_constant fmt, ScanShape): two states a wave up to 16 (four a wave, in half the waves and two workgroups a CU, took 3152 us for 2547,
+// T4096 B32 D1024 N16 bf16: its registers leave one wave a SIMD).
 template <class Fn>
 int with_bwd_shape(int fmt, int N, Fn f) {
   return with_fmt(fmt, [&](auto F) {

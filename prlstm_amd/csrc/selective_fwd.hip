@@ -48,9 +48,9 @@ struct FwdChunk {
   unsigned char cut;
 };
 
-// MAP: only each segment's map (nothing of the last segment, whose map nothing reads).  What B and C
-// read is kept twice, so that one barrier a chunk is enough: a wave is in C of chunk k or B of chunk
-// k + 1 while another still is in C of chunk k, and A of chunk k + 2 comes behind the next barrier.
+// MAP: only each segment's map (nothing of the last segment, whose map nothing reads).  Between two barriers a
+// wave has C of the chunk before, B of this one and A of the next, which do not depend on each other, so the
+// latency of each one's chains lies behind the others' work; what they exchange is kept twice.
 template <int F, class P, bool MAP>
 __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
   constexpr int L = P::L, PS = P::PS, S = P::S, W = P::W;
@@ -72,17 +72,17 @@ __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
     for (int i = 0; i < seg; ++i) {
       const float2 m = a.map_s[((size_t)i * a.B + q.b) * a.D + q.ch];
       float v[S];
-      load_pairs(a.map_h, q, a, (size_t)i * a.B + q.b, v);
+      load_kept(a.map_h, q, a, (size_t)i * a.B + q.b, v);
 #pragma unroll
       for (int n = 0; n < S; ++n)
         h[n] = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), h[n], v[n]);
     }
   }
   float total = 0.f, low = 0.f;  // the sum of dt and what its roundings lost
-  unsigned any = 0, cuts = 0;
+  unsigned any = 0;
 
-  FwdChunk<F, P> next;  // the loads of the next chunk
-  Rows<F, P> xr(a.x, q, tb), dr(a.delta, q, tb), zr(a.z, q, tb), yr(a.y, q, tb);
+  FwdChunk<F, P> next;  // the loads of the chunk after the next
+  Rows<F, P> xr(a.x, q, tb), dr(a.delta, q, tb), zr(a.z, q, tb), yr(a.y, q, tb - L);
   auto load = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
@@ -98,7 +98,9 @@ __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
     dr.move(1);
     zr.move(1);
   };
-  float x_now[PS], z_now[PS], x_next[PS], z_next[PS];  // what A leaves for C
+  struct Kept {
+    float x[PS], z[PS];
+  } before, now, then;  // what A leaves for C
   auto stage = [&](int t0, int par) {  // A
 #pragma unroll
     for (int i = 0; i < PS; ++i) {
@@ -109,114 +111,106 @@ __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
       dt = soft ? dt : u;
       dt = t0 + s < te && q.ok ? dt : 0.f;
       sdt[par][s][q.lane] = float2{dt, dt * x};
-      x_next[i] = x;
-      if (!MAP) z_next[i] = Elem<F>::up(next.z[i]);
+      then.x[i] = x;
+      then.z[i] = MAP ? 0.f : Elem<F>::up(next.z[i]);
     }
     next.bc.store(sb[par], sc[par]);
   };
-  auto run = [&](auto cut, int par) {  // B
+  auto run = [&](auto cut, int par, unsigned cuts) {  // B
     constexpr bool CUT = decltype(cut)::value;
-    constexpr int G = 4;  // steps whose operands are read from LDS ahead
-    struct Ahead {
-      float2 dt[G];
-      float b[G][S], c[G][S];
-    } r[2];
-    auto read = [&](int s0, Ahead& v) {
-#pragma unroll
-      for (int s = 0; s < G; ++s) {
-        v.dt[s] = sdt[par][s0 + s][q.lane];
-        load_row<S>(&sb[par][s0 + s][q.n0], v.b[s]);
-        if (!MAP) load_row<S>(&sc[par][s0 + s][q.n0], v.c[s]);
-      }
-    };
     float part = 0.f;
-    read(0, r[0]);
 #pragma unroll
-    for (int s0 = 0; s0 < L; s0 += G) {
-      if (s0 + G < L) read(s0 + G, r[(s0 / G + 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead
-      const Ahead& v = r[(s0 / G) & 1];
+    for (int s = 0; s < L; ++s) {
+      const float2 dt = sdt[par][s][q.lane];
+      float b[S], c[S], y = 0.f;
+      load_row<S>(&sb[par][s][q.n0], b);
+      if (!MAP) load_row<S>(&sc[par][s][q.n0], c);
+      const bool zero = CUT && (cuts >> s & 1);
 #pragma unroll
-      for (int k = 0; k < G; ++k) {
-        const int s = s0 + k;
-        const bool zero = CUT && (cuts >> s & 1);
-        float y = 0.f;
-#pragma unroll
-        for (int n = 0; n < S; ++n) {
-          const float f = exp2_f(v.dt[k].x * a2[n]), e = v.dt[k].y * v.b[k][n];
-          const float g = __builtin_fmaf(f, h[n], e);
-          h[n] = zero ? e : g;
-          if (!MAP) y = n ? __builtin_fmaf(v.c[k][n], h[n], y) : v.c[k][n] * h[n];
-        }
-        if (MAP) part += v.dt[k].x;
-        if (!MAP) sy[par][q.w][s][q.lane] = y;
+      for (int n = 0; n < S; ++n) {
+        const float f = exp2_f(dt.x * a2[n]), e = dt.y * b[n];
+        const float g = __builtin_fmaf(f, h[n], e);
+        h[n] = zero ? e : g;
+        if (!MAP) y = n ? __builtin_fmaf(c[n], h[n], y) : c[n] * h[n];
       }
+      if (MAP) part += dt.x;
+      if (!MAP) sy[par][q.w][s][q.lane] = y;
     }
     if (MAP) {  // compensated: thousands of small dt
       const float v = part - low, t = total + v;
       low = (t - total) - v;
       total = t;
-      any |= cuts;
     }
   };
+  auto finish = [&](int t0, int par) {  // C
+#pragma unroll
+    for (int i = 0; i < PS; ++i) {
+      const int s = q.w + W * i, t = t0 + s;
+      if (L < W && s >= L) break;
+      float y = skip * before.x[i];
+#pragma unroll
+      for (int v = 0; v < W; ++v) y += sy[par][v][s][q.lane];
+      y *= gate_of<F>(before.z[i], gated);
+      yr.store(i, off, t >= tb && t < te, y);
+    }
+    yr.move(1);
+  };
 
+  unsigned cuts = 0;
+  now = Kept{};
+  then = Kept{};
   if (tb < te) {
     load(tb);
     stage(tb, 0);
     cuts = cuts_of(a.reset, next.cut);
-    if (tb + L < te) load(tb + L);
+    load(tb + L);
   }
   lds_barrier();
   int par = 0;
   for (int t0 = tb; t0 < te; t0 += L, par ^= 1) {
-#pragma unroll
-    for (int i = 0; i < PS; ++i) {
-      x_now[i] = x_next[i];
-      if (!MAP) z_now[i] = z_next[i];
-    }
-    if (!MAP && a.ck && q.ok) store_pairs(a.ck, q, a, (size_t)(t0 / L) * a.B + q.b, h);
-    if (cuts)
-      run(std::true_type{}, par);
-    else
-      run(std::false_type{}, par);
-    if (t0 + L < te) {
+    before = now;
+    now = then;
+    if (!MAP && a.ck && q.ok) store_kept(a.ck, q, a, (size_t)(t0 / L) * a.B + q.b, h);
+    any |= cuts;
+    auto all = [&](auto cut) {
+      run(cut, par, cuts);
+      if (!MAP) finish(t0 - L, par ^ 1);
       stage(t0 + L, par ^ 1);
-      cuts = cuts_of(a.reset, next.cut);
-      if (t0 + 2 * L < te) load(t0 + 2 * L);
-    }
+    };
+    if (cuts)
+      all(std::true_type{});
+    else
+      all(std::false_type{});
+    cuts = cuts_of(a.reset, next.cut);
+    load(t0 + 2 * L);
     lds_barrier();
-    if (!MAP) {  // C
-#pragma unroll
-      for (int i = 0; i < PS; ++i) {
-        const int s = q.w + W * i, t = t0 + s;
-        if (L < W && s >= L) break;
-        float y = skip * x_now[i];
-#pragma unroll
-        for (int v = 0; v < W; ++v) y += sy[par][v][s][q.lane];
-        y *= gate_of<F>(z_now[i], gated);
-        yr.store(i, off, t < te, y);
-      }
-      yr.move(1);
-    }
+  }
+  if (!MAP && tb < te) {
+    before = now;
+    finish(tb + (te - tb - 1) / L * L, par ^ 1);
   }
   if (MAP) {
     if (!q.ok) return;
-    store_pairs(a.map_h, q, a, (size_t)seg * a.B + q.b, h);
+    store_kept(a.map_h, q, a, (size_t)seg * a.B + q.b, h);
     if (q.w == 0) a.map_s[((size_t)seg * a.B + q.b) * a.D + q.ch] = float2{total, any ? 1.f : 0.f};
   } else if (te == a.T) {
     store_states(a.h_n, q, a, h);
   }
 }
 
-// f(integral_constant fmt, ScanShape).
+// f(integral_constant fmt, ScanShape): four states a wave where every CU gets two workgroups or more, whose
+// barriers then hide behind each other, and two a wave (so twice the waves) where it gets fewer.  us, bf16,
+// 16 states, four / two a wave: T4096 B16 D1024 (256 workgroups) 678 / 547; fp16 T16383 B1 D1024 in 512
+// segments' workgroups 117 / 147.  One state a wave (16 waves): 658 and 172.
 template <class Fn>
-int with_fwd_shape(int fmt, int N, Fn f) {
+int with_fwd_shape(int fmt, int N, long long workgroups, Fn f) {
   return with_fmt(fmt, [&](auto F) {
+    const bool many = workgroups >= 512;
     switch (scan_states(N)) {
-      case 4: return f(F, ScanShape<2, 2>{});
-      case 8: return f(F, ScanShape<4, 2>{});
-      case 16: return f(F, ScanShape<8, 2>{});
-      case 32: return f(F, ScanShape<16, 2>{});
+      case 4: return many ? f(F, ScanShape<1, 4>{}) : f(F, ScanShape<2, 2>{});
+      case 8: return many ? f(F, ScanShape<2, 4>{}) : f(F, ScanShape<4, 2>{});
+      case 16: return many ? f(F, ScanShape<4, 4>{}) : f(F, ScanShape<8, 2>{});
+      case 32: return many ? f(F, ScanShape<8, 4>{}) : f(F, ScanShape<16, 2>{});
       default: return f(F, ScanShape<16, 4>{});
     }
   });
@@ -323,7 +317,7 @@ int hsl_selective_fwd(const void* x, long long x_t, long long x_b, const void* d
   g.seg_steps = p.seg_steps;
   g.nseg = p.nseg;
   g.map_h = static_cast<float*>(ws);
-  return with_fwd_shape(fmt, N, [&](auto F, auto shape) {
+  return with_fwd_shape(fmt, N, (long long)p.tiles * B * p.nseg, [&](auto F, auto shape) {
     constexpr int kF = decltype(F)::value;
     using P = decltype(shape);
     if (step) {
