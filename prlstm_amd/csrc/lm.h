@@ -175,6 +175,17 @@ __device__ __forceinline__ float sum_rows(float (&r)[16], int lane) {
   return (b1 ? r[1] : r[0]) + lane_move<0xb1>(b1 ? r[0] : r[1]);                                       // quad 1,0,3,2
 }
 
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+constexpr float kLog2e = 1.44269502162933349609375f;
+
+// sigmoid(z) next to values of format F.  Rounding z log2 e to fp32 counts as one more rounding of z, which
+// 16-bit results (2^-9 or 2^-12 of themselves) do not show, so exp is one product and v_exp_f32 there.
+template <int F>
+__device__ __forceinline__ float gate_sigmoid(float z) {
+  if constexpr (F == kElemF32) return sigmoid_f(z);
+  return __builtin_amdgcn_rcpf(1.f + exp2_f(-kLog2e * z));
+}
+
 // f(integral_constant<int, fmt>) for the element format of a call.
 template <class Fn>
 int with_fmt(int fmt, Fn f) {

@@ -27,7 +27,6 @@ constexpr int kShortRow = 2048;      // logits of a row that one wave takes
 constexpr long long kLaunchRows = 1 << 23;  // workgroups of a launch: their threads stay below 2^32
 constexpr int kRowLanes = 4;         // of a group in a row of one workgroup
 constexpr int kCandidates = 2048;    // elements that may be ranked among a row's alternatives
-constexpr float kLog2e = 1.44269502162933349609375f;
 constexpr float kLowest = -3.402823466e38f;
 // A running sum keeps its reference until a logit exceeds it by this much: e^8 is far from
 // overflow, and the terms of sd stay within 8 + their distance from the largest logit.

@@ -62,9 +62,6 @@ __device__ __forceinline__ float softplus_f(float u, float e) {
   return fmaxf(u, 0.f) + __builtin_fmaf(__builtin_amdgcn_logf(w), 0.693147182464599609375f, e - (w - 1.f));
 }
 
-__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
-constexpr float kLog2e = 1.44269502162933349609375f;
-
 // The decay exp(a S) of a segment whose dt sum to S.  One that underflows is held at the smallest
 // number, so that an infinite state stays infinite.
 __device__ __forceinline__ float segment_decay(float a2, float S) {
@@ -221,13 +218,6 @@ __device__ __forceinline__ void load_row(const float* p, float (&v)[S]) {
   }
 }
 
-// sigmoid(z).  A 16-bit z has an error of 2^-9 (bf16) or 2^-12 of itself, against which that of rounding
-// z log2 e to fp32 does not count, so exp is one product and v_exp_f32 there.
-template <int F>
-__device__ __forceinline__ float gate_sigmoid(float z) {
-  if constexpr (F == kElemF32) return sigmoid_f(z);
-  return __builtin_amdgcn_rcpf(1.f + exp2_f(-kLog2e * z));
-}
 // z sigmoid(z), 1 where there is no z.
 template <int F>
 __device__ __forceinline__ float gate_of(float z, bool there) {

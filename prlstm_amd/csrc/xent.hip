@@ -18,7 +18,6 @@
 namespace hsl {
 namespace {
 
-constexpr float kLog2eX = 1.44269502162933349609375f;
 constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl (or fp32 logits)
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -29,13 +28,13 @@ __device__ __forceinline__ bool all_masked(float m, float s) { return m == neg_i
 // exp(l + ref / log2 e): the product and the difference are rounded once, which moves the result by
 // 2^-24 of l's and the reference's size, as much as their own roundings do.
 __device__ __forceinline__ float exp2_of(float l, float ref) {
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2eX, ref));
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, ref));
 }
 
 // Joins (m, sum exp(l - m)) of two parts of a row.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float big = fmaxf(m, m2), r = big == neg_inf() ? 0.f : big;
-  s = s * __builtin_amdgcn_exp2f((m - r) * kLog2eX) + s2 * __builtin_amdgcn_exp2f((m2 - r) * kLog2eX);
+  s = s * __builtin_amdgcn_exp2f((m - r) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - r) * kLog2e);
   m = big;
 }
 
@@ -174,7 +173,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
         }
         if (found && n < a.N) a.own[n] = l;
       }
-      const float ref = m == neg_inf() ? 0.f : -m * kLog2eX;
+      const float ref = m == neg_inf() ? 0.f : -m * kLog2e;
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -298,7 +297,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     for (int j = 0; j < 2; ++j) {
       const float4 row = info[par].rows[q.c + j * 32];
       const int own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
-      const float gi = row.z * row.y, ref = -row.x * kLog2eX;
+      const float gi = row.z * row.y, ref = -row.x * kLog2e;
       const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
       // a masked logit has none whatever arrives, nor has a row without a gradient whatever it holds
       const bool plain =
@@ -489,7 +488,7 @@ __global__ __launch_bounds__(256) void xent_f32_stats_kernel(const float* __rest
   for (int v = threadIdx.x; v < V; v += 256) {
     const float x = row[v];
     const float big = fmaxf(m, x), r = big == neg_inf() ? 0.f : big;
-    s = s * __builtin_amdgcn_exp2f((m - r) * kLog2eX) + exp_f(x - r);
+    s = s * __builtin_amdgcn_exp2f((m - r) * kLog2e) + exp_f(x - r);
     m = big;
   }
 #pragma unroll
