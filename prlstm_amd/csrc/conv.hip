@@ -20,15 +20,15 @@ namespace {
 constexpr int kBlock = 8;      // steps whose loads are issued together
 constexpr int kMaxTaps = 4;
 constexpr int kMaxSeg = 256;   // steps that an fp32 sum runs over
-constexpr int kFwdWaves = 4, kBwdWaves = 8;
+constexpr int kWaves = 4;        // of a workgroup
 
 // A call's split: a row of the work is one segment of one batch row, row = segment * B + b; a wave
 // holds 64 >> log2g rows of 1 << log2g vectors each, and `tiles` waves cover a row's vectors.
 struct ConvPlan {
   int per, log2g, tiles, seg, nseg;
   long long rows;
-  int row_blocks(int waves) const {
-    const int each = waves * (64 >> log2g);
+  int row_blocks() const {
+    const int each = kWaves * (64 >> log2g);
     return (int)((rows + each - 1) / each);
   }
 };
@@ -138,7 +138,7 @@ __device__ __forceinline__ void load_taps(const ConvArgs& a, int j, float (&w)[K
 // Forward.  Bound by HBM: 50 us at T4096 B16 D1024 K4, bf16 (268 MB, 5.4 TB/s).  Whole blocks of steps run
 // without a test per step: with the tests, and exp in full precision, it was 66 us.
 template <int F, int E, int K, bool RESET>
-__global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
+__global__ __launch_bounds__(kWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   using T_ = typename Elem<F>::T;
   const ConvPlace<E> q(a);
   if (!q.ok) return;
@@ -193,13 +193,14 @@ __global__ __launch_bounds__(kFwdWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   }
 }
 
-// Backward.  E = 4, for which the window, the taps and both kinds of sums fit into 128 registers.  95 us at
-// T4096 B16 D1024 K4, bf16 (403 MB, 4.2 TB/s); with a test per step, and of every weight's sum for the steps
-// behind the segment, it was 117 us, the vector units as busy as the memory.
+// Backward.  E = 4: the window, the taps and both kinds of sums take 150 registers, so 3 waves share a SIMD
+// (held to 128 registers for a fourth, they spill: 127 us for the call).  93 us at T4096 B16 D1024 K4, bf16
+// (403 MB, 4.3 TB/s); with a test per step, and of every weight's sum for the steps behind the segment, it
+// was 117 us, the vector units as busy as the memory.
 template <int F, int E, int K, bool RESET>
-__global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
+__global__ __launch_bounds__(kWaves * 64) void conv_bwd_kernel(ConvArgs a) {
   using T_ = typename Elem<F>::T;
-  __shared__ float sm[kBwdWaves][K + 1][64 * E];
+  __shared__ float sm[kWaves][K + 1][64 * E];
   const ConvPlace<E> q(a);
   const Walk<F, E, K, RESET> walk(a, q);
   float w[K][E], bias[E], dw[K + 1][E];  // dw[K]: the bias's
@@ -312,12 +313,12 @@ __global__ __launch_bounds__(kBwdWaves * 64) void conv_bwd_kernel(ConvArgs a) {
   __syncthreads();
   const int tile = blockIdx.x % a.p.tiles;
   float* const out = a.part + (long long)(blockIdx.x / a.p.tiles) * (K + 1) * a.D;
-  for (int i = threadIdx.x; i < (K + 1) * g * E; i += kBwdWaves * 64) {
+  for (int i = threadIdx.x; i < (K + 1) * g * E; i += kWaves * 64) {
     const int k = i / (g * E), l = i % (g * E), vec = (tile << a.p.log2g) + l / E;
     if (vec >= a.p.per) continue;
     float v = 0.f;
 #pragma unroll
-    for (int n = 0; n < kBwdWaves; ++n) v += sm[n][k][l];
+    for (int n = 0; n < kWaves; ++n) v += sm[n][k][l];
     out[(long long)k * a.D + min(vec * E, a.D - E) + l % E] = v;
   }
 }
@@ -474,7 +475,7 @@ int hsl_conv_fwd(const void* x, long long x_t, long long x_b, const float* w, co
       a.silu = silu;
       const int e = fwd_vec(D, fmt);
       a.p = plan_conv(T, B, D, e);
-      const dim3 grid((unsigned)a.p.row_blocks(kFwdWaves) * a.p.tiles), block(kFwdWaves * 64);
+      const dim3 grid((unsigned)a.p.row_blocks() * a.p.tiles), block(kWaves * 64);
       if (e == 1)
         hipLaunchKernelGGL((conv_fwd_kernel<kF, 1, kK, kR>), grid, block, 0, s, a);
       else
@@ -487,7 +488,7 @@ int hsl_conv_fwd(const void* x, long long x_t, long long x_b, const float* w, co
 
 size_t hsl_conv_ws_bytes(int T, int B, int D, int K) {
   if (check_conv("hsl_conv_ws_bytes", T, B, D, K, kElemF32) != HSL_OK || B == 0 || D == 0) return 0;
-  return (size_t)plan_conv(T, B, D, bwd_vec(D)).row_blocks(kBwdWaves) * (K + 1) * D * sizeof(float);
+  return (size_t)plan_conv(T, B, D, bwd_vec(D)).row_blocks() * (K + 1) * D * sizeof(float);
 }
 
 int hsl_conv_bwd(const void* x, long long x_t, long long x_b, const float* w, const float* bias, const void* state,
@@ -519,11 +520,11 @@ int hsl_conv_bwd(const void* x, long long x_t, long long x_b, const float* w, co
     a.D = D;
     a.silu = silu;
     a.p = plan_conv(T, B, D, bwd_vec(D));
-    parts = a.p.row_blocks(kBwdWaves);
+    parts = a.p.row_blocks();
     HSL_CHECK(with_conv(fmt, K, reset != nullptr, [&](auto F, auto KK, auto R) {
       constexpr int kF = decltype(F)::value, kK = decltype(KK)::value;
       constexpr bool kR = decltype(R)::value;
-      const dim3 grid((unsigned)parts * a.p.tiles), block(kBwdWaves * 64);
+      const dim3 grid((unsigned)parts * a.p.tiles), block(kWaves * 64);
       if (bwd_vec(D) == 1)
         hipLaunchKernelGGL((conv_bwd_kernel<kF, 1, kK, kR>), grid, block, 0, s, a);
       else
