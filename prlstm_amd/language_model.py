@@ -3,16 +3,22 @@
 Token ids are embedded (``embedding``), run through a ``HeadStartLSTM`` layer and gated recurrences
 (``gated_recurrence``), and projected on the vocabulary; the log probabilities of the next tokens
 (``token_logprobs``) are the training loss and what a server answers with.  ``step`` takes one token of
-each of a batch of streams and updates their state in place.
+each of a batch of streams and updates their state in place.  On request selective layers
+(``causal_conv``, ``selective_scan``) follow, and the loss is computed without the logits
+(``linear_cross_entropy``).
 
 ``python -m prlstm_amd.language_model`` trains one on walks around a circle and continues them.
 """
+
+import math
 
 import torch
 import torch.nn as nn
 
 from . import HeadStartLSTM
+from .cross_entropy import linear_cross_entropy
 from .lm import embedding, gated_recurrence, gated_recurrence_step, token_logprobs
+from .selective import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 
 
 class GatedLayer(nn.Module):
@@ -35,11 +41,61 @@ class GatedLayer(nn.Module):
         return x + out
 
 
+class SelectiveLayer(nn.Module):
+    """``x + project(selective_scan(causal_conv(u), ..., z))`` with u and z projections of the normalised
+    x to twice its width: a short convolution, then ``states`` states per channel whose step, input and
+    output the convolution's output chooses.  Its state is the pair of theirs."""
+
+    TAPS = 4
+
+    def __init__(self, width, states=16):
+        super().__init__()
+        inner, rank = 2 * width, -(-width // 16)
+        self.inner, self.rank, self.states = inner, rank, states
+        self.norm = nn.LayerNorm(width)
+        self.enter = nn.Linear(width, 2 * inner, bias=False)
+        self.taps = nn.Parameter(torch.randn(inner, self.TAPS) * self.TAPS ** -0.5)
+        self.taps_bias = nn.Parameter(torch.zeros(inner))
+        self.choose = nn.Linear(inner, rank + 2 * states, bias=False)
+        self.widen = nn.Linear(rank, inner, bias=False)
+        # steps of 0.001 to 0.1 at first, and states that fade 1 to `states` times as fast
+        dt = torch.exp(torch.empty(inner).uniform_(math.log(1e-3), math.log(1e-1)))
+        self.delta_bias = nn.Parameter(torch.log(torch.expm1(dt)))
+        self.log_a = nn.Parameter(torch.log(torch.arange(1.0, states + 1)).repeat(inner, 1))
+        self.skip = nn.Parameter(torch.ones(inner))
+        self.leave = nn.Linear(inner, width, bias=False)
+
+    def state(self, batch):
+        like = self.taps
+        return (like.new_zeros(batch, self.TAPS - 1, self.inner),
+                torch.zeros(batch, self.inner, self.states, dtype=torch.float32, device=like.device))
+
+    def chosen(self, u):
+        """delta, a, b and c of the scan."""
+        delta, b, c = self.choose(u).split((self.rank, self.states, self.states), -1)
+        return self.widen(delta), -torch.exp(self.log_a.float()), b, c
+
+    def forward(self, x, state=None, reset=None):
+        last, h = (None, None) if state is None else state
+        u, z = self.enter(self.norm(x)).chunk(2, -1)
+        u, last = causal_conv(u, self.taps, self.taps_bias, last, reset)
+        y, h = selective_scan(u, *self.chosen(u), self.skip, z, self.delta_bias, h, reset)
+        return x + self.leave(y), (last, h)
+
+    def step(self, x, state, reset=None):
+        last, h = state
+        u, z = self.enter(self.norm(x)).chunk(2, -1)
+        u, _ = causal_conv_step(u, last, self.taps, self.taps_bias, reset, state_out=last)
+        y, _ = selective_scan_step(u, *self.chosen(u), h, self.skip, z, self.delta_bias, reset, h_out=h)
+        return x + self.leave(y)
+
+
 class LanguageModel(nn.Module):
     """Next-token model over time-major ids [T, B].  A negative id is a padded position: its
-    embedding is zero and it is not scored."""
+    embedding is zero and it is not scored.  ``selective`` layers of ``states`` states per channel
+    follow the gated ones."""
 
-    def __init__(self, vocab, width, layers=2, parallel=True):
+    def __init__(self, vocab, width, layers=2, parallel=True, selective=0, states=16):
         super().__init__()
         self.vocab, self.width = vocab, width
         self.weight = nn.Parameter(torch.randn(vocab, width) * width ** -0.5)
@@ -47,12 +103,15 @@ class LanguageModel(nn.Module):
         self.layers = nn.ModuleList(GatedLayer(width) for _ in range(layers))
         self.norm = nn.LayerNorm(width)
         self.head = nn.Linear(width, vocab)
+        self.layers.extend(SelectiveLayer(width, states) for _ in range(selective))
 
     def state(self, batch):
-        """The state of ``batch`` new streams: the LSTM's (h, c) and each gated layer's, in fp32."""
+        """The state of ``batch`` new streams: the LSTM's (h, c) and each gated layer's, in fp32, then
+        each selective layer's pair."""
         like = dict(dtype=torch.float32, device=self.weight.device)
         zeros = lambda: torch.zeros(batch, self.width, **like)  # noqa: E731
-        return (zeros(), zeros()), [zeros() for _ in self.layers]
+        return (zeros(), zeros()), [layer.state(batch) if isinstance(layer, SelectiveLayer) else zeros()
+                                    for layer in self.layers]
 
     def logits(self, x):
         return self.head(self.norm(x))
@@ -73,9 +132,8 @@ class LanguageModel(nn.Module):
             parts.append(y)
         return torch.cat(parts), h, c
 
-    def forward(self, ids, state=None, reset=None):
-        """(logits [T, B, V], the state behind them).  Where ``reset`` [T, B] is set a new document
-        begins: nothing of any layer's state passes."""
+    def hidden(self, ids, state=None, reset=None):
+        """(what the projection on the vocabulary reads before it is normalised, the state behind it)."""
         (h, c), gated = self.state(ids.shape[1]) if state is None else state
         x = embedding(ids, self.weight, scale=self.width ** 0.5)
         y, h, c = self.run_lstm(x, h.to(x.dtype), c.to(x.dtype), reset)
@@ -84,13 +142,22 @@ class LanguageModel(nn.Module):
         for layer, h0 in zip(self.layers, gated):
             x, h1 = layer(x, h0, reset)
             after.append(h1)
-        return self.logits(x), ((h.float(), c.float()), after)
+        return x, ((h.float(), c.float()), after)
 
-    def loss(self, ids, targets, reset=None):
-        """Mean negative log probability of targets [T, B] (negative: not scored)."""
-        logits, _ = self(ids, reset=reset)
+    def forward(self, ids, state=None, reset=None):
+        """(logits [T, B, V], the state behind them).  Where ``reset`` [T, B] is set a new document
+        begins: nothing of any layer's state passes."""
+        x, after = self.hidden(ids, state, reset)
+        return self.logits(x), after
+
+    def loss(self, ids, targets, reset=None, keep_logits=True):
+        """Mean negative log probability of targets [T, B] (negative: not scored).  With
+        ``keep_logits=False`` neither the logits nor their gradient are in memory at once."""
+        x, _ = self.hidden(ids, reset=reset)
         scored = (targets >= 0).sum().clamp_min(1)
-        return -token_logprobs(logits, targets).logp.sum() / scored
+        if not keep_logits:
+            return linear_cross_entropy(self.norm(x), self.head.weight, targets, self.head.bias).sum() / scored
+        return -token_logprobs(self.logits(x), targets).logp.sum() / scored
 
     @torch.no_grad()
     def step(self, ids, state, top=0):
