@@ -19,6 +19,7 @@ namespace hsl {
 namespace {
 
 constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl (or fp32 logits)
+constexpr int kPieceWidth = 1 << 21;        // tokens at most: 256 rows of dl lie within 2^31 bytes
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
@@ -570,7 +571,8 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   XentPlan p;
   const size_t es = fmt == kElemF32 ? 4 : 2;
   const int all = up_to(V, kMmTile);
-  const long long fit = std::max<long long>(1, (long long)(kPieceBytes / es / std::max(1, N)) / kMmTile) * kMmTile;
+  const long long room = std::min<long long>(kPieceWidth, kPieceBytes / es / std::max(1, N));
+  const long long fit = std::max<long long>(1, room / kMmTile) * kMmTile;
   p.piece = (int)std::min<long long>(all, fit);
   p.pieces = (all + p.piece - 1) / p.piece;
   p.piece = up_to((all + p.pieces - 1) / p.pieces, kMmTile);
@@ -595,13 +597,13 @@ int check_xent(const char* who, long long N, int V, int D, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
   if (N < 0 || V < 0 || D < 0) return fail(HSL_ERR_ARG, "%s: negative size (N=%lld V=%d D=%d)", who, N, V, D);
   if (V == 0 || D == 0) return fail(HSL_ERR_ARG, "%s: an empty projection (V=%d D=%d)", who, V, D);
-  // a launch holds fewer than 2^32 threads, and rows of a tile lie within 2^31 bytes
-  if (N >= (1ll << 31) - 256 || V >= 0x7fffffff - 256 || D >= (1 << 20) ||
+  // a launch holds fewer than 2^32 threads (256 a row at most), and rows of a tile lie within 2^31 bytes
+  if (N >= (1ll << 24) || V >= 0x7fffffff - 256 || D >= (1 << 20) ||
       ((N + 255) / 256) * (((long long)V + 255) / 256) >= (1ll << 22) ||
       ((N + 255) / 256 + ((long long)V + 255) / 256) * ((D + 255) / 256) >= (1ll << 22))
     return fail(HSL_ERR_UNSUPPORTED,
-                "%s: N=%lld V=%d D=%d is beyond one launch (needs D < 2^20 and fewer than 2^22 tiles of 256 x 256 of "
-                "each product)",
+                "%s: N=%lld V=%d D=%d is beyond one launch (needs N < 2^24, D < 2^20 and fewer than 2^22 tiles of 256 x "
+                "256 of each product)",
                 who, N, V, D);
   return HSL_OK;
 }

@@ -63,6 +63,13 @@ def _weight(name, t, shape, x):
     return t.float().contiguous()
 
 
+def _check_out(name, out, source):
+    """An output that the caller gives: it may be the operand it replaces, but not a part of it."""
+    p, q, size = out.data_ptr(), 0 if source is None else source.data_ptr(), out.nbytes
+    if p != q and q - size < p < q + size:
+        raise RuntimeError(f"{name} overlaps the state that it is computed from")
+
+
 def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -151,7 +158,7 @@ def causal_conv(x, weight, bias=None, state=None, reset=None, activation="silu")
 def causal_conv_step(x, state, weight, bias=None, reset=None, activation="silu", state_out=None):
     """One step of ``causal_conv`` without gradients, for serving: x [B, D], state [B, K-1, D] (None:
     zeros), reset [B].  Returns (y [B, D], the new state); ``state_out`` receives the state where it is
-    given, and may be state itself.
+    given; it may be state itself, and shares no memory with the other operands.
     """
     fmt, weight, bias, k, silu = _conv_check(x, weight, bias, state, reset, activation, 1)
     b, d = x.shape
@@ -161,6 +168,7 @@ def causal_conv_step(x, state, weight, bias=None, reset=None, activation="silu",
     given = state_out is not None
     if given:
         _check_like("state_out", state_out, (b, k - 1, d), x)
+        _check_out("state_out", state_out, state)
     else:
         state_out = x.new_empty(b, k - 1, d)
     x = _unit_inner(x)
@@ -279,7 +287,8 @@ def selective_scan(x, delta, a, b, c, d=None, z=None, delta_bias=None, h0=None, 
 def selective_scan_step(x, delta, a, b, c, h, d=None, z=None, delta_bias=None, reset=None, softplus=True, h_out=None):
     """One step of ``selective_scan`` without gradients, for serving: x, delta and z [B, D], b and c
     [B, N], the state h [B, D, N] in fp32 (None: zeros), reset [B].  Returns (y [B, D] in x's dtype,
-    the new state in fp32); ``h_out`` receives the state where it is given, and may be h itself.
+    the new state in fp32); ``h_out`` receives the state where it is given; it may be h itself, and
+    shares no memory with the other operands.
     """
     fmt, a, d, delta_bias = _scan_check(x, delta, a, b, c, d, z, delta_bias, h, reset, 1)
     bsz, width = x.shape
@@ -291,7 +300,9 @@ def selective_scan_step(x, delta, a, b, c, h, d=None, z=None, delta_bias=None, r
             raise RuntimeError(f"{name} must be a contiguous float32 tensor {state} on {x.device}, got {t.dtype} "
                                f"{tuple(t.shape)} on {t.device}")
     given = h_out is not None
-    if not given:
+    if given:
+        _check_out("h_out", h_out, h)
+    else:
         h_out = torch.empty(state, dtype=torch.float32, device=x.device)
     x, delta, b, c = _unit_inner(x), _unit_inner(delta), _unit_inner(b), _unit_inner(c)
     z = None if z is None else _unit_inner(z)

@@ -34,6 +34,22 @@ def test_refusals(call):
     _refused(call(N=(1 << 31) - 1, V=1), 2, b"beyond one launch")
 
 
+@pytest.mark.parametrize("call", [_fwd, _bwd])
+def test_more_rows_than_a_launch_has(call):
+    """A workgroup of 256 threads a row: 2^24 rows would be 2^32 threads, which wrap."""
+    for fmt in (0, 1, 2):
+        _refused(call(N=1 << 24, V=1, fmt=fmt, p=1), 2, b"beyond one launch")
+        assert _lib.load().hsl_xent_ws_bytes(1 << 24, 1, 8, fmt, 1) == 0
+        _refused(call(N=(1 << 24) - 1, V=1, fmt=fmt, p=1), 1, b"workspace 0 bytes")
+
+
+def test_a_piece_is_no_wider_than_its_offsets():
+    """256 rows of a piece's dl lie within 2^31 bytes, so few rows do not make it wider than 2^21 tokens."""
+    f = _lib.load().hsl_xent_ws_bytes
+    more = [f(3, 1 << e, 8, 0, 1) - f(3, 1 << e, 8, 0, 0) for e in (21, 22, 24)]  # dl, beside what both keep
+    assert more[0] >= 3 * 2 << 21 and more[1] <= more[0] and more[2] <= more[0]
+
+
 def test_calls_without_positions_do_nothing():
     assert _fwd(N=0) == 0 and _bwd(N=0) == 0
 
