@@ -7,9 +7,15 @@
 // vocabulary and whose columns are the positions, so that a lane has 64 logits of each of 2 positions in
 // registers.  The forward reduces them to the tile's largest logit and sum of exponentials, from which a
 // second kernel makes the loss; no logit leaves the registers.  The backward computes the logits again,
-// a piece of the vocabulary at a time, and writes the piece's dl, rounded to 16 bits (as every operand
-// of a product on these instructions is; its error of half a step is what rounding dx and dw once costs
-// again), from which one launch makes the piece's dw and adds to dx, both in fp32.
+// a piece of the vocabulary at a time, and writes the piece's dl in fp16, from which one launch makes the
+// piece's dw and adds to dx, both in fp32.
+//   Rounding dl is the one error that a sum of two roundings' size in dx and dw would show, and fp16's is
+// 2^-11 where bf16's, 2^-8, is as large as that of the results themselves (with it bf16 gradients were 1.4
+// times as far from the exact ones as when rounded once, few rows' up to twice).  So bf16 operands enter
+// these two products as fp16 too, which holds their 8 bits.  Range is made up for by powers of two: a row of dl
+// is scaled to |g| = 2^14 .. 2^15, x to as large an element less what its row's g is below the largest one, a
+// bf16 w to as large an element; the results take them back.  What is then below fp16's 2^-24 counts as 0: a
+// probability below 2^-38, an element 2^-38 of its operand's largest.
 // fp32 operands: pieces of the logits are products on the library's fp32 kernels, kept in fp32.
 #include <algorithm>
 
@@ -236,38 +242,171 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 }
 
 
-// A power of two that brings the largest |dloss| to 2^14 .. 2^15, and its inverse: fp16 has 2^-14 for
-// its smallest normal number, and the gradients of a mean over thousands of rows are far below it.
-__global__ __launch_bounds__(1024) void xent_scale_kernel(const float* dloss, float* scale, int N) {
-  __shared__ float sm[16];
-  float m = 0.f;
-  for (long long n = threadIdx.x; n < N; n += 1024) m = fmaxf(m, __builtin_fabsf(dloss[n]));
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) m = fmaxf(m, __shfl_xor(m, k));
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x) return;
-  for (int k = 1; k < 16; ++k) m = fmaxf(m, sm[k]);
-  const int e = m == 0.f ? 14 : (int)(__float_as_uint(m) >> 23) - 127;
-  const int up = min(100, max(-100, 14 - e));
-  scale[0] = __uint_as_float((unsigned)(127 + up) << 23);
-  scale[1] = __uint_as_float((unsigned)(127 - up) << 23);
+// A row's gradient: none where the target is outside of the vocabulary or nothing but masks is in the row.
+__device__ __forceinline__ float row_gradient(float2 stats, int target, float dloss) {
+  return target >= 0 && !all_masked(stats.x, stats.y) ? dloss : 0.f;
 }
-
-// What the backward needs of each row.  No gradient where the target is outside of the vocabulary or
-// nothing but masks is in the row.
+// What the backward needs of each row: the largest logit, g / sum, g, and 2^(its exponent less the largest row's),
+// negative where the target is masked.
+__device__ __forceinline__ float4 row_of(float2 s, float g, int t, const float* bias, float part) {
+  return float4{s.x, g * (1.f / s.y), g, t >= 0 && bias && bias[t] == neg_inf() ? -part : part};
+}
 __global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ stats, const int* __restrict__ target,
                                                         const float* __restrict__ dloss, const float* bias,
-                                                        const float* scale, float4* rows, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;  // up to whole tiles
-  if (n >= N) {
-    rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+                                                        float4* rows, int N) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n < N) rows[n] = row_of(stats[n], row_gradient(stats[n], target[n], dloss[n]), target[n], bias, 1.f);
+}
+
+// 16-bit operands' scales.  The rows of a matrix among the threads of `blocks` workgroups: 1 << lg of them a row.
+struct RowSplit {
+  int lg, blocks;
+  long long rows;
+};
+constexpr int kTopExp = 14;  // of the largest element of what is scaled
+struct ScaleArgs {
+  const unsigned short *x, *w;  // of width elements, a multiple of 8, at ldx and ldw
+  long long ldx, ldw;
+  int width;
+  RowSplit rx, rw;              // rw: no workgroups for an fp16 w
+  int blocks_g;                 // for the rows' gradients
+  const float2* stats;
+  const int* target;
+  const float *dloss, *bias;
+  unsigned* part;               // the workgroups' largest magnitudes
+  int* exps;                    // [3]: exponents of the largest g, of x's scale and of w's
+  unsigned short *hx, *hw;      // the scaled operands in fp16, dense
+  float4* rows;
+  int* row_exp;
+  int N;
+};
+
+__device__ __forceinline__ unsigned block_max(unsigned m) {
+  __shared__ unsigned sm[4];
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) m = max(m, (unsigned)__shfl_xor((int)m, k));
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
+  __syncthreads();
+  return max(max(sm[0], sm[1]), max(sm[2], sm[3]));
+}
+__device__ __forceinline__ int exp_of(float v) { return (int)((__float_as_uint(v) >> 23) & 0xff) - 127; }
+// f(row, vector) for the vectors of 8 elements of workgroup `block`'s rows, 4 rows at a time; there is no such
+// row where it is -1.
+template <class Fn>
+__device__ __forceinline__ void for_rows(const RowSplit& r, int vecs, int block, Fn f) {
+  const long long step = (long long)r.blocks * (256 >> r.lg);
+  const int mine = threadIdx.x & ((1 << r.lg) - 1);
+  for (long long row = (long long)block * (256 >> r.lg) + (threadIdx.x >> r.lg); row < r.rows; row += 4 * step)
+    for (int c = mine; c < vecs; c += 1 << r.lg) {
+      long long at[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) at[k] = row + k * step < r.rows ? row + k * step : -1;
+      f(at, c);
+    }
+}
+
+// The largest finite magnitudes, as bits: of elements in a workgroup's rows, or of rows' gradients in fp32.
+template <bool FP16>
+__global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
+  constexpr unsigned kInf = FP16 ? 0x7c00 : 0x7f80;
+  const int b = blockIdx.x;
+  unsigned m = 0;
+  if (b < a.rx.blocks + a.rw.blocks) {
+    const bool is_x = b < a.rx.blocks;
+    const unsigned short* const p = is_x ? a.x : a.w;
+    const long long ld = is_x ? a.ldx : a.ldw;
+    for_rows(is_x ? a.rx : a.rw, a.width / 8, is_x ? b : b - a.rx.blocks, [&](const long long(&row)[4], int c) {
+      mm_u4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = row[k] < 0 ? mm_u4{} : *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned lo = v[k][e] & 0x7fff, hi = (v[k][e] >> 16) & 0x7fff;
+          m = max(m, max(lo < kInf ? lo : 0, hi < kInf ? hi : 0));
+        }
+    });
+  } else {
+    for (long long n = (b - a.rx.blocks - a.rw.blocks) * 256 + threadIdx.x; n < a.N; n += a.blocks_g * 256) {
+      const unsigned g = __float_as_uint(row_gradient(a.stats[n], a.target[n], a.dloss[n])) & 0x7fffffff;
+      m = max(m, g < 0x7f800000 ? g : 0);
+    }
+  }
+  m = block_max(m);
+  if (threadIdx.x == 0) a.part[b] = m;
+}
+
+// The scaled operands, and the rows.
+template <bool FP16>
+__global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
+  using E = Elem<FP16 ? kElemF16 : kElemBf16>;
+  const int b = blockIdx.x;
+  const bool is_x = b < a.rx.blocks, is_w = !is_x && b < a.rx.blocks + a.rw.blocks;
+  const int first = is_x ? 0 : a.rx.blocks, count = is_x ? a.rx.blocks : a.rw.blocks;
+  unsigned g = 0, m = 0;
+  if (!is_w)
+    for (int i = threadIdx.x; i < a.blocks_g; i += 256) g = max(g, a.part[a.rx.blocks + a.rw.blocks + i]);
+  if (is_x || is_w)
+    for (int i = threadIdx.x; i < count; i += 256) m = max(m, a.part[first + i]);
+  g = block_max(g);
+  __syncthreads();
+  m = block_max(m);
+  constexpr int kLeast = kTopExp - 126;  // 2^126 is the largest power of two that a row of small g is scaled by
+  const int top = g ? max(kLeast, exp_of(__uint_as_float(g))) : 0;
+  const int up = m ? kTopExp - exp_of(E::up((unsigned short)m)) : 0;
+  auto exponent = [&](float g) {
+    return g == 0.f || !(__builtin_fabsf(g) < __builtin_inff()) ? top : max(kLeast, exp_of(g));
+  };
+  if (is_x || is_w) {
+    if (threadIdx.x == 0 && b == first) a.exps[is_x ? 1 : 2] = up;
+    const unsigned short* const p = is_x ? a.x : a.w;
+    unsigned short* const out = is_x ? a.hx : a.hw;
+    const long long ld = is_x ? a.ldx : a.ldw;
+    for_rows(is_x ? a.rx : a.rw, a.width / 8, b - first, [&](const long long(&row)[4], int c) {
+      mm_u4 v[4];
+      int e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (row[k] < 0) continue;
+        v[k] = *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+        e[k] = up;
+        if (is_x) e[k] += exponent(row_gradient(a.stats[row[k]], a.target[row[k]], a.dloss[row[k]])) - top;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (row[k] < 0) continue;
+        unsigned short h[8];
+        __builtin_memcpy(h, &v[k], 16);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __builtin_ldexpf(E::up(h[i]), e[k]);
+        down_all<kElemF16, 8>(f, h);
+        __builtin_memcpy(&v[k], h, 16);
+        *reinterpret_cast<mm_u4*>(out + row[k] * a.width + c * 8) = v[k];
+      }
+    });
     return;
   }
-  const float2 s = stats[n];
-  const int t = target[n];
-  const float g = t >= 0 && !all_masked(s.x, s.y) ? dloss[n] * (scale ? scale[0] : 1.f) : 0.f;
-  rows[n] = float4{s.x, 1.f / s.y, g, t >= 0 && bias && bias[t] == neg_inf() ? 0.f : g};
+  const int blocks = gridDim.x - a.rx.blocks - a.rw.blocks, block = b - a.rx.blocks - a.rw.blocks;
+  if (block == 0 && threadIdx.x == 0) {
+    a.exps[0] = top;
+    if (a.rw.blocks == 0) a.exps[2] = 0;
+  }
+  const int all = (a.N + kMmTile - 1) / kMmTile * kMmTile;
+  for (int n = block * 256 + threadIdx.x; n < all; n += blocks * 256) {  // up to whole tiles
+    if (n >= a.N) {
+      a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+      continue;
+    }
+    const float2 s = a.stats[n];
+    const int t = a.target[n];
+    const float g = row_gradient(s, t, a.dloss[n]);
+    const int e = exponent(g);
+    a.rows[n] = row_of(s, __builtin_ldexpf(g, kTopExp - e), t, a.bias, __builtin_ldexpf(1.f, e - top));
+    a.row_exp[n] = e;
+  }
 }
 
 // The tile's dl goes from the registers to memory: an exchange between the half-waves gives every lane 8
@@ -298,7 +437,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     for (int j = 0; j < 2; ++j) {
       const float4 row = info[par].rows[q.c + j * 32];
       const int own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
-      const float gi = row.z * row.y, ref = -row.x * kLog2e;
+      const float gi = row.y, ref = -row.x * kLog2e;
+      const float hot = __float_as_int(row.w) < 0 ? 0.f : row.z;
       const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
       // a masked logit has none whatever arrives, nor has a row without a gradient whatever it holds
       const bool plain =
@@ -321,7 +461,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
         }
         if (owns) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] -= own == i * 32 + 8 * (r >> 2) + (r & 3) ? row.w : 0.f;
+          for (int r = 0; r < 16; ++r) acc[i][j][r] -= own == i * 32 + 8 * (r >> 2) + (r & 3) ? hot : 0.f;
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -331,7 +471,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
             const float f[4] = {acc[i][j][8 * k + 2 * e], acc[i][j][8 * k + 2 * e + 1], acc[i][j][8 * k + 4 + 2 * e],
                                 acc[i][j][8 * k + 5 + 2 * e]};
             unsigned short h[4];
-            down_all<FP16 ? kElemF16 : kElemBf16, 4>(f, h);
+            down_all<kElemF16, 4>(f, h);
             __builtin_memcpy(&lo[e], h, 4);
             __builtin_memcpy(&hi[e], h + 2, 4);
           }
@@ -348,10 +488,11 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     }
     if (a.dbias) {  // in fp32, from before the rounding
       float f[2][16];
+      const float p0 = __builtin_fabsf(info[par].rows[q.c].w), p1 = __builtin_fabsf(info[par].rows[q.c + 32].w);
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
         const int u = 2 * k, i = u / 16, r = u % 16;
-        f[k / 16][k % 16] = add16(acc[i][0][r] + acc[i][1][r], acc[i][0][r + 1] + acc[i][1][r + 1]);
+        f[k / 16][k % 16] = add16(acc[i][0][r] * p0 + acc[i][1][r] * p1, acc[i][0][r + 1] * p0 + acc[i][1][r + 1] * p1);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -368,7 +509,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
 }
 
 // dbias of a piece from its tiles' sums, in fp64: 32 tokens by 8 strips of the tiles.
-__global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict__ part, const float* scale, float* dbias,
+__global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict__ part, const int* exps, float* dbias,
                                                         int V, long long ld, int tiles) {
   __shared__ double sm[8][32];
   const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, v = blockIdx.x * 32 + c;
@@ -379,21 +520,21 @@ __global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict_
   __syncthreads();
   if (strip || v >= V) return;
   for (int k = 1; k < 8; ++k) s += sm[k][c];
-  dbias[v] = (float)(scale ? s * scale[1] : s);
+  dbias[v] = (float)ldexp(s, exps[0] - kTopExp);
 }
 
 struct OutArgs {
-  const unsigned short *dl, *w, *x;
+  const unsigned short *dl, *w, *x;  // in fp16
   long long ld, ldw, ldx;   // of dl (the piece's padded width), w and x
   float *dx, *dw;           // planes [split][N][D] and [split][ld][D]; dw null: straight to dw16
   unsigned short* dw16;
-  const float* scale;
+  const int* exps;
   int N, V, D, Dk;          // V: the piece's tokens; Dk: the width that x and w have in memory
   int tiles_n, tiles_d, tiles_v, splits_x, splits_w, k_x, k_w, add;
 };
 
 // One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.
-template <bool FP16>
+template <int F>
 __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   const int count_x = a.splits_x * a.tiles_n * a.tiles_d;
@@ -408,21 +549,21 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
     const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
     const MmOperand A{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
     const MmOperand B{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
-    MmPipe<FP16, false, true> mm;
+    MmPipe<true, false, true> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   } else {
     const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
     const MmOperand A{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
     const MmOperand B{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
-    MmPipe<FP16, true, true> mm;
+    MmPipe<true, true, true> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int r0 = tm * kMmTile + (wave >> 2) * 128 + 4 * half, c0 = td * kMmTile + (wave & 3) * 64 + (lane & 31);
   const int rows = is_x ? a.N : a.V;
-  const float back = a.scale ? a.scale[1] : 1.f;
+  const int back = a.exps[0] - kTopExp - a.exps[1];
   float* const plane = is_x ? a.dx + (size_t)split * a.N * a.D : a.dw ? a.dw + (size_t)split * a.ld * a.D : nullptr;
   const bool add = is_x && a.add;
 #pragma unroll
@@ -439,22 +580,25 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
         if (plane)
           plane[at] = add ? plane[at] + acc[i][j][r] : acc[i][j][r];
         else
-          a.dw16[at] = Elem<FP16 ? kElemF16 : kElemBf16>::down(acc[i][j][r] * back);
+          a.dw16[at] = Elem<F>::down(__builtin_ldexpf(acc[i][j][r], back));
       }
     }
 }
 
-// out = the planes' sum, in their order.
+// Rows of `cols` of the sum of the planes, in their order, without their scales (row_exp: those of the rows).
 template <int F>
 __global__ __launch_bounds__(256) void xent_planes_kernel(const float* __restrict__ planes, size_t plane, int splits,
-                                                          const float* scale, void* out, size_t n) {
-  using T_ = typename Elem<F>::T;
-  const float back = scale ? scale[1] : 1.f;
-  const size_t stride = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-    float v = planes[i];
-    for (int s = 1; s < splits; ++s) v += planes[s * plane + i];
-    static_cast<T_*>(out)[i] = Elem<F>::down(v * back);
+                                                          const int* exps, const int* row_exp, void* out, RowSplit r,
+                                                          int cols) {
+  const long long step = (long long)r.blocks * (256 >> r.lg);
+  for (long long row = (long long)blockIdx.x * (256 >> r.lg) + (threadIdx.x >> r.lg); row < r.rows; row += step) {
+    const int back = row_exp ? row_exp[row] - kTopExp - exps[2] : exps[0] - kTopExp - exps[1];
+    for (int c = threadIdx.x & ((1 << r.lg) - 1); c < cols; c += 1 << r.lg) {
+      const size_t i = (size_t)row * cols + c;
+      float v = planes[i];
+      for (int s = 1; s < splits; ++s) v += planes[s * plane + i];
+      static_cast<typename Elem<F>::T*>(out)[i] = Elem<F>::down(__builtin_ldexpf(v, back));
+    }
   }
 }
 
@@ -518,7 +662,7 @@ __global__ __launch_bounds__(256) void xent_f32_grad_kernel(float* __restrict__ 
   float* const p = l + n * ld;
   const float4 row = rows[n];
   const int own = target[n] - v0;
-  const float gi = row.z * row.y;
+  const float gi = row.y;
   for (int v = threadIdx.x; v < V; v += 256) {
     const float x = p[v];
     float d = exp_f(x - row.x) * gi;
@@ -561,6 +705,15 @@ __global__ __launch_bounds__(256) void xent_f32_add_kernel(float* __restrict__ o
 
 int up_to(long long n, int unit) { return (int)((n + unit - 1) / unit * unit); }
 unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 1 << 16); }
+
+RowSplit split_rows(long long rows, int units, int most) {
+  RowSplit r{0, 0, rows};
+  while (r.lg < 8 && (1 << r.lg) < units) ++r.lg;
+  const int each = 256 >> r.lg;
+  r.blocks = (int)std::min<long long>(most, (rows + each - 1) / each);
+  return r;
+}
+constexpr int kScaleBlocks = 1024;  // for an operand
 
 struct XentPlan {
   int piece, pieces;  // tokens of a piece: a multiple of 256
@@ -620,8 +773,9 @@ struct XentSpace {
   float* own;
   float2* part;
   float4* rows;
-  float* scale;
-  unsigned short *packed_x, *packed_w;
+  unsigned* part_max;
+  int *exps, *row_exp;
+  unsigned short *packed_x, *packed_w, *scaled_x, *scaled_w;
   char* dl;  // 16-bit dl, or fp32 logits
   float *bias, *dbias, *dx, *dw;
   void* gemm;
@@ -640,7 +794,9 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     s.part = c.take<float2>(fmt == kElemF32 ? (size_t)N : (size_t)N * ((V + kMmTile - 1) / kMmTile));
   } else {
     s.rows = c.take<float4>(up_to(N, kMmTile));
-    s.scale = c.take<float>(2);
+    s.part_max = c.take<unsigned>(3 * kScaleBlocks);
+    s.exps = c.take<int>(3);
+    s.row_exp = c.take<int>(N);
   }
   if (fmt == kElemF32) {
     s.dl = c.take<char>((size_t)N * p.piece * 4);
@@ -651,6 +807,8 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
     s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
     if (backward) {
+      s.scaled_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
+      if (fmt == kElemBf16) s.scaled_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
       s.dl = c.take<char>((size_t)N * p.piece * 2);
       s.dbias = c.take<float>((size_t)p.tiles_n * p.piece);
       s.dx = c.take<float>((size_t)p.splits_x * N * D);
@@ -794,19 +952,14 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     HSL_HIP(hipGetLastError());
     return HSL_OK;
   }
-  const float* scale = nullptr;
-  if (fmt == kElemF16) {
-    hipLaunchKernelGGL(xent_scale_kernel, dim3(1), dim3(1024), 0, st, dloss, s.scale, n);
-    scale = s.scale;
-  }
   hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
                      tgt64, bias, s.target, s.bias, n, V);
-  hipLaunchKernelGGL(xent_rows_kernel, dim3((n + 255) / 256), dim3(256), 0, st,
-                     reinterpret_cast<const float2*>(stats), s.target, dloss, bias, scale, s.rows, n);
   HSL_HIP(hipGetLastError());
   if (fmt == kElemF32) {
     float* const l = reinterpret_cast<float*>(s.dl);
     const float *xf = static_cast<const float*>(x), *wf = static_cast<const float*>(w);
+    hipLaunchKernelGGL(xent_rows_kernel, dim3((n + 255) / 256), dim3(256), 0, st,
+                       reinterpret_cast<const float2*>(stats), s.target, dloss, bias, s.rows, n);
     for (int v0 = 0; v0 < V; v0 += p.piece) {
       const int v = std::min(p.piece, V - v0);
       HSL_CHECK(gemm_run(f32_product(xf, wf + v0 * ldw, bias ? bias + v0 : nullptr, l, n, v, D, (int)ldx, (int)ldw,
@@ -837,6 +990,43 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   HSL_CHECK(device_info(&info));
   XentOperands o;
   HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
+  ScaleArgs sc{};
+  sc.x = o.x;
+  sc.w = o.w;
+  sc.ldx = o.ldx;
+  sc.ldw = o.ldw;
+  sc.width = o.width;
+  sc.rx = split_rows(n, o.width / 8, kScaleBlocks);
+  if (fmt == kElemBf16) sc.rw = split_rows(V, o.width / 8, kScaleBlocks);
+  sc.blocks_g = std::min(kScaleBlocks, (n + 1023) / 1024);
+  sc.stats = reinterpret_cast<const float2*>(stats);
+  sc.target = s.target;
+  sc.dloss = dloss;
+  sc.bias = bias;
+  sc.part = s.part_max;
+  sc.exps = s.exps;
+  sc.hx = s.scaled_x;
+  sc.hw = s.scaled_w;
+  sc.rows = s.rows;
+  sc.row_exp = s.row_exp;
+  sc.N = n;
+  const int scaled = sc.rx.blocks + sc.rw.blocks;
+  const int rows_blocks = std::min(kScaleBlocks, (n + 255) / 256);
+  if (fmt == kElemF16) {
+    hipLaunchKernelGGL(xent_max_kernel<true>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
+    hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
+  } else {
+    hipLaunchKernelGGL(xent_max_kernel<false>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
+    hipLaunchKernelGGL(xent_scaled_kernel<false>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
+  }
+  HSL_HIP(hipGetLastError());
+  const unsigned short* const out_w = fmt == kElemBf16 ? s.scaled_w : o.w;
+  const long long out_ldw = fmt == kElemBf16 ? o.width : o.ldw;
+  auto sum_planes = [&](const float* planes, size_t plane, int splits, const int* row_exp, void* out, long long rows) {
+    const RowSplit r = split_rows(rows, D, 1 << 16);
+    hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>, dim3(r.blocks),
+                       dim3(256), 0, st, planes, plane, splits, s.exps, row_exp, out, r, D);
+  };
   for (int v0 = 0; v0 < V; v0 += p.piece) {
     const int v = std::min(p.piece, V - v0);
     const int tiles_v = (v + kMmTile - 1) / kMmTile;  // the last piece may have fewer
@@ -856,15 +1046,15 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.dbias = dbias ? s.dbias : nullptr;
     OutArgs g{};
     g.dl = a.dl;
-    g.w = a.w.p;
-    g.x = o.x;
+    g.w = out_w + v0 * out_ldw;
+    g.x = s.scaled_x;
     g.ld = (long long)tiles_v * kMmTile;
-    g.ldw = o.ldw;
-    g.ldx = o.ldx;
+    g.ldw = out_ldw;
+    g.ldx = o.width;
     g.dx = s.dx;
     g.dw = p.splits_w > 1 ? s.dw : nullptr;
     g.dw16 = static_cast<unsigned short*>(dw) + (size_t)v0 * D;
-    g.scale = scale;
+    g.exps = s.exps;
     g.N = n;
     g.V = v;
     g.D = D;
@@ -881,24 +1071,18 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
     if (fmt == kElemF16) {
       hipLaunchKernelGGL(xent_grad_kernel<true>, grid, block, 0, st, a);
-      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<true>, grid_out, block, 0, st, g);
+      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<kElemF16>, grid_out, block, 0, st, g);
     } else {
       hipLaunchKernelGGL(xent_grad_kernel<false>, grid, block, 0, st, a);
-      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<false>, grid_out, block, 0, st, g);
+      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<kElemBf16>, grid_out, block, 0, st, g);
     }
     if (dbias)
-      hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, scale, dbias + v0, v, g.ld,
+      hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, s.exps, dbias + v0, v, g.ld,
                          p.tiles_n);
-    if (dw && g.dw)
-      hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>,
-                         dim3(grid_of((size_t)v * D)), dim3(256), 0, st, s.dw, (size_t)g.ld * D, p.splits_w, scale,
-                         static_cast<void*>(g.dw16), (size_t)v * D);
+    if (dw && g.dw) sum_planes(s.dw, (size_t)g.ld * D, p.splits_w, nullptr, g.dw16, v);
     HSL_HIP(hipGetLastError());
   }
-  if (dx)
-    hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>,
-                       dim3(grid_of((size_t)n * D)), dim3(256), 0, st, s.dx, (size_t)n * D, p.splits_x, scale, dx,
-                       (size_t)n * D);
+  if (dx) sum_planes(s.dx, (size_t)n * D, p.splits_x, s.row_exp, dx, n);
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }

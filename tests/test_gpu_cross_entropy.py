@@ -3,11 +3,13 @@
 Tolerances.  A logit is a sum of D exact products (16-bit operands) or of D products, in fp32: off by at most
 (D + 4) 2^-24 of the sum of the products' sizes; `shift` is the largest of these of a row.  The loss is off
 by twice that and a few roundings of its parts.  A probability is off by the factor exp(2 shift + 2^-18), the
-last for exp's and the sum's own roundings.  16-bit operands: dl is rounded to the operands' type (half a
-step of itself; fp16 has it scaled, with 2^-38 of the largest |dloss| for its smallest step), then a
-product's sum of n terms is off by (n + 8) 2^-24 of their sizes, and the result is rounded once.  What is
-below the smallest normal number, 2^-126, may be 0: a probability, a gradient dl, or either of the later two
-of the three pieces that an fp32 product's operand is split into: 4 2^-126 of each dl.
+last for exp's and the sum's own roundings.  16-bit operands: dl is rounded to fp16 (2^-11 of itself), then a
+product's sum of n terms is off by (n + 8) 2^-24 of their sizes, and the result is rounded once.  fp16's last
+place is 2^-24, so that what is rounded there is off by 2^-25; the scales put 2^14 or more at each row's g, at
+the largest element of x times the largest g (an element of a row whose g is smaller has as much less), and at
+that of a bf16 w: 2^-39 of g for dl, 2^-39 max|x| max|g| / |g| for x, 2^-39 max|w| for w.  What is below the
+smallest normal number, 2^-126, may be 0: a probability, a gradient dl, or either of the later two of the three
+pieces that an fp32 product's operand is split into: 4 2^-126 of each dl.
 """
 
 import math
@@ -56,6 +58,24 @@ def within(name, got, want, bound):
     assert not bool(bad.any()), (name, int(bad.sum()), off[bad].max().item())
 
 
+def bounds(x, w, targets, dl, parts, shift, dloss):
+    """The error of dl in fp32, and those of dx and dw before they are rounded."""
+    (n, v), d = dl.shape, x.shape[1]
+    slack = (torch.expm1(2 * shift)[:, None] + 2 ** -18) * parts
+    x64, w64, g = x.detach().double().cpu().abs(), w.detach().double().cpu().abs(), dloss.detach().double().cpu().abs()
+    err, off_x, off_w = slack + 4 * 2.0 ** -126, torch.zeros(n, 1), 0.0
+    if x.dtype is not torch.float32 and n:
+        g = torch.where((targets.cpu() >= 0) & (targets.cpu() < v), g, torch.zeros_like(g))
+        err = err + 2.0 ** -11 * dl.abs() + 2.0 ** -39 * g[:, None]
+        off_x = 2.0 ** -39 * x64.max() * (g.max() / torch.where(g > 0, g, g.max().clamp_min(1e-300)))[:, None]
+        if x.dtype is torch.bfloat16:
+            off_w = 2.0 ** -39 * w64.max()
+    reach = parts + err  # what dl is at most
+    bound_x = err @ w64 + (reach * off_w).sum(1, keepdim=True) + (v + 8) * U * (reach @ w64)
+    bound_w = err.t() @ x64 + (reach * off_x).sum(0)[:, None] + (n + 8) * U * (reach.t() @ x64)
+    return slack, bound_x, bound_w
+
+
 def check(x, w, targets, bias, dloss):
     leaves = [t.detach().requires_grad_(True) for t in (x, w, bias) if t is not None]
     loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], targets, bias=leaves[2] if bias is not None else None)
@@ -69,15 +89,11 @@ def check(x, w, targets, bias, dloss):
     shift = (d + 4) * U * size
     finite = torch.where(torch.isfinite(want), want.abs(), torch.zeros_like(want))
     within("loss", loss, want, 2 * shift + 16 * U * (finite + size + math.log(v + 1)) + 2 ** -20)
-    step = torch.finfo(x.dtype).eps / 2 if x.dtype is not torch.float32 else 0.0
-    least = dloss.abs().max().item() * 2.0 ** -38 if x.dtype is torch.float16 and n else 4 * 2.0 ** -126
-    # of dl: the probability's error and its rounding
-    slack = (torch.expm1(2 * shift)[:, None] + 2 ** -18) * parts
-    err = slack + step * dl.abs() + least
+    slack, bound_x, bound_w = bounds(x, w, targets, dl, parts, shift, dloss)
     x64, w64 = x.detach().double().cpu(), w.detach().double().cpu()
     assert grads[0].dtype is x.dtype and grads[1].dtype is w.dtype
-    within("dx", grads[0], dl @ w64, err @ w64.abs() + (v + 8) * U * (parts @ w64.abs()))
-    within("dw", grads[1], dl.t() @ x64, err.t() @ x64.abs() + (n + 8) * U * (parts.t() @ x64.abs()))
+    within("dx", grads[0], dl @ w64, bound_x)
+    within("dw", grads[1], dl.t() @ x64, bound_w)
     if bias is not None:
         within("dbias", grads[2], dl.sum(0), slack.sum(0) + 40 * U * parts.sum(0))
     return loss, grads
@@ -179,6 +195,45 @@ def test_sizes_of_the_gradient(dev, scale):
     within("dbias", got[2], dl.sum(0), slack.sum(0) + 40 * U * parts.sum(0))
     if scale == 1e30:
         assert not bool(torch.isnan(got[0]).any())
+
+
+def test_gradients_of_unlike_rows(dev):
+    """Rows' gradients over 30 decades, each as precise as alone; whatever comes with a row that is not scored."""
+    x, w, t, b, dloss = inputs(dev, torch.bfloat16, 61, 400, 24, bias=True)
+    check(x, w, t, b, dloss * 10.0 ** torch.linspace(-15, 15, 61, device=dev))
+    t[7], t[40], t[41] = -1, -1, -5
+    want = check(x, w, t, b, dloss)[1]
+    for other in (1e30, float("inf"), float("nan"), 0.0):
+        dloss[[7, 40, 41]] = other
+        for g, k in zip(check(x, w, t, b, torch.where(t < 0, torch.zeros_like(dloss), dloss))[1], want):
+            assert torch.equal(g, k)
+        leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
+        loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+        for g, k in zip(torch.autograd.grad(loss, leaves, dloss), want):
+            assert torch.equal(g, k)
+
+
+def test_sizes_of_the_operands(dev):
+    """Operands near the ends of bf16's range, whose products fp16 could not hold."""
+    x, w, t, b, dloss = inputs(dev, torch.bfloat16, 40, 300, 24)
+    for up in (2.0 ** 60, 2.0 ** -60):
+        check(x * up, w / up, t, b, dloss)
+    check(x * 0, w, t, b, dloss)
+    check(x, w * 0, t, b, dloss)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 2, 200])
+def test_gradients_are_rounded_once(dev, dtype, n):
+    """As far from the exact ones as their rounding, not as two of them: the products' own error is at most
+    2^-11 of their terms' sizes, an eighth of bf16's half step."""
+    x, w, t, b, dloss = inputs(dev, dtype, n, 500, 32)
+    grads = check(x, w, t, b, dloss)[1]
+    _, dl, _, _ = reference(x, w, t, b, dloss)
+    for g, k in zip(grads, (dl @ w.double().cpu(), dl.t() @ x.double().cpu())):
+        once = (k.to(dtype).double() - k).norm()
+        own = 2.0 ** -11 * k.norm() * 2  # sums of terms of random signs are as large as their errors
+        assert (g.double().cpu() - k).norm() <= once + own
 
 
 @pytest.mark.parametrize("dtype", TYPES)
