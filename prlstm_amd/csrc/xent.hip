@@ -533,9 +533,12 @@ struct OutArgs {
   int tiles_n, tiles_d, tiles_v, splits_x, splits_w, k_x, k_w, add;
 };
 
-// One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.
+// One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.  A tile's
+// rows are the width's, so that a lane has 4 neighbouring elements of a result's row in registers and, from an
+// exchange between the half-waves, 8 of a 16-bit one.
 template <int F>
 __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
+  using T_ = typename Elem<F>::T;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   const int count_x = a.splits_x * a.tiles_n * a.tiles_d;
   const bool is_x = (int)blockIdx.x < count_x;
@@ -547,42 +550,86 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   const int dcols = a.Dk - td * kMmTile;
   if (is_x) {
     const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
-    const MmOperand A{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
-    const MmOperand B{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
-    MmPipe<true, false, true> mm;
+    const MmOperand A{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
+    const MmOperand B{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
+    MmPipe<true, true, false> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   } else {
     const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
-    const MmOperand A{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
-    const MmOperand B{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
+    const MmOperand A{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
+    const MmOperand B{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
     MmPipe<true, true, true> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   }
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-  const int r0 = tm * kMmTile + (wave >> 2) * 128 + 4 * half, c0 = td * kMmTile + (wave & 3) * 64 + (lane & 31);
+  const int d0 = td * kMmTile + (wave >> 2) * 128, r0 = tm * kMmTile + (wave & 3) * 64 + (lane & 31);
   const int rows = is_x ? a.N : a.V;
   const int back = a.exps[0] - kTopExp - a.exps[1];
   float* const plane = is_x ? a.dx + (size_t)split * a.N * a.D : a.dw ? a.dw + (size_t)split * a.ld * a.D : nullptr;
   const bool add = is_x && a.add;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = r0 + i * 32 + 8 * (r >> 2) + (r & 3);
+  for (int j = 0; j < 2; ++j) {
+    const int row = r0 + j * 32;
+    if (plane) {
       if (row >= rows) continue;
+      float* const to = plane + (size_t)row * a.D;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = c0 + j * 32;
-        if (c >= a.D) continue;
-        const size_t at = (size_t)row * a.D + c;
-        if (plane)
-          plane[at] = add ? plane[at] + acc[i][j][r] : acc[i][j][r];
-        else
-          a.dw16[at] = Elem<F>::down(__builtin_ldexpf(acc[i][j][r], back));
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = d0 + i * 32 + 8 * q + 4 * half;
+          float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          if (d + 4 <= a.D) {
+            Pack<kElemF32, 4> w;
+            if (add) {
+              w = load_pack<kElemF32, 4>(to + d);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] += w.v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.v[e] = v[e];
+            __builtin_memcpy(to + d, &w, sizeof(w));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d + e < a.D) to[d + e] = add ? to[d + e] + v[e] : v[e];
+          }
+        }
+    } else {
+      T_* const to = a.dw16 + (size_t)row * a.D;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          mm_u4 v;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float f[4] = {__builtin_ldexpf(acc[i][j][8 * k + 2 * e], back),
+                                __builtin_ldexpf(acc[i][j][8 * k + 2 * e + 1], back),
+                                __builtin_ldexpf(acc[i][j][8 * k + 4 + 2 * e], back),
+                                __builtin_ldexpf(acc[i][j][8 * k + 5 + 2 * e], back)};
+            unsigned short h[4];
+            unsigned lo, hi;
+            down_all<F, 4>(f, h);
+            __builtin_memcpy(&lo, h, 4);
+            __builtin_memcpy(&hi, h + 2, 4);
+            const auto x = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+            v[e] = x[0];
+            v[2 + e] = x[1];
+          }
+          const int d = d0 + i * 32 + 16 * k + 8 * half;
+          if (row < rows && d + 8 <= a.D) {
+            __builtin_memcpy(to + d, &v, 16);
+          } else if (row < rows) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (d + e < a.D) to[d + e] = (T_)(v[e / 2] >> (16 * (e % 2)));
+          }
+        }
     }
+  }
 }
 
 // Rows of `cols` of the sum of the planes, in their order, without their scales (row_exp: those of the rows).
