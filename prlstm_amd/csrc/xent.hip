@@ -16,6 +16,8 @@
 // is scaled to |g| = 2^14 .. 2^15, x to as large an element less what its row's g is below the largest one, a
 // bf16 w to as large an element; the results take them back.  What is then below fp16's 2^-24 counts as 0: a
 // probability below 2^-38, an element 2^-38 of its operand's largest.
+//   Up to 128 rows, which leave half of a tile empty, a bf16 dl is kept as two bf16 rows instead, its value and
+// the rest (2^-17 of it remain), whose products the sums join: no copy of w is made for few rows.
 // fp32 operands: pieces of the logits are products on the library's fp32 kernels, kept in fp32.
 #include <algorithm>
 
@@ -409,12 +411,28 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   }
 }
 
+// For a dl in two rows: x twice, and nothing is scaled.  A workgroup a row.
+__global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
+  const int n = blockIdx.x;
+  if (n < 2 * a.N) {
+    const unsigned short* const from = a.x + (n < a.N ? n : n - a.N) * a.ldx;
+    for (int c = threadIdx.x * 8; c < a.width; c += 2048)
+      *reinterpret_cast<mm_u4*>(a.hx + (size_t)n * a.width + c) = *reinterpret_cast<const mm_u4*>(from + c);
+  }
+  if (threadIdx.x) return;
+  if (n < 3) a.exps[n] = n == 0 ? kTopExp : 0;
+  a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+  if (n >= a.N) return;
+  a.rows[n] = row_of(a.stats[n], row_gradient(a.stats[n], a.target[n], a.dloss[n]), a.target[n], a.bias, 1.f);
+  a.row_exp[n] = kTopExp;
+}
+
 // The tile's dl goes from the registers to memory: an exchange between the half-waves gives every lane 8
 // neighbouring tokens of a position.  The 16 stores of a lane are always issued, whatever lies outside, so
 // that the next product's waits can leave them out.
-template <bool FP16>
+template <bool FP16, bool TWO>
 __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
-  constexpr int kStores = 16;
+  constexpr int kStores = TWO ? 32 : 16;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float sums[4][kMmTile];
@@ -465,24 +483,33 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          unsigned lo[2], hi[2];  // 4 tokens of groups 2 k and 2 k + 1
+          mm_u4 v, rest;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float f[4] = {acc[i][j][8 * k + 2 * e], acc[i][j][8 * k + 2 * e + 1], acc[i][j][8 * k + 4 + 2 * e],
-                                acc[i][j][8 * k + 5 + 2 * e]};
-            unsigned short h[4];
-            down_all<kElemF16, 4>(f, h);
-            __builtin_memcpy(&lo[e], h, 4);
-            __builtin_memcpy(&hi[e], h + 2, 4);
-          }
-          mm_u4 v;
+          for (int e = 0; e < 2; ++e) {  // 2 tokens of groups 2 k and 2 k + 1
+            float f[4] = {acc[i][j][8 * k + 2 * e], acc[i][j][8 * k + 2 * e + 1], acc[i][j][8 * k + 4 + 2 * e],
+                          acc[i][j][8 * k + 5 + 2 * e]};
+            auto put = [&](mm_u4& to) {
+              unsigned short h[4];
+              unsigned lo, hi;
+              down_all<TWO ? kElemBf16 : kElemF16, 4>(f, h);
+              __builtin_memcpy(&lo, h, 4);
+              __builtin_memcpy(&hi, h + 2, 4);
+              const auto x = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
+              to[e] = x[0];
+              to[2 + e] = x[1];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const auto x = __builtin_amdgcn_permlane32_swap(lo[e], hi[e], false, false);
-            v[e] = x[0];
-            v[2 + e] = x[1];
+              for (int c = 0; c < 4; ++c) {
+                const float top = Elem<kElemBf16>::up(h[c]);
+                f[c] = __builtin_fabsf(top) < __builtin_inff() ? f[c] - top : 0.f;
+              }
+            };
+            put(v);
+            if constexpr (TWO) put(rest);
           }
           __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)off + (i * 32 + 16 * k) * 2, 0, 0);
+          if constexpr (TWO)
+            __builtin_amdgcn_raw_buffer_store_b128(rest, out, (int)(off == kOffNone ? off : off + a.N * (unsigned)ld * 2) +
+                                                                 (i * 32 + 16 * k) * 2, 0, 0);
         }
       }
     }
@@ -524,7 +551,7 @@ __global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict_
 }
 
 struct OutArgs {
-  const unsigned short *dl, *w, *x;  // in fp16
+  const unsigned short *dl, *w, *x;  // of the product's type
   long long ld, ldw, ldx;   // of dl (the piece's padded width), w and x
   float *dx, *dw;           // planes [split][N][D] and [split][ld][D]; dw null: straight to dw16
   unsigned short* dw16;
@@ -536,7 +563,7 @@ struct OutArgs {
 // One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.  A tile's
 // rows are the width's, so that a lane has 4 neighbouring elements of a result's row in registers and, from an
 // exchange between the half-waves, 8 of a 16-bit one.
-template <int F>
+template <int F, bool FP16>
 __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   using T_ = typename Elem<F>::T;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
@@ -552,14 +579,14 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
     const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
     const MmOperand A{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
     const MmOperand B{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
-    MmPipe<true, true, false> mm;
+    MmPipe<FP16, true, false> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   } else {
     const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
     const MmOperand A{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
     const MmOperand B{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
-    MmPipe<true, true, true> mm;
+    MmPipe<FP16, true, true> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   }
@@ -647,6 +674,29 @@ __global__ __launch_bounds__(256) void xent_planes_kernel(const float* __restric
       static_cast<typename Elem<F>::T*>(out)[i] = Elem<F>::down(__builtin_ldexpf(v, back));
     }
   }
+}
+
+// The same of many planes of few rows, for which a thread an element is neither enough of them nor of the loads:
+// 4 strips of the planes, 8 loads at a time (104 planes of 7 rows of 576: 5 us, 59 as above).
+constexpr int kManyPlanes = 8;
+template <int F>
+__global__ __launch_bounds__(256) void xent_many_planes_kernel(const float* __restrict__ planes, size_t plane,
+                                                               int splits, const int* exps, const int* row_exp,
+                                                               void* out, int cols) {
+  __shared__ float sm[4][64];
+  const int c = threadIdx.x & 63, strip = threadIdx.x >> 6;
+  const size_t i = (size_t)blockIdx.x * 64 + c;
+  float v = 0.f;
+  if (i < plane) {
+#pragma unroll 8
+    for (int s = strip; s < splits; s += 4) v += planes[s * plane + i];
+  }
+  sm[strip][c] = v;
+  __syncthreads();
+  if (strip || i >= plane) return;
+  v = (sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]);
+  const int back = row_exp ? row_exp[i / cols] - kTopExp - exps[2] : exps[0] - kTopExp - exps[1];
+  static_cast<typename Elem<F>::T*>(out)[i] = Elem<F>::down(__builtin_ldexpf(v, back));
 }
 
 template <int F>
@@ -793,6 +843,8 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   return p;
 }
 
+bool in_two(int N, int fmt) { return fmt == kElemBf16 && N <= kMmTile / 2; }
+
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
   if (N < 0 || V < 0 || D < 0) return fail(HSL_ERR_ARG, "%s: negative size (N=%lld V=%d D=%d)", who, N, V, D);
@@ -832,7 +884,8 @@ constexpr size_t kGemmRoom = 64u << 20;
 
 XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   XentSpace s{};
-  const XentPlan p = plan_xent(N, V, D, fmt);
+  const bool two = backward && in_two(N, fmt);
+  const XentPlan p = plan_xent(two ? 2 * N : N, V, D, fmt);
   Carver c(base, 0);
   s.target = c.take<int>(up_to(N, kMmTile));
   s.bias = c.take<float>(up_to(V, kMmTile));
@@ -854,11 +907,12 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
     s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
     if (backward) {
-      s.scaled_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
-      if (fmt == kElemBf16) s.scaled_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
-      s.dl = c.take<char>((size_t)N * p.piece * 2);
+      const size_t rows = two ? 2 * N : N;
+      s.scaled_x = c.take<unsigned short>(rows * up_to(D, 8));
+      if (fmt == kElemBf16 && !two) s.scaled_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
+      s.dl = c.take<char>(rows * p.piece * 2);
       s.dbias = c.take<float>((size_t)p.tiles_n * p.piece);
-      s.dx = c.take<float>((size_t)p.splits_x * N * D);
+      s.dx = c.take<float>(p.splits_x * rows * D);
       if (p.splits_w > 1) s.dw = c.take<float>((size_t)p.splits_w * p.piece * D);
     }
   }
@@ -981,7 +1035,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   if (N > 0 && (!targets || !stats || !dloss || !x || !w))
     return fail(HSL_ERR_ARG, "hsl_xent_bwd: null pointer");
   if (N > 0) HSL_CHECK(check_rows("hsl_xent_bwd", ldx, ldw, D));
-  const XentPlan p = plan_xent(n, V, D, fmt);
+  const bool two = in_two(n, fmt);
+  const XentPlan p = plan_xent(two ? 2 * n : n, V, D, fmt);
   XentSpace s = xent_space(ws, n, V, D, fmt, true);
   if (N > 0 && (!ws || ws_bytes < s.bytes))
     return fail(HSL_ERR_ARG, "hsl_xent_bwd: workspace %zu bytes, need %zu", ws_bytes, s.bytes);
@@ -1059,7 +1114,9 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   sc.N = n;
   const int scaled = sc.rx.blocks + sc.rw.blocks;
   const int rows_blocks = std::min(kScaleBlocks, (n + 255) / 256);
-  if (fmt == kElemF16) {
+  if (two) {
+    hipLaunchKernelGGL(xent_twice_kernel, dim3(kMmTile), dim3(256), 0, st, sc);
+  } else if (fmt == kElemF16) {
     hipLaunchKernelGGL(xent_max_kernel<true>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
     hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
   } else {
@@ -1067,8 +1124,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     hipLaunchKernelGGL(xent_scaled_kernel<false>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
   }
   HSL_HIP(hipGetLastError());
-  const unsigned short* const out_w = fmt == kElemBf16 ? s.scaled_w : o.w;
-  const long long out_ldw = fmt == kElemBf16 ? o.width : o.ldw;
+  const unsigned short* const out_w = s.scaled_w ? s.scaled_w : o.w;
+  const long long out_ldw = s.scaled_w ? o.width : o.ldw;
   auto sum_planes = [&](const float* planes, size_t plane, int splits, const int* row_exp, void* out, long long rows) {
     const RowSplit r = split_rows(rows, D, 1 << 16);
     hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>, dim3(r.blocks),
@@ -1102,7 +1159,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.dw = p.splits_w > 1 ? s.dw : nullptr;
     g.dw16 = static_cast<unsigned short*>(dw) + (size_t)v0 * D;
     g.exps = s.exps;
-    g.N = n;
+    g.N = two ? 2 * n : n;
     g.V = v;
     g.D = D;
     g.Dk = o.width;
@@ -1116,20 +1173,31 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.add = v0 > 0;
     const dim3 grid(std::min(tiles_v * p.tiles_n, info.num_cus)), block(kMmThreads);
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
-    if (fmt == kElemF16) {
-      hipLaunchKernelGGL(xent_grad_kernel<true>, grid, block, 0, st, a);
-      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<kElemF16>, grid_out, block, 0, st, g);
-    } else {
-      hipLaunchKernelGGL(xent_grad_kernel<false>, grid, block, 0, st, a);
-      if (grid_out.x) hipLaunchKernelGGL(xent_out_kernel<kElemBf16>, grid_out, block, 0, st, g);
-    }
+    auto run = [&](auto F, auto FP16, auto TWO) {
+      hipLaunchKernelGGL((xent_grad_kernel<decltype(F)::value == kElemF16, decltype(TWO)::value>), grid, block, 0, st, a);
+      if (grid_out.x)
+        hipLaunchKernelGGL((xent_out_kernel<decltype(F)::value, decltype(FP16)::value>), grid_out, block, 0, st, g);
+    };
+    using Bf16 = std::integral_constant<int, kElemBf16>;
+    if (fmt == kElemF16)
+      run(std::integral_constant<int, kElemF16>{}, std::true_type{}, std::false_type{});
+    else if (two)
+      run(Bf16{}, std::false_type{}, std::true_type{});
+    else
+      run(Bf16{}, std::true_type{}, std::false_type{});
     if (dbias)
       hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, s.exps, dbias + v0, v, g.ld,
                          p.tiles_n);
     if (dw && g.dw) sum_planes(s.dw, (size_t)g.ld * D, p.splits_w, nullptr, g.dw16, v);
     HSL_HIP(hipGetLastError());
   }
-  if (dx) sum_planes(s.dx, (size_t)n * D, p.splits_x, s.row_exp, dx, n);
+  const int planes = two ? 2 * p.splits_x : p.splits_x;
+  if (dx && planes < kManyPlanes)
+    sum_planes(s.dx, (size_t)n * D, planes, s.row_exp, dx, n);
+  else if (dx)
+    hipLaunchKernelGGL(fmt == kElemF16 ? xent_many_planes_kernel<kElemF16> : xent_many_planes_kernel<kElemBf16>,
+                       dim3((unsigned)(((size_t)n * D + 63) / 64)), dim3(256), 0, st, s.dx, (size_t)n * D, planes,
+                       s.exps, s.row_exp, dx, D);
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }
