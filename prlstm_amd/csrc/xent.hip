@@ -52,10 +52,10 @@ struct LogitArgs {
   // Filled up to whole tiles:
   const float* bias;  // the piece's, zeros where there is none; -inf beyond the vocabulary
   const int* target;  // the positions' targets (of the whole vocabulary)
-  const float4* rows;  // backward: m, 1 / sum, g (scaled), g or 0 where the target is masked; zeros beyond N
+  const float4* rows;  // backward: as of row_of(); zeros beyond N
   int v_first;        // the piece's first token
   int V, N, D, tiles_v, tiles_n;
-  float2* part;     // forward: [tile_v][N]
+  float2* part;     // forward: [tile_v or workgroup][N]
   float* own;       // forward: [N], the target's logit
   unsigned short* dl;  // backward: [N][tiles_v * 256]
   float* dbias;        // backward: [tile_n][tiles_v * 256], or null
@@ -203,6 +203,77 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
   }
 }
 
+// The forward of few rows, which would leave a tile of 256 empty: 32 tokens times 32 columns a workgroup and step,
+// whose operands go from memory to the registers of the matrix instructions (the rows' from the caches), 64 of the
+// width at a time by each of 4 waves and the next ones already on their way.  The waves' sums meet in LDS, where each
+// takes the logits of a quarter of the registers.  Bound by reading w: 10 us at 8 rows and 32768 tokens of width 512
+// in bf16 (33 MB, 3.4 TB/s; 17 us in tiles).  Up to 16 rows: the call takes 69, 41 and 30 us there for 131072 tokens
+// of width 1024 and 512 and 68480 of 576, in tiles 63, 39 and 38; at 32 rows, whose reads cost as much as w's, 84,
+// 48 and 34.  (64 tokens a step halve those, but leave fewer workgroups: 67, 43 and 35 at 16.)
+constexpr int kFewRows = 16, kFewChunk = 64, kFewBlocks = 1024;
+template <bool FP16>
+__global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
+  __shared__ float sm[4][16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, half = lane >> 5;
+  const int groups = (a.V + 31) / 32, width = a.w.k;
+  const int target = n < a.N ? a.target[n] : -1;
+  const unsigned short* const xr = a.x.p + min(n, a.N - 1) * a.x.ld + 8 * half;
+  mm_u4 w0[4], w1[4], x0[4], x1[4];
+  auto load = [&](int group, int k, mm_u4(&w)[4], mm_u4(&x)[4]) {
+    const unsigned short* const wr = a.w.p + min(group * 32 + n, a.V - 1) * a.w.ld + 8 * half;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = k + 16 * i;
+      const bool in = at + 8 * half < width;
+      x[i] = in ? *reinterpret_cast<const mm_u4*>(xr + at) : mm_u4{};
+      w[i] = in ? *reinterpret_cast<const mm_u4*>(wr + at) : mm_u4{};
+    }
+  };
+  float m = neg_inf(), sum = 0.f;
+  load(blockIdx.x, wave * kFewChunk, w0, x0);
+  for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+    f16v acc{};
+    for (int k = wave * kFewChunk; k < width; k += 4 * kFewChunk) {
+      const bool last = k + 4 * kFewChunk >= width;
+      const int next = last ? group + (int)gridDim.x : group;
+      if (next < groups) load(next, last ? wave * kFewChunk : k + 4 * kFewChunk, w1, x1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc = mm_mfma<FP16>(w0[i], x0[i], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x0[i] = x1[i];
+        w0[i] = w1[i];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sm[wave][r][lane] = acc[r];
+    __syncthreads();
+    float l[4], big = m;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int reg = 4 * wave + r, v = group * 32 + 8 * wave + 4 * half + r;
+      l[r] = (sm[0][reg][lane] + sm[1][reg][lane]) + (sm[2][reg][lane] + sm[3][reg][lane]) + a.bias[v];
+      if (v == target) a.own[n] = l[r];
+      big = fmaxf(big, l[r]);
+    }
+    const float ref = big == neg_inf() ? 0.f : -big * kLog2e;
+    sum *= exp2_of(m, ref);  // (0 for the first m, -inf)
+    m = big;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum += exp2_of(l[r], ref);
+    __syncthreads();
+  }
+  join(m, sum, __shfl_xor(m, 32), __shfl_xor(sum, 32));
+  sm[wave][0][lane] = m;
+  sm[wave][1][lane] = sum;
+  __syncthreads();
+  if (wave || half || n >= a.N) return;
+#pragma unroll
+  for (int k = 1; k < 4; ++k) join(m, sum, sm[k][0][lane], sm[k][1][lane]);
+  a.part[(size_t)blockIdx.x * a.N + n] = float2{m, sum};
+}
+
 // Targets as 32-bit numbers (-1: not scored, -2: beyond the vocabulary), and the bias, up to whole tiles.
 __global__ __launch_bounds__(256) void xent_prepare_kernel(const void* targets, int tgt64, const float* bias,
                                                           int* target, float* bias_out, int N, int V) {
@@ -214,22 +285,26 @@ __global__ __launch_bounds__(256) void xent_prepare_kernel(const void* targets, 
   if (i < (V + kMmTile - 1) / kMmTile * kMmTile) bias_out[i] = i >= V ? neg_inf() : bias ? bias[i] : 0.f;
 }
 
-// The loss and the row's (m, sum exp(l - m)) from its tiles' parts: 32 positions by 8 strips of the tiles.
+// The loss and the row's (m, sum exp(l - m)) from its parts: 8 positions by 32 strips of them.
 __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ own,
                                                         const int* __restrict__ target, float* loss, float2* stats,
-                                                        unsigned* err, int N, int tiles) {
-  __shared__ float2 sm[8][32];
-  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+                                                        unsigned* err, int N, int parts) {
+  __shared__ float2 sm[4][8];
+  const int c = threadIdx.x & 7, strip = threadIdx.x >> 3, n = blockIdx.x * 8 + c;
   float m = neg_inf(), s = 0.f;
-  if (n < N)
-    for (int t = strip; t < tiles; t += 8) {
+  if (n < N) {
+#pragma unroll 4
+    for (int t = strip; t < parts; t += 32) {
       const float2 p = part[(size_t)t * N + n];
       join(m, s, p.x, p.y);
     }
-  sm[strip][c] = float2{m, s};
+  }
+#pragma unroll
+  for (int k = 8; k < 64; k *= 2) join(m, s, __shfl_xor(m, k), __shfl_xor(s, k));
+  if ((threadIdx.x & 63) < 8) sm[threadIdx.x >> 6][c] = float2{m, s};
   __syncthreads();
   if (strip || n >= N) return;
-  for (int k = 1; k < 8; ++k) join(m, s, sm[k][c].x, sm[k][c].y);
+  for (int k = 1; k < 4; ++k) join(m, s, sm[k][c].x, sm[k][c].y);
   stats[n] = float2{m, s};
   const bool masked = all_masked(m, s);
   const int t = target[n];
@@ -843,6 +918,7 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   return p;
 }
 
+int few_blocks(int V) { return std::min(kFewBlocks, (V + 31) / 32); }
 bool in_two(int N, int fmt) { return fmt == kElemBf16 && N <= kMmTile / 2; }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
@@ -891,7 +967,8 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   s.bias = c.take<float>(up_to(V, kMmTile));
   if (!backward) {
     s.own = c.take<float>(N);
-    s.part = c.take<float2>(fmt == kElemF32 ? (size_t)N : (size_t)N * ((V + kMmTile - 1) / kMmTile));
+    const int parts = fmt == kElemF32 ? 1 : N <= kFewRows ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
+    s.part = c.take<float2>((size_t)N * parts);
   } else {
     s.rows = c.take<float4>(up_to(N, kMmTile));
     s.part_max = c.take<unsigned>(3 * kScaleBlocks);
@@ -1014,13 +1091,22 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.tiles_n = (n + kMmTile - 1) / kMmTile;
     a.part = s.part;
     a.own = s.own;
-    const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
-    if (fmt == kElemF16)
-      hipLaunchKernelGGL(xent_stats_kernel<true>, grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL(xent_stats_kernel<false>, grid, block, 0, st, a);
+    if (n <= kFewRows) {
+      tiles = few_blocks(V);
+      const dim3 grid(tiles), block(256);
+      if (fmt == kElemF16)
+        hipLaunchKernelGGL(xent_few_kernel<true>, grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL(xent_few_kernel<false>, grid, block, 0, st, a);
+    } else {
+      const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
+      if (fmt == kElemF16)
+        hipLaunchKernelGGL(xent_stats_kernel<true>, grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL(xent_stats_kernel<false>, grid, block, 0, st, a);
+    }
   }
-  hipLaunchKernelGGL(xent_join_kernel, dim3((n + 31) / 32), dim3(256), 0, st, s.part, s.own, s.target, loss,
+  hipLaunchKernelGGL(xent_join_kernel, dim3((n + 7) / 8), dim3(256), 0, st, s.part, s.own, s.target, loss,
                      reinterpret_cast<float2*>(stats), err, n, tiles);
   HSL_HIP(hipGetLastError());
   return HSL_OK;
