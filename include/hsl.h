@@ -472,7 +472,8 @@ int hsl_selective_bwd(const void* x, long long x_t, long long x_b,
  * sum_v exp(l[n][v] - m)) with the largest logit m, for the backward.  A negative target gives loss
  * 0; one >= V NaN, and raises bit 1 of the device word.  A row of nothing but masks (-inf) has m = -inf and
  * loss inf.  N is less than 2^24, D 1 or more and less than 2^20, V 1 or more, and N and V have fewer than 2^22 tiles
- * of 256 x 256. */
+ * of 256 x 256.  16-bit rows of a D that is a multiple of 8 begin at multiples of 16 bytes, fewer than 2^21 elements
+ * apart. */
 size_t hsl_xent_ws_bytes(long long N, int V, int D, int fmt, int backward);
 int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias,
                  const void* targets, int tgt64, float* loss, float* stats,

@@ -13,12 +13,16 @@ from .selective import _needs_grad, _weight
 
 
 def _rows(t):
-    """(t with dense rows that do not overlap, the elements between them)."""
+    """(t with dense rows that do not overlap, the elements between them).  16-bit rows that the kernels could read
+    in place but for where they begin are copied."""
     t = _unit_inner(t)
     n, d = t.shape
-    if n > 1 and t.stride(0) < d:
-        t = t.contiguous()
-    return t, max(t.stride(0), d) if n > 1 else d
+    ld = t.stride(0) if n > 1 else d
+    if ld < d:
+        t, ld = t.contiguous(), d
+    if d % 8 == 0 and t.dtype is not torch.float32 and (ld % 8 or ld >= 1 << 21 or t.data_ptr() % 16):
+        t, ld = t.clone(memory_format=torch.contiguous_format), d
+    return t, ld
 
 
 def _xent_fwd(x, weight, bias, targets, fmt, ids64):

@@ -16,8 +16,11 @@
 // is scaled to |g| = 2^14 .. 2^15, x to as large an element less what its row's g is below the largest one, a
 // bf16 w to as large an element; the results take them back.  What is then below fp16's 2^-24 counts as 0: a
 // probability below 2^-38, an element 2^-38 of its operand's largest.
-//   Up to 128 rows, which leave half of a tile empty, a bf16 dl is kept as two bf16 rows instead, its value and
-// the rest (2^-17 of it remain), whose products the sums join: no copy of w is made for few rows.
+//   For few rows dl is kept as two rows, its value and the rest, whose products the sums join: a bf16 one in bf16
+// up to 128 rows (2^-17 of it remain), which leave half of a tile empty, so that no copy of w is made for them; an
+// fp16 one up to 512 (2^-22), whose error would otherwise be 1.4 times that of one rounding, and by chance more
+// where few rows' are added (0.00035 for 0.00021), at the cost of twice the products (8192 rows would take half as
+// long again).
 // fp32 operands: pieces of the logits are products on the library's fp32 kernels, kept in fp32.
 #include <algorithm>
 
@@ -355,7 +358,7 @@ struct ScaleArgs {
   unsigned short *hx, *hw;      // the scaled operands in fp16, dense
   float4* rows;
   int* row_exp;
-  int N;
+  int N, twice;                 // twice: hx has x again behind it
 };
 
 __device__ __forceinline__ unsigned block_max(unsigned m) {
@@ -462,6 +465,7 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
         down_all<kElemF16, 8>(f, h);
         __builtin_memcpy(&v[k], h, 16);
         *reinterpret_cast<mm_u4*>(out + row[k] * a.width + c * 8) = v[k];
+        if (is_x && a.twice) *reinterpret_cast<mm_u4*>(out + (row[k] + a.N) * a.width + c * 8) = v[k];
       }
     });
     return;
@@ -486,7 +490,7 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   }
 }
 
-// For a dl in two rows: x twice, and nothing is scaled.  A workgroup a row.
+// For a bf16 dl in two rows (N <= kMmTile / 2): x twice, and nothing is scaled.  A workgroup a row.
 __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
   const int n = blockIdx.x;
   if (n < 2 * a.N) {
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
 // that the next product's waits can leave them out.
 template <bool FP16, bool TWO>
 __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
-  constexpr int kStores = TWO ? 32 : 16;
+  constexpr int kStores = TWO ? 32 : 16, kDl = TWO && !FP16 ? kElemBf16 : kElemF16;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float sums[4][kMmTile];
@@ -566,7 +570,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
             auto put = [&](mm_u4& to) {
               unsigned short h[4];
               unsigned lo, hi;
-              down_all<TWO ? kElemBf16 : kElemF16, 4>(f, h);
+              down_all<kDl, 4>(f, h);
               __builtin_memcpy(&lo, h, 4);
               __builtin_memcpy(&hi, h + 2, 4);
               const auto x = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
@@ -574,7 +578,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
               to[2 + e] = x[1];
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                const float top = Elem<kElemBf16>::up(h[c]);
+                const float top = Elem<kDl>::up(h[c]);
                 f[c] = __builtin_fabsf(top) < __builtin_inff() ? f[c] - top : 0.f;
               }
             };
@@ -919,7 +923,7 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
 }
 
 int few_blocks(int V) { return std::min(kFewBlocks, (V + 31) / 32); }
-bool in_two(int N, int fmt) { return fmt == kElemBf16 && N <= kMmTile / 2; }
+bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kElemBf16 ? kMmTile / 2 : 512); }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
@@ -939,6 +943,16 @@ int check_xent(const char* who, long long N, int V, int D, int fmt) {
 int check_rows(const char* who, long long ldx, long long ldw, int D) {
   if (ldx < D || ldw < D || ldx >= (1ll << 31) || ldw >= (1ll << 31))
     return fail(HSL_ERR_ARG, "%s: row strides %lld and %lld, must be D=%d or more and below 2^31", who, ldx, ldw, D);
+  return HSL_OK;
+}
+
+int check_begin(const char* who, const void* x, long long ldx, const void* w, long long ldw, int D, int fmt) {
+  auto readable = [](const void* p, long long ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 21);
+  };
+  if (fmt != kElemF32 && D % 8 == 0 && (!readable(x, ldx) || !readable(w, ldw)))
+    return fail(HSL_ERR_ARG, "%s: rows of D=%d must begin at multiples of 16 bytes, fewer than 2^21 elements apart (row "
+                             "strides %lld and %lld)", who, D, ldx, ldw);
   return HSL_OK;
 }
 
@@ -981,8 +995,10 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     s.gemm_bytes = kGemmRoom;
     s.gemm = c.take<char>(kGemmRoom);
   } else {
-    s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
-    s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
+    if (D % 8) {
+      s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
+      s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
+    }
     if (backward) {
       const size_t rows = two ? 2 * N : N;
       s.scaled_x = c.take<unsigned short>(rows * up_to(D, 8));
@@ -997,35 +1013,29 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   return s;
 }
 
-// 16-bit operands as the tiles read them: rows of a multiple of 8 elements at 16-byte steps.
+// 16-bit operands as the tiles read them: rows of a multiple of 8 elements at 16-byte steps, copied where D is none.
 struct XentOperands {
   const unsigned short *x, *w;
   long long ldx, ldw;
   int width;
 };
-bool tiles_read(const void* p, long long ld, int D) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 21) && D % 8 == 0;
-}
-int xent_operands(const void* x, long long ldx, const void* w, long long ldw, const XentSpace& s, int N, int V, int D,
-                  hipStream_t st, XentOperands* o) {
-  o->width = up_to(D, 8);
+int xent_operands(const void* x, long long ldx, const void* w, long long ldw, const XentSpace& s, int N,
+                  int V, int D, hipStream_t st, XentOperands* o) {
   o->x = static_cast<const unsigned short*>(x);
   o->w = static_cast<const unsigned short*>(w);
   o->ldx = ldx;
   o->ldw = ldw;
-  if (!tiles_read(x, ldx, D)) {
+  o->width = up_to(D, 8);
+  if (D % 8) {
     hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)N * o->width)), dim3(256), 0, st, o->x, ldx, s.packed_x,
                        (long long)N, D, o->width);
-    o->x = s.packed_x;
-    o->ldx = o->width;
-  }
-  if (!tiles_read(w, ldw, D)) {
     hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)V * o->width)), dim3(256), 0, st, o->w, ldw, s.packed_w,
                        (long long)V, D, o->width);
+    HSL_HIP(hipGetLastError());
+    o->x = s.packed_x;
     o->w = s.packed_w;
-    o->ldw = o->width;
+    o->ldx = o->ldw = o->width;
   }
-  HSL_HIP(hipGetLastError());
   return HSL_OK;
 }
 
@@ -1057,6 +1067,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   XentSpace s = xent_space(ws, n, V, D, fmt, false);
   if (!ws || ws_bytes < s.bytes)
     return fail(HSL_ERR_ARG, "hsl_xent_fwd: workspace %zu bytes, need %zu", ws_bytes, s.bytes);
+  HSL_CHECK(check_begin("hsl_xent_fwd", x, ldx, w, ldw, D, fmt));
   hipStream_t st = static_cast<hipStream_t>(stream);
   unsigned* err = nullptr;
   HSL_CHECK(device_error_word(&err));
@@ -1126,6 +1137,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   XentSpace s = xent_space(ws, n, V, D, fmt, true);
   if (N > 0 && (!ws || ws_bytes < s.bytes))
     return fail(HSL_ERR_ARG, "hsl_xent_bwd: workspace %zu bytes, need %zu", ws_bytes, s.bytes);
+  if (N > 0) HSL_CHECK(check_begin("hsl_xent_bwd", x, ldx, w, ldw, D, fmt));
   if (N == 0) {  // no position: the weights' gradients are zeros
     if (!dw && !dbias) return HSL_OK;
     const size_t count = (size_t)V * D;
@@ -1200,7 +1212,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   sc.N = n;
   const int scaled = sc.rx.blocks + sc.rw.blocks;
   const int rows_blocks = std::min(kScaleBlocks, (n + 255) / 256);
-  if (two) {
+  sc.twice = two;
+  if (two && fmt == kElemBf16) {
     hipLaunchKernelGGL(xent_twice_kernel, dim3(kMmTile), dim3(256), 0, st, sc);
   } else if (fmt == kElemF16) {
     hipLaunchKernelGGL(xent_max_kernel<true>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
@@ -1230,7 +1243,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.N = n;
     a.D = D;
     a.tiles_v = tiles_v;
-    a.tiles_n = p.tiles_n;
+    a.tiles_n = (n + kMmTile - 1) / kMmTile;
     a.rows = s.rows;
     a.dl = reinterpret_cast<unsigned short*>(s.dl);
     a.dbias = dbias ? s.dbias : nullptr;
@@ -1257,7 +1270,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.k_x = p.k_x;
     g.k_w = p.k_w;
     g.add = v0 > 0;
-    const dim3 grid(std::min(tiles_v * p.tiles_n, info.num_cus)), block(kMmThreads);
+    const dim3 grid(std::min(tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
     auto run = [&](auto F, auto FP16, auto TWO) {
       hipLaunchKernelGGL((xent_grad_kernel<decltype(F)::value == kElemF16, decltype(TWO)::value>), grid, block, 0, st, a);
@@ -1265,15 +1278,18 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
         hipLaunchKernelGGL((xent_out_kernel<decltype(F)::value, decltype(FP16)::value>), grid_out, block, 0, st, g);
     };
     using Bf16 = std::integral_constant<int, kElemBf16>;
-    if (fmt == kElemF16)
-      run(std::integral_constant<int, kElemF16>{}, std::true_type{}, std::false_type{});
+    using F16 = std::integral_constant<int, kElemF16>;
+    if (fmt == kElemF16 && two)
+      run(F16{}, std::true_type{}, std::true_type{});
+    else if (fmt == kElemF16)
+      run(F16{}, std::true_type{}, std::false_type{});
     else if (two)
       run(Bf16{}, std::false_type{}, std::true_type{});
     else
       run(Bf16{}, std::true_type{}, std::false_type{});
     if (dbias)
       hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, s.exps, dbias + v0, v, g.ld,
-                         p.tiles_n);
+                         a.tiles_n);
     if (dw && g.dw) sum_planes(s.dw, (size_t)g.ld * D, p.splits_w, nullptr, g.dw16, v);
     HSL_HIP(hipGetLastError());
   }

@@ -34,6 +34,16 @@ def test_refusals(call):
     _refused(call(N=(1 << 31) - 1, V=1), 2, b"beyond one launch")
 
 
+def test_rows_that_cannot_be_read_in_place():
+    """Where D is a multiple of 8, 16-bit rows are read 16 bytes at a time; the pointers are not read before."""
+    lib, room = _lib.load(), 1 << 40
+    for x, ldx, w, ldw in ((2, 8, 16, 8), (16, 12, 16, 8), (16, 8, 16, 1 << 21), (16, 8, 24, 8)):
+        rest = (16, 16, 0, 16, 16)
+        _refused(lib.hsl_xent_fwd(x, ldx, w, ldw, *rest, 16, room, 4, 5, 8, 0, None), 1, b"multiples of 16 bytes")
+        _refused(lib.hsl_xent_bwd(x, ldx, w, ldw, *rest, 16, 16, 16, 16, room, 4, 5, 8, 1, None), 1,
+                 b"multiples of 16 bytes")
+
+
 @pytest.mark.parametrize("call", [_fwd, _bwd])
 def test_more_rows_than_a_launch_has(call):
     """A workgroup of 256 threads a row: 2^24 rows would be 2^32 threads, which wrap."""
