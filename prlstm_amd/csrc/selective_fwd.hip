@@ -5,19 +5,28 @@
 
 namespace hsl {
 
-// Segments: where the channels give fewer than 256 workgroups' worth of waves, the time is cut into
-// segments that run as workgroups of their own, after a pass that finds each segment's state from zero
-// and its sum of dt (the decay over it is exp(a times that)).
+// Segments: where the channels give too few workgroups, the time is cut into segments that run as workgroups of
+// their own, after a pass that finds each segment's state from zero and its sum of dt (the decay over it is exp(a
+// times that)).  us with / without, forward and backward, bf16, 16 states, T4096:
+//   128 workgroups 335, 813 / 491, 1239;  160: 375, 1121 / 520, 1247;  192: 491, 1461 / 520, 1252;
+//   256: 603, 1511 / 527, 1271;  384, one and a half for a CU: 740, 2228 / 1030, 2490.
+// Up to 8 states a workgroup has fewer than 8 waves, so more segments pay: T1024, 256 workgroups of 8 states 111, 240
+// / 127, 277, of 4 states 98, 242 / 119, 320 (512: 165, 433 / 137, 341).  Not many more, as each one adds up the maps
+// of those before it: 16 workgroups of 4 states in 32 segments 79, 161, in 128 103, 239.
 ScanPlan plan_scan(int T, int B, int D, int N) {
   ScanPlan p;
   p.tiles = (D + kChannels - 1) / kChannels;
-  const int chunk = scan_chunk(N), nchunks = (T + chunk - 1) / chunk;
-  const long long have = (long long)p.tiles * B;
+  const int chunk = scan_chunk(N), nchunks = (T + chunk - 1) / chunk, states = scan_states(N), waves = states / 2;
+  const long long have = std::max(1ll, (long long)p.tiles * B);
   p.nseg = 1;
   p.seg_steps = std::max(1, nchunks) * chunk;
-  if (have < 192 && nchunks >= 8) {
-    const int want = (int)std::min<long long>(nchunks / 4, (512 + have - 1) / std::max(1ll, have));
-    const int per = (nchunks + want - 1) / want;
+  long long want = 1;
+  if (have < 192) want = (512 + have - 1) / have;
+  if (states <= 8 && have <= 256) want = std::max(want, std::min(16ll, (4096 / waves + have - 1) / have));
+  if (states == 16 && have > 256 && have <= 384) want = 2;
+  if (want > 1 && nchunks >= 8) {
+    want = std::min<long long>(want, nchunks / 4);
+    const int per = (int)((nchunks + want - 1) / want);
     p.seg_steps = per * chunk;
     p.nseg = (nchunks + per - 1) / per;
   }
@@ -198,19 +207,20 @@ __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
   }
 }
 
-// f(integral_constant fmt, ScanShape): four states a wave where every CU gets two workgroups or more, whose
-// barriers then hide behind each other, and two a wave (so twice the waves) where it gets fewer.  us, bf16,
-// 16 states, four / two a wave: T4096 B16 D1024 (256 workgroups) 678 / 547; fp16 T16383 B1 D1024 in 512
-// segments' workgroups 117 / 147.  One state a wave (16 waves): 658 and 172.
+// f(integral_constant fmt, ScanShape).  16 states: four a wave where every CU gets two workgroups or more, whose
+// barriers then hide behind each other, and two a wave (so twice the waves) where it gets fewer; us, bf16, four / two
+// a wave: T4096 B16 D1024 (256 workgroups) 678 / 547, T1024 and 512 workgroups 191 / 250, fp16 T16383 B1 D1024 in 512
+// segments' workgroups 117 / 147; one state a wave (16 waves): 658 for the first.  32 states: four a wave, 343 / 360
+// at T1024 and 512 workgroups, 172 / 177 at 256.  8 states: two a wave, 125 with 196 for four and 107 for
+// one at 256 workgroups, 153 with 249 and 221 at 512.  4 states: one a wave, 119 with 171 for two and 971 for four.
 template <class Fn>
 int with_fwd_shape(int fmt, int N, long long workgroups, Fn f) {
   return with_fmt(fmt, [&](auto F) {
-    const bool many = workgroups >= 512;
     switch (scan_states(N)) {
-      case 4: return many ? f(F, ScanShape<1, 4>{}) : f(F, ScanShape<2, 2>{});
-      case 8: return many ? f(F, ScanShape<2, 4>{}) : f(F, ScanShape<4, 2>{});
-      case 16: return many ? f(F, ScanShape<4, 4>{}) : f(F, ScanShape<8, 2>{});
-      case 32: return many ? f(F, ScanShape<8, 4>{}) : f(F, ScanShape<16, 2>{});
+      case 4: return f(F, ScanShape<4, 1>{});
+      case 8: return f(F, ScanShape<4, 2>{});
+      case 16: return workgroups >= 512 ? f(F, ScanShape<4, 4>{}) : f(F, ScanShape<8, 2>{});
+      case 32: return f(F, ScanShape<8, 4>{});
       default: return f(F, ScanShape<16, 4>{});
     }
   });
