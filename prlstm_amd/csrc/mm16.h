@@ -18,6 +18,10 @@
 // Pieces beyond the operand's rows or k read as zeros (a buffer's bounds), nothing outside is touched.
 // Operands have 16-byte aligned rows.
 //
+// SPLIT: fp32 operands as three bf16 pieces each (x = x0 + x1 + x2, 8 bits a piece), in planes: the product is six
+// products of pieces, the smallest first, as one of six times the depth; what is left out, x1 w2, x2 w1 and x2 w2, is
+// below 2^-25 of |x| |w|.
+//
 // The copies are written in assembly because the compiler, which cannot tell the four slices apart, would
 // wait for all copies before each read.  So the waits for them are written too: a wave's copies, loads and
 // stores end in order, so a wait for all but the last n is right where at least n were issued behind
@@ -51,6 +55,7 @@ struct MmOperand {
   const unsigned short* p;
   long long ld;
   int rows, k;
+  long long plane = 0;  // elements between pieces
 };
 
 // For an operand of assembly that has to be in a scalar register.
@@ -65,9 +70,10 @@ struct MmLoad {
     ld = (unsigned)(o.ld * 2);
     row = (TRANS ? lane >> 5 : lane >> 2) * ld;
   }
-  // Copies the slice from k0 on to the operand's place in LDS.
-  __device__ __forceinline__ void copy(const MmOperand& o, int k0, unsigned lds, int wave) const {
-    const unsigned long long base = (unsigned long long)(o.p + (TRANS ? k0 * o.ld : (long long)k0));
+  // Copies piece `piece`'s slice from k0 on to the operand's place in LDS.
+  __device__ __forceinline__ void copy(const MmOperand& o, int piece, int k0, unsigned lds, int wave) const {
+    const unsigned long long base =
+        (unsigned long long)(o.p + piece * o.plane + (TRANS ? k0 * o.ld : (long long)k0));
     const unsigned lo = mm_uniform((unsigned)base), hi = mm_uniform((unsigned)(base >> 32));
     const mm_u4 rsrc = {lo, hi & 0xffffu, 0x7fffffffu, 0x00020000u};
     const unsigned step = mm_uniform(ld), to = mm_uniform(lds);
@@ -158,7 +164,7 @@ __device__ __forceinline__ f16v mm_mfma(mm_u4 a, mm_u4 b, f16v c) {
 // The products of a workgroup's tiles, one after the other: while a tile's last slices multiply, the next
 // one's first are copied, so that they have arrived when its product begins.  lds: kMmLds bytes that hold
 // nothing else from begin() on.
-template <bool FP16, bool TA, bool TB>
+template <bool FP16, bool TA, bool TB, bool SPLIT = false>
 struct MmPipe {
   MmOperand A, B;
   MmLoad<TA> la;
@@ -166,12 +172,19 @@ struct MmPipe {
   MmRead<TA, 4> ra;
   MmRead<TB, 2> rb;
   const char* lds;
-  int wave, stage, slices;  // stage: where the tile's first slice lies; slices: of a tile
+  int wave, stage, slices, per;  // stage: where the tile's first slice lies; slices: of a tile; per: of a pair of pieces
 
   __device__ __forceinline__ void copy(const MmOperand& a, const MmOperand& b, int slice, int at) const {
     const unsigned p = (unsigned)(unsigned long long)(const mm_lds_char*)lds + (at % kMmStages) * kMmStage;
-    la.copy(a, slice * kMmSlice, p, wave);
-    lb.copy(b, slice * kMmSlice, p + kMmOperand, wave);
+    int pa = 0, pb = 0;
+    if constexpr (SPLIT) {
+      const int pair = (slice >= per) + (slice >= 2 * per) + (slice >= 3 * per) + (slice >= 4 * per) + (slice >= 5 * per);
+      slice -= pair * per;
+      pa = 0x118 >> (2 * pair) & 3;  // 0 2 1 0 1 0
+      pb = 0x052 >> (2 * pair) & 3;  // 2 0 1 1 0 0
+    }
+    la.copy(a, pa, slice * kMmSlice, p, wave);
+    lb.copy(b, pb, slice * kMmSlice, p + kMmOperand, wave);
   }
   // Every tile has k up to K and the same strides as this first one.
   __device__ __forceinline__ void begin(const char* space, const MmOperand& a, const MmOperand& b, int K) {
@@ -180,7 +193,8 @@ struct MmPipe {
     B = b;
     lds = space;
     stage = 0;
-    slices = max(kMmStages, (K + kMmSlice - 1) / kMmSlice);  // slices beyond K are zeros
+    per = max(0, (K + kMmSlice - 1) / kMmSlice);
+    slices = max(kMmStages, SPLIT ? 6 * per : per);  // slices beyond K are zeros
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     la.init(A, lane);
     lb.init(B, lane);

@@ -3,12 +3,12 @@
 //   dl[n][v] = g[n] (exp(l[n][v]) / sum - [v = target[n]]),   g = dloss (0 for a target < 0),
 //   dx = dl w,   dw = dl^T x,   dbias = sum_n dl.
 //
-// 16-bit operands: one kernel multiplies 256 x 256 tiles (mm16.h) whose rows are tokens of the
+// One kernel multiplies 256 x 256 tiles (mm16.h) whose rows are tokens of the
 // vocabulary and whose columns are the positions, so that a lane has 64 logits of each of 2 positions in
 // registers.  The forward reduces them to the tile's largest logit and sum of exponentials, from which a
 // second kernel makes the loss; no logit leaves the registers.  The backward computes the logits again,
-// a piece of the vocabulary at a time, and writes the piece's dl in fp16, from which one launch makes the
-// piece's dw and adds to dx, both in fp32.
+// a piece of the vocabulary at a time, and writes the piece's dl, for 16-bit operands in fp16, from which one launch
+// makes the piece's dw and adds to dx, both in fp32.
 //   Rounding dl is the one error that a sum of two roundings' size in dx and dw would show, and fp16's is
 // 2^-11 where bf16's, 2^-8, is as large as that of the results themselves (with it bf16 gradients were 1.4
 // times as far from the exact ones as when rounded once, few rows' up to twice).  So bf16 operands enter
@@ -21,7 +21,8 @@
 // fp16 one up to 512 (2^-22), whose error would otherwise be 1.4 times that of one rounding, and by chance more
 // where few rows' are added (0.00035 for 0.00021), at the cost of twice the products (8192 rows would take half as
 // long again).
-// fp32 operands: pieces of the logits are products on the library's fp32 kernels, kept in fp32.
+// fp32 operands: the same in three bf16 pieces each (mm16.h), dl too; the weight's are made for a piece of the
+// vocabulary at a time.
 #include <algorithm>
 
 #include "mm16.h"
@@ -29,7 +30,7 @@
 namespace hsl {
 namespace {
 
-constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl (or fp32 logits)
+constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl
 constexpr int kPieceWidth = 1 << 21;        // tokens at most: 256 rows of dl lie within 2^31 bytes
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -60,7 +61,7 @@ struct LogitArgs {
   int V, N, D, tiles_v, tiles_n;
   float2* part;     // forward: [tile_v or workgroup][N]
   float* own;       // forward: [N], the target's logit
-  unsigned short* dl;  // backward: [N][tiles_v * 256]
+  unsigned short* dl;  // backward: [parts][N][tiles_v * 256]
   float* dbias;        // backward: [tile_n][tiles_v * 256], or null
 };
 
@@ -98,7 +99,7 @@ struct LogitWalk {
   }
   __device__ __forceinline__ MmOperand rows_of(const MmOperand& o, int tile) const {
     const int first = tile * kMmTile;
-    return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), there() ? o.k : 0};
+    return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), there() ? o.k : 0, o.plane};
   }
   __device__ __forceinline__ MmOperand w() const { return rows_of(a.w, there() ? tv : 0); }
   __device__ __forceinline__ MmOperand x() const { return rows_of(a.x, there() ? tn : 0); }
@@ -146,12 +147,12 @@ __device__ __forceinline__ void add_bias(const LogitPlace& q, const float* bias,
   }
 }
 
-template <bool FP16>
+template <int F>
 __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float2 sm[2][kMmTile];
-  MmPipe<FP16, false, false> mm;
+  MmPipe<F == kElemF16, false, false, F == kElemF32> mm;
   LogitWalk walk(a);
   walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   mm.begin(lds, walk.w(), walk.x(), a.D);
@@ -331,13 +332,6 @@ __device__ __forceinline__ float row_gradient(float2 stats, int target, float dl
 __device__ __forceinline__ float4 row_of(float2 s, float g, int t, const float* bias, float part) {
   return float4{s.x, g * (1.f / s.y), g, t >= 0 && bias && bias[t] == neg_inf() ? -part : part};
 }
-__global__ __launch_bounds__(256) void xent_rows_kernel(const float2* __restrict__ stats, const int* __restrict__ target,
-                                                        const float* __restrict__ dloss, const float* bias,
-                                                        float4* rows, int N) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n < N) rows[n] = row_of(stats[n], row_gradient(stats[n], target[n], dloss[n]), target[n], bias, 1.f);
-}
-
 // 16-bit operands' scales.  The rows of a matrix among the threads of `blocks` workgroups: 1 << lg of them a row.
 struct RowSplit {
   int lg, blocks;
@@ -490,33 +484,71 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   }
 }
 
-// For a bf16 dl in two rows (N <= kMmTile / 2): x twice, and nothing is scaled.  A workgroup a row.
-__global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
-  const int n = blockIdx.x;
-  if (n < 2 * a.N) {
-    const unsigned short* const from = a.x + (n < a.N ? n : n - a.N) * a.ldx;
-    for (int c = threadIdx.x * 8; c < a.width; c += 2048)
-      *reinterpret_cast<mm_u4*>(a.hx + (size_t)n * a.width + c) = *reinterpret_cast<const mm_u4*>(from + c);
-  }
-  if (threadIdx.x) return;
+// The rows where nothing is scaled.
+__global__ __launch_bounds__(256) void xent_rows_kernel(ScaleArgs a) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
   if (n < 3) a.exps[n] = n == 0 ? kTopExp : 0;
-  a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+  a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};  // up to whole tiles
   if (n >= a.N) return;
   a.rows[n] = row_of(a.stats[n], row_gradient(a.stats[n], a.target[n], a.dloss[n]), a.target[n], a.bias, 1.f);
   a.row_exp[n] = kTopExp;
 }
 
+// x twice, for a bf16 dl in two rows.  A workgroup a row.
+__global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
+  const int n = blockIdx.x;
+  const unsigned short* const from = a.x + (n < a.N ? n : n - a.N) * a.ldx;
+  for (int c = threadIdx.x * 8; c < a.width; c += 2048)
+    *reinterpret_cast<mm_u4*>(a.hx + (size_t)n * a.width + c) = *reinterpret_cast<const mm_u4*>(from + c);
+}
+
+// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.
+__global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld, unsigned short* dst,
+                                                         RowSplit r, int cols, int width) {
+  const size_t plane = (size_t)r.rows * width;
+  for_rows(r, width / 8, blockIdx.x, [&](const long long(&row)[4], int c) {
+    float f[4][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* const p = src + row[k] * ld + c * 8;
+      if (row[k] >= 0 && c * 8 + 8 <= cols) {
+        const Pack<kElemF32, 4> lo = load_pack<kElemF32, 4>(p), hi = load_pack<kElemF32, 4>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[k][e] = e < 4 ? lo.v[e] : hi.v[e - 4];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[k][e] = row[k] >= 0 && c * 8 + e < cols ? p[e] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (row[k] < 0) continue;
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        unsigned short h[8];
+        down_all<kElemBf16, 8>(f[k], h);
+        mm_u4 v;
+        __builtin_memcpy(&v, h, 16);
+        *reinterpret_cast<mm_u4*>(dst + q * plane + (size_t)row[k] * width + c * 8) = v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[k][e] -= Elem<kElemBf16>::up(h[e]);
+      }
+    }
+  });
+}
+
 // The tile's dl goes from the registers to memory: an exchange between the half-waves gives every lane 8
-// neighbouring tokens of a position.  The 16 stores of a lane are always issued, whatever lies outside, so
+// neighbouring tokens of a position.  A lane's stores, 16 a part, are always issued, whatever lies outside, so
 // that the next product's waits can leave them out.
-template <bool FP16, bool TWO>
+// PARTS: how many numbers of the product's type a dl is kept in.
+template <int F, int PARTS>
 __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
-  constexpr int kStores = TWO ? 32 : 16, kDl = TWO && !FP16 ? kElemBf16 : kElemF16;
+  constexpr int kStores = 16 * PARTS, kDl = PARTS > 1 && F != kElemF16 ? kElemBf16 : kElemF16;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float sums[4][kMmTile];
   const long long ld = (long long)a.tiles_v * kMmTile;
-  MmPipe<FP16, false, false> mm;
+  MmPipe<F == kElemF16, false, false, F == kElemF32> mm;
   LogitWalk walk(a);
   walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   mm.begin(lds, walk.w(), walk.x(), a.D);
@@ -528,8 +560,10 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     mm.template run<kStores>(acc, walk.w(), walk.x(), !first, [&] { walk.info(&info[par ^ 1], mm.wave); });
     const LogitPlace q(tv, tn);
     add_bias(q, info[par].bias, acc);
-    const auto out = __builtin_amdgcn_make_buffer_rsrc(a.dl + (long long)tn * kMmTile * ld + tv * kMmTile, (short)0,
-                                                       0x7fffffff, 0x00020000);
+    auto out_of = [&](int part) {
+      return __builtin_amdgcn_make_buffer_rsrc(a.dl + ((long long)part * a.N + tn * kMmTile) * ld + tv * kMmTile, (short)0,
+                                               0x7fffffff, 0x00020000);
+    };
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float4 row = info[par].rows[q.c + j * 32];
@@ -562,33 +596,31 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          mm_u4 v, rest;
+          mm_u4 v[PARTS];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {  // 2 tokens of groups 2 k and 2 k + 1
             float f[4] = {acc[i][j][8 * k + 2 * e], acc[i][j][8 * k + 2 * e + 1], acc[i][j][8 * k + 4 + 2 * e],
                           acc[i][j][8 * k + 5 + 2 * e]};
-            auto put = [&](mm_u4& to) {
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
               unsigned short h[4];
               unsigned lo, hi;
               down_all<kDl, 4>(f, h);
               __builtin_memcpy(&lo, h, 4);
               __builtin_memcpy(&hi, h + 2, 4);
               const auto x = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
-              to[e] = x[0];
-              to[2 + e] = x[1];
+              v[part][e] = x[0];
+              v[part][2 + e] = x[1];
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
                 const float top = Elem<kDl>::up(h[c]);
                 f[c] = __builtin_fabsf(top) < __builtin_inff() ? f[c] - top : 0.f;
               }
-            };
-            put(v);
-            if constexpr (TWO) put(rest);
+            }
           }
-          __builtin_amdgcn_raw_buffer_store_b128(v, out, (int)off + (i * 32 + 16 * k) * 2, 0, 0);
-          if constexpr (TWO)
-            __builtin_amdgcn_raw_buffer_store_b128(rest, out, (int)(off == kOffNone ? off : off + a.N * (unsigned)ld * 2) +
-                                                                 (i * 32 + 16 * k) * 2, 0, 0);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            __builtin_amdgcn_raw_buffer_store_b128(v[part], out_of(part), (int)off + (i * 32 + 16 * k) * 2, 0, 0);
         }
       }
     }
@@ -632,7 +664,8 @@ __global__ __launch_bounds__(256) void xent_bias_kernel(const float* __restrict_
 struct OutArgs {
   const unsigned short *dl, *w, *x;  // of the product's type
   long long ld, ldw, ldx;   // of dl (the piece's padded width), w and x
-  float *dx, *dw;           // planes [split][N][D] and [split][ld][D]; dw null: straight to dw16
+  long long plane_w;        // between w's pieces
+  float *dx, *dw;           // planes [split][N][D] and [split][ld][D] (one: dw itself); dw null: straight to dw16
   unsigned short* dw16;
   const int* exps;
   int N, V, D, Dk;          // V: the piece's tokens; Dk: the width that x and w have in memory
@@ -642,9 +675,9 @@ struct OutArgs {
 // One piece's share of dx = dl w (the first splits_x tiles_n tiles_d workgroups) and its dw = dl^T x.  A tile's
 // rows are the width's, so that a lane has 4 neighbouring elements of a result's row in registers and, from an
 // exchange between the half-waves, 8 of a 16-bit one.
-template <int F, bool FP16>
+template <int F, bool FP16>  // of the results, and whether the product's type is fp16
 __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
-  using T_ = typename Elem<F>::T;
+  constexpr bool kSplit = F == kElemF32;
   __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
   const int count_x = a.splits_x * a.tiles_n * a.tiles_d;
   const bool is_x = (int)blockIdx.x < count_x;
@@ -656,16 +689,17 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   const int dcols = a.Dk - td * kMmTile;
   if (is_x) {
     const int k0 = split * a.k_x, k1 = min((int)a.ld, k0 + a.k_x);
-    const MmOperand A{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0};
-    const MmOperand B{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0};
-    MmPipe<FP16, true, false> mm;
+    const MmOperand A{a.w + k0 * a.ldw + td * kMmTile, a.ldw, dcols, min(a.V, k1) - k0, a.plane_w};
+    const MmOperand B{a.dl + (long long)tm * kMmTile * a.ld + k0, a.ld, min(kMmTile, a.N - tm * kMmTile), k1 - k0,
+                      a.N * a.ld};
+    MmPipe<FP16, true, false, kSplit> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   } else {
     const int k0 = split * a.k_w, k1 = min(a.N, k0 + a.k_w);
-    const MmOperand A{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0};
-    const MmOperand B{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0};
-    MmPipe<FP16, true, true> mm;
+    const MmOperand A{a.x + k0 * a.ldx + td * kMmTile, a.ldx, dcols, k1 - k0, a.N * a.ldx};
+    const MmOperand B{a.dl + k0 * a.ld + tm * kMmTile, a.ld, kMmTile, k1 - k0, a.N * a.ld};
+    MmPipe<FP16, true, true, kSplit> mm;
     mm.begin(lds, A, B, k1 - k0);
     mm.template run<0>(acc, MmOperand{A.p, A.ld, 0, 0}, MmOperand{B.p, B.ld, 0, 0}, false, [] {});
   }
@@ -703,8 +737,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
               if (d + e < a.D) to[d + e] = add ? to[d + e] + v[e] : v[e];
           }
         }
-    } else {
-      T_* const to = a.dw16 + (size_t)row * a.D;
+    } else if constexpr (!kSplit) {
+      unsigned short* const to = a.dw16 + (size_t)row * a.D;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -731,7 +765,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
           } else if (row < rows) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (d + e < a.D) to[d + e] = (T_)(v[e / 2] >> (16 * (e % 2)));
+              if (d + e < a.D) to[d + e] = (unsigned short)(v[e / 2] >> (16 * (e % 2)));
           }
         }
     }
@@ -761,18 +795,18 @@ constexpr int kManyPlanes = 8;
 template <int F>
 __global__ __launch_bounds__(256) void xent_many_planes_kernel(const float* __restrict__ planes, size_t plane,
                                                                int splits, const int* exps, const int* row_exp,
-                                                               void* out, int cols) {
+                                                               void* out, size_t n, int cols) {
   __shared__ float sm[4][64];
   const int c = threadIdx.x & 63, strip = threadIdx.x >> 6;
   const size_t i = (size_t)blockIdx.x * 64 + c;
   float v = 0.f;
-  if (i < plane) {
+  if (i < n) {
 #pragma unroll 8
     for (int s = strip; s < splits; s += 4) v += planes[s * plane + i];
   }
   sm[strip][c] = v;
   __syncthreads();
-  if (strip || i >= plane) return;
+  if (strip || i >= n) return;
   v = (sm[0][c] + sm[1][c]) + (sm[2][c] + sm[3][c]);
   const int back = row_exp ? row_exp[i / cols] - kTopExp - exps[2] : exps[0] - kTopExp - exps[1];
   static_cast<typename Elem<F>::T*>(out)[i] = Elem<F>::down(__builtin_ldexpf(v, back));
@@ -796,87 +830,6 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const unsigned short* __
   }
 }
 
-// ---- fp32 operands ------------------------------------------------------------------------
-
-// Joins a piece of the logits [N][ld] with what the pieces before it gave, a workgroup a row.
-__global__ __launch_bounds__(256) void xent_f32_stats_kernel(const float* __restrict__ l, long long ld, int V, int v0,
-                                                             const int* __restrict__ target, float2* stats, float* own,
-                                                             int first) {
-  __shared__ float2 sm[4];
-  const int n = blockIdx.x;
-  const float* const row = l + n * ld;
-  float m = neg_inf(), s = 0.f;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float x = row[v];
-    const float big = fmaxf(m, x), r = big == neg_inf() ? 0.f : big;
-    s = s * __builtin_amdgcn_exp2f((m - r) * kLog2e) + exp_f(x - r);
-    m = big;
-  }
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) join(m, s, __shfl_xor(m, k), __shfl_xor(s, k));
-  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = float2{m, s};
-  __syncthreads();
-  if (threadIdx.x) return;
-  for (int k = 1; k < 4; ++k) join(m, s, sm[k].x, sm[k].y);
-  if (!first) {
-    const float2 p = stats[n];
-    float m0 = p.x, s0 = p.y;
-    join(m0, s0, m, s);
-    m = m0;
-    s = s0;
-  }
-  stats[n] = float2{m, s};
-  const int t = target[n] - v0;
-  if (t >= 0 && t < V) own[n] = row[t];
-}
-
-// dl of a piece in place of its logits.
-__global__ __launch_bounds__(256) void xent_f32_grad_kernel(float* __restrict__ l, long long ld, int V, int v0,
-                                                            const int* __restrict__ target,
-                                                            const float4* __restrict__ rows) {
-  const int n = blockIdx.x;
-  float* const p = l + n * ld;
-  const float4 row = rows[n];
-  const int own = target[n] - v0;
-  const float gi = row.y;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float x = p[v];
-    float d = exp_f(x - row.x) * gi;
-    if (v == own) d -= row.z;
-    p[v] = row.z == 0.f || x == neg_inf() ? 0.f : d;
-  }
-}
-
-// Sums of columns of [N][ld], in fp64: 32 columns a workgroup, 32 strips of the rows.
-__global__ __launch_bounds__(1024) void xent_f32_bias_kernel(const float* __restrict__ l, long long ld, float* dbias,
-                                                             int V, int N) {
-  __shared__ double sm[32][32];
-  const int c = threadIdx.x & 31, strip = threadIdx.x >> 5, v = blockIdx.x * 32 + c;
-  double s = 0.0;
-  if (v < V) {
-    int n = strip;
-    for (; n + 96 < N; n += 128) {
-      float x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = l[(n + 32 * k) * ld + v];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s += x[k];
-    }
-    for (; n < N; n += 32) s += l[n * ld + v];
-  }
-  sm[strip][c] = s;
-  __syncthreads();
-  if (strip || v >= V) return;
-  for (int k = 1; k < 32; ++k) s += sm[k][c];
-  dbias[v] = (float)s;
-}
-
-__global__ __launch_bounds__(256) void xent_f32_add_kernel(float* __restrict__ out, const float* __restrict__ v,
-                                                           size_t n) {
-  const size_t stride = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) out[i] += v[i];
-}
-
 // ---- host ---------------------------------------------------------------------------------
 
 int up_to(long long n, int unit) { return (int)((n + unit - 1) / unit * unit); }
@@ -898,9 +851,10 @@ struct XentPlan {
 };
 XentPlan plan_xent(int N, int V, int D, int fmt) {
   XentPlan p;
-  const size_t es = fmt == kElemF32 ? 4 : 2;
+  const bool split = fmt == kElemF32;
   const int all = up_to(V, kMmTile);
-  const long long room = std::min<long long>(kPieceWidth, kPieceBytes / es / std::max(1, N));
+  long long room = std::min<long long>(kPieceWidth, kPieceBytes / (split ? 6 : 2) / std::max(1, N));
+  if (split) room = std::min<long long>(room, kPieceBytes / 6 / up_to(D, 8));  // the weight's pieces are as large at most
   const long long fit = std::max<long long>(1, room / kMmTile) * kMmTile;
   p.piece = (int)std::min<long long>(all, fit);
   p.pieces = (all + p.piece - 1) / p.piece;
@@ -912,18 +866,23 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   // k of a workgroup such that the two products' work makes about 256 equal shares
   const double total = (double)p.tiles_d * ((double)p.tiles_n * p.piece + (double)p.tiles_v * N);
   const int share = std::max(512, (int)std::min(1e9, total / 256));
-  auto split = [&](int k, int* splits, int* each) {
+  auto share_out = [&](int k, int* splits, int* each) {
     *splits = std::max(1, (int)(((long long)k + share / 2) / share));
     *each = std::max(kMmSlice, up_to((k + *splits - 1) / *splits, kMmSlice));
     *splits = std::max(1, (k + *each - 1) / *each);
   };
-  split(p.piece, &p.splits_x, &p.k_x);
-  split(N, &p.splits_w, &p.k_w);
+  share_out(p.piece, &p.splits_x, &p.k_x);
+  share_out(N, &p.splits_w, &p.k_w);
   return p;
 }
 
 int few_blocks(int V) { return std::min(kFewBlocks, (V + 31) / 32); }
 bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kElemBf16 ? kMmTile / 2 : 512); }
+
+// The parts that the forward's statistics of a row are joined from.
+int forward_parts(int N, int V, int fmt) {
+  return fmt != kElemF32 && N <= kFewRows ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
+}
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
   if (!elem_fmt_ok(fmt)) return fail(HSL_ERR_ARG, "%s: format %d is not 0 (bf16), 1 (fp16) or 2 (fp32)", who, fmt);
@@ -964,85 +923,96 @@ struct XentSpace {
   float4* rows;
   unsigned* part_max;
   int *exps, *row_exp;
-  unsigned short *packed_x, *packed_w, *scaled_x, *scaled_w;
-  char* dl;  // 16-bit dl, or fp32 logits
+  unsigned short *own_x, *own_w;  // the operands as the tiles read them, where they are not that
+  unsigned short *scaled_x, *scaled_w, *dl;
   float *bias, *dbias, *dx, *dw;
-  void* gemm;
-  size_t gemm_bytes, bytes;
+  size_t bytes;
 };
-constexpr size_t kGemmRoom = 64u << 20;
 
 XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   XentSpace s{};
-  const bool two = backward && in_two(N, fmt);
+  const bool two = backward && in_two(N, fmt), split = fmt == kElemF32;
   const XentPlan p = plan_xent(two ? 2 * N : N, V, D, fmt);
+  const int width = up_to(D, 8);
   Carver c(base, 0);
   s.target = c.take<int>(up_to(N, kMmTile));
   s.bias = c.take<float>(up_to(V, kMmTile));
+  if (split) {
+    s.own_x = c.take<unsigned short>((size_t)3 * N * width);
+    s.own_w = c.take<unsigned short>((size_t)3 * std::min(V, p.piece) * width);
+  } else if (D % 8) {
+    s.own_x = c.take<unsigned short>((size_t)N * width);
+    s.own_w = c.take<unsigned short>((size_t)V * width);
+  }
   if (!backward) {
     s.own = c.take<float>(N);
-    const int parts = fmt == kElemF32 ? 1 : N <= kFewRows ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
-    s.part = c.take<float2>((size_t)N * parts);
-  } else {
-    s.rows = c.take<float4>(up_to(N, kMmTile));
-    s.part_max = c.take<unsigned>(3 * kScaleBlocks);
-    s.exps = c.take<int>(3);
-    s.row_exp = c.take<int>(N);
+    s.part = c.take<float2>((size_t)N * forward_parts(N, V, fmt));
+    s.bytes = c.off;
+    return s;
   }
-  if (fmt == kElemF32) {
-    s.dl = c.take<char>((size_t)N * p.piece * 4);
-    if (backward) s.dx = c.take<float>((size_t)N * D);
-    s.gemm_bytes = kGemmRoom;
-    s.gemm = c.take<char>(kGemmRoom);
-  } else {
-    if (D % 8) {
-      s.packed_x = c.take<unsigned short>((size_t)N * up_to(D, 8));
-      s.packed_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
-    }
-    if (backward) {
-      const size_t rows = two ? 2 * N : N;
-      s.scaled_x = c.take<unsigned short>(rows * up_to(D, 8));
-      if (fmt == kElemBf16 && !two) s.scaled_w = c.take<unsigned short>((size_t)V * up_to(D, 8));
-      s.dl = c.take<char>(rows * p.piece * 2);
-      s.dbias = c.take<float>((size_t)p.tiles_n * p.piece);
-      s.dx = c.take<float>(p.splits_x * rows * D);
-      if (p.splits_w > 1) s.dw = c.take<float>((size_t)p.splits_w * p.piece * D);
-    }
-  }
+  s.rows = c.take<float4>(up_to(N, kMmTile));
+  s.part_max = c.take<unsigned>(3 * kScaleBlocks);
+  s.exps = c.take<int>(3);
+  s.row_exp = c.take<int>(N);
+  const size_t rows = two ? 2 * N : N, parts = split ? 3 : 1;
+  if (!split) s.scaled_x = c.take<unsigned short>(rows * width);
+  if (fmt == kElemBf16 && !two) s.scaled_w = c.take<unsigned short>((size_t)V * width);
+  s.dl = c.take<unsigned short>(parts * rows * p.piece);
+  s.dbias = c.take<float>((size_t)p.tiles_n * p.piece);
+  if (!split || p.splits_x > 1) s.dx = c.take<float>(p.splits_x * rows * D);
+  if (p.splits_w > 1) s.dw = c.take<float>((size_t)p.splits_w * p.piece * D);
   s.bytes = c.off;
   return s;
 }
 
-// 16-bit operands as the tiles read them: rows of a multiple of 8 elements at 16-byte steps, copied where D is none.
+// Operands as the tiles read them: rows of a multiple of 8 elements at 16-byte steps, of fp32 ones the pieces.
 struct XentOperands {
+  const void *x0, *w0;
   const unsigned short *x, *w;
-  long long ldx, ldw;
-  int width;
-};
-int xent_operands(const void* x, long long ldx, const void* w, long long ldw, const XentSpace& s, int N,
-                  int V, int D, hipStream_t st, XentOperands* o) {
-  o->x = static_cast<const unsigned short*>(x);
-  o->w = static_cast<const unsigned short*>(w);
-  o->ldx = ldx;
-  o->ldw = ldw;
-  o->width = up_to(D, 8);
-  if (D % 8) {
-    hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)N * o->width)), dim3(256), 0, st, o->x, ldx, s.packed_x,
-                       (long long)N, D, o->width);
-    hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)V * o->width)), dim3(256), 0, st, o->w, ldw, s.packed_w,
-                       (long long)V, D, o->width);
-    HSL_HIP(hipGetLastError());
-    o->x = s.packed_x;
-    o->w = s.packed_w;
-    o->ldx = o->ldw = o->width;
-  }
-  return HSL_OK;
-}
+  long long ldx, ldw, ldw0;
+  int N, D, width, fmt;
+  unsigned short* own_w;
 
-GemmDesc f32_product(const float* A, const float* B, const float* bias, float* C, int M, int N, int K, int lda, int ldb,
-                     int ldc, int trans_a, int trans_b, int acc64) {
-  return GemmDesc{A, B, bias, C, M, N, K, lda, ldb, ldc, trans_a, trans_b, acc64};
-}
+  int init(const void* x_, long long ldx_, const void* w_, long long ldw_, const XentSpace& s, int N_, int V, int D_,
+           int fmt_, hipStream_t st) {
+    x0 = x_;
+    w0 = w_;
+    ldw0 = ldw_;
+    N = N_;
+    D = D_;
+    fmt = fmt_;
+    width = up_to(D, 8);
+    own_w = s.own_w;
+    x = static_cast<const unsigned short*>(x_);
+    w = static_cast<const unsigned short*>(w_);
+    ldx = ldx_;
+    ldw = ldw_;
+    if (s.own_x) x = s.own_x;
+    if (s.own_w) w = s.own_w;
+    if (s.own_x) ldx = ldw = width;
+    if (fmt == kElemF32) {
+      split(static_cast<const float*>(x0), ldx_, s.own_x, N, st);
+    } else if (D % 8) {
+      hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)N * width)), dim3(256), 0, st,
+                         static_cast<const unsigned short*>(x0), ldx_, s.own_x, (long long)N, D, width);
+      hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)V * width)), dim3(256), 0, st,
+                         static_cast<const unsigned short*>(w0), ldw_, s.own_w, (long long)V, D, width);
+    }
+    HSL_HIP(hipGetLastError());
+    return HSL_OK;
+  }
+  void split(const float* src, long long ld, unsigned short* dst, int rows, hipStream_t st) const {
+    const RowSplit r = split_rows(rows, width / 8, 1 << 16);
+    hipLaunchKernelGGL(xent_split_kernel, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width);
+  }
+  // The v tokens from v0 on.
+  MmOperand tokens(int v0, int v, hipStream_t st) const {
+    if (fmt != kElemF32) return {w + v0 * ldw, ldw, v, width};
+    split(static_cast<const float*>(w0) + v0 * ldw0, ldw0, own_w, v, st);
+    return {own_w, ldw, v, width, (long long)v * width};
+  }
+  MmOperand positions() const { return {x, ldx, N, width, (long long)N * width}; }
+};
 
 }  // namespace
 }  // namespace hsl
@@ -1075,50 +1045,38 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   HSL_CHECK(device_info(&info));
   hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
                      tgt64, bias, s.target, s.bias, n, V);
-  int tiles = 1;
-  if (fmt == kElemF32) {
-    const XentPlan p = plan_xent(n, V, D, fmt);
-    for (int v0 = 0; v0 < V; v0 += p.piece) {
-      const int v = std::min(p.piece, V - v0);
-      float* const l = reinterpret_cast<float*>(s.dl);
-      HSL_CHECK(gemm_run(f32_product(static_cast<const float*>(x), static_cast<const float*>(w) + v0 * ldw,
-                                     bias ? bias + v0 : nullptr, l, n, v, D, (int)ldx, (int)ldw, p.piece, 0, 1, 0),
-                         s.gemm, s.gemm_bytes, st));
-      hipLaunchKernelGGL(xent_f32_stats_kernel, dim3(n), dim3(256), 0, st, l, (long long)p.piece, v, v0, s.target,
-                         s.part, s.own, v0 == 0);
-    }
-  } else {
-    XentOperands o;
-    HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
-    LogitArgs a{};
-    a.w = {o.w, o.ldw, V, o.width};
-    a.x = {o.x, o.ldx, n, o.width};
-    a.bias = s.bias;
-    a.target = s.target;
-    a.V = V;
-    a.N = n;
-    a.D = D;
-    a.tiles_v = tiles = (V + kMmTile - 1) / kMmTile;
-    a.tiles_n = (n + kMmTile - 1) / kMmTile;
-    a.part = s.part;
-    a.own = s.own;
-    if (n <= kFewRows) {
-      tiles = few_blocks(V);
-      const dim3 grid(tiles), block(256);
-      if (fmt == kElemF16)
-        hipLaunchKernelGGL(xent_few_kernel<true>, grid, block, 0, st, a);
-      else
-        hipLaunchKernelGGL(xent_few_kernel<false>, grid, block, 0, st, a);
-    } else {
-      const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
-      if (fmt == kElemF16)
-        hipLaunchKernelGGL(xent_stats_kernel<true>, grid, block, 0, st, a);
-      else
-        hipLaunchKernelGGL(xent_stats_kernel<false>, grid, block, 0, st, a);
-    }
+  XentOperands o;
+  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, st));
+  LogitArgs a{};
+  a.x = o.positions();
+  a.target = s.target;
+  a.N = n;
+  a.D = D;
+  a.tiles_n = (n + kMmTile - 1) / kMmTile;
+  a.own = s.own;
+  const int piece = fmt == kElemF32 ? plan_xent(n, V, D, fmt).piece : V;
+  for (int v0 = 0; v0 < V; v0 += piece) {
+    const int v = std::min(piece, V - v0);
+    a.w = o.tokens(v0, v, st);
+    a.bias = s.bias + v0;
+    a.v_first = v0;
+    a.V = v;
+    a.tiles_v = (v + kMmTile - 1) / kMmTile;
+    a.part = s.part + (size_t)(v0 / kMmTile) * n;
+    const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
+    if (fmt == kElemF32)
+      hipLaunchKernelGGL(xent_stats_kernel<kElemF32>, grid, block, 0, st, a);
+    else if (n <= kFewRows && fmt == kElemF16)
+      hipLaunchKernelGGL(xent_few_kernel<true>, dim3(few_blocks(V)), dim3(256), 0, st, a);
+    else if (n <= kFewRows)
+      hipLaunchKernelGGL(xent_few_kernel<false>, dim3(few_blocks(V)), dim3(256), 0, st, a);
+    else if (fmt == kElemF16)
+      hipLaunchKernelGGL(xent_stats_kernel<kElemF16>, grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL(xent_stats_kernel<kElemBf16>, grid, block, 0, st, a);
   }
   hipLaunchKernelGGL(xent_join_kernel, dim3((n + 7) / 8), dim3(256), 0, st, s.part, s.own, s.target, loss,
-                     reinterpret_cast<float2*>(stats), err, n, tiles);
+                     reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, fmt));
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }
@@ -1155,41 +1113,11 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
                      tgt64, bias, s.target, s.bias, n, V);
   HSL_HIP(hipGetLastError());
-  if (fmt == kElemF32) {
-    float* const l = reinterpret_cast<float*>(s.dl);
-    const float *xf = static_cast<const float*>(x), *wf = static_cast<const float*>(w);
-    hipLaunchKernelGGL(xent_rows_kernel, dim3((n + 255) / 256), dim3(256), 0, st,
-                       reinterpret_cast<const float2*>(stats), s.target, dloss, bias, s.rows, n);
-    for (int v0 = 0; v0 < V; v0 += p.piece) {
-      const int v = std::min(p.piece, V - v0);
-      HSL_CHECK(gemm_run(f32_product(xf, wf + v0 * ldw, bias ? bias + v0 : nullptr, l, n, v, D, (int)ldx, (int)ldw,
-                                     p.piece, 0, 1, 0),
-                         s.gemm, s.gemm_bytes, st));
-      hipLaunchKernelGGL(xent_f32_grad_kernel, dim3(n), dim3(256), 0, st, l, (long long)p.piece, v, v0, s.target,
-                         s.rows);
-      if (dbias)
-        hipLaunchKernelGGL(xent_f32_bias_kernel, dim3((v + 31) / 32), dim3(1024), 0, st, l, (long long)p.piece,
-                           dbias + v0, v, n);
-      if (dx) {
-        float* const out = v0 ? s.dx : static_cast<float*>(dx);
-        HSL_CHECK(gemm_run(f32_product(l, wf + v0 * ldw, nullptr, out, n, D, v, p.piece, (int)ldw, D, 0, 0, 1),
-                           s.gemm, s.gemm_bytes, st));
-        if (v0)
-          hipLaunchKernelGGL(xent_f32_add_kernel, dim3(grid_of((size_t)n * D)), dim3(256), 0, st,
-                             static_cast<float*>(dx), s.dx, (size_t)n * D);
-      }
-      if (dw)
-        HSL_CHECK(gemm_run(f32_product(l, xf, nullptr, static_cast<float*>(dw) + (size_t)v0 * D, v, D, n, p.piece,
-                                       (int)ldx, D, 1, 0, 1),
-                           s.gemm, s.gemm_bytes, st));
-      HSL_HIP(hipGetLastError());
-    }
-    return HSL_OK;
-  }
   DeviceInfo info;
   HSL_CHECK(device_info(&info));
   XentOperands o;
-  HSL_CHECK(xent_operands(x, ldx, w, ldw, s, n, V, D, st, &o));
+  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, st));
+  const bool split = fmt == kElemF32;
   ScaleArgs sc{};
   sc.x = o.x;
   sc.w = o.w;
@@ -1210,32 +1138,42 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   sc.rows = s.rows;
   sc.row_exp = s.row_exp;
   sc.N = n;
-  const int scaled = sc.rx.blocks + sc.rw.blocks;
-  const int rows_blocks = std::min(kScaleBlocks, (n + 255) / 256);
   sc.twice = two;
-  if (two && fmt == kElemBf16) {
-    hipLaunchKernelGGL(xent_twice_kernel, dim3(kMmTile), dim3(256), 0, st, sc);
+  const int scaled = sc.rx.blocks + sc.rw.blocks, row_blocks = (n + 255) / 256;
+  if (split || (two && fmt == kElemBf16)) {
+    hipLaunchKernelGGL(xent_rows_kernel, dim3(row_blocks), dim3(256), 0, st, sc);
+    if (two) hipLaunchKernelGGL(xent_twice_kernel, dim3(2 * n), dim3(256), 0, st, sc);
   } else if (fmt == kElemF16) {
     hipLaunchKernelGGL(xent_max_kernel<true>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
-    hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
+    hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + std::min(kScaleBlocks, row_blocks)), dim3(256), 0, st, sc);
   } else {
     hipLaunchKernelGGL(xent_max_kernel<false>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
-    hipLaunchKernelGGL(xent_scaled_kernel<false>, dim3(scaled + rows_blocks), dim3(256), 0, st, sc);
+    hipLaunchKernelGGL(xent_scaled_kernel<false>, dim3(scaled + std::min(kScaleBlocks, row_blocks)), dim3(256), 0, st,
+                       sc);
   }
   HSL_HIP(hipGetLastError());
-  const unsigned short* const out_w = s.scaled_w ? s.scaled_w : o.w;
-  const long long out_ldw = s.scaled_w ? o.width : o.ldw;
-  auto sum_planes = [&](const float* planes, size_t plane, int splits, const int* row_exp, void* out, long long rows) {
-    const RowSplit r = split_rows(rows, D, 1 << 16);
-    hipLaunchKernelGGL(fmt == kElemF16 ? xent_planes_kernel<kElemF16> : xent_planes_kernel<kElemBf16>, dim3(r.blocks),
-                       dim3(256), 0, st, planes, plane, splits, s.exps, row_exp, out, r, D);
+  auto sum_planes = [&](const float* planes, size_t plane, int count, const int* row_exp, void* out, long long rows) {
+    HSL_CHECK(with_fmt(fmt, [&](auto F) {
+      constexpr int kF = decltype(F)::value;
+      const RowSplit r = split_rows(rows, D, 1 << 16);
+      if (count < kManyPlanes)
+        hipLaunchKernelGGL(xent_planes_kernel<kF>, dim3(r.blocks), dim3(256), 0, st, planes, plane, count, s.exps,
+                           row_exp, out, r, D);
+      else
+        hipLaunchKernelGGL(xent_many_planes_kernel<kF>, dim3((unsigned)(((size_t)rows * D + 63) / 64)), dim3(256), 0, st,
+                           planes, plane, count, s.exps, row_exp, out, (size_t)rows * D, D);
+      HSL_HIP(hipGetLastError());
+      return (int)HSL_OK;
+    }));
+    return (int)HSL_OK;
   };
+  float* const planes_x = s.dx ? s.dx : static_cast<float*>(dx);  // fp32: one plane is dx itself
   for (int v0 = 0; v0 < V; v0 += p.piece) {
     const int v = std::min(p.piece, V - v0);
     const int tiles_v = (v + kMmTile - 1) / kMmTile;  // the last piece may have fewer
     LogitArgs a{};
-    a.w = {o.w + v0 * o.ldw, o.ldw, v, o.width};
-    a.x = {o.x, o.ldx, n, o.width};
+    a.w = o.tokens(v0, v, st);
+    a.x = o.positions();
     a.bias = s.bias + v0;
     a.target = s.target;
     a.v_first = v0;
@@ -1245,17 +1183,18 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.tiles_v = tiles_v;
     a.tiles_n = (n + kMmTile - 1) / kMmTile;
     a.rows = s.rows;
-    a.dl = reinterpret_cast<unsigned short*>(s.dl);
+    a.dl = s.dl;
     a.dbias = dbias ? s.dbias : nullptr;
     OutArgs g{};
     g.dl = a.dl;
-    g.w = out_w + v0 * out_ldw;
-    g.x = s.scaled_x;
+    g.w = s.scaled_w ? s.scaled_w + (size_t)v0 * o.width : a.w.p;
+    g.x = split ? o.x : s.scaled_x;
     g.ld = (long long)tiles_v * kMmTile;
-    g.ldw = out_ldw;
+    g.ldw = s.scaled_w ? o.width : a.w.ld;
     g.ldx = o.width;
-    g.dx = s.dx;
-    g.dw = p.splits_w > 1 ? s.dw : nullptr;
+    g.plane_w = a.w.plane;
+    g.dx = planes_x;
+    g.dw = p.splits_w > 1 ? s.dw : split && dw ? static_cast<float*>(dw) + (size_t)v0 * D : nullptr;
     g.dw16 = static_cast<unsigned short*>(dw) + (size_t)v0 * D;
     g.exps = s.exps;
     g.N = two ? 2 * n : n;
@@ -1272,35 +1211,35 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.add = v0 > 0;
     const dim3 grid(std::min(tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
-    auto run = [&](auto F, auto FP16, auto TWO) {
-      hipLaunchKernelGGL((xent_grad_kernel<decltype(F)::value == kElemF16, decltype(TWO)::value>), grid, block, 0, st, a);
+    auto run = [&](auto F, auto PARTS, auto FP16) {
+      hipLaunchKernelGGL((xent_grad_kernel<decltype(F)::value, decltype(PARTS)::value>), grid, block, 0, st, a);
       if (grid_out.x)
         hipLaunchKernelGGL((xent_out_kernel<decltype(F)::value, decltype(FP16)::value>), grid_out, block, 0, st, g);
     };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
     using Bf16 = std::integral_constant<int, kElemBf16>;
     using F16 = std::integral_constant<int, kElemF16>;
-    if (fmt == kElemF16 && two)
-      run(F16{}, std::true_type{}, std::true_type{});
+    if (split)
+      run(std::integral_constant<int, kElemF32>{}, std::integral_constant<int, 3>{}, std::false_type{});
+    else if (fmt == kElemF16 && two)
+      run(F16{}, Two{}, std::true_type{});
     else if (fmt == kElemF16)
-      run(F16{}, std::true_type{}, std::false_type{});
+      run(F16{}, One{}, std::true_type{});
     else if (two)
-      run(Bf16{}, std::false_type{}, std::true_type{});
+      run(Bf16{}, Two{}, std::false_type{});
     else
-      run(Bf16{}, std::true_type{}, std::false_type{});
+      run(Bf16{}, One{}, std::true_type{});
     if (dbias)
       hipLaunchKernelGGL(xent_bias_kernel, dim3((v + 31) / 32), dim3(256), 0, st, s.dbias, s.exps, dbias + v0, v, g.ld,
                          a.tiles_n);
-    if (dw && g.dw) sum_planes(s.dw, (size_t)g.ld * D, p.splits_w, nullptr, g.dw16, v);
     HSL_HIP(hipGetLastError());
+    if (dw && p.splits_w > 1) {
+      void* const out = split ? static_cast<void*>(static_cast<float*>(dw) + (size_t)v0 * D) : g.dw16;
+      HSL_CHECK(sum_planes(s.dw, (size_t)g.ld * D, p.splits_w, nullptr, out, v));
+    }
   }
-  const int planes = two ? 2 * p.splits_x : p.splits_x;
-  if (dx && planes < kManyPlanes)
-    sum_planes(s.dx, (size_t)n * D, planes, s.row_exp, dx, n);
-  else if (dx)
-    hipLaunchKernelGGL(fmt == kElemF16 ? xent_many_planes_kernel<kElemF16> : xent_many_planes_kernel<kElemBf16>,
-                       dim3((unsigned)(((size_t)n * D + 63) / 64)), dim3(256), 0, st, s.dx, (size_t)n * D, planes,
-                       s.exps, s.row_exp, dx, D);
-  HSL_HIP(hipGetLastError());
+  if (dx && s.dx) HSL_CHECK(sum_planes(s.dx, (size_t)n * D, two ? 2 * p.splits_x : p.splits_x, s.row_exp, dx, n));
   return HSL_OK;
 }
 
