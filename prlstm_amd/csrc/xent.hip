@@ -863,9 +863,9 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   p.tiles_n = (N + kMmTile - 1) / kMmTile;
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.tiles_v = p.piece / kMmTile;
-  // k of a workgroup such that the two products' work makes about 256 equal shares
+  // k of a workgroup such that the two products' work makes about 256 equal shares (of fp32 operands, a k is six)
   const double total = (double)p.tiles_d * ((double)p.tiles_n * p.piece + (double)p.tiles_v * N);
-  const int share = std::max(512, (int)std::min(1e9, total / 256));
+  const int share = std::max(split ? 128 : 512, (int)std::min(1e9, total / 256));
   auto share_out = [&](int k, int* splits, int* each) {
     *splits = std::max(1, (int)(((long long)k + share / 2) / share));
     *each = std::max(kMmSlice, up_to((k + *splits - 1) / *splits, kMmSlice));
