@@ -38,16 +38,14 @@ __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 // A row of nothing but masks (m is -inf beside a sum of NaN where every logit is NaN).
 __device__ __forceinline__ bool all_masked(float m, float s) { return m == neg_inf() && s == 0.f; }
 
-// exp(l + ref / log2 e): the product and the difference are rounded once, which moves the result by
-// 2^-24 of l's and the reference's size, as much as their own roundings do.
-__device__ __forceinline__ float exp2_of(float l, float ref) {
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(l, kLog2e, ref));
-}
+// exp(l - m).  (A fused l log2 e - m log2 e would spare the difference, but is off by 2^-24 of l's and m's size rather
+// than of their difference's: 1e-6 of a probability at logits of 20.)
+__device__ __forceinline__ float exp_from(float l, float m) { return __builtin_amdgcn_exp2f((l - m) * kLog2e); }
 
 // Joins (m, sum exp(l - m)) of two parts of a row.
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
   const float big = fmaxf(m, m2), r = big == neg_inf() ? 0.f : big;
-  s = s * __builtin_amdgcn_exp2f((m - r) * kLog2e) + s2 * __builtin_amdgcn_exp2f((m2 - r) * kLog2e);
+  s = s * exp_from(m, r) + s2 * exp_from(m2, r);
   m = big;
 }
 
@@ -186,12 +184,12 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
         }
         if (found && n < a.N) a.own[n] = l;
       }
-      const float ref = m == neg_inf() ? 0.f : -m * kLog2e;
+      const float ref = m == neg_inf() ? 0.f : m;
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += exp2_of(acc[i][j][r], ref);
+        for (int r = 0; r < 16; ++r) s += exp_from(acc[i][j][r], ref);
         __builtin_amdgcn_sched_barrier(0);
       }
       join(m, s, __shfl_xor(m, 32), __shfl_xor(s, 32));
@@ -261,11 +259,11 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
       if (v == target) a.own[n] = l[r];
       big = fmaxf(big, l[r]);
     }
-    const float ref = big == neg_inf() ? 0.f : -big * kLog2e;
-    sum *= exp2_of(m, ref);  // (0 for the first m, -inf)
+    const float ref = big == neg_inf() ? 0.f : big;
+    sum *= exp_from(m, ref);  // (0 for the first m, -inf)
     m = big;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sum += exp2_of(l[r], ref);
+    for (int r = 0; r < 4; ++r) sum += exp_from(l[r], ref);
     __syncthreads();
   }
   join(m, sum, __shfl_xor(m, 32), __shfl_xor(sum, 32));
@@ -568,7 +566,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     for (int j = 0; j < 2; ++j) {
       const float4 row = info[par].rows[q.c + j * 32];
       const int own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
-      const float gi = row.y, ref = -row.x * kLog2e;
+      const float gi = row.y, ref = row.x;
       const float hot = __float_as_int(row.w) < 0 ? 0.f : row.z;
       const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
       // a masked logit has none whatever arrives, nor has a row without a gradient whatever it holds
@@ -582,11 +580,11 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
         __builtin_amdgcn_sched_barrier(0);  // 16 values at a time in registers beside the rest
         if (plain) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = exp2_of(acc[i][j][r], ref) * gi;
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = exp_from(acc[i][j][r], ref) * gi;
         } else {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float d = exp2_of(acc[i][j][r], ref) * gi;
+            const float d = exp_from(acc[i][j][r], ref) * gi;
             acc[i][j][r] = row.z == 0.f || acc[i][j][r] == neg_inf() ? 0.f : d;
           }
         }
