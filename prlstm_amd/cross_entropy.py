@@ -25,12 +25,13 @@ def _rows(t):
     return t, ld
 
 
-def _xent_fwd(x, weight, bias, targets, fmt, ids64):
+def _xent_fwd(x, weight, bias, targets, fmt, ids64, keep):
+    """(loss, the rows' statistics for the backward, or None)."""
     (x, ldx), (weight, ldw) = _rows(x), _rows(weight)
     n, d = x.shape
     v = weight.shape[0]
     f32 = dict(dtype=torch.float32, device=x.device)
-    loss, stats = torch.empty(n, **f32), torch.empty(n, 2, **f32)
+    loss, stats = torch.empty(n, **f32), torch.empty(n, 2, **f32) if keep else None
     nbytes = _size("hsl_xent_ws_bytes", n, v, d, fmt, 0)
     ws = _ws(nbytes, x)
     P = _lib.ptr
@@ -43,7 +44,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, targets, fmt, ids64):
         ctx.set_materialize_grads(False)
-        loss, stats = _xent_fwd(x, weight, bias, targets, fmt, ids64)
+        loss, stats = _xent_fwd(x, weight, bias, targets, fmt, ids64, True)
         ctx.save_for_backward(x, weight, bias, targets, stats)
         ctx.meta = (fmt, ids64)
         return loss
@@ -102,5 +103,5 @@ def linear_cross_entropy(x, weight, targets, bias=None):
     if _needs_grad(x, weight, bias):
         loss = LinearCrossEntropyFn.apply(flat, weight, bias, targets, fmt, ids64)
     else:
-        loss, _ = _xent_fwd(flat, weight, bias, targets, fmt, ids64)
+        loss, _ = _xent_fwd(flat, weight, bias, targets, fmt, ids64, False)
     return loss if len(lead) == 1 else loss.reshape(lead)

@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
   __syncthreads();
   if (strip || n >= N) return;
   for (int k = 1; k < 4; ++k) join(m, s, sm[k][c].x, sm[k][c].y);
-  stats[n] = float2{m, s};
+  if (stats) stats[n] = float2{m, s};
   const bool masked = all_masked(m, s);
   const int t = target[n];
   float v = 0.f;
@@ -877,9 +877,13 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
 int few_blocks(int V) { return std::min(kFewBlocks, (V + 31) / 32); }
 bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kElemBf16 ? kMmTile / 2 : 512); }
 
+// Whether xent_few_kernel runs.  Not where a backward follows: its logits, the tiles', are rounded in another order,
+// and a probability of them against the other ones' sum would be off by as much (dbias of 12 rows: 3.3e-7, 2.1e-7 from
+// the same ones).
+bool takes_few(int N, int fmt, bool alone) { return alone && fmt != kElemF32 && N <= kFewRows; }
 // The parts that the forward's statistics of a row are joined from.
-int forward_parts(int N, int V, int fmt) {
-  return fmt != kElemF32 && N <= kFewRows ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
+int forward_parts(int N, int V, int fmt, bool alone) {
+  return takes_few(N, fmt, alone) ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
 }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
@@ -944,7 +948,7 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   }
   if (!backward) {
     s.own = c.take<float>(N);
-    s.part = c.take<float2>((size_t)N * forward_parts(N, V, fmt));
+    s.part = c.take<float2>((size_t)N * std::max(forward_parts(N, V, fmt, true), forward_parts(N, V, fmt, false)));
     s.bytes = c.off;
     return s;
   }
@@ -1029,7 +1033,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
                  void* stream) {
   HSL_CHECK(check_xent("hsl_xent_fwd", N, V, D, fmt));
   if (N == 0) return HSL_OK;
-  if (!targets || !loss || !stats || !x || !w) return fail(HSL_ERR_ARG, "hsl_xent_fwd: null pointer");
+  if (!targets || !loss || !x || !w) return fail(HSL_ERR_ARG, "hsl_xent_fwd: null pointer");
   HSL_CHECK(check_rows("hsl_xent_fwd", ldx, ldw, D));
   const int n = (int)N;
   XentSpace s = xent_space(ws, n, V, D, fmt, false);
@@ -1052,6 +1056,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   a.D = D;
   a.tiles_n = (n + kMmTile - 1) / kMmTile;
   a.own = s.own;
+  const bool few = takes_few(n, fmt, !stats);
   const int piece = fmt == kElemF32 ? plan_xent(n, V, D, fmt).piece : V;
   for (int v0 = 0; v0 < V; v0 += piece) {
     const int v = std::min(piece, V - v0);
@@ -1064,9 +1069,9 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
     if (fmt == kElemF32)
       hipLaunchKernelGGL(xent_stats_kernel<kElemF32>, grid, block, 0, st, a);
-    else if (n <= kFewRows && fmt == kElemF16)
+    else if (few && fmt == kElemF16)
       hipLaunchKernelGGL(xent_few_kernel<true>, dim3(few_blocks(V)), dim3(256), 0, st, a);
-    else if (n <= kFewRows)
+    else if (few)
       hipLaunchKernelGGL(xent_few_kernel<false>, dim3(few_blocks(V)), dim3(256), 0, st, a);
     else if (fmt == kElemF16)
       hipLaunchKernelGGL(xent_stats_kernel<kElemF16>, grid, block, 0, st, a);
@@ -1074,7 +1079,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
       hipLaunchKernelGGL(xent_stats_kernel<kElemBf16>, grid, block, 0, st, a);
   }
   hipLaunchKernelGGL(xent_join_kernel, dim3((n + 7) / 8), dim3(256), 0, st, s.part, s.own, s.target, loss,
-                     reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, fmt));
+                     reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, fmt, !stats));
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }
