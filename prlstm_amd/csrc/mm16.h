@@ -18,9 +18,11 @@
 // Pieces beyond the operand's rows or k read as zeros (a buffer's bounds), nothing outside is touched.
 // Operands have 16-byte aligned rows.
 //
+// AF = 2 in place of 4: a tile of 128 rows, for products that have too few tiles of 256 for the chip's CUs.
+//
 // SPLIT: fp32 operands as three bf16 pieces each (x = x0 + x1 + x2, 8 bits a piece), in planes: the product is six
-// products of pieces, the smallest first, as one of six times the depth; what is left out, x1 w2, x2 w1 and x2 w2, is
-// below 2^-25 of |x| |w|.
+// products of pieces, the smallest first, of each slice in turn (so that a piece's slice, which three of them take, comes
+// from the caches); what is left out, x1 w2, x2 w1 and x2 w2, is below 2^-25 of |x| |w|.
 //
 // The copies are written in assembly because the compiler, which cannot tell the four slices apart, would
 // wait for all copies before each read.  So the waits for them are written too: a wave's copies, loads and
@@ -33,11 +35,13 @@
 namespace hsl {
 
 constexpr int kMmTile = 256, kMmSlice = 32, kMmThreads = 512, kMmStages = 4;
-constexpr int kMmOperand = kMmTile * kMmSlice * 2;  // bytes of one operand's slice
-constexpr int kMmStage = 2 * kMmOperand;
-constexpr int kMmLds = kMmStages * kMmStage;
-constexpr int kMmCopies = kMmOperand / 1024 / (kMmThreads / 64);  // instructions of a wave for an operand's slice
-static_assert(kMmCopies == 2, "the counts in MmTile's waits");
+constexpr int kMmFrag = 64 * kMmSlice * 2;        // bytes of a slice's 64 rows: 32 of each of A's two rows of waves
+constexpr int kMmOperand = 4 * kMmFrag;           // of one operand's slice
+constexpr int mm_lds(int af) { return kMmStages * (af * kMmFrag + kMmOperand); }
+constexpr int kMmLds = mm_lds(4);
+// Instructions of a wave for the slice of an operand of n fragments.
+constexpr int mm_copies(int n) { return n * kMmFrag / 1024 / (kMmThreads / 64); }
+static_assert(mm_copies(4) == 2 && mm_copies(2) == 1, "whole instructions");
 
 typedef __bf16 mm_bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 mm_h8 __attribute__((ext_vector_type(8)));
@@ -47,7 +51,9 @@ typedef __attribute__((address_space(3))) char mm_lds_char;
 
 // acc[i][j]: rows 32 i, columns 32 j of the wave's block (rows from 128 (wave / 4), columns from
 // 64 (wave % 4)): lane l, register r is row 8 (r / 4) + 4 (l / 32) + r % 4, column l % 32.
-typedef float MmAcc[4][2][16];
+template <int AF>
+using MmAccOf = float[AF][2][16];
+typedef MmAccOf<4> MmAcc;
 
 // An operand from its tile's first row and first k on: `rows` of its tile's 256 exist, and k of them.
 // ld (elements) is between rows in memory, or between k where TRANS.
@@ -61,7 +67,7 @@ struct MmOperand {
 // For an operand of assembly that has to be in a scalar register.
 __device__ __forceinline__ unsigned mm_uniform(unsigned v) { return (unsigned)__builtin_amdgcn_readfirstlane((int)v); }
 
-template <bool TRANS>
+template <bool TRANS, int N>  // N fragments
 struct MmLoad {
   unsigned row, ld;  // bytes: of the lane's row (TRANS: k) among a copy's 16 (2), between rows
   int lane;
@@ -79,8 +85,8 @@ struct MmLoad {
     const unsigned step = mm_uniform(ld), to = mm_uniform(lds);
     const int left = o.k - k0;
 #pragma unroll
-    for (int j = 0; j < kMmCopies; ++j) {
-      const int n = wave * kMmCopies + j;  // of the operand's 16 copies
+    for (int j = 0; j < mm_copies(N); ++j) {
+      const int n = wave * mm_copies(N) + j;  // of the operand's 4 N copies
       int c, first;
       bool in;
       if constexpr (TRANS) {
@@ -164,27 +170,29 @@ __device__ __forceinline__ f16v mm_mfma(mm_u4 a, mm_u4 b, f16v c) {
 // The products of a workgroup's tiles, one after the other: while a tile's last slices multiply, the next
 // one's first are copied, so that they have arrived when its product begins.  lds: kMmLds bytes that hold
 // nothing else from begin() on.
-template <bool FP16, bool TA, bool TB, bool SPLIT = false>
+template <bool FP16, bool TA, bool TB, bool SPLIT = false, int AF = 4>
 struct MmPipe {
+  static_assert(AF == 4 || (AF == 2 && !TA), "a transposed slice has 256 rows");
+  static constexpr int kA = AF * kMmFrag, kStage = kA + kMmOperand, kCopies = mm_copies(AF) + mm_copies(4);
   MmOperand A, B;
-  MmLoad<TA> la;
-  MmLoad<TB> lb;
-  MmRead<TA, 4> ra;
+  MmLoad<TA, AF> la;
+  MmLoad<TB, 4> lb;
+  MmRead<TA, AF> ra;
   MmRead<TB, 2> rb;
   const char* lds;
-  int wave, stage, slices, per;  // stage: where the tile's first slice lies; slices: of a tile; per: of a pair of pieces
+  int wave, stage, slices;  // stage: where the tile's first slice lies; slices: of a tile
 
   __device__ __forceinline__ void copy(const MmOperand& a, const MmOperand& b, int slice, int at) const {
-    const unsigned p = (unsigned)(unsigned long long)(const mm_lds_char*)lds + (at % kMmStages) * kMmStage;
+    const unsigned p = (unsigned)(unsigned long long)(const mm_lds_char*)lds + (at % kMmStages) * kStage;
     int pa = 0, pb = 0;
     if constexpr (SPLIT) {
-      const int pair = (slice >= per) + (slice >= 2 * per) + (slice >= 3 * per) + (slice >= 4 * per) + (slice >= 5 * per);
-      slice -= pair * per;
+      const int pair = (unsigned)slice % 6;
+      slice = (unsigned)slice / 6;
       pa = 0x118 >> (2 * pair) & 3;  // 0 2 1 0 1 0
       pb = 0x052 >> (2 * pair) & 3;  // 2 0 1 1 0 0
     }
     la.copy(a, pa, slice * kMmSlice, p, wave);
-    lb.copy(b, pb, slice * kMmSlice, p + kMmOperand, wave);
+    lb.copy(b, pb, slice * kMmSlice, p + kA, wave);
   }
   // Every tile has k up to K and the same strides as this first one.
   __device__ __forceinline__ void begin(const char* space, const MmOperand& a, const MmOperand& b, int K) {
@@ -193,34 +201,33 @@ struct MmPipe {
     B = b;
     lds = space;
     stage = 0;
-    per = max(0, (K + kMmSlice - 1) / kMmSlice);
-    slices = max(kMmStages, SPLIT ? 6 * per : per);  // slices beyond K are zeros
+    slices = max(kMmStages, (SPLIT ? 6 : 1) * ((K + kMmSlice - 1) / kMmSlice));  // slices beyond K are zeros
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     la.init(A, lane);
     lb.init(B, lane);
-    ra.init((wave >> 2) * 128, lane);
+    ra.init((wave >> 2) * 32 * AF, lane);
     rb.init((wave & 3) * 64, lane);
 #pragma unroll
     for (int s = 0; s < kMmStages; ++s) copy(A, B, s, s);
-    asm volatile("s_waitcnt vmcnt(12)\n\ts_barrier" ::: "memory");  // 3 slices of 4 copies may be on their way
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(3 * kCopies) : "memory");  // 3 slices may be on their way
   }
   // acc = this tile's product; nextA, nextB: the next tile, or operands without k.  with_next() is called
   // before the first copy for it.  LATER (a count): loads and stores that the wave has issued for sure since the
   // product before, which the waits for the copies before them leave out; later: whether there was one.
   template <int LATER, class Fn>
-  __device__ __forceinline__ void run(MmAcc& acc, const MmOperand& nextA, const MmOperand& nextB, bool later,
+  __device__ __forceinline__ void run(MmAccOf<AF>& acc, const MmOperand& nextA, const MmOperand& nextB, bool later,
                                       Fn with_next) {
-    f16v sum[4][2];
+    f16v sum[AF][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AF; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) sum[i][j] = f16v{};
-    auto place = [&](int slice) { return lds + ((stage + slice) % kMmStages) * kMmStage; };
-    mm_u4 a0[4], b0[2], a1[4], b1[2];
+    auto place = [&](int slice) { return lds + ((stage + slice) % kMmStages) * kStage; };
+    mm_u4 a0[AF], b0[2], a1[AF], b1[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a0[i] = ra.read(place(0), 0, i);
+    for (int i = 0; i < AF; ++i) a0[i] = ra.read(place(0), 0, i);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) b0[j] = rb.read(place(0) + kMmOperand, 0, j);
+    for (int j = 0; j < 2; ++j) b0[j] = rb.read(place(0) + kA, 0, j);
     // The order is fixed: between two products there is always something to issue, and there is a product
     // to run while the wave is at the barrier.
     auto fixed = [] { __builtin_amdgcn_sched_barrier(0); };
@@ -233,47 +240,45 @@ struct MmPipe {
       const char* const now = place(it);
       const char* const next = place(it + 1);
       product(a0[0], b0, 0);
-      b1[0] = rb.read(now + kMmOperand, 1, 0);
-      b1[1] = rb.read(now + kMmOperand, 1, 1);
+      b1[0] = rb.read(now + kA, 1, 0);
+      b1[1] = rb.read(now + kA, 1, 1);
       a1[0] = ra.read(now, 1, 0);
       fixed();
       product(a0[1], b0, 1);
-      a1[1] = ra.read(now, 1, 1);
-      a1[2] = ra.read(now, 1, 2);
-      a1[3] = ra.read(now, 1, 3);
+#pragma unroll
+      for (int i = 1; i < AF; ++i) a1[i] = ra.read(now, 1, i);
       fixed();
-      product(a0[2], b0, 2);
-      product(a0[3], b0, 3);
+#pragma unroll
+      for (int i = 2; i < AF; ++i) product(a0[i], b0, i);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       product(a1[0], b1, 0);
       // this slice is in registers and the next one has arrived: 2 more may be on their way, and behind the
       // slices that were copied before it, what `later` says
       if (LATER > 0 && later && it < kMmStages - 1)
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(8 + LATER) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(2 * kCopies + LATER) : "memory");
       else
-        asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(2 * kCopies) : "memory");
       fixed();
       // (the last time, of the next tile: they are read again behind the epilogue rather than kept)
-      b0[0] = rb.read(next + kMmOperand, 0, 0);
-      b0[1] = rb.read(next + kMmOperand, 0, 1);
+      b0[0] = rb.read(next + kA, 0, 0);
+      b0[1] = rb.read(next + kA, 0, 1);
       a0[0] = ra.read(next, 0, 0);
       fixed();
-      product(a1[1], b1, 1);
-      a0[1] = ra.read(next, 0, 1);
-      a0[2] = ra.read(next, 0, 2);
-      a0[3] = ra.read(next, 0, 3);
+      if constexpr (AF > 2) product(a1[1], b1, 1);
+#pragma unroll
+      for (int i = 1; i < AF; ++i) a0[i] = ra.read(next, 0, i);
       fixed();
-      product(a1[2], b1, 2);
+      if constexpr (AF > 2) product(a1[2], b1, 2);
       copy(from_a, from_b, ahead, stage + it);  // to where this slice lay
       fixed();
-      product(a1[3], b1, 3);
+      product(a1[AF - 1], b1, AF - 1);
     };
     int it = 0;
     for (; it < slices - kMmStages; ++it) slice(it, A, B, it + kMmStages);
     with_next();
     for (; it < slices; ++it) slice(it, nextA, nextB, it + kMmStages - slices);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < AF; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll

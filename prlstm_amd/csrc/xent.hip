@@ -84,7 +84,8 @@ struct TileInfo {
 };
 static_assert(sizeof(TileInfo) == 8 * 1024, "a copy of 1 KB by each wave");
 
-// One workgroup's walk over the tiles.
+// One workgroup's walk over the tiles of 64 AF tokens by 256 positions.
+template <int AF>
 struct LogitWalk {
   const LogitArgs& a;
   int id, tv, tn;
@@ -95,12 +96,12 @@ struct LogitWalk {
     id += gridDim.x;
     if (there()) find();
   }
-  __device__ __forceinline__ MmOperand rows_of(const MmOperand& o, int tile) const {
-    const int first = tile * kMmTile;
-    return {o.p + first * o.ld, o.ld, min(kMmTile, o.rows - first), there() ? o.k : 0, o.plane};
+  __device__ __forceinline__ MmOperand rows_of(const MmOperand& o, int tile, int rows) const {
+    const int first = tile * rows;
+    return {o.p + first * o.ld, o.ld, min(rows, o.rows - first), there() ? o.k : 0, o.plane};
   }
-  __device__ __forceinline__ MmOperand w() const { return rows_of(a.w, there() ? tv : 0); }
-  __device__ __forceinline__ MmOperand x() const { return rows_of(a.x, there() ? tn : 0); }
+  __device__ __forceinline__ MmOperand w() const { return rows_of(a.w, there() ? tv : 0, 64 * AF); }
+  __device__ __forceinline__ MmOperand x() const { return rows_of(a.x, there() ? tn : 0, kMmTile); }
   // Wave w copies piece w of the tile's information.
   __device__ __forceinline__ void info(TileInfo* to, int wave) const {
     const char* from = reinterpret_cast<const char*>(a.target + tn * kMmTile);
@@ -109,30 +110,32 @@ struct LogitWalk {
       from = reinterpret_cast<const char*>(a.rows + tn * kMmTile) + wave * 1024;
       in = in && a.rows;
     } else if (wave == 5) {
-      from = reinterpret_cast<const char*>(a.bias + tv * kMmTile);
+      from = reinterpret_cast<const char*>(a.bias + tv * 64 * AF);  // 256 of them, the last tile's too
     }
     mm_copy_kb(from, in, to, wave);
   }
 };
 
 // A lane's place in a tile: tokens v0 + 32 i + 8 q + e (q, e < 4) and positions n0 + 32 j.
+template <int AF>
 struct LogitPlace {
   int lane, wave, half, v, c, v0, n0;
   __device__ __forceinline__ LogitPlace(int tv, int tn) {
     lane = threadIdx.x & 63;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     half = lane >> 5;
-    v = (wave >> 2) * 128;
+    v = (wave >> 2) * 32 * AF;
     c = (wave & 3) * 64 + (lane & 31);
-    v0 = tv * kMmTile + v + 4 * half;
+    v0 = tv * 64 * AF + v + 4 * half;
     n0 = tn * kMmTile + c;
   }
 };
 
 // Adds the bias, which is there for every call: a branch around it would have the compiler move all sums.
-__device__ __forceinline__ void add_bias(const LogitPlace& q, const float* bias, MmAcc& acc) {
+template <int AF>
+__device__ __forceinline__ void add_bias(const LogitPlace<AF>& q, const float* bias, MmAccOf<AF>& acc) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < AF; ++i) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const f4 b = *reinterpret_cast<const f4*>(bias + q.v + 4 * q.half + i * 32 + 8 * k);
@@ -145,35 +148,35 @@ __device__ __forceinline__ void add_bias(const LogitPlace& q, const float* bias,
   }
 }
 
-template <int F>
+template <int F, int AF>
 __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
+  __shared__ __attribute__((aligned(1024))) char lds[mm_lds(AF)];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
   __shared__ float2 sm[2][kMmTile];
-  MmPipe<F == kElemF16, false, false, F == kElemF32> mm;
-  LogitWalk walk(a);
+  MmPipe<F == kElemF16, false, false, F == kElemF32, AF> mm;
+  LogitWalk<AF> walk(a);
   walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   mm.begin(lds, walk.w(), walk.x(), a.D);
   for (int par = 0; walk.there(); par ^= 1) {
     const int tv = walk.tv, tn = walk.tn;
     walk.next();
-    MmAcc acc;
+    MmAccOf<AF> acc;
     mm.template run<0>(acc, walk.w(), walk.x(), false, [&] { walk.info(&info[par ^ 1], mm.wave); });
-    const LogitPlace q(tv, tn);
+    const LogitPlace<AF> q(tv, tn);
     add_bias(q, info[par].bias, acc);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int n = q.n0 + j * 32, own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
       float m = neg_inf();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < AF; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
-      if (__any((unsigned)own < 128u)) {  // few waves have a target among their tokens
+      if (__any((unsigned)own < 32u * AF)) {  // few waves have a target among their tokens
         float l = 0.f;
         bool found = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < AF; ++i) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const bool here = own == i * 32 + 8 * (r >> 2) + (r & 3);
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
       const float ref = m == neg_inf() ? 0.f : m;
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < AF; ++i) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s += exp_from(acc[i][j][r], ref);
         __builtin_amdgcn_sched_barrier(0);
@@ -536,30 +539,31 @@ __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict
 }
 
 // The tile's dl goes from the registers to memory: an exchange between the half-waves gives every lane 8
-// neighbouring tokens of a position.  A lane's stores, 16 a part, are always issued, whatever lies outside, so
+// neighbouring tokens of a position.  A lane's stores, 4 AF a part, are always issued, whatever lies outside, so
 // that the next product's waits can leave them out.
 // PARTS: how many numbers of the product's type a dl is kept in.
-template <int F, int PARTS>
+template <int F, int PARTS, int AF>
 __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
-  constexpr int kStores = 16 * PARTS, kDl = PARTS > 1 && F != kElemF16 ? kElemBf16 : kElemF16;
-  __shared__ __attribute__((aligned(1024))) char lds[kMmLds];
+  constexpr int kStores = 4 * AF * PARTS, kDl = PARTS > 1 && F != kElemF16 ? kElemBf16 : kElemF16;
+  __shared__ __attribute__((aligned(1024))) char lds[mm_lds(AF)];
   __shared__ __attribute__((aligned(1024))) TileInfo info[2];
-  __shared__ float sums[4][kMmTile];
-  const long long ld = (long long)a.tiles_v * kMmTile;
-  MmPipe<F == kElemF16, false, false, F == kElemF32> mm;
-  LogitWalk walk(a);
+  __shared__ float sums[4][64 * AF];
+  constexpr int kTokens = 64 * AF;
+  const long long ld = (long long)a.tiles_v * kTokens;
+  MmPipe<F == kElemF16, false, false, F == kElemF32, AF> mm;
+  LogitWalk<AF> walk(a);
   walk.info(&info[0], __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
   mm.begin(lds, walk.w(), walk.x(), a.D);
   bool first = true;
   for (int par = 0; walk.there(); par ^= 1, first = false) {
     const int tv = walk.tv, tn = walk.tn;
     walk.next();
-    MmAcc acc;
+    MmAccOf<AF> acc;
     mm.template run<kStores>(acc, walk.w(), walk.x(), !first, [&] { walk.info(&info[par ^ 1], mm.wave); });
-    const LogitPlace q(tv, tn);
+    const LogitPlace<AF> q(tv, tn);
     add_bias(q, info[par].bias, acc);
     auto out_of = [&](int part) {
-      return __builtin_amdgcn_make_buffer_rsrc(a.dl + ((long long)part * a.N + tn * kMmTile) * ld + tv * kMmTile, (short)0,
+      return __builtin_amdgcn_make_buffer_rsrc(a.dl + ((long long)part * a.N + tn * kMmTile) * ld + tv * kTokens, (short)0,
                                                0x7fffffff, 0x00020000);
     };
 #pragma unroll
@@ -568,7 +572,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
       const int own = info[par].target[q.c + j * 32] - a.v_first - q.v0;
       const float gi = row.y, ref = row.x;
       const float hot = __float_as_int(row.w) < 0 ? 0.f : row.z;
-      const bool owns = __any((unsigned)own < 128u);  // few waves have a target among their tokens
+      const bool owns = __any((unsigned)own < 32u * AF);  // few waves have a target among their tokens
       // a masked logit has none whatever arrives, nor has a row without a gradient whatever it holds
       const bool plain =
           __all(__builtin_fabsf(gi) < __builtin_inff() && __builtin_fabsf(row.x) < __builtin_inff());
@@ -576,7 +580,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
       const unsigned off =
           q.n0 + j * 32 < a.N ? (unsigned)((q.c + j * 32) * ld + q.v + 8 * q.half) * 2 : kOffNone;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < AF; ++i) {
         __builtin_amdgcn_sched_barrier(0);  // 16 values at a time in registers beside the rest
         if (plain) {
 #pragma unroll
@@ -623,23 +627,23 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
       }
     }
     if (a.dbias) {  // in fp32, from before the rounding
-      float f[2][16];
+      float f[AF / 2][16];
       const float p0 = __builtin_fabsf(info[par].rows[q.c].w), p1 = __builtin_fabsf(info[par].rows[q.c + 32].w);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
+      for (int k = 0; k < 8 * AF; ++k) {
         const int u = 2 * k, i = u / 16, r = u % 16;
         f[k / 16][k % 16] = add16(acc[i][0][r] * p0 + acc[i][1][r] * p1, acc[i][0][r + 1] * p0 + acc[i][1][r + 1] * p1);
       }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < AF / 2; ++k) {
         const float v = sum_rows(f[k], q.lane);
         const int u = 2 * (16 * k + (q.lane & 15)) + ((q.lane >> 4) & 1), i = u / 16, r = u % 16;
         sums[q.wave & 3][q.v + i * 32 + 8 * (r >> 2) + 4 * q.half + (r & 3)] = v;
       }
       lds_barrier();
       const int c = threadIdx.x;
-      if (c < kMmTile)
-        a.dbias[(size_t)tn * ld + tv * kMmTile + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+      if (c < kTokens)
+        a.dbias[(size_t)tn * ld + tv * kTokens + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
     }
   }
 }
@@ -881,9 +885,20 @@ bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kEle
 // and a probability of them against the other ones' sum would be off by as much (dbias of 12 rows: 3.3e-7, 2.1e-7 from
 // the same ones).
 bool takes_few(int N, int fmt, bool alone) { return alone && fmt != kElemF32 && N <= kFewRows; }
+// The tokens that the forward takes at a time.
+int forward_piece(int N, int V, int D, int fmt) {
+  return fmt == kElemF32 ? std::min(V, plan_xent(N, V, D, fmt).piece) : V;
+}
+// Fragments of 64 tokens of the logits' tiles, 2 where that takes less rounds of the 256 CUs: half a tile costs a little
+// more than half.
+int logit_frags(int N, int V) {
+  const long long tiles = (long long)((N + kMmTile - 1) / kMmTile) * ((V + kMmTile - 1) / kMmTile);
+  return 11 * ((2 * tiles + 255) / 256) < 20 * ((tiles + 255) / 256) ? 2 : 4;
+}
 // The parts that the forward's statistics of a row are joined from.
-int forward_parts(int N, int V, int fmt, bool alone) {
-  return takes_few(N, fmt, alone) ? few_blocks(V) : (V + kMmTile - 1) / kMmTile;
+int forward_parts(int N, int V, int D, int fmt, bool alone) {
+  const int tokens = 64 * logit_frags(N, forward_piece(N, V, D, fmt));
+  return takes_few(N, fmt, alone) ? few_blocks(V) : (V + tokens - 1) / tokens;
 }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
@@ -938,7 +953,7 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   const int width = up_to(D, 8);
   Carver c(base, 0);
   s.target = c.take<int>(up_to(N, kMmTile));
-  s.bias = c.take<float>(up_to(V, kMmTile));
+  s.bias = c.take<float>(up_to(V, kMmTile) + kMmTile / 2);  // a last tile of 128 has 256 copied
   if (split) {
     s.own_x = c.take<unsigned short>((size_t)3 * N * width);
     s.own_w = c.take<unsigned short>((size_t)3 * std::min(V, p.piece) * width);
@@ -948,7 +963,7 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   }
   if (!backward) {
     s.own = c.take<float>(N);
-    s.part = c.take<float2>((size_t)N * std::max(forward_parts(N, V, fmt, true), forward_parts(N, V, fmt, false)));
+    s.part = c.take<float2>((size_t)N * std::max(forward_parts(N, V, D, fmt, true), forward_parts(N, V, D, fmt, false)));
     s.bytes = c.off;
     return s;
   }
@@ -1057,29 +1072,32 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   a.tiles_n = (n + kMmTile - 1) / kMmTile;
   a.own = s.own;
   const bool few = takes_few(n, fmt, !stats);
-  const int piece = fmt == kElemF32 ? plan_xent(n, V, D, fmt).piece : V;
+  const int piece = forward_piece(n, V, D, fmt), frags = logit_frags(n, piece);
   for (int v0 = 0; v0 < V; v0 += piece) {
     const int v = std::min(piece, V - v0);
     a.w = o.tokens(v0, v, st);
     a.bias = s.bias + v0;
     a.v_first = v0;
     a.V = v;
-    a.tiles_v = (v + kMmTile - 1) / kMmTile;
-    a.part = s.part + (size_t)(v0 / kMmTile) * n;
+    a.tiles_v = (v + 64 * frags - 1) / (64 * frags);
+    a.part = s.part + (size_t)(v0 / (64 * frags)) * n;
     const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
-    if (fmt == kElemF32)
-      hipLaunchKernelGGL(xent_stats_kernel<kElemF32>, grid, block, 0, st, a);
-    else if (few && fmt == kElemF16)
+    if (few && fmt == kElemF16)
       hipLaunchKernelGGL(xent_few_kernel<true>, dim3(few_blocks(V)), dim3(256), 0, st, a);
     else if (few)
       hipLaunchKernelGGL(xent_few_kernel<false>, dim3(few_blocks(V)), dim3(256), 0, st, a);
-    else if (fmt == kElemF16)
-      hipLaunchKernelGGL(xent_stats_kernel<kElemF16>, grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL(xent_stats_kernel<kElemBf16>, grid, block, 0, st, a);
+      HSL_CHECK(with_fmt(fmt, [&](auto F) {
+        constexpr int kF = decltype(F)::value;
+        if (frags == 2)
+          hipLaunchKernelGGL((xent_stats_kernel<kF, 2>), grid, block, 0, st, a);
+        else
+          hipLaunchKernelGGL((xent_stats_kernel<kF, 4>), grid, block, 0, st, a);
+        return (int)HSL_OK;
+      }));
   }
   hipLaunchKernelGGL(xent_join_kernel, dim3((n + 7) / 8), dim3(256), 0, st, s.part, s.own, s.target, loss,
-                     reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, fmt, !stats));
+                     reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, D, fmt, !stats));
   HSL_HIP(hipGetLastError());
   return HSL_OK;
 }
@@ -1171,6 +1189,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     return (int)HSL_OK;
   };
   float* const planes_x = s.dx ? s.dx : static_cast<float*>(dx);  // fp32: one plane is dx itself
+  const int frags = logit_frags(n, std::min(V, p.piece));
   for (int v0 = 0; v0 < V; v0 += p.piece) {
     const int v = std::min(p.piece, V - v0);
     const int tiles_v = (v + kMmTile - 1) / kMmTile;  // the last piece may have fewer
@@ -1183,7 +1202,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     a.V = v;
     a.N = n;
     a.D = D;
-    a.tiles_v = tiles_v;
+    a.tiles_v = tiles_v * (4 / frags);  // dl and dbias to whole tiles of 256
     a.tiles_n = (n + kMmTile - 1) / kMmTile;
     a.rows = s.rows;
     a.dl = s.dl;
@@ -1212,12 +1231,16 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     g.k_x = p.k_x;
     g.k_w = p.k_w;
     g.add = v0 > 0;
-    const dim3 grid(std::min(tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
+    const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
     const dim3 grid_out((g.splits_x * g.tiles_n + g.splits_w * tiles_v) * g.tiles_d);
     auto run = [&](auto F, auto PARTS, auto FP16) {
-      hipLaunchKernelGGL((xent_grad_kernel<decltype(F)::value, decltype(PARTS)::value>), grid, block, 0, st, a);
+      constexpr int kF = decltype(F)::value, kParts = decltype(PARTS)::value;
+      if (frags == 2)
+        hipLaunchKernelGGL((xent_grad_kernel<kF, kParts, 2>), grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL((xent_grad_kernel<kF, kParts, 4>), grid, block, 0, st, a);
       if (grid_out.x)
-        hipLaunchKernelGGL((xent_out_kernel<decltype(F)::value, decltype(FP16)::value>), grid_out, block, 0, st, g);
+        hipLaunchKernelGGL((xent_out_kernel<kF, decltype(FP16)::value>), grid_out, block, 0, st, g);
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;

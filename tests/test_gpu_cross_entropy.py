@@ -252,6 +252,13 @@ def test_sizes_of_the_operands(dev):
     check(x, w * 0, t, b, dloss)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(300, 17000, 40), (300, 40000, 24), (1100, 20500, 24)])
+def test_many_tiles(dev, dtype, n, v, d):
+    """Tiles of 256 tokens (134, 405 of them) and of 128 (628), one and several for a workgroup."""
+    check(*inputs(dev, dtype, n, v, d, bias=True, pad=True))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n", [1, 2, 200])
 def test_gradients_are_rounded_once(dev, dtype, n):
