@@ -24,6 +24,7 @@
 // fp32 operands: the same in three bf16 pieces each (mm16.h), dl too; the weight's are made for a piece of the
 // vocabulary at a time.
 #include <algorithm>
+#include <cmath>
 
 #include "mm16.h"
 
@@ -846,6 +847,26 @@ RowSplit split_rows(long long rows, int units, int most) {
 }
 constexpr int kScaleBlocks = 1024;  // for an operand
 
+// When 256 CUs that take `nx` workgroups of length x and then `nw` of length w, in order, are done.
+double rounds_time(double nx, double x, double nw, double w) {
+  const double full = std::floor(nx / 256);
+  double late = nx - 256 * full, time[2] = {full * x, (full + 1) * x}, cus[2] = {256 - late, late};
+  if (late == 0) time[1] = time[0];
+  if (nw > 256 * 64) {  // so many that their lengths do not tell
+    time[0] += std::floor(nw / 256) * w;
+    time[1] += std::floor(nw / 256) * w;
+    nw -= 256 * std::floor(nw / 256);
+  }
+  double done = std::max(time[0], cus[1] > 0 ? time[1] : 0);
+  while (nw > 0) {
+    const int g = cus[1] == 0 || time[0] <= time[1] ? 0 : 1;
+    nw -= cus[g];
+    time[g] += w;
+    done = std::max(done, time[g]);
+  }
+  return done;
+}
+
 struct XentPlan {
   int piece, pieces;  // tokens of a piece: a multiple of 256
   int tiles_n, tiles_d, tiles_v;
@@ -865,16 +886,33 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   p.tiles_n = (N + kMmTile - 1) / kMmTile;
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.tiles_v = p.piece / kMmTile;
-  // k of a workgroup such that the two products' work makes about 256 equal shares (of fp32 operands, a k is six)
+  // k of a workgroup: the two products' work in about 256 equal shares, or 384, 512 or 768 where those should end a
+  // quarter sooner (2500 fp32 rows, 3100 tokens of width 1999: 264 of the first would take two rounds of the 256 CUs, 448
+  // smaller ones two of half the length, 1152 -> 1070 us for the pass; by less they lose, as the last workgroups of a
+  // round run faster than a full chip's: 5227 bf16 rows, 53383 tokens of width 299 1120 -> 1215).  An fp32 k is six, and
+  // a share's start and end cost about 400.
   const double total = (double)p.tiles_d * ((double)p.tiles_n * p.piece + (double)p.tiles_v * N);
-  const int share = std::max(split ? 128 : 512, (int)std::min(1e9, total / 256));
-  auto share_out = [&](int k, int* splits, int* each) {
-    *splits = std::max(1, (int)(((long long)k + share / 2) / share));
-    *each = std::max(kMmSlice, up_to((k + *splits - 1) / *splits, kMmSlice));
-    *splits = std::max(1, (k + *each - 1) / *each);
-  };
-  share_out(p.piece, &p.splits_x, &p.k_x);
-  share_out(N, &p.splits_w, &p.k_w);
+  const int least = split ? 128 : 512, ends = split ? 64 : 400;
+  double best = 0;
+  for (int parts : {256, 384, 512, 768}) {
+    const int share = std::max(least, (int)std::min(1e9, total / parts));
+    auto share_out = [&](int k, int* splits, int* each) {
+      *splits = std::max(1, (int)(((long long)k + share / 2) / share));
+      *each = std::max(kMmSlice, up_to((k + *splits - 1) / *splits, kMmSlice));
+      *splits = std::max(1, (k + *each - 1) / *each);
+    };
+    int sx, kx, sw, kw;
+    share_out(p.piece, &sx, &kx);
+    share_out(N, &sw, &kw);
+    const double time = rounds_time((double)sx * p.tiles_n * p.tiles_d, kx + ends, (double)sw * p.tiles_v * p.tiles_d,
+                                    kw + ends);
+    if (parts > 256 && time > 0.75 * best) continue;
+    best = time;
+    p.splits_x = sx;
+    p.k_x = kx;
+    p.splits_w = sw;
+    p.k_w = kw;
+  }
   return p;
 }
 
