@@ -189,7 +189,8 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
   // A chunk's steps forwards with their decays and states kept, then backwards: in two halves where four
   // states a wave would not leave the registers for all of it (the first half then runs three times).
   // SLOW: a reset in the chunk, or lanes without a channel
-  constexpr int kHalves = S == 4 ? 2 : 1, H = L / kHalves, G = S == 4 ? 1 : 4;  // G: steps whose operands are read from LDS ahead
+  constexpr int kHalves = S == 4 ? 2 : 1, H = L / kHalves;
+  constexpr int G = S == 4 ? 1 : 4;  // steps whose operands are read from LDS ahead
   auto run = [&](auto slow, int t0) {
     constexpr bool SLOW = decltype(slow)::value;
     float f[H][S], hs[H][S], start[S], cda[S] = {};
@@ -430,8 +431,8 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__
   }
 }
 
-// f(integral_constant fmt, ScanShape): two states a wave up to 16 (four a wave, in half the waves and two workgroups a CU, took 3152 us for 2547,
-// T4096 B32 D1024 N16 bf16: its registers leave one wave a SIMD).
+// f(integral_constant fmt, ScanShape): two states a wave up to 16 (four a wave, in half the waves and two workgroups a
+// CU, took 3152 us for 2547, T4096 B32 D1024 N16 bf16: its registers leave one wave a SIMD).
 template <class Fn>
 int with_bwd_shape(int fmt, int N, Fn f) {
   return with_fmt(fmt, [&](auto F) {

@@ -505,8 +505,8 @@ __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
 }
 
 // The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.
-__global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld, unsigned short* dst,
-                                                         RowSplit r, int cols, int width) {
+__global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld,
+                                                         unsigned short* dst, RowSplit r, int cols, int width) {
   const size_t plane = (size_t)r.rows * width;
   for_rows(r, width / 8, blockIdx.x, [&](const long long(&row)[4], int c) {
     float f[4][8];
@@ -564,8 +564,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
     const LogitPlace<AF> q(tv, tn);
     add_bias(q, info[par].bias, acc);
     auto out_of = [&](int part) {
-      return __builtin_amdgcn_make_buffer_rsrc(a.dl + ((long long)part * a.N + tn * kMmTile) * ld + tv * kTokens, (short)0,
-                                               0x7fffffff, 0x00020000);
+      unsigned short* const p = a.dl + ((long long)part * a.N + tn * kMmTile) * ld + tv * kTokens;
+      return __builtin_amdgcn_make_buffer_rsrc(p, (short)0, 0x7fffffff, 0x00020000);
     };
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -685,6 +685,11 @@ __global__ __launch_bounds__(kMmThreads) void xent_out_kernel(OutArgs a) {
   const int count_x = a.splits_x * a.tiles_n * a.tiles_d;
   const bool is_x = (int)blockIdx.x < count_x;
   int id = is_x ? blockIdx.x : blockIdx.x - count_x;
+  {  // workgroups i and i + 8 share an XCD and its L2: each XCD has a contiguous range, whose tiles of the width take
+     // the same dl (515 -> 502 us for a piece of 16384 tokens at 8192 rows of width 1024)
+    const int even = (is_x ? count_x : (int)gridDim.x - count_x) & ~7;
+    if (id < even) id = (id % 8) * (even / 8) + id / 8;
+  }
   const int td = id % a.tiles_d;
   id /= a.tiles_d;
   const int tiles = is_x ? a.tiles_n : a.tiles_v, tm = id % tiles, split = id / tiles;
@@ -877,7 +882,7 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   const bool split = fmt == kElemF32;
   const int all = up_to(V, kMmTile);
   long long room = std::min<long long>(kPieceWidth, kPieceBytes / (split ? 6 : 2) / std::max(1, N));
-  if (split) room = std::min<long long>(room, kPieceBytes / 6 / up_to(D, 8));  // the weight's pieces are as large at most
+  if (split) room = std::min<long long>(room, kPieceBytes / 6 / up_to(D, 8));  // the weight's pieces are no larger
   const long long fit = std::max<long long>(1, room / kMmTile) * kMmTile;
   p.piece = (int)std::min<long long>(all, fit);
   p.pieces = (all + p.piece - 1) / p.piece;
@@ -887,10 +892,10 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.tiles_v = p.piece / kMmTile;
   // k of a workgroup: the two products' work in about 256 equal shares, or 384, 512 or 768 where those should end a
-  // quarter sooner (2500 fp32 rows, 3100 tokens of width 1999: 264 of the first would take two rounds of the 256 CUs, 448
-  // smaller ones two of half the length, 1152 -> 1070 us for the pass; by less they lose, as the last workgroups of a
-  // round run faster than a full chip's: 5227 bf16 rows, 53383 tokens of width 299 1120 -> 1215).  An fp32 k is six, and
-  // a share's start and end cost about 400.
+  // quarter sooner (2500 fp32 rows, 3100 tokens of width 1999: 264 of the first would take two rounds of the 256 CUs,
+  // 448 smaller ones two of half the length, 1152 -> 1070 us for the pass; by less they lose, as the last workgroups
+  // of a round run faster than a full chip's: 5227 bf16 rows, 53383 tokens of width 299 1120 -> 1215).  An fp32 k is
+  // six, and a share's start and end cost about 400.
   const double total = (double)p.tiles_d * ((double)p.tiles_n * p.piece + (double)p.tiles_v * N);
   const int least = split ? 128 : 512, ends = split ? 64 : 400;
   double best = 0;
@@ -927,8 +932,8 @@ bool takes_few(int N, int fmt, bool alone) { return alone && fmt != kElemF32 && 
 int forward_piece(int N, int V, int D, int fmt) {
   return fmt == kElemF32 ? std::min(V, plan_xent(N, V, D, fmt).piece) : V;
 }
-// Fragments of 64 tokens of the logits' tiles, 2 where that takes less rounds of the 256 CUs: half a tile costs a little
-// more than half.
+// Fragments of 64 tokens of the logits' tiles, 2 where that takes less rounds of the 256 CUs: half a tile costs a
+// little more than half (700 fp32 rows, 10007 tokens of width 650, 120 tiles: 105 -> 83 us).
 int logit_frags(int N, int V) {
   const long long tiles = (long long)((N + kMmTile - 1) / kMmTile) * ((V + kMmTile - 1) / kMmTile);
   return 11 * ((2 * tiles + 255) / 256) < 20 * ((tiles + 255) / 256) ? 2 : 4;
@@ -948,8 +953,8 @@ int check_xent(const char* who, long long N, int V, int D, int fmt) {
       ((N + 255) / 256) * (((long long)V + 255) / 256) >= (1ll << 22) ||
       ((N + 255) / 256 + ((long long)V + 255) / 256) * ((D + 255) / 256) >= (1ll << 22))
     return fail(HSL_ERR_UNSUPPORTED,
-                "%s: N=%lld V=%d D=%d is beyond one launch (needs N < 2^24, D < 2^20 and fewer than 2^22 tiles of 256 x "
-                "256 of each product)",
+                "%s: N=%lld V=%d D=%d is beyond one launch (needs N < 2^24, D < 2^20 and fewer than 2^22 tiles of 256 "
+                "x 256 of each product)",
                 who, N, V, D);
   return HSL_OK;
 }
@@ -965,8 +970,10 @@ int check_begin(const char* who, const void* x, long long ldx, const void* w, lo
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < (1 << 21);
   };
   if (fmt != kElemF32 && D % 8 == 0 && (!readable(x, ldx) || !readable(w, ldw)))
-    return fail(HSL_ERR_ARG, "%s: rows of D=%d must begin at multiples of 16 bytes, fewer than 2^21 elements apart (row "
-                             "strides %lld and %lld)", who, D, ldx, ldw);
+    return fail(HSL_ERR_ARG,
+                "%s: rows of D=%d must begin at multiples of 16 bytes, fewer than 2^21 elements apart (row strides %lld "
+                "and %lld)",
+                who, D, ldx, ldw);
   return HSL_OK;
 }
 
@@ -1001,7 +1008,8 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   }
   if (!backward) {
     s.own = c.take<float>(N);
-    s.part = c.take<float2>((size_t)N * std::max(forward_parts(N, V, D, fmt, true), forward_parts(N, V, D, fmt, false)));
+    const int parts = std::max(forward_parts(N, V, D, fmt, true), forward_parts(N, V, D, fmt, false));
+    s.part = c.take<float2>((size_t)N * parts);
     s.bytes = c.off;
     return s;
   }
@@ -1204,7 +1212,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     if (two) hipLaunchKernelGGL(xent_twice_kernel, dim3(2 * n), dim3(256), 0, st, sc);
   } else if (fmt == kElemF16) {
     hipLaunchKernelGGL(xent_max_kernel<true>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
-    hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + std::min(kScaleBlocks, row_blocks)), dim3(256), 0, st, sc);
+    hipLaunchKernelGGL(xent_scaled_kernel<true>, dim3(scaled + std::min(kScaleBlocks, row_blocks)), dim3(256), 0, st,
+                       sc);
   } else {
     hipLaunchKernelGGL(xent_max_kernel<false>, dim3(scaled + sc.blocks_g), dim3(256), 0, st, sc);
     hipLaunchKernelGGL(xent_scaled_kernel<false>, dim3(scaled + std::min(kScaleBlocks, row_blocks)), dim3(256), 0, st,
@@ -1219,8 +1228,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
         hipLaunchKernelGGL(xent_planes_kernel<kF>, dim3(r.blocks), dim3(256), 0, st, planes, plane, count, s.exps,
                            row_exp, out, r, D);
       else
-        hipLaunchKernelGGL(xent_many_planes_kernel<kF>, dim3((unsigned)(((size_t)rows * D + 63) / 64)), dim3(256), 0, st,
-                           planes, plane, count, s.exps, row_exp, out, (size_t)rows * D, D);
+        hipLaunchKernelGGL(xent_many_planes_kernel<kF>, dim3((unsigned)(((size_t)rows * D + 63) / 64)), dim3(256), 0,
+                           st, planes, plane, count, s.exps, row_exp, out, (size_t)rows * D, D);
       HSL_HIP(hipGetLastError());
       return (int)HSL_OK;
     }));

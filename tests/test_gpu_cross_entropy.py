@@ -306,7 +306,8 @@ def test_some_gradients(dev):
     """Only what is asked for, whatever the rest is."""
     x, w, t, b, dloss = inputs(dev, torch.bfloat16, 60, 300, 40, bias=True)
     leaves = [s.detach().requires_grad_(True) for s in (x, w, b)]
-    all_of = torch.autograd.grad(prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2]), leaves, dloss)
+    loss = prlstm_amd.linear_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+    all_of = torch.autograd.grad(loss, leaves, dloss)
     for k in range(3):
         args = [x, w, b]
         args[k] = leaves[k]
@@ -336,7 +337,8 @@ def test_refusals(dev):
                        (lambda: f(z(3, 4, dt=torch.float64), z(5, 4, dt=torch.float64), t), "x must be"),
                        (lambda: f(z(3, 4), z(5, 4), t.float()), "int64 or int32"),
                        (lambda: f(z(3, 4), z(5, 4), t, bias=z(4)), "bias must"),
-                       (lambda: f(z(3, 4), z(0, 4), t), "must not be empty"), (lambda: f(z(3, 0), z(5, 0), t), "must not be empty"),
+                       (lambda: f(z(3, 4), z(0, 4), t), "must not be empty"),
+                       (lambda: f(z(3, 0), z(5, 0), t), "must not be empty"),
                        (lambda: f(z(3, 4), z(5, 4), t.cpu()), "targets is on"),
                        (lambda: f(z(3, 4), z(5, 4).cpu(), t), "weight must be")):
         with pytest.raises(RuntimeError, match=text):

@@ -97,7 +97,8 @@ def test_loss_beyond_32_bits(dev, n, v, d, dtype):
     dx, dw = torch.autograd.grad(loss, (big_x, big_w), dl)
     want, ref_dl, parts, size = xent.reference(x, w, t, None, dloss)
     shift = (d + 4) * xent.U * size
-    xent.within("loss", loss[n - rows:], want, 2 * shift + 16 * xent.U * (want.abs() + size + math.log(v + 1)) + 2 ** -20)
+    xent.within("loss", loss[n - rows:], want,
+                2 * shift + 16 * xent.U * (want.abs() + size + math.log(v + 1)) + 2 ** -20)
     _, bound_x, bound_w = xent.bounds(x, w, t, ref_dl, parts, shift, dloss)
     xent.within("dx", dx[n - rows:], ref_dl @ w.double().cpu(), bound_x)
     xent.within("dw", dw[kept.to(dev)], ref_dl.t() @ x.double().cpu(), bound_w)
@@ -120,7 +121,8 @@ def _calls(dev):
         ("scan_step", lambda o: prlstm_amd.selective_scan_step(**o)[0],
          dict(x=r(2, 5), delta=r(2, 5), a=-r(5, 3).abs(), b=r(2, 3), c=r(2, 3), h=r(2, 5, 3), d=r(5), z=r(2, 5),
               delta_bias=r(5))),
-        ("loss", lambda o: prlstm_amd.linear_cross_entropy(targets=t, **o), dict(x=r(6, 2, 5), weight=r(7, 5), bias=r(7))),
+        ("loss", lambda o: prlstm_amd.linear_cross_entropy(targets=t, **o),
+         dict(x=r(6, 2, 5), weight=r(7, 5), bias=r(7))),
     ]
 
 
@@ -130,7 +132,8 @@ def test_operands_that_do_not_fit(dev):
         call(operands)
         for k, v in operands.items():
             others = [v[0], torch.cat((v, v), -1), torch.cat((v, v)), v.cpu(), v.double() if k == "x" else v.int()]
-            if k in ("delta", "b", "c", "z") or (name, k) in (("conv", "state"), ("conv_step", "state"), ("loss", "weight")):
+            if k in ("delta", "b", "c", "z") or (name, k) in (("conv", "state"), ("conv_step", "state"),
+                                                              ("loss", "weight")):
                 others.append(v.bfloat16())
             for i, other in enumerate(others):
                 if (name, k, i) == ("conv", "x", 2):
