@@ -299,7 +299,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
   const int c = threadIdx.x & 7, strip = threadIdx.x >> 3, n = blockIdx.x * 8 + c;
   float m = neg_inf(), s = 0.f;
   if (n < N) {
-#pragma unroll 4
+#pragma unroll 8
     for (int t = strip; t < parts; t += 32) {
       const float2 p = part[(size_t)t * N + n];
       join(m, s, p.x, p.y);
