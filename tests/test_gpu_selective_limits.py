@@ -230,3 +230,35 @@ def test_two_graphs(dev):
         torch.cuda.synchronize()
         for (_, out, _), w in zip(made, want):
             assert all(torch.equal(a, b) for a, b in zip(out, w)), order
+
+
+def test_two_streams(dev):
+    """The whole chain on two streams at a time: neither call sees the other's workspaces."""
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    chains = []
+    for T, B, D, N, V, dtype in ((2000, 1, 128, 16, 3000, BF16), (600, 3, 72, 7, 700, torch.float32)):
+        o = dict(u=r(T, B, D).to(dtype), taps=r(D, 4), delta=r(T, B, D).to(dtype), a=-r(D, N).abs() - 0.1,
+                 b=r(T, B, N).to(dtype), c=r(T, B, N).to(dtype), w=(r(V, D) * D ** -0.5).to(dtype))
+        t, dl = torch.randint(0, V, (T, B), generator=g).to(dev), r(T, B)
+
+        def chain(o=o, t=t, dl=dl):
+            leaves = {k: v.detach().requires_grad_(True) for k, v in o.items()}
+            x, _ = prlstm_amd.causal_conv(leaves["u"], leaves["taps"])
+            y, _ = prlstm_amd.selective_scan(x, *(leaves[k] for k in ("delta", "a", "b", "c")))
+            loss = prlstm_amd.linear_cross_entropy(y, leaves["w"], t)
+            return loss.detach(), *torch.autograd.grad(loss, list(leaves.values()), dl)
+
+        chains.append(chain)
+    want = [chain() for chain in chains]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in chains]
+    for _ in range(4):
+        got = []
+        for s, chain in zip(streams, chains):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(chain())
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
