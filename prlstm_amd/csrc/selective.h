@@ -28,8 +28,7 @@ constexpr int kMaxStates = 64;
 template <int W_, int S_>
 struct ScanShape {
   static constexpr int W = W_, S = S_, N = W * S;
-  // Steps of a chunk, which is also what lies between two kept states.  Sixteen waves have 128
-  // registers each, which hold the backward's copy of 8 steps.
+  // Steps of a chunk, which is also what lies between two kept states.
   static constexpr int L = N > 32 ? 8 : 16;
   static constexpr int PS = L >= W ? L / W : 1;  // steps that a wave has in A and C
 };

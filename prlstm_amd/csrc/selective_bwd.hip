@@ -186,11 +186,12 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
     }
     m.bc.store(sb, sc);
   };
-  // A chunk's steps forwards with their decays and states kept, then backwards: in two halves where four
-  // states a wave would not leave the registers for all of it (the first half then runs three times).
+  // A chunk's steps forwards with their decays and states kept, then backwards: in two parts where four states a wave
+  // would not leave the registers for all of it, in four where eight are (a part's steps run once more for each part
+  // behind it).
   // SLOW: a reset in the chunk, or lanes without a channel
-  constexpr int kHalves = S == 4 ? 2 : 1, H = L / kHalves;
-  constexpr int G = S == 4 ? 1 : 4;  // steps whose operands are read from LDS ahead
+  constexpr int kParts = S == 8 ? 4 : S == 4 ? 2 : 1, H = L / kParts;
+  constexpr int G = S >= 4 ? 1 : 4;  // steps whose operands are read from LDS ahead
   auto run = [&](auto slow, int t0) {
     constexpr bool SLOW = decltype(slow)::value;
     float f[H][S], hs[H][S], start[S], cda[S] = {};
@@ -235,32 +236,26 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
         for (int n = 0; n < S; ++n) start[n] = h[n];
       }
     };
-    constexpr int kRegs = H * S / 2;  // of sums over rows, four values each
-    static_assert(L * S / 2 % 16 == 0, "sum_rows takes 16");
-    float sums[kHalves * kRegs > 16 ? kRegs : kHalves * kRegs];
-    constexpr bool kEach = kHalves * kRegs > 16;  // the half's sums are finished with it
-    auto finish_sums = [&](int s0, int count) {
+    // Sums over rows, four values each; they are finished when there are 16.
+    static_assert(L * S / 2 % 16 == 0 && (H * S / 2 % 16 == 0 || 16 % (H * S / 2) == 0), "sum_rows takes 16");
+    float sums[16];
+    auto finish_sums = [&](int s0) {
       const int row = q.lane >> 4;
       float* const out = a.part_bc + (((size_t)q.tile * a.T + t0) * a.B + q.b) * (2 * P::N) + (row & 1) * P::N +
                          q.n0 + (row >> 1);
-#pragma unroll
-      for (int k = 0; k < count / 16; ++k) {
-        float r16[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) r16[i] = sums[16 * k + i];
-        const float v = sum_rows(r16, q.lane);
-        const int r = 16 * k + (q.lane & 15), s = s0 + r / (S / 2), n = r % (S / 2) * 2;
-        if (t0 + s < te) out[(size_t)s * a.B * (2 * P::N) + n] = v;
-      }
+      const float v = sum_rows(sums, q.lane);
+      const int r = q.lane & 15, s = s0 + r / (S / 2), n = r % (S / 2) * 2;
+      if (t0 + s < te) out[(size_t)s * a.B * (2 * P::N) + n] = v;
     };
 #pragma unroll
-    for (int half = kHalves - 1; half >= 0; --half) {
-      const int s0 = half * H;
+    for (int part = kParts - 1; part >= 0; --part) {
+      const int s0 = part * H;
 #pragma unroll
       for (int n = 0; n < S; ++n) start[n] = hin[n];
-      if (half) {
-        forwards(0, std::false_type{});
-        asm volatile("" ::: "memory");  // what it read is read again rather than kept for the other half
+#pragma unroll
+      for (int before = 0; before < part; ++before) {
+        forwards(before * H, std::false_type{});
+        asm volatile("" ::: "memory");  // what it read is read again rather than kept for the other parts
       }
       forwards(s0, std::true_type{});
       struct Ahead {
@@ -311,12 +306,11 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
         // rows 0..3: b of state n, c of state n, b of state n + 1, c of state n + 1
 #pragma unroll
         for (int n = 0; n < S; n += 2)
-          sums[(kEach ? k : s) * (S / 2) + n / 2] = add16(add32(vb[n], vb[n + 1]), add32(vc[n], vc[n + 1]));
+          sums[(s * (S / 2) + n / 2) % 16] = add16(add32(vb[n], vb[n + 1]), add32(vc[n], vc[n + 1]));
+        if (s * (S / 2) % 16 == 0) finish_sums(s);
       }
-      if (kEach) finish_sums(s0, kRegs);
       asm volatile("" ::: "memory");
     }
-    if (!kEach) finish_sums(0, kHalves * kRegs);
 #pragma unroll
     for (int n = 0; n < S; ++n) da[n].add(cda[n]);
   };
@@ -432,7 +426,8 @@ __global__ __launch_bounds__(256) void scan_sum_kernel(const float* __restrict__
 }
 
 // f(integral_constant fmt, ScanShape): two states a wave up to 16 (four a wave, in half the waves and two workgroups a
-// CU, took 3152 us for 2547, T4096 B32 D1024 N16 bf16: its registers leave one wave a SIMD).
+// CU, took 3152 us for 2547, T4096 B32 D1024 N16 bf16: its registers leave one wave a SIMD).  64 states: eight a wave,
+// 2891 us at T1024 B32 D1024 in four parts, 3308 in two; four a wave, whose 16 waves have 128 registers each, 5253.
 template <class Fn>
 int with_bwd_shape(int fmt, int N, Fn f) {
   return with_fmt(fmt, [&](auto F) {
@@ -441,7 +436,7 @@ int with_bwd_shape(int fmt, int N, Fn f) {
       case 8: return f(F, ScanShape<4, 2>{});
       case 16: return f(F, ScanShape<8, 2>{});
       case 32: return f(F, ScanShape<8, 4>{});
-      default: return f(F, ScanShape<16, 4>{});
+      default: return f(F, ScanShape<8, 8>{});
     }
   });
 }
