@@ -87,7 +87,7 @@ template <int F, class P>
 __global__ __launch_bounds__(P::W * 64) void scan_bwd_map_kernel(ScanArgs a) {
   constexpr int L = P::L, S = P::S;
   __shared__ float2 sdt[L][64];  // dt, dy
-  __shared__ __attribute__((aligned(16))) float sb[L][P::N], sc[L][P::N];
+  __shared__ __attribute__((aligned(32))) float sb[L][P::N], sc[L][P::N];
   const ScanPlace<P> q(a);
   const unsigned off = q.ok ? q.ch * (unsigned)sizeof(typename Elem<F>::T) : kOffNone;
   const int seg = blockIdx.y + 1, tb = seg * a.seg_steps, te = min(a.T, tb + a.seg_steps);
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(P::W * 64) void scan_bwd_kernel(ScanArgs a) {
   constexpr int L = P::L, PS = P::PS, S = P::S, W = P::W;
   __shared__ float2 sdt[L][64];  // dt, dt x
   __shared__ float sdy[L][64];
-  __shared__ __attribute__((aligned(16))) float sb[L][P::N], sc[L][P::N];
+  __shared__ __attribute__((aligned(32))) float sb[L][P::N], sc[L][P::N];
   __shared__ float sp[3][W][L][64];  // the waves' parts of sum G b, sum a P and y
   const ScanPlace<P> q(a);
   const unsigned off = q.ok ? q.ch * (unsigned)sizeof(typename Elem<F>::T) : kOffNone;
