@@ -216,41 +216,89 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
 // in bf16 (33 MB, 3.4 TB/s; 17 us in tiles).  Up to 16 rows: the call takes 69, 41 and 30 us there for 131072 tokens
 // of width 1024 and 512 and 68480 of 576, in tiles 63, 39 and 38; at 32 rows, whose reads cost as much as w's, 84,
 // 48 and 34.  (64 tokens a step halve those, but leave fewer workgroups: 67, 43 and 35 at 16.)
-constexpr int kFewRows = 16, kFewChunk = 64, kFewBlocks = 1024;
-template <bool FP16>
+// fp32 operands: w is read as it is and cut into its three pieces (mm16.h) in registers, 32 of the width at a time; x's
+// pieces are made before (16 rows, 83328 tokens of width 256: 45 us for the call, 112 in tiles with w's pieces made).
+constexpr int kFewBlocks = 1024;
+constexpr int few_rows(int fmt) { return fmt == kElemF32 ? 32 : 16; }
+template <int F>
+struct FewChunk {  // a lane's operands of kSteps instructions' 16 k
+  static constexpr bool kSplit = F == kElemF32;
+  static constexpr int kSteps = kSplit ? 2 : 4, kPieces = kSplit ? 3 : 1;
+  mm_u4 x[kSteps][kPieces], w[kSteps][kSplit ? 2 : 1];
+  // The lane's eight k from `at` on in step 0; xr, wr: its rows of x and w.
+  __device__ __forceinline__ void load(const LogitArgs& a, const unsigned short* xr, const void* wr, int at) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i, at += 16) {
+      const bool in = at < a.x.k;
+#pragma unroll
+      for (int q = 0; q < kPieces; ++q)
+        x[i][q] = in ? *reinterpret_cast<const mm_u4*>(xr + q * a.x.plane + at) : mm_u4{};
+      if constexpr (!kSplit) {
+        w[i][0] = in ? *reinterpret_cast<const mm_u4*>(static_cast<const unsigned short*>(wr) + at) : mm_u4{};
+      } else {
+        const float* const p = static_cast<const float*>(wr) + at;
+        if (at + 8 <= a.D) {
+          __builtin_memcpy(w[i], p, 32);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[i][e / 4][e % 4] = at + e < a.D ? __float_as_uint(p[e]) : 0u;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ f16v product(f16v acc) const {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if constexpr (!kSplit) {
+        acc = mm_mfma<F == kElemF16>(w[i][0], x[i][0], acc);
+      } else {
+        float f[8];
+        mm_u4 v[3];
+        __builtin_memcpy(f, w[i], 32);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          unsigned short h[8];
+          down_all<kElemBf16, 8>(f, h);
+          __builtin_memcpy(&v[q], h, 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] -= Elem<kElemBf16>::up(h[e]);
+        }
+        acc = mm_mfma<false>(v[0], x[i][2], acc);
+        acc = mm_mfma<false>(v[2], x[i][0], acc);
+        acc = mm_mfma<false>(v[1], x[i][1], acc);
+        acc = mm_mfma<false>(v[0], x[i][1], acc);
+        acc = mm_mfma<false>(v[1], x[i][0], acc);
+        acc = mm_mfma<false>(v[0], x[i][0], acc);
+      }
+    }
+    return acc;
+  }
+};
+template <int F>
 __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
+  constexpr int kChunk = 16 * FewChunk<F>::kSteps;
+  constexpr size_t kBytes = F == kElemF32 ? 4 : 2;
   __shared__ float sm[4][16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, half = lane >> 5;
-  const int groups = (a.V + 31) / 32, width = a.w.k;
+  const int groups = (a.V + 31) / 32, width = a.x.k;
   const int target = n < a.N ? a.target[n] : -1;
-  const unsigned short* const xr = a.x.p + min(n, a.N - 1) * a.x.ld + 8 * half;
-  mm_u4 w0[4], w1[4], x0[4], x1[4];
-  auto load = [&](int group, int k, mm_u4(&w)[4], mm_u4(&x)[4]) {
-    const unsigned short* const wr = a.w.p + min(group * 32 + n, a.V - 1) * a.w.ld + 8 * half;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = k + 16 * i;
-      const bool in = at + 8 * half < width;
-      x[i] = in ? *reinterpret_cast<const mm_u4*>(xr + at) : mm_u4{};
-      w[i] = in ? *reinterpret_cast<const mm_u4*>(wr + at) : mm_u4{};
-    }
+  const unsigned short* const xr = a.x.p + min(n, a.N - 1) * a.x.ld;
+  auto load = [&](int group, int k, FewChunk<F>& c) {
+    const char* const wr = reinterpret_cast<const char*>(a.w.p) + min(group * 32 + n, a.V - 1) * a.w.ld * kBytes;
+    c.load(a, xr, wr, k + 8 * half);
   };
   float m = neg_inf(), sum = 0.f;
-  load(blockIdx.x, wave * kFewChunk, w0, x0);
+  FewChunk<F> now, next;
+  load(blockIdx.x, wave * kChunk, now);
   for (int group = blockIdx.x; group < groups; group += gridDim.x) {
     f16v acc{};
-    for (int k = wave * kFewChunk; k < width; k += 4 * kFewChunk) {
-      const bool last = k + 4 * kFewChunk >= width;
-      const int next = last ? group + (int)gridDim.x : group;
-      if (next < groups) load(next, last ? wave * kFewChunk : k + 4 * kFewChunk, w1, x1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc = mm_mfma<FP16>(w0[i], x0[i], acc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x0[i] = x1[i];
-        w0[i] = w1[i];
-      }
+    for (int k = wave * kChunk; k < width; k += 4 * kChunk) {
+      const bool last = k + 4 * kChunk >= width;
+      const int to = last ? group + (int)gridDim.x : group;
+      if (to < groups) load(to, last ? wave * kChunk : k + 4 * kChunk, next);
+      acc = now.product(acc);
+      now = next;
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) sm[wave][r][lane] = acc[r];
@@ -927,7 +975,7 @@ bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kEle
 // Whether xent_few_kernel runs.  Not where a backward follows: its logits, the tiles', are rounded in another order,
 // and a probability of them against the other ones' sum would be off by as much (dbias of 12 rows: 3.3e-7, 2.1e-7 from
 // the same ones).
-bool takes_few(int N, int fmt, bool alone) { return alone && fmt != kElemF32 && N <= kFewRows; }
+bool takes_few(int N, int fmt, bool alone) { return alone && N <= few_rows(fmt); }
 // The tokens that the forward takes at a time.
 int forward_piece(int N, int V, int D, int fmt) {
   return fmt == kElemF32 ? std::min(V, plan_xent(N, V, D, fmt).piece) : V;
@@ -1118,29 +1166,26 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   a.tiles_n = (n + kMmTile - 1) / kMmTile;
   a.own = s.own;
   const bool few = takes_few(n, fmt, !stats);
-  const int piece = forward_piece(n, V, D, fmt), frags = logit_frags(n, piece);
+  const int piece = few ? V : forward_piece(n, V, D, fmt), frags = logit_frags(n, piece);
   for (int v0 = 0; v0 < V; v0 += piece) {
     const int v = std::min(piece, V - v0);
-    a.w = o.tokens(v0, v, st);
+    a.w = few && fmt == kElemF32 ? MmOperand{static_cast<const unsigned short*>(w), ldw, V, D} : o.tokens(v0, v, st);
     a.bias = s.bias + v0;
     a.v_first = v0;
     a.V = v;
     a.tiles_v = (v + 64 * frags - 1) / (64 * frags);
     a.part = s.part + (size_t)(v0 / (64 * frags)) * n;
     const dim3 grid(std::min(a.tiles_v * a.tiles_n, info.num_cus)), block(kMmThreads);
-    if (few && fmt == kElemF16)
-      hipLaunchKernelGGL(xent_few_kernel<true>, dim3(few_blocks(V)), dim3(256), 0, st, a);
-    else if (few)
-      hipLaunchKernelGGL(xent_few_kernel<false>, dim3(few_blocks(V)), dim3(256), 0, st, a);
-    else
-      HSL_CHECK(with_fmt(fmt, [&](auto F) {
-        constexpr int kF = decltype(F)::value;
-        if (frags == 2)
-          hipLaunchKernelGGL((xent_stats_kernel<kF, 2>), grid, block, 0, st, a);
-        else
-          hipLaunchKernelGGL((xent_stats_kernel<kF, 4>), grid, block, 0, st, a);
-        return (int)HSL_OK;
-      }));
+    HSL_CHECK(with_fmt(fmt, [&](auto F) {
+      constexpr int kF = decltype(F)::value;
+      if (few)
+        hipLaunchKernelGGL(xent_few_kernel<kF>, dim3(few_blocks(V)), dim3(256), 0, st, a);
+      else if (frags == 2)
+        hipLaunchKernelGGL((xent_stats_kernel<kF, 2>), grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL((xent_stats_kernel<kF, 4>), grid, block, 0, st, a);
+      return (int)HSL_OK;
+    }));
   }
   hipLaunchKernelGGL(xent_join_kernel, dim3((n + 7) / 8), dim3(256), 0, st, s.part, s.own, s.target, loss,
                      reinterpret_cast<float2*>(stats), err, n, forward_parts(n, V, D, fmt, !stats));
