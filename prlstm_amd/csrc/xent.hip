@@ -209,7 +209,7 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
   }
 }
 
-// The forward of few rows, which would leave a tile of 256 empty: 32 tokens times 32 columns a workgroup and step,
+// The forward of few rows, which would leave a tile of 256 empty: 32 tokens times 32 rows a workgroup and step,
 // whose operands go from memory to the registers of the matrix instructions (the rows' from the caches), 64 of the
 // width at a time by each of 4 waves and the next ones already on their way.  The waves' sums meet in LDS, where each
 // takes the logits of a quarter of the registers.  Bound by reading w: 10 us at 8 rows and 32768 tokens of width 512
@@ -217,9 +217,10 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
 // of width 1024 and 512 and 68480 of 576, in tiles 63, 39 and 38; at 32 rows, whose reads cost as much as w's, 84,
 // 48 and 34.  (64 tokens a step halve those, but leave fewer workgroups: 67, 43 and 35 at 16.)
 // fp32 operands: w is read as it is and cut into its three pieces (mm16.h) in registers, 32 of the width at a time; x's
-// pieces are made before (16 rows, 83328 tokens of width 256: 45 us for the call, 112 in tiles with w's pieces made).
+// pieces are made before.  Up to 64 rows, 32 at a time: 83328 tokens of width 256 take 45 us at 16 rows, 82 at 64 and 112
+// at 96 in this way, 113 in tiles, for which w's pieces are made; 131072 of 1024 265, 523 and 775, 620 in tiles.
 constexpr int kFewBlocks = 1024;
-constexpr int few_rows(int fmt) { return fmt == kElemF32 ? 32 : 16; }
+constexpr int few_rows(int fmt) { return fmt == kElemF32 ? 64 : 16; }
 template <int F>
 struct FewChunk {  // a lane's operands of kSteps instructions' 16 k
   static constexpr bool kSplit = F == kElemF32;
@@ -280,12 +281,12 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
   constexpr size_t kBytes = F == kElemF32 ? 4 : 2;
   __shared__ float sm[4][16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 31, half = lane >> 5;
+  const int col = lane & 31, n = blockIdx.y * 32 + col, half = lane >> 5;
   const int groups = (a.V + 31) / 32, width = a.x.k;
   const int target = n < a.N ? a.target[n] : -1;
   const unsigned short* const xr = a.x.p + min(n, a.N - 1) * a.x.ld;
   auto load = [&](int group, int k, FewChunk<F>& c) {
-    const char* const wr = reinterpret_cast<const char*>(a.w.p) + min(group * 32 + n, a.V - 1) * a.w.ld * kBytes;
+    const char* const wr = reinterpret_cast<const char*>(a.w.p) + min(group * 32 + col, a.V - 1) * a.w.ld * kBytes;
     c.load(a, xr, wr, k + 8 * half);
   };
   float m = neg_inf(), sum = 0.f;
@@ -1179,7 +1180,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     HSL_CHECK(with_fmt(fmt, [&](auto F) {
       constexpr int kF = decltype(F)::value;
       if (few)
-        hipLaunchKernelGGL(xent_few_kernel<kF>, dim3(few_blocks(V)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL(xent_few_kernel<kF>, dim3(few_blocks(V), (n + 31) / 32), dim3(256), 0, st, a);
       else if (frags == 2)
         hipLaunchKernelGGL((xent_stats_kernel<kF, 2>), grid, block, 0, st, a);
       else

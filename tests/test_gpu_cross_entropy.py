@@ -87,7 +87,7 @@ def check(x, w, targets, bias, dloss):
     v = w.shape[0]
     shift = (d + 4) * U * size
     finite = torch.where(torch.isfinite(want), want.abs(), torch.zeros_like(want))
-    if n > (32 if x.dtype is torch.float32 else 16):  # fewer rows alone are summed in another order
+    if n > (64 if x.dtype is torch.float32 else 16):  # fewer rows alone are summed in another order
         assert torch.equal(torch.nan_to_num(alone, -1.0), torch.nan_to_num(loss, -1.0))
     within("loss alone", alone, want, 2 * shift + 16 * U * (finite + size + math.log(v + 1)) + 2 ** -20)
     within("loss", loss, want, 2 * shift + 16 * U * (finite + size + math.log(v + 1)) + 2 ** -20)
@@ -201,7 +201,7 @@ def test_sizes_of_the_gradient(dev, scale):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n", [1, 7, 16, 17, 32, 33, 128, 129])
+@pytest.mark.parametrize("n", [1, 7, 16, 17, 33, 64, 65, 128, 129])
 def test_few_rows(dev, dtype, n):
     """Around the sizes where another kernel takes over: whole runs of tokens masked, among them targets, rows not
     scored, logits far below zero, a row of NaN."""
