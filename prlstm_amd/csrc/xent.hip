@@ -217,8 +217,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
 // of width 1024 and 512 and 68480 of 576, in tiles 63, 39 and 38; at 32 rows, whose reads cost as much as w's, 84,
 // 48 and 34.  (64 tokens a step halve those, but leave fewer workgroups: 67, 43 and 35 at 16.)
 // fp32 operands: w is read as it is and cut into its three pieces (mm16.h) in registers, 32 of the width at a time; x's
-// pieces are made before.  Up to 64 rows, 32 at a time: 83328 tokens of width 256 take 45 us at 16 rows, 82 at 64 and 112
-// at 96 in this way, 113 in tiles, for which w's pieces are made; 131072 of 1024 265, 523 and 775, 620 in tiles.
+// pieces are made before.  Up to 64 rows, 32 at a time: 83328 tokens of width 256 take 45 us at 16 rows, 82 at 64 and
+// 112 at 96 in this way, 113 in tiles, for which w's pieces are made; 131072 of 1024 265, 523 and 775, 620 in tiles.
 constexpr int kFewBlocks = 1024;
 constexpr int few_rows(int fmt) { return fmt == kElemF32 ? 64 : 16; }
 template <int F>
@@ -1020,8 +1020,8 @@ int check_begin(const char* who, const void* x, long long ldx, const void* w, lo
   };
   if (fmt != kElemF32 && D % 8 == 0 && (!readable(x, ldx) || !readable(w, ldw)))
     return fail(HSL_ERR_ARG,
-                "%s: rows of D=%d must begin at multiples of 16 bytes, fewer than 2^21 elements apart (row strides %lld "
-                "and %lld)",
+                "%s: rows of D=%d must begin at multiples of 16 bytes, fewer than 2^21 elements apart (row strides "
+                "%lld and %lld)",
                 who, D, ldx, ldw);
   return HSL_OK;
 }
