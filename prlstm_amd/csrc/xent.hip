@@ -62,6 +62,7 @@ struct LogitArgs {
   float* own;       // forward: [N], the target's logit
   unsigned short* dl;  // backward: [parts][N][tiles_v * 256]
   float* dbias;        // backward: [tile_n][tiles_v * 256], or null
+  float* dl_rows;      // backward of few rows: [V][R]
 };
 
 __device__ __forceinline__ void xent_tile_order(int tiles_m, int tiles_n, int id, int* tm, int* tn) {
@@ -275,7 +276,8 @@ struct FewChunk {  // a lane's operands of kSteps instructions' 16 k
     return acc;
   }
 };
-template <int F>
+// R: 0 for the statistics; otherwise the backward's logits, of which it leaves dl as [token][R] in fp32.
+template <int F, int R>
 __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
   constexpr int kChunk = 16 * FewChunk<F>::kSteps;
   constexpr size_t kBytes = F == kElemF32 ? 4 : 2;
@@ -283,7 +285,8 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, n = blockIdx.y * 32 + col, half = lane >> 5;
   const int groups = (a.V + 31) / 32, width = a.x.k;
-  const int target = n < a.N ? a.target[n] : -1;
+  const int target = n < a.N ? a.target[n] - a.v_first : -1;
+  const float4 row = R > 0 && n < a.N ? a.rows[n] : float4{0.f, 0.f, 0.f, 0.f};
   const unsigned short* const xr = a.x.p + min(n, a.N - 1) * a.x.ld;
   auto load = [&](int group, int k, FewChunk<F>& c) {
     const char* const wr = reinterpret_cast<const char*>(a.w.p) + min(group * 32 + col, a.V - 1) * a.w.ld * kBytes;
@@ -309,16 +312,26 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
     for (int r = 0; r < 4; ++r) {
       const int reg = 4 * wave + r, v = group * 32 + 8 * wave + 4 * half + r;
       l[r] = (sm[0][reg][lane] + sm[1][reg][lane]) + (sm[2][reg][lane] + sm[3][reg][lane]) + a.bias[v];
-      if (v == target) a.own[n] = l[r];
-      big = fmaxf(big, l[r]);
+      if constexpr (R == 0) {
+        if (v == target) a.own[n] = l[r];
+        big = fmaxf(big, l[r]);
+      } else {
+        float d = exp_from(l[r], row.x) * row.y;
+        d = row.z == 0.f || l[r] == neg_inf() ? 0.f : d;
+        if (v == target) d -= __float_as_int(row.w) < 0 ? 0.f : row.z;
+        if (n < R && v < a.V) a.dl_rows[(size_t)v * R + n] = d;
+      }
     }
-    const float ref = big == neg_inf() ? 0.f : big;
-    sum *= exp_from(m, ref);  // (0 for the first m, -inf)
-    m = big;
+    if constexpr (R == 0) {
+      const float ref = big == neg_inf() ? 0.f : big;
+      sum *= exp_from(m, ref);  // (0 for the first m, -inf)
+      m = big;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sum += exp_from(l[r], ref);
+      for (int r = 0; r < 4; ++r) sum += exp_from(l[r], ref);
+    }
     __syncthreads();
   }
+  if constexpr (R > 0) return;
   join(m, sum, __shfl_xor(m, 32), __shfl_xor(sum, 32));
   sm[wave][0][lane] = m;
   sm[wave][1][lane] = sum;
@@ -327,6 +340,81 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
 #pragma unroll
   for (int k = 1; k < 4; ++k) join(m, sum, sm[k][0][lane], sm[k][1][lane]);
   a.part[(size_t)blockIdx.x * a.N + n] = float2{m, sum};
+}
+
+// dx and dw of few fp32 rows from dl [V][R], which is uniform: a thread has 4 columns (2 at 32 rows) of all rows
+// of x and of its sums for dx in registers, and takes a range of the tokens' rows of w, whose dw it leaves.
+// Bound by reading w and writing dw: 204 us at 5 rows and 131072 tokens of width 1024 (1.07 GB, 5.3 TB/s).  The
+// pass takes 683 us there, 844 at 16 rows and 1017 at 32, on tiles, for which all of w's pieces are made, 1563;
+// at 64 rows with a column a thread 1846, so that up to 32 go this way.
+// dx: planes [range][N][D]; dw, dx: may be null.
+struct FewOutArgs {
+  const float *w, *x, *dl;
+  long long ldw, ldx;
+  float *dw, *dx;
+  int V, N, D, per, add;  // per: tokens of a range
+};
+template <int R>
+__global__ __launch_bounds__(256) void xent_few_out_kernel(FewOutArgs a) {
+  constexpr int E = R <= 16 ? 4 : 2;
+  typedef const __attribute__((address_space(4))) float Uniform;  // for scalar loads; nothing is stored there
+
+  int d = (blockIdx.x * 256 + threadIdx.x) * E;
+  if (d >= a.D) return;
+  d = min(d, a.D - E);  // the last columns, beside the neighbour's: both store the same
+  const int v0 = blockIdx.y * a.per, v1 = min(a.V, v0 + a.per);
+  float x[R][E], acc[R][E];
+#pragma unroll
+  for (int n = 0; n < R; ++n)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[n][e] = n < a.N ? a.x[n * a.ldx + d + e] : 0.f;
+      acc[n][e] = 0.f;
+    }
+  constexpr int kAhead = 4;
+  Pack<kElemF32, E> w[kAhead];
+  auto load = [&](int v) { return load_pack<kElemF32, E>(a.w + min(v, a.V - 1) * a.ldw + d); };
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) w[k] = load(v0 + k);
+  for (int v = v0; v < v1; v += kAhead) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (v + k >= v1) break;
+      Uniform* const g = (Uniform*)(unsigned long long)(a.dl + (size_t)(v + k) * R);
+      Pack<kElemF32, E> o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = 0.f;
+#pragma unroll
+      for (int n = 0; n < R; ++n)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          acc[n][e] = __builtin_fmaf(g[n], w[k].v[e], acc[n][e]);
+          o.v[e] = __builtin_fmaf(g[n], x[n][e], o.v[e]);
+        }
+      w[k] = load(v + k + kAhead);
+      if (a.dw) __builtin_memcpy(a.dw + (size_t)(v + k) * a.D + d, &o, sizeof(o));
+    }
+  }
+  if (!a.dx) return;
+  float* const to = a.dx + (size_t)blockIdx.y * a.N * a.D + d;
+#pragma unroll
+  for (int n = 0; n < R; ++n) {
+    if (n >= a.N) continue;  // (a break would have the compiler keep the loop, and the sums in memory)
+    Pack<kElemF32, E> o{};
+    if (a.add) o = load_pack<kElemF32, E>(to + (size_t)n * a.D);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.v[e] += acc[n][e];
+    __builtin_memcpy(to + (size_t)n * a.D, &o, sizeof(o));
+  }
+}
+template <int R>
+__global__ __launch_bounds__(256) void xent_few_bias_kernel(const float* __restrict__ dl, float* dbias, int V) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  double s = 0.0;
+#pragma unroll
+  for (int n = 0; n < R; ++n) s += dl[(size_t)v * R + n];
+  dbias[v] = (float)s;
 }
 
 // Targets as 32-bit numbers (-1: not scored, -2: beyond the vocabulary), and the bias, up to whole tiles.
@@ -973,10 +1061,28 @@ XentPlan plan_xent(int N, int V, int D, int fmt) {
 int few_blocks(int V) { return std::min(kFewBlocks, (V + 31) / 32); }
 bool in_two(int N, int fmt) { return fmt == kElemF32 ? false : N <= (fmt == kElemBf16 ? kMmTile / 2 : 512); }
 
-// Whether xent_few_kernel runs.  Not where a backward follows: its logits, the tiles', are rounded in another order,
-// and a probability of them against the other ones' sum would be off by as much (dbias of 12 rows: 3.3e-7, 2.1e-7 from
-// the same ones).
-bool takes_few(int N, int fmt, bool alone) { return alone && N <= few_rows(fmt); }
+// Whether the backward runs on xent_few_kernel and xent_few_out_kernel.
+bool takes_few_back(int N, int D, int fmt) { return fmt == kElemF32 && N <= 32 && D >= 4; }
+// Whether the forward runs on xent_few_kernel.  Not where a backward on tiles follows: its logits are rounded in
+// another order, and a probability of them against the other ones' sum would be off by as much (dbias of 12 fp16 rows:
+// 3.3e-7, 2.1e-7 from the same ones).
+bool takes_few(int N, int D, int fmt, bool alone) {
+  return alone ? N <= few_rows(fmt) : takes_few_back(N, D, fmt);
+}
+// The backward of few fp32 rows: R of its rows of dl, the tokens it takes at a time, and their ranges.
+struct FewPlan {
+  int R, piece, columns, ranges, per;
+};
+FewPlan plan_few(int N, int V, int D) {
+  FewPlan p;
+  p.R = N <= 8 ? 8 : N <= 16 ? 16 : 32;
+  const int each = p.R <= 16 ? 1024 : 512;  // columns of a workgroup
+  p.piece = (int)std::min<long long>(V, kPieceBytes / 4 / p.R);
+  p.columns = (D + each - 1) / each;
+  p.ranges = std::max(1, std::min((p.piece + 31) / 32, 1024 / p.columns));
+  p.per = (p.piece + p.ranges - 1) / p.ranges;
+  return p;
+}
 // The tokens that the forward takes at a time.
 int forward_piece(int N, int V, int D, int fmt) {
   return fmt == kElemF32 ? std::min(V, plan_xent(N, V, D, fmt).piece) : V;
@@ -990,7 +1096,7 @@ int logit_frags(int N, int V) {
 // The parts that the forward's statistics of a row are joined from.
 int forward_parts(int N, int V, int D, int fmt, bool alone) {
   const int tokens = 64 * logit_frags(N, forward_piece(N, V, D, fmt));
-  return takes_few(N, fmt, alone) ? few_blocks(V) : (V + tokens - 1) / tokens;
+  return takes_few(N, D, fmt, alone) ? few_blocks(V) : (V + tokens - 1) / tokens;
 }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
@@ -1036,7 +1142,7 @@ struct XentSpace {
   int *exps, *row_exp;
   unsigned short *own_x, *own_w;  // the operands as the tiles read them, where they are not that
   unsigned short *scaled_x, *scaled_w, *dl;
-  float *bias, *dbias, *dx, *dw;
+  float *bias, *dbias, *dx, *dw, *dl_rows;
   size_t bytes;
 };
 
@@ -1050,7 +1156,8 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
   s.bias = c.take<float>(up_to(V, kMmTile) + kMmTile / 2);  // a last tile of 128 has 256 copied
   if (split) {
     s.own_x = c.take<unsigned short>((size_t)3 * N * width);
-    s.own_w = c.take<unsigned short>((size_t)3 * std::min(V, p.piece) * width);
+    if (!(backward && takes_few_back(N, D, fmt)))
+      s.own_w = c.take<unsigned short>((size_t)3 * std::min(V, p.piece) * width);
   } else if (D % 8) {
     s.own_x = c.take<unsigned short>((size_t)N * width);
     s.own_w = c.take<unsigned short>((size_t)V * width);
@@ -1063,6 +1170,15 @@ XentSpace xent_space(void* base, int N, int V, int D, int fmt, bool backward) {
     return s;
   }
   s.rows = c.take<float4>(up_to(N, kMmTile));
+  if (takes_few_back(N, D, fmt)) {
+    const FewPlan f = plan_few(N, V, D);
+    s.exps = c.take<int>(3);
+    s.row_exp = c.take<int>(N);
+    s.dl_rows = c.take<float>((size_t)f.piece * f.R);
+    s.dx = c.take<float>((size_t)f.ranges * N * D);
+    s.bytes = c.off;
+    return s;
+  }
   s.part_max = c.take<unsigned>(3 * kScaleBlocks);
   s.exps = c.take<int>(3);
   s.row_exp = c.take<int>(N);
@@ -1166,7 +1282,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   a.D = D;
   a.tiles_n = (n + kMmTile - 1) / kMmTile;
   a.own = s.own;
-  const bool few = takes_few(n, fmt, !stats);
+  const bool few = takes_few(n, D, fmt, !stats);
   const int piece = few ? V : forward_piece(n, V, D, fmt), frags = logit_frags(n, piece);
   for (int v0 = 0; v0 < V; v0 += piece) {
     const int v = std::min(piece, V - v0);
@@ -1180,7 +1296,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
     HSL_CHECK(with_fmt(fmt, [&](auto F) {
       constexpr int kF = decltype(F)::value;
       if (few)
-        hipLaunchKernelGGL(xent_few_kernel<kF>, dim3(few_blocks(V), (n + 31) / 32), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((xent_few_kernel<kF, 0>), dim3(few_blocks(V), (n + 31) / 32), dim3(256), 0, st, a);
       else if (frags == 2)
         hipLaunchKernelGGL((xent_stats_kernel<kF, 2>), grid, block, 0, st, a);
       else
@@ -1281,6 +1397,55 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
     }));
     return (int)HSL_OK;
   };
+  if (s.dl_rows) {  // few fp32 rows
+    const FewPlan f = plan_few(n, V, D);
+    for (int v0 = 0; v0 < V; v0 += f.piece) {
+      const int v = std::min(f.piece, V - v0);
+      const float* const wp = static_cast<const float*>(w) + v0 * ldw;
+      LogitArgs a{};
+      a.w = {reinterpret_cast<const unsigned short*>(wp), ldw, v, D};
+      a.x = o.positions();
+      a.bias = s.bias + v0;
+      a.target = s.target;
+      a.v_first = v0;
+      a.V = v;
+      a.N = n;
+      a.D = D;
+      a.rows = s.rows;
+      a.dl_rows = s.dl_rows;
+      FewOutArgs g{};
+      g.w = wp;
+      g.x = static_cast<const float*>(x);
+      g.dl = s.dl_rows;
+      g.ldw = ldw;
+      g.ldx = ldx;
+      g.dw = dw ? static_cast<float*>(dw) + (size_t)v0 * D : nullptr;
+      g.dx = dx ? s.dx : nullptr;
+      g.V = v;
+      g.N = n;
+      g.D = D;
+      g.per = f.per;
+      g.add = v0 > 0;
+      auto run = [&](auto RR) {
+        constexpr int kR = decltype(RR)::value;
+        hipLaunchKernelGGL((xent_few_kernel<kElemF32, kR>), dim3(few_blocks(v)), dim3(256), 0, st, a);
+        if (dw || dx)
+          hipLaunchKernelGGL(xent_few_out_kernel<kR>, dim3(f.columns, f.ranges), dim3(256), 0, st, g);
+        if (dbias)
+          hipLaunchKernelGGL(xent_few_bias_kernel<kR>, dim3((v + 255) / 256), dim3(256), 0, st, s.dl_rows, dbias + v0,
+                             v);
+      };
+      if (f.R == 8)
+        run(std::integral_constant<int, 8>{});
+      else if (f.R == 16)
+        run(std::integral_constant<int, 16>{});
+      else
+        run(std::integral_constant<int, 32>{});
+      HSL_HIP(hipGetLastError());
+    }
+    if (dx) HSL_CHECK(sum_planes(s.dx, (size_t)n * D, f.ranges, s.row_exp, dx, n));
+    return HSL_OK;
+  }
   float* const planes_x = s.dx ? s.dx : static_cast<float*>(dx);  // fp32: one plane is dx itself
   const int frags = logit_frags(n, std::min(V, p.piece));
   for (int v0 = 0; v0 < V; v0 += p.piece) {

@@ -115,7 +115,7 @@ def inputs(dev, dtype, n, v, d, bias=False, pad=False, seed=0):
     return x.to(dtype).to(dev), w.to(dtype).to(dev), t.to(dev), b, dloss.to(dev)
 
 
-SIZES = [(1, 1, 1), (1, 300, 8), (2, 2, 5), (3, 257, 64), (5, 1000, 72), (70, 513, 130), (256, 256, 64),
+SIZES = [(1, 1, 1), (9, 40, 3), (40, 100, 2), (20, 77, 6), (64, 90, 1100), (1, 300, 8), (2, 2, 5), (3, 257, 64), (5, 1000, 72), (70, 513, 130), (256, 256, 64),
          (300, 700, 264), (257, 255, 17), (33, 5000, 40), (600, 90, 500), (1, 20000, 128)]
 
 
