@@ -359,9 +359,9 @@ __global__ __launch_bounds__(256) void xent_few_out_kernel(FewOutArgs a) {
   constexpr int E = R <= 16 ? 4 : 2;
   typedef const __attribute__((address_space(4))) float Uniform;  // for scalar loads; nothing is stored there
 
-  int d = (blockIdx.x * 256 + threadIdx.x) * E;
-  if (d >= a.D) return;
-  d = min(d, a.D - E);  // the last columns, beside the neighbour's: both store the same
+  const int own = (blockIdx.x * 256 + threadIdx.x) * E;
+  if (own >= a.D) return;
+  const int d = min(own, a.D - E);  // the last columns, beside the neighbour's: both store the same of dw
   const int v0 = blockIdx.y * a.per, v1 = min(a.V, v0 + a.per);
   float x[R][E], acc[R][E];
 #pragma unroll
@@ -400,11 +400,18 @@ __global__ __launch_bounds__(256) void xent_few_out_kernel(FewOutArgs a) {
 #pragma unroll
   for (int n = 0; n < R; ++n) {
     if (n >= a.N) continue;  // (a break would have the compiler keep the loop, and the sums in memory)
-    Pack<kElemF32, E> o{};
-    if (a.add) o = load_pack<kElemF32, E>(to + (size_t)n * a.D);
+    float* const row = to + (size_t)n * a.D;
+    if (d == own) {
+      Pack<kElemF32, E> o{};
+      if (a.add) o = load_pack<kElemF32, E>(row);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o.v[e] += acc[n][e];
-    __builtin_memcpy(to + (size_t)n * a.D, &o, sizeof(o));
+      for (int e = 0; e < E; ++e) o.v[e] += acc[n][e];
+      __builtin_memcpy(row, &o, sizeof(o));
+    } else {  // a sum that is added to has one owner
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (d + e >= own) row[e] = (a.add ? row[e] : 0.f) + acc[n][e];
+    }
   }
 }
 template <int R>

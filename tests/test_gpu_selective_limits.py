@@ -77,7 +77,8 @@ def test_scan_beyond_32_bits(dev):
 
 @pytest.mark.parametrize("n,v,d,dtype", [((1 << 21) + 70, 64, 1024, BF16), (70, (1 << 21) + 1000, 1024, BF16),
                                           (3, 9000011, 16, BF16), ((1 << 21) + 70, 5, 1030, torch.float32),
-                                          (30, 4500011, 500, torch.float32)])
+                                          (30, 4500011, 500, torch.float32),
+                                          (30, 2200011, 257, torch.float32)])
 def test_loss_beyond_32_bits(dev, n, v, d, dtype):
     """Only the last rows have a gradient, and all tokens but the first and last 500 are masked."""
     rows, kept = min(n, 70), torch.arange(v)
