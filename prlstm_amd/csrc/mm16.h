@@ -212,7 +212,8 @@ struct MmPipe {
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(3 * kCopies) : "memory");  // 3 slices may be on their way
   }
   // acc = this tile's product; nextA, nextB: the next tile, or operands without k.  with_next() is called
-  // before the first copy for it.  LATER (a count): loads and stores that the wave has issued for sure since the
+  // before the first copy for it: where a tile has no more slices than are in LDS, before any barrier of run(), so
+  // that other waves may still be behind the tile before.  LATER (a count): loads and stores that the wave has issued for sure since the
   // product before, which the waits for the copies before them leave out; later: whether there was one.
   template <int LATER, class Fn>
   __device__ __forceinline__ void run(MmAccOf<AF>& acc, const MmOperand& nextA, const MmOperand& nextB, bool later,

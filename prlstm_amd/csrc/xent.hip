@@ -789,6 +789,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_grad_kernel(LogitArgs a) {
       const int c = threadIdx.x;
       if (c < kTokens)
         a.dbias[(size_t)tn * ld + tv * kTokens + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+    } else if (mm.slices == kMmStages) {
+      lds_barrier();  // the next product copies over info[par] at once; a longer one has a barrier before it does
     }
   }
 }
