@@ -34,6 +34,8 @@ namespace {
 constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl
 constexpr int kPieceWidth = 1 << 21;        // tokens at most: 256 rows of dl lie within 2^31 bytes
 
+constexpr float kLargest = 3.402823466e38f;
+
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
 // A row of nothing but masks (m is -inf beside a sum of NaN where every logit is NaN).
@@ -55,7 +57,7 @@ struct LogitArgs {
   // Filled up to whole tiles:
   const float* bias;  // the piece's, zeros where there is none; -inf beyond the vocabulary
   const int* target;  // the positions' targets (of the whole vocabulary)
-  const float4* rows;  // backward: as of row_of(); zeros beyond N
+  const float4* rows;  // backward: as of row_of(), beyond N of row_beyond()
   int v_first;        // the piece's first token
   int V, N, D, tiles_v, tiles_n;
   float2* part;     // forward: [tile_v or workgroup][N]
@@ -478,6 +480,12 @@ __device__ __forceinline__ float row_gradient(float2 stats, int target, float dl
 __device__ __forceinline__ float4 row_of(float2 s, float g, int t, const float* bias, float part) {
   return float4{s.x, g * (1.f / s.y), g, t >= 0 && bias && bias[t] == neg_inf() ? -part : part};
 }
+// A row beyond the last one has no gradient, and its logits are the bias alone: measured from the largest number they
+// leave exp 0, where 0 would make one above 88 infinite.  (first: the first row's; where a bias is infinite, so is its
+// largest logit, and rows with such a reference are computed with a test of each logit.)
+__device__ __forceinline__ float4 row_beyond(float2 first) {
+  return float4{__builtin_fabsf(first.x) < __builtin_inff() ? kLargest : __builtin_inff(), 0.f, 0.f, 0.f};
+}
 // 16-bit operands' scales.  The rows of a matrix among the threads of `blocks` workgroups: 1 << lg of them a row.
 struct RowSplit {
   int lg, blocks;
@@ -618,7 +626,7 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   const int all = (a.N + kMmTile - 1) / kMmTile * kMmTile;
   for (int n = block * 256 + threadIdx.x; n < all; n += blocks * 256) {  // up to whole tiles
     if (n >= a.N) {
-      a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};
+      a.rows[n] = row_beyond(a.stats[0]);
       continue;
     }
     const float2 s = a.stats[n];
@@ -634,8 +642,10 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
 __global__ __launch_bounds__(256) void xent_rows_kernel(ScaleArgs a) {
   const int n = blockIdx.x * 256 + threadIdx.x;
   if (n < 3) a.exps[n] = n == 0 ? kTopExp : 0;
-  a.rows[n] = float4{0.f, 0.f, 0.f, 0.f};  // up to whole tiles
-  if (n >= a.N) return;
+  if (n >= a.N) {  // up to whole tiles
+    a.rows[n] = row_beyond(a.stats[0]);
+    return;
+  }
   a.rows[n] = row_of(a.stats[n], row_gradient(a.stats[n], a.target[n], a.dloss[n]), a.target[n], a.bias, 1.f);
   a.row_exp[n] = kTopExp;
 }
