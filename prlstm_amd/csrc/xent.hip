@@ -35,6 +35,7 @@ constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl
 constexpr int kPieceWidth = 1 << 21;        // tokens at most: 256 rows of dl lie within 2^31 bytes
 
 constexpr float kLargest = 3.402823466e38f;
+constexpr float kPieceEnd = 0x1.ffp127f;  // the least number that bf16 rounds to infinity
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
@@ -352,6 +353,7 @@ __global__ __launch_bounds__(256) void xent_few_kernel(LogitArgs a) {
 // dx: planes [range][N][D]; dw, dx: may be null.
 struct FewOutArgs {
   const float *w, *x, *dl;
+  const float4* rows;
   long long ldw, ldx;
   float *dw, *dx;
   int V, N, D, per, add;  // per: tokens of a range
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(256) void xent_few_out_kernel(FewOutArgs a) {
   for (int n = 0; n < R; ++n)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      x[n][e] = n < a.N ? a.x[n * a.ldx + d + e] : 0.f;
+      x[n][e] = n < a.N && a.rows[n].z != 0.f ? a.x[n * a.ldx + d + e] : 0.f;
       acc[n][e] = 0.f;
     }
   constexpr int kAhead = 4;
@@ -471,10 +473,17 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 }
 
 
-// A row's gradient: none where the target is outside of the vocabulary or nothing but masks is in the row.
-__device__ __forceinline__ float row_gradient(float2 stats, int target, float dloss) {
-  return target >= 0 && !all_masked(stats.x, stats.y) ? dloss : 0.f;
-}
+// Rows' gradients: none where the target is outside of the vocabulary or nothing but masks is in the row.  What such a
+// row of x holds (padding that nothing has written, say) must not reach dw, neither NaN times 0 nor by the scale.
+struct RowGradients {
+  const float2* stats;
+  const int* target;
+  const float* dloss;
+  __device__ __forceinline__ float operator()(long long n) const {
+    const float2 s = stats[n];
+    return target[n] >= 0 && !all_masked(s.x, s.y) ? dloss[n] : 0.f;
+  }
+};
 // What the backward needs of each row: the largest logit, g / sum, g, and 2^(its exponent less the largest row's),
 // negative where the target is masked.
 __device__ __forceinline__ float4 row_of(float2 s, float g, int t, const float* bias, float part) {
@@ -498,9 +507,8 @@ struct ScaleArgs {
   int width;
   RowSplit rx, rw;              // rw: no workgroups for an fp16 w
   int blocks_g;                 // for the rows' gradients
-  const float2* stats;
-  const int* target;
-  const float *dloss, *bias;
+  RowGradients g;
+  const float* bias;
   unsigned* part;               // the workgroups' largest magnitudes
   int* exps;                    // [3]: exponents of the largest g, of x's scale and of w's
   unsigned short *hx, *hw;      // the scaled operands in fp16, dense
@@ -533,7 +541,8 @@ __device__ __forceinline__ void for_rows(const RowSplit& r, int vecs, int block,
     }
 }
 
-// The largest finite magnitudes, as bits: of elements in a workgroup's rows, or of rows' gradients in fp32.
+// The largest finite magnitudes, as bits: of elements in a workgroup's rows (of x's, those that have a gradient), or of
+// rows' gradients in fp32.
 template <bool FP16>
 __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
   constexpr unsigned kInf = FP16 ? 0x7c00 : 0x7f80;
@@ -546,8 +555,10 @@ __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
     for_rows(is_x ? a.rx : a.rw, a.width / 8, is_x ? b : b - a.rx.blocks, [&](const long long(&row)[4], int c) {
       mm_u4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        v[k] = row[k] < 0 ? mm_u4{} : *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+      for (int k = 0; k < 4; ++k) {
+        const bool counts = row[k] >= 0 && !(is_x && a.g(row[k]) == 0.f);
+        v[k] = counts ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -558,7 +569,7 @@ __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
     });
   } else {
     for (long long n = (b - a.rx.blocks - a.rw.blocks) * 256 + threadIdx.x; n < a.N; n += a.blocks_g * 256) {
-      const unsigned g = __float_as_uint(row_gradient(a.stats[n], a.target[n], a.dloss[n])) & 0x7fffffff;
+      const unsigned g = __float_as_uint(a.g(n)) & 0x7fffffff;
       m = max(m, g < 0x7f800000 ? g : 0);
     }
   }
@@ -598,9 +609,9 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (row[k] < 0) continue;
-        v[k] = *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
-        e[k] = up;
-        if (is_x) e[k] += exponent(row_gradient(a.stats[row[k]], a.target[row[k]], a.dloss[row[k]])) - top;
+        const float g = is_x ? a.g(row[k]) : 1.f;
+        v[k] = g == 0.f ? mm_u4{} : *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+        e[k] = up + (is_x ? exponent(g) - top : 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -626,14 +637,13 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   const int all = (a.N + kMmTile - 1) / kMmTile * kMmTile;
   for (int n = block * 256 + threadIdx.x; n < all; n += blocks * 256) {  // up to whole tiles
     if (n >= a.N) {
-      a.rows[n] = row_beyond(a.stats[0]);
+      a.rows[n] = row_beyond(a.g.stats[0]);
       continue;
     }
-    const float2 s = a.stats[n];
-    const int t = a.target[n];
-    const float g = row_gradient(s, t, a.dloss[n]);
+    const float g = a.g(n);
     const int e = exponent(g);
-    a.rows[n] = row_of(s, __builtin_ldexpf(g, kTopExp - e), t, a.bias, __builtin_ldexpf(1.f, e - top));
+    a.rows[n] = row_of(a.g.stats[n], __builtin_ldexpf(g, kTopExp - e), a.g.target[n], a.bias,
+                       __builtin_ldexpf(1.f, e - top));
     a.row_exp[n] = e;
   }
 }
@@ -643,24 +653,28 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(ScaleArgs a) {
   const int n = blockIdx.x * 256 + threadIdx.x;
   if (n < 3) a.exps[n] = n == 0 ? kTopExp : 0;
   if (n >= a.N) {  // up to whole tiles
-    a.rows[n] = row_beyond(a.stats[0]);
+    a.rows[n] = row_beyond(a.g.stats[0]);
     return;
   }
-  a.rows[n] = row_of(a.stats[n], row_gradient(a.stats[n], a.target[n], a.dloss[n]), a.target[n], a.bias, 1.f);
+  a.rows[n] = row_of(a.g.stats[n], a.g(n), a.g.target[n], a.bias, 1.f);
   a.row_exp[n] = kTopExp;
 }
 
 // x twice, for a bf16 dl in two rows.  A workgroup a row.
 __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
-  const int n = blockIdx.x;
-  const unsigned short* const from = a.x + (n < a.N ? n : n - a.N) * a.ldx;
+  const int n = blockIdx.x, row = n < a.N ? n : n - a.N;
+  const unsigned short* const from = a.x + row * a.ldx;
+  const bool there = a.g(row) != 0.f;
   for (int c = threadIdx.x * 8; c < a.width; c += 2048)
-    *reinterpret_cast<mm_u4*>(a.hx + (size_t)n * a.width + c) = *reinterpret_cast<const mm_u4*>(from + c);
+    *reinterpret_cast<mm_u4*>(a.hx + (size_t)n * a.width + c) =
+        there ? *reinterpret_cast<const mm_u4*>(from + c) : mm_u4{};
 }
 
-// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.
+// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.  g: the backward's, whose rows
+// without a gradient lose what no piece holds (the rest stays, as their logits are not to exceed the forward's).
 __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld,
-                                                         unsigned short* dst, RowSplit r, int cols, int width) {
+                                                         unsigned short* dst, RowSplit r, int cols, int width,
+                                                         RowGradients g) {
   const size_t plane = (size_t)r.rows * width;
   for_rows(r, width / 8, blockIdx.x, [&](const long long(&row)[4], int c) {
     float f[4][8];
@@ -679,6 +693,10 @@ __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (row[k] < 0) continue;
+      if (g.stats && g(row[k]) == 0.f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[k][e] = __builtin_fabsf(f[k][e]) < kPieceEnd ? f[k][e] : 0.f;
+      }
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
         unsigned short h[8];
@@ -1221,7 +1239,7 @@ struct XentOperands {
   unsigned short* own_w;
 
   int init(const void* x_, long long ldx_, const void* w_, long long ldw_, const XentSpace& s, int N_, int V, int D_,
-           int fmt_, hipStream_t st) {
+           int fmt_, const RowGradients& g, hipStream_t st) {
     x0 = x_;
     w0 = w_;
     ldw0 = ldw_;
@@ -1238,7 +1256,7 @@ struct XentOperands {
     if (s.own_w) w = s.own_w;
     if (s.own_x) ldx = ldw = width;
     if (fmt == kElemF32) {
-      split(static_cast<const float*>(x0), ldx_, s.own_x, N, st);
+      split(static_cast<const float*>(x0), ldx_, s.own_x, N, g, st);
     } else if (D % 8) {
       hipLaunchKernelGGL(xent_pack_kernel, dim3(grid_of((size_t)N * width)), dim3(256), 0, st,
                          static_cast<const unsigned short*>(x0), ldx_, s.own_x, (long long)N, D, width);
@@ -1248,14 +1266,15 @@ struct XentOperands {
     HSL_HIP(hipGetLastError());
     return HSL_OK;
   }
-  void split(const float* src, long long ld, unsigned short* dst, int rows, hipStream_t st) const {
+  void split(const float* src, long long ld, unsigned short* dst, int rows, const RowGradients& g,
+             hipStream_t st) const {
     const RowSplit r = split_rows(rows, width / 8, 1 << 16);
-    hipLaunchKernelGGL(xent_split_kernel, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width);
+    hipLaunchKernelGGL(xent_split_kernel, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width, g);
   }
   // The v tokens from v0 on.
   MmOperand tokens(int v0, int v, hipStream_t st) const {
     if (fmt != kElemF32) return {w + v0 * ldw, ldw, v, width};
-    split(static_cast<const float*>(w0) + v0 * ldw0, ldw0, own_w, v, st);
+    split(static_cast<const float*>(w0) + v0 * ldw0, ldw0, own_w, v, RowGradients{}, st);
     return {own_w, ldw, v, width, (long long)v * width};
   }
   MmOperand positions() const { return {x, ldx, N, width, (long long)N * width}; }
@@ -1293,7 +1312,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   hipLaunchKernelGGL(xent_prepare_kernel, dim3((std::max(n, V) + 255) / 256), dim3(256), 0, st, targets,
                      tgt64, bias, s.target, s.bias, n, V);
   XentOperands o;
-  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, st));
+  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, RowGradients{}, st));
   LogitArgs a{};
   a.x = o.positions();
   a.target = s.target;
@@ -1364,7 +1383,8 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   DeviceInfo info;
   HSL_CHECK(device_info(&info));
   XentOperands o;
-  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, st));
+  const RowGradients rows{reinterpret_cast<const float2*>(stats), s.target, dloss};
+  HSL_CHECK(o.init(x, ldx, w, ldw, s, n, V, D, fmt, rows, st));
   const bool split = fmt == kElemF32;
   ScaleArgs sc{};
   sc.x = o.x;
@@ -1375,9 +1395,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
   sc.rx = split_rows(n, o.width / 8, kScaleBlocks);
   if (fmt == kElemBf16) sc.rw = split_rows(V, o.width / 8, kScaleBlocks);
   sc.blocks_g = std::min(kScaleBlocks, (n + 1023) / 1024);
-  sc.stats = reinterpret_cast<const float2*>(stats);
-  sc.target = s.target;
-  sc.dloss = dloss;
+  sc.g = rows;
   sc.bias = bias;
   sc.part = s.part_max;
   sc.exps = s.exps;
@@ -1436,6 +1454,7 @@ int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, con
       g.w = wp;
       g.x = static_cast<const float*>(x);
       g.dl = s.dl_rows;
+      g.rows = s.rows;
       g.ldw = ldw;
       g.ldx = ldx;
       g.dw = dw ? static_cast<float*>(dw) + (size_t)v0 * D : nullptr;
