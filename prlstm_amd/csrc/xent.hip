@@ -474,7 +474,8 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const float2* __restrict
 
 
 // Rows' gradients: none where the target is outside of the vocabulary or nothing but masks is in the row.  What such a
-// row of x holds (padding that nothing has written, say) must not reach dw, neither NaN times 0 nor by the scale.
+// row of x holds (padding that nothing has written, say) must not reach dw, neither NaN times 0 nor by the scale, and a
+// masked token's weight sets no scale either.
 struct RowGradients {
   const float2* stats;
   const int* target;
@@ -515,6 +516,10 @@ struct ScaleArgs {
   float4* rows;
   int* row_exp;
   int N, twice;                 // twice: hx has x again behind it
+  // Whether a row is multiplied by anything but 0: a position that has a gradient, a token that is not masked.
+  __device__ __forceinline__ bool counts(bool is_x, long long row) const {
+    return is_x ? g(row) != 0.f : !bias || bias[row] != neg_inf();
+  }
 };
 
 __device__ __forceinline__ unsigned block_max(unsigned m) {
@@ -541,8 +546,7 @@ __device__ __forceinline__ void for_rows(const RowSplit& r, int vecs, int block,
     }
 }
 
-// The largest finite magnitudes, as bits: of elements in a workgroup's rows (of x's, those that have a gradient), or of
-// rows' gradients in fp32.
+// The largest finite magnitudes, as bits: of elements in a workgroup's rows that count, or of rows' gradients in fp32.
 template <bool FP16>
 __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
   constexpr unsigned kInf = FP16 ? 0x7c00 : 0x7f80;
@@ -556,8 +560,7 @@ __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
       mm_u4 v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const bool counts = row[k] >= 0 && !(is_x && a.g(row[k]) == 0.f);
-        v[k] = counts ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+        v[k] = row[k] >= 0 && a.counts(is_x, row[k]) ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -609,9 +612,8 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (row[k] < 0) continue;
-        const float g = is_x ? a.g(row[k]) : 1.f;
-        v[k] = g == 0.f ? mm_u4{} : *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
-        e[k] = up + (is_x ? exponent(g) - top : 0);
+        v[k] = a.counts(is_x, row[k]) ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+        e[k] = up + (is_x ? exponent(a.g(row[k])) - top : 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {

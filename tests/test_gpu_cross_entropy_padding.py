@@ -79,3 +79,21 @@ def test_what_rows_that_are_not_scored_hold(dev, dtype, n, held, d):
     if dtype is not torch.float32:
         for g, k in zip(got, want):
             assert torch.equal(g, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [5, 40, 150, 300, 600])
+def test_what_masked_tokens_weigh(dev, dtype, n):
+    """Large weights of tokens that a bias of -inf masks: nothing of the other results is less precise."""
+    x, w, t, b, dloss = xent.inputs(dev, dtype, n, 700, 40, bias=True, pad=True)
+    b[3::7] = -math.inf
+    t = torch.where(t % 7 == 3, t - 1, t)
+    bad = w.clone()
+    bad[3::7] = 6e4 if dtype is torch.float16 else 1e30
+    w[3::7] = 0.0  # the size of what is not masked alone
+    loss, want = _grads(x, w, t, b, dloss)
+    loss2, got = _grads(x, bad, t, b, dloss)
+    assert torch.equal(loss, loss2) and not bool(got[1][3::7].any()) and not bool(got[2][3::7].any())
+    _within(got, x, w, t, b, dloss)
+    for g, k in zip(got, want):
+        assert torch.equal(g, k)
