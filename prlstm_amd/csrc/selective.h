@@ -63,10 +63,12 @@ __device__ __forceinline__ float softplus_f(float u, float e) {
   return fmaxf(u, 0.f) + __builtin_fmaf(__builtin_amdgcn_logf(w), 0.693147182464599609375f, e - (w - 1.f));
 }
 
-// The decay exp(a S) of a segment whose dt sum to S.  One that underflows is held at the smallest
-// number, so that an infinite state stays infinite.
-__device__ __forceinline__ float segment_decay(float a2, float S) {
-  return fmaxf(exp2_f(a2 * S), __uint_as_float(1u));
+// A state v behind a segment that takes it times the decay exp(a S), S the sum of the segment's dt.  The power of two
+// comes apart from the rest, as a decay beyond fp32's range need not make the product that: a state of 0 stays 0 and a
+// small one grows as it would step by step (a above 0, or dt below), and an infinite one stays infinite.
+__device__ __forceinline__ float through_segment(float a2, float S, float v) {
+  const float p = fminf(fmaxf(a2 * S, -1024.f), 1024.f), whole = __builtin_ceilf(p);
+  return __builtin_ldexpf(v * exp2_f(p - whole), (int)whole);
 }
 
 // A workgroup's place, and its lane's channel (clamped into the row where `ok` is false).

@@ -76,7 +76,7 @@ __device__ __forceinline__ void enter_reverse(const ScanArgs& a, const ScanPlace
     load_kept(a.map_h, q, a, (size_t)(i - 1) * a.B + q.b, v);
 #pragma unroll
     for (int n = 0; n < P::S; ++n) {
-      const float u = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), U[n], v[n]);
+      const float u = m.y != 0.f ? v[n] : through_segment(a2[n], m.x, U[n]) + v[n];
       U[n] = q.ok ? u : 0.f;
     }
   }

@@ -84,7 +84,7 @@ __global__ __launch_bounds__(P::W * 64) void scan_fwd_kernel(ScanArgs a) {
       load_kept(a.map_h, q, a, (size_t)i * a.B + q.b, v);
 #pragma unroll
       for (int n = 0; n < S; ++n)
-        h[n] = m.y != 0.f ? v[n] : __builtin_fmaf(segment_decay(a2[n], m.x), h[n], v[n]);
+        h[n] = m.y != 0.f ? v[n] : through_segment(a2[n], m.x, h[n]) + v[n];
     }
   }
   float total = 0.f, low = 0.f;  // the sum of dt and what its roundings lost
