@@ -217,14 +217,19 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
 // whose operands go from memory to the registers of the matrix instructions (the rows' from the caches), 64 of the
 // width at a time by each of 4 waves and the next ones already on their way.  The waves' sums meet in LDS, where each
 // takes the logits of a quarter of the registers.  Bound by reading w: 10 us at 8 rows and 32768 tokens of width 512
-// in bf16 (33 MB, 3.4 TB/s; 17 us in tiles).  Up to 16 rows: the call takes 69, 41 and 30 us there for 131072 tokens
-// of width 1024 and 512 and 68480 of 576, in tiles 63, 39 and 38; at 32 rows, whose reads cost as much as w's, 84,
-// 48 and 34.  (64 tokens a step halve those, but leave fewer workgroups: 67, 43 and 35 at 16.)
+// in bf16 (33 MB, 3.4 TB/s).  Calls of so many rows in this way / in tiles, us, w from memory (from the caches):
+//   131072 of 1024:  8 rows 75 / 66 (59 / 59), 16 rows 87 / 67 (67 / 60)
+//   131072 of 512:   46 / 43 (37 / 38), 51 / 43 (40 / 38);  of 256: 30 / 31 (25 / 28), 31 / 31 (27 / 28)
+//   32768 of 512:    19 / 18 (15.0 / 15.4), 20 / 18 (16 / 16)
+//   68480 of 576:    32 / 37 (27 / 35), 36 / 37 (29 / 35);  10000 of 2048: 23 / 33 (20 / 32), 27 / 34 (21 / 32)
+// so up to 16 rows where the tiles would leave a fifth of the CUs idle (the last line) or the width is 256 or less,
+// otherwise up to 8; at 32 rows, whose reads cost as much as w's, 131072 of 1024 take 84.  (64 tokens a step halve
+// those, but leave fewer workgroups: 67, 43 and 35 at 16 rows and 131072 of 1024 and 512 and 68480 of 576.)
 // fp32 operands: w is read as it is and cut into its three pieces (mm16.h) in registers, 32 of the width at a time; x's
 // pieces are made before.  Up to 64 rows, 32 at a time: 83328 tokens of width 256 take 45 us at 16 rows, 82 at 64 and
 // 112 at 96 in this way, 113 in tiles, for which w's pieces are made; 131072 of 1024 265, 523 and 775, 620 in tiles.
 constexpr int kFewBlocks = 1024;
-constexpr int few_rows(int fmt) { return fmt == kElemF32 ? 64 : 16; }
+constexpr int kFewRows = 8, kFewRowsUnfilled = 16, kFewRowsF32 = 64;
 template <int F>
 struct FewChunk {  // a lane's operands of kSteps instructions' 16 k
   static constexpr bool kSplit = F == kElemF32;
@@ -560,7 +565,8 @@ __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
       mm_u4 v[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        v[k] = row[k] >= 0 && a.counts(is_x, row[k]) ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+        const bool counts = row[k] >= 0 && a.counts(is_x, row[k]);
+        v[k] = counts ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -1105,8 +1111,11 @@ bool takes_few_back(int N, int D, int fmt) { return fmt == kElemF32 && N <= 32 &
 // Whether the forward runs on xent_few_kernel.  Not where a backward on tiles follows: its logits are rounded in
 // another order, and a probability of them against the other ones' sum would be off by as much (dbias of 12 fp16 rows:
 // 3.3e-7, 2.1e-7 from the same ones).
-bool takes_few(int N, int D, int fmt, bool alone) {
-  return alone ? N <= few_rows(fmt) : takes_few_back(N, D, fmt);
+bool takes_few(int N, int V, int D, int fmt, bool alone) {
+  if (!alone) return takes_few_back(N, D, fmt);
+  if (fmt == kElemF32) return N <= kFewRowsF32;
+  const long long tiles = ((long long)V + 127) / 128, rounds = (tiles + 255) / 256;  // of 128 tokens, one column
+  return N <= kFewRows || (N <= kFewRowsUnfilled && (D <= 256 || 5 * tiles < 4 * 256 * rounds));
 }
 // The backward of few fp32 rows: R of its rows of dl, the tokens it takes at a time, and their ranges.
 struct FewPlan {
@@ -1135,7 +1144,7 @@ int logit_frags(int N, int V) {
 // The parts that the forward's statistics of a row are joined from.
 int forward_parts(int N, int V, int D, int fmt, bool alone) {
   const int tokens = 64 * logit_frags(N, forward_piece(N, V, D, fmt));
-  return takes_few(N, D, fmt, alone) ? few_blocks(V) : (V + tokens - 1) / tokens;
+  return takes_few(N, V, D, fmt, alone) ? few_blocks(V) : (V + tokens - 1) / tokens;
 }
 
 int check_xent(const char* who, long long N, int V, int D, int fmt) {
@@ -1322,7 +1331,7 @@ int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, con
   a.D = D;
   a.tiles_n = (n + kMmTile - 1) / kMmTile;
   a.own = s.own;
-  const bool few = takes_few(n, D, fmt, !stats);
+  const bool few = takes_few(n, V, D, fmt, !stats);
   const int piece = few ? V : forward_piece(n, V, D, fmt), frags = logit_frags(n, piece);
   for (int v0 = 0; v0 < V; v0 += piece) {
     const int v = std::min(piece, V - v0);

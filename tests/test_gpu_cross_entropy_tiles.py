@@ -33,3 +33,12 @@ def test_without_a_gradient_of_the_bias(dev, dtype, n, v, d):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_many_short_tiles_against_64_bits(dev, dtype):
     xent.check(*xent.inputs(dev, dtype, 1100, 20500, 72, pad=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [8, 9, 16, 17])
+@pytest.mark.parametrize("v,d", [(32768, 264), (32768, 256), (26300, 264), (26100, 264)])
+def test_few_rows_of_tiles_that_fill_the_chip(dev, dtype, n, v, d):
+    """From 9 to 16 rows the vocabulary and the width decide whether the scoring runs on tiles (256, 206 or 204 of
+    128 tokens on 256 CUs)."""
+    xent.check(*xent.inputs(dev, dtype, n, v, d, bias=True, pad=True))
