@@ -487,7 +487,8 @@ struct RowGradients {
   const float* dloss;
   __device__ __forceinline__ float operator()(long long n) const {
     const float2 s = stats[n];
-    return target[n] >= 0 && !all_masked(s.x, s.y) ? dloss[n] : 0.f;
+    const float g = dloss[n];  // (three loads at a time)
+    return target[n] >= 0 && !all_masked(s.x, s.y) ? g : 0.f;
   }
 };
 // What the backward needs of each row: the largest logit, g / sum, g, and 2^(its exponent less the largest row's),
@@ -563,18 +564,22 @@ __global__ __launch_bounds__(256) void xent_max_kernel(ScaleArgs a) {
     const long long ld = is_x ? a.ldx : a.ldw;
     for_rows(is_x ? a.rx : a.rw, a.width / 8, is_x ? b : b - a.rx.blocks, [&](const long long(&row)[4], int c) {
       mm_u4 v[4];
+      bool counts[4];  // (not a condition of the loads, which then would wait for it)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const bool counts = row[k] >= 0 && a.counts(is_x, row[k]);
-        v[k] = counts ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+        v[k] = row[k] < 0 ? mm_u4{} : *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+        counts[k] = row[k] >= 0 && a.counts(is_x, row[k]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        unsigned most = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned lo = v[k][e] & 0x7fff, hi = (v[k][e] >> 16) & 0x7fff;
-          m = max(m, max(lo < kInf ? lo : 0, hi < kInf ? hi : 0));
+          most = max(most, max(lo < kInf ? lo : 0, hi < kInf ? hi : 0));
         }
+        m = max(m, counts[k] ? most : 0);
+      }
     });
   } else {
     for (long long n = (b - a.rx.blocks - a.rw.blocks) * 256 + threadIdx.x; n < a.N; n += a.blocks_g * 256) {
@@ -615,15 +620,18 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
     for_rows(is_x ? a.rx : a.rw, a.width / 8, b - first, [&](const long long(&row)[4], int c) {
       mm_u4 v[4];
       int e[4];
+      bool counts[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (row[k] < 0) continue;
-        v[k] = a.counts(is_x, row[k]) ? *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8) : mm_u4{};
+        v[k] = *reinterpret_cast<const mm_u4*>(p + row[k] * ld + c * 8);
+        counts[k] = a.counts(is_x, row[k]);
         e[k] = up + (is_x ? exponent(a.g(row[k])) - top : 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (row[k] < 0) continue;
+        if (!counts[k]) v[k] = mm_u4{};
         unsigned short h[8];
         __builtin_memcpy(h, &v[k], 16);
         float f[8];
@@ -678,16 +686,19 @@ __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
         there ? *reinterpret_cast<const mm_u4*>(from + c) : mm_u4{};
 }
 
-// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.  g: the backward's, whose rows
-// without a gradient lose what no piece holds (the rest stays, as their logits are not to exceed the forward's).
+// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.  ROWS: of x for the backward; its
+// rows without a gradient lose what no piece holds (the rest stays, as their logits are not to exceed the forward's).
+template <bool ROWS>
 __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld,
                                                          unsigned short* dst, RowSplit r, int cols, int width,
                                                          RowGradients g) {
   const size_t plane = (size_t)r.rows * width;
   for_rows(r, width / 8, blockIdx.x, [&](const long long(&row)[4], int c) {
     float f[4][8];
+    bool none[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      none[k] = ROWS && row[k] >= 0 && g(row[k]) == 0.f;
       const float* const p = src + row[k] * ld + c * 8;
       if (row[k] >= 0 && c * 8 + 8 <= cols) {
         const Pack<kElemF32, 4> lo = load_pack<kElemF32, 4>(p), hi = load_pack<kElemF32, 4>(p + 4);
@@ -701,7 +712,7 @@ __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (row[k] < 0) continue;
-      if (g.stats && g(row[k]) == 0.f) {
+      if (ROWS && none[k]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[k][e] = __builtin_fabsf(f[k][e]) < kPieceEnd ? f[k][e] : 0.f;
       }
@@ -1280,7 +1291,10 @@ struct XentOperands {
   void split(const float* src, long long ld, unsigned short* dst, int rows, const RowGradients& g,
              hipStream_t st) const {
     const RowSplit r = split_rows(rows, width / 8, 1 << 16);
-    hipLaunchKernelGGL(xent_split_kernel, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width, g);
+    if (g.stats)
+      hipLaunchKernelGGL(xent_split_kernel<true>, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width, g);
+    else
+      hipLaunchKernelGGL(xent_split_kernel<false>, dim3(r.blocks), dim3(256), 0, st, src, ld, dst, r, D, width, g);
   }
   // The v tokens from v0 on.
   MmOperand tokens(int v0, int v, hipStream_t st) const {
