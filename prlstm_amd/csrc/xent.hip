@@ -15,7 +15,7 @@
 // these two products as fp16 too, which holds their 8 bits.  Range is made up for by powers of two: a row of dl
 // is scaled to |g| = 2^14 .. 2^15, x to as large an element less what its row's g is below the largest one, a
 // bf16 w to as large an element; the results take them back.  What is then below fp16's 2^-24 counts as 0: a
-// probability below 2^-38, an element 2^-38 of its operand's largest.
+// probability below 2^-38, an element 2^-38 of its operand's largest (of x: times its row's |g| over the largest |g|).
 //   For few rows dl is kept as two rows, its value and the rest, whose products the sums join: a bf16 one in bf16
 // up to 128 rows (2^-17 of it remain), which leave half of a tile empty, so that no copy of w is made for them; an
 // fp16 one up to 512 (2^-22), whose error would otherwise be 1.4 times that of one rounding, and by chance more
@@ -34,7 +34,6 @@ namespace {
 constexpr size_t kPieceBytes = 256u << 20;  // of a piece's dl
 constexpr int kPieceWidth = 1 << 21;        // tokens at most: 256 rows of dl lie within 2^31 bytes
 
-constexpr float kLargest = 3.402823466e38f;
 constexpr float kPieceEnd = 0x1.ffp127f;  // the least number that bf16 rounds to infinity
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
@@ -496,12 +495,9 @@ struct RowGradients {
 __device__ __forceinline__ float4 row_of(float2 s, float g, int t, const float* bias, float part) {
   return float4{s.x, g * (1.f / s.y), g, t >= 0 && bias && bias[t] == neg_inf() ? -part : part};
 }
-// A row beyond the last one has no gradient, and its logits are the bias alone: measured from the largest number they
-// leave exp 0, where 0 would make one above 88 infinite.  (first: the first row's; where a bias is infinite, so is its
-// largest logit, and rows with such a reference are computed with a test of each logit.)
-__device__ __forceinline__ float4 row_beyond(float2 first) {
-  return float4{__builtin_fabsf(first.x) < __builtin_inff() ? kLargest : __builtin_inff(), 0.f, 0.f, 0.f};
-}
+// A row beyond the last one has no gradient, and its logits are the bias alone, whose exponential may be infinite: its
+// reference has it computed with a test.
+__device__ __forceinline__ float4 row_beyond() { return float4{__builtin_inff(), 0.f, 0.f, 0.f}; }
 // 16-bit operands' scales.  The rows of a matrix among the threads of `blocks` workgroups: 1 << lg of them a row.
 struct RowSplit {
   int lg, blocks;
@@ -653,7 +649,7 @@ __global__ __launch_bounds__(256) void xent_scaled_kernel(ScaleArgs a) {
   const int all = (a.N + kMmTile - 1) / kMmTile * kMmTile;
   for (int n = block * 256 + threadIdx.x; n < all; n += blocks * 256) {  // up to whole tiles
     if (n >= a.N) {
-      a.rows[n] = row_beyond(a.g.stats[0]);
+      a.rows[n] = row_beyond();
       continue;
     }
     const float g = a.g(n);
@@ -669,7 +665,7 @@ __global__ __launch_bounds__(256) void xent_rows_kernel(ScaleArgs a) {
   const int n = blockIdx.x * 256 + threadIdx.x;
   if (n < 3) a.exps[n] = n == 0 ? kTopExp : 0;
   if (n >= a.N) {  // up to whole tiles
-    a.rows[n] = row_beyond(a.g.stats[0]);
+    a.rows[n] = row_beyond();
     return;
   }
   a.rows[n] = row_of(a.g.stats[n], a.g(n), a.g.target[n], a.bias, 1.f);
@@ -686,8 +682,8 @@ __global__ __launch_bounds__(256) void xent_twice_kernel(ScaleArgs a) {
         there ? *reinterpret_cast<const mm_u4*>(from + c) : mm_u4{};
 }
 
-// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.  ROWS: of x for the backward; its
-// rows without a gradient lose what no piece holds (the rest stays, as their logits are not to exceed the forward's).
+// The three pieces of fp32 rows, in planes of rows of `width` with zeros behind `cols`.  ROWS: of x for the backward;
+// its rows without a gradient lose what no piece holds (the rest stays: their logits must not exceed the forward's).
 template <bool ROWS>
 __global__ __launch_bounds__(256) void xent_split_kernel(const float* __restrict__ src, long long ld,
                                                          unsigned short* dst, RowSplit r, int cols, int width,

@@ -97,3 +97,16 @@ def test_what_masked_tokens_weigh(dev, dtype, n):
     _within(got, x, w, t, b, dloss)
     for g, k in zip(got, want):
         assert torch.equal(g, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [5, 300])
+def test_an_infinite_weight_that_rules_a_token_out(dev, dtype, n):
+    """Logits of -inf from the product: no gradient of that token's bias, whatever 0 times the weight is behind the last
+    row."""
+    x, w, t, b, dloss = xent.inputs(dev, dtype, n, 700, 40, bias=True)
+    x, t = x.abs() + 0.1, t.clamp_min(1)
+    w[0] = -math.inf
+    loss, (_, dw, db) = _grads(x, w, t, b, dloss)
+    assert bool(torch.isfinite(loss).all()) and bool(torch.isfinite(db).all()) and bool(torch.isfinite(dw).all())
+    assert not bool(dw[0].any()) and db[0].item() == 0 and bool(db.any())
