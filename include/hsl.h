@@ -469,18 +469,18 @@ int hsl_selective_bwd(const void* x, long long x_t, long long x_b,
 /* Cross entropy of the logits l = x w^T + bias without keeping them: x [N, D] and w [V, D] (row
  * strides ldx and ldw, at least D) in the format fmt, bias [V] in fp32 (may be NULL), targets int64
  * (tgt64 != 0) or int32:  loss[n] = log sum_v exp(l[n][v]) - l[n][targets[n]], and stats[n] = (m,
- * sum_v exp(l[n][v] - m)) with the largest logit m, for the backward (NULL: none follows).  A negative target gives loss
- * 0; one >= V NaN, and raises bit 1 of the device word.  A row of nothing but masks (-inf) has m = -inf and
- * loss inf.  N is less than 2^24, D 1 or more and less than 2^20, V 1 or more, and N and V have fewer than 2^22 tiles
- * of 256 x 256.  16-bit rows of a D that is a multiple of 8 begin at multiples of 16 bytes, fewer than 2^21 elements
- * apart. */
+ * sum_v exp(l[n][v] - m)) with the largest logit m, for the backward (NULL: none follows).  A negative
+ * target gives loss 0; one >= V NaN, and raises bit 1 of the device word.  A row of nothing but masks
+ * (-inf) has m = -inf and loss inf.  N is less than 2^24, D 1 or more and less than 2^20, V 1 or more, and
+ * N and V have fewer than 2^22 tiles of 256 x 256.  16-bit rows of a D that is a multiple of 8 begin at
+ * multiples of 16 bytes, fewer than 2^21 elements apart. */
 size_t hsl_xent_ws_bytes(long long N, int V, int D, int fmt, int backward);
 int hsl_xent_fwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias,
                  const void* targets, int tgt64, float* loss, float* stats,
                  void* ws, size_t ws_bytes, long long N, int V, int D, int fmt, void* stream);
 /* dx [N, D], dw [V, D] (each contiguous, may be NULL) and dbias [V] (may be NULL) from dloss.  A
- * position whose target is outside of the vocabulary, a row of nothing but masks and a masked logit
- * have no gradient. */
+ * position whose target is outside of the vocabulary (whatever its row of x holds), a row of nothing but
+ * masks and a masked logit have no gradient. */
 int hsl_xent_bwd(const void* x, long long ldx, const void* w, long long ldw, const float* bias,
                  const void* targets, int tgt64, const float* stats, const float* dloss,
                  void* dx, void* dw, float* dbias, void* ws, size_t ws_bytes,

@@ -75,11 +75,13 @@ def linear_cross_entropy(x, weight, targets, bias=None):
     """``-log softmax(x weight^T + bias)`` at ``targets``, in fp32 and shaped as targets: x [..., D] and
     weight [V, D] in one dtype, targets [...] (int64 or int32), bias [V].
 
-    A negative target is a position that is not scored: loss 0, no gradient.  One at or beyond V gives
-    NaN, no gradient, and raises the device word that ``prlstm_amd.check_errors`` reports.  A bias of
-    ``-inf`` masks a token, which then has no gradient; a masked target has loss ``inf``, and a row of
-    nothing but masks has no gradient at all.  x, weight and bias have gradients; with 16-bit operands those
-    of the logits are rounded to 16 bits before they are multiplied, and every sum is fp32.
+    A negative target is a position that is not scored: loss 0, no gradient, and nothing that its row of
+    x holds (NaN, infinities) reaches those of weight and bias.  One at or beyond V gives NaN, no gradient,
+    and raises the device word that ``prlstm_amd.check_errors`` reports.  A bias of ``-inf`` masks a token
+    whose logits are finite without it, and which then has no gradient; a masked target has loss ``inf``,
+    and a row of nothing but masks has no gradient at all.  x, weight and bias have gradients; with 16-bit
+    operands those of the logits are rounded to 16 bits before they are multiplied (up to 128 bf16 and 512
+    fp16 rows: kept as two 16-bit numbers), and every sum is fp32.
     """
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise RuntimeError(f"x must be [..., D] and weight [V, D], got shapes {tuple(x.shape)} and "

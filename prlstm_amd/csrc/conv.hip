@@ -135,8 +135,9 @@ __device__ __forceinline__ void load_taps(const ConvArgs& a, int j, float (&w)[K
   }
 }
 
-// Forward.  Bound by HBM: 50 us at T4096 B16 D1024 K4, bf16 (268 MB, 5.4 TB/s).  Whole blocks of steps run
-// without a test per step: with the tests, and exp in full precision, it was 66 us.
+// Forward.  Bound by HBM: 63 us at T4096 B16 D1024 K4, bf16 (268 MB, 4.3 TB/s), 50 on an input of which the caches
+// hold a part.  Whole blocks of steps run without a test per step: with the tests, and exp in full precision, the
+// latter was 66 us.
 template <int F, int E, int K, bool RESET>
 __global__ __launch_bounds__(kWaves * 64) void conv_fwd_kernel(ConvArgs a) {
   using T_ = typename Elem<F>::T;

@@ -1,5 +1,5 @@
 // Helpers shared by the language-model operators (embed.hip, gated.hip, logprob.hip, conv.hip,
-// selective.hip, xent.hip).
+// selective_fwd.hip and selective_bwd.hip through selective.h, xent.hip through mm16.h).
 #pragma once
 
 #include <type_traits>

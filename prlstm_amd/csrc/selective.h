@@ -12,8 +12,9 @@
 //   C  every wave sums, gates and stores y of the steps that it had in A.
 // Steps behind the last have dt = 0 and x = 0, which keeps the state.  What bounds it is the vector units
 // and the latency of their chains: 6 issue slots per state and step (v_exp_f32, at half rate, takes two), about 60
-// per channel and step.  T4096 B16 D1024 N16, bf16: forward 520 us, the vector units half of it busy (0.48 ns per
-// 1000 states; 0.35 with 32 rows), backward 1270 (1.18), two thirds; its streams alone would take 110 and 190.
+// per channel and step.  T4096 B16 D1024 N16, bf16, in a training pass: forward 572 us (551 at least), the vector
+// units half of it busy (0.53 ns per 1000 states; 0.35 with 32 rows), backward 1278 (1.19), two thirds; its streams
+// alone would take 110 and 190.
 // Streams are read and written through buffers whose bounds drop what lies outside, without branches.
 #pragma once
 

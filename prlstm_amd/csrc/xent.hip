@@ -215,8 +215,8 @@ __global__ __launch_bounds__(kMmThreads) void xent_stats_kernel(LogitArgs a) {
 // The forward of few rows, which would leave a tile of 256 empty: 32 tokens times 32 rows a workgroup and step,
 // whose operands go from memory to the registers of the matrix instructions (the rows' from the caches), 64 of the
 // width at a time by each of 4 waves and the next ones already on their way.  The waves' sums meet in LDS, where each
-// takes the logits of a quarter of the registers.  Bound by reading w: 10 us at 8 rows and 32768 tokens of width 512
-// in bf16 (33 MB, 3.4 TB/s).  Calls of so many rows in this way / in tiles, us, w from memory (from the caches):
+// takes the logits of a quarter of the registers.  Bound by reading w: 11 us at 8 rows and 32768 tokens of width 512
+// in bf16 (33 MB, 3.0 TB/s).  Calls of so many rows in this way / in tiles, us, w from memory (from the caches):
 //   131072 of 1024:  8 rows 75 / 66 (59 / 59), 16 rows 87 / 67 (67 / 60)
 //   131072 of 512:   46 / 43 (37 / 38), 51 / 43 (40 / 38);  of 256: 30 / 31 (25 / 28), 31 / 31 (27 / 28)
 //   32768 of 512:    19 / 18 (15.0 / 15.4), 20 / 18 (16 / 16)

@@ -1,5 +1,5 @@
-"""linear_cross_entropy's backward of 16-bit operands in scaled fp16 (more than 128 bf16 rows; fp16 ones in two numbers up
-to 512 rows): gradients and operands of sizes far apart.  Tolerances as in test_gpu_cross_entropy."""
+"""linear_cross_entropy's backward of 16-bit operands in scaled fp16 (more than 128 bf16 rows; fp16 ones in two numbers
+up to 512 rows): gradients and operands of sizes far apart.  Tolerances as in test_gpu_cross_entropy."""
 
 import pytest
 import torch

@@ -19,8 +19,8 @@ def _gradients(x, w, t, b, dloss, bias_too):
 @pytest.mark.parametrize("n,v", [(1100, 20500), (1100, 40000), (500, 40000)])
 @pytest.mark.parametrize("d", [24, 32, 64, 128, 136])
 def test_without_a_gradient_of_the_bias(dev, dtype, n, v, d):
-    """Up to a width of 128 a tile's product has no more slices than are in LDS.  405 tiles of 256 x 256 and 1570 and 628
-    of 128 x 256 on 256 CUs: dx and dw are the same bits without a bias, with one of zeros that needs no gradient
+    """Up to a width of 128 a tile's product has no more slices than are in LDS.  405 tiles of 256 x 256 and 1570 and
+    628 of 128 x 256 on 256 CUs: dx and dw are the same bits without a bias, with one of zeros that needs no gradient
     and with one that needs its own, whose sums meet behind a barrier of their own; and every time."""
     x, w, t, _, dloss = xent.inputs(dev, dtype, n, v, d, pad=True)
     zeros = torch.zeros(v, device=dev)
